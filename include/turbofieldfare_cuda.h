@@ -816,6 +816,94 @@ tf_status tf_moe_block_forward_ep(tf_ep* ep, void* stream, const tf_moe_layer* l
 tf_status tf_stack_forward_ep(tf_ep* ep, void* stream, const tf_moe_layer* layers, const void* const* norm_weights_bf16,
                               uint32_t layer_count, float eps, void* hidden, uint32_t tokens, tf_ep_buffers* buffers);
 
+/* ---- attention over a quantised, paged cache ---- */
+/* Keys and values of past tokens in the affine format of the weights (group 64, bf16 scale and bias per group,
+ * value = code * scale + bias) with 8- or 4-bit codes (4-bit: low nibble = even column). Caller-owned device planes:
+ *   codes          [num_pages][kv_heads][page_size][head_dim * bits / 8] bytes
+ *   scales, biases [num_pages][kv_heads][page_size][head_dim / 64] bf16
+ * page_size: a power of two from 16 to 65536; head_dim: 64, 128, 256 or 512; every plane 16-byte aligned. The
+ * reference keeps fp16 rings and linear buffers (Runtime/KVCache/KVCacheManager.swift:26-50). */
+typedef struct tf_kv_cache {
+    void *k_codes, *k_scales, *k_biases, *v_codes, *v_scales, *v_biases;
+    uint32_t num_pages, page_size, kv_heads, head_dim, bits;
+} tf_kv_cache;
+
+/* Where the rows of a call belong. Row r with row_offsets[b] <= r < row_offsets[b + 1] is row i = r - row_offsets[b] of
+ * sequence b and stands for its token context_lengths[b] + i, which lives on page
+ * page_table[b * page_table_stride + token / page_size]. Device arrays:
+ *   row_offsets [sequences + 1], ascending, row_offsets[sequences] <= rows; rows from there on (a padded batch) are not touched;
+ *   context_lengths [sequences]; page_table [sequences][page_table_stride]; positions [rows] (see the calls; may be NULL
+ *   where a call does not need them).
+ * No call reads or writes outside a table or a plane, whatever the arrays hold: a row or token whose page is not in
+ * [0, num_pages), or lies beyond the table, is left out, and tf_device_status reports 0x7F000051; offsets that descend or pass
+ * `rows` are cut, and it reports 0x7F000052. */
+typedef struct tf_kv_batch {
+    const int32_t* row_offsets;
+    const int32_t* context_lengths;
+    const int32_t* page_table;
+    const int32_t* positions;
+    uint32_t page_table_stride, sequences, rows;
+} tf_kv_batch;
+
+/* What follows the QKV projection of a layer, in one launch: RMS norm of every head (fp32 statistics; q and k times
+ * their bf16 weight [head_dim] when given, v without a weight and only when norm_v != 0), rotation of q and k, q to q_out,
+ * and k and v quantised into the cache at the rows' tokens (`cache` may be NULL) and / or to k_out and v_out (each may be NULL;
+ * without a cache both are needed). Outputs are rounded once.
+ * Rotation: for j < rotated_pairs the elements j and j + rotated_pairs of a head turn by positions[r] * frequencies[j]
+ * (fp32 table on the device; the angle is reduced in 64 bits, so far positions keep their precision); the rest stays.
+ * rotated_pairs: a multiple of head_dim / 32, at most head_dim / 2; 0: no rotation, frequencies and positions may be NULL.
+ * Quantising is that of the weights (Quantization.swift:63-101,135-176): scale = bf16((max - min) / (2^bits - 1)), bias =
+ * bf16(min), scale 1 where max == min; a group that holds an infinity or a NaN gets NaN planes and reads back as NaN.
+ * q, k, v are act_dtype rows [rows][heads * head_dim] with strides in elements (one packed row may hold all three); k and
+ * v may be the same rows. Outputs may be their own inputs, but k_out may not be k where v is k too. Pointers must be
+ * 16-byte aligned and strides multiples of 8. Tokens of one call must be distinct: two rows that name the same slot of a page
+ * (a page shared by two sequences that both append to it) leave either's values, group by group.
+ * With cache == NULL only `rows` and `positions` of the batch are read, and all rows are done.
+ * Replaces fused_qkv_epilogue (Metal/Fusions/fused.metal:86), the per-head norms (Metal/Primitives/rmsnorm.metal:101,128),
+ * rope_default_neox / rope_proportional_neox (Metal/Primitives/rope.metal:52,75) and the KV blit. */
+tf_status tf_qkv_epilogue(tf_context* ctx, void* stream,
+                          const void* q, uint32_t q_stride_elements, const void* k, uint32_t k_stride_elements,
+                          const void* v, uint32_t v_stride_elements,
+                          const void* q_weight_bf16, const void* k_weight_bf16, int norm_v,
+                          const float* frequencies, uint32_t rotated_pairs, float eps,
+                          void* q_out, uint32_t q_out_stride_elements, void* k_out, uint32_t k_out_stride_elements,
+                          void* v_out, uint32_t v_out_stride_elements,
+                          const tf_kv_batch* batch, const tf_kv_cache* cache,
+                          uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, tf_dtype act_dtype);
+
+/* Cached rows back as act_dtype rows [rows][kv_heads * head_dim]: row r of the batch is its token (with context_lengths of
+ * zero: the sequences' prefixes). Values are code * scale + bias in fp32, rounded once. k_out or v_out may be NULL.
+ * positions are not used. Strides are multiples of 8, pointers 16-byte aligned. */
+tf_status tf_kv_cache_read(tf_context* ctx, void* stream, const tf_kv_cache* cache, const tf_kv_batch* batch,
+                           void* k_out, uint32_t k_out_stride_elements, void* v_out, uint32_t v_out_stride_elements,
+                           tf_dtype act_dtype);
+
+/* Scratch of tf_tree_attention for one head_dim: partial results of long sequences that several thread blocks share.
+ * A workspace serves one call at a time: calls that may overlap on the GPU (other streams, graphs replayed side by
+ * side) need one each. Nothing in it has to survive between calls. */
+typedef struct tf_attention_workspace tf_attention_workspace;
+tf_status tf_attention_workspace_create(tf_context* ctx, uint32_t head_dim, tf_attention_workspace** out);
+void tf_attention_workspace_destroy(tf_attention_workspace* ws);
+uint64_t tf_attention_workspace_bytes(const tf_attention_workspace* ws);
+
+/* Attention of the newest rows of every sequence over the cache, which already holds them (tf_qkv_epilogue before):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j over the tokens j that a row sees, query head h with kv head h / (q_heads / kv_heads).
+ * Row i of a sequence with c = context_lengths[b] cached tokens sees
+ *   - token j < c: always, or with window > 0 when p - j < window, p = max(positions[r], c) with a tree_mask, c + i without;
+ *   - token c + j (row j of this call): bit j % 64 of tree_mask[r * mask_words + j / 64] (the row's ancestors in a tree of
+ *     drafted tokens and itself; rows from 64 * mask_words on are seen by nobody), or, with tree_mask == NULL (a chain; one token
+ *     is the shortest), j <= i, and with a window i - j < window.
+ * A row that sees nothing becomes zero. Infinities and NaN in the cache reach only the rows that see them.
+ * positions are read only with a tree_mask and a window. q and out: act_dtype rows [rows][q_heads * head_dim], 16-byte
+ * aligned, strides multiples of 8; out may be q. softmax and sums are fp32.
+ * Any number of rows, contexts and sequences; the lengths stay on the device, and the call can be captured.
+ * Replaces attention_decode_partial / _gqa_swa_partial / _combine (Metal/Attention/attention.metal:135,227,343) and
+ * attention_prefill_causal_tiled (Metal/Prefill/prefill.metal:836); the reference drafts no tokens. */
+tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32_t q_stride_elements,
+                            void* out, uint32_t out_stride_elements, const tf_kv_cache* cache, const tf_kv_batch* batch,
+                            const uint64_t* tree_mask, uint32_t mask_words, uint32_t window, float scale,
+                            uint32_t q_heads, tf_dtype act_dtype, tf_attention_workspace* ws);
+
 #ifdef __cplusplus
 }
 #endif

@@ -80,6 +80,18 @@ class DeviceRoutes(C.Structure):
                                   "chunk_group", "chunk_start", "counters")]
 
 
+class KVCacheDesc(C.Structure):
+    """tf_kv_cache: planes and dimensions of a quantised, paged key/value cache."""
+    _fields_ = ([(n, vp) for n in ("k_codes", "k_scales", "k_biases", "v_codes", "v_scales", "v_biases")] +
+                [(n, u32) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "bits")])
+
+
+class KVBatchDesc(C.Structure):
+    """tf_kv_batch: where the rows of a call belong."""
+    _fields_ = ([(n, vp) for n in ("row_offsets", "context_lengths", "page_table", "positions")] +
+                [(n, u32) for n in ("page_table_stride", "sequences", "rows")])
+
+
 _PLANES = [vp, u64, vp, u64, vp, u64]   # weights, scales, biases with offsets
 
 SIGNATURES = {
@@ -199,6 +211,14 @@ SIGNATURES = {
     "tf_ep_pack_push": (C.c_int, [vp, vp, vp, u32, vp, u32, u32, u32, u32, u32, vp, u64, u32, vp, u32, u32, u32, u64, vp]),
     "tf_lm_head_greedy_int4": (C.c_int, [vp, vp, vp, u64, vp, u64, *_PLANES, vp, u32, u32, f32]),
     "tf_post_attn_setup": (C.c_int, [vp, vp, vp, u32, vp, u32, vp, u32, vp, u32, vp, u32, vp, vp, vp, u32, u32, f32]),
+    "tf_qkv_epilogue": (C.c_int, [vp, vp, vp, u32, vp, u32, vp, u32, vp, vp, C.c_int, vp, u32, f32, vp, u32, vp, u32, vp, u32,
+                                  C.POINTER(KVBatchDesc), C.POINTER(KVCacheDesc), u32, u32, u32, C.c_int]),
+    "tf_kv_cache_read": (C.c_int, [vp, vp, C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), vp, u32, vp, u32, C.c_int]),
+    "tf_attention_workspace_create": (C.c_int, [vp, u32, C.POINTER(vp)]),
+    "tf_attention_workspace_destroy": (None, [vp]),
+    "tf_attention_workspace_bytes": (u64, [vp]),
+    "tf_tree_attention": (C.c_int, [vp, vp, vp, u32, vp, u32, C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), vp, u32, u32, f32, u32,
+                                    C.c_int, vp]),
     "tf_layer_tail": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, f32, f32]),
 }
 

@@ -1,0 +1,7 @@
+// Attention over the quantised cache for heads of 128 elements.
+#include "attention.cuh"
+
+namespace tf {
+template tf_status attend<128, 4>(tf_context*, cudaStream_t, const AttnArgs&, const tf_attention_workspace*, bool);
+template tf_status attend<128, 8>(tf_context*, cudaStream_t, const AttnArgs&, const tf_attention_workspace*, bool);
+}  // namespace tf

@@ -1,0 +1,129 @@
+// Which tiles of which rows a block of the attention takes: lengths, units and shares. Host and device code alike, so that the CPU tests walk
+// every block of a call.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace tf {
+
+constexpr int kTile = 64;                                      // tokens
+
+// What a block leaves for the unit that its share ends in: where the other shares are and which rows they hold.
+struct ShareInfo {
+    uint32_t active, last_block;
+    uint32_t row0, flat0, valid, head;    // first row of the sequence; first (token, head) row of the unit and how many; kv head
+    uint64_t unused;
+};
+
+struct AttnArgs {
+    const uint16_t* q;
+    uint16_t* out;
+    KvPlanes k, v;
+    KvTable table;
+    const int32_t *row_offsets, *context_lengths, *positions;
+    const unsigned long long* mask;
+    float* partial;
+    ShareInfo* info;
+    uint32_t* error;
+    uint32_t q_stride, out_stride, sequences, rows, kv_heads, group, mask_words, window;
+    float scale;
+};
+
+template <typename T>
+__host__ __device__ __forceinline__ T lesser(T a, T b) { return a < b ? a : b; }
+
+// The lengths of a sequence, cut to what the arrays and the table can hold.
+struct Sequence {
+    uint32_t row0, rows;      // its rows of the call
+    int64_t context;          // cached tokens before them
+    __host__ __device__ __forceinline__ void load(const AttnArgs& a, uint32_t b, bool report) {
+        const int64_t begin = a.row_offsets[b], end = a.row_offsets[b + 1], c = a.context_lengths[b];
+        const int64_t lo = begin < 0 ? 0 : begin > (int64_t)a.rows ? (int64_t)a.rows : begin;
+        const int64_t hi = end < lo ? lo : end > (int64_t)a.rows ? (int64_t)a.rows : end;
+        row0 = (uint32_t)lo;
+        rows = (uint32_t)(hi - lo);
+        context = c < 0 ? 0 : c;
+        if (report) {
+            if (lo != begin || hi != end) *a.error = kErrKvOffsets;
+            if (rows && (c < 0 || context + rows > (int64_t)a.table.stride << a.table.page_log2)) *a.error = kErrKvPage;
+        }
+    }
+};
+
+// The tokens that the rows [flat0, flat0 + MT) of a sequence's kv head may see, in tiles.
+struct UnitRange {
+    int64_t end;              // tokens from here on are seen by no row
+    int64_t tile0;
+    uint32_t tiles;           // at least one, so that rows which see nothing are still written
+    __host__ __device__ __forceinline__ void set(const AttnArgs& a, const Sequence& s, uint32_t flat0, uint32_t mt) {
+        const uint32_t first = flat0 / a.group, last_flat = (uint32_t)(lesser((uint64_t)flat0 + mt, (uint64_t)s.rows * a.group) - 1), last = last_flat / a.group;
+        const int64_t drafted = a.mask ? (int64_t)lesser((uint64_t)s.rows, (uint64_t)a.mask_words * 64) : (int64_t)last + 1;
+        int64_t low = 0;
+        if (a.window) low = s.context + (a.mask ? 0 : (int64_t)first) - (int64_t)a.window + 1;
+        if (low < 0) low = 0;
+        end = lesser(s.context + drafted, (int64_t)a.table.stride << a.table.page_log2);
+        tile0 = low / kTile;
+        const int64_t stop = (end + kTile - 1) / kTile;
+        tiles = stop > tile0 ? (uint32_t)(stop - tile0) : 1u;
+    }
+};
+
+// A place in the row of all tiles: sequence, kv head, unit of rows, tile.
+template <int MT>
+struct Cursor {
+    Sequence seq;
+    UnitRange range;
+    uint32_t b, head, flat0, tile;       // tile counts from range.tile0
+    __host__ __device__ __forceinline__ uint64_t flat_rows(const AttnArgs& a) const { return (uint64_t)seq.rows * a.group; }
+    // to the first tile of the next unit
+    __host__ __device__ __forceinline__ void next_unit(const AttnArgs& a) {
+        tile = 0;
+        if ((uint64_t)flat0 + MT < flat_rows(a)) {
+            flat0 += MT;
+        } else if (flat0 = 0; ++head == a.kv_heads) {
+            head = 0;
+            do { if (++b >= a.sequences) return; seq.load(a, b, false); } while (seq.rows == 0);
+        }
+        range.set(a, seq, flat0, MT);
+    }
+    __host__ __device__ __forceinline__ void advance(const AttnArgs& a) { if (++tile == range.tiles) next_unit(a); }
+};
+
+// Tiles of a sequence's rows for one kv head, over all its units.
+template <int MT>
+__host__ __device__ __forceinline__ uint64_t sequence_tiles(const AttnArgs& a, const Sequence& s) {
+    uint64_t n = 0;
+    for (uint64_t f = 0; f < (uint64_t)s.rows * a.group; f += MT) {
+        UnitRange r;
+        r.set(a, s, (uint32_t)f, MT);
+        n += r.tiles;
+    }
+    return n;
+}
+
+// The place `left` tiles into the tiles of sequence b, which has more than that.
+template <int MT>
+__host__ __device__ __forceinline__ void place_in_sequence(const AttnArgs& a, uint32_t b, uint64_t left, uint32_t (&place)[4]) {
+    Sequence s;
+    s.load(a, b, false);
+    const uint64_t n = sequence_tiles<MT>(a, s);
+    place[0] = b;
+    place[1] = (uint32_t)(left / n);
+    left %= n;
+    for (uint64_t f = 0;; f += MT) {
+        UnitRange r;
+        r.set(a, s, (uint32_t)f, MT);
+        if (left < r.tiles) {
+            place[2] = (uint32_t)f;
+            place[3] = (uint32_t)left;
+            return;
+        }
+        left -= r.tiles;
+    }
+}
+
+// First tile of block c's share of `total`, and the block whose share holds the tile before `end`.
+__host__ __device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t blocks, uint32_t c) { return total * c / blocks; }
+__host__ __device__ __forceinline__ uint32_t share_of_last(uint64_t total, uint32_t blocks, uint64_t end) { return (uint32_t)((end * blocks - 1) / total); }
+
+}  // namespace tf
