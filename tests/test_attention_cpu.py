@@ -23,7 +23,7 @@ static int64_t pick(int64_t lo, int64_t hi) { return lo + (int64_t)(rng() % (uin
 
 // Every block of a call walks its share as the kernel does: units are covered tile by tile exactly once, and the blocks that share a unit are those
 // that the join will read. Tokens are looked up in the table on the way; what comes back is inside of the planes.
-template <int MT>
+template <int MT, int TILE>
 static void walk(const AttnArgs& a, uint32_t grid) {
     uint64_t total = 0;
     std::vector<uint64_t> before(a.sequences + 1, 0);
@@ -31,7 +31,7 @@ static void walk(const AttnArgs& a, uint32_t grid) {
         Sequence s;
         s.load(a, b, true);
         CHECK(s.row0 + (uint64_t)s.rows <= a.rows && s.context >= 0);
-        total += sequence_tiles<MT>(a, s) * a.kv_heads;
+        total += sequence_tiles<MT, TILE>(a, s) * a.kv_heads;
         before[b + 1] = total;
     }
     const uint32_t blocks = (uint32_t)lesser((uint64_t)grid, total);
@@ -46,11 +46,11 @@ static void walk(const AttnArgs& a, uint32_t grid) {
         uint32_t b = 0;
         while (before[b + 1] <= item) ++b;
         uint32_t place[4];
-        place_in_sequence<MT>(a, b, item - before[b], place);
-        Cursor<MT> now;
+        place_in_sequence<MT, TILE>(a, b, item - before[b], place);
+        Cursor<MT, TILE> now;
         now.b = place[0]; now.head = place[1]; now.flat0 = place[2]; now.tile = place[3];
         now.seq.load(a, now.b, false);
-        now.range.set(a, now.seq, now.flat0, MT);
+        now.range.set(a, now.seq, now.flat0, MT, TILE);
         std::set<int> slots;
         while (item < stop) {
             const Unit u{now.b, now.head, now.flat0};
@@ -60,8 +60,8 @@ static void walk(const AttnArgs& a, uint32_t grid) {
             CHECK(now.flat0 < now.flat_rows(a) && segment > 0);
             CHECK(now.range.end <= (int64_t)a.table.stride << a.table.page_log2);
             for (uint32_t k = 0; k < segment; ++k) {
-                const int64_t token0 = (now.range.tile0 + now.tile + k) * kTile;
-                for (int i = 0; i < 4; ++i)
+                const int64_t token0 = (now.range.tile0 + now.tile + k) * TILE;
+                for (int i = 0; i < TILE / 16; ++i)
                     if (token0 + 16 * i < now.range.end) CHECK(a.table.page(now.b, token0 + 16 * i) < (int32_t)a.table.pages);
             }
             seen[u].push_back({c, segment});
@@ -118,9 +118,11 @@ static void shares() {
         static const unsigned long long word = 0;
         if (pick(0, 1)) { a.mask = &word; a.mask_words = (uint32_t)pick(1, 2); }
         const uint32_t grid = (uint32_t)(pick(0, 1) ? 296 : pick(1, 500));
-        walk<16>(a, grid);
-        walk<32>(a, grid);
-        walk<64>(a, grid);
+        walk<8, 16>(a, grid);
+        walk<16, 16>(a, 3 * grid);
+        walk<16, 64>(a, grid);
+        walk<64, 64>(a, grid);
+        walk<128, 64>(a, grid);
         CHECK(bad || error == 0);
     }
 }
@@ -140,8 +142,22 @@ static void places() {
     CHECK(S::OFF_STAGE % 128 == 0 && S::STAGE % 128 == 0 && S::SMEM <= 227 * 1024 && S::STAGES >= 2);
     CHECK(S::OFF_P % 16 == 0 && S::OFF_RED % 16 == 0 && S::OFF_VRED % 16 == 0 && S::OFF_O % 16 == 0 && S::OFF_SV % 16 == 0 && S::OFF_BV % 16 == 0);
 }
+template <int D, int BITS, int RB>
+static void rows_places() {
+    using S = RowsShape<D, BITS, RB>;
+    std::set<uint32_t> k, v;
+    for (uint32_t r = 0; r < kRowsTile; ++r)
+        for (uint32_t p = 0; p < S::PIECES; ++p) {
+            const uint32_t x = S::k_at(r, p * 16), y = S::v_at(r, p * 16);
+            CHECK(x % 16 == 0 && y % 16 == 0 && x + 16 <= S::CODES && y + 16 <= S::CODES);
+            CHECK(k.insert(x).second && v.insert(y).second);
+            for (uint32_t byte = 0; byte < 16; byte += 2) CHECK(S::k_at(r, p * 16 + byte) == x + byte && S::v_at(r, p * 16 + byte) == y + byte);
+        }
+    CHECK(kRowsTile * S::PIECES % kWarp == 0 && (8 * S::G) % 8 == 0);
+    CHECK(S::STAGES >= 2 && S::STAGES <= 31 && S::BLOCKS * (S::SMEM + 1024 + 256) <= 227 * 1024);
+}
 template <int D, int BITS>
-static void places() { places<D, BITS, 16>(); places<D, BITS, 32>(); places<D, BITS, 64>(); }
+static void places() { places<D, BITS, 16>(); places<D, BITS, 32>(); places<D, BITS, 64>(); rows_places<D, BITS, 8>(); }
 
 // Refusals: none of them reaches the device.
 static tf_context context;

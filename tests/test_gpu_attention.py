@@ -173,6 +173,34 @@ def test_rows_that_see_nothing_are_zero_and_masked_values_reach_nobody(tf_ctx, w
     _close(got[clean], want[clean], tol[clean])
 
 
+@pytest.mark.parametrize("rows", [[4], [40]])
+def test_large_values_reach_only_the_rows_that_see_them(tf_ctx, workspaces, rows):
+    """A drafted token with values 10^5 times the others', seen by itself alone: the other rows keep their precision. The same for
+    what stands in a page behind the sequence's last token."""
+    case = Case(18, rows, [20], 1, 128, 8, 16, DEV)
+    t = 20 + 1
+    for i in (4, 5):
+        case.planes[i][int(case.table[0, t // 16]), :, t % 16] *= 1e5
+    last = 20 + rows[0]
+    case.planes[4][int(case.table[0, last // 16]), :, last % 16:] = 3e38
+    case.planes[5][int(case.table[0, last // 16]), :, last % 16:] = -3e38
+    case.upload()
+    masks = [{j for j in range(i + 1) if j != 1} for i in range(rows[0])]
+    masks[1] = {0, 1}
+    q = _q(case, 2, BF16)
+    got = _run(tf_ctx, workspaces, case, q, BF16, masks=masks)
+    see = [ref.visible(rows[0], 20, 0, masks)]
+    want, tol = ref.attention(case, q, see, 128 ** -0.5, half_step(BF16))
+    others = [r for r in range(rows[0]) if r != 1]
+    _close(got[[1]], want[[1]], tol[[1]])
+    # the tolerance's share for probabilities below fp16's least step goes by the largest value that is seen
+    kept = Case.of_cache(case.cache, case.table, rows, [20])
+    for i in (4, 5):
+        kept.planes[i][int(case.table[0, t // 16]), :, t % 16] = 0.0
+    want, tol = ref.attention(kept, q, see, 128 ** -0.5, half_step(BF16))
+    _close(got[others], want[others], tol[others])
+
+
 @pytest.mark.parametrize("value_scale", [1e-6, 1e4, 1e30])
 def test_values_outside_of_fp16(tf_ctx, workspaces, value_scale):
     case = Case(9, [2, 1], [90, 300], 2, 64, 8, 16, DEV, value_scale=value_scale).upload()

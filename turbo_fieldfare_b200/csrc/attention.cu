@@ -17,8 +17,8 @@ tf_status tf_attention_workspace_create(tf_context* ctx, uint32_t head_dim, tf_a
     ws->device = ctx->device;
     ws->head_dim = head_dim;
     ws->row_capacity = (uint32_t)ctx->sm_count * 128;          // two blocks of 64 rows per SM, or eight of 16
-    ws->max_blocks = (uint32_t)ctx->sm_count * 8;
-    const uint64_t partial = (uint64_t)2 * ws->row_capacity * (head_dim + 2) * sizeof(float), info = (uint64_t)ws->max_blocks * sizeof(tf::ShareInfo);
+    ws->max_workers = (uint32_t)ctx->sm_count * 16;
+    const uint64_t partial = (uint64_t)2 * ws->row_capacity * (head_dim + 2) * sizeof(float), info = (uint64_t)ws->max_workers * sizeof(tf::ShareInfo);
     cudaError_t e = cudaMalloc(&ws->partial, partial);
     if (e == cudaSuccess) e = cudaMalloc(&ws->info, info);
     if (e != cudaSuccess) {

@@ -20,10 +20,12 @@
 // value in the group, is below the 16-bit output's. Sums are fp32.
 #pragma once
 
-#include "attention_launch.cuh"
+#include "attention_rows.cuh"
 #include "mma_gemv.cuh"
 
 namespace tf {
+
+constexpr int kTile = 64;                                      // tokens
 
 constexpr int kAttnThreads = 256, kAttnWarps = kAttnThreads / kWarp;
 constexpr int kCombineThreads = 128;
@@ -99,7 +101,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, g = lane / 4, t = lane % 4;
 
     // ---- this block's share of the tiles ----
-    Cursor<MT> now;
+    Cursor<MT, kTile> now;
     uint64_t total, item, stop;
     uint32_t blocks;
     {
@@ -109,7 +111,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
         for (uint32_t b = b0; b < b1; ++b) {
             Sequence s;
             s.load(a, b, blockIdx.x == 0);
-            mine += sequence_tiles<MT>(a, s) * a.kv_heads;
+            mine += sequence_tiles<MT, kTile>(a, s) * a.kv_heads;
         }
         uint64_t upto = mine;
 #pragma unroll
@@ -137,9 +139,9 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
             for (uint32_t b = b0; b < b1; ++b) {
                 Sequence s;
                 s.load(a, b, false);
-                const uint64_t n = sequence_tiles<MT>(a, s) * a.kv_heads;
+                const uint64_t n = sequence_tiles<MT, kTile>(a, s) * a.kv_heads;
                 if (left < n) {
-                    place_in_sequence<MT>(a, b, left, s_start);
+                    place_in_sequence<MT, kTile>(a, b, left, s_start);
                     break;
                 }
                 left -= n;
@@ -148,11 +150,11 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
         __syncthreads();
         now.b = s_start[0]; now.head = s_start[1]; now.flat0 = s_start[2]; now.tile = s_start[3];
         now.seq.load(a, now.b, false);
-        now.range.set(a, now.seq, now.flat0, MT);
+        now.range.set(a, now.seq, now.flat0, MT, kTile);
     }
 
     // ---- loads of a tile ----
-    Cursor<MT> next = now;
+    Cursor<MT, kTile> next = now;
     uint64_t next_item = item;
     // pages of the four runs of 16 tokens of a tile, as this thread's rows need them; -1: left out
     auto load_tile = [&](uint32_t stage) {
@@ -187,7 +189,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
         cp_async_commit();
     };
     // the runs of 16 tokens of the current tile that have a page
-    auto runs_of = [&](const Cursor<MT>& c) -> uint32_t {
+    auto runs_of = [&](const Cursor<MT, kTile>& c) -> uint32_t {
         const int64_t token0 = (c.range.tile0 + c.tile) * kTile;
         uint32_t m = 0;
 #pragma unroll
@@ -671,7 +673,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
             if (from_start && tid == 0) {
                 const uint64_t end_item = item - segment + now.range.tiles;      // of the unit; it begins in this share
                 ShareInfo& info = a.info[blockIdx.x];
-                info.last_block = share_of_last(total, blocks, end_item);
+                info.last = share_of_last(total, blocks, end_item);
                 info.row0 = now.seq.row0;
                 info.flat0 = now.flat0;
                 info.valid = valid;
@@ -694,7 +696,7 @@ attention_combine_kernel(const AttnArgs a) {
     const ShareInfo info = a.info[c];
     const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, r = blockIdx.y * (kCombineThreads / kWarp) + warp;
     if (!info.active || r >= info.valid) return;
-    const uint32_t parts = info.last_block - c + 1;
+    const uint32_t parts = info.last - c + 1;
     constexpr size_t kSlot = (size_t)MT * (D + 2);
     auto slot = [&](uint32_t p) { return a.partial + (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kSlot; };
     float top = -INFINITY;
@@ -748,7 +750,7 @@ static tf_status launch_attention(tf_context* ctx, cudaStream_t st, const AttnAr
     if (s != TF_OK) return s;
     uint32_t blocks = resident_blocks(ctx, kernel, blocks_cache, kAttnThreads, S::SMEM);
     if (blocks > ws->row_capacity / MT) blocks = ws->row_capacity / MT;
-    if (blocks > ws->max_blocks) blocks = ws->max_blocks;
+    if (blocks > ws->max_workers) blocks = ws->max_workers;
     TF_REQUIRE(ctx, blocks > 0, TF_ERR_CUDA, "tf_tree_attention: the kernel does not fit on the device");
     kernel<<<blocks, kAttnThreads, S::SMEM, st>>>(a);
     const tf_status t = check_launch(ctx, "tf_tree_attention");
@@ -761,6 +763,7 @@ template <int D, int BITS>
 tf_status attend(tf_context* ctx, cudaStream_t st, const AttnArgs& a, const tf_attention_workspace* ws, bool bf16) {
     // Rows of one kv head in a mean sequence: units of 16 rows while they hold them, else of 64, which read a tile once for four times as many.
     const uint64_t mean = ((uint64_t)a.rows + a.sequences - 1) / a.sequences * a.group;
+    if (mean <= 8) return bf16 ? launch_rows<D, BITS, 8, true>(ctx, st, a, ws) : launch_rows<D, BITS, 8, false>(ctx, st, a, ws);
     if (mean <= 16) return bf16 ? launch_attention<D, BITS, 16, true>(ctx, st, a, ws) : launch_attention<D, BITS, 16, false>(ctx, st, a, ws);
     return bf16 ? launch_attention<D, BITS, 64, true>(ctx, st, a, ws) : launch_attention<D, BITS, 64, false>(ctx, st, a, ws);
 }

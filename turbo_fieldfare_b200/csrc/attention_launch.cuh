@@ -5,10 +5,10 @@
 
 struct tf_attention_workspace {
     int device = 0;
-    uint32_t head_dim = 0, row_capacity = 0, max_blocks = 0;   // rows of one partial slot times blocks
+    uint32_t head_dim = 0, row_capacity = 0, max_workers = 0;   // rows of one partial slot times blocks
     uint64_t bytes = 0;
     float* partial = nullptr;      // [2 x blocks][rows][head_dim + 2]
-    void* info = nullptr;          // [max_blocks] ShareInfo
+    void* info = nullptr;          // [max_workers] ShareInfo
 };
 
 namespace tf {

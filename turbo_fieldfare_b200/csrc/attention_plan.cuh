@@ -1,16 +1,14 @@
-// Which tiles of which rows a block of the attention takes: lengths, units and shares. Host and device code alike, so that the CPU tests walk
-// every block of a call.
+// Which tiles of which rows a worker of the attention takes: lengths, units and shares. Host and device code alike, so that the CPU tests walk
+// every worker of a call.
 #pragma once
 
 #include "kv_cache.cuh"
 
 namespace tf {
 
-constexpr int kTile = 64;                                      // tokens
-
-// What a block leaves for the unit that its share ends in: where the other shares are and which rows they hold.
+// What a worker (a thread block or a warp) leaves for the unit that its share ends in: where the other shares are and which rows they hold.
 struct ShareInfo {
-    uint32_t active, last_block;
+    uint32_t active, last;
     uint32_t row0, flat0, valid, head;    // first row of the sequence; first (token, head) row of the unit and how many; kv head
     uint64_t unused;
 };
@@ -55,25 +53,26 @@ struct UnitRange {
     int64_t end;              // tokens from here on are seen by no row
     int64_t tile0;
     uint32_t tiles;           // at least one, so that rows which see nothing are still written
-    __host__ __device__ __forceinline__ void set(const AttnArgs& a, const Sequence& s, uint32_t flat0, uint32_t mt) {
+    __host__ __device__ __forceinline__ void set(const AttnArgs& a, const Sequence& s, uint32_t flat0, uint32_t mt, int tile) {
         const uint32_t first = flat0 / a.group, last_flat = (uint32_t)(lesser((uint64_t)flat0 + mt, (uint64_t)s.rows * a.group) - 1), last = last_flat / a.group;
         const int64_t drafted = a.mask ? (int64_t)lesser((uint64_t)s.rows, (uint64_t)a.mask_words * 64) : (int64_t)last + 1;
         int64_t low = 0;
         if (a.window) low = s.context + (a.mask ? 0 : (int64_t)first) - (int64_t)a.window + 1;
         if (low < 0) low = 0;
         end = lesser(s.context + drafted, (int64_t)a.table.stride << a.table.page_log2);
-        tile0 = low / kTile;
-        const int64_t stop = (end + kTile - 1) / kTile;
+        tile0 = low / tile;
+        const int64_t stop = (end + tile - 1) / tile;
         tiles = stop > tile0 ? (uint32_t)(stop - tile0) : 1u;
     }
 };
 
 // A place in the row of all tiles: sequence, kv head, unit of rows, tile.
-template <int MT>
+template <int MT, int TILE>
 struct Cursor {
     Sequence seq;
     UnitRange range;
     uint32_t b, head, flat0, tile;       // tile counts from range.tile0
+    __host__ __device__ __forceinline__ int64_t token0() const { return (range.tile0 + tile) * TILE; }
     __host__ __device__ __forceinline__ uint64_t flat_rows(const AttnArgs& a) const { return (uint64_t)seq.rows * a.group; }
     // to the first tile of the next unit
     __host__ __device__ __forceinline__ void next_unit(const AttnArgs& a) {
@@ -84,35 +83,35 @@ struct Cursor {
             head = 0;
             do { if (++b >= a.sequences) return; seq.load(a, b, false); } while (seq.rows == 0);
         }
-        range.set(a, seq, flat0, MT);
+        range.set(a, seq, flat0, MT, TILE);
     }
     __host__ __device__ __forceinline__ void advance(const AttnArgs& a) { if (++tile == range.tiles) next_unit(a); }
 };
 
 // Tiles of a sequence's rows for one kv head, over all its units.
-template <int MT>
+template <int MT, int TILE>
 __host__ __device__ __forceinline__ uint64_t sequence_tiles(const AttnArgs& a, const Sequence& s) {
     uint64_t n = 0;
     for (uint64_t f = 0; f < (uint64_t)s.rows * a.group; f += MT) {
         UnitRange r;
-        r.set(a, s, (uint32_t)f, MT);
+        r.set(a, s, (uint32_t)f, MT, TILE);
         n += r.tiles;
     }
     return n;
 }
 
 // The place `left` tiles into the tiles of sequence b, which has more than that.
-template <int MT>
+template <int MT, int TILE>
 __host__ __device__ __forceinline__ void place_in_sequence(const AttnArgs& a, uint32_t b, uint64_t left, uint32_t (&place)[4]) {
     Sequence s;
     s.load(a, b, false);
-    const uint64_t n = sequence_tiles<MT>(a, s);
+    const uint64_t n = sequence_tiles<MT, TILE>(a, s);
     place[0] = b;
     place[1] = (uint32_t)(left / n);
     left %= n;
     for (uint64_t f = 0;; f += MT) {
         UnitRange r;
-        r.set(a, s, (uint32_t)f, MT);
+        r.set(a, s, (uint32_t)f, MT, TILE);
         if (left < r.tiles) {
             place[2] = (uint32_t)f;
             place[3] = (uint32_t)left;
@@ -122,8 +121,8 @@ __host__ __device__ __forceinline__ void place_in_sequence(const AttnArgs& a, ui
     }
 }
 
-// First tile of block c's share of `total`, and the block whose share holds the tile before `end`.
-__host__ __device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t blocks, uint32_t c) { return total * c / blocks; }
-__host__ __device__ __forceinline__ uint32_t share_of_last(uint64_t total, uint32_t blocks, uint64_t end) { return (uint32_t)((end * blocks - 1) / total); }
+// First tile of worker c's share of `total`, and the worker whose share holds the tile before `end`.
+__host__ __device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t workers, uint32_t c) { return total * c / workers; }
+__host__ __device__ __forceinline__ uint32_t share_of_last(uint64_t total, uint32_t workers, uint64_t end) { return (uint32_t)((end * workers - 1) / total); }
 
 }  // namespace tf

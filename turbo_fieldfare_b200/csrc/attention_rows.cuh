@@ -1,0 +1,739 @@
+// Attention over the quantised, paged cache for units of at most eight (or sixteen) rows: decode steps and small trees.
+//
+// What bounds it is HBM: a cached token's codes and planes are read once and used for a handful of rows. So everything that is not
+// unpacking is kept out of the way. A worker is one warp: it owns its share of the tiles (16 tokens each), its ring of stages, filled by its own
+// cp.async, its running maximum, sum and product; no thread block ever meets at a barrier, and the shares of a unit are joined by
+// attention_rows_combine_kernel in the workers' order, which is a property of the lengths alone.
+//
+// Logits, S[row][token] = Q K^T (mma.sync m16n8k16, rows as A, tokens as B): an 8-bit code c enters as the fp16 subnormal c * 2^-24 (one PRMT
+// per two codes), a 4-bit one as c * 2^-24 or, against a q pre-scaled by 1/16, c * 2^-20 (one AND). Scale and bias come in fp32 per
+// group: s (q . c) + b sum(q). The accumulators of S hold (row g; tokens 2t, 2t + 1), which is the B fragment of the second product,
+// O^T[element][row] = V^T P^T, with V's codes as A, again as subnormals: the value scale goes into the probability, p' = p s 2^-E rounded to
+// fp16, and what the bias adds is summed in fp32, sum p b. So that the rounding of p' weighs a code's distance from the centre of the codes, not the code
+// itself, sum (p s - 2^E p') * centre is added to that sum. E is a row's own, after the largest p s so far (tokens that it does not see have p = 0
+// and no say), and m a maximum that is raised only when a logit exceeds it by 8: a vote each per tile, and what was summed is rescaled
+// only when one of them moves.
+#pragma once
+
+#include "attention_launch.cuh"
+#include "mma_gemv.cuh"
+
+namespace tf {
+
+constexpr int kRowsTile = 16;                                  // tokens: a tile never straddles two pages
+
+template <int D, int BITS, int RB>
+struct RowsShape {
+    static constexpr int G = D / 64, ROW = D * BITS / 8, PIECES = ROW / 16, NR = RB / 8;
+    static constexpr int CODES = kRowsTile * ROW, PLANE = kRowsTile * G * 2, STAGE = 2 * CODES + 4 * PLANE;
+    // Heads of 512: the rows of q are read from shared memory, since the product alone takes 128 registers.
+    static constexpr bool Q_SHARED = D == 512;
+    static constexpr int Q_BYTES = Q_SHARED ? D / 16 * kWarp * 8 : 0;
+    static constexpr int WARPS = D == 512 ? (BITS == 8 ? 1 : 2) : 4, BLOCKS = D == 512 ? (BITS == 8 ? 5 : 3) : D == 256 ? 2 : 3;
+    static constexpr int THREADS = WARPS * kWarp;
+    static constexpr int FIT = (227 * 1024 / BLOCKS - 1024 - 256 - WARPS * Q_BYTES) / (WARPS * STAGE), STAGES = FIT > 8 ? 8 : FIT;
+    static constexpr int SMEM = WARPS * (STAGES * STAGE + Q_BYTES);
+    static constexpr int GH = G < 4 ? G : 4;                   // groups whose planes are in registers at a time
+    static_assert(STAGES >= 2 && STAGE % 128 == 0, "a ring needs two stages");
+    // 16-byte pieces are moved within their 128-byte lines so that the reads of a quarter or half warp meet every bank once
+    static __host__ __device__ __forceinline__ uint32_t k_at(uint32_t row, uint32_t byte) {
+        uint32_t at = row * ROW + byte;
+        if constexpr (BITS == 8) { if constexpr (ROW >= 128) at ^= (row & 1u) << 6; }
+        else if constexpr (ROW >= 128) at ^= (row & 3u) << 5;
+        else if constexpr (ROW == 64) at ^= ((row >> 1) & 1u) << 5;
+        return at;
+    }
+    static __host__ __device__ __forceinline__ uint32_t v_at(uint32_t row, uint32_t byte) { return (row * ROW + byte) ^ (((row >> 1) & 3u) << 5); }
+};
+
+__device__ __forceinline__ void rows_cp_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void rows_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float rows_exp2(float x) {          // 2^x; results below fp32's normal range are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t rows_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t rows_pair(float lo, float hi) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+        return rows_half2(lo, hi);
+    }
+}
+__device__ __forceinline__ int rows_exponent(float v) { return max(-126, min((int)((__float_as_uint(v) >> 23) & 255u) - 127, 126)); }
+__device__ __forceinline__ float rows_power(int e) { return __uint_as_float((uint32_t)(max(-126, min(e, 127)) + 127) << 23); }
+
+// bf16 values of two neighbouring tokens (2i, then 2i + 1) in the N groups from `first` on, of planes of G groups. N = 1: one word holds both.
+template <int G, int N>
+struct PlanePair {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const uint8_t* plane, int pair, int first) {
+        const uint8_t* p = plane + pair * (4 * G) + 2 * first;
+        if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+        else if constexpr (N == G) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+        else {
+            const uint2 v0 = *reinterpret_cast<const uint2*>(p), v1 = *reinterpret_cast<const uint2*>(p + 2 * G);
+            w[0] = v0.x; w[1] = v0.y; w[2] = v1.x; w[3] = v1.y;
+        }
+    }
+    __device__ __forceinline__ float at(int token, int grp) const {
+        const int i = token * N + grp;
+        return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    }
+    // The largest magnitudes of either token so far, in both halves of its word (N = 1: both tokens' in the first word); a NaN stays.
+    __device__ __forceinline__ void raise(__nv_bfloat162& most0, __nv_bfloat162& most1) const {
+        auto word = [&](int i) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])); };
+        if constexpr (N == 1) {
+            most0 = __hmax2_nan(most0, word(0));
+        } else {
+            __nv_bfloat162 a = word(0), b = word(N / 2);
+            if constexpr (N == 4) { a = __hmax2_nan(a, word(1)); b = __hmax2_nan(b, word(3)); }
+            most0 = __hmax2_nan(most0, __hmax2_nan(a, __lowhigh2highlow(a)));
+            most1 = __hmax2_nan(most1, __hmax2_nan(b, __lowhigh2highlow(b)));
+        }
+    }
+};
+
+template <int D, int BITS, int RB, bool BF16>
+__global__ void __launch_bounds__(RowsShape<D, BITS, RB>::THREADS, RowsShape<D, BITS, RB>::BLOCKS)
+attention_rows_kernel(const __grid_constant__ AttnArgs a) {
+    using S = RowsShape<D, BITS, RB>;
+    constexpr int G = S::G, NR = S::NR, W = S::WARPS;
+    constexpr float kCentre = BITS == 8 ? 128.0f : 8.0f;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ unsigned long long s_scan[W];
+    __shared__ uint32_t s_start[W][4];
+    const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, g = lane / 4, t = lane % 4;
+    const uint32_t workers_max = gridDim.x * W, worker = blockIdx.x * W + warp;
+
+    // ---- the shares of this block's warps ----
+    uint64_t total = 0;
+    {
+        const uint32_t per = (a.sequences + S::THREADS - 1) / S::THREADS, b0 = lesser((uint64_t)per * tid, (uint64_t)a.sequences),
+                       b1 = lesser((uint64_t)b0 + per, (uint64_t)a.sequences);
+        uint64_t mine = 0;
+        for (uint32_t b = b0; b < b1; ++b) {
+            Sequence s;
+            s.load(a, b, blockIdx.x == 0);
+            mine += sequence_tiles<RB, kRowsTile>(a, s) * a.kv_heads;
+        }
+        uint64_t upto = mine;
+#pragma unroll
+        for (int off = 1; off < kWarp; off <<= 1) {
+            const uint64_t o = __shfl_up_sync(kFullMask, upto, off);
+            if (lane >= off) upto += o;
+        }
+        if (lane == kWarp - 1) s_scan[warp] = upto;
+        __syncthreads();
+        uint64_t before = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w == warp) before = total;
+            total += s_scan[w];
+        }
+        before += upto - mine;
+        const uint32_t workers = (uint32_t)lesser((uint64_t)workers_max, total);
+#pragma unroll 1
+        for (int w = 0; w < W; ++w) {
+            if (blockIdx.x * W + w >= workers) break;
+            const uint64_t item = share_begin(total, workers, blockIdx.x * W + w);
+            if (item >= before && item < before + mine) {
+                uint64_t left = item - before;
+                for (uint32_t b = b0; b < b1; ++b) {
+                    Sequence s;
+                    s.load(a, b, false);
+                    const uint64_t n = sequence_tiles<RB, kRowsTile>(a, s) * a.kv_heads;
+                    if (left < n) {
+                        place_in_sequence<RB, kRowsTile>(a, b, left, s_start[w]);
+                        break;
+                    }
+                    left -= n;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const uint32_t workers = (uint32_t)lesser((uint64_t)workers_max, total);
+    if (lane == 0) a.info[worker].active = 0;
+    if (worker >= workers) return;
+    uint64_t item = share_begin(total, workers, worker);
+    const uint64_t stop = share_begin(total, workers, worker + 1);
+    Cursor<RB, kRowsTile> now;
+    now.b = s_start[warp][0]; now.head = s_start[warp][1]; now.flat0 = s_start[warp][2]; now.tile = s_start[warp][3];
+    now.seq.load(a, now.b, false);
+    now.range.set(a, now.seq, now.flat0, RB, kRowsTile);
+
+    // ---- this warp's ring ----
+    uint8_t* ring = smem + warp * (S::STAGES * S::STAGE);
+    uint2* q_shared = reinterpret_cast<uint2*>(smem + W * S::STAGES * S::STAGE + warp * S::Q_BYTES) + lane;       // [D / 16][lanes]
+    const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+    Cursor<RB, kRowsTile> next = now;
+    uint32_t ahead = (uint32_t)(stop - item);                  // tiles not requested yet
+    uint32_t there = 0;                                        // a bit per stage: its tile has a page
+    int32_t next_page = a.table.page(next.b, next.token0());
+    auto request = [&](uint32_t stage) {
+        there &= ~(1u << stage);
+        if (next_page >= 0) {
+            there |= 1u << stage;
+            const size_t row = (((size_t)next_page * a.kv_heads + next.head) << a.table.page_log2) + ((uint32_t)next.token0() & ((1u << a.table.page_log2) - 1u));
+            const uint32_t base = ring_addr + stage * S::STAGE;
+            const uint8_t *kc = a.k.codes + row * S::ROW + lane * 16, *vc = a.v.codes + row * S::ROW + lane * 16;
+#pragma unroll
+            for (int i = 0; i < (kRowsTile * S::PIECES) / kWarp; ++i) {
+                const uint32_t id = lane + i * kWarp, r = id / S::PIECES, byte = id % S::PIECES * 16;
+                rows_cp_async(base + S::k_at(r, byte), kc + i * 512);
+                rows_cp_async(base + S::CODES + S::v_at(r, byte), vc + i * 512);
+            }
+            // planes: 2 G pieces each
+            if (8 * G >= kWarp || lane < 8 * G) {
+#pragma unroll
+                for (int i = 0; i < (8 * G + kWarp - 1) / kWarp; ++i) {
+                    const uint32_t id = lane + i * kWarp, plane = id / (2 * G), c = id % (2 * G);
+                    const uint16_t* src = plane == 0 ? a.k.scales : plane == 1 ? a.k.biases : plane == 2 ? a.v.scales : a.v.biases;
+                    rows_cp_async(base + 2 * S::CODES + plane * S::PLANE + c * 16, src + row * G + c * 8);
+                }
+            }
+        }
+        if (--ahead) {
+            next.advance(a);
+            next_page = next.token0() < next.range.end ? a.table.page(next.b, next.token0()) : -1;
+        }
+    };
+    if (next.token0() >= next.range.end) next_page = -1;
+#pragma unroll 1
+    for (int i = 0; i < S::STAGES - 1; ++i) {
+        if (ahead) request(i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    uint32_t stage = 0;
+    while (item < stop) {
+        // ---- a unit's segment: the rows of q as A fragments, their sums per group, what they see ----
+        const uint32_t valid = (uint32_t)lesser((uint64_t)RB, now.flat_rows(a) - now.flat0);
+        const bool from_start = now.tile == 0;
+        const uint32_t segment = (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), stop - item);
+        const bool to_end = now.tile + segment == now.range.tiles;
+        uint32_t qf[NR][S::Q_SHARED ? 1 : D / 16][2];
+        float q_sum[NR][G], factor[NR], m[NR], l[NR], b_sum[NR][G];
+        int32_t low[NR];                                       // first token that the row sees, from the unit's first tile on
+        uint32_t node[NR];
+        int32_t low_most = 0;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const uint32_t r = g + 8 * n, flat = now.flat0 + r;
+            const bool is = r < valid;
+            node[n] = is ? flat / a.group : 0;
+            const uint16_t* src = a.q + (size_t)(now.seq.row0 + node[n]) * a.q_stride + (size_t)(now.head * a.group + (is ? flat % a.group : 0)) * D + 16 * t;
+            uint32_t raw[G][8];
+            float most = 0.0f;
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+                const uint4 lo = is ? *reinterpret_cast<const uint4*>(src + grp * 64) : make_uint4(0, 0, 0, 0);
+                const uint4 hi = is ? *reinterpret_cast<const uint4*>(src + grp * 64 + 8) : make_uint4(0, 0, 0, 0);
+                raw[grp][0] = lo.x; raw[grp][1] = lo.y; raw[grp][2] = lo.z; raw[grp][3] = lo.w;
+                raw[grp][4] = hi.x; raw[grp][5] = hi.y; raw[grp][6] = hi.z; raw[grp][7] = hi.w;
+            }
+            auto value = [&](int grp, int j) {
+                const uint16_t h = (uint16_t)(raw[grp][j / 2] >> (16 * (j % 2)));
+                return BF16 ? bf16_bits_to_float(h) : f16_bits_to_float(h);
+            };
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(value(grp, j)));
+            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+            const int e = most > 0.0f ? max(rows_exponent(most) - 7, -126) : 0;      // the row's largest element to [128, 256)
+            const float down = rows_power(-e);
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+                float sum = 0.0f;
+                // element j of the lane's sixteen as fp16, a 4-bit code's odd ones by a sixteenth
+                auto part = [&](int j) {
+                    const bool sixteenth = BITS == 4 && (j % 2);
+                    const __half h = __float2half_rn(value(grp, j) * (sixteenth ? down * 0.0625f : down));
+                    sum += __half2float(h) * (sixteenth ? 16.0f : 1.0f);
+                    return (uint32_t)__half_as_ushort(h);
+                };
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    uint32_t lo, hi;
+                    if constexpr (BITS == 8) {
+                        lo = part(4 * ks) | part(4 * ks + 1) << 16;
+                        hi = part(4 * ks + 2) | part(4 * ks + 3) << 16;
+                    } else {
+                        const int j = 8 * (ks / 2) + 2 * (ks % 2);
+                        lo = part(j) | part(j + 4) << 16;
+                        hi = part(j + 1) | part(j + 5) << 16;
+                    }
+                    if constexpr (S::Q_SHARED) {
+                        q_shared[(grp * 4 + ks) * kWarp] = make_uint2(lo, hi);      // read by this lane alone
+                    } else {
+                        qf[n][grp * 4 + ks][0] = lo;
+                        qf[n][grp * 4 + ks][1] = hi;
+                    }
+                }
+                sum += __shfl_xor_sync(kFullMask, sum, 1);
+                sum += __shfl_xor_sync(kFullMask, sum, 2);
+                q_sum[n][grp] = sum * 5.9604644775390625e-8f;  // 2^-24, as the products
+                b_sum[n][grp] = 0.0f;
+            }
+            factor[n] = 16777216.0f * rows_power(e) * a.scale * 1.4426950408889634f;
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
+            low[n] = 0;
+            if (a.window && is) {
+                const int64_t pos = a.mask ? max((int64_t)a.positions[now.seq.row0 + node[n]], now.seq.context) : now.seq.context + node[n];
+                const int64_t first = pos - (int64_t)a.window + 1 - now.range.tile0 * kRowsTile;
+                low[n] = (int32_t)max((int64_t)0, lesser(first, (int64_t)0x7FFFFFFF));
+            }
+            low_most = max(low_most, low[n]);
+        }
+        if (a.window) low_most = (int32_t)__reduce_max_sync(kFullMask, (uint32_t)low_most);
+        float o[NR][G][4][4];
+        int e_v[NR];                                           // exponent that the row's products p s are divided by, and 2^-E
+        float down_v[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            e_v[n] = -126;
+            down_v[n] = rows_power(126);
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][grp][j][0] = o[n][grp][j][1] = o[n][grp][j][2] = o[n][grp][j][3] = 0.0f;
+        // tokens of the segment before this place are seen by every row without a look at a mask, if their tile starts at low_most or later
+        const int64_t open_end = lesser(now.seq.context, now.range.end) - now.range.tile0 * kRowsTile;
+        int32_t rel0 = now.tile * kRowsTile;
+
+#pragma unroll 1
+        for (uint32_t done = 0; done < segment; ++done, rel0 += kRowsTile) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
+            __syncwarp();
+            const uint8_t* st = ring + stage * S::STAGE;
+            const bool has_page = there >> stage & 1u;
+
+            // ---- logits: n tile 0 holds tokens 0 to 7, n tile 1 tokens 8 to 15 ----
+            float x[2][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[0][c] = x[1][c] = 0.0f;
+            PlanePair<G, S::GH> ks_lo, ks_hi, kb_lo, kb_hi;
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+                if (grp % S::GH == 0) {
+                    ks_lo.load(st + 2 * S::CODES, t, grp); ks_hi.load(st + 2 * S::CODES, t + 4, grp);
+                    kb_lo.load(st + 2 * S::CODES + S::PLANE, t, grp); kb_hi.load(st + 2 * S::CODES + S::PLANE, t + 4, grp);
+                }
+                const int gh = grp % S::GH;
+                uint32_t w[2][4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    if constexpr (BITS == 8) {
+                        const uint4 c = *reinterpret_cast<const uint4*>(st + S::k_at(g + 8 * n, grp * 64 + 16 * t));
+                        w[n][0] = c.x; w[n][1] = c.y; w[n][2] = c.z; w[n][3] = c.w;
+                    } else {
+                        const uint2 c = *reinterpret_cast<const uint2*>(st + S::k_at(g + 8 * n, grp * 32 + 8 * t));
+                        w[n][0] = c.x; w[n][1] = c.x >> 8; w[n][2] = c.y; w[n][3] = c.y >> 8;
+                    }
+                }
+                float acc[2][4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[0][c] = acc[1][c] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    uint2 qs;
+                    if constexpr (S::Q_SHARED) qs = q_shared[(grp * 4 + ks) * kWarp];
+                    else qs = make_uint2(qf[0][grp * 4 + ks][0], qf[0][grp * 4 + ks][1]);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        uint32_t b0, b1;
+                        if constexpr (BITS == 8) {
+                            b0 = gm_prmt(w[n][ks], 0, 0x4140);
+                            b1 = gm_prmt(w[n][ks], 0, 0x4342);
+                        } else {
+                            b0 = w[n][ks] & 0x000F000Fu;
+                            b1 = w[n][ks] & 0x00F000F0u;
+                        }
+                        if constexpr (NR == 2) rows_mma(acc[n], qs.x, qf[NR - 1][grp * 4 + ks][0], qs.y, qf[NR - 1][grp * 4 + ks][1], b0, b1);
+                        else rows_mma(acc[n], qs.x, 0u, qs.y, 0u, b0, b1);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    x[0][2 * n] = fmaf(ks_lo.at(0, gh), acc[0][2 * n], fmaf(kb_lo.at(0, gh), q_sum[n][grp], x[0][2 * n]));
+                    x[0][2 * n + 1] = fmaf(ks_lo.at(1, gh), acc[0][2 * n + 1], fmaf(kb_lo.at(1, gh), q_sum[n][grp], x[0][2 * n + 1]));
+                    x[1][2 * n] = fmaf(ks_hi.at(0, gh), acc[1][2 * n], fmaf(kb_hi.at(0, gh), q_sum[n][grp], x[1][2 * n]));
+                    x[1][2 * n + 1] = fmaf(ks_hi.at(1, gh), acc[1][2 * n + 1], fmaf(kb_hi.at(1, gh), q_sum[n][grp], x[1][2 * n + 1]));
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                x[0][2 * n] *= factor[n]; x[0][2 * n + 1] *= factor[n];
+                x[1][2 * n] *= factor[n]; x[1][2 * n + 1] *= factor[n];
+            }
+            if (!(has_page && rel0 >= low_most && rel0 + kRowsTile <= open_end)) {
+                if (!has_page && lane == 0 && rel0 + now.range.tile0 * kRowsTile < now.range.end) *a.error = kErrKvPage;
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int32_t rel = rel0 + 2 * t + (c & 1) + (c & 2) * 4;
+                        const int64_t token = now.range.tile0 * kRowsTile + rel;
+                        bool seen = has_page && g + 8 * n < (int)valid && token < now.range.end;
+                        if (seen) {
+                            if (token < now.seq.context) {
+                                seen = rel >= low[n];
+                            } else {
+                                const uint32_t j = (uint32_t)(token - now.seq.context);
+                                if (a.mask) seen = (a.mask[(size_t)(now.seq.row0 + node[n]) * a.mask_words + (j >> 6)] >> (j & 63u)) & 1ull;
+                                else seen = j <= node[n] && (!a.window || node[n] - j < a.window);
+                            }
+                        }
+                        if (!seen) x[c >> 1][2 * n + (c & 1)] = -INFINITY;
+                    }
+                }
+            }
+
+            // ---- does a maximum move? ----
+            float over = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+                over = fmaxf(over, fmaxf(fmaxf(x[0][2 * n], x[0][2 * n + 1]), fmaxf(x[1][2 * n], x[1][2 * n + 1])) - m[n]);
+            // what was summed of rows g + 8 n, times f: their accumulators lie in the columns of other lanes
+            auto rescale = [&](int n, float f) {
+                const float f0 = __shfl_sync(kFullMask, f, 8 * t), f1 = __shfl_sync(kFullMask, f, 8 * t + 4);      // rows 2t, 2t + 1
+#pragma unroll
+                for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { o[n][grp][j][0] *= f0; o[n][grp][j][1] *= f1; o[n][grp][j][2] *= f0; o[n][grp][j][3] *= f1; }
+            };
+            if (__any_sync(kFullMask, over > 8.0f)) {
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    float top = fmaxf(fmaxf(x[0][2 * n], x[0][2 * n + 1]), fmaxf(x[1][2 * n], x[1][2 * n + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+                    const float m_new = fmaxf(m[n], top), alpha = m_new == -INFINITY ? 1.0f : rows_exp2(m[n] - m_new);
+                    m[n] = m_new;
+                    l[n] *= alpha;
+#pragma unroll
+                    for (int grp = 0; grp < G; ++grp) b_sum[n][grp] *= alpha;
+                    rescale(n, alpha);
+                }
+            }
+
+            // ---- probabilities, at most 2^8 ----
+            float p[NR][4];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                const float base = m[n] == -INFINITY ? 0.0f : m[n];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) p[n][c] = rows_exp2(x[c >> 1][2 * n + (c & 1)] - base);
+                l[n] += (p[n][0] + p[n][1]) + (p[n][2] + p[n][3]);
+            }
+
+            // ---- does a row's exponent move, is a value plane not finite? ----
+            const uint8_t *vs_plane = st + 2 * S::CODES + 2 * S::PLANE, *vb_plane = vs_plane + S::PLANE;
+            PlanePair<G, S::GH> vs_lo, vs_hi, vb_lo, vb_hi;
+            auto load_value_planes = [&](int first) {
+                vs_lo.load(vs_plane, t, first); vs_hi.load(vs_plane, t + 4, first);
+                vb_lo.load(vb_plane, t, first); vb_hi.load(vb_plane, t + 4, first);
+            };
+            const __nv_bfloat162 none = __float2bfloat162_rn(0.0f), finite = __halves2bfloat162(__ushort_as_bfloat16(0x7F7F), __ushort_as_bfloat16(0x7F7F));
+            __nv_bfloat162 most_s[4] = {none, none, none, none}, most_b = none;     // per token; a NaN stays
+#pragma unroll
+            for (int first = 0; first < G; first += S::GH) {
+                load_value_planes(first);
+                vs_lo.raise(most_s[0], most_s[1]); vs_hi.raise(most_s[2], most_s[3]);
+                vb_lo.raise(most_b, most_b); vb_hi.raise(most_b, most_b);
+            }
+            bool moves = !__hble2(most_b, finite);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                float most = 0.0f;
+#pragma unroll
+                for (int key = 0; key < 4; ++key) {
+                    const float s = S::GH == 1 ? __uint_as_float((*reinterpret_cast<const uint32_t*>(&most_s[key & 2])) << (key & 1 ? 0 : 16) & 0xFFFF0000u)
+                                               : __uint_as_float((*reinterpret_cast<const uint32_t*>(&most_s[key])) & 0xFFFF0000u);
+                    const float z = p[n][key] * s;
+                    most = z <= most ? most : z;               // a NaN stays
+                }
+                moves |= !(most * down_v[n] < 16384.0f);
+            }
+            bool broken = false;
+            if (__any_sync(kFullMask, moves)) {
+                bool bad = !__hble2(most_b, finite);
+#pragma unroll
+                for (int key = 0; key < 4; ++key) bad |= !__hble2(most_s[key], finite);
+                broken = __any_sync(kFullMask, bad);
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    float most = 0.0f;
+#pragma unroll
+                    for (int first = 0; first < G; first += S::GH) {
+                        load_value_planes(first);
+#pragma unroll
+                        for (int gh = 0; gh < S::GH; ++gh)
+#pragma unroll
+                            for (int key = 0; key < 4; ++key) {
+                                const float s = fabsf(key < 2 ? vs_lo.at(key, gh) : vs_hi.at(key - 2, gh));
+                                if (s <= 3.402823466e38f) most = fmaxf(most, p[n][key] * s);       // a NaN of p leaves it as it is
+                            }
+                    }
+                    most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+                    most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+                    const int e_new = min(max(e_v[n], rows_exponent(most) - 3), 119);              // now below 16
+                    rescale(n, rows_power(e_v[n] - e_new));
+                    e_v[n] = e_new;
+                    down_v[n] = rows_power(-e_new);
+                }
+            }
+            float pd[NR][4], up_v[NR];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) up_v[n] = rows_power(e_v[n]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int key = 0; key < 4; ++key) pd[n][key] = p[n][key] * down_v[n];
+
+            // ---- values ----
+            const uint8_t* vt = st + S::CODES;
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+                if (G > S::GH && grp % S::GH == 0) load_value_planes(grp);
+                const int gh = grp % S::GH;
+                uint32_t pb[NR][2];
+                float s[4], b[4];
+#pragma unroll
+                for (int key = 0; key < 4; ++key) {
+                    s[key] = key < 2 ? vs_lo.at(key, gh) : vs_hi.at(key - 2, gh);
+                    b[key] = key < 2 ? vb_lo.at(key, gh) : vb_hi.at(key - 2, gh);
+                    // planes that are not finite count as zeros, and a row whose probability there is not zero becomes NaN in this group
+                    if (broken && !(fabsf(s[key]) <= 3.402823466e38f && fabsf(b[key]) <= 3.402823466e38f)) {
+                        s[key] = b[key] = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < NR; ++n)
+                            if (p[n][key] > 0.0f) b_sum[n][grp] = __int_as_float(0x7FC00000);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    const float p0 = pd[n][0] * s[0], p1 = pd[n][1] * s[1], p2 = pd[n][2] * s[2], p3 = pd[n][3] * s[3];
+                    pb[n][0] = rows_half2(p0, p1);
+                    pb[n][1] = rows_half2(p2, p3);
+                    const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&pb[n][0])), r1 = __half22float2(*reinterpret_cast<const __half2*>(&pb[n][1]));
+                    b_sum[n][grp] = fmaf(kCentre * up_v[n], ((p0 - r0.x) + (p1 - r0.y)) + ((p2 - r1.x) + (p3 - r1.y)), b_sum[n][grp]);
+#pragma unroll
+                    for (int key = 0; key < 4; ++key) b_sum[n][grp] = fmaf(p[n][key], b[key], b_sum[n][grp]);
+                }
+                // A: rows g and g + 8 of m tile j are elements 8g + j and 8g + 4 + j of the group
+                uint32_t av[4][4];
+                if constexpr (BITS == 8) {
+                    uint2 w[4];
+#pragma unroll
+                    for (int key = 0; key < 4; ++key) w[key] = *reinterpret_cast<const uint2*>(vt + S::v_at(2 * t + (key & 1) + (key & 2) * 4, grp * 64 + 8 * g));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {               // tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+                        const uint2 wa = w[2 * h], wb = w[2 * h + 1];
+                        const uint32_t lo0 = gm_prmt(wa.x, wb.x, 0x5140), lo1 = gm_prmt(wa.x, wb.x, 0x7362), hi0 = gm_prmt(wa.y, wb.y, 0x5140), hi1 = gm_prmt(wa.y, wb.y, 0x7362);
+                        av[0][2 * h] = gm_prmt(lo0, 0, 0x4140); av[0][2 * h + 1] = gm_prmt(hi0, 0, 0x4140);
+                        av[1][2 * h] = gm_prmt(lo0, 0, 0x4342); av[1][2 * h + 1] = gm_prmt(hi0, 0, 0x4342);
+                        av[2][2 * h] = gm_prmt(lo1, 0, 0x4140); av[2][2 * h + 1] = gm_prmt(hi1, 0, 0x4140);
+                        av[3][2 * h] = gm_prmt(lo1, 0, 0x4342); av[3][2 * h + 1] = gm_prmt(hi1, 0, 0x4342);
+                    }
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int key = 0; key < 4; ++key) w[key] = *reinterpret_cast<const uint32_t*>(vt + S::v_at(2 * t + (key & 1) + (key & 2) * 4, grp * 32 + 4 * g));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t lo = gm_prmt(w[2 * h], w[2 * h + 1], 0x5410), hi = gm_prmt(w[2 * h], w[2 * h + 1], 0x7632);
+                        av[0][2 * h] = lo & 0x000F000Fu; av[0][2 * h + 1] = hi & 0x000F000Fu;
+                        av[1][2 * h] = lo & 0x00F000F0u; av[1][2 * h + 1] = hi & 0x00F000F0u;      // sixteen times the code
+                        av[2][2 * h] = lo >> 8 & 0x000F000Fu; av[2][2 * h + 1] = hi >> 8 & 0x000F000Fu;
+                        av[3][2 * h] = lo >> 8 & 0x00F000F0u; av[3][2 * h + 1] = hi >> 8 & 0x00F000F0u;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) rows_mma(o[n][grp][j], av[j][0], av[j][1], av[j][2], av[j][3], pb[n][0], pb[n][1]);
+            }
+
+            __syncwarp();                                      // the stage's values are in registers of all lanes
+            if (ahead) request(stage == 0 ? S::STAGES - 1 : stage - 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        }
+        item += segment;
+
+        // ---- the segment's result: out^T = 2^E 2^24 o + b_sum, over l ----
+        const bool whole = from_start && to_end;
+        float* part = a.partial + (size_t)(2 * worker + (from_start ? 1 : 0)) * RB * (D + 2);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            float sum = l[n];
+            sum += __shfl_xor_sync(kFullMask, sum, 1);
+            sum += __shfl_xor_sync(kFullMask, sum, 2);
+            if (!whole && t == 0 && g + 8 * n < (int)valid) {
+                part[g + 8 * n] = m[n];
+                part[RB + g + 8 * n] = sum;
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float up0 = rows_power(__shfl_sync(kFullMask, e_v[n], 8 * t)), up1 = rows_power(__shfl_sync(kFullMask, e_v[n], 8 * t + 4));
+            const float inv0 = __shfl_sync(kFullMask, inv, 8 * t), inv1 = __shfl_sync(kFullMask, inv, 8 * t + 4);
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+                float b = b_sum[n][grp];
+                b += __shfl_xor_sync(kFullMask, b, 1);
+                b += __shfl_xor_sync(kFullMask, b, 2);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {                  // rows 2t and 2t + 1
+                    const int r = 2 * t + c + 8 * n;
+                    const float bc = __shfl_sync(kFullMask, b, 8 * t + 4 * c);
+                    if (r >= (int)valid) continue;
+                    const float up = c ? up1 : up0;
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float unit = BITS == 4 && j % 2 ? 1048576.0f : 16777216.0f;
+                        v[j] = fmaf(up, unit * o[n][grp][j][c], bc);
+                        v[4 + j] = fmaf(up, unit * o[n][grp][j][2 + c], bc);
+                    }
+                    const int d = grp * 64 + 8 * g;
+                    if (whole) {
+                        const float i = c ? inv1 : inv0;
+                        const uint32_t flat = now.flat0 + r;
+                        uint16_t* dst = a.out + (size_t)(now.seq.row0 + flat / a.group) * a.out_stride + (size_t)(now.head * a.group + flat % a.group) * D + d;
+                        *reinterpret_cast<uint4*>(dst) = make_uint4(rows_pair<BF16>(v[0] * i, v[1] * i), rows_pair<BF16>(v[2] * i, v[3] * i),
+                                                                    rows_pair<BF16>(v[4] * i, v[5] * i), rows_pair<BF16>(v[6] * i, v[7] * i));
+                    } else {
+                        float* dst = part + 2 * RB + (size_t)r * D + d;
+                        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    }
+                }
+            }
+        }
+        if (!whole && from_start && lane == 0) {
+            ShareInfo& info = a.info[worker];
+            info.last = share_of_last(total, workers, item - segment + now.range.tiles);      // the unit begins in this share
+            info.row0 = now.seq.row0;
+            info.flat0 = now.flat0;
+            info.valid = valid;
+            info.head = now.head;
+            info.active = 1;
+        }
+        if (item < stop) now.next_unit(a);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Joins the shares of the unit that worker c's share ends in: the block's warps over its rows, and where it has few over the shares of a row.
+constexpr int kRowsCombineThreads = 256, kRowsCombineWarps = kRowsCombineThreads / kWarp;
+template <int D, int RB, bool BF16>
+__global__ void __launch_bounds__(kRowsCombineThreads)
+attention_rows_combine_kernel(const AttnArgs a) {
+    constexpr int VEC = D / 32, BATCH = 8;
+    constexpr size_t kSlot = (size_t)RB * (D + 2);
+    __shared__ float s_sum[kRowsCombineWarps][D + 1];
+    pdl_wait();
+    const uint32_t c = blockIdx.x;
+    const ShareInfo info = a.info[c];
+    if (!info.active) return;
+    const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, parts = info.last - c + 1;
+    const uint32_t rows_at_once = min(info.valid, (uint32_t)kRowsCombineWarps), per_row = kRowsCombineWarps / rows_at_once, sub = warp % per_row;
+    auto slot = [&](uint32_t p) { return a.partial + (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kSlot; };
+    for (uint32_t r0 = 0; r0 < info.valid; r0 += rows_at_once) {
+        const uint32_t r = r0 + warp / per_row;
+        const bool busy = warp / per_row < rows_at_once && r < info.valid;
+        float top = -INFINITY, sum = 0.0f, v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
+        if (busy) {
+            for (uint32_t p = lane; p < parts; p += kWarp) top = fmaxf(top, slot(p)[r]);
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+            const float base = top == -INFINITY ? 0.0f : top;
+            const uint32_t mine = (parts + per_row - 1 - sub) / per_row;             // shares sub, sub + per_row, ...
+            for (uint32_t i0 = 0; i0 < mine; i0 += BATCH) {
+                float w[BATCH], x[BATCH][VEC], l[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const bool is = i0 + i < mine;
+                    const float* s = slot(sub + (is ? i0 + i : 0) * per_row);
+                    w[i] = is ? s[r] : -INFINITY;
+                    l[i] = s[RB + r];
+                    const float* src = s + 2 * RB + (size_t)r * D + lane * VEC;
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) {
+                        const float2 y = *reinterpret_cast<const float2*>(src + e);
+                        x[i][e] = y.x;
+                        x[i][e + 1] = y.y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    if (i0 + i >= mine) break;
+                    const float f = exp2f(w[i] - base);
+                    sum = fmaf(f, l[i], sum);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[e] = fmaf(f, x[i][e], v[e]);
+                }
+            }
+        }
+        if (per_row > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s_sum[warp][lane * VEC + e] = v[e];
+            if (lane == 0) s_sum[warp][D] = sum;
+            __syncthreads();
+            if (sub == 0)
+                for (uint32_t k = 1; k < per_row; ++k) {
+                    sum += s_sum[warp + k][D];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[e] += s_sum[warp + k][lane * VEC + e];
+                }
+        }
+        if (!busy || sub != 0) continue;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const uint32_t flat = info.flat0 + r;
+        uint16_t* dst = a.out + (size_t)(info.row0 + flat / a.group) * a.out_stride + (size_t)(info.head * a.group + flat % a.group) * D + lane * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv, v[e + 1] * inv);
+    }
+}
+
+template <int D, int BITS, int RB, bool BF16>
+static tf_status launch_rows(tf_context* ctx, cudaStream_t st, const AttnArgs& a, const tf_attention_workspace* ws) {
+    using S = RowsShape<D, BITS, RB>;
+    auto kernel = attention_rows_kernel<D, BITS, RB, BF16>;
+    static DeviceSmemCache smem_cache;
+    static ResidentBlocksCache blocks_cache;
+    const tf_status s = ensure_dynamic_smem(ctx, kernel, smem_cache, S::SMEM);
+    if (s != TF_OK) return s;
+    uint32_t blocks = resident_blocks(ctx, kernel, blocks_cache, S::THREADS, S::SMEM);
+    blocks = lesser(blocks, lesser(ws->row_capacity / RB, ws->max_workers) / S::WARPS);
+    TF_REQUIRE(ctx, blocks > 0, TF_ERR_CUDA, "tf_tree_attention: the kernel does not fit on the device");
+    kernel<<<blocks, S::THREADS, S::SMEM, st>>>(a);
+    const tf_status t = check_launch(ctx, "tf_tree_attention");
+    if (t != TF_OK) return t;
+    TF_CUDA(ctx, launch_pdl(attention_rows_combine_kernel<D, RB, BF16>, dim3(blocks * S::WARPS), dim3(kRowsCombineThreads), 0, st, a));
+    return check_launch(ctx, "tf_tree_attention (join)");
+}
+
+}  // namespace tf
