@@ -21,12 +21,16 @@ tf_status tf_attention_workspace_create(tf_context* ctx, uint32_t head_dim, tf_a
     const uint64_t partial = (uint64_t)2 * ws->row_capacity * (head_dim + 2) * sizeof(float), info = (uint64_t)ws->max_workers * sizeof(tf::ShareInfo);
     cudaError_t e = cudaMalloc(&ws->partial, partial);
     if (e == cudaSuccess) e = cudaMalloc(&ws->info, info);
+    const uint64_t tickets = (uint64_t)3 * 2 * ws->max_workers * sizeof(uint32_t);      // kJoin^3 shares are more than there are workers
+    if (e == cudaSuccess) e = cudaMalloc(&ws->tickets, tickets);
+    if (e == cudaSuccess) e = cudaMemset(ws->tickets, 0, tickets);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);                  // calls may come on streams that do not wait for this one
     if (e != cudaSuccess) {
         cudaGetLastError();
         tf_attention_workspace_destroy(ws);
         return tf::fail(ctx, TF_ERR_OUT_OF_MEMORY, "%s: %s", name, cudaGetErrorString(e));
     }
-    ws->bytes = partial + info;
+    ws->bytes = partial + info + tickets;
     *out = ws;
     return TF_OK;
 }
@@ -36,6 +40,7 @@ void tf_attention_workspace_destroy(tf_attention_workspace* ws) {
     const tf::DeviceScope scope(ws->device);
     if (ws->partial) cudaFree(ws->partial);
     if (ws->info) cudaFree(ws->info);
+    if (ws->tickets) cudaFree(ws->tickets);
     delete ws;
 }
 
@@ -77,7 +82,7 @@ tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32
     a.table = {batch->page_table, batch->page_table_stride, cache->num_pages, tf::log2_of(cache->page_size)};
     a.row_offsets = batch->row_offsets; a.context_lengths = batch->context_lengths; a.positions = batch->positions;
     a.mask = reinterpret_cast<const unsigned long long*>(tree_mask); a.mask_words = mask_words;
-    a.partial = ws->partial; a.info = static_cast<tf::ShareInfo*>(ws->info);
+    a.partial = ws->partial; a.info = static_cast<tf::ShareInfo*>(ws->info); a.tickets = ws->tickets; a.ticket_stride = 2 * ws->max_workers;
     a.error = ctx->device_error;
     a.q_stride = q_stride; a.out_stride = out_stride;
     a.sequences = batch->sequences; a.rows = batch->rows; a.kv_heads = cache->kv_heads; a.group = group;

@@ -9,6 +9,7 @@ struct tf_attention_workspace {
     uint64_t bytes = 0;
     float* partial = nullptr;      // [2 x blocks][rows][head_dim + 2]
     void* info = nullptr;          // [max_workers] ShareInfo
+    uint32_t* tickets = nullptr;   // [3 levels][2 x max_workers], zero between calls
 };
 
 namespace tf {

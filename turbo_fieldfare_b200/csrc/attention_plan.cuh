@@ -22,10 +22,14 @@ struct AttnArgs {
     const unsigned long long* mask;
     float* partial;
     ShareInfo* info;
+    uint32_t* tickets;        // [levels][ticket_stride], zero between calls
+    uint32_t ticket_stride;
     uint32_t* error;
     uint32_t q_stride, out_stride, sequences, rows, kv_heads, group, mask_words, window;
     float scale;
 };
+
+constexpr int kJoin = 16;             // shares that are joined at a time
 
 template <typename T>
 __host__ __device__ __forceinline__ T lesser(T a, T b) { return a < b ? a : b; }
@@ -59,7 +63,9 @@ struct UnitRange {
         int64_t low = 0;
         if (a.window) low = s.context + (a.mask ? 0 : (int64_t)first) - (int64_t)a.window + 1;
         if (low < 0) low = 0;
-        end = lesser(s.context + drafted, (int64_t)a.table.stride << a.table.page_log2);
+        // (and below 2^31 less a tile, so that tokens are 32-bit numbers: a cache of more would be 2^37 bytes at the least)
+        end = lesser(lesser(s.context + drafted, (int64_t)a.table.stride << a.table.page_log2), (int64_t)0x7FFFFF00);
+        if (low > end) low = end;
         tile0 = low / tile;
         const int64_t stop = (end + tile - 1) / tile;
         tiles = stop > tile0 ? (uint32_t)(stop - tile0) : 1u;

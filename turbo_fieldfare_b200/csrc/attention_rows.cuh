@@ -2,15 +2,17 @@
 //
 // What bounds it is HBM: a cached token's codes and planes are read once and used for a handful of rows. So everything that is not
 // unpacking is kept out of the way. A worker is one warp: it owns its share of the tiles (16 tokens each), its ring of stages, filled by its own
-// cp.async, its running maximum, sum and product; no thread block ever meets at a barrier, and the shares of a unit are joined by
-// attention_rows_combine_kernel in the workers' order, which is a property of the lengths alone.
+// cp.async, its running maximum, sum and product; no thread block meets at a barrier after the start, and the shares of a unit are joined
+// by the worker that is the last to leave one (rows_join), in the workers' order, which is a property of the lengths alone.
 //
-// Logits, S[row][token] = Q K^T (mma.sync m16n8k16, rows as A, tokens as B): an 8-bit code c enters as the fp16 subnormal c * 2^-24 (one PRMT
+// Logits, S^T[token][row] = K Q^T (mma.sync m16n8k16, tokens as A, rows as B): an 8-bit code c enters as the fp16 subnormal c * 2^-24 (one PRMT
 // per two codes), a 4-bit one as c * 2^-24 or, against a q pre-scaled by 1/16, c * 2^-20 (one AND). Scale and bias come in fp32 per
-// group: s (q . c) + b sum(q). The accumulators of S hold (row g; tokens 2t, 2t + 1), which is the B fragment of the second product,
+// group: s (q . c) + b sum(q). An 8x8 transpose of the logits (movmatrix on their halves, exact) gives a lane row g and the tokens
+// 2t, 2t + 1, which is the B fragment of the second product,
 // O^T[element][row] = V^T P^T, with V's codes as A, again as subnormals: the value scale goes into the probability, p' = p s 2^-E rounded to
-// fp16, and what the bias adds is summed in fp32, sum p b. So that the rounding of p' weighs a code's distance from the centre of the codes, not the code
-// itself, sum (p s - 2^E p') * centre is added to that sum. E is a row's own, after the largest p s so far (tokens that it does not see have p = 0
+// fp16, and what the bias adds is summed in fp32. The rounding of p' shall weigh a code's distance from the centre of the codes, not the code
+// itself: sum p' (c - centre) = sum p' c - centre sum p', with sum p' of all groups by one more MMA each into the rows of a common
+// accumulator, against sum p (b + centre s). E is a row's own, after the largest p s so far (tokens that it does not see have p = 0
 // and no say), and m a maximum that is raised only when a logit exceeds it by 8: a vote each per tile, and what was summed is rescaled
 // only when one of them moves.
 #pragma once
@@ -53,6 +55,11 @@ __device__ __forceinline__ void rows_mma(float (&c)[4], uint32_t a0, uint32_t a1
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The first product of a chain.
+__device__ __forceinline__ void rows_mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ float rows_exp2(float x) {          // 2^x; results below fp32's normal range are zero
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -74,6 +81,19 @@ __device__ __forceinline__ uint32_t rows_pair(float lo, float hi) {
 __device__ __forceinline__ int rows_exponent(float v) { return max(-126, min((int)((__float_as_uint(v) >> 23) & 255u) - 127, 126)); }
 __device__ __forceinline__ float rows_power(int e) { return __uint_as_float((uint32_t)(max(-126, min(e, 127)) + 127) << 23); }
 
+// bf16 values of one token in the N groups from `first` on, of planes of G groups.
+template <int G, int N>
+struct TokenPlane {
+    uint32_t w[N / 2 + (N == 1)];
+    __device__ __forceinline__ void load(const uint8_t* plane, int token, int first) {
+        const uint8_t* p = plane + token * (2 * G) + 2 * first;
+        if constexpr (N == 1) w[0] = *reinterpret_cast<const uint16_t*>(p);
+        else if constexpr (N == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+    }
+    __device__ __forceinline__ float at(int grp) const { return __uint_as_float(grp % 2 ? w[grp / 2] & 0xFFFF0000u : w[grp / 2] << 16); }
+};
+
 // bf16 values of two neighbouring tokens (2i, then 2i + 1) in the N groups from `first` on, of planes of G groups. N = 1: one word holds both.
 template <int G, int N>
 struct PlanePair {
@@ -92,6 +112,10 @@ struct PlanePair {
         const int i = token * N + grp;
         return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
     }
+    __device__ __forceinline__ void raise_all(__nv_bfloat162& most) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+    }
     // The largest magnitudes of either token so far, in both halves of its word (N = 1: both tokens' in the first word); a NaN stays.
     __device__ __forceinline__ void raise(__nv_bfloat162& most0, __nv_bfloat162& most1) const {
         auto word = [&](int i) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])); };
@@ -105,6 +129,109 @@ struct PlanePair {
         }
     }
 };
+
+// Zeros in the place of value planes that are not finite; bit key * G + grp: it was so at the lane's token `key` (2t, 2t + 1, 2t + 8, 2t + 9).
+template <int G>
+__device__ __noinline__ uint32_t rows_sanitise(uint8_t* scales, int plane_bytes, int t) {
+    uint16_t *vs = reinterpret_cast<uint16_t*>(scales), *vb = reinterpret_cast<uint16_t*>(scales + plane_bytes);
+    uint32_t flags = 0;
+    for (int i = 0; i < 4 * G; ++i) {
+        const int at = (2 * t + (i / G & 1) + (i / G & 2) * 4) * G + i % G;
+        if ((vs[at] & 0x7F80) == 0x7F80 || (vb[at] & 0x7F80) == 0x7F80) flags |= 1u << i;
+    }
+    __syncwarp();                                              // all lanes have seen them
+    for (int i = 0; i < 4 * G; ++i)
+        if (flags >> i & 1u) {
+            const int at = (2 * t + (i / G & 1) + (i / G & 2) * 4) * G + i % G;
+            vs[at] = vb[at] = 0;                               // the lanes of a column write the same
+        }
+    __syncwarp();
+    return flags;
+}
+
+// Joins the shares of a unit, sixteen at a time: the worker that is the last to leave its share of a group joins the group, in the order of the
+// shares, into the place of its first, and goes on as that group's worker among the groups. Tickets are back at zero when their
+// group is joined. Part 0 lies in worker c0's second slot, part i in worker c0 + i's first.
+template <int D, int RB, bool BF16>
+__device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_t head, uint32_t flat0, uint32_t c0, uint32_t i, uint32_t parts, uint32_t valid, int lane) {
+    constexpr int VEC = D / 32, BATCH = 4;
+    constexpr size_t kSlot = (size_t)RB * (D + 2);
+    auto place = [&](uint32_t p) { return p == 0 ? 2 * c0 + 1 : 2 * (c0 + p); };
+    uint32_t span = 1;
+    for (uint32_t* tickets = a.tickets; parts > 1; tickets += a.ticket_stride, span *= kJoin) {
+        const uint32_t group = i / kJoin, base = group * kJoin, members = min((uint32_t)kJoin, parts - base);
+        __threadfence();                                       // this worker's share, or the group that it joined, before its ticket
+        __syncwarp();
+        uint32_t old = 0;
+        if (lane == 0) old = atomicAdd(tickets + place(base * span), 1u);
+        if (__shfl_sync(kFullMask, old, 0) != members - 1) return;
+        if (lane == 0) tickets[place(base * span)] = 0;
+        __threadfence();
+        const bool final = parts <= kJoin;
+        float* first = a.partial + place(base * span) * kSlot;
+        for (uint32_t r = 0; r < valid; ++r) {
+            const float* mine = a.partial + place((base + min((uint32_t)lane, members - 1)) * span) * kSlot;      // the slots may have been in L1 before
+            const float mp = (uint32_t)lane < members ? __ldcg(mine + r) : -INFINITY, lp = (uint32_t)lane < members ? __ldcg(mine + RB + r) : 0.0f;
+            float top = mp;
+#pragma unroll
+            for (int off = kJoin / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+            top = __shfl_sync(kFullMask, top, 0);
+            const float w = (uint32_t)lane < members ? exp2f(mp - (top == -INFINITY ? 0.0f : top)) : 0.0f;
+            float sum = 0.0f, v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
+            for (uint32_t p0 = 0; p0 < members; p0 += BATCH) {
+                float2 x[BATCH][VEC / 2];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    if (p0 + k >= members) break;
+                    const float2* src = reinterpret_cast<const float2*>(a.partial + place((base + p0 + k) * span) * kSlot + 2 * RB + (size_t)r * D + lane * VEC);
+#pragma unroll
+                    for (int e = 0; e < VEC / 2; ++e) x[k][e] = __ldcg(src + e);
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    if (p0 + k >= members) break;
+                    const float wk = __shfl_sync(kFullMask, w, p0 + k);
+                    sum = fmaf(wk, __shfl_sync(kFullMask, lp, p0 + k), sum);
+#pragma unroll
+                    for (int e = 0; e < VEC / 2; ++e) {
+                        v[2 * e] = fmaf(wk, x[k][e].x, v[2 * e]);
+                        v[2 * e + 1] = fmaf(wk, x[k][e].y, v[2 * e + 1]);
+                    }
+                }
+            }
+            if (final) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const uint32_t flat = flat0 + r;
+                uint16_t* dst = a.out + (size_t)(row0 + flat / a.group) * a.out_stride + (size_t)(head * a.group + flat % a.group) * D + lane * VEC;
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv, v[e + 1] * inv);
+            } else {
+                if (lane == 0) {
+                    first[r] = top;
+                    first[RB + r] = sum;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) *reinterpret_cast<float2*>(first + 2 * RB + (size_t)r * D + lane * VEC + e) = make_float2(v[e], v[e + 1]);
+            }
+        }
+        parts = (parts + kJoin - 1) / kJoin;
+        i = group;
+    }
+}
+
+template <int RB>
+__device__ __noinline__ void rows_next_unit(const AttnArgs& a, Cursor<RB, kRowsTile>& c) { c.next_unit(a); }
+
+// 8x8 transpose over a warp of fp32 values, exact: lane (g, t) gives elements (g, 2t) and (g, 2t + 1) and gets (2t, g) and (2t + 1, g).
+__device__ __forceinline__ void rows_transpose(float& x0, float& x1) {
+    uint32_t lo = gm_prmt(__float_as_uint(x0), __float_as_uint(x1), 0x5410), hi = gm_prmt(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(lo));
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(hi));
+    x0 = __uint_as_float(gm_prmt(lo, hi, 0x5410));
+    x1 = __uint_as_float(gm_prmt(lo, hi, 0x7632));
+}
 
 template <int D, int BITS, int RB, bool BF16>
 __global__ void __launch_bounds__(RowsShape<D, BITS, RB>::THREADS, RowsShape<D, BITS, RB>::BLOCKS)
@@ -166,7 +293,6 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
         __syncthreads();
     }
     const uint32_t workers = (uint32_t)lesser((uint64_t)workers_max, total);
-    if (lane == 0) a.info[worker].active = 0;
     if (worker >= workers) return;
     uint64_t item = share_begin(total, workers, worker);
     const uint64_t stop = share_begin(total, workers, worker + 1);
@@ -175,26 +301,45 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
     now.seq.load(a, now.b, false);
     now.range.set(a, now.seq, now.flat0, RB, kRowsTile);
 
-    // ---- this warp's ring ----
+    // ---- this warp's ring: what the next request needs is in registers, the rest of its cursor in memory ----
     uint8_t* ring = smem + warp * (S::STAGES * S::STAGE);
-    uint2* q_shared = reinterpret_cast<uint2*>(smem + W * S::STAGES * S::STAGE + warp * S::Q_BYTES) + lane;       // [D / 16][lanes]
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+    uint2* q_shared = reinterpret_cast<uint2*>(smem + W * S::STAGES * S::STAGE + warp * S::Q_BYTES) + lane;       // [D / 16][lanes]
     Cursor<RB, kRowsTile> next = now;
     uint32_t ahead = (uint32_t)(stop - item);                  // tiles not requested yet
     uint32_t there = 0;                                        // a bit per stage: its tile has a page
-    int32_t next_page = a.table.page(next.b, next.token0());
+    uint32_t next_left, next_token, next_end, next_head;
+    const int32_t* next_table;
+    int32_t next_page;
+    auto look_up = [&] {
+        next_page = -1;
+        if (next_token < next_end) {
+            const int32_t p = next_table[next_token >> a.table.page_log2];
+            if (p >= 0 && (uint32_t)p < a.table.pages) next_page = p;
+        }
+    };
+    auto enter_unit = [&] {
+        next_left = next.range.tiles - next.tile;
+        next_token = (uint32_t)next.token0();
+        next_end = (uint32_t)next.range.end;
+        next_head = next.head;
+        next_table = a.table.table + (size_t)next.b * a.table.stride;
+        look_up();
+    };
+    const uint32_t k_dst = S::k_at(lane / S::PIECES, lane % S::PIECES * 16), v_dst = S::CODES + S::v_at(lane / S::PIECES, lane % S::PIECES * 16);
     auto request = [&](uint32_t stage) {
         there &= ~(1u << stage);
         if (next_page >= 0) {
             there |= 1u << stage;
-            const size_t row = (((size_t)next_page * a.kv_heads + next.head) << a.table.page_log2) + ((uint32_t)next.token0() & ((1u << a.table.page_log2) - 1u));
+            const size_t row = (((size_t)next_page * a.kv_heads + next_head) << a.table.page_log2) + (next_token & ((1u << a.table.page_log2) - 1u));
             const uint32_t base = ring_addr + stage * S::STAGE;
             const uint8_t *kc = a.k.codes + row * S::ROW + lane * 16, *vc = a.v.codes + row * S::ROW + lane * 16;
 #pragma unroll
-            for (int i = 0; i < (kRowsTile * S::PIECES) / kWarp; ++i) {
-                const uint32_t id = lane + i * kWarp, r = id / S::PIECES, byte = id % S::PIECES * 16;
-                rows_cp_async(base + S::k_at(r, byte), kc + i * 512);
-                rows_cp_async(base + S::CODES + S::v_at(r, byte), vc + i * 512);
+            for (int i = 0; i < kRowsTile * S::PIECES / kWarp; ++i) {
+                // rows first and on of the tile: their swizzle on top of the lane's own
+                const uint32_t first = i * kWarp / S::PIECES, k_more = S::k_at(first, 0) ^ (first * S::ROW), v_more = S::v_at(first, 0) ^ (first * S::ROW);
+                rows_cp_async(((base + k_dst) ^ k_more) + i * 512, kc + i * 512);
+                rows_cp_async(((base + v_dst) ^ v_more) + i * 512, vc + i * 512);
             }
             // planes: 2 G pieces each
             if (8 * G >= kWarp || lane < 8 * G) {
@@ -202,31 +347,45 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 for (int i = 0; i < (8 * G + kWarp - 1) / kWarp; ++i) {
                     const uint32_t id = lane + i * kWarp, plane = id / (2 * G), c = id % (2 * G);
                     const uint16_t* src = plane == 0 ? a.k.scales : plane == 1 ? a.k.biases : plane == 2 ? a.v.scales : a.v.biases;
-                    rows_cp_async(base + 2 * S::CODES + plane * S::PLANE + c * 16, src + row * G + c * 8);
+                    rows_cp_async(base + 2 * S::CODES + id * 16, src + row * G + c * 8);
                 }
             }
         }
         if (--ahead) {
-            next.advance(a);
-            next_page = next.token0() < next.range.end ? a.table.page(next.b, next.token0()) : -1;
+            if (--next_left) {
+                next_token += kRowsTile;
+                look_up();
+            } else {
+                rows_next_unit(a, next);
+                enter_unit();
+            }
         }
     };
-    if (next.token0() >= next.range.end) next_page = -1;
+    enter_unit();
 #pragma unroll 1
     for (int i = 0; i < S::STAGES - 1; ++i) {
         if (ahead) request(i);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
+    // ---- where this lane reads: codes of tokens g and g + 8 (K), of tokens 2t, 2t + 1, 2t + 8, 2t + 9 (V) ----
+    constexpr int KB = BITS * 8, KV = 128 / KB < G ? 128 / KB : G;           // bytes of a group; groups whose swizzles differ
+    uint32_t k_off[KV], v_off[KV];
+#pragma unroll
+    for (int i = 0; i < KV; ++i) {
+        k_off[i] = S::k_at(g, i * KB + t * (BITS * 2));
+        v_off[i] = S::CODES + S::v_at(2 * t, i * KB + g * BITS);
+    }
+
     uint32_t stage = 0;
     while (item < stop) {
-        // ---- a unit's segment: the rows of q as A fragments, their sums per group, what they see ----
+        // ---- a unit's segment: the rows of q as B fragments, their sums per group, what they see ----
         const uint32_t valid = (uint32_t)lesser((uint64_t)RB, now.flat_rows(a) - now.flat0);
-        const bool from_start = now.tile == 0;
-        const uint32_t segment = (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), stop - item);
-        const bool to_end = now.tile + segment == now.range.tiles;
+        const uint32_t first_tile = now.tile;
+        const uint32_t segment = (uint32_t)lesser((uint64_t)(now.range.tiles - first_tile), stop - item);
+        const bool from_start = first_tile == 0, whole = from_start && segment == now.range.tiles;
         uint32_t qf[NR][S::Q_SHARED ? 1 : D / 16][2];
-        float q_sum[NR][G], factor[NR], m[NR], l[NR], b_sum[NR][G];
+        float q_sum[NR][G][2], factor[NR], m[NR], l[NR], b_sum[NR][G];       // q_sum: of rows 2t and 2t + 1; the others: of row g
         int32_t low[NR];                                       // first token that the row sees, from the unit's first tile on
         uint32_t node[NR];
         int32_t low_most = 0;
@@ -287,7 +446,9 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 }
                 sum += __shfl_xor_sync(kFullMask, sum, 1);
                 sum += __shfl_xor_sync(kFullMask, sum, 2);
-                q_sum[n][grp] = sum * 5.9604644775390625e-8f;  // 2^-24, as the products
+                sum *= 5.9604644775390625e-8f;                 // 2^-24, as the products
+                q_sum[n][grp][0] = __shfl_sync(kFullMask, sum, 8 * t);
+                q_sum[n][grp][1] = __shfl_sync(kFullMask, sum, 8 * t + 4);
                 b_sum[n][grp] = 0.0f;
             }
             factor[n] = 16777216.0f * rows_power(e) * a.scale * 1.4426950408889634f;
@@ -302,108 +463,109 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             low_most = max(low_most, low[n]);
         }
         if (a.window) low_most = (int32_t)__reduce_max_sync(kFullMask, (uint32_t)low_most);
-        float o[NR][G][4][4];
+        float o[NR][G][4][4], ones[NR][4];                     // ones: sums of the rounded p', row grp for group grp
         int e_v[NR];                                           // exponent that the row's products p s are divided by, and 2^-E
         float down_v[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
+            ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0.0f;
             e_v[n] = -126;
             down_v[n] = rows_power(126);
-        }
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
 #pragma unroll
             for (int grp = 0; grp < G; ++grp)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[n][grp][j][0] = o[n][grp][j][1] = o[n][grp][j][2] = o[n][grp][j][3] = 0.0f;
-        // tokens of the segment before this place are seen by every row without a look at a mask, if their tile starts at low_most or later
-        const int64_t open_end = lesser(now.seq.context, now.range.end) - now.range.tile0 * kRowsTile;
-        int32_t rel0 = now.tile * kRowsTile;
+        }
+        // From the unit's first tile on: tokens before open_end are cached ones; every row sees them from low_most on.
+        const int32_t base_token = (int32_t)(now.range.tile0 * kRowsTile), open_end = (int32_t)(lesser(now.seq.context, now.range.end) - base_token),
+                      end_rel = (int32_t)(now.range.end - base_token);
+        int32_t rel0 = first_tile * kRowsTile;
 
 #pragma unroll 1
-        for (uint32_t done = 0; done < segment; ++done, rel0 += kRowsTile) {
+        for (uint32_t left = segment; left; --left, rel0 += kRowsTile) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
             __syncwarp();
             const uint8_t* st = ring + stage * S::STAGE;
-            const bool has_page = there >> stage & 1u;
 
-            // ---- logits: n tile 0 holds tokens 0 to 7, n tile 1 tokens 8 to 15 ----
-            float x[2][4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) x[0][c] = x[1][c] = 0.0f;
-            PlanePair<G, S::GH> ks_lo, ks_hi, kb_lo, kb_hi;
+            // ---- logits: rows of the accumulator are tokens g and g + 8, columns the rows 2t and 2t + 1 of q ----
+            float x[NR][4] = {};
+            const uint8_t* planes = st + 2 * S::CODES;
+            TokenPlane<G, S::GH> ks_lo, ks_hi, kb_lo, kb_hi;
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
                 if (grp % S::GH == 0) {
-                    ks_lo.load(st + 2 * S::CODES, t, grp); ks_hi.load(st + 2 * S::CODES, t + 4, grp);
-                    kb_lo.load(st + 2 * S::CODES + S::PLANE, t, grp); kb_hi.load(st + 2 * S::CODES + S::PLANE, t + 4, grp);
+                    ks_lo.load(planes, g, grp); ks_hi.load(planes, g + 8, grp);
+                    kb_lo.load(planes + S::PLANE, g, grp); kb_hi.load(planes + S::PLANE, g + 8, grp);
                 }
                 const int gh = grp % S::GH;
                 uint32_t w[2][4];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
+                    const uint8_t* at = st + k_off[grp % KV] + grp / KV * 128 + n * 8 * S::ROW;
                     if constexpr (BITS == 8) {
-                        const uint4 c = *reinterpret_cast<const uint4*>(st + S::k_at(g + 8 * n, grp * 64 + 16 * t));
+                        const uint4 c = *reinterpret_cast<const uint4*>(at);
                         w[n][0] = c.x; w[n][1] = c.y; w[n][2] = c.z; w[n][3] = c.w;
                     } else {
-                        const uint2 c = *reinterpret_cast<const uint2*>(st + S::k_at(g + 8 * n, grp * 32 + 8 * t));
+                        const uint2 c = *reinterpret_cast<const uint2*>(at);
                         w[n][0] = c.x; w[n][1] = c.x >> 8; w[n][2] = c.y; w[n][3] = c.y >> 8;
                     }
                 }
-                float acc[2][4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[0][c] = acc[1][c] = 0.0f;
+                float acc[NR][4];
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
-                    uint2 qs;
-                    if constexpr (S::Q_SHARED) qs = q_shared[(grp * 4 + ks) * kWarp];
-                    else qs = make_uint2(qf[0][grp * 4 + ks][0], qf[0][grp * 4 + ks][1]);
+                    uint32_t a0, a1, a2, a3;
+                    if constexpr (BITS == 8) {
+                        a0 = gm_prmt(w[0][ks], 0, 0x4140); a1 = gm_prmt(w[1][ks], 0, 0x4140);
+                        a2 = gm_prmt(w[0][ks], 0, 0x4342); a3 = gm_prmt(w[1][ks], 0, 0x4342);
+                    } else {
+                        a0 = w[0][ks] & 0x000F000Fu; a1 = w[1][ks] & 0x000F000Fu;
+                        a2 = w[0][ks] & 0x00F000F0u; a3 = w[1][ks] & 0x00F000F0u;
+                    }
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        uint32_t b0, b1;
-                        if constexpr (BITS == 8) {
-                            b0 = gm_prmt(w[n][ks], 0, 0x4140);
-                            b1 = gm_prmt(w[n][ks], 0, 0x4342);
-                        } else {
-                            b0 = w[n][ks] & 0x000F000Fu;
-                            b1 = w[n][ks] & 0x00F000F0u;
-                        }
-                        if constexpr (NR == 2) rows_mma(acc[n], qs.x, qf[NR - 1][grp * 4 + ks][0], qs.y, qf[NR - 1][grp * 4 + ks][1], b0, b1);
-                        else rows_mma(acc[n], qs.x, 0u, qs.y, 0u, b0, b1);
+                    for (int n = 0; n < NR; ++n) {
+                        uint2 q;
+                        if constexpr (S::Q_SHARED) q = q_shared[(grp * 4 + ks) * kWarp];
+                        else q = make_uint2(qf[n][grp * 4 + ks][0], qf[n][grp * 4 + ks][1]);
+                        if (ks == 0) rows_mma_first(acc[n], a0, a1, a2, a3, q.x, q.y);
+                        else rows_mma(acc[n], a0, a1, a2, a3, q.x, q.y);
                     }
                 }
+                const float s0 = ks_lo.at(gh), s1 = ks_hi.at(gh), b0 = kb_lo.at(gh), b1 = kb_hi.at(gh);
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    x[0][2 * n] = fmaf(ks_lo.at(0, gh), acc[0][2 * n], fmaf(kb_lo.at(0, gh), q_sum[n][grp], x[0][2 * n]));
-                    x[0][2 * n + 1] = fmaf(ks_lo.at(1, gh), acc[0][2 * n + 1], fmaf(kb_lo.at(1, gh), q_sum[n][grp], x[0][2 * n + 1]));
-                    x[1][2 * n] = fmaf(ks_hi.at(0, gh), acc[1][2 * n], fmaf(kb_hi.at(0, gh), q_sum[n][grp], x[1][2 * n]));
-                    x[1][2 * n + 1] = fmaf(ks_hi.at(1, gh), acc[1][2 * n + 1], fmaf(kb_hi.at(1, gh), q_sum[n][grp], x[1][2 * n + 1]));
+                    x[n][0] = fmaf(s0, acc[n][0], fmaf(b0, q_sum[n][grp][0], x[n][0]));
+                    x[n][1] = fmaf(s0, acc[n][1], fmaf(b0, q_sum[n][grp][1], x[n][1]));
+                    x[n][2] = fmaf(s1, acc[n][2], fmaf(b1, q_sum[n][grp][0], x[n][2]));
+                    x[n][3] = fmaf(s1, acc[n][3], fmaf(b1, q_sum[n][grp][1], x[n][3]));
                 }
             }
+            // from here on a lane has row g (+ 8 n) and the tokens 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-                x[0][2 * n] *= factor[n]; x[0][2 * n + 1] *= factor[n];
-                x[1][2 * n] *= factor[n]; x[1][2 * n + 1] *= factor[n];
+                rows_transpose(x[n][0], x[n][1]);
+                rows_transpose(x[n][2], x[n][3]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[n][c] *= factor[n];
             }
-            if (!(has_page && rel0 >= low_most && rel0 + kRowsTile <= open_end)) {
-                if (!has_page && lane == 0 && rel0 + now.range.tile0 * kRowsTile < now.range.end) *a.error = kErrKvPage;
+            if (!((there >> stage & 1u) && rel0 >= low_most && rel0 + kRowsTile <= open_end)) {
+                const bool has_page = there >> stage & 1u;
+                if (!has_page && lane == 0 && rel0 < end_rel) *a.error = kErrKvPage;
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int32_t rel = rel0 + 2 * t + (c & 1) + (c & 2) * 4;
-                        const int64_t token = now.range.tile0 * kRowsTile + rel;
-                        bool seen = has_page && g + 8 * n < (int)valid && token < now.range.end;
+                        bool seen = has_page && g + 8 * n < (int)valid && rel < end_rel;
                         if (seen) {
-                            if (token < now.seq.context) {
+                            if (rel < open_end) {
                                 seen = rel >= low[n];
                             } else {
-                                const uint32_t j = (uint32_t)(token - now.seq.context);
+                                const uint32_t j = (uint32_t)((int64_t)base_token + rel - now.seq.context);
                                 if (a.mask) seen = (a.mask[(size_t)(now.seq.row0 + node[n]) * a.mask_words + (j >> 6)] >> (j & 63u)) & 1ull;
                                 else seen = j <= node[n] && (!a.window || node[n] - j < a.window);
                             }
                         }
-                        if (!seen) x[c >> 1][2 * n + (c & 1)] = -INFINITY;
+                        if (!seen) x[n][c] = -INFINITY;
                     }
                 }
             }
@@ -411,11 +573,11 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             // ---- does a maximum move? ----
             float over = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NR; ++n)
-                over = fmaxf(over, fmaxf(fmaxf(x[0][2 * n], x[0][2 * n + 1]), fmaxf(x[1][2 * n], x[1][2 * n + 1])) - m[n]);
+            for (int n = 0; n < NR; ++n) over = fmaxf(over, fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) - m[n]);
             // what was summed of rows g + 8 n, times f: their accumulators lie in the columns of other lanes
             auto rescale = [&](int n, float f) {
                 const float f0 = __shfl_sync(kFullMask, f, 8 * t), f1 = __shfl_sync(kFullMask, f, 8 * t + 4);      // rows 2t, 2t + 1
+                ones[n][0] *= f0; ones[n][1] *= f1;
 #pragma unroll
                 for (int grp = 0; grp < G; ++grp)
 #pragma unroll
@@ -424,7 +586,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             if (__any_sync(kFullMask, over > 8.0f)) {
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    float top = fmaxf(fmaxf(x[0][2 * n], x[0][2 * n + 1]), fmaxf(x[1][2 * n], x[1][2 * n + 1]));
+                    float top = fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
                     top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
                     const float m_new = fmaxf(m[n], top), alpha = m_new == -INFINITY ? 1.0f : rows_exp2(m[n] - m_new);
@@ -442,12 +604,12 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             for (int n = 0; n < NR; ++n) {
                 const float base = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) p[n][c] = rows_exp2(x[c >> 1][2 * n + (c & 1)] - base);
+                for (int c = 0; c < 4; ++c) p[n][c] = rows_exp2(x[n][c] - base);
                 l[n] += (p[n][0] + p[n][1]) + (p[n][2] + p[n][3]);
             }
 
             // ---- does a row's exponent move, is a value plane not finite? ----
-            const uint8_t *vs_plane = st + 2 * S::CODES + 2 * S::PLANE, *vb_plane = vs_plane + S::PLANE;
+            const uint8_t *vs_plane = planes + 2 * S::PLANE, *vb_plane = vs_plane + S::PLANE;
             PlanePair<G, S::GH> vs_lo, vs_hi, vb_lo, vb_hi;
             auto load_value_planes = [&](int first) {
                 vs_lo.load(vs_plane, t, first); vs_hi.load(vs_plane, t + 4, first);
@@ -459,7 +621,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             for (int first = 0; first < G; first += S::GH) {
                 load_value_planes(first);
                 vs_lo.raise(most_s[0], most_s[1]); vs_hi.raise(most_s[2], most_s[3]);
-                vb_lo.raise(most_b, most_b); vb_hi.raise(most_b, most_b);
+                vb_lo.raise_all(most_b); vb_hi.raise_all(most_b);
             }
             bool moves = !__hble2(most_b, finite);
 #pragma unroll
@@ -474,44 +636,53 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 }
                 moves |= !(most * down_v[n] < 16384.0f);
             }
-            bool broken = false;
             if (__any_sync(kFullMask, moves)) {
                 bool bad = !__hble2(most_b, finite);
 #pragma unroll
                 for (int key = 0; key < 4; ++key) bad |= !__hble2(most_s[key], finite);
-                broken = __any_sync(kFullMask, bad);
+                if (__any_sync(kFullMask, bad)) {
+                    // Planes that are not finite become zeros in the stage, and a row whose probability there is not zero a NaN in that group.
+                    const uint32_t flags = rows_sanitise<G>(ring + stage * S::STAGE + 2 * S::CODES + 2 * S::PLANE, S::PLANE, t);
+#pragma unroll
+                    for (int key = 0; key < 4; ++key)
+#pragma unroll
+                        for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+                            for (int n = 0; n < NR; ++n)
+                                if ((flags >> (key * G + grp) & 1u) && p[n][key] > 0.0f) b_sum[n][grp] = __int_as_float(0x7FC00000);
+                    load_value_planes(0);
+                }
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
                     float most = 0.0f;
 #pragma unroll
                     for (int first = 0; first < G; first += S::GH) {
-                        load_value_planes(first);
+                        if (G > S::GH) load_value_planes(first);
 #pragma unroll
                         for (int gh = 0; gh < S::GH; ++gh)
 #pragma unroll
-                            for (int key = 0; key < 4; ++key) {
-                                const float s = fabsf(key < 2 ? vs_lo.at(key, gh) : vs_hi.at(key - 2, gh));
-                                if (s <= 3.402823466e38f) most = fmaxf(most, p[n][key] * s);       // a NaN of p leaves it as it is
-                            }
+                            for (int key = 0; key < 4; ++key)
+                                most = fmaxf(most, p[n][key] * fabsf(key < 2 ? vs_lo.at(key, gh) : vs_hi.at(key - 2, gh)));      // a NaN of p leaves it as it is
                     }
                     most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
                     most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
                     const int e_new = min(max(e_v[n], rows_exponent(most) - 3), 119);              // now below 16
-                    rescale(n, rows_power(e_v[n] - e_new));
+                    const float fit = rows_power(e_v[n] - e_new);
+                    rescale(n, fit);
                     e_v[n] = e_new;
                     down_v[n] = rows_power(-e_new);
                 }
             }
-            float pd[NR][4], up_v[NR];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) up_v[n] = rows_power(e_v[n]);
+            float pd[NR][4], pc[NR][4];
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int key = 0; key < 4; ++key) pd[n][key] = p[n][key] * down_v[n];
+                for (int key = 0; key < 4; ++key) {
+                    pd[n][key] = p[n][key] * down_v[n];
+                    pc[n][key] = p[n][key] * kCentre;
+                }
 
             // ---- values ----
-            const uint8_t* vt = st + S::CODES;
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
                 if (G > S::GH && grp % S::GH == 0) load_value_planes(grp);
@@ -522,33 +693,25 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 for (int key = 0; key < 4; ++key) {
                     s[key] = key < 2 ? vs_lo.at(key, gh) : vs_hi.at(key - 2, gh);
                     b[key] = key < 2 ? vb_lo.at(key, gh) : vb_hi.at(key - 2, gh);
-                    // planes that are not finite count as zeros, and a row whose probability there is not zero becomes NaN in this group
-                    if (broken && !(fabsf(s[key]) <= 3.402823466e38f && fabsf(b[key]) <= 3.402823466e38f)) {
-                        s[key] = b[key] = 0.0f;
-#pragma unroll
-                        for (int n = 0; n < NR; ++n)
-                            if (p[n][key] > 0.0f) b_sum[n][grp] = __int_as_float(0x7FC00000);
-                    }
                 }
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    const float p0 = pd[n][0] * s[0], p1 = pd[n][1] * s[1], p2 = pd[n][2] * s[2], p3 = pd[n][3] * s[3];
-                    pb[n][0] = rows_half2(p0, p1);
-                    pb[n][1] = rows_half2(p2, p3);
-                    const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&pb[n][0])), r1 = __half22float2(*reinterpret_cast<const __half2*>(&pb[n][1]));
-                    b_sum[n][grp] = fmaf(kCentre * up_v[n], ((p0 - r0.x) + (p1 - r0.y)) + ((p2 - r1.x) + (p3 - r1.y)), b_sum[n][grp]);
+                    pb[n][0] = rows_half2(pd[n][0] * s[0], pd[n][1] * s[1]);
+                    pb[n][1] = rows_half2(pd[n][2] * s[2], pd[n][3] * s[3]);
 #pragma unroll
-                    for (int key = 0; key < 4; ++key) b_sum[n][grp] = fmaf(p[n][key], b[key], b_sum[n][grp]);
+                    for (int key = 0; key < 4; ++key) b_sum[n][grp] = fmaf(p[n][key], b[key], fmaf(pc[n][key], s[key], b_sum[n][grp]));
+                    const uint32_t one = g == grp ? 0x3C003C00u : 0u;
+                    rows_mma(ones[n], one, 0u, one, 0u, pb[n][0], pb[n][1]);
                 }
                 // A: rows g and g + 8 of m tile j are elements 8g + j and 8g + 4 + j of the group
                 uint32_t av[4][4];
+                const uint8_t* at = st + v_off[grp % KV] + grp / KV * 128;
+                // token 2t + 1: with rows of less than 128 bytes the swizzle moves it the other way for some lanes
+                const uint8_t* at1 = S::ROW >= 128 ? at + S::ROW : st + (v_off[grp % KV] ^ S::ROW) + grp / KV * 128;
                 if constexpr (BITS == 8) {
-                    uint2 w[4];
-#pragma unroll
-                    for (int key = 0; key < 4; ++key) w[key] = *reinterpret_cast<const uint2*>(vt + S::v_at(2 * t + (key & 1) + (key & 2) * 4, grp * 64 + 8 * g));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {               // tokens 2t, 2t + 1 and 2t + 8, 2t + 9
-                        const uint2 wa = w[2 * h], wb = w[2 * h + 1];
+                        const uint2 wa = *reinterpret_cast<const uint2*>(at + h * 8 * S::ROW), wb = *reinterpret_cast<const uint2*>(at1 + h * 8 * S::ROW);
                         const uint32_t lo0 = gm_prmt(wa.x, wb.x, 0x5140), lo1 = gm_prmt(wa.x, wb.x, 0x7362), hi0 = gm_prmt(wa.y, wb.y, 0x5140), hi1 = gm_prmt(wa.y, wb.y, 0x7362);
                         av[0][2 * h] = gm_prmt(lo0, 0, 0x4140); av[0][2 * h + 1] = gm_prmt(hi0, 0, 0x4140);
                         av[1][2 * h] = gm_prmt(lo0, 0, 0x4342); av[1][2 * h + 1] = gm_prmt(hi0, 0, 0x4342);
@@ -556,12 +719,10 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                         av[3][2 * h] = gm_prmt(lo1, 0, 0x4342); av[3][2 * h + 1] = gm_prmt(hi1, 0, 0x4342);
                     }
                 } else {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int key = 0; key < 4; ++key) w[key] = *reinterpret_cast<const uint32_t*>(vt + S::v_at(2 * t + (key & 1) + (key & 2) * 4, grp * 32 + 4 * g));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t lo = gm_prmt(w[2 * h], w[2 * h + 1], 0x5410), hi = gm_prmt(w[2 * h], w[2 * h + 1], 0x7632);
+                        const uint32_t wa = *reinterpret_cast<const uint32_t*>(at + h * 8 * S::ROW), wb = *reinterpret_cast<const uint32_t*>(at1 + h * 8 * S::ROW);
+                        const uint32_t lo = gm_prmt(wa, wb, 0x5410), hi = gm_prmt(wa, wb, 0x7632);
                         av[0][2 * h] = lo & 0x000F000Fu; av[0][2 * h + 1] = hi & 0x000F000Fu;
                         av[1][2 * h] = lo & 0x00F000F0u; av[1][2 * h + 1] = hi & 0x00F000F0u;      // sixteen times the code
                         av[2][2 * h] = lo >> 8 & 0x000F000Fu; av[2][2 * h + 1] = hi >> 8 & 0x000F000Fu;
@@ -581,8 +742,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
         }
         item += segment;
 
-        // ---- the segment's result: out^T = 2^E 2^24 o + b_sum, over l ----
-        const bool whole = from_start && to_end;
+        // ---- the segment's result: out^T = 2^E (2^24 o - centre * ones) + b_sum, over l ----
         float* part = a.partial + (size_t)(2 * worker + (from_start ? 1 : 0)) * RB * (D + 2);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -604,15 +764,15 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {                  // rows 2t and 2t + 1
                     const int r = 2 * t + c + 8 * n;
-                    const float bc = __shfl_sync(kFullMask, b, 8 * t + 4 * c);
+                    const float bc = __shfl_sync(kFullMask, b, 8 * t + 4 * c), centred = -kCentre * __shfl_sync(kFullMask, ones[n][c], 4 * grp + t);
                     if (r >= (int)valid) continue;
                     const float up = c ? up1 : up0;
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float unit = BITS == 4 && j % 2 ? 1048576.0f : 16777216.0f;
-                        v[j] = fmaf(up, unit * o[n][grp][j][c], bc);
-                        v[4 + j] = fmaf(up, unit * o[n][grp][j][2 + c], bc);
+                        v[j] = fmaf(up, fmaf(unit, o[n][grp][j][c], centred), bc);
+                        v[4 + j] = fmaf(up, fmaf(unit, o[n][grp][j][2 + c], centred), bc);
                     }
                     const int d = grp * 64 + 8 * g;
                     if (whole) {
@@ -629,93 +789,14 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 }
             }
         }
-        if (!whole && from_start && lane == 0) {
-            ShareInfo& info = a.info[worker];
-            info.last = share_of_last(total, workers, item - segment + now.range.tiles);      // the unit begins in this share
-            info.row0 = now.seq.row0;
-            info.flat0 = now.flat0;
-            info.valid = valid;
-            info.head = now.head;
-            info.active = 1;
+        if (!whole) {
+            const uint64_t unit_item = item - segment - (uint64_t)first_tile;
+            const uint32_t c0 = share_of_last(total, workers, unit_item + 1), parts = share_of_last(total, workers, unit_item + now.range.tiles) - c0 + 1;
+            rows_join<D, RB, BF16>(a, now.seq.row0, now.head, now.flat0, c0, worker - c0, parts, valid, lane);
         }
-        if (item < stop) now.next_unit(a);
+        if (item < stop) rows_next_unit(a, now);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-}
-
-// Joins the shares of the unit that worker c's share ends in: the block's warps over its rows, and where it has few over the shares of a row.
-constexpr int kRowsCombineThreads = 256, kRowsCombineWarps = kRowsCombineThreads / kWarp;
-template <int D, int RB, bool BF16>
-__global__ void __launch_bounds__(kRowsCombineThreads)
-attention_rows_combine_kernel(const AttnArgs a) {
-    constexpr int VEC = D / 32, BATCH = 8;
-    constexpr size_t kSlot = (size_t)RB * (D + 2);
-    __shared__ float s_sum[kRowsCombineWarps][D + 1];
-    pdl_wait();
-    const uint32_t c = blockIdx.x;
-    const ShareInfo info = a.info[c];
-    if (!info.active) return;
-    const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, parts = info.last - c + 1;
-    const uint32_t rows_at_once = min(info.valid, (uint32_t)kRowsCombineWarps), per_row = kRowsCombineWarps / rows_at_once, sub = warp % per_row;
-    auto slot = [&](uint32_t p) { return a.partial + (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kSlot; };
-    for (uint32_t r0 = 0; r0 < info.valid; r0 += rows_at_once) {
-        const uint32_t r = r0 + warp / per_row;
-        const bool busy = warp / per_row < rows_at_once && r < info.valid;
-        float top = -INFINITY, sum = 0.0f, v[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
-        if (busy) {
-            for (uint32_t p = lane; p < parts; p += kWarp) top = fmaxf(top, slot(p)[r]);
-#pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
-            const float base = top == -INFINITY ? 0.0f : top;
-            const uint32_t mine = (parts + per_row - 1 - sub) / per_row;             // shares sub, sub + per_row, ...
-            for (uint32_t i0 = 0; i0 < mine; i0 += BATCH) {
-                float w[BATCH], x[BATCH][VEC], l[BATCH];
-#pragma unroll
-                for (int i = 0; i < BATCH; ++i) {
-                    const bool is = i0 + i < mine;
-                    const float* s = slot(sub + (is ? i0 + i : 0) * per_row);
-                    w[i] = is ? s[r] : -INFINITY;
-                    l[i] = s[RB + r];
-                    const float* src = s + 2 * RB + (size_t)r * D + lane * VEC;
-#pragma unroll
-                    for (int e = 0; e < VEC; e += 2) {
-                        const float2 y = *reinterpret_cast<const float2*>(src + e);
-                        x[i][e] = y.x;
-                        x[i][e + 1] = y.y;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < BATCH; ++i) {
-                    if (i0 + i >= mine) break;
-                    const float f = exp2f(w[i] - base);
-                    sum = fmaf(f, l[i], sum);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) v[e] = fmaf(f, x[i][e], v[e]);
-                }
-            }
-        }
-        if (per_row > 1) {
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) s_sum[warp][lane * VEC + e] = v[e];
-            if (lane == 0) s_sum[warp][D] = sum;
-            __syncthreads();
-            if (sub == 0)
-                for (uint32_t k = 1; k < per_row; ++k) {
-                    sum += s_sum[warp + k][D];
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) v[e] += s_sum[warp + k][lane * VEC + e];
-                }
-        }
-        if (!busy || sub != 0) continue;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const uint32_t flat = info.flat0 + r;
-        uint16_t* dst = a.out + (size_t)(info.row0 + flat / a.group) * a.out_stride + (size_t)(info.head * a.group + flat % a.group) * D + lane * VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv, v[e + 1] * inv);
-    }
 }
 
 template <int D, int BITS, int RB, bool BF16>
@@ -730,10 +811,7 @@ static tf_status launch_rows(tf_context* ctx, cudaStream_t st, const AttnArgs& a
     blocks = lesser(blocks, lesser(ws->row_capacity / RB, ws->max_workers) / S::WARPS);
     TF_REQUIRE(ctx, blocks > 0, TF_ERR_CUDA, "tf_tree_attention: the kernel does not fit on the device");
     kernel<<<blocks, S::THREADS, S::SMEM, st>>>(a);
-    const tf_status t = check_launch(ctx, "tf_tree_attention");
-    if (t != TF_OK) return t;
-    TF_CUDA(ctx, launch_pdl(attention_rows_combine_kernel<D, RB, BF16>, dim3(blocks * S::WARPS), dim3(kRowsCombineThreads), 0, st, a));
-    return check_launch(ctx, "tf_tree_attention (join)");
+    return check_launch(ctx, "tf_tree_attention");
 }
 
 }  // namespace tf
