@@ -34,22 +34,26 @@ static void walk(const AttnArgs& a, uint32_t grid) {
         total += sequence_tiles<MT, TILE>(a, s) * a.kv_heads;
         before[b + 1] = total;
     }
-    const uint32_t blocks = (uint32_t)lesser((uint64_t)grid, total);
+    Shares shares;
+    shares.set(total, grid);
+    const uint32_t blocks = shares.workers;
+    CHECK(shares.begin(0) == 0 && shares.begin(blocks) == total);
     using Unit = std::tuple<uint32_t, uint32_t, uint32_t>;
     std::map<Unit, std::vector<std::pair<uint32_t, uint32_t>>> seen;       // unit -> (block, tiles) in order
     std::map<Unit, uint32_t> tiles;
     std::map<Unit, uint32_t> first_block, said;
     for (uint32_t c = 0; c < blocks; ++c) {
-        uint64_t item = share_begin(total, blocks, c);
-        const uint64_t stop = share_begin(total, blocks, c + 1);
-        CHECK(item < stop);
+        uint64_t item = shares.begin(c);
+        const uint64_t stop = shares.begin(c + 1);
+        CHECK(item < stop && shares.of(item) == c && shares.of(stop - 1) == c);
         uint32_t b = 0;
         while (before[b + 1] <= item) ++b;
-        uint32_t place[4];
-        place_in_sequence<MT, TILE>(a, b, item - before[b], place);
+        uint32_t place[3];
         Cursor<MT, TILE> now;
-        now.b = place[0]; now.head = place[1]; now.flat0 = place[2]; now.tile = place[3];
-        now.seq.load(a, now.b, false);
+        now.b = b;
+        now.seq.load(a, b, false);
+        place_in_sequence<MT, TILE>(a, now.seq, item - before[b], place);
+        now.head = place[0]; now.flat0 = place[1]; now.tile = place[2];
         now.range.set(a, now.seq, now.flat0, MT, TILE);
         std::set<int> slots;
         while (item < stop) {
@@ -70,7 +74,7 @@ static void walk(const AttnArgs& a, uint32_t grid) {
             item += segment;
             if (from_start) {
                 first_block[u] = c;
-                said[u] = share_of_last(total, blocks, item - segment + now.range.tiles);
+                said[u] = shares.of(item - segment + now.range.tiles - 1);
             }
             now.tile += segment - 1;
             if (item < stop) { CHECK(to_end); now.next_unit(a); CHECK(now.b < a.sequences); }
@@ -91,7 +95,14 @@ static void walk(const AttnArgs& a, uint32_t grid) {
     }
 }
 
-static void shares() {
+static void divisions() {
+    for (int i = 0; i < 100000; ++i) {
+        const uint64_t a = rng() >> pick(0, 63), b = (rng() >> pick(0, 63)) | 1;
+        CHECK(Shares::divide(a, b) == a / b);
+    }
+}
+
+static void all_shares() {
     for (int round = 0; round < 400; ++round) {
         const uint32_t n = (uint32_t)pick(1, 40);
         const bool bad = round % 4 == 3;
@@ -153,7 +164,7 @@ static void rows_places() {
             CHECK(k.insert(x).second && v.insert(y).second);
             for (uint32_t byte = 0; byte < 16; byte += 2) CHECK(S::k_at(r, p * 16 + byte) == x + byte && S::v_at(r, p * 16 + byte) == y + byte);
         }
-    CHECK(kRowsTile * S::PIECES % kWarp == 0 && (8 * S::G) % 8 == 0);
+    CHECK(kRowsTile * S::PIECES % kWarp == 0 && S::SWAP % 16 == 0);
     CHECK(S::STAGES >= 2 && S::STAGES <= 31 && S::BLOCKS * (S::SMEM + 1024 + 256) <= 227 * 1024);
 }
 template <int D, int BITS>
@@ -258,7 +269,8 @@ static void refusals() {
 }
 
 int main() {
-    shares();
+    divisions();
+    all_shares();
     places<64, 4>(); places<64, 8>(); places<128, 4>(); places<128, 8>(); places<256, 4>(); places<256, 8>(); places<512, 4>(); places<512, 8>();
     refusals();
     std::printf("all fine\n");

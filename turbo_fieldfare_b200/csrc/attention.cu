@@ -18,10 +18,10 @@ tf_status tf_attention_workspace_create(tf_context* ctx, uint32_t head_dim, tf_a
     ws->head_dim = head_dim;
     ws->row_capacity = (uint32_t)ctx->sm_count * 128;          // two blocks of 64 rows per SM, or eight of 16
     ws->max_workers = (uint32_t)ctx->sm_count * 16;
-    const uint64_t partial = (uint64_t)2 * ws->row_capacity * (head_dim + 2) * sizeof(float), info = (uint64_t)ws->max_workers * sizeof(tf::ShareInfo);
+    const uint64_t partial = (uint64_t)2 * ws->row_capacity * (head_dim + 4) * sizeof(float), info = (uint64_t)ws->max_workers * sizeof(tf::ShareInfo);
     cudaError_t e = cudaMalloc(&ws->partial, partial);
     if (e == cudaSuccess) e = cudaMalloc(&ws->info, info);
-    const uint64_t tickets = (uint64_t)3 * 2 * ws->max_workers * sizeof(uint32_t);      // kJoin^3 shares are more than there are workers
+    const uint64_t tickets = (uint64_t)3 * 4 * ws->max_workers * sizeof(uint32_t);      // kJoin^3 shares are more than there are workers
     if (e == cudaSuccess) e = cudaMalloc(&ws->tickets, tickets);
     if (e == cudaSuccess) e = cudaMemset(ws->tickets, 0, tickets);
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);                  // calls may come on streams that do not wait for this one
@@ -82,7 +82,7 @@ tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32
     a.table = {batch->page_table, batch->page_table_stride, cache->num_pages, tf::log2_of(cache->page_size)};
     a.row_offsets = batch->row_offsets; a.context_lengths = batch->context_lengths; a.positions = batch->positions;
     a.mask = reinterpret_cast<const unsigned long long*>(tree_mask); a.mask_words = mask_words;
-    a.partial = ws->partial; a.info = static_cast<tf::ShareInfo*>(ws->info); a.tickets = ws->tickets; a.ticket_stride = 2 * ws->max_workers;
+    a.partial = ws->partial; a.info = static_cast<tf::ShareInfo*>(ws->info); a.tickets = ws->tickets; a.ticket_stride = 4 * ws->max_workers;
     a.error = ctx->device_error;
     a.q_stride = q_stride; a.out_stride = out_stride;
     a.sequences = batch->sequences; a.rows = batch->rows; a.kv_heads = cache->kv_heads; a.group = group;

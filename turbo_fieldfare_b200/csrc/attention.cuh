@@ -103,7 +103,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
     // ---- this block's share of the tiles ----
     Cursor<MT, kTile> now;
     uint64_t total, item, stop;
-    uint32_t blocks;
+    Shares shares;
     {
         const uint32_t per = (a.sequences + kAttnThreads - 1) / kAttnThreads, b0 = min((uint64_t)per * tid, (uint64_t)a.sequences),
                        b1 = min((uint64_t)b0 + per, (uint64_t)a.sequences);
@@ -129,11 +129,11 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
             total += s_scan[w];
         }
         before += upto - mine;
-        blocks = (uint32_t)min((uint64_t)gridDim.x, total);
+        shares.set(total, gridDim.x);
         if (tid == 0) a.info[blockIdx.x].active = 0;
-        if (blockIdx.x >= blocks) return;
-        item = share_begin(total, blocks, blockIdx.x);
-        stop = share_begin(total, blocks, blockIdx.x + 1);
+        if (blockIdx.x >= shares.workers) return;
+        item = shares.begin(blockIdx.x);
+        stop = shares.begin(blockIdx.x + 1);
         if (item >= before && item < before + mine) {
             uint64_t left = item - before;
             for (uint32_t b = b0; b < b1; ++b) {
@@ -141,7 +141,9 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
                 s.load(a, b, false);
                 const uint64_t n = sequence_tiles<MT, kTile>(a, s) * a.kv_heads;
                 if (left < n) {
-                    place_in_sequence<MT, kTile>(a, b, left, s_start);
+                    uint32_t place[3];
+                    place_in_sequence<MT, kTile>(a, s, left, place);
+                    s_start[0] = b; s_start[1] = place[0]; s_start[2] = place[1]; s_start[3] = place[2];
                     break;
                 }
                 left -= n;
@@ -673,7 +675,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
             if (from_start && tid == 0) {
                 const uint64_t end_item = item - segment + now.range.tiles;      // of the unit; it begins in this share
                 ShareInfo& info = a.info[blockIdx.x];
-                info.last = share_of_last(total, blocks, end_item);
+                info.last = shares.of(end_item - 1);
                 info.row0 = now.seq.row0;
                 info.flat0 = now.flat0;
                 info.valid = valid;

@@ -106,29 +106,47 @@ __host__ __device__ __forceinline__ uint64_t sequence_tiles(const AttnArgs& a, c
     return n;
 }
 
-// The place `left` tiles into the tiles of sequence b, which has more than that.
+// The place `left` tiles into a sequence's tiles, of which there are more: kv head, first row of the unit, tile of the unit.
 template <int MT, int TILE>
-__host__ __device__ __forceinline__ void place_in_sequence(const AttnArgs& a, uint32_t b, uint64_t left, uint32_t (&place)[4]) {
-    Sequence s;
-    s.load(a, b, false);
+__host__ __device__ __forceinline__ void place_in_sequence(const AttnArgs& a, const Sequence& s, uint64_t left, uint32_t (&place)[3]) {
     const uint64_t n = sequence_tiles<MT, TILE>(a, s);
-    place[0] = b;
-    place[1] = (uint32_t)(left / n);
-    left %= n;
+    place[0] = 0;
+    while (left >= n) {
+        left -= n;
+        ++place[0];
+    }
     for (uint64_t f = 0;; f += MT) {
         UnitRange r;
         r.set(a, s, (uint32_t)f, MT, TILE);
         if (left < r.tiles) {
-            place[2] = (uint32_t)f;
-            place[3] = (uint32_t)left;
+            place[1] = (uint32_t)f;
+            place[2] = (uint32_t)left;
             return;
         }
         left -= r.tiles;
     }
 }
 
-// First tile of worker c's share of `total`, and the worker whose share holds the tile before `end`.
-__host__ __device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t workers, uint32_t c) { return total * c / workers; }
-__host__ __device__ __forceinline__ uint32_t share_of_last(uint64_t total, uint32_t workers, uint64_t end) { return (uint32_t)((end * workers - 1) / total); }
+// `total` tiles in shares that differ by one at the most: the first `more` workers have one more than `each`. No more workers than tiles.
+struct Shares {
+    uint64_t total;
+    uint32_t workers, more;
+    uint64_t each;
+    __host__ __device__ __forceinline__ void set(uint64_t tiles, uint32_t most) {
+        total = tiles;
+        workers = (uint32_t)lesser((uint64_t)most, tiles);
+        each = workers ? divide(tiles, workers) : 0;
+        more = (uint32_t)(tiles - each * workers);
+    }
+    __host__ __device__ __forceinline__ uint64_t begin(uint32_t c) const { return each * c + lesser(c, more); }
+    __host__ __device__ __forceinline__ uint32_t of(uint64_t tile) const {
+        const uint64_t longer = (each + 1) * more;
+        return (uint32_t)(tile < longer ? divide(tile, each + 1) : more + divide(tile - longer, each));
+    }
+    // 64-bit division takes four times as long as this for numbers of 32 bits
+    static __host__ __device__ __forceinline__ uint64_t divide(uint64_t a, uint64_t b) {
+        return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
+    }
+};
 
 }  // namespace tf

@@ -26,16 +26,16 @@ constexpr int kRowsTile = 16;                                  // tokens: a tile
 
 template <int D, int BITS, int RB>
 struct RowsShape {
-    static constexpr int G = D / 64, ROW = D * BITS / 8, PIECES = ROW / 16, NR = RB / 8;
+    // A head of 512 is shared by two warps, which have half of its elements each (DW) and add their logits.
+    static constexpr int DW = D < 256 ? D : 256, SPLIT = D / DW, G = DW / 64, GROUPS = D / 64;
+    static constexpr int ROW = DW * BITS / 8, ROW_BYTES = D * BITS / 8, PIECES = ROW / 16, NR = RB / 8;      // of a warp's part, and of the cache's row
     static constexpr int CODES = kRowsTile * ROW, PLANE = kRowsTile * G * 2, STAGE = 2 * CODES + 4 * PLANE;
-    // Heads of 512: the rows of q are read from shared memory, since the product alone takes 128 registers.
-    static constexpr bool Q_SHARED = D == 512;
-    static constexpr int Q_BYTES = Q_SHARED ? D / 16 * kWarp * 8 : 0;
-    static constexpr int WARPS = D == 512 ? (BITS == 8 ? 1 : 2) : 4, BLOCKS = D == 512 ? (BITS == 8 ? 5 : 3) : D == 256 ? 2 : 3;
+    static constexpr int WARPS = 4, WORKERS = WARPS / SPLIT, BLOCKS = D >= 256 ? 2 : 3;
     static constexpr int THREADS = WARPS * kWarp;
-    static constexpr int FIT = (227 * 1024 / BLOCKS - 1024 - 256 - WARPS * Q_BYTES) / (WARPS * STAGE), STAGES = FIT > 8 ? 8 : FIT;
-    static constexpr int SMEM = WARPS * (STAGES * STAGE + Q_BYTES);
-    static constexpr int GH = G < 4 ? G : 4;                   // groups whose planes are in registers at a time
+    static constexpr int SWAP = SPLIT > 1 ? 2 * WARPS * kWarp * NR * 16 : 0;                       // logits of the other warp, by turns in two buffers
+    static constexpr int FIT = (227 * 1024 / BLOCKS - 1024 - 256 - SWAP) / (WARPS * STAGE), STAGES = FIT > 8 ? 8 : FIT;
+    static constexpr int SMEM = WARPS * STAGES * STAGE + SWAP;
+    static constexpr int GH = G;                               // groups whose planes are in registers at a time
     static_assert(STAGES >= 2 && STAGE % 128 == 0, "a ring needs two stages");
     // 16-byte pieces are moved within their 128-byte lines so that the reads of a quarter or half warp meet every bank once
     static __host__ __device__ __forceinline__ uint32_t k_at(uint32_t row, uint32_t byte) {
@@ -50,6 +50,9 @@ struct RowsShape {
 
 __device__ __forceinline__ void rows_cp_async(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void rows_cp_async_8(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void rows_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -151,12 +154,14 @@ __device__ __noinline__ uint32_t rows_sanitise(uint8_t* scales, int plane_bytes,
 
 // Joins the shares of a unit, sixteen at a time: the worker that is the last to leave its share of a group joins the group, in the order of the
 // shares, into the place of its first, and goes on as that group's worker among the groups. Tickets are back at zero when their
-// group is joined. Part 0 lies in worker c0's second slot, part i in worker c0 + i's first.
-template <int D, int RB, bool BF16>
-__device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_t head, uint32_t flat0, uint32_t c0, uint32_t i, uint32_t parts, uint32_t valid, int lane) {
-    constexpr int VEC = D / 32, BATCH = 4;
-    constexpr size_t kSlot = (size_t)RB * (D + 2);
-    auto place = [&](uint32_t p) { return p == 0 ? 2 * c0 + 1 : 2 * (c0 + p); };
+// group is joined. Share 0 lies in worker c0's second slot, share i in worker c0 + i's first; a slot is [rows] maxima, [rows] sums and
+// [rows][DW] products of each of the SPLIT parts of the head's elements, which are joined apart.
+template <int D, int DW, int RB, bool BF16>
+__device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_t head, uint32_t flat0, uint32_t c0, uint32_t i, uint32_t parts, uint32_t valid,
+                                       uint32_t half, int lane) {
+    constexpr int VEC = DW / 32, SPLIT = D / DW, BATCH = VEC >= 8 ? 8 : 16;
+    constexpr uint32_t kSlot = RB * (DW + 2);
+    auto place = [&](uint32_t p) { return (p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * SPLIT + half; };
     uint32_t span = 1;
     for (uint32_t* tickets = a.tickets; parts > 1; tickets += a.ticket_stride, span *= kJoin) {
         const uint32_t group = i / kJoin, base = group * kJoin, members = min((uint32_t)kJoin, parts - base);
@@ -168,32 +173,39 @@ __device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_
         if (lane == 0) tickets[place(base * span)] = 0;
         __threadfence();
         const bool final = parts <= kJoin;
-        float* first = a.partial + place(base * span) * kSlot;
+        float* first = a.partial + (size_t)place(base * span) * kSlot;
         for (uint32_t r = 0; r < valid; ++r) {
-            const float* mine = a.partial + place((base + min((uint32_t)lane, members - 1)) * span) * kSlot;      // the slots may have been in L1 before
+            // past L1, which may hold a slot as it was before
+            const float* mine = a.partial + (size_t)place((base + min((uint32_t)lane, members - 1)) * span) * kSlot;
             const float mp = (uint32_t)lane < members ? __ldcg(mine + r) : -INFINITY, lp = (uint32_t)lane < members ? __ldcg(mine + RB + r) : 0.0f;
-            float top = mp;
-#pragma unroll
-            for (int off = kJoin / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
-            top = __shfl_sync(kFullMask, top, 0);
-            const float w = (uint32_t)lane < members ? exp2f(mp - (top == -INFINITY ? 0.0f : top)) : 0.0f;
-            float sum = 0.0f, v[VEC];
+            float top = 0.0f, w = 0.0f, sum = 0.0f, v[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
-            for (uint32_t p0 = 0; p0 < members; p0 += BATCH) {
+#pragma unroll
+            for (uint32_t p0 = 0; p0 < kJoin; p0 += BATCH) {
+                if (p0 >= members) break;
                 float2 x[BATCH][VEC / 2];
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
-                    if (p0 + k >= members) break;
-                    const float2* src = reinterpret_cast<const float2*>(a.partial + place((base + p0 + k) * span) * kSlot + 2 * RB + (size_t)r * D + lane * VEC);
+                    const float2* src = reinterpret_cast<const float2*>(a.partial + (size_t)place((base + min(p0 + k, members - 1)) * span) * kSlot + 2 * RB + r * DW + lane * VEC);
 #pragma unroll
                     for (int e = 0; e < VEC / 2; ++e) x[k][e] = __ldcg(src + e);
+                }
+                if (p0 == 0) {
+                    top = mp;
+#pragma unroll
+                    for (int off = kJoin / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+                    top = __shfl_sync(kFullMask, top, 0);
+                    w = (uint32_t)lane < members ? rows_exp2(mp - (top == -INFINITY ? 0.0f : top)) : 0.0f;
+                    sum = w * lp;
+#pragma unroll
+                    for (int off = kJoin / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
+                    sum = __shfl_sync(kFullMask, sum, 0);
                 }
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
                     if (p0 + k >= members) break;
                     const float wk = __shfl_sync(kFullMask, w, p0 + k);
-                    sum = fmaf(wk, __shfl_sync(kFullMask, lp, p0 + k), sum);
 #pragma unroll
                     for (int e = 0; e < VEC / 2; ++e) {
                         v[2 * e] = fmaf(wk, x[k][e].x, v[2 * e]);
@@ -204,7 +216,7 @@ __device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_
             if (final) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const uint32_t flat = flat0 + r;
-                uint16_t* dst = a.out + (size_t)(row0 + flat / a.group) * a.out_stride + (size_t)(head * a.group + flat % a.group) * D + lane * VEC;
+                uint16_t* dst = a.out + (size_t)(row0 + flat / a.group) * a.out_stride + (size_t)(head * a.group + flat % a.group) * D + half * DW + lane * VEC;
 #pragma unroll
                 for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv, v[e + 1] * inv);
             } else {
@@ -213,7 +225,7 @@ __device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_
                     first[RB + r] = sum;
                 }
 #pragma unroll
-                for (int e = 0; e < VEC; e += 2) *reinterpret_cast<float2*>(first + 2 * RB + (size_t)r * D + lane * VEC + e) = make_float2(v[e], v[e + 1]);
+                for (int e = 0; e < VEC; e += 2) *reinterpret_cast<float2*>(first + 2 * RB + r * DW + lane * VEC + e) = make_float2(v[e], v[e + 1]);
             }
         }
         parts = (parts + kJoin - 1) / kJoin;
@@ -240,71 +252,64 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int G = S::G, NR = S::NR, W = S::WARPS;
     constexpr float kCentre = BITS == 8 ? 128.0f : 8.0f;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ unsigned long long s_scan[W];
-    __shared__ uint32_t s_start[W][4];
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, g = lane / 4, t = lane % 4;
-    const uint32_t workers_max = gridDim.x * W, worker = blockIdx.x * W + warp;
+    const uint32_t half = warp % S::SPLIT, worker = blockIdx.x * S::WORKERS + warp / S::SPLIT;
 
-    // ---- the shares of this block's warps ----
-    uint64_t total = 0;
-    {
-        const uint32_t per = (a.sequences + S::THREADS - 1) / S::THREADS, b0 = lesser((uint64_t)per * tid, (uint64_t)a.sequences),
-                       b1 = lesser((uint64_t)b0 + per, (uint64_t)a.sequences);
-        uint64_t mine = 0;
-        for (uint32_t b = b0; b < b1; ++b) {
-            Sequence s;
-            s.load(a, b, blockIdx.x == 0);
-            mine += sequence_tiles<RB, kRowsTile>(a, s) * a.kv_heads;
-        }
-        uint64_t upto = mine;
-#pragma unroll
-        for (int off = 1; off < kWarp; off <<= 1) {
-            const uint64_t o = __shfl_up_sync(kFullMask, upto, off);
-            if (lane >= off) upto += o;
-        }
-        if (lane == kWarp - 1) s_scan[warp] = upto;
-        __syncthreads();
-        uint64_t before = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w == warp) before = total;
-            total += s_scan[w];
-        }
-        before += upto - mine;
-        const uint32_t workers = (uint32_t)lesser((uint64_t)workers_max, total);
-#pragma unroll 1
-        for (int w = 0; w < W; ++w) {
-            if (blockIdx.x * W + w >= workers) break;
-            const uint64_t item = share_begin(total, workers, blockIdx.x * W + w);
-            if (item >= before && item < before + mine) {
-                uint64_t left = item - before;
-                for (uint32_t b = b0; b < b1; ++b) {
-                    Sequence s;
-                    s.load(a, b, false);
-                    const uint64_t n = sequence_tiles<RB, kRowsTile>(a, s) * a.kv_heads;
-                    if (left < n) {
-                        place_in_sequence<RB, kRowsTile>(a, b, left, s_start[w]);
-                        break;
-                    }
-                    left -= n;
-                }
-            }
-        }
-        __syncthreads();
-    }
-    const uint32_t workers = (uint32_t)lesser((uint64_t)workers_max, total);
-    if (worker >= workers) return;
-    uint64_t item = share_begin(total, workers, worker);
-    const uint64_t stop = share_begin(total, workers, worker + 1);
+    // ---- this worker's share: every warp goes over the sequences, 32 at a time ----
     Cursor<RB, kRowsTile> now;
-    now.b = s_start[warp][0]; now.head = s_start[warp][1]; now.flat0 = s_start[warp][2]; now.tile = s_start[warp][3];
-    now.seq.load(a, now.b, false);
-    now.range.set(a, now.seq, now.flat0, RB, kRowsTile);
+    Shares shares;
+    uint64_t item, stop;
+    {
+        auto tiles_of = [&](uint32_t b, Sequence& s, bool report) -> uint64_t {
+            if (b >= a.sequences) return 0;
+            s.load(a, b, report);
+            return sequence_tiles<RB, kRowsTile>(a, s) * a.kv_heads;
+        };
+        uint64_t total = 0;
+#pragma unroll 4
+        for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWarp) {
+            Sequence s;
+            total += tiles_of(b0 + lane, s, blockIdx.x == 0);
+        }
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(kFullMask, total, off);
+        shares.set(total, gridDim.x * S::WORKERS);
+        if (worker >= shares.workers) return;
+        item = shares.begin(worker);
+        stop = shares.begin(worker + 1);
+        uint64_t before = 0;
+        for (uint32_t b0 = 0;; b0 += kWarp) {                  // ends: item is below the total
+            Sequence s = {};
+            const uint64_t mine = tiles_of(b0 + lane, s, false);
+            uint64_t upto = mine;
+#pragma unroll
+            for (int off = 1; off < kWarp; off <<= 1) {
+                const uint64_t o = __shfl_up_sync(kFullMask, upto, off);
+                if (lane >= off) upto += o;
+            }
+            const uint64_t all = __shfl_sync(kFullMask, upto, kWarp - 1);
+            if (item < before + all) {
+                const int owner = __ffs(__ballot_sync(kFullMask, before + upto > item)) - 1;
+                const uint64_t left = item - before - __shfl_sync(kFullMask, upto - mine, owner);
+                now.b = b0 + owner;
+                now.seq.row0 = __shfl_sync(kFullMask, s.row0, owner);
+                now.seq.rows = __shfl_sync(kFullMask, s.rows, owner);
+                now.seq.context = __shfl_sync(kFullMask, s.context, owner);
+                uint32_t place[3];
+                place_in_sequence<RB, kRowsTile>(a, now.seq, left, place);
+                now.head = place[0]; now.flat0 = place[1]; now.tile = place[2];
+                break;
+            }
+            before += all;
+        }
+        now.range.set(a, now.seq, now.flat0, RB, kRowsTile);
+    }
 
     // ---- this warp's ring: what the next request needs is in registers, the rest of its cursor in memory ----
     uint8_t* ring = smem + warp * (S::STAGES * S::STAGE);
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-    uint2* q_shared = reinterpret_cast<uint2*>(smem + W * S::STAGES * S::STAGE + warp * S::Q_BYTES) + lane;       // [D / 16][lanes]
+    float4* swap = reinterpret_cast<float4*>(smem + W * S::STAGES * S::STAGE);       // [2][warps][NR][lanes]
+    uint32_t turn = 0;
     Cursor<RB, kRowsTile> next = now;
     uint32_t ahead = (uint32_t)(stop - item);                  // tiles not requested yet
     uint32_t there = 0;                                        // a bit per stage: its tile has a page
@@ -313,7 +318,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
     int32_t next_page;
     auto look_up = [&] {
         next_page = -1;
-        if (next_token < next_end) {
+        if (next_token < next_end) {                           // (the table is read once per page)
             const int32_t p = next_table[next_token >> a.table.page_log2];
             if (p >= 0 && (uint32_t)p < a.table.pages) next_page = p;
         }
@@ -333,28 +338,34 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             there |= 1u << stage;
             const size_t row = (((size_t)next_page * a.kv_heads + next_head) << a.table.page_log2) + (next_token & ((1u << a.table.page_log2) - 1u));
             const uint32_t base = ring_addr + stage * S::STAGE;
-            const uint8_t *kc = a.k.codes + row * S::ROW + lane * 16, *vc = a.v.codes + row * S::ROW + lane * 16;
+            const size_t from = (row + lane / S::PIECES) * S::ROW_BYTES + half * S::ROW + lane % S::PIECES * 16;
+            const uint8_t *kc = a.k.codes + from, *vc = a.v.codes + from;
 #pragma unroll
             for (int i = 0; i < kRowsTile * S::PIECES / kWarp; ++i) {
-                // rows first and on of the tile: their swizzle on top of the lane's own
-                const uint32_t first = i * kWarp / S::PIECES, k_more = S::k_at(first, 0) ^ (first * S::ROW), v_more = S::v_at(first, 0) ^ (first * S::ROW);
-                rows_cp_async(((base + k_dst) ^ k_more) + i * 512, kc + i * 512);
-                rows_cp_async(((base + v_dst) ^ v_more) + i * 512, vc + i * 512);
+                // rows `first` and on of the tile: their swizzle on top of the lane's own
+                const uint32_t first = i * kWarp / S::PIECES, src = first * S::ROW_BYTES, k_more = S::k_at(first, 0) ^ (first * S::ROW), v_more = S::v_at(first, 0) ^ (first * S::ROW);
+                rows_cp_async(((base + k_dst) ^ k_more) + i * 512, kc + src);
+                rows_cp_async(((base + v_dst) ^ v_more) + i * 512, vc + src);
             }
-            // planes: 2 G pieces each
-            if (8 * G >= kWarp || lane < 8 * G) {
+            if constexpr (S::SPLIT > 1) {
+                // planes: eight bytes of a token each
 #pragma unroll
-                for (int i = 0; i < (8 * G + kWarp - 1) / kWarp; ++i) {
-                    const uint32_t id = lane + i * kWarp, plane = id / (2 * G), c = id % (2 * G);
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t id = lane + i * kWarp, plane = id / kRowsTile, token = id % kRowsTile;
                     const uint16_t* src = plane == 0 ? a.k.scales : plane == 1 ? a.k.biases : plane == 2 ? a.v.scales : a.v.biases;
-                    rows_cp_async(base + 2 * S::CODES + id * 16, src + row * G + c * 8);
+                    rows_cp_async_8(base + 2 * S::CODES + id * 8, src + (row + token) * S::GROUPS + half * S::G);
                 }
+            } else if (8 * G == kWarp || lane < 8 * G) {
+                // planes: 2 G pieces each
+                const uint32_t plane = lane / (2 * G), c = lane % (2 * G);
+                const uint16_t* src = plane == 0 ? a.k.scales : plane == 1 ? a.k.biases : plane == 2 ? a.v.scales : a.v.biases;
+                rows_cp_async(base + 2 * S::CODES + lane * 16, src + row * G + c * 8);
             }
         }
         if (--ahead) {
             if (--next_left) {
                 next_token += kRowsTile;
-                look_up();
+                if ((next_token & ((1u << a.table.page_log2) - 1u)) == 0 || next_token >= next_end) look_up();
             } else {
                 rows_next_unit(a, next);
                 enter_unit();
@@ -384,7 +395,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
         const uint32_t first_tile = now.tile;
         const uint32_t segment = (uint32_t)lesser((uint64_t)(now.range.tiles - first_tile), stop - item);
         const bool from_start = first_tile == 0, whole = from_start && segment == now.range.tiles;
-        uint32_t qf[NR][S::Q_SHARED ? 1 : D / 16][2];
+        uint32_t qf[NR][4 * G][2];
         float q_sum[NR][G][2], factor[NR], m[NR], l[NR], b_sum[NR][G];       // q_sum: of rows 2t and 2t + 1; the others: of row g
         int32_t low[NR];                                       // first token that the row sees, from the unit's first tile on
         uint32_t node[NR];
@@ -394,7 +405,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             const uint32_t r = g + 8 * n, flat = now.flat0 + r;
             const bool is = r < valid;
             node[n] = is ? flat / a.group : 0;
-            const uint16_t* src = a.q + (size_t)(now.seq.row0 + node[n]) * a.q_stride + (size_t)(now.head * a.group + (is ? flat % a.group : 0)) * D + 16 * t;
+            const uint16_t* src = a.q + (size_t)(now.seq.row0 + node[n]) * a.q_stride + (size_t)(now.head * a.group + (is ? flat % a.group : 0)) * D + half * S::DW + 16 * t;
             uint32_t raw[G][8];
             float most = 0.0f;
 #pragma unroll
@@ -414,6 +425,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(value(grp, j)));
             most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
             most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+            // (of this warp's part of it: the product is brought back before parts are added)
             const int e = most > 0.0f ? max(rows_exponent(most) - 7, -126) : 0;      // the row's largest element to [128, 256)
             const float down = rows_power(-e);
 #pragma unroll
@@ -437,12 +449,8 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                         lo = part(j) | part(j + 4) << 16;
                         hi = part(j + 1) | part(j + 5) << 16;
                     }
-                    if constexpr (S::Q_SHARED) {
-                        q_shared[(grp * 4 + ks) * kWarp] = make_uint2(lo, hi);      // read by this lane alone
-                    } else {
-                        qf[n][grp * 4 + ks][0] = lo;
-                        qf[n][grp * 4 + ks][1] = hi;
-                    }
+                    qf[n][grp * 4 + ks][0] = lo;
+                    qf[n][grp * 4 + ks][1] = hi;
                 }
                 sum += __shfl_xor_sync(kFullMask, sum, 1);
                 sum += __shfl_xor_sync(kFullMask, sum, 2);
@@ -523,11 +531,8 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                     }
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
-                        uint2 q;
-                        if constexpr (S::Q_SHARED) q = q_shared[(grp * 4 + ks) * kWarp];
-                        else q = make_uint2(qf[n][grp * 4 + ks][0], qf[n][grp * 4 + ks][1]);
-                        if (ks == 0) rows_mma_first(acc[n], a0, a1, a2, a3, q.x, q.y);
-                        else rows_mma(acc[n], a0, a1, a2, a3, q.x, q.y);
+                        if (ks == 0) rows_mma_first(acc[n], a0, a1, a2, a3, qf[n][grp * 4][0], qf[n][grp * 4][1]);
+                        else rows_mma(acc[n], a0, a1, a2, a3, qf[n][grp * 4 + ks][0], qf[n][grp * 4 + ks][1]);
                     }
                 }
                 const float s0 = ks_lo.at(gh), s1 = ks_hi.at(gh), b0 = kb_lo.at(gh), b1 = kb_hi.at(gh);
@@ -546,6 +551,19 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 rows_transpose(x[n][2], x[n][3]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) x[n][c] *= factor[n];
+            }
+            if constexpr (S::SPLIT > 1) {
+                float4* mine = swap + ((turn * W + warp) * NR) * kWarp + lane;
+                const float4* other = swap + ((turn * W + (warp ^ 1)) * NR) * kWarp + lane;
+#pragma unroll
+                for (int n = 0; n < NR; ++n) mine[n * kWarp] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + warp / 2) : "memory");
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    const float4 y = other[n * kWarp];
+                    x[n][0] += y.x; x[n][1] += y.y; x[n][2] += y.z; x[n][3] += y.w;
+                }
+                turn ^= 1;
             }
             if (!((there >> stage & 1u) && rel0 >= low_most && rel0 + kRowsTile <= open_end)) {
                 const bool has_page = there >> stage & 1u;
@@ -743,7 +761,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
         item += segment;
 
         // ---- the segment's result: out^T = 2^E (2^24 o - centre * ones) + b_sum, over l ----
-        float* part = a.partial + (size_t)(2 * worker + (from_start ? 1 : 0)) * RB * (D + 2);
+        float* part = a.partial + (size_t)((2 * worker + (from_start ? 1 : 0)) * S::SPLIT + half) * RB * (S::DW + 2);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             float sum = l[n];
@@ -778,11 +796,11 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                     if (whole) {
                         const float i = c ? inv1 : inv0;
                         const uint32_t flat = now.flat0 + r;
-                        uint16_t* dst = a.out + (size_t)(now.seq.row0 + flat / a.group) * a.out_stride + (size_t)(now.head * a.group + flat % a.group) * D + d;
+                        uint16_t* dst = a.out + (size_t)(now.seq.row0 + flat / a.group) * a.out_stride + (size_t)(now.head * a.group + flat % a.group) * D + half * S::DW + d;
                         *reinterpret_cast<uint4*>(dst) = make_uint4(rows_pair<BF16>(v[0] * i, v[1] * i), rows_pair<BF16>(v[2] * i, v[3] * i),
                                                                     rows_pair<BF16>(v[4] * i, v[5] * i), rows_pair<BF16>(v[6] * i, v[7] * i));
                     } else {
-                        float* dst = part + 2 * RB + (size_t)r * D + d;
+                        float* dst = part + 2 * RB + r * S::DW + d;
                         *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
                         *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
                     }
@@ -791,8 +809,8 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
         }
         if (!whole) {
             const uint64_t unit_item = item - segment - (uint64_t)first_tile;
-            const uint32_t c0 = share_of_last(total, workers, unit_item + 1), parts = share_of_last(total, workers, unit_item + now.range.tiles) - c0 + 1;
-            rows_join<D, RB, BF16>(a, now.seq.row0, now.head, now.flat0, c0, worker - c0, parts, valid, lane);
+            const uint32_t c0 = shares.of(unit_item), parts = shares.of(unit_item + now.range.tiles - 1) - c0 + 1;
+            rows_join<D, S::DW, RB, BF16>(a, now.seq.row0, now.head, now.flat0, c0, worker - c0, parts, valid, half, lane);
         }
         if (item < stop) rows_next_unit(a, now);
     }
@@ -808,7 +826,7 @@ static tf_status launch_rows(tf_context* ctx, cudaStream_t st, const AttnArgs& a
     const tf_status s = ensure_dynamic_smem(ctx, kernel, smem_cache, S::SMEM);
     if (s != TF_OK) return s;
     uint32_t blocks = resident_blocks(ctx, kernel, blocks_cache, S::THREADS, S::SMEM);
-    blocks = lesser(blocks, lesser(ws->row_capacity / RB, ws->max_workers) / S::WARPS);
+    blocks = lesser(blocks, lesser(ws->row_capacity / RB, ws->max_workers) / S::WORKERS);
     TF_REQUIRE(ctx, blocks > 0, TF_ERR_CUDA, "tf_tree_attention: the kernel does not fit on the device");
     kernel<<<blocks, S::THREADS, S::SMEM, st>>>(a);
     return check_launch(ctx, "tf_tree_attention");
