@@ -62,11 +62,11 @@ static void walk(const AttnArgs& a, uint32_t grid) {
             const uint32_t segment = (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), stop - item);
             const bool to_end = now.tile + segment == now.range.tiles;
             CHECK(now.flat0 < now.flat_rows(a) && segment > 0);
-            CHECK(now.range.end <= (int64_t)a.table.stride << a.table.page_log2);
+            CHECK((int64_t)now.range.end <= (int64_t)a.table.stride << a.table.page_log2);
             for (uint32_t k = 0; k < segment; ++k) {
-                const int64_t token0 = (now.range.tile0 + now.tile + k) * TILE;
+                const int64_t token0 = (int64_t)(now.range.tile0 + now.tile + k) * TILE;
                 for (int i = 0; i < TILE / 16; ++i)
-                    if (token0 + 16 * i < now.range.end) CHECK(a.table.page(now.b, token0 + 16 * i) < (int32_t)a.table.pages);
+                    if (token0 + 16 * i < (int64_t)now.range.end) CHECK(a.table.page(now.b, token0 + 16 * i) < (int32_t)a.table.pages);
             }
             seen[u].push_back({c, segment});
             tiles[u] = now.range.tiles;

@@ -173,6 +173,25 @@ def test_rows_that_see_nothing_are_zero_and_masked_values_reach_nobody(tf_ctx, w
     _close(got[clean], want[clean], tol[clean])
 
 
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("rows", [7, 40])
+def test_a_token_that_is_not_finite_at_any_place_of_a_tile(tf_ctx, workspaces, dim, bits, rows):
+    """A drafted token that no row sees, at every place of a tile of 16, with planes that are not finite, one at a time."""
+    for place in range(16):
+        context = 32 + place                                    # row 0 stands at `place` of its tile
+        case = Case(50 + place, [rows], [context], 1, dim, bits, 16, DEV)
+        for i, bad in ((1, float("nan")), (2, float("inf")), (4, float("inf")), (5, float("nan"))):
+            plane = case.planes[i][int(case.table[0, context // 16]), :, context % 16]
+            old = plane.clone()
+            plane[:, -1] = bad
+            case.upload()
+            plane.copy_(old)
+            masks = [{j for j in range(1, r + 1)} for r in range(rows)]
+            q = _q(case, 2, F16)
+            got = _run(tf_ctx, workspaces, case, q, F16, masks=masks)
+            _close(got, *ref.attention(case, q, [ref.visible(rows, context, 0, masks)], dim ** -0.5, half_step(F16)))
+
+
 @pytest.mark.parametrize("rows", [[4], [40]])
 def test_large_values_reach_only_the_rows_that_see_them(tf_ctx, workspaces, rows):
     """A drafted token with values 10^5 times the others', seen by itself alone: the other rows keep their precision. The same for

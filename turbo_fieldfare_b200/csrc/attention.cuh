@@ -160,7 +160,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
     uint64_t next_item = item;
     // pages of the four runs of 16 tokens of a tile, as this thread's rows need them; -1: left out
     auto load_tile = [&](uint32_t stage) {
-        const int64_t token0 = (next.range.tile0 + next.tile) * kTile;
+        const int64_t token0 = next.token0();
         int32_t page[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) page[i] = token0 + 16 * i < next.range.end ? a.table.page(next.b, token0 + 16 * i) : -1;
@@ -192,7 +192,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
     };
     // the runs of 16 tokens of the current tile that have a page
     auto runs_of = [&](const Cursor<MT, kTile>& c) -> uint32_t {
-        const int64_t token0 = (c.range.tile0 + c.tile) * kTile;
+        const int64_t token0 = c.token0();
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -257,8 +257,8 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
                     }
                 }
                 if (a.window) {
-                    const int64_t pos = a.mask ? max((int64_t)a.positions[now.seq.row0 + token], now.seq.context) : now.seq.context + token;
-                    const int64_t l = pos - (int64_t)a.window + 1 - now.range.tile0 * kTile;
+                    const int64_t pos = a.mask ? max((int64_t)a.positions[now.seq.row0 + token], (int64_t)now.seq.context) : (int64_t)now.seq.context + token;
+                    const int64_t l = pos - (int64_t)a.window + 1 - (int64_t)now.range.tile0 * kTile;
                     low = (int32_t)max((int64_t)0, min(l, (int64_t)0x7FFFFFFF));
                 }
             }
@@ -312,7 +312,7 @@ tree_attention_kernel(const __grid_constant__ AttnArgs a) {
 
         for (uint32_t done = 0; done < segment; ++done, ++item) {
             const uint32_t runs = runs_of(now);
-            const int64_t token0 = (now.range.tile0 + now.tile) * kTile;
+            const int64_t token0 = now.token0();
             const int32_t rel0 = now.tile * kTile;             // of the tile's first token, as row_low counts
             cp_async_wait<S::STAGES - 2>();
             __syncthreads();                                   // the tile has landed for all

@@ -34,41 +34,48 @@ constexpr int kJoin = 16;             // shares that are joined at a time
 template <typename T>
 __host__ __device__ __forceinline__ T lesser(T a, T b) { return a < b ? a : b; }
 
+// Tokens are 32-bit numbers: from here on none is looked at (a cache of more would be 2^37 bytes at the least).
+constexpr uint32_t kMostTokens = 0x7FFFFF00u;
+
 // The lengths of a sequence, cut to what the arrays and the table can hold.
 struct Sequence {
     uint32_t row0, rows;      // its rows of the call
-    int64_t context;          // cached tokens before them
+    uint32_t context;         // cached tokens before them
     __host__ __device__ __forceinline__ void load(const AttnArgs& a, uint32_t b, bool report) {
-        const int64_t begin = a.row_offsets[b], end = a.row_offsets[b + 1], c = a.context_lengths[b];
-        const int64_t lo = begin < 0 ? 0 : begin > (int64_t)a.rows ? (int64_t)a.rows : begin;
-        const int64_t hi = end < lo ? lo : end > (int64_t)a.rows ? (int64_t)a.rows : end;
+        const int32_t begin = a.row_offsets[b], end = a.row_offsets[b + 1], c = a.context_lengths[b];
+        const int32_t most = (int32_t)a.rows, lo = begin < 0 ? 0 : begin > most ? most : begin, hi = end < lo ? lo : end > most ? most : end;
         row0 = (uint32_t)lo;
         rows = (uint32_t)(hi - lo);
-        context = c < 0 ? 0 : c;
+        context = c < 0 ? 0u : (uint32_t)c;
         if (report) {
             if (lo != begin || hi != end) *a.error = kErrKvOffsets;
-            if (rows && (c < 0 || context + rows > (int64_t)a.table.stride << a.table.page_log2)) *a.error = kErrKvPage;
+            if (rows && (c < 0 || (uint64_t)context + rows > (uint64_t)a.table.stride << a.table.page_log2)) *a.error = kErrKvPage;
         }
     }
 };
 
-// The tokens that the rows [flat0, flat0 + MT) of a sequence's kv head may see, in tiles.
+// The tokens that the rows [flat0, flat0 + mt) of a sequence's kv head may see, in tiles.
 struct UnitRange {
-    int64_t end;              // tokens from here on are seen by no row
-    int64_t tile0;
-    uint32_t tiles;           // at least one, so that rows which see nothing are still written
-    __host__ __device__ __forceinline__ void set(const AttnArgs& a, const Sequence& s, uint32_t flat0, uint32_t mt, int tile) {
-        const uint32_t first = flat0 / a.group, last_flat = (uint32_t)(lesser((uint64_t)flat0 + mt, (uint64_t)s.rows * a.group) - 1), last = last_flat / a.group;
-        const int64_t drafted = a.mask ? (int64_t)lesser((uint64_t)s.rows, (uint64_t)a.mask_words * 64) : (int64_t)last + 1;
-        int64_t low = 0;
-        if (a.window) low = s.context + (a.mask ? 0 : (int64_t)first) - (int64_t)a.window + 1;
-        if (low < 0) low = 0;
-        // (and below 2^31 less a tile, so that tokens are 32-bit numbers: a cache of more would be 2^37 bytes at the least)
-        end = lesser(lesser(s.context + drafted, (int64_t)a.table.stride << a.table.page_log2), (int64_t)0x7FFFFF00);
-        if (low > end) low = end;
+    uint32_t end;             // tokens from here on are seen by no row
+    uint32_t tile0, tiles;    // at least one tile, so that rows which see nothing are still written
+    __host__ __device__ __forceinline__ void set(const AttnArgs& a, const Sequence& s, uint32_t flat0, uint32_t mt, uint32_t tile) {
+        uint32_t first = 0, drafted = s.rows;
+        if ((uint64_t)s.rows * a.group > mt) {                 // (a lone unit needs no division)
+            first = flat0 / a.group;
+            if (!a.mask) drafted = lesser((flat0 + mt - 1) / a.group + 1, s.rows);
+        }
+        if (a.mask && (drafted >> 6) >= a.mask_words) drafted = a.mask_words * 64;
+        end = s.context + drafted;                             // both below 2^31
+        const uint32_t held = (a.table.stride - 1) >> (31 - a.table.page_log2) ? kMostTokens : lesser(a.table.stride << a.table.page_log2, kMostTokens);
+        end = lesser(end, held);
+        uint32_t low = 0;
+        if (a.window) {
+            const uint32_t from = s.context + (a.mask ? 0u : first) + 1;
+            low = from > a.window ? lesser(from - a.window, end) : 0u;
+        }
         tile0 = low / tile;
-        const int64_t stop = (end + tile - 1) / tile;
-        tiles = stop > tile0 ? (uint32_t)(stop - tile0) : 1u;
+        const uint32_t stop = (end + tile - 1) / tile;
+        tiles = stop > tile0 ? stop - tile0 : 1u;
     }
 };
 
@@ -78,12 +85,12 @@ struct Cursor {
     Sequence seq;
     UnitRange range;
     uint32_t b, head, flat0, tile;       // tile counts from range.tile0
-    __host__ __device__ __forceinline__ int64_t token0() const { return (range.tile0 + tile) * TILE; }
-    __host__ __device__ __forceinline__ uint64_t flat_rows(const AttnArgs& a) const { return (uint64_t)seq.rows * a.group; }
+    __host__ __device__ __forceinline__ uint32_t token0() const { return (range.tile0 + tile) * TILE; }
+    __host__ __device__ __forceinline__ uint32_t flat_rows(const AttnArgs& a) const { return seq.rows * a.group; }
     // to the first tile of the next unit
     __host__ __device__ __forceinline__ void next_unit(const AttnArgs& a) {
         tile = 0;
-        if ((uint64_t)flat0 + MT < flat_rows(a)) {
+        if (flat0 + MT < flat_rows(a)) {
             flat0 += MT;
         } else if (flat0 = 0; ++head == a.kv_heads) {
             head = 0;
@@ -98,33 +105,13 @@ struct Cursor {
 template <int MT, int TILE>
 __host__ __device__ __forceinline__ uint64_t sequence_tiles(const AttnArgs& a, const Sequence& s) {
     uint64_t n = 0;
-    for (uint64_t f = 0; f < (uint64_t)s.rows * a.group; f += MT) {
+    const uint32_t flat_rows = s.rows * a.group;               // below 2^31
+    for (uint32_t f = 0; f < flat_rows; f += MT) {
         UnitRange r;
-        r.set(a, s, (uint32_t)f, MT, TILE);
+        r.set(a, s, f, MT, TILE);
         n += r.tiles;
     }
     return n;
-}
-
-// The place `left` tiles into a sequence's tiles, of which there are more: kv head, first row of the unit, tile of the unit.
-template <int MT, int TILE>
-__host__ __device__ __forceinline__ void place_in_sequence(const AttnArgs& a, const Sequence& s, uint64_t left, uint32_t (&place)[3]) {
-    const uint64_t n = sequence_tiles<MT, TILE>(a, s);
-    place[0] = 0;
-    while (left >= n) {
-        left -= n;
-        ++place[0];
-    }
-    for (uint64_t f = 0;; f += MT) {
-        UnitRange r;
-        r.set(a, s, (uint32_t)f, MT, TILE);
-        if (left < r.tiles) {
-            place[1] = (uint32_t)f;
-            place[2] = (uint32_t)left;
-            return;
-        }
-        left -= r.tiles;
-    }
 }
 
 // `total` tiles in shares that differ by one at the most: the first `more` workers have one more than `each`. No more workers than tiles.
@@ -148,5 +135,26 @@ struct Shares {
         return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
     }
 };
+
+// The place `left` tiles into a sequence's tiles, of which there are more: kv head, first row of the unit, tile of the unit.
+template <int MT, int TILE>
+__host__ __device__ __forceinline__ void place_in_sequence(const AttnArgs& a, const Sequence& s, uint64_t left, uint32_t (&place)[3]) {
+    const uint64_t n = sequence_tiles<MT, TILE>(a, s);
+    place[0] = 0;
+    if (left >= n) {
+        place[0] = (uint32_t)Shares::divide(left, n);
+        left -= n * place[0];
+    }
+    for (uint32_t f = 0;; f += MT) {
+        UnitRange r;
+        r.set(a, s, f, MT, TILE);
+        if (left < r.tiles) {
+            place[1] = f;
+            place[2] = (uint32_t)left;
+            return;
+        }
+        left -= r.tiles;
+    }
+}
 
 }  // namespace tf

@@ -13,12 +13,14 @@
 // fp16, and what the bias adds is summed in fp32. The rounding of p' shall weigh a code's distance from the centre of the codes, not the code
 // itself: sum p' (c - centre) = sum p' c - centre sum p', with sum p' of all groups by one more MMA each into the rows of a common
 // accumulator, against sum p (b + centre s). E is a row's own, after the largest p s so far (tokens that it does not see have p = 0
-// and no say), and m a maximum that is raised only when a logit exceeds it by 8: a vote each per tile, and what was summed is rescaled
-// only when one of them moves.
+// and no say), and m a maximum that is raised only when a logit exceeds it by 8: one vote per tile, and what was summed is
+// rescaled only when one of them moves.
 #pragma once
 
 #include "attention_launch.cuh"
 #include "mma_gemv.cuh"
+
+#include <type_traits>
 
 namespace tf {
 
@@ -68,9 +70,18 @@ __device__ __forceinline__ float rows_exp2(float x) {          // 2^x; results b
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float rows_max_nan(float a, float b) {      // a NaN stays
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 __device__ __forceinline__ uint32_t rows_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t rows_mul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t rows_pair(float lo, float hi) {
@@ -159,44 +170,47 @@ __device__ __noinline__ uint32_t rows_sanitise(uint8_t* scales, int plane_bytes,
 template <int D, int DW, int RB, bool BF16>
 __device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_t head, uint32_t flat0, uint32_t c0, uint32_t i, uint32_t parts, uint32_t valid,
                                        uint32_t half, int lane) {
-    constexpr int VEC = DW / 32, SPLIT = D / DW, BATCH = VEC >= 8 ? 8 : 16;
+    // Loops that are short in code: a block runs them once or twice, and what is not in the instruction cache yet costs more than the work.
+    constexpr int VEC = DW / 32, SPLIT = D / DW, BATCH = VEC == 8 ? 8 : 16;
     constexpr uint32_t kSlot = RB * (DW + 2);
+    using Vec = std::conditional_t<VEC == 2, float2, float4>;
+    constexpr int VECS = VEC / (sizeof(Vec) / 4);
     auto place = [&](uint32_t p) { return (p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * SPLIT + half; };
     uint32_t span = 1;
+#pragma unroll 1
     for (uint32_t* tickets = a.tickets; parts > 1; tickets += a.ticket_stride, span *= kJoin) {
         const uint32_t group = i / kJoin, base = group * kJoin, members = min((uint32_t)kJoin, parts - base);
-        __threadfence();                                       // this worker's share, or the group that it joined, before its ticket
-        __syncwarp();
+        uint32_t* ticket = tickets + place(base * span);
+        __syncwarp();                                          // this worker's share, or the group that it joined, before its ticket
         uint32_t old = 0;
-        if (lane == 0) old = atomicAdd(tickets + place(base * span), 1u);
+        if (lane == 0) asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(ticket) : "memory");
         if (__shfl_sync(kFullMask, old, 0) != members - 1) return;
-        if (lane == 0) tickets[place(base * span)] = 0;
-        __threadfence();
-        const bool final = parts <= kJoin;
+        __syncwarp();                                          // what the others left, after their tickets
+        if (lane == 0) *ticket = 0;
+        const bool final = parts <= kJoin, is = (uint32_t)lane < members;
         float* first = a.partial + (size_t)place(base * span) * kSlot;
+        const float* mine = a.partial + (size_t)place((base + (is ? lane : 0)) * span) * kSlot;
+#pragma unroll 1
         for (uint32_t r = 0; r < valid; ++r) {
             // past L1, which may hold a slot as it was before
-            const float* mine = a.partial + (size_t)place((base + min((uint32_t)lane, members - 1)) * span) * kSlot;
-            const float mp = (uint32_t)lane < members ? __ldcg(mine + r) : -INFINITY, lp = (uint32_t)lane < members ? __ldcg(mine + RB + r) : 0.0f;
-            float top = 0.0f, w = 0.0f, sum = 0.0f, v[VEC];
+            const float mp = is ? __ldcg(mine + r) : -INFINITY, lp = is ? __ldcg(mine + RB + r) : 0.0f;
+            float w = 0.0f, v[VEC], top = mp, sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
-#pragma unroll
-            for (uint32_t p0 = 0; p0 < kJoin; p0 += BATCH) {
-                if (p0 >= members) break;
-                float2 x[BATCH][VEC / 2];
+#pragma unroll 1
+            for (uint32_t p0 = 0; p0 < members; p0 += BATCH) {
+                Vec x[BATCH][VECS];
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
-                    const float2* src = reinterpret_cast<const float2*>(a.partial + (size_t)place((base + min(p0 + k, members - 1)) * span) * kSlot + 2 * RB + r * DW + lane * VEC);
+                    const Vec* src = reinterpret_cast<const Vec*>(a.partial + (size_t)place((base + min(p0 + k, members - 1)) * span) * kSlot + 2 * RB + r * DW + lane * VEC);
 #pragma unroll
-                    for (int e = 0; e < VEC / 2; ++e) x[k][e] = __ldcg(src + e);
+                    for (int e = 0; e < VECS; ++e) x[k][e] = __ldcg(src + e);
                 }
                 if (p0 == 0) {
-                    top = mp;
 #pragma unroll
                     for (int off = kJoin / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
                     top = __shfl_sync(kFullMask, top, 0);
-                    w = (uint32_t)lane < members ? rows_exp2(mp - (top == -INFINITY ? 0.0f : top)) : 0.0f;
+                    w = is ? rows_exp2(mp - (top == -INFINITY ? 0.0f : top)) : 0.0f;
                     sum = w * lp;
 #pragma unroll
                     for (int off = kJoin / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
@@ -204,13 +218,10 @@ __device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_
                 }
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
-                    if (p0 + k >= members) break;
-                    const float wk = __shfl_sync(kFullMask, w, p0 + k);
+                    // a slot behind the last one counts for nothing, whatever it holds
+                    const float wk = __shfl_sync(kFullMask, w, (p0 + k) & 31);
 #pragma unroll
-                    for (int e = 0; e < VEC / 2; ++e) {
-                        v[2 * e] = fmaf(wk, x[k][e].x, v[2 * e]);
-                        v[2 * e + 1] = fmaf(wk, x[k][e].y, v[2 * e + 1]);
-                    }
+                    for (int e = 0; e < VEC; ++e) v[e] = p0 + k < members ? fmaf(wk, reinterpret_cast<const float*>(x[k])[e], v[e]) : v[e];
                 }
             }
             if (final) {
@@ -325,8 +336,8 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
     };
     auto enter_unit = [&] {
         next_left = next.range.tiles - next.tile;
-        next_token = (uint32_t)next.token0();
-        next_end = (uint32_t)next.range.end;
+        next_token = next.token0();
+        next_end = next.range.end;
         next_head = next.head;
         next_table = a.table.table + (size_t)next.b * a.table.stride;
         look_up();
@@ -391,7 +402,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
     uint32_t stage = 0;
     while (item < stop) {
         // ---- a unit's segment: the rows of q as B fragments, their sums per group, what they see ----
-        const uint32_t valid = (uint32_t)lesser((uint64_t)RB, now.flat_rows(a) - now.flat0);
+        const uint32_t valid = lesser((uint32_t)RB, now.flat_rows(a) - now.flat0);
         const uint32_t first_tile = now.tile;
         const uint32_t segment = (uint32_t)lesser((uint64_t)(now.range.tiles - first_tile), stop - item);
         const bool from_start = first_tile == 0, whole = from_start && segment == now.range.tiles;
@@ -406,8 +417,10 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             const bool is = r < valid;
             node[n] = is ? flat / a.group : 0;
             const uint16_t* src = a.q + (size_t)(now.seq.row0 + node[n]) * a.q_stride + (size_t)(now.head * a.group + (is ? flat % a.group : 0)) * D + half * S::DW + 16 * t;
+            // Sixteen elements of each group: as fp16 they are the fragments of four steps, but for 4-bit codes, whose order within eight elements is
+            // (0, 4, 1, 5, 2, 6, 3, 7) and whose odd ones come sixteenfold. The row is brought to one range by a power of two, its largest
+            // element to [128, 256), where fp16 rows do not have it (8-bit codes) or as far as fp16 has the power.
             uint32_t raw[G][8];
-            float most = 0.0f;
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
                 const uint4 lo = is ? *reinterpret_cast<const uint4*>(src + grp * 64) : make_uint4(0, 0, 0, 0);
@@ -415,48 +428,47 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 raw[grp][0] = lo.x; raw[grp][1] = lo.y; raw[grp][2] = lo.z; raw[grp][3] = lo.w;
                 raw[grp][4] = hi.x; raw[grp][5] = hi.y; raw[grp][6] = hi.z; raw[grp][7] = hi.w;
             }
-            auto value = [&](int grp, int j) {
-                const uint16_t h = (uint16_t)(raw[grp][j / 2] >> (16 * (j % 2)));
-                return BF16 ? bf16_bits_to_float(h) : f16_bits_to_float(h);
-            };
+            int e = 0;
+            if constexpr (BF16 || BITS == 4) {
+                uint32_t most = 0;                             // magnitudes order as their bits do
 #pragma unroll
-            for (int grp = 0; grp < G; ++grp)
+                for (int grp = 0; grp < G; ++grp)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(value(grp, j)));
-            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-            // (of this warp's part of it: the product is brought back before parts are added)
-            const int e = most > 0.0f ? max(rows_exponent(most) - 7, -126) : 0;      // the row's largest element to [128, 256)
-            const float down = rows_power(-e);
+                    for (int i = 0; i < 8; ++i) most = __vmaxu2(most, raw[grp][i] & 0x7FFF7FFFu);
+                most = max(most & 0xFFFFu, most >> 16);
+                most = max(most, __shfl_xor_sync(kFullMask, most, 1));
+                most = max(most, __shfl_xor_sync(kFullMask, most, 2));
+                const float top = BF16 ? bf16_bits_to_float((uint16_t)most) : f16_bits_to_float((uint16_t)most);
+                if (top > 0.0f && top <= 3.402823466e38f) e = BF16 ? max(rows_exponent(top) - 7, -126) : min(max(rows_exponent(top) - 7, -15), 15);
+                const float down = rows_power(-e);
+#pragma unroll
+                for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if constexpr (BF16) raw[grp][i] = rows_half2(__uint_as_float(raw[grp][i] << 16) * down, __uint_as_float(raw[grp][i] & 0xFFFF0000u) * down);
+                        else raw[grp][i] = rows_mul2(raw[grp][i], rows_half2(down, down));
+                    }
+            }
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
-                float sum = 0.0f;
-                // element j of the lane's sixteen as fp16, a 4-bit code's odd ones by a sixteenth
-                auto part = [&](int j) {
-                    const bool sixteenth = BITS == 4 && (j % 2);
-                    const __half h = __float2half_rn(value(grp, j) * (sixteenth ? down * 0.0625f : down));
-                    sum += __half2float(h) * (sixteenth ? 16.0f : 1.0f);
-                    return (uint32_t)__half_as_ushort(h);
-                };
+                float sum[4];
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
-                    uint32_t lo, hi;
-                    if constexpr (BITS == 8) {
-                        lo = part(4 * ks) | part(4 * ks + 1) << 16;
-                        hi = part(4 * ks + 2) | part(4 * ks + 3) << 16;
-                    } else {
-                        const int j = 8 * (ks / 2) + 2 * (ks % 2);
-                        lo = part(j) | part(j + 4) << 16;
-                        hi = part(j + 1) | part(j + 5) << 16;
+                    uint32_t lo = raw[grp][2 * ks], hi = raw[grp][2 * ks + 1];
+                    if constexpr (BITS == 4) {
+                        const uint32_t u = raw[grp][4 * (ks / 2) + ks % 2], v = raw[grp][4 * (ks / 2) + ks % 2 + 2];       // elements (j, j + 1) and (j + 4, j + 5)
+                        lo = gm_prmt(u, v, 0x5410);
+                        hi = gm_sixteenth(gm_prmt(u, v, 0x7632));
                     }
                     qf[n][grp * 4 + ks][0] = lo;
                     qf[n][grp * 4 + ks][1] = hi;
+                    // sums of the rows 2t and 2t + 1 by a product with ones (sixteens)
+                    const uint32_t one = 0x3C003C00u, other = BITS == 4 ? 0x4C004C00u : one;
+                    if (ks == 0) rows_mma_first(sum, one, one, other, other, lo, hi);
+                    else rows_mma(sum, one, one, other, other, lo, hi);
                 }
-                sum += __shfl_xor_sync(kFullMask, sum, 1);
-                sum += __shfl_xor_sync(kFullMask, sum, 2);
-                sum *= 5.9604644775390625e-8f;                 // 2^-24, as the products
-                q_sum[n][grp][0] = __shfl_sync(kFullMask, sum, 8 * t);
-                q_sum[n][grp][1] = __shfl_sync(kFullMask, sum, 8 * t + 4);
+                q_sum[n][grp][0] = sum[0] * 5.9604644775390625e-8f;                  // 2^-24, as the products
+                q_sum[n][grp][1] = sum[1] * 5.9604644775390625e-8f;
                 b_sum[n][grp] = 0.0f;
             }
             factor[n] = 16777216.0f * rows_power(e) * a.scale * 1.4426950408889634f;
@@ -464,8 +476,8 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             l[n] = 0.0f;
             low[n] = 0;
             if (a.window && is) {
-                const int64_t pos = a.mask ? max((int64_t)a.positions[now.seq.row0 + node[n]], now.seq.context) : now.seq.context + node[n];
-                const int64_t first = pos - (int64_t)a.window + 1 - now.range.tile0 * kRowsTile;
+                const int64_t pos = a.mask ? max((int64_t)a.positions[now.seq.row0 + node[n]], (int64_t)now.seq.context) : (int64_t)now.seq.context + node[n];
+                const int64_t first = pos - (int64_t)a.window + 1 - (int64_t)now.range.tile0 * kRowsTile;
                 low[n] = (int32_t)max((int64_t)0, lesser(first, (int64_t)0x7FFFFFFF));
             }
             low_most = max(low_most, low[n]);
@@ -485,8 +497,8 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 for (int j = 0; j < 4; ++j) o[n][grp][j][0] = o[n][grp][j][1] = o[n][grp][j][2] = o[n][grp][j][3] = 0.0f;
         }
         // From the unit's first tile on: tokens before open_end are cached ones; every row sees them from low_most on.
-        const int32_t base_token = (int32_t)(now.range.tile0 * kRowsTile), open_end = (int32_t)(lesser(now.seq.context, now.range.end) - base_token),
-                      end_rel = (int32_t)(now.range.end - base_token);
+        const int32_t base_token = (int32_t)(now.range.tile0 * kRowsTile), open_end = (int32_t)lesser(now.seq.context, now.range.end) - base_token,
+                      end_rel = (int32_t)now.range.end - base_token;
         int32_t rel0 = first_tile * kRowsTile;
 
 #pragma unroll 1
@@ -578,7 +590,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                             if (rel < open_end) {
                                 seen = rel >= low[n];
                             } else {
-                                const uint32_t j = (uint32_t)((int64_t)base_token + rel - now.seq.context);
+                                const uint32_t j = (uint32_t)(base_token + rel) - now.seq.context;
                                 if (a.mask) seen = (a.mask[(size_t)(now.seq.row0 + node[n]) * a.mask_words + (j >> 6)] >> (j & 63u)) & 1ull;
                                 else seen = j <= node[n] && (!a.window || node[n] - j < a.window);
                             }
@@ -588,45 +600,20 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 }
             }
 
-            // ---- does a maximum move? ----
-            float over = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < NR; ++n) over = fmaxf(over, fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) - m[n]);
-            // what was summed of rows g + 8 n, times f: their accumulators lie in the columns of other lanes
-            auto rescale = [&](int n, float f) {
-                const float f0 = __shfl_sync(kFullMask, f, 8 * t), f1 = __shfl_sync(kFullMask, f, 8 * t + 4);      // rows 2t, 2t + 1
-                ones[n][0] *= f0; ones[n][1] *= f1;
-#pragma unroll
-                for (int grp = 0; grp < G; ++grp)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) { o[n][grp][j][0] *= f0; o[n][grp][j][1] *= f1; o[n][grp][j][2] *= f0; o[n][grp][j][3] *= f1; }
-            };
-            if (__any_sync(kFullMask, over > 8.0f)) {
-#pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                    float top = fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
-                    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
-                    const float m_new = fmaxf(m[n], top), alpha = m_new == -INFINITY ? 1.0f : rows_exp2(m[n] - m_new);
-                    m[n] = m_new;
-                    l[n] *= alpha;
-#pragma unroll
-                    for (int grp = 0; grp < G; ++grp) b_sum[n][grp] *= alpha;
-                    rescale(n, alpha);
-                }
-            }
-
             // ---- probabilities, at most 2^8 ----
-            float p[NR][4];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
+            float p[NR][4], over = -INFINITY;
+            auto raise_p = [&](int n) {
                 const float base = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) p[n][c] = rows_exp2(x[n][c] - base);
-                l[n] += (p[n][0] + p[n][1]) + (p[n][2] + p[n][3]);
+            };
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                over = fmaxf(over, fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) - m[n]);
+                raise_p(n);
             }
 
-            // ---- does a row's exponent move, is a value plane not finite? ----
+            // ---- does a maximum or a row's exponent move, is a value plane not finite? ----
             const uint8_t *vs_plane = planes + 2 * S::PLANE, *vb_plane = vs_plane + S::PLANE;
             PlanePair<G, S::GH> vs_lo, vs_hi, vb_lo, vb_hi;
             auto load_value_planes = [&](int first) {
@@ -641,7 +628,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 vs_lo.raise(most_s[0], most_s[1]); vs_hi.raise(most_s[2], most_s[3]);
                 vb_lo.raise_all(most_b); vb_hi.raise_all(most_b);
             }
-            bool moves = !__hble2(most_b, finite);
+            bool moves = over > 8.0f || !__hble2(most_b, finite);
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 float most = 0.0f;
@@ -649,12 +636,25 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 for (int key = 0; key < 4; ++key) {
                     const float s = S::GH == 1 ? __uint_as_float((*reinterpret_cast<const uint32_t*>(&most_s[key & 2])) << (key & 1 ? 0 : 16) & 0xFFFF0000u)
                                                : __uint_as_float((*reinterpret_cast<const uint32_t*>(&most_s[key])) & 0xFFFF0000u);
-                    const float z = p[n][key] * s;
-                    most = z <= most ? most : z;               // a NaN stays
+                    most = rows_max_nan(most, p[n][key] * s);
                 }
                 moves |= !(most * down_v[n] < 16384.0f);
             }
             if (__any_sync(kFullMask, moves)) {
+                float alpha[NR];
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    float top = fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
+                    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+                    const float m_new = fmaxf(m[n], top);
+                    alpha[n] = m_new == -INFINITY ? 1.0f : rows_exp2(m[n] - m_new);
+                    m[n] = m_new;
+                    l[n] *= alpha[n];
+                    raise_p(n);
+#pragma unroll
+                    for (int grp = 0; grp < G; ++grp) b_sum[n][grp] *= alpha[n];
+                }
                 bool bad = !__hble2(most_b, finite);
 #pragma unroll
                 for (int key = 0; key < 4; ++key) bad |= !__hble2(most_s[key], finite);
@@ -674,19 +674,21 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 for (int n = 0; n < NR; ++n) {
                     float most = 0.0f;
 #pragma unroll
-                    for (int first = 0; first < G; first += S::GH) {
-                        if (G > S::GH) load_value_planes(first);
+                    for (int grp = 0; grp < G; ++grp)
 #pragma unroll
-                        for (int gh = 0; gh < S::GH; ++gh)
-#pragma unroll
-                            for (int key = 0; key < 4; ++key)
-                                most = fmaxf(most, p[n][key] * fabsf(key < 2 ? vs_lo.at(key, gh) : vs_hi.at(key - 2, gh)));      // a NaN of p leaves it as it is
-                    }
+                        for (int key = 0; key < 4; ++key)
+                            most = fmaxf(most, p[n][key] * fabsf(key < 2 ? vs_lo.at(key, grp) : vs_hi.at(key - 2, grp)));      // a NaN of p leaves it as it is
                     most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
                     most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
                     const int e_new = min(max(e_v[n], rows_exponent(most) - 3), 119);              // now below 16
-                    const float fit = rows_power(e_v[n] - e_new);
-                    rescale(n, fit);
+                    // what was summed of rows g + 8 n: their accumulators lie in the columns of other lanes
+                    const float f = alpha[n] * rows_power(e_v[n] - e_new);
+                    const float f0 = __shfl_sync(kFullMask, f, 8 * t), f1 = __shfl_sync(kFullMask, f, 8 * t + 4);      // rows 2t, 2t + 1
+                    ones[n][0] *= f0; ones[n][1] *= f1;
+#pragma unroll
+                    for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { o[n][grp][j][0] *= f0; o[n][grp][j][1] *= f1; o[n][grp][j][2] *= f0; o[n][grp][j][3] *= f1; }
                     e_v[n] = e_new;
                     down_v[n] = rows_power(-e_new);
                 }
@@ -698,6 +700,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 for (int key = 0; key < 4; ++key) {
                     pd[n][key] = p[n][key] * down_v[n];
                     pc[n][key] = p[n][key] * kCentre;
+                    l[n] += p[n][key];
                 }
 
             // ---- values ----
