@@ -14,7 +14,7 @@ SRC = r'''
 #include <set>
 #include <tuple>
 #include <vector>
-#include "attention.cuh"
+#include "attention_tiles.cuh"
 using namespace tf;
 #define CHECK(c) do { if (!(c)) { std::printf("line %d: %s\n", __LINE__, #c); std::exit(1); } } while (0)
 
@@ -31,7 +31,7 @@ static void walk(const AttnArgs& a, uint32_t grid) {
         Sequence s;
         s.load(a, b, true);
         CHECK(s.row0 + (uint64_t)s.rows <= a.rows && s.context >= 0);
-        total += sequence_tiles<MT, TILE>(a, s) * a.kv_heads;
+        total += sequence_tiles<MT, TILE>(a, s) * a.kv_heads * a.head_parts;
         before[b + 1] = total;
     }
     Shares shares;
@@ -84,7 +84,7 @@ static void walk(const AttnArgs& a, uint32_t grid) {
     for (uint32_t b = 0; b < a.sequences; ++b) {
         Sequence s;
         s.load(a, b, false);
-        units += ((uint64_t)s.rows * a.group + MT - 1) / MT * a.kv_heads;
+        units += ((uint64_t)s.rows * a.group + MT - 1) / MT * a.kv_heads * a.head_parts;
     }
     CHECK(seen.size() == units);
     for (auto& [u, parts] : seen) {
@@ -124,6 +124,7 @@ static void all_shares() {
         for (auto& p : table) p = bad && pick(0, 3) == 0 ? (int32_t)rng() : (int32_t)pick(0, a.table.pages - 1);
         a.table.table = table.data();
         a.row_offsets = offsets.data(); a.context_lengths = contexts.data();
+        a.head_parts = (uint32_t)pick(1, 2);
         a.sequences = n; a.kv_heads = (uint32_t)pick(1, 8); a.group = (uint32_t)pick(1, 9);
         a.window = pick(0, 1) ? 0 : (uint32_t)pick(1, 300);
         static const unsigned long long word = 0;
@@ -131,27 +132,28 @@ static void all_shares() {
         const uint32_t grid = (uint32_t)(pick(0, 1) ? 296 : pick(1, 500));
         walk<8, 16>(a, grid);
         walk<16, 16>(a, 3 * grid);
-        walk<16, 64>(a, grid);
-        walk<64, 64>(a, grid);
+        walk<128, 32>(a, grid);
         walk<128, 64>(a, grid);
+        walk<128, 128>(a, grid);
         CHECK(bad || error == 0);
     }
 }
 
 // What lands in shared memory: every 16-byte piece of a tile at a place of its own, inside of the codes.
-template <int D, int BITS, int MT>
-static void places() {
-    using S = AttnShape<D, BITS, MT>;
-    std::set<uint32_t> k, v;
-    for (uint32_t r = 0; r < kTile; ++r)
-        for (uint32_t p = 0; p < S::PIECES; ++p) {
-            const uint32_t x = S::k_at(r, p * 16), y = S::v_at(r, p * 16);
-            CHECK(x % 16 == 0 && y % 16 == 0 && x + 16 <= S::CODES && y + 16 <= S::CODES);
-            CHECK(k.insert(x).second && v.insert(y).second);
-            for (uint32_t byte = 0; byte < 16; byte += 2) CHECK(S::k_at(r, p * 16 + byte) == x + byte && S::v_at(r, p * 16 + byte) == y + byte);
-        }
-    CHECK(S::OFF_STAGE % 128 == 0 && S::STAGE % 128 == 0 && S::SMEM <= 227 * 1024 && S::STAGES >= 2);
-    CHECK(S::OFF_P % 16 == 0 && S::OFF_RED % 16 == 0 && S::OFF_VRED % 16 == 0 && S::OFF_O % 16 == 0 && S::OFF_SV % 16 == 0 && S::OFF_BV % 16 == 0);
+template <int D, int BITS>
+static void tile_places() {
+    using S = TilesShape<D, BITS>;
+    for (uint32_t rows : {(uint32_t)S::MT, (uint32_t)S::TILE}) {
+        std::set<uint32_t> at;
+        for (uint32_t r = 0; r < rows; ++r)
+            for (uint32_t c = 0; c < D / 8; ++c) {
+                const uint32_t x = S::chunk_at(rows, r, c);
+                CHECK(x % 16 == 0 && x + 16 <= rows * D * 2 && at.insert(x).second);
+            }
+    }
+    // every piece of a tile belongs to one thread's turn
+    CHECK(S::UNPACK % S::K_ROW == 0 && S::UNPACK % S::V_ROW == 0);
+    CHECK(S::OFF_K % 1024 == 0 && S::OFF_V % 1024 == 0 && S::OFF_META % 1024 == 0 && S::K_BYTES % 1024 == 0 && S::V_BYTES % 1024 == 0);
 }
 template <int D, int BITS, int RB>
 static void rows_places() {
@@ -168,7 +170,7 @@ static void rows_places() {
     CHECK(S::STAGES >= 2 && S::STAGES <= 31 && S::BLOCKS * (S::SMEM + 1024 + 256) <= 227 * 1024);
 }
 template <int D, int BITS>
-static void places() { places<D, BITS, 16>(); places<D, BITS, 32>(); places<D, BITS, 64>(); rows_places<D, BITS, 8>(); }
+static void places() { tile_places<D, BITS>(); rows_places<D, BITS, 8>(); }
 
 // Refusals: none of them reaches the device.
 static tf_context context;

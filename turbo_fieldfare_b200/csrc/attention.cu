@@ -86,7 +86,7 @@ tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32
     a.error = ctx->device_error;
     a.q_stride = q_stride; a.out_stride = out_stride;
     a.sequences = batch->sequences; a.rows = batch->rows; a.kv_heads = cache->kv_heads; a.group = group;
-    a.window = window; a.scale = scale;
+    a.window = window; a.scale = scale; a.head_parts = 1;
     const tf::DeviceScope scope(ctx->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool bf16 = act_dtype == TF_BF16;

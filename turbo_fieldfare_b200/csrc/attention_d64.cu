@@ -1,5 +1,5 @@
 // Attention over the quantised cache for heads of 64 elements.
-#include "attention.cuh"
+#include "attention_tiles.cuh"
 
 namespace tf {
 template tf_status attend<64, 4>(tf_context*, cudaStream_t, const AttnArgs&, const tf_attention_workspace*, bool);

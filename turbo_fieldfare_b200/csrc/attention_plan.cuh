@@ -26,6 +26,7 @@ struct AttnArgs {
     uint32_t ticket_stride;
     uint32_t* error;
     uint32_t q_stride, out_stride, sequences, rows, kv_heads, group, mask_words, window;
+    uint32_t head_parts;      // units per kv head whose values are parts of the head's
     float scale;
 };
 
@@ -92,7 +93,7 @@ struct Cursor {
         tile = 0;
         if (flat0 + MT < flat_rows(a)) {
             flat0 += MT;
-        } else if (flat0 = 0; ++head == a.kv_heads) {
+        } else if (flat0 = 0; ++head == a.kv_heads * a.head_parts) {
             head = 0;
             do { if (++b >= a.sequences) return; seq.load(a, b, false); } while (seq.rows == 0);
         }

@@ -244,6 +244,56 @@ __device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_
     }
 }
 
+// A worker's share, found by a whole warp that goes over the sequences 32 at a time. False: there are fewer tiles than workers.
+template <int MT, int TILE>
+__device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t worker, uint32_t workers_most, int lane, bool report, Cursor<MT, TILE>& now, Shares& shares,
+                                           uint64_t& item, uint64_t& stop) {
+    auto tiles_of = [&](uint32_t b, Sequence& s, bool tell) -> uint64_t {
+        if (b >= a.sequences) return 0;
+        s.load(a, b, tell);
+        return sequence_tiles<MT, TILE>(a, s) * a.kv_heads * a.head_parts;
+    };
+    uint64_t total = 0;
+#pragma unroll 4
+    for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWarp) {
+        Sequence s;
+        total += tiles_of(b0 + lane, s, report);
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(kFullMask, total, off);
+    shares.set(total, workers_most);
+    if (worker >= shares.workers) return false;
+    item = shares.begin(worker);
+    stop = shares.begin(worker + 1);
+    uint64_t before = 0;
+    for (uint32_t b0 = 0;; b0 += kWarp) {                      // ends: item is below the total
+        Sequence s = {};
+        const uint64_t mine = tiles_of(b0 + lane, s, false);
+        uint64_t upto = mine;
+#pragma unroll
+        for (int off = 1; off < kWarp; off <<= 1) {
+            const uint64_t o = __shfl_up_sync(kFullMask, upto, off);
+            if (lane >= off) upto += o;
+        }
+        const uint64_t all = __shfl_sync(kFullMask, upto, kWarp - 1);
+        if (item < before + all) {
+            const int owner = __ffs(__ballot_sync(kFullMask, before + upto > item)) - 1;
+            const uint64_t left = item - before - __shfl_sync(kFullMask, upto - mine, owner);
+            now.b = b0 + owner;
+            now.seq.row0 = __shfl_sync(kFullMask, s.row0, owner);
+            now.seq.rows = __shfl_sync(kFullMask, s.rows, owner);
+            now.seq.context = __shfl_sync(kFullMask, s.context, owner);
+            uint32_t place[3];
+            place_in_sequence<MT, TILE>(a, now.seq, left, place);
+            now.head = place[0]; now.flat0 = place[1]; now.tile = place[2];
+            break;
+        }
+        before += all;
+    }
+    now.range.set(a, now.seq, now.flat0, MT, TILE);
+    return true;
+}
+
 template <int RB>
 __device__ __noinline__ void rows_next_unit(const AttnArgs& a, Cursor<RB, kRowsTile>& c) { c.next_unit(a); }
 
@@ -266,55 +316,10 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, g = lane / 4, t = lane % 4;
     const uint32_t half = warp % S::SPLIT, worker = blockIdx.x * S::WORKERS + warp / S::SPLIT;
 
-    // ---- this worker's share: every warp goes over the sequences, 32 at a time ----
     Cursor<RB, kRowsTile> now;
     Shares shares;
     uint64_t item, stop;
-    {
-        auto tiles_of = [&](uint32_t b, Sequence& s, bool report) -> uint64_t {
-            if (b >= a.sequences) return 0;
-            s.load(a, b, report);
-            return sequence_tiles<RB, kRowsTile>(a, s) * a.kv_heads;
-        };
-        uint64_t total = 0;
-#pragma unroll 4
-        for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWarp) {
-            Sequence s;
-            total += tiles_of(b0 + lane, s, blockIdx.x == 0);
-        }
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(kFullMask, total, off);
-        shares.set(total, gridDim.x * S::WORKERS);
-        if (worker >= shares.workers) return;
-        item = shares.begin(worker);
-        stop = shares.begin(worker + 1);
-        uint64_t before = 0;
-        for (uint32_t b0 = 0;; b0 += kWarp) {                  // ends: item is below the total
-            Sequence s = {};
-            const uint64_t mine = tiles_of(b0 + lane, s, false);
-            uint64_t upto = mine;
-#pragma unroll
-            for (int off = 1; off < kWarp; off <<= 1) {
-                const uint64_t o = __shfl_up_sync(kFullMask, upto, off);
-                if (lane >= off) upto += o;
-            }
-            const uint64_t all = __shfl_sync(kFullMask, upto, kWarp - 1);
-            if (item < before + all) {
-                const int owner = __ffs(__ballot_sync(kFullMask, before + upto > item)) - 1;
-                const uint64_t left = item - before - __shfl_sync(kFullMask, upto - mine, owner);
-                now.b = b0 + owner;
-                now.seq.row0 = __shfl_sync(kFullMask, s.row0, owner);
-                now.seq.rows = __shfl_sync(kFullMask, s.rows, owner);
-                now.seq.context = __shfl_sync(kFullMask, s.context, owner);
-                uint32_t place[3];
-                place_in_sequence<RB, kRowsTile>(a, now.seq, left, place);
-                now.head = place[0]; now.flat0 = place[1]; now.tile = place[2];
-                break;
-            }
-            before += all;
-        }
-        now.range.set(a, now.seq, now.flat0, RB, kRowsTile);
-    }
+    if (!find_share<RB, kRowsTile>(a, worker, gridDim.x * S::WORKERS, lane, blockIdx.x == 0, now, shares, item, stop)) return;
 
     // ---- this warp's ring: what the next request needs is in registers, the rest of its cursor in memory ----
     uint8_t* ring = smem + warp * (S::STAGES * S::STAGE);

@@ -68,19 +68,6 @@ __device__ __forceinline__ uint32_t float_to_pair(float a, float b) {
     }
 }
 
-// WORDS 32-bit words at p, which is aligned to them (to 16 bytes from four words on).
-template <int WORDS>
-__device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], const void* p) {
-    if constexpr (WORDS == 1) w[0] = *static_cast<const uint32_t*>(p);
-    else if constexpr (WORDS == 2) { const uint2 t = *static_cast<const uint2*>(p); w[0] = t.x; w[1] = t.y; }
-    else {
-#pragma unroll
-        for (int i = 0; i < WORDS / 4; ++i) {
-            const uint4 t = static_cast<const uint4*>(p)[i];
-            w[4 * i] = t.x; w[4 * i + 1] = t.y; w[4 * i + 2] = t.z; w[4 * i + 3] = t.w;
-        }
-    }
-}
 template <int WORDS>
 __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[WORDS]) {
     if constexpr (WORDS == 1) *static_cast<uint32_t*>(p) = w[0];

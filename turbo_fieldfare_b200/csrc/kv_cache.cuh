@@ -38,6 +38,19 @@ inline uint32_t log2_of(uint32_t power) {
     return n;
 }
 
+// WORDS 32-bit words at p, which is aligned to them (to 16 bytes from four words on).
+template <int WORDS>
+__device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], const void* p) {
+    if constexpr (WORDS == 1) w[0] = *static_cast<const uint32_t*>(p);
+    else if constexpr (WORDS == 2) { const uint2 t = *static_cast<const uint2*>(p); w[0] = t.x; w[1] = t.y; }
+    else {
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i) {
+            const uint4 t = static_cast<const uint4*>(p)[i];
+            w[4 * i] = t.x; w[4 * i + 1] = t.y; w[4 * i + 2] = t.z; w[4 * i + 3] = t.w;
+        }
+    }
+}
 // Page of a token of sequence `seq`, or -1: outside the table or the planes.
 struct KvTable {
     const int32_t* table;
