@@ -2,16 +2,18 @@
 //
 // With this many rows the products bound it, 4 * 128 * D FLOP per token and unit, next to the unpacking, which a unit pays once for its 128 rows.
 // One persistent block per SM; 8 warps unpack, one issues the MMAs, 4 do the softmax, a thread per row. For tile i of TILE tokens:
-//   unpack:  codes and planes from global memory (requested a tile ahead) -> K_i, V_i in fp16, [64 elements][token][128 bytes] with the 128-byte
-//            swizzle, two buffers each
+//   unpack:  codes and planes, by cp.async a tile ahead into places of the thread's own -> K_i, V_i in fp16, [64 elements][token][128 bytes] with the
+//            128-byte swizzle (K in one buffer: it is free again when its logits are there, long before the next ones are wanted)
 //   MMA:     S_i = Q K_i^T into tensor memory (two buffers), then O += P_(i-1) V_(i-1); K is K-major, V, as it lies, MN-major
 //   softmax: S_i -> registers -> mask, 2^(x - m), P_i as fp16 into tensor memory (the A operand of the second product)
+// The loops are rolled where registers allow it: three kinds of warps share an SM's instruction caches, and straight-line code of all of them
+// waited for instructions most of the time (9600 clocks a tile instead of what the notes of the measurements give).
 // K_i and V_i carry (code - centre) s + (bias + centre s) rounded to fp16, 2^-11 of the value: logits see it as an error of about 2^-12 |q||k| / sqrt(D),
-// of the size of the output's own rounding to 16 bits. The planes are divided by powers of two that follow the largest of the tile (K) or
-// of all tiles so far (V), so caches outside of fp16's range work; a token's values keep their precision beside others up to 2^20 times as large.
-// m is raised only when a logit exceeds it by 8, and what O holds is rescaled only then, or when V's exponent grows. TILE * D is 16384 but for heads of 64,
-// so the buffers of all head sizes have the same size; heads of 512, whose product would fill tensor memory alone, are two units
-// with half of the values each.
+// of the size of the output's own rounding to 16 bits. A token's values are divided by a power of two of its own first; K's comes back with the
+// logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far: tokens that a row
+// does not see have no say, and no cache leaves fp16's range. m is raised only when a logit exceeds it by 8, and what O holds is
+// rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
+// are two units with half of the values each.
 #pragma once
 
 #include "async_copy.cuh"
@@ -28,9 +30,15 @@ struct TilesShape {
     static constexpr int ROW_BYTES = D * BITS / 8, PIECE = 2 * BITS;          // bytes of 16 codes
     static constexpr int K_ROW = D / 16, V_ROW = DV / 16;                     // pieces of a token
     static constexpr int K_EACH = TILE * K_ROW / UNPACK, V_EACH = TILE * V_ROW / UNPACK;
-    static constexpr int RUNS = TILE / 16;
+    static constexpr int V_BUFS = D == 512 ? 1 : 2;
+    static constexpr bool SAME = K_ROW == V_ROW;                              // a thread's pieces of K and V are of the same tokens
     static constexpr int Q_BYTES = MT * D * 2, K_BYTES = TILE * D * 2, V_BYTES = TILE * DV * 2;
-    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * K_BYTES, OFF_META = OFF_V + 2 * V_BYTES, META = 1024, SMEM = OFF_META + META + 1024;
+    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + K_BYTES;
+    // what the unpacking threads have requested, [piece][thread]: codes; (scale, bias) words, of V for two tiles; pages of the next tiles
+    static constexpr int OFF_KC = OFF_V + V_BUFS * V_BYTES, OFF_VC = OFF_KC + K_EACH * UNPACK * PIECE, OFF_KS = OFF_VC + V_EACH * UNPACK * PIECE,
+                         OFF_VS = OFF_KS + K_EACH * UNPACK * 8, OFF_KP = OFF_VS + 2 * V_EACH * UNPACK * 8, OFF_VP = SAME ? OFF_KP : OFF_KP + K_EACH * UNPACK * 4,
+                         OFF_META = OFF_VP + 2 * V_EACH * UNPACK * 4;
+    static constexpr int META = (256 + 2 * TILE * 9 + 127) / 128 * 128, SMEM = OFF_META + META + 1024;
     // tensor memory, in columns
     static constexpr int COL_S = 0, COL_P = 2 * TILE, COL_O = 3 * TILE, COLS = 512;
     static_assert(COL_O + DV <= COLS && SMEM <= 227 * 1024 && K_EACH * UNPACK == TILE * K_ROW && V_EACH * UNPACK == TILE * V_ROW, "sizes");
@@ -40,16 +48,16 @@ struct TilesShape {
     }
 };
 
-// What the unpacking warps tell the softmax about a tile, and the rest of the block's small things.
+// What the unpacking warps tell the softmax about tiles (two of them), and the block's barriers.
+template <int TILE>
 struct TilesMeta {
-    unsigned long long bars[16];
+    unsigned long long bars[24];
     uint32_t tmem, dead;
-    float largest[2][2][8];        // [tile parity][K, V][warp]
-    int32_t e_k[2], e_v[2];
-    uint32_t runs[2], any_bad[2];
-    uint32_t bad[2][4][4];         // value planes that are not finite: [tile parity][group][32 tokens]
+    uint8_t flags[2][8];           // per unpacking warp: something in `bad`
+    alignas(16) float k_up[2][TILE];           // what a token's logits are multiplied with: its power of two, the scale, log2 e
+    alignas(16) float v_up[2][TILE];           // a token's power of two
+    uint8_t bad[2][TILE];          // bit g: value planes of group g are not finite; bit 7: the token's page is missing
 };
-static_assert(sizeof(TilesMeta) <= 1024, "meta");
 
 __device__ __forceinline__ uint64_t tiles_desc(uint32_t addr, uint32_t leading, uint32_t stride) {     // 128-byte swizzle
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -121,26 +129,41 @@ __device__ __forceinline__ void tiles_unpack(const uint32_t (&w)[BITS / 2], floa
     out[1] = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
+__device__ __forceinline__ void tiles_cp_async(uint32_t dst, const void* src, uint32_t bytes, bool there) {      // 16, 8 or 4 bytes; zeros if not there
+    const uint32_t n = there ? bytes : 0u;
+    if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
 template <int D, int BITS, bool BF16>
 __global__ void __launch_bounds__(TilesShape<D, BITS>::THREADS, 1)
 attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     using S = TilesShape<D, BITS>;
+    using Meta = TilesMeta<S::TILE>;
     constexpr int MT = S::MT, TILE = S::TILE;
     constexpr float kCentre = BITS == 8 ? 128.0f : 8.0f;
+    static_assert(sizeof(Meta) <= S::META, "meta");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;      // the swizzle goes by the address
     uint8_t* smem = smem_raw + (base - (uint32_t)__cvta_generic_to_shared(smem_raw));
-    TilesMeta& meta = *reinterpret_cast<TilesMeta*>(smem + S::OFF_META);
+    Meta& meta = *reinterpret_cast<Meta*>(smem + S::OFF_META);
     const uint32_t bars = base + S::OFF_META;
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
-    // barriers of tile i: buffer i % 2, phase i / 2 % 2
-    auto k_full = [&](uint32_t i) { return bars + (i & 1) * 8; };
-    auto v_full = [&](uint32_t i) { return bars + 16 + (i & 1) * 8; };
-    auto k_free = [&](uint32_t i) { return bars + 32 + (i & 1) * 8; };      // S_i is there
-    auto v_free = [&](uint32_t i) { return bars + 48 + (i & 1) * 8; };      // O holds tile i
+    // Barriers of tile i and the phase in which they are done with it, by the number of their buffers.
+    auto k_full = [&] { return bars; };
+    auto k_free = [&] { return bars + 8; };                                 // K's buffer: the logits of tile i are there
+    auto v_full = [&](uint32_t i) { return bars + 16 + (i % S::V_BUFS) * 8; };
+    auto v_free = [&](uint32_t i) { return bars + 32 + (i % S::V_BUFS) * 8; };
+    auto s_full = [&](uint32_t i) { return bars + 48 + (i & 1) * 8; };
     auto s_free = [&](uint32_t i) { return bars + 64 + (i & 1) * 8; };      // S_i and what is told about tile i have been read
     auto p_full = [&](uint32_t i) { return bars + 80 + (i & 1) * 8; };
-    const uint32_t q_full = bars + 96, all_done = bars + 104;
+    auto o_done = [&](uint32_t i) { return bars + 96 + (i & 1) * 8; };      // O holds tile i, P_i has been read
+    auto told = [&](uint32_t i) { return bars + 128 + (i & 1) * 8; };       // as K_i is, for the softmax: K's own barrier may be past it
+    const uint32_t q_full = bars + 112, all_done = bars + 120;
+    auto one = [](uint32_t i) { return i & 1u; };
+    auto two = [](uint32_t i) { return i >> 1 & 1u; };
+    auto of_v = [](uint32_t i) { return i / S::V_BUFS & 1u; };
     volatile uint32_t* dead = &meta.dead;
     auto wait_lane = [&](uint32_t bar, uint32_t phase) -> bool {
         for (uint32_t round = 0; round < kMbarSpinLimit / 1024; ++round) {
@@ -157,17 +180,18 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     };
     // of a whole warp
     auto wait = [&](uint32_t bar, uint32_t phase) -> bool { return __all_sync(kFullMask, wait_lane(bar, phase)); };
-    auto phase = [](uint32_t i) { return (i >> 1) & 1u; };
-    auto phase_before = [](uint32_t i) { return ((i >> 1) & 1u) ^ 1u; };    // of the buffer's use by tile i - 2
 
     if (tid == 0) {
+        mbar_init(k_full(), S::UNPACK_WARPS);
+        mbar_init(k_free(), 1);
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(k_full(i), S::UNPACK_WARPS);
-            mbar_init(v_full(i), S::UNPACK_WARPS);
-            mbar_init(k_free(i), 1);
-            mbar_init(v_free(i), 1);
+            mbar_init(bars + 16 + i * 8, S::UNPACK_WARPS);
+            mbar_init(bars + 32 + i * 8, 1);
+            mbar_init(s_full(i), 1);
             mbar_init(s_free(i), S::SOFT_WARPS);
             mbar_init(p_full(i), S::SOFT_WARPS);
+            mbar_init(o_done(i), 1);
+            mbar_init(told(i), S::UNPACK_WARPS);
         }
         mbar_init(q_full, S::SOFT_WARPS);
         mbar_init(all_done, 1);
@@ -190,142 +214,193 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
 
     if (warp >= S::SOFT_WARPS && warp < S::WARPS - 1) {
         // ===================== unpacking =====================
+        // A thread's piece j of K (V) is sixteen elements of one token; what it requests lies in places that it alone reads, so a wait for its own
+        // copies is all it takes. While tile i is unpacked, tile i + 1 is requested, by page numbers that were requested a tile before.
         const uint32_t u = tid - S::SOFT_WARPS * kWarp, uw = u / kWarp;
-        uint32_t kr[S::K_EACH][BITS / 2], vr[S::V_EACH][BITS / 2];
-        uint16_t ks[S::K_EACH], kb[S::K_EACH], vs[S::V_EACH], vb[S::V_EACH];
-        uint32_t runs = 0;
-        Cursor<MT, TILE> next = now;
-        // rows of tile `next`, which the pieces of this thread belong to; a piece without one is zeros
-        auto row_of = [&](uint32_t key, bool& there) -> size_t {
-            const uint32_t token = next.token0() + key;
-            int32_t page = -1;
-            if (token < next.range.end) {
-                page = a.table.table[(size_t)next.b * a.table.stride + (token >> a.table.page_log2)];
-                if (page >= 0 && (uint32_t)page >= a.table.pages) page = -1;
-            }
-            there = page >= 0;
-            return there ? (((size_t)page * a.kv_heads + next.head / S::PARTS) << a.table.page_log2) + (token & ((1u << a.table.page_log2) - 1u)) : 0;
+        const uint32_t k_piece = u % S::K_ROW, v_piece = u % S::V_ROW;
+        const uint32_t page_mask = (1u << a.table.page_log2) - 1u;
+        struct Tile { uint32_t token0, end, head; const int32_t* table; };
+        auto tile_of = [&](const Cursor<MT, TILE>& c) { return Tile{c.token0(), c.range.end, c.head, a.table.table + (size_t)c.b * a.table.stride}; };
+        auto k_key = [&](uint32_t j) { return (u + j * S::UNPACK) / S::K_ROW; };
+        auto v_key = [&](uint32_t j) { return (u + j * S::UNPACK) / S::V_ROW; };
+        // places of page numbers: of V for even and odd tiles, of K the same ones or (heads of 512) one
+        auto v_page = [&](uint32_t i, uint32_t j) { return S::OFF_VP + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 4; };
+        auto k_page = [&](uint32_t i, uint32_t j) { return S::SAME ? v_page(i, j) : S::OFF_KP + (j * S::UNPACK + u) * 4; };
+        auto page_at = [&](uint32_t off) { return *reinterpret_cast<const int32_t*>(smem + off); };
+        auto ask_page = [&](const Tile& t, uint32_t key, uint32_t off) {
+            const uint32_t token = t.token0 + key;
+            if (token < t.end) tiles_cp_async(base + off, t.table + (token >> a.table.page_log2), 4, true);
         };
-        auto load_piece = [&](uint32_t (&r)[BITS / 2], uint16_t& s, uint16_t& b, const KvPlanes& p, uint32_t key, uint32_t piece) {
+        // the cache's row of a token (a number below 2^32, as the entry point has checked), and whether there is one
+        auto row_at = [&](const Tile& t, uint32_t key, int32_t page, bool& there) -> uint32_t {
+            const uint32_t token = t.token0 + key;
+            there = token < t.end && page >= 0 && (uint32_t)page < a.table.pages;
+            return there ? (((uint32_t)page * a.kv_heads + t.head / S::PARTS) << a.table.page_log2) + (token & page_mask) : 0u;
+        };
+        // the 32-bit word that holds a group's 16-bit scale (bias), and which half of it
+        auto ask_planes = [&](const KvPlanes& p, uint32_t row, uint32_t grp, bool there, uint32_t off) {
+            const size_t at = ((size_t)row * S::G + grp) & ~(size_t)1;
+            tiles_cp_async(base + off, p.scales + at, 4, there);
+            tiles_cp_async(base + off + 4, p.biases + at, 4, there);
+        };
+        const uint32_t k_half = S::G == 1 ? k_key(0) & 1u : k_piece / 4 & 1u, v_half = S::G == 1 ? v_key(0) & 1u : v_piece / 4 & 1u;
+        auto read_planes = [&](uint32_t off, uint32_t half, float& s, float& b) {        // the bias centred
+            const uint2 w = *reinterpret_cast<const uint2*>(smem + off);
+            s = __uint_as_float(half ? w.x & 0xFFFF0000u : w.x << 16);
+            b = fmaf(kCentre, s, __uint_as_float(half ? w.y & 0xFFFF0000u : w.y << 16));
+        };
+        auto ask_k = [&](const Tile& t, uint32_t i, uint32_t j) {
             bool there;
-            const size_t row = row_of(key, there);
-#pragma unroll
-            for (int j = 0; j < BITS / 2; ++j) r[j] = 0;
-            s = b = 0;
-            if (there) {
-                load_words(r, p.codes + row * S::ROW_BYTES + piece * S::PIECE);
-                s = p.scales[row * S::G + piece / 4];
-                b = p.biases[row * S::G + piece / 4];
+            const uint32_t row = row_at(t, k_key(j), page_at(k_page(i, j)), there);
+            tiles_cp_async(base + S::OFF_KC + (j * S::UNPACK + u) * S::PIECE, a.k.codes + (size_t)row * S::ROW_BYTES + k_piece * S::PIECE, S::PIECE, there);
+            ask_planes(a.k, row, k_piece / 4, there, S::OFF_KS + (j * S::UNPACK + u) * 8);
+        };
+        auto ask_v_planes = [&](const Tile& t, uint32_t i, uint32_t j) {
+            bool there;
+            const uint32_t row = row_at(t, v_key(j), page_at(v_page(i, j)), there);
+            ask_planes(a.v, row, v_piece / 4 + t.head % S::PARTS * S::GV, there, S::OFF_VS + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 8);
+        };
+        auto ask_v = [&](const Tile& t, uint32_t i, uint32_t j) {
+            bool there;
+            const uint32_t row = row_at(t, v_key(j), page_at(v_page(i, j)), there);
+            tiles_cp_async(base + S::OFF_VC + (j * S::UNPACK + u) * S::PIECE, a.v.codes + (size_t)row * S::ROW_BYTES + (v_piece + t.head % S::PARTS * S::V_ROW) * S::PIECE, S::PIECE,
+                           there);
+        };
+        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+        auto landed = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
+        // the largest of a token's lanes
+        auto token_most = [&](float v, int lanes) {
+            for (int off = lanes / 2; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, off));
+            return v;
+        };
+        auto magnitude = [&](float s, float b) { return fmaxf(kCentre * fabsf(s), fabsf(b)); };
+        auto exponent = [&](float most) { return min(max(rows_exponent(most) - 7, -126), 119); };      // both parts of a value below 2^8
+        auto store = [&](uint32_t buffer, const uint32_t (&r)[BITS / 2], float s, float b, uint32_t key, uint32_t piece) {
+            uint4 h[2];
+            tiles_unpack<BITS>(r, s, b, h);
+            // the two chunks in the order in which eight lanes meet eight different banks
+            const uint32_t odd = S::K_ROW >= 8 ? piece / 4 & 1u : 0u, at = buffer + key * 128 + (piece / 4) * (TILE * 128), c0 = (piece % 4 * 2 + odd) ^ (key & 7u);
+            *reinterpret_cast<uint4*>(smem + at + c0 * 16) = odd ? h[1] : h[0];
+            *reinterpret_cast<uint4*>(smem + at + (c0 ^ 1u) * 16) = odd ? h[0] : h[1];
+        };
+        Cursor<MT, TILE> next = now;                           // of the tile that pages are asked for
+        uint32_t left = busy ? (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), stop - item) : 0, ahead = 0;
+        Tile t0 = {}, t1 = {}, t2 = {};                        // tiles i, i + 1, i + 2
+        auto step = [&] {                                      // `next` one tile on, if there is one
+            if (++ahead >= count) return;
+            if (--left == 0) {
+                next.next_unit(a);
+                left = (uint32_t)lesser((uint64_t)next.range.tiles, (uint64_t)(count - ahead));
+            } else {
+                ++next.tile;
             }
         };
-        auto load_k = [&] {
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) load_piece(kr[j], ks[j], kb[j], a.k, (u + j * S::UNPACK) / S::K_ROW, u % S::K_ROW);
-        };
-        auto load_v = [&] {
-#pragma unroll
-            for (int j = 0; j < S::V_EACH; ++j)
-                load_piece(vr[j], vs[j], vb[j], a.v, (u + j * S::UNPACK) / S::V_ROW, u % S::V_ROW + next.head % S::PARTS * S::V_ROW);
-            bool there = false;
-            if (lane < S::RUNS) row_of(lane * 16, there);
-            runs = __ballot_sync(kFullMask, there);
-        };
-        if (count) { load_k(); load_v(); }
-        int e_v = -126;
-        uint32_t segment = busy ? (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), stop - item) : 0;      // tiles left of the unit at hand
+        if (count) {
+            t0 = t1 = tile_of(next);
+            for (int j = 0; j < S::K_EACH; ++j) ask_page(t0, k_key(j), k_page(0, j));
+            if (!S::SAME)
+                for (int j = 0; j < S::V_EACH; ++j) ask_page(t0, v_key(j), v_page(0, j));
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            for (int j = 0; j < S::K_EACH; ++j) ask_k(t0, 0, j);
+            for (int j = 0; j < S::V_EACH; ++j) ask_v_planes(t0, 0, j);
+            step();
+            t1 = tile_of(next);
+            if (count > 1) {
+                for (int j = 0; j < S::K_EACH; ++j) ask_page(t1, k_key(j), k_page(1, j));
+                if (!S::SAME)
+                    for (int j = 0; j < S::V_EACH; ++j) ask_page(t1, v_key(j), v_page(1, j));
+            }
+            commit();
+            for (int j = 0; j < S::V_EACH; ++j) ask_v(t0, 0, j);
+            commit();
+            step();
+            t2 = tile_of(next);
+        }
+        // A wait that runs out is told to all, whose later waits end at once; every warp goes through all tiles.
+#pragma unroll 1
         for (uint32_t i = 0; i < count; ++i) {
-            const uint32_t st = i & 1;
-            // A wait that runs out is told to all, whose later waits end at once: every warp goes through all tiles, since they meet at a barrier in each.
-            if (i >= 2 && wait(k_free(i), phase_before(i))) wait(s_free(i), phase_before(i));
-            // ---- the planes' largest magnitudes ----
-            float most_k = 0.0f, most_v = 0.0f;
-            uint32_t broken = 0;
-            auto measure = [&](uint16_t s16, uint16_t b16, float& most) -> bool {
-                const float s = bf16_bits_to_float(s16), b = fmaf(kCentre, s, bf16_bits_to_float(b16)), mag = fmaxf(kCentre * fabsf(s), fabsf(b));
-                const bool fine = s - s == 0.0f && b - b == 0.0f;
-                if (fine) most = fmaxf(most, mag);
-                return fine;
-            };
+            // ---- K_i, what is told about tile i; K_(i+1) and the planes of V_(i+1) are requested, and the pages of tile i + 2 ----
+            landed();
+            if (i >= 1) wait(k_free(), one(i - 1));
+            if (i >= 2) wait(s_free(i), two(i - 2));
+            uint32_t any = 0;
+#pragma unroll 1
+            for (int j = 0; j < S::V_EACH; ++j) {
+                const uint32_t key = v_key(j), token = t0.token0 + key;
+                float s, b;
+                read_planes(S::OFF_VS + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 8, v_half, s, b);
+                const bool broken = !(s - s == 0.0f && b - b == 0.0f);
+                const float most = token_most(broken ? 0.0f : magnitude(s, b), S::V_ROW);
+                const int32_t page = page_at(v_page(i, j));
+                const bool missing = token < t0.end && !(page >= 0 && (uint32_t)page < a.table.pages);
+                const uint32_t of_token = __ballot_sync(kFullMask, broken) >> (lane / S::V_ROW * S::V_ROW);
+                if (v_piece == 0) {
+                    uint32_t bits = missing ? 0x80u : 0u;
 #pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) measure(ks[j], kb[j], most_k);
-#pragma unroll
-            for (int j = 0; j < S::V_EACH; ++j)
-                if (!measure(vs[j], vb[j], most_v)) broken |= 1u << j;
-            most_k = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(most_k)));
-            most_v = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(most_v)));
-            if (lane == 0) {
-                meta.largest[st][0][uw] = most_k;
-                meta.largest[st][1][uw] = most_v;
-            }
-            if (uw == 0) {
-                if (lane < 16) meta.bad[st][lane / 4][lane % 4] = 0;
-                if (lane == 0) {
-                    meta.any_bad[st] = 0;
-                    meta.runs[st] = runs;
+                    for (int g = 0; g < S::GV; ++g) bits |= (of_token >> (4 * g) & 1u) << g;
+                    meta.v_up[i & 1][key] = rows_power(exponent(most));
+                    meta.bad[i & 1][key] = (uint8_t)bits;
+                    any |= bits;
+                    if (missing) *a.error = kErrKvPage;
                 }
             }
-            asm volatile("bar.sync 1, %0;" ::"n"(S::UNPACK) : "memory");
-            float top_k = 0.0f, top_v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                top_k = fmaxf(top_k, meta.largest[st][0][w]);
-                top_v = fmaxf(top_v, meta.largest[st][1][w]);
+            any = __any_sync(kFullMask, any != 0);
+#pragma unroll 1
+            for (int j = 0; j < S::K_EACH; ++j) {
+                const uint32_t key = k_key(j);
+                uint32_t r[BITS / 2];
+                load_words(r, smem + S::OFF_KC + (j * S::UNPACK + u) * S::PIECE);
+                float s, b;
+                read_planes(S::OFF_KS + (j * S::UNPACK + u) * 8, k_half, s, b);
+                const bool broken = !(s - s == 0.0f && b - b == 0.0f);
+                const int e = exponent(token_most(broken ? 0.0f : magnitude(s, b), S::K_ROW));
+                const float down = rows_power(-e);
+                if (k_piece == 0) meta.k_up[i & 1][key] = rows_power(e) * (a.scale * 1.4426950408889634f);
+                store(S::OFF_K, r, s * down, b * down, key, k_piece);
+                if (i + 1 < count) ask_k(t1, i + 1, j);
             }
-            const int e_k = min(max(rows_exponent(top_k) - 7, -126), 119);           // both parts of a value below 2^8
-            e_v = min(max(e_v, rows_exponent(top_v) - 7), 119);
-            if (u == 0) {
-                meta.e_k[st] = e_k;
-                meta.e_v[st] = e_v;
-            }
-            if (broken) {
-#pragma unroll
-                for (int j = 0; j < S::V_EACH; ++j)
-                    if (broken >> j & 1u) {
-                        const uint32_t key = (u + j * S::UNPACK) / S::V_ROW;
-                        atomicOr(&meta.bad[st][u % S::V_ROW / 4][key / 32], 1u << (key % 32));
-                        meta.any_bad[st] = 1;
-                        vs[j] = vb[j] = 0;
-                    }
-            }
-            // ---- K ----
-            auto store = [&](uint32_t buffer, const uint32_t (&r)[BITS / 2], uint16_t s16, uint16_t b16, float down, uint32_t key, uint32_t piece) {
-                const float s = bf16_bits_to_float(s16);
-                uint4 h[2];
-                tiles_unpack<BITS>(r, s * down, fmaf(kCentre, s, bf16_bits_to_float(b16)) * down, h);
-                // the two chunks in the order in which eight lanes meet eight different banks
-                const uint32_t odd = S::K_ROW >= 8 ? piece / 4 & 1u : 0u, at = buffer + key * 128 + (piece / 4) * (TILE * 128);
-                const uint4 first = odd ? h[1] : h[0], second = odd ? h[0] : h[1];
-                const uint32_t c0 = (piece % 4 * 2 + odd) ^ (key & 7u);
-                *reinterpret_cast<uint4*>(smem + at + c0 * 16) = first;
-                *reinterpret_cast<uint4*>(smem + at + (c0 ^ 1u) * 16) = second;
-            };
-            const float down_k = rows_power(-e_k), down_v = rows_power(-e_v);
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j)
-                store(S::OFF_K + st * S::K_BYTES, kr[j], ks[j], kb[j], down_k, (u + j * S::UNPACK) / S::K_ROW, u % S::K_ROW);
+            if (lane == 0) meta.flags[i & 1][uw] = (uint8_t)any;
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(k_full(i));
-            const bool more = i + 1 < count;
-            if (more) {
-                if (--segment == 0) {
-                    next.next_unit(a);
-                    segment = (uint32_t)lesser((uint64_t)next.range.tiles, (uint64_t)(count - i - 1));
-                } else {
-                    ++next.tile;
-                }
-                load_k();
+            if (lane == 0) {
+                mbar_arrive(k_full());
+                mbar_arrive(told(i));
             }
-            // ---- V ----
-            if (i >= 2) wait(v_free(i), phase_before(i));
-#pragma unroll
-            for (int j = 0; j < S::V_EACH; ++j)
-                store(S::OFF_V + st * S::V_BYTES, vr[j], vs[j], vb[j], down_v, (u + j * S::UNPACK) / S::V_ROW, u % S::V_ROW);
+            if (i + 1 < count) {
+#pragma unroll 1
+                for (int j = 0; j < S::V_EACH; ++j) ask_v_planes(t1, i + 1, j);
+            }
+            if (i + 2 < count) {
+                for (int j = 0; j < S::K_EACH; ++j) ask_page(t2, k_key(j), k_page(i + 2, j));
+                if (!S::SAME)
+                    for (int j = 0; j < S::V_EACH; ++j) ask_page(t2, v_key(j), v_page(i + 2, j));
+            }
+            commit();
+            // ---- V_i; the codes of V_(i+1) are requested ----
+            landed();
+            if (i >= S::V_BUFS) wait(v_free(i), of_v(i - S::V_BUFS));
+#pragma unroll 1
+            for (int j = 0; j < S::V_EACH; ++j) {
+                const uint32_t key = v_key(j);
+                uint32_t r[BITS / 2];
+                load_words(r, smem + S::OFF_VC + (j * S::UNPACK + u) * S::PIECE);
+                float s, b;
+                read_planes(S::OFF_VS + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 8, v_half, s, b);
+                if (!(s - s == 0.0f && b - b == 0.0f)) s = b = 0.0f;
+                const float down = __uint_as_float(0x7F000000u - __float_as_uint(meta.v_up[i & 1][key]));      // the reciprocal of a power of two
+                store(S::OFF_V + (i % S::V_BUFS) * S::V_BYTES, r, s * down, b * down, key, v_piece);
+                if (i + 1 < count) ask_v(t1, i + 1, j);
+            }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(v_full(i));
-            if (more) load_v();
+            commit();
+            t0 = t1;
+            t1 = t2;
+            step();
+            t2 = tile_of(next);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == S::WARPS - 1) {
         // ===================== MMA issuer =====================
         constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(TILE >> 3) << 17) | ((uint32_t)(MT >> 4) << 24);
@@ -333,27 +408,29 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         uint32_t segment = 0, segments = 0;
         bool opens = false;                                    // tile i - 1 is its unit's first here: its product starts O anew
         auto logits = [&](uint32_t i) -> bool {
-            if (!wait(k_full(i), phase(i)) || (i >= 2 && !wait(s_free(i), phase_before(i)))) return false;
+            if (!wait(k_full(), one(i)) || (i >= 2 && !wait(s_free(i), two(i - 2)))) return false;
             tiles_fence_after();
             if (lane == 0) {
-                const uint64_t q0 = tiles_desc(base, 16, 1024), k0 = tiles_desc(base + S::OFF_K + (i & 1) * S::K_BYTES, 16, 1024);
+                const uint64_t q0 = tiles_desc(base, 16, 1024), k0 = tiles_desc(base + S::OFF_K, 16, 1024);
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e)
                     tiles_mma_ss(tmem + S::COL_S + (i & 1) * TILE, q0 + (((e / 4) * (MT * 128) + e % 4 * 32) >> 4), k0 + (((e / 4) * (TILE * 128) + e % 4 * 32) >> 4),
                                  idesc_s, e > 0);
-                tiles_commit(k_free(i));
+                tiles_commit(s_full(i));
+                tiles_commit(k_free());
             }
             __syncwarp();
             return true;
         };
         auto values = [&](uint32_t j) -> bool {
-            if (!wait(p_full(j), phase(j)) || !wait(v_full(j), phase(j))) return false;
+            if (!wait(p_full(j), two(j)) || !wait(v_full(j), of_v(j))) return false;
             tiles_fence_after();
             if (lane == 0) {
-                const uint64_t v0 = tiles_desc(base + S::OFF_V + (j & 1) * S::V_BYTES, TILE * 128, 1024);
+                const uint64_t v0 = tiles_desc(base + S::OFF_V + (j % S::V_BUFS) * S::V_BYTES, TILE * 128, 1024);
 #pragma unroll
                 for (int e = 0; e < TILE / 16; ++e)
                     tiles_mma_ts(tmem + S::COL_O, tmem + S::COL_P + (j & 1) * (TILE / 2) + e * 8, v0 + (e * 2048 >> 4), idesc_o, e > 0 || !opens);
+                tiles_commit(o_done(j));
                 tiles_commit(v_free(j));
             }
             __syncwarp();
@@ -405,7 +482,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             most = max(most & 0xFFFFu, most >> 16);
             const float q_top = BF16 ? bf16_bits_to_float((uint16_t)most) : f16_bits_to_float((uint16_t)most);
             const int e_q = q_top > 0.0f && q_top <= 3.402823466e38f ? max(rows_exponent(q_top), -126) : 0;      // the largest element to [1, 2)
-            const float down = rows_power(-e_q), factor = rows_power(e_q) * a.scale * 1.4426950408889634f;
+            const float down = rows_power(-e_q), q_up = rows_power(e_q);
 #pragma unroll 2
             for (int c = 0; c < D / 8; ++c) {
                 const uint4 v = is ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
@@ -430,87 +507,142 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 low = (uint32_t)max((int64_t)0, lesser(pos - (int64_t)a.window + 1, (int64_t)kMostTokens));
             }
             const uint32_t low_most = __reduce_max_sync(kFullMask, low), open_end = lesser(now.seq.context, now.range.end);
-            float m = -INFINITY, l = 0.0f;
-            int e_o = -126;                                    // exponent of what O holds
+            float m = -INFINITY, l = 0.0f;                     // l and O: in units of 2^(m + E)
+            int e_o = -126;
             uint32_t poison = 0;                               // groups that are not a number
-            const uint32_t stop_i = i + segment;
+            const uint32_t begin_i = i, stop_i = i + segment;
             uint32_t token0 = now.token0();
+#pragma unroll 1
             for (; i < stop_i; ++i, token0 += TILE) {
                 const uint32_t st = i & 1;
-                ok = wait(k_free(i), phase(i)) && wait(k_full(i), phase(i));         // S_i; what is told about the tile
+                ok = wait(s_full(i), two(i)) && wait(told(i), two(i));
                 if (!ok) break;
                 tiles_fence_after();
-                const int e_k = meta.e_k[st], e_v = meta.e_v[st];
-                const uint32_t runs = meta.runs[st], any_bad = meta.any_bad[st];
-                const float f = factor * rows_power(e_k);
-                // ---- what the row sees ----
-                const bool open = runs == (1u << S::RUNS) - 1u && token0 >= low_most && token0 + TILE <= open_end;
-                uint32_t seen[TILE / 32];
-#pragma unroll
-                for (int w = 0; w < TILE / 32; ++w) seen[w] = 0xFFFFFFFFu;
-                if (!open) {
-#pragma unroll
-                    for (int w = 0; w < TILE / 32; ++w) {
-                        const uint32_t t0 = token0 + 32 * w;
-                        auto below = [&](uint32_t end) { return end <= t0 ? 0u : end - t0 >= 32 ? 0xFFFFFFFFu : (1u << (end - t0)) - 1u; };      // tokens before `end`
-                        uint32_t see = below(open_end) & ~below(low);
-                        const uint32_t drafted = below(now.range.end) & ~below(now.seq.context);
-                        if (drafted) {
-                            const uint32_t shift = t0 < now.seq.context ? now.seq.context - t0 : 0, j = t0 + shift - now.seq.context;      // row j at bit `shift`
-                            if (a.mask) {
-                                const unsigned long long* bits = a.mask + (size_t)(now.seq.row0 + node) * a.mask_words;
-                                const uint32_t word = j >> 6, off = j & 63u;
-                                unsigned long long b = word < a.mask_words ? bits[word] >> off : 0ull;
-                                if (off && word + 1 < a.mask_words) b |= bits[word + 1] << (64 - off);
-                                see |= (uint32_t)b << shift & drafted;
-                            } else {
-                                uint32_t chain = below(now.seq.context + node + 1);
-                                if (a.window && node + 1 > a.window) chain &= ~below(now.seq.context + node + 1 - a.window);
-                                see |= chain & drafted;
-                            }
+                const uint2 flags = *reinterpret_cast<const uint2*>(meta.flags[st]);
+                const bool odd = (flags.x | flags.y) != 0;
+                const bool open = !odd && token0 >= low_most && token0 + TILE <= open_end;
+                // the tokens of chunk w that the row sees
+                auto see = [&](int w) -> uint32_t {
+                    const uint32_t t0 = token0 + 32 * w;
+                    auto below = [&](uint32_t end) { return end <= t0 ? 0u : end - t0 >= 32 ? 0xFFFFFFFFu : (1u << (end - t0)) - 1u; };      // tokens before `end`
+                    uint32_t seen = below(open_end) & ~below(low);
+                    const uint32_t drafted = below(now.range.end) & ~below(now.seq.context);
+                    if (drafted) {
+                        const uint32_t shift = t0 < now.seq.context ? now.seq.context - t0 : 0, j = t0 + shift - now.seq.context;      // row j at bit `shift`
+                        if (a.mask) {
+                            const unsigned long long* bits = a.mask + (size_t)(now.seq.row0 + node) * a.mask_words;
+                            const uint32_t word = j >> 6, off = j & 63u;
+                            unsigned long long b = word < a.mask_words ? bits[word] >> off : 0ull;
+                            if (off && word + 1 < a.mask_words) b |= bits[word + 1] << (64 - off);
+                            seen |= (uint32_t)b << shift & drafted;
+                        } else {
+                            uint32_t chain = below(now.seq.context + node + 1);
+                            if (a.window && node + 1 > a.window) chain &= ~below(now.seq.context + node + 1 - a.window);
+                            seen |= chain & drafted;
                         }
-                        if (!(runs >> (2 * w) & 1u)) see &= 0xFFFF0000u;
-                        if (!(runs >> (2 * w + 1) & 1u)) see &= 0x0000FFFFu;
-                        seen[w] = is ? see : 0u;
                     }
-                    if (tid == 0) {
-                        const uint32_t held = token0 >= now.range.end ? 0u : lesser((now.range.end - token0 + 15) / 16, (uint32_t)S::RUNS);
-                        if (runs != (1u << held) - 1u) *a.error = kErrKvPage;
-                    }
-                }
-                // the logits of 32 tokens, in base 2
+                    if (odd)
+                        for (int j = 0; j < 32; ++j)
+                            if (meta.bad[st][32 * w + j] & 0x80u) seen &= ~(1u << j);
+                    return is ? seen : 0u;
+                };
+                // the logits of 32 tokens, in base 2 but for the row's power of two
                 auto load_logits = [&](int w, float (&x)[32]) {
                     uint32_t raw[32];
                     tiles_ld32(lanes + S::COL_S + st * TILE + w * 32, raw);
                     tiles_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(raw[j]) * f;
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 up = *reinterpret_cast<const float4*>(&meta.k_up[st][32 * w + j]);
+                        x[j] = __uint_as_float(raw[j]) * up.x;
+                        x[j + 1] = __uint_as_float(raw[j + 1]) * up.y;
+                        x[j + 2] = __uint_as_float(raw[j + 2]) * up.z;
+                        x[j + 3] = __uint_as_float(raw[j + 3]) * up.w;
+                    }
                     if (!open) {
+                        const uint32_t seen = see(w);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] = seen[w] >> j & 1u ? x[j] : -INFINITY;
+                        for (int j = 0; j < 32; ++j) x[j] = seen >> j & 1u ? x[j] : -INFINITY;
                     }
                 };
                 // ---- maximum ----
                 float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
                 for (int w = 0; w < TILE / 32; ++w) {
                     float x[32];
                     load_logits(w, x);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
                 }
+                top *= q_up;
                 float alpha = 1.0f;
                 if (top > m + 8.0f) {
                     alpha = rows_exp2(m - top);                // m = -inf: zero
                     m = top;
                 }
-                l *= alpha;
-                alpha *= rows_power(e_o - e_v);
-                e_o = e_v;
-                const float shift = m == -INFINITY ? 0.0f : m;
-                // ---- O, when a maximum or the exponent moved ----
-                if (i > stop_i - segment && __any_sync(kFullMask, alpha != 1.0f)) {
-                    ok = wait(v_free(i - 1), phase(i - 1));
+                // ---- probabilities, two to a column ----
+                if (i >= 2) {
+                    ok = wait(o_done(i), two(i - 2));          // P's buffer has been read
+                    if (!ok) break;
+                }
+                float sum;
+                for (int round = 0;; ++round) {
+                    const float shift = (m == -INFINITY ? 0.0f : m) + (float)e_o;
+                    float heavy = 0.0f;
+                    sum = 0.0f;
+#pragma unroll 1
+                    for (int w = 0; w < TILE / 32; ++w) {
+                        float x[32];
+                        uint32_t p[16];
+                        load_logits(w, x);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 up = *reinterpret_cast<const float4*>(&meta.v_up[st][32 * w + j]);
+                            const float p0 = rows_exp2(fmaf(x[j], q_up, -shift)), p1 = rows_exp2(fmaf(x[j + 1], q_up, -shift));
+                            const float p2 = rows_exp2(fmaf(x[j + 2], q_up, -shift)), p3 = rows_exp2(fmaf(x[j + 3], q_up, -shift));
+                            sum += (p0 + p1) + (p2 + p3);
+                            const float v0 = p0 * up.x, v1 = p1 * up.y, v2 = p2 * up.z, v3 = p3 * up.w;
+                            heavy = fmaxf(fmaxf(heavy, fmaxf(v0, v1)), fmaxf(v2, v3));
+                            p[j / 2] = rows_half2(v0, v1);
+                            p[j / 2 + 1] = rows_half2(v2, v3);
+                        }
+                        tiles_st16(lanes + S::COL_P + st * (TILE / 2) + w * 16, p);
+                        if (odd) {
+                            // a row that gives a token weight whose planes are not finite in a group becomes NaN there
+#pragma unroll 1
+                            for (int j = 0; j < 32; ++j) {
+                                const uint32_t bad = meta.bad[st][32 * w + j] & 0x7Fu;
+                                if (bad && (see(w) >> j & 1u)) {
+                                    float z = 0.0f;
+#pragma unroll
+                                    for (int k = 0; k < 32; ++k) z = k == j ? x[k] : z;
+                                    if (rows_exp2(fmaf(z, q_up, -shift)) > 0.0f) poison |= bad;
+                                }
+                            }
+                        }
+                    }
+                    if (!__any_sync(kFullMask, heavy > 16384.0f) || round == 2) break;
+                    tiles_wait_st();                           // the next round stores to the same columns
+                    // E of the rows that have outgrown it: their largest p' to below 16, by what it is when nothing is divided
+                    float most = 0.0f;
+                    const float plain = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+                    for (int w = 0; w < TILE / 32; ++w) {
+                        float x[32];
+                        load_logits(w, x);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) most = fmaxf(most, rows_exp2(fmaf(x[j], q_up, -plain)) * meta.v_up[st][32 * w + j]);
+                    }
+                    if (heavy > 16384.0f) {
+                        const int e_new = min(max(e_o, rows_exponent(most) - 3), 119);
+                        alpha *= rows_power(e_o - e_new);
+                        e_o = e_new;
+                    }
+                }
+                l = fmaf(l, alpha, sum);
+                // ---- O, when m or E moved ----
+                if (i > begin_i && __any_sync(kFullMask, alpha != 1.0f)) {
+                    ok = wait(o_done(i - 1), two(i - 1));
                     if (!ok) break;
                     tiles_fence_after();
 #pragma unroll 1
@@ -522,36 +654,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                         for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
                         tiles_st32(lanes + S::COL_O + c, o);
                     }
-                    tiles_wait_st();
                 }
-                // ---- probabilities, at most 2^8, two to a column ----
-                if (i >= 2) {
-                    ok = wait(v_free(i), phase_before(i));     // P's buffer has been read
-                    if (!ok) break;
-                }
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < TILE / 32; ++w) {
-                    float x[32];
-                    uint32_t p[16];
-                    load_logits(w, x);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float p0 = rows_exp2(x[2 * j] - shift), p1 = rows_exp2(x[2 * j + 1] - shift);
-                        sum += p0 + p1;
-                        p[j] = rows_half2(p0, p1);
-                    }
-                    tiles_st16(lanes + S::COL_P + st * (TILE / 2) + w * 16, p);
-                    if (any_bad) {
-                        // a row that gives a token weight whose planes are not finite in a group becomes NaN there
-                        uint32_t live = 0;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) live |= (p[j] & 0x7FFFu ? 1u : 0u) << (2 * j) | (p[j] & 0x7FFF0000u ? 2u : 0u) << (2 * j);
-#pragma unroll
-                        for (int g = 0; g < S::GV; ++g) poison |= live & meta.bad[st][g][w] ? 1u << g : 0u;
-                    }
-                }
-                l += sum;
                 tiles_wait_st();
                 tiles_fence_before();
                 __syncwarp();
@@ -562,14 +665,14 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             }
             if (!ok) break;
             // ---- the segment's result ----
-            if (!wait(v_free(i - 1), phase(i - 1))) break;
+            if (!wait(o_done(i - 1), two(i - 1))) break;
             tiles_fence_after();
             float* part = a.partial + (size_t)(2 * blockIdx.x + (from_start ? 1 : 0)) * MT * (S::DV + 2);
             if (!whole && is) {
-                part[r] = m;
+                part[r] = m + (float)e_o;
                 part[MT + r] = l;
             }
-            const float up = rows_power(e_o), inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) * up : up;
+            const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
             uint16_t* dst = a.out + (size_t)(now.seq.row0 + node) * a.out_stride + (size_t)(head * a.group + flat % a.group) * D + now.head % S::PARTS * S::DV;
             float* pdst = part + 2 * MT + (size_t)r * S::DV;
 #pragma unroll 1
@@ -597,7 +700,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             tiles_fence_before();
             if (!whole && from_start && tid == 0) {
                 ShareInfo& info = a.info[blockIdx.x];
-                info.last = shares.of(item + stop_i - 1 + (now.range.tiles - segment));
+                info.last = shares.of(item + begin_i + now.range.tiles - 1);
                 info.row0 = now.seq.row0;
                 info.flat0 = now.flat0;
                 info.valid = valid;
