@@ -152,7 +152,7 @@ static void tile_places() {
             }
     }
     // every piece of a tile belongs to one thread's turn
-    CHECK(S::UNPACK % S::K_ROW == 0 && S::UNPACK % S::V_ROW == 0);
+    CHECK(S::UNPACK % S::K_ROW == 0 && S::UNPACK % S::V_ROW == 0 && sizeof(TilesMeta<S::TILE, S::UNPACK_WARPS>) <= S::META);
     CHECK(S::OFF_K % 1024 == 0 && S::OFF_V % 1024 == 0 && S::OFF_META % 16 == 0 && S::K_BYTES % 1024 == 0 && S::V_BYTES % 1024 == 0 && S::SMEM <= 227 * 1024);
 }
 template <int D, int BITS, int RB>

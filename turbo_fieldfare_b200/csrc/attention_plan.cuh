@@ -131,10 +131,11 @@ struct Shares {
         const uint64_t longer = (each + 1) * more;
         return (uint32_t)(tile < longer ? divide(tile, each + 1) : more + divide(tile - longer, each));
     }
-    // 64-bit division takes four times as long as this for numbers of 32 bits
+    // A 32-bit division where the numbers are (a 64-bit one takes four times as long); the other is kept out of line.
     static __host__ __device__ __forceinline__ uint64_t divide(uint64_t a, uint64_t b) {
-        return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
+        return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : divide_wide(a, b);
     }
+    static __host__ __device__ __noinline__ uint64_t divide_wide(uint64_t a, uint64_t b) { return a / b; }
 };
 
 // The place `left` tiles into a sequence's tiles, of which there are more: kv head, first row of the unit, tile of the unit.

@@ -244,39 +244,31 @@ __device__ __noinline__ void rows_join(const AttnArgs& a, uint32_t row0, uint32_
     }
 }
 
-// A worker's share, found by a whole warp that goes over the sequences 32 at a time. False: there are fewer tiles than workers.
+// A worker's share, found by a whole warp that goes over the sequences 32 at a time, first for the total, then for the place. False: there are fewer
+// tiles than workers. One body for both turns: what a block runs once costs what it takes to fetch its instructions.
 template <int MT, int TILE>
 __device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t worker, uint32_t workers_most, int lane, bool report, Cursor<MT, TILE>& now, Shares& shares,
                                            uint64_t& item, uint64_t& stop) {
-    auto tiles_of = [&](uint32_t b, Sequence& s, bool tell) -> uint64_t {
-        if (b >= a.sequences) return 0;
-        s.load(a, b, tell);
-        return sequence_tiles<MT, TILE>(a, s) * a.kv_heads * a.head_parts;
-    };
-    uint64_t total = 0;
-#pragma unroll 4
-    for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWarp) {
-        Sequence s;
-        total += tiles_of(b0 + lane, s, report);
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(kFullMask, total, off);
-    shares.set(total, workers_most);
-    if (worker >= shares.workers) return false;
-    item = shares.begin(worker);
-    stop = shares.begin(worker + 1);
+    shares.total = 0;
+    item = stop = 0;
     uint64_t before = 0;
-    for (uint32_t b0 = 0;; b0 += kWarp) {                      // ends: item is below the total
+    bool placing = false;
+#pragma unroll 1
+    for (uint32_t b0 = 0;;) {
         Sequence s = {};
-        const uint64_t mine = tiles_of(b0 + lane, s, false);
+        uint64_t mine = 0;
+        if (b0 + lane < a.sequences) {
+            s.load(a, b0 + lane, report && !placing);
+            mine = sequence_tiles<MT, TILE>(a, s) * a.kv_heads * a.head_parts;
+        }
         uint64_t upto = mine;
-#pragma unroll
+#pragma unroll 1
         for (int off = 1; off < kWarp; off <<= 1) {
             const uint64_t o = __shfl_up_sync(kFullMask, upto, off);
             if (lane >= off) upto += o;
         }
         const uint64_t all = __shfl_sync(kFullMask, upto, kWarp - 1);
-        if (item < before + all) {
+        if (placing && item < before + all) {
             const int owner = __ffs(__ballot_sync(kFullMask, before + upto > item)) - 1;
             const uint64_t left = item - before - __shfl_sync(kFullMask, upto - mine, owner);
             now.b = b0 + owner;
@@ -286,12 +278,21 @@ __device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t worker, u
             uint32_t place[3];
             place_in_sequence<MT, TILE>(a, now.seq, left, place);
             now.head = place[0]; now.flat0 = place[1]; now.tile = place[2];
-            break;
+            now.range.set(a, now.seq, now.flat0, MT, TILE);
+            return true;
         }
         before += all;
+        b0 += kWarp;
+        if (b0 >= a.sequences) {                               // the second time this is not reached: item is below the total
+            shares.set(before, workers_most);
+            if (worker >= shares.workers) return false;
+            item = shares.begin(worker);
+            stop = shares.begin(worker + 1);
+            before = 0;
+            b0 = 0;
+            placing = true;
+        }
     }
-    now.range.set(a, now.seq, now.flat0, MT, TILE);
-    return true;
 }
 
 template <int RB>

@@ -3,7 +3,7 @@
 // With this many rows the products bound it, 4 * 128 * D FLOP per token and unit, next to the unpacking, which a unit pays once for its 128 rows.
 // One persistent block per SM; 8 warps unpack, one issues the MMAs, 4 do the softmax, a thread per row. For tile i of TILE tokens:
 //   unpack:  codes and planes, by cp.async a tile ahead into places of the thread's own -> K_i, V_i in fp16, [64 elements][token][128 bytes] with the
-//            128-byte swizzle (K in one buffer: it is free again when its logits are there, long before the next ones are wanted)
+//            128-byte swizzle (K in two buffers but for heads of 512, V in one: V_(i+1) is unpacked behind K_(i+2), while O takes V_i)
 //   MMA:     S_i = Q K_i^T into tensor memory (two buffers), then O += P_(i-1) V_(i-1); K is K-major, V, as it lies, MN-major
 //   softmax: S_i -> registers -> mask, 2^(x - m), P_i as fp16 into tensor memory (the A operand of the second product)
 // The loops are rolled where registers allow it: three kinds of warps share an SM's instruction caches, and straight-line code of all of them
@@ -22,23 +22,24 @@
 namespace tf {
 
 constexpr uint32_t kErrAttentionWait = 0x7F000053u;           // a bounded wait of attention_tiles_kernel ran out
+constexpr uint32_t kLooks = 1u << 18;                         // looks of a bounded wait
 
 template <int D, int BITS>
 struct TilesShape {
     static constexpr int MT = 128, TILE = D == 512 ? 32 : D == 256 ? 64 : 128, DV = D < 256 ? D : 256, PARTS = D / DV, G = D / 64, GV = DV / 64;
-    static constexpr int SOFT_WARPS = 4, UNPACK_WARPS = 8, WARPS = SOFT_WARPS + UNPACK_WARPS + 1, THREADS = WARPS * kWarp, UNPACK = UNPACK_WARPS * kWarp;
+    static constexpr int SOFT_WARPS = 8, UNPACK_WARPS = 8, WARPS = SOFT_WARPS + UNPACK_WARPS + 1, THREADS = WARPS * kWarp, UNPACK = UNPACK_WARPS * kWarp;
     static constexpr int ROW_BYTES = D * BITS / 8, PIECE = 2 * BITS;          // bytes of 16 codes
     static constexpr int K_ROW = D / 16, V_ROW = DV / 16;                     // pieces of a token
     static constexpr int K_EACH = TILE * K_ROW / UNPACK, V_EACH = TILE * V_ROW / UNPACK;
-    static constexpr int V_BUFS = D == 512 ? 1 : 2;
-    static constexpr bool SAME = K_ROW == V_ROW;                              // a thread's pieces of K and V are of the same tokens
+    static constexpr int K_BUFS = D == 512 ? 1 : 2;
     static constexpr int Q_BYTES = MT * D * 2, K_BYTES = TILE * D * 2, V_BYTES = TILE * DV * 2;
-    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + K_BYTES;
-    // what the unpacking threads have requested, [piece][thread]: codes; (scale, bias) words, of V for two tiles; pages of the next tiles
-    static constexpr int OFF_KC = OFF_V + V_BUFS * V_BYTES, OFF_VC = OFF_KC + K_EACH * UNPACK * PIECE, OFF_KS = OFF_VC + V_EACH * UNPACK * PIECE,
-                         OFF_VS = OFF_KS + K_EACH * UNPACK * 8, OFF_KP = OFF_VS + 2 * V_EACH * UNPACK * 8, OFF_VP = SAME ? OFF_KP : OFF_KP + K_EACH * UNPACK * 4,
-                         OFF_META = OFF_VP + 2 * V_EACH * UNPACK * 4;
-    static constexpr int META = (256 + 2 * TILE * 9 + 127) / 128 * 128, SMEM = OFF_META + META + 1024;
+    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + K_BUFS * K_BYTES;
+    static constexpr int CHUNK = TILE / 2 < 32 ? TILE / 2 : 32;                // logits that a softmax thread has in registers at a time, of its half of a tile
+    // what the unpacking warps have requested: codes [piece][thread]; planes of four tiles [token][4]; pages of two
+    static constexpr int PLANES = 2 * G < 4 ? 4 : 2 * G;                      // bytes of a token's plane, or of two tokens' with one group
+    static constexpr int OFF_KC = OFF_V + V_BYTES, OFF_VC = OFF_KC + K_EACH * UNPACK * PIECE, OFF_PL = OFF_VC + V_EACH * UNPACK * PIECE,
+                         OFF_PG = OFF_PL + 4 * TILE * 4 * PLANES, OFF_META = OFF_PG + 2 * TILE * 4;
+    static constexpr int META = (512 + 4 * UNPACK_WARPS * 5 + 4 * TILE * 9 + TILE + 127) / 128 * 128 + 2 * MT * 8 + MT * 4, SMEM = OFF_META + META + 1024;
     // tensor memory, in columns
     static constexpr int COL_S = 0, COL_P = 2 * TILE, COL_O = 3 * TILE, COLS = 512;
     static_assert(COL_O + DV <= COLS && SMEM <= 227 * 1024 && K_EACH * UNPACK == TILE * K_ROW && V_EACH * UNPACK == TILE * V_ROW, "sizes");
@@ -48,15 +49,19 @@ struct TilesShape {
     }
 };
 
-// What the unpacking warps tell the softmax about tiles (two of them), and the block's barriers.
-template <int TILE>
+// What the unpacking warps tell the softmax about tiles (four of them), and the block's barriers.
+template <int TILE, int WARPS>
 struct TilesMeta {
-    unsigned long long bars[24];
+    unsigned long long bars[14];
     uint32_t tmem, dead;
-    uint8_t flags[2][8];           // per unpacking warp: something in `bad`
-    alignas(16) float k_up[2][TILE];           // what a token's logits are multiplied with: its power of two, the scale, log2 e
-    alignas(16) float v_up[2][TILE];           // a token's power of two
-    uint8_t bad[2][TILE];          // bit g: value planes of group g are not finite; bit 7: the token's page is missing
+    alignas(16) uint8_t flags[4][WARPS];      // per unpacking warp: something in `bad`
+    alignas(16) float v_most[4][WARPS];       // per unpacking warp: the largest of v_up
+    alignas(16) float k_up[4][TILE];          // what a token's logits are multiplied with: its power of two, the scale, log2 e
+    alignas(16) float v_up[4][TILE];          // a token's power of two
+    uint8_t bad[4][TILE];          // bit g: value planes of group g are not finite; bit 7: the token's page is missing
+    int8_t e_k[TILE];              // exponent of the power of two of K, where it is not zero for all of a warp's
+    float pair[2][128][2];         // between the two softmax threads of a row, by turns
+    float q_up[128];               // a row's power of two
 };
 
 __device__ __forceinline__ uint64_t tiles_desc(uint32_t addr, uint32_t leading, uint32_t stride) {     // 128-byte swizzle
@@ -73,7 +78,7 @@ __device__ __forceinline__ void tiles_mma_ts(uint32_t d, uint32_t a, uint64_t b,
 __device__ __forceinline__ void tiles_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void tiles_ld32(uint32_t addr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tiles_ld(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
                  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
@@ -81,17 +86,26 @@ __device__ __forceinline__ void tiles_ld32(uint32_t addr, uint32_t (&r)[32]) {
                    "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tiles_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tiles_st(uint32_t addr, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
                  "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
                  ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
                    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
-__device__ __forceinline__ void tiles_st16(uint32_t addr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tiles_st(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
                    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tiles_ld(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tiles_st(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tiles_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tiles_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -136,11 +150,14 @@ __device__ __forceinline__ void tiles_cp_async(uint32_t dst, const void* src, ui
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
+template <int MT, int TILE>
+__device__ __noinline__ void tiles_next_unit(const AttnArgs& a, Cursor<MT, TILE>& c) { c.next_unit(a); }
+
 template <int D, int BITS, bool BF16>
 __global__ void __launch_bounds__(TilesShape<D, BITS>::THREADS, 1)
 attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     using S = TilesShape<D, BITS>;
-    using Meta = TilesMeta<S::TILE>;
+    using Meta = TilesMeta<S::TILE, S::UNPACK_WARPS>;
     constexpr int MT = S::MT, TILE = S::TILE;
     constexpr float kCentre = BITS == 8 ? 128.0f : 8.0f;
     static_assert(sizeof(Meta) <= S::META, "meta");
@@ -150,28 +167,26 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     Meta& meta = *reinterpret_cast<Meta*>(smem + S::OFF_META);
     const uint32_t bars = base + S::OFF_META;
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
-    // Barriers of tile i and the phase in which they are done with it, by the number of their buffers.
-    auto k_full = [&] { return bars; };
-    auto k_free = [&] { return bars + 8; };                                 // K's buffer: the logits of tile i are there
-    auto v_full = [&](uint32_t i) { return bars + 16 + (i % S::V_BUFS) * 8; };
-    auto v_free = [&](uint32_t i) { return bars + 32 + (i % S::V_BUFS) * 8; };
-    auto s_full = [&](uint32_t i) { return bars + 48 + (i & 1) * 8; };
-    auto s_free = [&](uint32_t i) { return bars + 64 + (i & 1) * 8; };      // S_i and what is told about tile i have been read
-    auto p_full = [&](uint32_t i) { return bars + 80 + (i & 1) * 8; };
-    auto o_done = [&](uint32_t i) { return bars + 96 + (i & 1) * 8; };      // O holds tile i, P_i has been read
-    auto told = [&](uint32_t i) { return bars + 128 + (i & 1) * 8; };       // as K_i is, for the softmax: K's own barrier may be past it
-    const uint32_t q_full = bars + 112, all_done = bars + 120;
+    // Barriers of tile i and the phase in which they are done with it, by the number of their buffers. The issuer's order makes one stand for others:
+    // a commit counts all MMAs before it, so S_i there (s_full, k_free) means that O holds tile i - 2, and that the softmax had left
+    // tile i - 2 (its probabilities were waited for).
+    auto k_full = [&](uint32_t i) { return bars + (i % S::K_BUFS) * 8; };
+    auto k_free = [&](uint32_t i) { return bars + 16 + (i % S::K_BUFS) * 8; };       // K's buffer: the logits of tile i are there
+    auto s_full = [&](uint32_t i) { return bars + 32 + (i & 1) * 8; };      // S_i, and by an arrival of the issuer what it saw: what is told about tile i
+    auto p_full = [&](uint32_t i) { return bars + 48 + (i & 1) * 8; };      // P_i; S_i has been read, and what was told
+    auto o_done = [&](uint32_t i) { return bars + 64 + (i & 1) * 8; };      // O holds tile i
+    const uint32_t q_full = bars + 80, all_done = bars + 88, v_full = bars + 96;
     auto one = [](uint32_t i) { return i & 1u; };
     auto two = [](uint32_t i) { return i >> 1 & 1u; };
-    auto of_v = [](uint32_t i) { return i / S::V_BUFS & 1u; };
+    auto of_k = [](uint32_t i) { return i / S::K_BUFS & 1u; };
     volatile uint32_t* dead = &meta.dead;
     auto wait_lane = [&](uint32_t bar, uint32_t phase) -> bool {
-        for (uint32_t round = 0; round < kMbarSpinLimit / 1024; ++round) {
-            for (uint32_t i = 0; i < 1024; ++i) {
-                uint32_t ok;
-                asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(phase) : "memory");
-                if (ok) return true;
-            }
+        // a look sleeps until the phase is complete, 10 us at the most: warps that wait leave the issue slots to the others
+        for (uint32_t look = 0; look < kLooks; ++look) {
+            uint32_t ok;
+            asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+                         : "=r"(ok) : "r"(bar), "r"(phase), "r"(10000u) : "memory");
+            if (ok) return true;
             if (*dead) return false;
         }
         *dead = 1;
@@ -182,16 +197,13 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     auto wait = [&](uint32_t bar, uint32_t phase) -> bool { return __all_sync(kFullMask, wait_lane(bar, phase)); };
 
     if (tid == 0) {
-        mbar_init(k_full(), S::UNPACK_WARPS);
-        mbar_init(k_free(), 1);
+        mbar_init(v_full, S::UNPACK_WARPS);
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(bars + 16 + i * 8, S::UNPACK_WARPS);
-            mbar_init(bars + 32 + i * 8, 1);
-            mbar_init(s_full(i), 1);
-            mbar_init(s_free(i), S::SOFT_WARPS);
+            mbar_init(bars + i * 8, S::UNPACK_WARPS);
+            mbar_init(bars + 16 + i * 8, 1);
+            mbar_init(s_full(i), 2);
             mbar_init(p_full(i), S::SOFT_WARPS);
             mbar_init(o_done(i), 1);
-            mbar_init(told(i), S::UNPACK_WARPS);
         }
         mbar_init(q_full, S::SOFT_WARPS);
         mbar_init(all_done, 1);
@@ -214,74 +226,90 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
 
     if (warp >= S::SOFT_WARPS && warp < S::WARPS - 1) {
         // ===================== unpacking =====================
-        // A thread's piece j of K (V) is sixteen elements of one token; what it requests lies in places that it alone reads, so a wait for its own
-        // copies is all it takes. While tile i is unpacked, tile i + 1 is requested, by page numbers that were requested a tile before.
+        // A thread's piece j of K (V) is sixteen elements of one token. All pieces of a token belong to one warp, which requests what it unpacks a tile
+        // ahead: codes to places of the thread's own, planes and page numbers to places of the token's; a wait for its own copies and a
+        // __syncwarp is all it takes. What lies behind the sequence, or has no page, is zeros.
         const uint32_t u = tid - S::SOFT_WARPS * kWarp, uw = u / kWarp;
-        const uint32_t k_piece = u % S::K_ROW, v_piece = u % S::V_ROW;
-        const uint32_t page_mask = (1u << a.table.page_log2) - 1u;
+        constexpr uint32_t kKeys = S::UNPACK / S::K_ROW;       // tokens between a thread's pieces of K
+        const uint32_t k_piece = u % S::K_ROW, v_piece = u % S::V_ROW, k_key0 = u / S::K_ROW;
+        // heads of 512 have two tokens of V to a warp and piece: those of its pieces 2 j and 2 j + 1 of K
+        const uint32_t v_key0 = D == 512 ? uw + (lane / 16) * 8 : k_key0;
+        constexpr uint32_t kVKeys = D == 512 ? 16 : kKeys;
+        const uint32_t page_mask = (1u << a.table.page_log2) - 1u, page_log2 = a.table.page_log2;
         struct Tile { uint32_t token0, end, head; const int32_t* table; };
         auto tile_of = [&](const Cursor<MT, TILE>& c) { return Tile{c.token0(), c.range.end, c.head, a.table.table + (size_t)c.b * a.table.stride}; };
-        auto k_key = [&](uint32_t j) { return (u + j * S::UNPACK) / S::K_ROW; };
-        auto v_key = [&](uint32_t j) { return (u + j * S::UNPACK) / S::V_ROW; };
-        // places of page numbers: of V for even and odd tiles, of K the same ones or (heads of 512) one
-        auto v_page = [&](uint32_t i, uint32_t j) { return S::OFF_VP + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 4; };
-        auto k_page = [&](uint32_t i, uint32_t j) { return S::SAME ? v_page(i, j) : S::OFF_KP + (j * S::UNPACK + u) * 4; };
-        auto page_at = [&](uint32_t off) { return *reinterpret_cast<const int32_t*>(smem + off); };
-        auto ask_page = [&](const Tile& t, uint32_t key, uint32_t off) {
-            const uint32_t token = t.token0 + key;
-            if (token < t.end) tiles_cp_async(base + off, t.table + (token >> a.table.page_log2), 4, true);
+        auto page_place = [&](uint32_t i, uint32_t key) { return S::OFF_PG + ((i & 1) * TILE + key) * 4; };
+        auto plane_place = [&](uint32_t i, uint32_t key) { return S::OFF_PL + ((i & 3) * TILE + key) * (4 * S::PLANES); };
+        auto ask_pages = [&](const Tile& t, uint32_t i) {
+#pragma unroll
+            for (int j = 0; j < S::K_EACH; ++j) {
+                const uint32_t key = k_key0 + j * kKeys, token = t.token0 + key;
+                if (k_piece == 0 && token < t.end) tiles_cp_async(base + page_place(i, key), t.table + (token >> page_log2), 4, true);
+            }
         };
-        // the cache's row of a token (a number below 2^32, as the entry point has checked), and whether there is one
-        auto row_at = [&](const Tile& t, uint32_t key, int32_t page, bool& there) -> uint32_t {
-            const uint32_t token = t.token0 + key;
-            there = token < t.end && page >= 0 && (uint32_t)page < a.table.pages;
-            return there ? (((uint32_t)page * a.kv_heads + t.head / S::PARTS) << a.table.page_log2) + (token & page_mask) : 0u;
+        // The cache's rows of a tile's tokens (numbers below 2^32 - 1, as the entry point has checked), kNone where there is none.
+        constexpr uint32_t kNone = 0xFFFFFFFFu;
+        uint32_t rows[S::K_EACH], rows_v[S::K_EACH];           // of the tile whose K is requested next, and whose V is
+        auto find_rows = [&](const Tile& t, uint32_t i) {
+#pragma unroll
+            for (int j = 0; j < S::K_EACH; ++j) {
+                const uint32_t key = k_key0 + j * kKeys, token = t.token0 + key;
+                const int32_t page = *reinterpret_cast<const int32_t*>(smem + page_place(i, key));
+                const bool is = token < t.end && page >= 0 && (uint32_t)page < a.table.pages;
+                rows[j] = is ? (((uint32_t)page * a.kv_heads + t.head / S::PARTS) << page_log2) + (token & page_mask) : kNone;
+            }
         };
-        // the 32-bit word that holds a group's 16-bit scale (bias), and which half of it
-        auto ask_planes = [&](const KvPlanes& p, uint32_t row, uint32_t grp, bool there, uint32_t off) {
-            const size_t at = ((size_t)row * S::G + grp) & ~(size_t)1;
-            tiles_cp_async(base + off, p.scales + at, 4, there);
-            tiles_cp_async(base + off + 4, p.biases + at, 4, there);
+        // planes: lane p of a token's first four takes plane p
+        const uint16_t* my_plane = k_piece == 0 ? a.k.scales : k_piece == 1 ? a.k.biases : k_piece == 2 ? a.v.scales : a.v.biases;
+        auto ask_k = [&](uint32_t i) {
+#pragma unroll
+            for (int j = 0; j < S::K_EACH; ++j) {
+                const bool is = rows[j] != kNone;
+                const size_t row = is ? rows[j] : 0;
+                tiles_cp_async(base + S::OFF_KC + (j * S::UNPACK + u) * S::PIECE, a.k.codes + row * S::ROW_BYTES + k_piece * S::PIECE, S::PIECE, is);
+                if (k_piece < 4)
+                    tiles_cp_async(base + plane_place(i, k_key0 + j * kKeys) + k_piece * S::PLANES, my_plane + (S::G == 1 ? row & ~(size_t)1 : row * S::G), S::PLANES, is);
+            }
         };
-        const uint32_t k_half = S::G == 1 ? k_key(0) & 1u : k_piece / 4 & 1u, v_half = S::G == 1 ? v_key(0) & 1u : v_piece / 4 & 1u;
-        auto read_planes = [&](uint32_t off, uint32_t half, float& s, float& b) {        // the bias centred
-            const uint2 w = *reinterpret_cast<const uint2*>(smem + off);
-            s = __uint_as_float(half ? w.x & 0xFFFF0000u : w.x << 16);
-            b = fmaf(kCentre, s, __uint_as_float(half ? w.y & 0xFFFF0000u : w.y << 16));
-        };
-        auto ask_k = [&](const Tile& t, uint32_t i, uint32_t j) {
-            bool there;
-            const uint32_t row = row_at(t, k_key(j), page_at(k_page(i, j)), there);
-            tiles_cp_async(base + S::OFF_KC + (j * S::UNPACK + u) * S::PIECE, a.k.codes + (size_t)row * S::ROW_BYTES + k_piece * S::PIECE, S::PIECE, there);
-            ask_planes(a.k, row, k_piece / 4, there, S::OFF_KS + (j * S::UNPACK + u) * 8);
-        };
-        auto ask_v_planes = [&](const Tile& t, uint32_t i, uint32_t j) {
-            bool there;
-            const uint32_t row = row_at(t, v_key(j), page_at(v_page(i, j)), there);
-            ask_planes(a.v, row, v_piece / 4 + t.head % S::PARTS * S::GV, there, S::OFF_VS + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 8);
-        };
-        auto ask_v = [&](const Tile& t, uint32_t i, uint32_t j) {
-            bool there;
-            const uint32_t row = row_at(t, v_key(j), page_at(v_page(i, j)), there);
-            tiles_cp_async(base + S::OFF_VC + (j * S::UNPACK + u) * S::PIECE, a.v.codes + (size_t)row * S::ROW_BYTES + (v_piece + t.head % S::PARTS * S::V_ROW) * S::PIECE, S::PIECE,
-                           there);
+        auto ask_v = [&](const Tile& t) {
+#pragma unroll
+            for (int j = 0; j < S::V_EACH; ++j) {
+                const uint32_t r = D == 512 ? (lane & 16 ? rows_v[(2 * j + 1) % S::K_EACH] : rows_v[2 * j % S::K_EACH]) : rows_v[j];
+                const bool is = r != kNone;
+                tiles_cp_async(base + S::OFF_VC + (j * S::UNPACK + u) * S::PIECE,
+                               a.v.codes + (size_t)(is ? r : 0) * S::ROW_BYTES + (v_piece + t.head % S::PARTS * S::V_ROW) * S::PIECE, S::PIECE, is);
+            }
         };
         auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-        auto landed = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
-        // the largest of a token's lanes
-        auto token_most = [&](float v, int lanes) {
-            for (int off = lanes / 2; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, off));
-            return v;
+        // scale and centred bias of a group of a token (which: 0 K, 2 V)
+        auto read_planes = [&](uint32_t i, uint32_t key, int which, uint32_t grp, float& s, float& b) {
+            const uint8_t* at = smem + plane_place(i, key) + which * S::PLANES + 2 * (S::G == 1 ? key & 1u : grp);
+            s = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(at));
+            b = fmaf(kCentre, s, bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(at + S::PLANES)));
         };
-        auto magnitude = [&](float s, float b) { return fmaxf(kCentre * fabsf(s), fabsf(b)); };
-        auto exponent = [&](float most) { return min(max(rows_exponent(most) - 7, -126), 119); };      // both parts of a value below 2^8
-        auto store = [&](uint32_t buffer, const uint32_t (&r)[BITS / 2], float s, float b, uint32_t key, uint32_t piece) {
+        auto magnitude = [&](float s, float b) { return fmaxf(kCentre * fabsf(s), fabsf(b)); };      // half of the largest value or more
+        // values of such sizes are fp16 numbers as they are, and exact to 2^-11 of the token's largest
+        auto plain = [&](float s, float b) {
+            const float m = magnitude(s, b);
+            return m >= 0.001953125f && m <= 16384.0f && fabsf(b) <= 16384.0f;       // the last: maxima drop a NaN
+        };
+        // sixteen codes; lanes of odd groups take the second eight first, so that eight lanes meet eight different banks when they store
+        const uint32_t k_odd = S::K_ROW >= 8 ? k_piece / 4 & 1u : 0u, v_odd = S::K_ROW >= 8 ? v_piece / 4 & 1u : 0u;
+        auto read_codes = [&](uint32_t off, uint32_t odd, uint32_t (&r)[BITS / 2]) {
+            if constexpr (BITS == 8) {
+                const uint2 x = *reinterpret_cast<const uint2*>(smem + off + 8 * odd), y = *reinterpret_cast<const uint2*>(smem + off + 8 - 8 * odd);
+                r[0] = x.x; r[1] = x.y; r[2] = y.x; r[3] = y.y;
+            } else {
+                r[0] = *reinterpret_cast<const uint32_t*>(smem + off + 4 * odd);
+                r[1] = *reinterpret_cast<const uint32_t*>(smem + off + 4 - 4 * odd);
+            }
+        };
+        auto store = [&](uint32_t buffer, const uint32_t (&r)[BITS / 2], float s, float b, uint32_t key, uint32_t piece, uint32_t odd) {
             uint4 h[2];
             tiles_unpack<BITS>(r, s, b, h);
-            // the two chunks in the order in which eight lanes meet eight different banks
-            const uint32_t odd = S::K_ROW >= 8 ? piece / 4 & 1u : 0u, at = buffer + key * 128 + (piece / 4) * (TILE * 128), c0 = (piece % 4 * 2 + odd) ^ (key & 7u);
-            *reinterpret_cast<uint4*>(smem + at + c0 * 16) = odd ? h[1] : h[0];
-            *reinterpret_cast<uint4*>(smem + at + (c0 ^ 1u) * 16) = odd ? h[0] : h[1];
+            const uint32_t at = buffer + key * 128 + (piece / 4) * (TILE * 128), c0 = (piece % 4 * 2 + odd) ^ (key & 7u);
+            *reinterpret_cast<uint4*>(smem + at + c0 * 16) = h[0];
+            *reinterpret_cast<uint4*>(smem + at + (c0 ^ 1u) * 16) = h[1];
         };
         Cursor<MT, TILE> next = now;                           // of the tile that pages are asked for
         uint32_t left = busy ? (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), stop - item) : 0, ahead = 0;
@@ -289,116 +317,183 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         auto step = [&] {                                      // `next` one tile on, if there is one
             if (++ahead >= count) return;
             if (--left == 0) {
-                next.next_unit(a);
+                tiles_next_unit<MT, TILE>(a, next);
                 left = (uint32_t)lesser((uint64_t)next.range.tiles, (uint64_t)(count - ahead));
             } else {
                 ++next.tile;
             }
         };
         if (count) {
-            t0 = t1 = tile_of(next);
-            for (int j = 0; j < S::K_EACH; ++j) ask_page(t0, k_key(j), k_page(0, j));
-            if (!S::SAME)
-                for (int j = 0; j < S::V_EACH; ++j) ask_page(t0, v_key(j), v_page(0, j));
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            for (int j = 0; j < S::K_EACH; ++j) ask_k(t0, 0, j);
-            for (int j = 0; j < S::V_EACH; ++j) ask_v_planes(t0, 0, j);
+            t0 = tile_of(next);
+            ask_pages(t0, 0);
             step();
             t1 = tile_of(next);
-            if (count > 1) {
-                for (int j = 0; j < S::K_EACH; ++j) ask_page(t1, k_key(j), k_page(1, j));
-                if (!S::SAME)
-                    for (int j = 0; j < S::V_EACH; ++j) ask_page(t1, v_key(j), v_page(1, j));
-            }
+            if (count > 1) ask_pages(t1, 1);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+            find_rows(t0, 0);
+            ask_k(0);
             commit();
-            for (int j = 0; j < S::V_EACH; ++j) ask_v(t0, 0, j);
-            commit();
+            commit();                                          // in the place of values: the waits below count groups
             step();
             t2 = tile_of(next);
         }
-        // A wait that runs out is told to all, whose later waits end at once; every warp goes through all tiles.
-#pragma unroll 1
-        for (uint32_t i = 0; i < count; ++i) {
-            // ---- K_i, what is told about tile i; K_(i+1) and the planes of V_(i+1) are requested, and the pages of tile i + 2 ----
-            landed();
-            if (i >= 1) wait(k_free(), one(i - 1));
-            if (i >= 2) wait(s_free(i), two(i - 2));
-            uint32_t any = 0;
-#pragma unroll 1
-            for (int j = 0; j < S::V_EACH; ++j) {
-                const uint32_t key = v_key(j), token = t0.token0 + key;
-                float s, b;
-                read_planes(S::OFF_VS + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 8, v_half, s, b);
-                const bool broken = !(s - s == 0.0f && b - b == 0.0f);
-                const float most = token_most(broken ? 0.0f : magnitude(s, b), S::V_ROW);
-                const int32_t page = page_at(v_page(i, j));
-                const bool missing = token < t0.end && !(page >= 0 && (uint32_t)page < a.table.pages);
-                const uint32_t of_token = __ballot_sync(kFullMask, broken) >> (lane / S::V_ROW * S::V_ROW);
-                if (v_piece == 0) {
-                    uint32_t bits = missing ? 0x80u : 0u;
+        // K_n, what is told about tile n; K_(n+1) and all planes of tile n + 1 are requested, and the pages of tile n + 2
+        bool fast_v = true;                                    // of tile n: its values need no power of two
+        auto unpack_k = [&](uint32_t n) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();
+            float ks[S::K_EACH], kb[S::K_EACH];
+            bool fast = true;
 #pragma unroll
-                    for (int g = 0; g < S::GV; ++g) bits |= (of_token >> (4 * g) & 1u) << g;
-                    meta.v_up[i & 1][key] = rows_power(exponent(most));
-                    meta.bad[i & 1][key] = (uint8_t)bits;
+            for (int j = 0; j < S::K_EACH; ++j) {
+                const uint32_t key = k_key0 + j * kKeys;
+                read_planes(n, key, 0, k_piece / 4, ks[j], kb[j]);
+                fast = fast && (plain(ks[j], kb[j]) || t0.token0 + key >= t0.end);
+            }
+#pragma unroll
+            for (int j = 0; j < S::V_EACH; ++j) {
+                const uint32_t key = v_key0 + j * kVKeys;
+                float s, b;
+                read_planes(n, key, 2, v_piece / 4 + t0.head % S::PARTS * S::GV, s, b);
+                fast = fast && (plain(s, b) || t0.token0 + key >= t0.end);
+            }
+            fast = __all_sync(kFullMask, fast);
+            if (fast) {
+#pragma unroll
+                for (int j = 0; j < S::K_EACH; ++j)
+                    if (k_piece == 0) {
+                        const uint32_t key = k_key0 + j * kKeys;
+                        meta.k_up[n & 3][key] = a.scale * 1.4426950408889634f;
+                        meta.v_up[n & 3][key] = 1.0f;
+                        meta.bad[n & 3][key] = 0;
+                    }
+                if (lane == 0) {
+                    meta.flags[n & 3][uw] = 0;
+                    meta.v_most[n & 3][uw] = 1.0f;
+                }
+            } else {
+                // a power of two per token, planes that are not finite, pages that are missing
+                uint32_t any = 0;
+                float v_most = 0.0f;
+#pragma unroll 1
+                for (int j = 0; j < S::K_EACH; ++j) {
+                    const uint32_t key = k_key0 + j * kKeys, token = t0.token0 + key;
+                    float s, b;
+                    read_planes(n, key, 0, k_piece / 4, s, b);
+                    float most = s - s == 0.0f && b - b == 0.0f ? magnitude(s, b) : 0.0f;
+                    for (int off = S::K_ROW / 2; off >= 4; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, off));
+                    const int e_k = min(max(rows_exponent(most) - 7, -126), 119);      // both parts of a value below 2^8
+                    most = 0.0f;
+                    uint32_t bits = 0;
+#pragma unroll 1
+                    for (int grp = 0; grp < S::GV; ++grp) {
+                        read_planes(n, key, 2, grp + t0.head % S::PARTS * S::GV, s, b);
+                        if (s - s == 0.0f && b - b == 0.0f) most = fmaxf(most, magnitude(s, b));
+                        else bits |= 1u << grp;
+                    }
+                    const int e_v = min(max(rows_exponent(most) - 7, -126), 119);
+                    const int32_t page = *reinterpret_cast<const int32_t*>(smem + page_place(n, key));
+                    if (token < t0.end && !(page >= 0 && (uint32_t)page < a.table.pages)) {
+                        bits |= 0x80u;
+                        *a.error = kErrKvPage;
+                    }
+                    if (token >= t0.end) bits = 0;
+                    if (k_piece == 0) {
+                        meta.k_up[n & 3][key] = rows_power(e_k) * (a.scale * 1.4426950408889634f);
+                        meta.v_up[n & 3][key] = rows_power(e_v);
+                        meta.bad[n & 3][key] = (uint8_t)bits;
+                        meta.e_k[key] = (int8_t)e_k;
+                    }
                     any |= bits;
-                    if (missing) *a.error = kErrKvPage;
+                    v_most = fmaxf(v_most, rows_power(e_v));
+                }
+                any = __any_sync(kFullMask, any != 0);
+                v_most = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(v_most)));
+                if (lane == 0) {
+                    meta.flags[n & 3][uw] = (uint8_t)any;
+                    meta.v_most[n & 3][uw] = v_most;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < S::K_EACH; ++j) {
+                    const float down = rows_power(-meta.e_k[k_key0 + j * kKeys]);
+                    ks[j] *= down;
+                    kb[j] *= down;
                 }
             }
-            any = __any_sync(kFullMask, any != 0);
-#pragma unroll 1
+            fast_v = fast;
+            const bool more = n + 1 < count;
+#pragma unroll
+            for (int j = 0; j < S::K_EACH; ++j) rows_v[j] = rows[j];           // of tile n: as they were
+            if (more) find_rows(t1, n + 1);
+#pragma unroll
             for (int j = 0; j < S::K_EACH; ++j) {
-                const uint32_t key = k_key(j);
                 uint32_t r[BITS / 2];
-                load_words(r, smem + S::OFF_KC + (j * S::UNPACK + u) * S::PIECE);
-                float s, b;
-                read_planes(S::OFF_KS + (j * S::UNPACK + u) * 8, k_half, s, b);
-                const bool broken = !(s - s == 0.0f && b - b == 0.0f);
-                const int e = exponent(token_most(broken ? 0.0f : magnitude(s, b), S::K_ROW));
-                const float down = rows_power(-e);
-                if (k_piece == 0) meta.k_up[i & 1][key] = rows_power(e) * (a.scale * 1.4426950408889634f);
-                store(S::OFF_K, r, s * down, b * down, key, k_piece);
-                if (i + 1 < count) ask_k(t1, i + 1, j);
+                read_codes(S::OFF_KC + (j * S::UNPACK + u) * S::PIECE, k_odd, r);
+                store(S::OFF_K + (n % S::K_BUFS) * S::K_BYTES, r, ks[j], kb[j], k_key0 + j * kKeys, k_piece, k_odd);
             }
-            if (lane == 0) meta.flags[i & 1][uw] = (uint8_t)any;
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(k_full());
-                mbar_arrive(told(i));
-            }
-            if (i + 1 < count) {
-#pragma unroll 1
-                for (int j = 0; j < S::V_EACH; ++j) ask_v_planes(t1, i + 1, j);
-            }
-            if (i + 2 < count) {
-                for (int j = 0; j < S::K_EACH; ++j) ask_page(t2, k_key(j), k_page(i + 2, j));
-                if (!S::SAME)
-                    for (int j = 0; j < S::V_EACH; ++j) ask_page(t2, v_key(j), v_page(i + 2, j));
-            }
+            if (lane == 0) mbar_arrive(k_full(n));
+            if (more) ask_k(n + 1);
+            if (n + 2 < count) ask_pages(t2, n + 2);
             commit();
-            // ---- V_i; the codes of V_(i+1) are requested ----
-            landed();
-            if (i >= S::V_BUFS) wait(v_free(i), of_v(i - S::V_BUFS));
-#pragma unroll 1
+        };
+        // V_n; the codes of V_(n+1) are requested
+        auto unpack_v = [&](uint32_t n, const Tile& t, const Tile& after, bool fast) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            float vs[S::V_EACH], vb[S::V_EACH];
+#pragma unroll
             for (int j = 0; j < S::V_EACH; ++j) {
-                const uint32_t key = v_key(j);
+                const uint32_t key = v_key0 + j * kVKeys;
+                read_planes(n, key, 2, v_piece / 4 + t.head % S::PARTS * S::GV, vs[j], vb[j]);
+                if (!fast) {
+                    const float down = __uint_as_float(0x7F000000u - __float_as_uint(meta.v_up[n & 3][key]));      // the reciprocal of a power of two
+                    const bool fine = vs[j] - vs[j] == 0.0f && vb[j] - vb[j] == 0.0f;
+                    vs[j] = fine ? vs[j] * down : 0.0f;
+                    vb[j] = fine ? vb[j] * down : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < S::V_EACH; ++j) {
                 uint32_t r[BITS / 2];
-                load_words(r, smem + S::OFF_VC + (j * S::UNPACK + u) * S::PIECE);
-                float s, b;
-                read_planes(S::OFF_VS + (((i & 1) * S::V_EACH + j) * S::UNPACK + u) * 8, v_half, s, b);
-                if (!(s - s == 0.0f && b - b == 0.0f)) s = b = 0.0f;
-                const float down = __uint_as_float(0x7F000000u - __float_as_uint(meta.v_up[i & 1][key]));      // the reciprocal of a power of two
-                store(S::OFF_V + (i % S::V_BUFS) * S::V_BYTES, r, s * down, b * down, key, v_piece);
-                if (i + 1 < count) ask_v(t1, i + 1, j);
+                read_codes(S::OFF_VC + (j * S::UNPACK + u) * S::PIECE, v_odd, r);
+                store(S::OFF_V, r, vs[j], vb[j], v_key0 + j * kVKeys, v_piece, v_odd);
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(v_full(i));
+            if (lane == 0) mbar_arrive(v_full);
+            if (n + 1 < count) ask_v(after);
             commit();
-            t0 = t1;
-            t1 = t2;
-            step();
-            t2 = tile_of(next);
+        };
+        // A wait that runs out is told to all, whose later waits end at once; every warp goes through all tiles. Commits alternate
+        // between K (with planes and pages) and V, as their uses do: K_(i+1), V_i, K_(i+2), ...; one later group may be pending at each wait.
+        if (count) {
+            unpack_k(0);
+            ask_v(t0);
+            commit();
+        }
+        Tile tv = t0, tv1 = t1;                                // tiles i, i + 1 of the values
+        bool fast_i = fast_v;
+#pragma unroll 1
+        for (uint32_t i = 0; i < count; ++i) {
+            const bool fast_now = fast_i;
+            if (i + 1 < count) {
+                t0 = t1;
+                t1 = t2;
+                step();
+                t2 = tile_of(next);
+                if (i + 1 >= S::K_BUFS) wait(k_free(i + 1), of_k(i + 1 - S::K_BUFS));
+                unpack_k(i + 1);
+                fast_i = fast_v;
+            } else {
+                commit();
+            }
+            if (i >= 1) wait(o_done(i - 1), two(i - 1));
+            unpack_v(i, tv, tv1, fast_now);
+            tv = tv1;
+            tv1 = t1;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == S::WARPS - 1) {
@@ -408,30 +503,30 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         uint32_t segment = 0, segments = 0;
         bool opens = false;                                    // tile i - 1 is its unit's first here: its product starts O anew
         auto logits = [&](uint32_t i) -> bool {
-            if (!wait(k_full(), one(i)) || (i >= 2 && !wait(s_free(i), two(i - 2)))) return false;
+            if (!wait(k_full(i), of_k(i))) return false;
             tiles_fence_after();
             if (lane == 0) {
-                const uint64_t q0 = tiles_desc(base, 16, 1024), k0 = tiles_desc(base + S::OFF_K, 16, 1024);
+                const uint64_t q0 = tiles_desc(base, 16, 1024), k0 = tiles_desc(base + S::OFF_K + (i % S::K_BUFS) * S::K_BYTES, 16, 1024);
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e)
                     tiles_mma_ss(tmem + S::COL_S + (i & 1) * TILE, q0 + (((e / 4) * (MT * 128) + e % 4 * 32) >> 4), k0 + (((e / 4) * (TILE * 128) + e % 4 * 32) >> 4),
                                  idesc_s, e > 0);
                 tiles_commit(s_full(i));
-                tiles_commit(k_free());
+                tiles_commit(k_free(i));
+                mbar_arrive(s_full(i));
             }
             __syncwarp();
             return true;
         };
         auto values = [&](uint32_t j) -> bool {
-            if (!wait(p_full(j), two(j)) || !wait(v_full(j), of_v(j))) return false;
+            if (!wait(v_full, one(j)) || !wait(p_full(j), two(j))) return false;
             tiles_fence_after();
             if (lane == 0) {
-                const uint64_t v0 = tiles_desc(base + S::OFF_V + (j % S::V_BUFS) * S::V_BYTES, TILE * 128, 1024);
+                const uint64_t v0 = tiles_desc(base + S::OFF_V, TILE * 128, 1024);
 #pragma unroll
                 for (int e = 0; e < TILE / 16; ++e)
                     tiles_mma_ts(tmem + S::COL_O, tmem + S::COL_P + (j & 1) * (TILE / 2) + e * 8, v0 + (e * 2048 >> 4), idesc_o, e > 0 || !opens);
                 tiles_commit(o_done(j));
-                tiles_commit(v_free(j));
             }
             __syncwarp();
             return true;
@@ -443,7 +538,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             if (new_unit || i == count) {
                 if (i > 0 && !values(i - 1)) break;
                 if (i == count) break;
-                if (i) now.next_unit(a);
+                if (i) tiles_next_unit<MT, TILE>(a, now);
                 segment = (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), (uint64_t)(count - i));
                 if (!wait(q_full, segments++ & 1u) || !logits(i)) break;
             } else if (!logits(i) || !values(i - 1)) {
@@ -455,75 +550,106 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         // nothing is in flight when the block leaves
         if (lane == 0) tiles_commit(all_done);
         __syncwarp();
-        for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
+        for (uint32_t look = 0; look < kLooks; ++look) {
             uint32_t ok;
-            asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(all_done), "r"(0u) : "memory");
+            asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+                         : "=r"(ok) : "r"(all_done), "r"(0u), "r"(10000u) : "memory");
             if (ok) break;
         }
     } else {
-        // ===================== softmax: a thread per row =====================
-        const uint32_t r = tid, lanes = tmem + ((uint32_t)warp * 32u << 16);
+        // ===================== softmax: two threads per row, warps w and w + 4, with half of a tile each =====================
+        const uint32_t quad = warp % 4, side = warp / 4, r = quad * 32 + lane, lanes = tmem + (quad * 32u << 16);
+        constexpr int CHUNK = S::CHUNK, HALF = TILE / 2;
+        uint32_t turn = 0;
+        // both threads' values of a pair, and a barrier of the two warps
+        auto swap = [&](float x, float& y) {
+            meta.pair[turn][r][side] = x;
+            asm volatile("bar.sync %0, 64;" ::"r"(2 + quad) : "memory");
+            y = meta.pair[turn][r][side ^ 1];
+            turn ^= 1;
+        };
         uint32_t i = 0;
         bool ok = true;
-        while (ok && i < count) {
+        while (i < count) {
             // ---- the unit's rows of q: fp16 in the operand's layout, brought to one range by a power of two ----
             const uint32_t valid = lesser((uint32_t)MT, now.flat_rows(a) - now.flat0), first_tile = now.tile;
             const uint32_t segment = (uint32_t)lesser((uint64_t)(now.range.tiles - first_tile), (uint64_t)(count - i));
             const bool is = r < valid, from_start = first_tile == 0, whole = from_start && segment == now.range.tiles;
             const uint32_t flat = now.flat0 + (is ? r : 0), node = flat / a.group, head = now.head / S::PARTS;
-            const uint16_t* src = a.q + (size_t)(now.seq.row0 + node) * a.q_stride + (size_t)(head * a.group + flat % a.group) * D;
-            uint32_t most = 0;
-            if (is)
+            {
+                // lanes side by side along the rows; bf16 rows are brought to one range, their largest element to [1, 2)
+                constexpr int ROW_LANES = D / 8 < 32 ? D / 8 : 32, EACH = D / 8 / ROW_LANES, AT_ONCE = S::SOFT_WARPS * kWarp / ROW_LANES;
+                const uint32_t row_lane = tid % ROW_LANES;
 #pragma unroll 4
-                for (int c = 0; c < D / 8; ++c) {
-                    const uint4 v = reinterpret_cast<const uint4*>(src)[c];
-                    most = __vmaxu2(__vmaxu2(__vmaxu2(most, v.x & 0x7FFF7FFFu), __vmaxu2(v.y & 0x7FFF7FFFu, v.z & 0x7FFF7FFFu)), v.w & 0x7FFF7FFFu);
-                }
-            most = max(most & 0xFFFFu, most >> 16);
-            const float q_top = BF16 ? bf16_bits_to_float((uint16_t)most) : f16_bits_to_float((uint16_t)most);
-            const int e_q = q_top > 0.0f && q_top <= 3.402823466e38f ? max(rows_exponent(q_top), -126) : 0;      // the largest element to [1, 2)
-            const float down = rows_power(-e_q), q_up = rows_power(e_q);
-#pragma unroll 2
-            for (int c = 0; c < D / 8; ++c) {
-                const uint4 v = is ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                uint32_t h[4];
+                for (uint32_t q = tid / ROW_LANES; q < MT; q += AT_ONCE) {
+                    const uint32_t f = now.flat0 + (q < valid ? q : 0);
+                    const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(now.seq.row0 + f / a.group) * a.q_stride + (size_t)(head * a.group + f % a.group) * D) + row_lane;
+                    uint4 v[EACH];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float lo = BF16 ? __uint_as_float(w[j] << 16) : f16_bits_to_float((uint16_t)w[j]);
-                    const float hi = BF16 ? __uint_as_float(w[j] & 0xFFFF0000u) : f16_bits_to_float((uint16_t)(w[j] >> 16));
-                    h[j] = rows_half2(lo * down, hi * down);
+                    for (int e = 0; e < EACH; ++e) v[e] = q < valid ? src[e * ROW_LANES] : make_uint4(0, 0, 0, 0);
+                    float up = 1.0f;
+                    if constexpr (BF16) {
+                        uint32_t most = 0;
+#pragma unroll
+                        for (int e = 0; e < EACH; ++e)
+                            most = __vmaxu2(__vmaxu2(__vmaxu2(most, v[e].x & 0x7FFF7FFFu), __vmaxu2(v[e].y & 0x7FFF7FFFu, v[e].z & 0x7FFF7FFFu)), v[e].w & 0x7FFF7FFFu);
+                        most = max(most & 0xFFFFu, most >> 16);
+#pragma unroll
+                        for (int off = ROW_LANES / 2; off >= 1; off >>= 1) most = max(most, __shfl_xor_sync(kFullMask, most, off));
+                        const float top = bf16_bits_to_float((uint16_t)most);
+                        const int e_q = top > 0.0f && top <= 3.402823466e38f ? max(rows_exponent(top), -126) : 0;
+                        const float down = rows_power(-e_q);
+                        up = rows_power(e_q);
+#pragma unroll
+                        for (int e = 0; e < EACH; ++e) {
+                            uint32_t* w = reinterpret_cast<uint32_t*>(&v[e]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) w[j] = rows_half2(__uint_as_float(w[j] << 16) * down, __uint_as_float(w[j] & 0xFFFF0000u) * down);
+                        }
+                    }
+                    if (row_lane == 0) meta.q_up[q] = up;
+#pragma unroll
+                    for (int e = 0; e < EACH; ++e) {
+                        const uint4 h = v[e];
+                        const uint4 out = BITS == 8 ? h : make_uint4(gm_prmt(h.x, h.z, 0x5410), gm_prmt(h.x, h.z, 0x7632), gm_prmt(h.y, h.w, 0x5410), gm_prmt(h.y, h.w, 0x7632));
+                        *reinterpret_cast<uint4*>(smem + S::chunk_at(MT, q, row_lane + e * ROW_LANES)) = out;
+                    }
                 }
-                const uint4 out = BITS == 8 ? make_uint4(h[0], h[1], h[2], h[3])
-                                            : make_uint4(gm_prmt(h[0], h[2], 0x5410), gm_prmt(h[0], h[2], 0x7632), gm_prmt(h[1], h[3], 0x5410), gm_prmt(h[1], h[3], 0x7632));
-                *reinterpret_cast<uint4*>(smem + S::chunk_at(MT, r, c)) = out;
             }
             fence_proxy_async();
-            __syncwarp();
+            asm volatile("bar.sync 1, %0;" ::"n"(S::SOFT_WARPS * kWarp) : "memory");           // the rows' powers of two
             if (lane == 0) mbar_arrive(q_full);
+            const float q_up = meta.q_up[r];
             uint32_t low = 0;                                  // first token that the row sees
             if (a.window && is) {
                 const int64_t pos = a.mask ? max((int64_t)a.positions[now.seq.row0 + node], (int64_t)now.seq.context) : (int64_t)now.seq.context + node;
                 low = (uint32_t)max((int64_t)0, lesser(pos - (int64_t)a.window + 1, (int64_t)kMostTokens));
             }
             const uint32_t low_most = __reduce_max_sync(kFullMask, low), open_end = lesser(now.seq.context, now.range.end);
-            float m = -INFINITY, l = 0.0f;                     // l and O: in units of 2^(m + E)
+            float m = -INFINITY, l = 0.0f;                     // of the row; l of this thread's tokens; l and O in units of 2^(m + E)
             int e_o = -126;
             uint32_t poison = 0;                               // groups that are not a number
             const uint32_t begin_i = i, stop_i = i + segment;
-            uint32_t token0 = now.token0();
+            uint32_t token0 = now.token0() + side * HALF;
+            // A wait that runs out is told to all, whose later waits end at once; the warps of a pair go through all tiles, since they meet in each.
 #pragma unroll 1
             for (; i < stop_i; ++i, token0 += TILE) {
                 const uint32_t st = i & 1;
-                ok = wait(s_full(i), two(i)) && wait(told(i), two(i));
-                if (!ok) break;
+                ok = wait(s_full(i), two(i));
                 tiles_fence_after();
-                const uint2 flags = *reinterpret_cast<const uint2*>(meta.flags[st]);
-                const bool odd = (flags.x | flags.y) != 0;
-                const bool open = !odd && token0 >= low_most && token0 + TILE <= open_end;
-                // the tokens of chunk w that the row sees
-                auto see = [&](int w) -> uint32_t {
-                    const uint32_t t0 = token0 + 32 * w;
+                uint32_t flags = 0;
+                float v_most = 0.0f;
+#pragma unroll
+                for (int w = 0; w < S::UNPACK_WARPS; w += 4) {
+                    flags |= *reinterpret_cast<const uint32_t*>(&meta.flags[i & 3][w]);
+                    const float4 v = *reinterpret_cast<const float4*>(&meta.v_most[i & 3][w]);
+                    v_most = fmaxf(fmaxf(v_most, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+                }
+                const bool odd = flags != 0;
+                const bool open = !odd && token0 >= low_most && token0 + HALF <= open_end;
+                // the tokens from `t0` on that the row sees, a chunk of them
+                auto see = [&](int c0) -> uint32_t {
+                    const uint32_t t0 = token0 + c0;
                     auto below = [&](uint32_t end) { return end <= t0 ? 0u : end - t0 >= 32 ? 0xFFFFFFFFu : (1u << (end - t0)) - 1u; };      // tokens before `end`
                     uint32_t seen = below(open_end) & ~below(low);
                     const uint32_t drafted = below(now.range.end) & ~below(now.seq.context);
@@ -542,133 +668,124 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                         }
                     }
                     if (odd)
-                        for (int j = 0; j < 32; ++j)
-                            if (meta.bad[st][32 * w + j] & 0x80u) seen &= ~(1u << j);
+                        for (int j = 0; j < CHUNK; ++j)
+                            if (meta.bad[i & 3][side * HALF + c0 + j] & 0x80u) seen &= ~(1u << j);
                     return is ? seen : 0u;
                 };
-                // the logits of 32 tokens, in base 2 but for the row's power of two
-                auto load_logits = [&](int w, float (&x)[32]) {
-                    uint32_t raw[32];
-                    tiles_ld32(lanes + S::COL_S + st * TILE + w * 32, raw);
+                // the logits of a chunk, in base 2 but for the row's power of two
+                auto load_logits = [&](int c0, float (&x)[CHUNK]) {
+                    uint32_t raw[CHUNK];
+                    tiles_ld(lanes + S::COL_S + st * TILE + side * HALF + c0, raw);
                     tiles_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 up = *reinterpret_cast<const float4*>(&meta.k_up[st][32 * w + j]);
+                    for (int j = 0; j < CHUNK; j += 4) {
+                        const float4 up = *reinterpret_cast<const float4*>(&meta.k_up[i & 3][side * HALF + c0 + j]);
                         x[j] = __uint_as_float(raw[j]) * up.x;
                         x[j + 1] = __uint_as_float(raw[j + 1]) * up.y;
                         x[j + 2] = __uint_as_float(raw[j + 2]) * up.z;
                         x[j + 3] = __uint_as_float(raw[j + 3]) * up.w;
                     }
                     if (!open) {
-                        const uint32_t seen = see(w);
+                        const uint32_t seen = see(c0);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] = seen >> j & 1u ? x[j] : -INFINITY;
+                        for (int j = 0; j < CHUNK; ++j) x[j] = seen >> j & 1u ? x[j] : -INFINITY;
                     }
                 };
                 // ---- maximum ----
-                float top = -INFINITY;
+                float top = -INFINITY, x[CHUNK];               // x: where a half is one chunk, it stays
 #pragma unroll 1
-                for (int w = 0; w < TILE / 32; ++w) {
-                    float x[32];
-                    load_logits(w, x);
+                for (int c0 = 0; c0 < HALF; c0 += CHUNK) {
+                    load_logits(c0, x);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
+                    for (int j = 0; j < CHUNK; ++j) top = fmaxf(top, x[j]);
                 }
-                top *= q_up;
+                float other;
+                swap(top, other);
+                top = fmaxf(top, other) * q_up;
                 float alpha = 1.0f;
                 if (top > m + 8.0f) {
                     alpha = rows_exp2(m - top);                // m = -inf: zero
                     m = top;
                 }
-                // ---- probabilities, two to a column ----
-                if (i >= 2) {
-                    ok = wait(o_done(i), two(i - 2));          // P's buffer has been read
-                    if (!ok) break;
-                }
-                float sum;
-                for (int round = 0;; ++round) {
-                    const float shift = (m == -INFINITY ? 0.0f : m) + (float)e_o;
+                const float base_m = m == -INFINITY ? 0.0f : m;
+                // ---- E: a value's power of two times 2^8, the largest probability, must not leave fp16 ----
+                if (__any_sync(kFullMask, v_most * rows_power(-e_o) > 64.0f)) {
                     float heavy = 0.0f;
-                    sum = 0.0f;
 #pragma unroll 1
-                    for (int w = 0; w < TILE / 32; ++w) {
-                        float x[32];
-                        uint32_t p[16];
-                        load_logits(w, x);
+                    for (int c0 = 0; c0 < HALF; c0 += CHUNK) {
+                        if (HALF > CHUNK) load_logits(c0, x);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 up = *reinterpret_cast<const float4*>(&meta.v_up[st][32 * w + j]);
-                            const float p0 = rows_exp2(fmaf(x[j], q_up, -shift)), p1 = rows_exp2(fmaf(x[j + 1], q_up, -shift));
-                            const float p2 = rows_exp2(fmaf(x[j + 2], q_up, -shift)), p3 = rows_exp2(fmaf(x[j + 3], q_up, -shift));
-                            sum += (p0 + p1) + (p2 + p3);
-                            const float v0 = p0 * up.x, v1 = p1 * up.y, v2 = p2 * up.z, v3 = p3 * up.w;
-                            heavy = fmaxf(fmaxf(heavy, fmaxf(v0, v1)), fmaxf(v2, v3));
-                            p[j / 2] = rows_half2(v0, v1);
-                            p[j / 2 + 1] = rows_half2(v2, v3);
-                        }
-                        tiles_st16(lanes + S::COL_P + st * (TILE / 2) + w * 16, p);
-                        if (odd) {
-                            // a row that gives a token weight whose planes are not finite in a group becomes NaN there
-#pragma unroll 1
-                            for (int j = 0; j < 32; ++j) {
-                                const uint32_t bad = meta.bad[st][32 * w + j] & 0x7Fu;
-                                if (bad && (see(w) >> j & 1u)) {
-                                    float z = 0.0f;
-#pragma unroll
-                                    for (int k = 0; k < 32; ++k) z = k == j ? x[k] : z;
-                                    if (rows_exp2(fmaf(z, q_up, -shift)) > 0.0f) poison |= bad;
-                                }
-                            }
-                        }
+                        for (int j = 0; j < CHUNK; ++j) heavy = fmaxf(heavy, rows_exp2(fmaf(x[j], q_up, -base_m)) * meta.v_up[i & 3][side * HALF + c0 + j]);
                     }
-                    if (!__any_sync(kFullMask, heavy > 16384.0f) || round == 2) break;
-                    tiles_wait_st();                           // the next round stores to the same columns
-                    // E of the rows that have outgrown it: their largest p' to below 16, by what it is when nothing is divided
-                    float most = 0.0f;
-                    const float plain = m == -INFINITY ? 0.0f : m;
-#pragma unroll 1
-                    for (int w = 0; w < TILE / 32; ++w) {
-                        float x[32];
-                        load_logits(w, x);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) most = fmaxf(most, rows_exp2(fmaf(x[j], q_up, -plain)) * meta.v_up[st][32 * w + j]);
-                    }
-                    if (heavy > 16384.0f) {
-                        const int e_new = min(max(e_o, rows_exponent(most) - 3), 119);
+                    swap(heavy, other);
+                    heavy = fmaxf(heavy, other);
+                    if (heavy * rows_power(-e_o) > 16384.0f || e_o == -126) {
+                        const int e_new = min(max(e_o, rows_exponent(heavy) - 3), 119);      // the row's largest p' below 16
                         alpha *= rows_power(e_o - e_new);
                         e_o = e_new;
                     }
                 }
+                // ---- probabilities, two to a column ----
+                const float shift = base_m + (float)e_o;
+                float sum = 0.0f;
+#pragma unroll 1
+                for (int c0 = 0; c0 < HALF; c0 += CHUNK) {
+                    uint32_t p[CHUNK / 2];
+                    if (HALF > CHUNK) load_logits(c0, x);
+#pragma unroll
+                    for (int j = 0; j < CHUNK; j += 4) {
+                        const float4 up = *reinterpret_cast<const float4*>(&meta.v_up[i & 3][side * HALF + c0 + j]);
+                        const float p0 = rows_exp2(fmaf(x[j], q_up, -shift)), p1 = rows_exp2(fmaf(x[j + 1], q_up, -shift));
+                        const float p2 = rows_exp2(fmaf(x[j + 2], q_up, -shift)), p3 = rows_exp2(fmaf(x[j + 3], q_up, -shift));
+                        sum += (p0 + p1) + (p2 + p3);
+                        p[j / 2] = rows_half2(p0 * up.x, p1 * up.y);
+                        p[j / 2 + 1] = rows_half2(p2 * up.z, p3 * up.w);
+                    }
+                    tiles_st(lanes + S::COL_P + st * (TILE / 2) + (side * HALF + c0) / 2, p);
+                    if (odd) {
+                        // a row that gives a token weight whose planes are not finite in a group becomes NaN there
+#pragma unroll 1
+                        for (int j = 0; j < CHUNK; ++j) {
+                            const uint32_t bad = meta.bad[i & 3][side * HALF + c0 + j] & 0x7Fu;
+                            if (bad) {
+                                float z = -INFINITY;
+#pragma unroll
+                                for (int k = 0; k < CHUNK; ++k) z = k == j ? x[k] : z;
+                                if (rows_exp2(fmaf(z, q_up, -base_m)) > 0.0f) poison |= bad;
+                            }
+                        }
+                    }
+                }
                 l = fmaf(l, alpha, sum);
-                // ---- O, when m or E moved ----
+                // ---- O, when m or E moved: half of its columns ----
                 if (i > begin_i && __any_sync(kFullMask, alpha != 1.0f)) {
-                    ok = wait(o_done(i - 1), two(i - 1));
-                    if (!ok) break;
+                    ok = wait(o_done(i - 1), two(i - 1)) && ok;
                     tiles_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < S::DV; c += 32) {
+                    for (int c = side * (S::DV / 2); c < (int)(side + 1) * (S::DV / 2); c += 32) {
                         uint32_t o[32];
-                        tiles_ld32(lanes + S::COL_O + c, o);
+                        tiles_ld(lanes + S::COL_O + c, o);
                         tiles_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                        tiles_st32(lanes + S::COL_O + c, o);
+                        tiles_st(lanes + S::COL_O + c, o);
                     }
                 }
                 tiles_wait_st();
                 tiles_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(s_free(i));
-                    mbar_arrive(p_full(i));
-                }
+                if (lane == 0) mbar_arrive(p_full(i));
             }
-            if (!ok) break;
             // ---- the segment's result ----
-            if (!wait(o_done(i - 1), two(i - 1))) break;
+            float other;
+            swap(l, other);
+            l += other;
+            swap(__uint_as_float(poison), other);
+            poison |= __float_as_uint(other);
+            ok = wait(o_done(i - 1), two(i - 1)) && ok;
             tiles_fence_after();
             float* part = a.partial + (size_t)(2 * blockIdx.x + (from_start ? 1 : 0)) * MT * (S::DV + 2);
-            if (!whole && is) {
+            if (!whole && is && side == 0) {
                 part[r] = m + (float)e_o;
                 part[MT + r] = l;
             }
@@ -676,12 +793,12 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             uint16_t* dst = a.out + (size_t)(now.seq.row0 + node) * a.out_stride + (size_t)(head * a.group + flat % a.group) * D + now.head % S::PARTS * S::DV;
             float* pdst = part + 2 * MT + (size_t)r * S::DV;
 #pragma unroll 1
-            for (int c = 0; c < S::DV; c += 32) {
+            for (int c = side * (S::DV / 2); c < (int)(side + 1) * (S::DV / 2); c += 32) {
                 uint32_t o[32];
-                tiles_ld32(lanes + S::COL_O + c, o);
+                tiles_ld(lanes + S::COL_O + c, o);
                 tiles_wait_ld();
                 const float by = poison >> (c / 64) & 1u ? __int_as_float(0x7FC00000) : inv;
-                if (is) {
+                if (is && ok) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         float v[8];
@@ -707,7 +824,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 info.head = now.head;
                 info.active = 1;
             }
-            if (i < count) now.next_unit(a);
+            if (i < count) tiles_next_unit<MT, TILE>(a, now);
         }
     }
     tiles_fence_before();

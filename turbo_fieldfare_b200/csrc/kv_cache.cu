@@ -14,7 +14,7 @@ tf_status check_kv_cache(tf_context* ctx, const char* name, const tf_kv_cache* c
                "%s: page_size %u is not a power of two from 16 to 65536", name, c->page_size);
     TF_REQUIRE(ctx, c->num_pages > 0 && c->num_pages <= 0x7FFFFFFFu && c->kv_heads > 0 && c->kv_heads <= 65535, TF_ERR_INVALID_ARGUMENT,
                "%s: num_pages and kv_heads must be positive (num_pages below 2^31, kv_heads below 65536)", name);
-    TF_REQUIRE(ctx, (uint64_t)c->num_pages * c->kv_heads * c->page_size <= 0xFFFFFFFFull, TF_ERR_UNSUPPORTED,
+    TF_REQUIRE(ctx, (uint64_t)c->num_pages * c->kv_heads * c->page_size < 0xFFFFFFFFull, TF_ERR_UNSUPPORTED,
                "%s: pages times heads times page size must be below 2^32", name);
     TF_REQUIRE(ctx, aligned(c->k_codes, 16) && aligned(c->k_scales, 16) && aligned(c->k_biases, 16) && aligned(c->v_codes, 16) &&
                         aligned(c->v_scales, 16) && aligned(c->v_biases, 16), TF_ERR_ALIGNMENT, "%s: cache planes must be 16-byte aligned", name);
