@@ -80,181 +80,301 @@ __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[WORDS])
     }
 }
 
-// One head's values, VEC per lane, as codes and planes of their groups of 64 at row `row` of the planes (a row is one token of one head).
+// Minimum and maximum that keep a NaN of either side.
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+// One head's values, VEC per lane, as codes and planes of their groups of 64 at row `row` of the planes (a row is one token of one head). The planes
+// are rounded to bf16, as the cache holds them, and the codes are those of the rounded planes: a value is off by half a code step where no rounding of
+// the bias or scale pushes it past the ends. A group that holds a NaN or an infinity, or whose planes have no bf16 value, gets NaN planes.
 template <int D>
 __device__ __forceinline__ void quantise_head(const float (&f)[D / 32], const KvPlanes& planes, size_t row, int bits, int lane) {
     constexpr int VEC = D / 32, LANES = 64 / VEC;            // lanes of a group
     float low = f[0], high = f[0];
-    bool bad = false;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        low = fminf(low, f[e]);
-        high = fmaxf(high, f[e]);
-        bad |= !(fabsf(f[e]) <= 3.402823466e38f);
+    for (int e = 1; e < VEC; ++e) {
+        low = min_nan(low, f[e]);
+        high = max_nan(high, f[e]);
     }
 #pragma unroll
     for (int off = LANES / 2; off >= 1; off >>= 1) {
-        low = fminf(low, __shfl_xor_sync(kFullMask, low, off));
-        high = fmaxf(high, __shfl_xor_sync(kFullMask, high, off));
+        low = min_nan(low, __shfl_xor_sync(kFullMask, low, off));
+        high = max_nan(high, __shfl_xor_sync(kFullMask, high, off));
     }
-    const int group = lane / LANES;
-    const unsigned lanes = (LANES == 32 ? kFullMask : ((1u << (LANES % 32)) - 1u)) << (group * LANES % 32);
-    bad = (__ballot_sync(kFullMask, bad) & lanes) != 0;
     const float top = bits == 8 ? 255.0f : 15.0f;
-    uint16_t s16 = __bfloat16_as_ushort(__float2bfloat16_rn(high == low ? 1.0f : __fdiv_rn(high - low, top)));
+    uint16_t s16 = __bfloat16_as_ushort(__float2bfloat16_rn(high == low ? 1.0f : (high - low) * (bits == 8 ? 1.0f / 255.0f : 1.0f / 15.0f)));
     uint16_t o16 = __bfloat16_as_ushort(__float2bfloat16_rn(low));
-    if (bad || (s16 & 0x7F80) == 0x7F80 || (o16 & 0x7F80) == 0x7F80) s16 = o16 = kBf16NaN;
+    const bool finite = low >= -3.402823466e38f && high <= 3.402823466e38f && (s16 & 0x7F80) != 0x7F80 && (o16 & 0x7F80) != 0x7F80;
+    if (!finite) s16 = o16 = kBf16NaN;
     const float scale = bf16_bits_to_float(s16), bias = bf16_bits_to_float(o16);
-    const float inv = scale == 0.0f ? 0.0f : __fdiv_rn(1.0f, scale);
-    uint32_t code[VEC];
+    const float inv = scale == 0.0f ? 0.0f : __frcp_rn(scale);
+    uint32_t code[VEC];                                       // in the low byte, under the bits of 2^23: added toward zero it leaves the whole part
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) code[e] = (uint32_t)fminf(fmaxf(floorf(__fadd_rn(__fmul_rn(f[e] - bias, inv), 0.5f)), 0.0f), top);   // a NaN becomes 0
+    for (int e = 0; e < VEC; ++e)
+        code[e] = __float_as_uint(__fadd_rz(fminf(fmaxf(__fadd_rn(__fmul_rn(f[e] - bias, inv), 0.5f), 0.0f), top), 8388608.0f));      // a NaN becomes 0
     if (bits == 8) {
         uint8_t* at = planes.codes + row * D + lane * VEC;
         if constexpr (VEC == 2) {
-            *reinterpret_cast<uint16_t*>(at) = (uint16_t)(code[0] | code[1] << 8);
+            *reinterpret_cast<uint16_t*>(at) = (uint16_t)__byte_perm(code[0], code[1], 0x0040);
         } else {
             uint32_t w[VEC / 4];
 #pragma unroll
-            for (int i = 0; i < VEC / 4; ++i) w[i] = code[4 * i] | code[4 * i + 1] << 8 | code[4 * i + 2] << 16 | code[4 * i + 3] << 24;
+            for (int i = 0; i < VEC / 4; ++i)
+                w[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040), __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410);
             store_words(at, w);
         }
     } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) code[e] = (code[e] & 15u) | (code[e + 1] & 15u) << 4;
         uint8_t* at = planes.codes + row * (D / 2) + lane * (VEC / 2);
-        if constexpr (VEC == 2) *at = (uint8_t)(code[0] | code[1] << 4);
-        else if constexpr (VEC == 4) *reinterpret_cast<uint16_t*>(at) = (uint16_t)(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
+        if constexpr (VEC == 2) *at = (uint8_t)code[0];
+        else if constexpr (VEC == 4) *reinterpret_cast<uint16_t*>(at) = (uint16_t)(code[0] | code[2] << 8);
         else {
             uint32_t w[VEC / 8];
 #pragma unroll
-            for (int i = 0; i < VEC / 8; ++i) {
-                w[i] = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[i] |= code[8 * i + e] << (4 * e);
-            }
+            for (int i = 0; i < VEC / 8; ++i) w[i] = code[8 * i] | code[8 * i + 2] << 8 | code[8 * i + 4] << 16 | code[8 * i + 6] << 24;
             store_words(at, w);
         }
     }
     if (lane % LANES == 0) {
-        planes.scales[row * (D / 64) + group] = s16;
-        planes.biases[row * (D / 64) + group] = o16;
+        const size_t at = row * (D / 64) + lane / LANES;
+        planes.scales[at] = s16;
+        planes.biases[at] = o16;
     }
 }
 
-// A block takes one row and up to 8 * HPW of its heads (q heads, then k, then v), a warp HPW of them, VEC = D / 32 consecutive elements per
-// lane. The row's angles are computed once per block and kept in shared memory; a pair's partner is a whole number of lanes away.
-template <int D, bool BF16, int HPW>
-__global__ void __launch_bounds__(kEpilogueThreads)
-qkv_epilogue_kernel(const EpilogueArgs a) {
+// (cos, sin) of a position's turn at one frequency. In turns: the whole ones are dropped in 64 bits, what is left is at most half a turn, where the
+// hardware's sine and cosine are off by 2^-21 at most: a thousandth of an fp16 step of the turned value.
+__device__ __forceinline__ float2 turn_of(int32_t position, float frequency) {
+    const double turns = (double)position * (double)frequency * 0.15915494309189533577;
+    const float x = 6.2831853071795865f * (float)(turns - rint(turns));
+    return make_float2(__cosf(x), __sinf(x));
+}
+
+// Where a row's token lies. state: 0: a row of no sequence, 1: its page is missing, 2: fine.
+struct RowPlace {
+    int state;
+    int32_t page;
+    uint32_t slot;
+};
+__device__ __forceinline__ bool place_row(const EpilogueArgs& a, uint32_t b, uint32_t row, RowPlace& place) {
+    const int64_t begin = a.row_offsets[b], end = a.row_offsets[b + 1];
+    if (row == 0 && (begin < 0 || begin > end || end > (int64_t)a.rows)) *a.error = kErrKvOffsets;
+    if (!(begin <= (int64_t)row && (int64_t)row < end)) return false;
+    const int64_t token = (int64_t)a.context_lengths[b] + ((int64_t)row - begin);
+    place.page = a.context_lengths[b] < 0 ? -1 : a.table.page(b, token);
+    place.slot = (uint32_t)token & ((1u << a.table.page_log2) - 1u);
+    place.state = place.page < 0 ? 1 : 2;
+    if (place.page < 0) *a.error = kErrKvPage;
+    return true;
+}
+
+// Heads of one kind: those of q, k or v.
+struct HeadKind {
+    const uint16_t *source, *weight;                           // of head 0 of the row; nullptr: no weight
+    uint16_t* out;                                             // head 0 of the row, or nullptr
+    KvPlanes cache;
+    uint32_t heads;
+    bool norm, turned, cached;
+};
+__device__ __forceinline__ HeadKind kind_of(const EpilogueArgs& a, int kind, uint32_t row) {
+    HeadKind r;
+    r.source = kind == 0 ? a.q + (size_t)row * a.q_stride : kind == 1 ? a.k + (size_t)row * a.k_stride : a.v + (size_t)row * a.v_stride;
+    r.weight = kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr;
+    r.out = kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out;
+    if (r.out) r.out += (size_t)row * (kind == 0 ? a.q_out_stride : kind == 1 ? a.k_out_stride : a.v_out_stride);
+    r.cache.codes = kind == 2 ? a.v_cache.codes : a.k_cache.codes;
+    r.cache.scales = kind == 2 ? a.v_cache.scales : a.k_cache.scales;
+    r.cache.biases = kind == 2 ? a.v_cache.biases : a.k_cache.biases;
+    r.heads = kind == 0 ? a.q_heads : a.kv_heads;
+    r.norm = kind != 2 || a.norm_v;
+    r.turned = kind != 2 && a.pairs;
+    r.cached = kind != 0 && a.has_cache;
+    return r;
+}
+
+// What a lane's elements y of the normed head become: y[e] * own[e] + partner's y * other[e]; weight and rotation in one. A pair's partner is a whole
+// number of lanes away. turn(j): (cos, sin) of pair j.
+template <int VEC>
+struct HeadTurn {
+    float own[VEC], other[VEC];
+    int from;
+};
+template <int VEC, typename Turn>
+__device__ __forceinline__ void make_turn(HeadTurn<VEC>& t, const uint16_t* weight, uint32_t pairs, int lane, Turn turn) {
+    const int apart = (int)pairs / VEC;                        // lanes between the elements of a pair
+    const bool lower = lane < apart, turned = lane < 2 * apart;
+    t.from = lower ? lane + apart : turned ? lane - apart : lane;
+    uint32_t w[VEC / 2], u[VEC / 2];
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) w[i] = u[i] = 0x3F803F80u;
+    if (weight) {
+        load_words(w, weight + lane * VEC);
+        load_words(u, weight + t.from * VEC);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const float mine = __uint_as_float(e % 2 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16), theirs = __uint_as_float(e % 2 ? u[e / 2] & 0xFFFF0000u : u[e / 2] << 16);
+        t.own[e] = mine;
+        t.other[e] = 0.0f;
+        if (turned) {
+            const float2 cs = turn((lower ? lane : t.from) * VEC + e);
+            t.own[e] = mine * cs.x;
+            t.other[e] = (lower ? -theirs : theirs) * cs.y;
+        }
+    }
+}
+
+// The head's values f times `inv`, weighed, turned and stored, with its row of the cache.
+template <int D, bool BF16>
+__device__ __forceinline__ void finish_head(float (&f)[D / 32], float inv, const HeadKind& kind, const HeadTurn<D / 32>& t, uint32_t h, size_t cache_row, int bits, int lane) {
     constexpr int VEC = D / 32;
-    __shared__ float2 turn[D / 2];                            // (cos, sin) of the row's angles
-    __shared__ int32_t s_page;
-    __shared__ uint32_t s_slot;
-    __shared__ int s_state;                                   // 0: a row of no sequence, 1: its page is missing, 2: fine
-    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    const uint32_t row = blockIdx.x, heads = a.q_heads + 2 * a.kv_heads;
-    const uint32_t first = blockIdx.y * (kEpilogueWarps * HPW) + warp;
-
-    uint32_t x[HPW][VEC / 2];
+    if (kind.norm) {
 #pragma unroll
-    for (int n = 0; n < HPW; ++n) {
-        const uint32_t h = first + n * kEpilogueWarps;
-        if (h >= heads) break;
-        const uint16_t* src = h < a.q_heads ? a.q + (size_t)row * a.q_stride + (size_t)h * D
-                              : h < a.q_heads + a.kv_heads ? a.k + (size_t)row * a.k_stride + (size_t)(h - a.q_heads) * D
-                                                           : a.v + (size_t)row * a.v_stride + (size_t)(h - a.q_heads - a.kv_heads) * D;
-        load_words(x[n], src + lane * VEC);
+        for (int e = 0; e < VEC; ++e) f[e] *= inv;
     }
-    if (threadIdx.x == 0) s_state = a.has_cache ? 0 : 2;
-    __syncthreads();
-    if (a.has_cache) {
-        for (uint32_t b = threadIdx.x; b < a.sequences; b += kEpilogueThreads) {
-            const int64_t begin = a.row_offsets[b], end = a.row_offsets[b + 1];
-            if (begin <= (int64_t)row && (int64_t)row < end) {
-                const int64_t token = (int64_t)a.context_lengths[b] + ((int64_t)row - begin);
-                const int32_t page = a.context_lengths[b] < 0 ? -1 : a.table.page(b, token);
-                s_page = page;
-                s_slot = (uint32_t)token & ((1u << a.table.page_log2) - 1u);
-                s_state = page < 0 ? 1 : 2;
-                if (page < 0) *a.error = kErrKvPage;
-            }
-            if (row == 0 && (begin < 0 || begin > end || end > (int64_t)a.rows)) *a.error = kErrKvOffsets;
-        }
+    if (kind.turned) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = fmaf(__shfl_sync(kFullMask, f[e], t.from), t.other[e], f[e] * t.own[e]);
+    } else if (kind.weight) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] *= t.own[e];
     }
-    for (uint32_t j = threadIdx.x; j < a.pairs; j += kEpilogueThreads) {
-        // in turns: the whole ones are dropped in 64 bits, what is left is at most half a turn
-        const double turns = (double)a.positions[row] * (double)a.frequencies[j] * 0.15915494309189533577;
-        float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        turn[j] = make_float2(c, s);
-    }
-    __syncthreads();
-    if (s_state == 0) return;
-
-#pragma unroll
-    for (int n = 0; n < HPW; ++n) {
-        const uint32_t h = first + n * kEpilogueWarps;
-        if (h >= heads) break;
-        const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
-        float f[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
-            const float2 t = pair_to_float<BF16>(x[n][i]);
-            f[2 * i] = t.x;
-            f[2 * i + 1] = t.y;
-        }
-        if (!is_v || a.norm_v) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) sum = fmaf(f[e], f[e], sum);
-            const float inv = rsqrtf(warp_sum(sum) / (float)D + a.eps);
-            const uint16_t* weight = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
-            uint32_t w[VEC / 2];
-            if (weight) load_words(w, weight + lane * VEC);
-#pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-                f[2 * i] *= inv;
-                f[2 * i + 1] *= inv;
-                if (weight) {
-                    f[2 * i] *= bf16_bits_to_float((uint16_t)w[i]);
-                    f[2 * i + 1] *= bf16_bits_to_float((uint16_t)(w[i] >> 16));
-                }
-            }
-        }
-        if (!is_v && a.pairs) {
-            const int apart = (int)a.pairs / VEC;              // lanes between the elements of a pair
-            const bool lower = lane < apart, turned = lane < 2 * apart;
-            const int from = lower ? lane + apart : turned ? lane - apart : lane;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float other = __shfl_sync(kFullMask, f[e], from);
-                if (turned) {
-                    const float2 t = turn[(lower ? lane : from) * VEC + e];
-                    f[e] = lower ? fmaf(-other, t.y, f[e] * t.x) : fmaf(other, t.y, f[e] * t.x);
-                }
-            }
-        }
+    if (kind.out) {
         uint32_t y[VEC / 2];
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) y[i] = float_to_pair<BF16>(f[2 * i], f[2 * i + 1]);
-        if (is_q) {
-            store_words(a.q_out + (size_t)row * a.q_out_stride + (size_t)h * D + lane * VEC, y);
-            continue;
-        }
-        const uint32_t kv = is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
-        uint16_t* out = is_v ? a.v_out : a.k_out;
-        if (out) store_words(out + (size_t)row * (is_v ? a.v_out_stride : a.k_out_stride) + (size_t)kv * D + lane * VEC, y);
-        if (a.has_cache && s_state == 2)
-            quantise_head<D>(f, is_v ? a.v_cache : a.k_cache, (((size_t)s_page * a.kv_heads + kv) << a.table.page_log2) + s_slot, a.bits, lane);
+        store_words(kind.out + (size_t)h * D + lane * VEC, y);
     }
+    if (kind.cached) quantise_head<D>(f, kind.cache, cache_row, bits, lane);
+}
+
+template <int D, bool BF16>
+__device__ __forceinline__ float unpack_head(float (&f)[D / 32], const uint32_t (&x)[D / 64]) {      // and this lane's sum of squares
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const float2 t = pair_to_float<BF16>(x[i]);
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+        sum = fmaf(t.x, t.x, sum);
+        sum = fmaf(t.y, t.y, sum);
+    }
+    return sum;
+}
+
+// Heads [first, last) of one kind of a row, by one warp, VEC = D / 32 consecutive elements of a head per lane. BATCH heads are requested while BATCH are
+// worked on; their sums of squares are added up together: at each of the first steps a lane hands on the half of the heads that it does not keep.
+template <int D, bool BF16, int BATCH, typename Place, typename Turn>
+__device__ __forceinline__ void epilogue_heads(const EpilogueArgs& a, HeadKind& kind, uint32_t first, uint32_t last, int lane, Place find_place, Turn turn) {
+    constexpr int VEC = D / 32;
+    uint32_t x[BATCH][VEC / 2];
+#pragma unroll
+    for (int n = 0; n < BATCH; ++n) load_words(x[n], kind.source + (size_t)min(first + n, last - 1) * D + lane * VEC);
+    const RowPlace place = find_place();
+    if (place.state == 0) return;
+    if (place.state == 1) kind.cached = false;
+    HeadTurn<VEC> t;
+    make_turn<VEC>(t, kind.weight, kind.turned ? a.pairs : 0, lane, turn);
+#pragma unroll 1
+    for (uint32_t h0 = first; h0 < last; h0 += BATCH) {
+        float f[BATCH][VEC], sum[BATCH];
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) sum[n] = unpack_head<D, BF16>(f[n], x[n]);
+        if (BATCH > 1) {
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) load_words(x[n], kind.source + (size_t)min(h0 + BATCH + n, last - 1) * D + lane * VEC);
+        }
+        int off = 16;
+#pragma unroll
+        for (int left = BATCH / 2; left >= 1; left /= 2, off /= 2)
+#pragma unroll
+            for (int n = 0; n < left; ++n) {
+                const bool upper = lane & off;                 // keeps the upper heads
+                sum[n] = __fadd_rn(upper ? sum[n + left] : sum[n], __shfl_xor_sync(kFullMask, upper ? sum[n] : sum[n + left], off));
+            }
+#pragma unroll
+        for (int o = 16 / BATCH; o >= 1; o /= 2) sum[0] = __fadd_rn(sum[0], __shfl_xor_sync(kFullMask, sum[0], o));
+        const float inv = rsqrtf(fmaf(sum[0], 1.0f / (float)D, a.eps));
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            const float mine = BATCH == 1 ? inv : __shfl_sync(kFullMask, inv, n * (kWarp / BATCH));       // a lane's highest bit is its head's highest
+            if (h0 + n < last)
+                finish_head<D, BF16>(f[n], mine, kind, t, h0 + n, (((size_t)place.page * a.kv_heads + h0 + n) << a.table.page_log2) + place.slot, a.bits, lane);
+        }
+    }
+}
+
+// Few rows: a block takes one row and eight of its heads (q heads, then k, then v), a warp per head. The row's place and angles are found once per block.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kEpilogueThreads)
+qkv_epilogue_kernel(const EpilogueArgs a) {
+    __shared__ float2 s_turn[D / 2];                          // (cos, sin) of the row's angles
+    __shared__ RowPlace s_place;
+    const uint32_t row = blockIdx.x;
+    uint32_t h = min(blockIdx.y * kEpilogueWarps + threadIdx.x / kWarp, a.q_heads + 2 * a.kv_heads - 1);       // the last head may be done twice
+    int which = 0;
+    if (h >= a.q_heads) { which = 1; h -= a.q_heads; }
+    if (which && h >= a.kv_heads) { which = 2; h -= a.kv_heads; }
+    HeadKind kind = kind_of(a, which, row);
+    epilogue_heads<D, BF16, 1>(a, kind, h, h + 1, threadIdx.x % kWarp, [&]() {
+        if (threadIdx.x == 0) s_place = {a.has_cache ? 0 : 2, 0, 0};
+        __syncthreads();
+        if (a.has_cache)
+            for (uint32_t b = threadIdx.x; b < a.sequences; b += kEpilogueThreads) {
+                RowPlace p;
+                if (place_row(a, b, row, p)) s_place = p;
+            }
+        for (uint32_t j = threadIdx.x; j < a.pairs; j += kEpilogueThreads) s_turn[j] = turn_of(a.positions[row], a.frequencies[j]);
+        __syncthreads();
+        return s_place; }, [&](int j) { return s_turn[j]; });
+}
+
+// Many rows: a block takes eight rows and up to eight heads of one kind, a warp per row. So the kind is known to the whole block (its branches and
+// addresses cost no lane's instructions), weights and angles of a lane's elements stay in registers, and no warp waits for another.
+constexpr uint32_t kBlockHeads = 8;
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kEpilogueThreads, D == 512 ? 2 : 3)
+qkv_epilogue_rows_kernel(const EpilogueArgs a) {
+    const int lane = threadIdx.x % kWarp;
+    const uint32_t q_chunks = (a.q_heads + kBlockHeads - 1) / kBlockHeads, kv_chunks = (a.kv_heads + kBlockHeads - 1) / kBlockHeads;
+    const uint32_t group = blockIdx.x / (q_chunks + 2 * kv_chunks), row = group * kEpilogueWarps + threadIdx.x / kWarp;
+    uint32_t chunk = blockIdx.x - group * (q_chunks + 2 * kv_chunks);
+    if (row >= a.rows) return;
+    int which = 0;
+    if (chunk >= q_chunks) { which = 1; chunk -= q_chunks; }
+    if (which && chunk >= kv_chunks) { which = 2; chunk -= kv_chunks; }
+    HeadKind kind = kind_of(a, which, row);
+    const uint32_t first = chunk * kBlockHeads;
+    const int32_t position = kind.turned ? a.positions[row] : 0;
+    epilogue_heads<D, BF16, D == 512 ? 2 : 4>(a, kind, first, min(first + kBlockHeads, kind.heads), lane, [&]() {
+        RowPlace place = {a.has_cache ? 0 : 2, 0, 0};
+        if (a.has_cache)
+            for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWarp) {
+                RowPlace p = {0, 0, 0};
+                const bool mine = b0 + lane < a.sequences && place_row(a, b0 + lane, row, p);
+                const uint32_t owner = __ballot_sync(kFullMask, mine);
+                if (owner) {
+                    const int from = __ffs(owner) - 1;
+                    place.state = __shfl_sync(kFullMask, p.state, from);
+                    place.page = __shfl_sync(kFullMask, p.page, from);
+                    place.slot = __shfl_sync(kFullMask, p.slot, from);
+                    if (row != 0) break;                       // the first row's warps look at all offsets
+                }
+            }
+        return place; }, [&](int j) { return turn_of(position, a.frequencies[j]); });
+}
+
+static uint64_t row_blocks(uint32_t rows, uint32_t q_heads, uint32_t kv_heads) {
+    return ((uint64_t)rows + kEpilogueWarps - 1) / kEpilogueWarps * (((uint64_t)q_heads + kBlockHeads - 1) / kBlockHeads + 2 * (((uint64_t)kv_heads + kBlockHeads - 1) / kBlockHeads));
 }
 
 template <int D, bool BF16>
 static void launch_epilogue(cudaStream_t st, const EpilogueArgs& a, uint32_t rows) {
     const uint32_t heads = a.q_heads + 2 * a.kv_heads;
-    // One head per warp while that leaves few blocks: a lone row's heads go through side by side. With four the angles are computed
-    // for four times as many heads.
-    if ((uint64_t)rows * ((heads + 7) / 8) <= 1184) qkv_epilogue_kernel<D, BF16, 1><<<dim3(rows, (heads + 7) / 8), kEpilogueThreads, 0, st>>>(a);
-    else qkv_epilogue_kernel<D, BF16, 4><<<dim3(rows, (heads + 31) / 32), kEpilogueThreads, 0, st>>>(a);
+    // A warp per head while those are few: a lone row's heads go through side by side.
+    if ((uint64_t)rows * ((heads + 7) / 8) <= 592) qkv_epilogue_kernel<D, BF16><<<dim3(rows, (heads + 7) / 8), kEpilogueThreads, 0, st>>>(a);
+    else qkv_epilogue_rows_kernel<D, BF16><<<(uint32_t)row_blocks(rows, a.q_heads, a.kv_heads), kEpilogueThreads, 0, st>>>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -270,10 +390,10 @@ struct ReadArgs {
     const int32_t *row_offsets, *context_lengths;
     KvTable table;
     uint32_t* error;
-    uint32_t sequences, rows, kv_heads, head_dim;
+    uint32_t sequences, rows, kv_heads, head_log2;
 };
 
-// A block takes eight rows; its warps find the rows' tokens, then every thread turns eight codes at a time into one 16-byte store.
+// A block takes eight rows of keys or values; its warps find the rows' tokens, then every thread turns eight codes at a time into one 16-byte store.
 template <int BITS, bool BF16>
 __global__ void __launch_bounds__(kReadThreads)
 kv_cache_read_kernel(const ReadArgs a) {
@@ -296,33 +416,48 @@ kv_cache_read_kernel(const ReadArgs a) {
         if (row == 0 && (begin < 0 || begin > end || end > (int64_t)a.rows)) *a.error = kErrKvOffsets;
     }
     __syncthreads();
-    const uint32_t per_head = a.head_dim / 8, per_row = a.kv_heads * per_head, groups = a.head_dim / 64;
     const int kv = blockIdx.y;                                 // keys or values
     if (!a.out[kv]) return;
     const KvPlanes p = a.planes[kv];
-    const uint32_t total = per_row * kReadRows;
-    for (uint32_t i = threadIdx.x; i < total; i += kReadThreads) {
-        const uint32_t r = i / per_row, c = i - r * per_row, h = c / per_head, e = c - h * per_head;
-        const int32_t page = s_page[r];
-        if (page < 0) continue;
-        const size_t at = (((size_t)page * a.kv_heads + h) << a.table.page_log2) + s_slot[r];
-        const float scale = bf16_bits_to_float(p.scales[at * groups + e / 8]), bias = bf16_bits_to_float(p.biases[at * groups + e / 8]);
-        uint32_t y[4];
-        if constexpr (BITS == 8) {
-            uint32_t w[2];
-            load_words(w, p.codes + at * a.head_dim + e * 8);
+    const uint32_t per_head_log2 = a.head_log2 - 3, per_row = a.kv_heads << per_head_log2, groups_log2 = a.head_log2 - 6;
+    // Eight values a time; a thread's next place is a fixed number of rows and values on. Four places are requested before the first is stored.
+    uint32_t r = threadIdx.x / per_row, c = threadIdx.x % per_row;
+    const uint32_t step_r = kReadThreads / per_row, step_c = kReadThreads % per_row;
+    constexpr int BATCH = 4;
+    while (r < kReadRows) {
+        uint32_t w[BATCH][BITS / 4], rr[BATCH], cc[BATCH];
+        uint16_t s16[BATCH], o16[BATCH];
+        bool is[BATCH];
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            rr[n] = r;
+            cc[n] = c;
+            is[n] = r < kReadRows && s_page[r] >= 0;
+            if (is[n]) {
+                const uint32_t h = c >> per_head_log2, e = c & ((1u << per_head_log2) - 1u);
+                const size_t at = (((size_t)s_page[r] * a.kv_heads + h) << a.table.page_log2) + s_slot[r];
+                load_words(w[n], p.codes + (at << a.head_log2) * BITS / 8 + e * BITS);
+                s16[n] = p.scales[(at << groups_log2) + e / 8];
+                o16[n] = p.biases[(at << groups_log2) + e / 8];
+            }
+            r += step_r;
+            c += step_c;
+            if (c >= per_row) { c -= per_row; ++r; }
+        }
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            if (!is[n]) continue;
+            const float scale = bf16_bits_to_float(s16[n]), bias = bf16_bits_to_float(o16[n]);
+            uint32_t y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t v = w[j / 2] >> (16 * (j % 2));
-                y[j] = float_to_pair<BF16>(fmaf((float)(v & 255u), scale, bias), fmaf((float)(v >> 8 & 255u), scale, bias));
+                uint32_t c0, c1;
+                if constexpr (BITS == 8) { c0 = w[n][j / 2] >> (16 * (j % 2)) & 255u; c1 = w[n][j / 2] >> (16 * (j % 2) + 8) & 255u; }
+                else { c0 = w[n][0] >> (8 * j) & 15u; c1 = w[n][0] >> (8 * j + 4) & 15u; }
+                y[j] = float_to_pair<BF16>(fmaf((float)c0, scale, bias), fmaf((float)c1, scale, bias));
             }
-        } else {
-            const uint32_t v = *reinterpret_cast<const uint32_t*>(p.codes + at * (a.head_dim / 2) + e * 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                y[j] = float_to_pair<BF16>(fmaf((float)(v >> (8 * j) & 15u), scale, bias), fmaf((float)(v >> (8 * j + 4) & 15u), scale, bias));
+            store_words(a.out[kv] + (size_t)(row0 + rr[n]) * a.out_stride[kv] + (size_t)cc[n] * 8, y);
         }
-        store_words(a.out[kv] + (size_t)(row0 + r) * a.out_stride[kv] + (size_t)c * 8, y);
     }
 }
 
@@ -373,6 +508,7 @@ tf_status tf_qkv_epilogue(tf_context* ctx, void* stream, const void* q, uint32_t
     TF_REQUIRE(ctx, eps >= 0.0f && eps <= 3.4e38f, TF_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", name);
     if (batch->rows == 0 || (cache && batch->sequences == 0)) return TF_OK;
     TF_REQUIRE(ctx, batch->rows <= 0x7FFFFFFFu, TF_ERR_INVALID_ARGUMENT, "%s: rows must be below 2^31", name);
+    TF_REQUIRE(ctx, tf::row_blocks(batch->rows, q_heads, kv_heads) <= 0x7FFFFFFFu, TF_ERR_UNSUPPORTED, "%s: too many rows for the number of heads", name);
     tf::EpilogueArgs a = {};
     a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
     a.q_weight = static_cast<const uint16_t*>(q_weight); a.k_weight = static_cast<const uint16_t*>(k_weight);
@@ -426,7 +562,7 @@ tf_status tf_kv_cache_read(tf_context* ctx, void* stream, const tf_kv_cache* cac
     a.row_offsets = batch->row_offsets; a.context_lengths = batch->context_lengths;
     a.table = tf::table_of(cache, batch);
     a.error = ctx->device_error;
-    a.sequences = batch->sequences; a.rows = batch->rows; a.kv_heads = cache->kv_heads; a.head_dim = cache->head_dim;
+    a.sequences = batch->sequences; a.rows = batch->rows; a.kv_heads = cache->kv_heads; a.head_log2 = tf::log2_of(cache->head_dim);
     const tf::DeviceScope scope(ctx->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const dim3 grid((batch->rows + tf::kReadRows - 1) / tf::kReadRows, 2);
