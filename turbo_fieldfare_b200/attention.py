@@ -45,12 +45,27 @@ def _check(name: str, t, device, dtypes, dims: int, contiguous: bool = True):
 
 def _row_stride(name: str, t, device, dtype, rows: int, cols: int) -> int:
     """Stride of a two-dimensional tensor of rows; columns are next to one another."""
+    try:                                                       # the common case first: what follows costs microseconds a call
+        if t.dtype is dtype and t.get_device() == device.index:
+            have, width = t.shape
+            stride, step = t.stride()
+            if have >= rows and width == cols and step == 1:
+                return stride if have > 1 or stride > cols else cols
+    except (AttributeError, ValueError):
+        pass
     _check(name, t, device, (dtype,), 2, contiguous=False)
     if t.shape[0] < rows or t.shape[1] != cols:
         raise ValueError(f"{name} must be [>= {rows}, {cols}], got {tuple(t.shape)}")
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the columns of a row must be next to one another")
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), cols)
+
+
+def _vector(name: str, t, device, dtype) -> int:
+    """Length of a contiguous one-dimensional tensor."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 1 and t.get_device() == device.index and t.is_contiguous()):
+        _check(name, t, device, (dtype,), 1)
+    return t.shape[0]
 
 
 class KVCache:
@@ -72,6 +87,7 @@ class KVCache:
             if t.shape[:3] != k_scales.shape[:3] or t.shape[3] not in ((width,) if t.dtype == torch.uint8 else (groups,)):
                 raise ValueError(f"cache planes disagree: {[tuple(p.shape) for p in self.planes]}")
         self._c = KVCacheDesc(*[_ptr(t) for t in self.planes], pages, page_size, heads, self.head_dim, self.bits)
+        self._ref, self._index = C.byref(self._c), k_codes.get_device()
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int, device="cuda") -> "KVCache":
@@ -110,6 +126,7 @@ class KVBatch:
             raise ValueError(f"{rows} rows need as many positions")
         self.row_offsets, self.context_lengths, self.page_table, self.positions, self.rows = row_offsets, context_lengths, page_table, positions, rows
         self._c = KVBatchDesc(_ptr(row_offsets), _ptr(context_lengths), _ptr(page_table), _ptr(positions), page_table.shape[1], self.sequences, rows)
+        self._ref, self._index = C.byref(self._c), row_offsets.get_device()
 
 
 class AttentionWorkspace:
@@ -139,7 +156,7 @@ class AttentionWorkspace:
 
 def _same_device(context: TurboContext, *parts):
     for p in parts:
-        if p is not None and (p.device.type != "cuda" or p.device.index != context.device):
+        if p is not None and p._index != context.device:
             raise ValueError(f"{type(p).__name__} is on {p.device}, the context on cuda:{context.device}")
 
 
@@ -158,22 +175,21 @@ class FusedQKVEpilogue:
         device, dtype, rows = batch.device, q.dtype, batch.rows
         if dtype not in _ACT:
             raise ValueError(f"rows are float16 or bfloat16, not {dtype}")
-        if q.dim() != 2 or k.dim() != 2 or head_dim <= 0 or q.shape[1] % head_dim or k.shape[1] % head_dim:
+        q_cols, kv_cols = q.shape[-1], k.shape[-1]
+        if q.dim() != 2 or k.dim() != 2 or head_dim <= 0 or q_cols % head_dim or kv_cols % head_dim:
             raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} are not rows of heads of {head_dim}")
-        q_cols, kv_cols = q.shape[1], k.shape[1]
-        strides = [_row_stride(n, t, device, dtype, rows, c) if t is not None else 0
-                   for n, t, c in (("q", q, q_cols), ("k", k, kv_cols), ("v", v, kv_cols), ("q_out", q_out, q_cols), ("k_out", k_out, kv_cols), ("v_out", v_out, kv_cols))]
+        q_stride, q_out_stride = _row_stride("q", q, device, dtype, rows, q_cols), _row_stride("q_out", q_out, device, dtype, rows, q_cols)
+        k_stride, v_stride = _row_stride("k", k, device, dtype, rows, kv_cols), _row_stride("v", v, device, dtype, rows, kv_cols)
+        k_out_stride = 0 if k_out is None else _row_stride("k_out", k_out, device, dtype, rows, kv_cols)
+        v_out_stride = 0 if v_out is None else _row_stride("v_out", v_out, device, dtype, rows, kv_cols)
         for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None:
-                _check(n, w, device, (torch.bfloat16,), 1)
-                if w.shape[0] != head_dim:
-                    raise ValueError(f"{n} has {w.shape[0]} elements, not {head_dim}")
-        if frequencies is not None:
-            _check("frequencies", frequencies, device, (torch.float32,), 1)
+            if w is not None and _vector(n, w, device, torch.bfloat16) != head_dim:
+                raise ValueError(f"{n} has {w.shape[0]} elements, not {head_dim}")
+        pairs = 0 if frequencies is None else _vector("frequencies", frequencies, device, torch.float32)
         ctx.check(ctx.lib.tf_qkv_epilogue(
-            ctx.handle, _stream_of(ctx, stream), _ptr(q), strides[0], _ptr(k), strides[1], _ptr(v), strides[2], _ptr(q_weight), _ptr(k_weight),
-            1 if norm_v else 0, _ptr(frequencies), 0 if frequencies is None else frequencies.shape[0], eps, _ptr(q_out), strides[3],
-            _ptr(k_out), strides[4], _ptr(v_out), strides[5], C.byref(batch._c), None if cache is None else C.byref(cache._c),
+            ctx.handle, _stream_of(ctx, stream), q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, _ptr(q_weight), _ptr(k_weight),
+            1 if norm_v else 0, _ptr(frequencies), pairs, eps, q_out.data_ptr(), q_out_stride,
+            _ptr(k_out), k_out_stride, _ptr(v_out), v_out_stride, batch._ref, None if cache is None else cache._ref,
             q_cols // head_dim, kv_cols // head_dim, head_dim, _ACT[dtype]))
 
 
@@ -191,9 +207,10 @@ class KVCacheRead:
         if out is None or out.dtype not in _ACT:
             raise ValueError("a read needs k_out or v_out, of float16 or bfloat16")
         cols = cache.kv_heads * cache.head_dim
-        strides = [_row_stride(n, t, batch.device, out.dtype, batch.rows, cols) if t is not None else 0 for n, t in (("k_out", k_out), ("v_out", v_out))]
-        ctx.check(ctx.lib.tf_kv_cache_read(ctx.handle, _stream_of(ctx, stream), C.byref(cache._c), C.byref(batch._c), _ptr(k_out), strides[0],
-                                           _ptr(v_out), strides[1], _ACT[out.dtype]))
+        k_stride = 0 if k_out is None else _row_stride("k_out", k_out, batch.device, out.dtype, batch.rows, cols)
+        v_stride = 0 if v_out is None else _row_stride("v_out", v_out, batch.device, out.dtype, batch.rows, cols)
+        ctx.check(ctx.lib.tf_kv_cache_read(ctx.handle, _stream_of(ctx, stream), cache._ref, batch._ref, _ptr(k_out), k_stride, _ptr(v_out), v_stride,
+                                           _ACT[out.dtype]))
 
 
 class TreeAttention:
@@ -213,7 +230,8 @@ class TreeAttention:
             raise ValueError(f"rows are float16 or bfloat16, not {q.dtype}")
         if q.dim() != 2 or q.shape[1] % cache.head_dim:
             raise ValueError(f"q {tuple(q.shape)} is not rows of heads of {cache.head_dim}")
-        strides = [_row_stride(n, t, batch.device, q.dtype, batch.rows, q.shape[1]) for n, t in (("q", q), ("out", out))]
+        cols = q.shape[1]
+        q_stride, out_stride = _row_stride("q", q, batch.device, q.dtype, batch.rows, cols), _row_stride("out", out, batch.device, q.dtype, batch.rows, cols)
         words = 0
         if tree_mask is not None:
             _check("tree_mask", tree_mask, batch.device, (torch.int64,), 2)
@@ -222,6 +240,6 @@ class TreeAttention:
                 raise ValueError(f"tree_mask has {tree_mask.shape[0]} rows, the batch {batch.rows}")
         if window < 0:
             raise ValueError("window must not be negative")
-        ctx.check(ctx.lib.tf_tree_attention(ctx.handle, _stream_of(ctx, stream), _ptr(q), strides[0], _ptr(out), strides[1], C.byref(cache._c),
-                                            C.byref(batch._c), _ptr(tree_mask), words, window, scale, q.shape[1] // cache.head_dim, _ACT[q.dtype],
+        ctx.check(ctx.lib.tf_tree_attention(ctx.handle, _stream_of(ctx, stream), q.data_ptr(), q_stride, out.data_ptr(), out_stride, cache._ref,
+                                            batch._ref, _ptr(tree_mask), words, window, scale, cols // cache.head_dim, _ACT[q.dtype],
                                             workspace.handle))

@@ -334,7 +334,7 @@ qkv_epilogue_kernel(const EpilogueArgs a) {
 // addresses cost no lane's instructions), weights and angles of a lane's elements stay in registers, and no warp waits for another.
 constexpr uint32_t kBlockHeads = 8;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kEpilogueThreads, D == 512 ? 2 : 3)
+__global__ void __launch_bounds__(kEpilogueThreads, D == 512 ? 2 : 4)
 qkv_epilogue_rows_kernel(const EpilogueArgs a) {
     const int lane = threadIdx.x % kWarp;
     const uint32_t q_chunks = (a.q_heads + kBlockHeads - 1) / kBlockHeads, kv_chunks = (a.kv_heads + kBlockHeads - 1) / kBlockHeads;
@@ -347,7 +347,7 @@ qkv_epilogue_rows_kernel(const EpilogueArgs a) {
     HeadKind kind = kind_of(a, which, row);
     const uint32_t first = chunk * kBlockHeads;
     const int32_t position = kind.turned ? a.positions[row] : 0;
-    epilogue_heads<D, BF16, D == 512 ? 2 : 4>(a, kind, first, min(first + kBlockHeads, kind.heads), lane, [&]() {
+    epilogue_heads<D, BF16, 2>(a, kind, first, min(first + kBlockHeads, kind.heads), lane, [&]() {
         RowPlace place = {a.has_cache ? 0 : 2, 0, 0};
         if (a.has_cache)
             for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWarp) {
