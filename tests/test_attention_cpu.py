@@ -152,8 +152,8 @@ static void tile_places() {
             }
     }
     // every piece of a tile belongs to one thread's turn
-    CHECK(S::UNPACK % S::K_ROW == 0 && S::UNPACK % S::V_ROW == 0 && sizeof(TilesMeta<S::TILE, S::UNPACK_WARPS>) <= S::META);
-    CHECK(S::OFF_K % 1024 == 0 && S::OFF_V % 1024 == 0 && S::OFF_META % 16 == 0 && S::K_BYTES % 1024 == 0 && S::V_BYTES % 1024 == 0 && S::SMEM <= 227 * 1024);
+    CHECK(S::UNPACK % S::K_ROW == 0 && S::UNPACK % S::V_ROW == 0 && S::K_EACH * S::UNPACK == S::TILE * S::K_ROW && sizeof(TilesMeta<S::TILE>) <= S::META);
+    CHECK(S::OFF_K % 1024 == 0 && S::OFF_V % 1024 == 0 && S::OFF_META % 16 == 0 && S::OFF_KC % 16 == 0 && S::OFF_VC % 16 == 0 && S::OFF_PL % 16 == 0 && S::OFF_KW % 16 == 0 && S::OFF_VW % 16 == 0 && S::K_BYTES % 1024 == 0 && S::V_BYTES % 1024 == 0 && S::SMEM <= 227 * 1024);
 }
 template <int D, int BITS, int RB>
 static void rows_places() {

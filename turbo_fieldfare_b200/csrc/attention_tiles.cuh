@@ -22,12 +22,12 @@
 namespace tf {
 
 constexpr uint32_t kErrAttentionWait = 0x7F000053u;           // a bounded wait of attention_tiles_kernel ran out
-constexpr uint32_t kLooks = 1u << 18;                         // looks of a bounded wait
+constexpr uint32_t kLooks = 1u << 22;                         // looks of a bounded wait
 
 template <int D, int BITS>
 struct TilesShape {
     static constexpr int MT = 128, TILE = D == 512 ? 32 : D == 256 ? 64 : 128, DV = D < 256 ? D : 256, PARTS = D / DV, G = D / 64, GV = DV / 64;
-    static constexpr int SOFT_WARPS = 8, UNPACK_WARPS = 8, WARPS = SOFT_WARPS + UNPACK_WARPS + 1, THREADS = WARPS * kWarp, UNPACK = UNPACK_WARPS * kWarp;
+    static constexpr int SOFT_WARPS = 8, UNPACK_WARPS = 8, MEASURE = SOFT_WARPS + UNPACK_WARPS, LOADER = MEASURE + 2, WARPS = LOADER + 2, THREADS = WARPS * kWarp, UNPACK = UNPACK_WARPS * kWarp;
     static constexpr int ROW_BYTES = D * BITS / 8, PIECE = 2 * BITS;          // bytes of 16 codes
     static constexpr int K_ROW = D / 16, V_ROW = DV / 16;                     // pieces of a token
     static constexpr int K_EACH = TILE * K_ROW / UNPACK, V_EACH = TILE * V_ROW / UNPACK;
@@ -35,11 +35,12 @@ struct TilesShape {
     static constexpr int Q_BYTES = MT * D * 2, K_BYTES = TILE * D * 2, V_BYTES = TILE * DV * 2;
     static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + K_BUFS * K_BYTES;
     static constexpr int CHUNK = TILE / 2 < 32 ? TILE / 2 : 32;                // logits that a softmax thread has in registers at a time, of its half of a tile
-    // what the unpacking warps have requested: codes [piece][thread]; planes of four tiles [token][4]; pages of two
-    static constexpr int PLANES = 2 * G < 4 ? 4 : 2 * G;                      // bytes of a token's plane, or of two tokens' with one group
-    static constexpr int OFF_KC = OFF_V + V_BYTES, OFF_VC = OFF_KC + K_EACH * UNPACK * PIECE, OFF_PL = OFF_VC + V_EACH * UNPACK * PIECE,
-                         OFF_PG = OFF_PL + 4 * TILE * 4 * PLANES, OFF_META = OFF_PG + 2 * TILE * 4;
-    static constexpr int META = (512 + 4 * UNPACK_WARPS * 5 + 4 * TILE * 9 + TILE + 127) / 128 * 128 + 2 * MT * 8 + MT * 4, SMEM = OFF_META + META + 1024;
+    // what the loader has requested: codes and planes as they lie in the cache; and what it made of the planes, of four tiles [token][groups]
+    static constexpr int KC_BUFS = TILE * ROW_BYTES > 8192 ? 1 : 2, V_ROW_BYTES = DV * BITS / 8;
+    static constexpr int KC_BYTES = TILE * ROW_BYTES, VC_BYTES = TILE * V_ROW_BYTES, PLANE = TILE * G * 2;
+    static constexpr int OFF_KC = OFF_V + V_BYTES, OFF_VC = OFF_KC + KC_BUFS * KC_BYTES, OFF_PL = OFF_VC + VC_BYTES, OFF_KW = OFF_PL + 2 * 4 * PLANE,
+                         OFF_VW = OFF_KW + 4 * TILE * G * 4, OFF_META = OFF_VW + 4 * TILE * GV * 4;
+    static constexpr int META = (28 * 8 + 224 + 8 * TILE * 9 + 127) / 128 * 128 + 2 * MT * 8 + MT * 4, SMEM = OFF_META + META + 1024;
     // tensor memory, in columns
     static constexpr int COL_S = 0, COL_P = 2 * TILE, COL_O = 3 * TILE, COLS = 512;
     static_assert(COL_O + DV <= COLS && SMEM <= 227 * 1024 && K_EACH * UNPACK == TILE * K_ROW && V_EACH * UNPACK == TILE * V_ROW, "sizes");
@@ -49,17 +50,17 @@ struct TilesShape {
     }
 };
 
-// What the unpacking warps tell the softmax about tiles (four of them), and the block's barriers.
-template <int TILE, int WARPS>
+// The block's barriers, what the loader tells about a tile whose planes are there, and what the measuring warps tell the softmax (of eight tiles).
+template <int TILE>
 struct TilesMeta {
-    unsigned long long bars[14];
+    unsigned long long bars[28];
     uint32_t tmem, dead;
-    alignas(16) uint8_t flags[4][WARPS];      // per unpacking warp: something in `bad`
-    alignas(16) float v_most[4][WARPS];       // per unpacking warp: the largest of v_up
-    alignas(16) float k_up[4][TILE];          // what a token's logits are multiplied with: its power of two, the scale, log2 e
-    alignas(16) float v_up[4][TILE];          // a token's power of two
-    uint8_t bad[4][TILE];          // bit g: value planes of group g are not finite; bit 7: the token's page is missing
-    int8_t e_k[TILE];              // exponent of the power of two of K, where it is not zero for all of a warp's
+    uint32_t flags[8][2];          // K's and V's: 1: powers of two that are not 1; 2: something in `bad`
+    float v_most[8];               // the largest of v_up
+    alignas(16) uint4 tile[4];     // first token, end of what is seen, the runs that have a page, first value group
+    alignas(16) float k_up[8][TILE];          // what a token's logits are multiplied with: its power of two, the scale, log2 e
+    alignas(16) float v_up[8][TILE];          // a token's power of two
+    uint8_t bad[8][TILE];          // bit g: value planes of group g are not finite; bit 7: the token's page is missing
     float pair[2][128][2];         // between the two softmax threads of a row, by turns
     float q_up[128];               // a row's power of two
 };
@@ -115,8 +116,7 @@ __device__ __forceinline__ void tiles_fence_after() { asm volatile("tcgen05.fenc
 // Sixteen codes as (code - centre) s + b in fp16, two 16-byte chunks of eight elements. 4-bit codes of eight elements come in the order
 // (0, 4, 1, 5, 2, 6, 3, 7), as one mask yields them: the rows of q are laid out alike, and the product's columns are put back at the end.
 template <int BITS>
-__device__ __forceinline__ void tiles_unpack(const uint32_t (&w)[BITS / 2], float scale, float bias, uint4 (&out)[2]) {
-    const __half2 s = __float2half2_rn(scale), b = __float2half2_rn(bias);
+__device__ __forceinline__ void tiles_unpack(const uint32_t (&w)[BITS / 2], __half2 s, __half2 b, uint4 (&out)[2]) {
     uint32_t h[8];
     auto put = [&](int i, uint32_t bits, float off, __half2 by) {
         const __half2 v = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(off)), by, b);
@@ -129,7 +129,7 @@ __device__ __forceinline__ void tiles_unpack(const uint32_t (&w)[BITS / 2], floa
             put(2 * i + 1, gm_prmt(w[i], 0x64646464u, 0x4342), -1152.0f, s);
         }
     } else {
-        const __half2 s16 = __float2half2_rn(scale * 0.0625f);
+        const __half2 s16 = __hmul2(s, __float2half2_rn(0.0625f));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t v = w[i] >> 8;
@@ -143,11 +143,21 @@ __device__ __forceinline__ void tiles_unpack(const uint32_t (&w)[BITS / 2], floa
     out[1] = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
-__device__ __forceinline__ void tiles_cp_async(uint32_t dst, const void* src, uint32_t bytes, bool there) {      // 16, 8 or 4 bytes; zeros if not there
-    const uint32_t n = there ? bytes : 0u;
-    if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ bool tiles_look(uint32_t bar, uint32_t phase) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(phase) : "memory");
+    return ok;
+}
+// Looks until the phase is over; a wait that runs out tells all others, which end at their next 64th look.
+static __device__ __noinline__ bool tiles_wait(uint32_t bar, uint32_t phase, volatile uint32_t* dead, uint32_t* error) {
+#pragma unroll 1
+    for (uint32_t look = 0; look < kLooks; ++look) {
+        if (tiles_look(bar, phase)) return true;
+        if (look % 64 == 0 && *dead) return false;
+    }
+    *dead = 1;
+    *error = kErrAttentionWait;
+    return false;
 }
 
 template <int MT, int TILE>
@@ -157,7 +167,7 @@ template <int D, int BITS, bool BF16>
 __global__ void __launch_bounds__(TilesShape<D, BITS>::THREADS, 1)
 attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     using S = TilesShape<D, BITS>;
-    using Meta = TilesMeta<S::TILE, S::UNPACK_WARPS>;
+    using Meta = TilesMeta<S::TILE>;
     constexpr int MT = S::MT, TILE = S::TILE;
     constexpr float kCentre = BITS == 8 ? 128.0f : 8.0f;
     static_assert(sizeof(Meta) <= S::META, "meta");
@@ -176,25 +186,20 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     auto p_full = [&](uint32_t i) { return bars + 48 + (i & 1) * 8; };      // P_i; S_i has been read, and what was told
     auto o_done = [&](uint32_t i) { return bars + 64 + (i & 1) * 8; };      // O holds tile i
     const uint32_t q_full = bars + 80, all_done = bars + 88, v_full = bars + 96;
+    auto pl_full = [&](uint32_t i) { return bars + 104 + (i & 1) * 8; };                   // planes
+    auto kc_full = [&](uint32_t i) { return bars + 120 + (i % S::KC_BUFS) * 8; };          // K's codes
+    auto kc_free = [&](uint32_t i) { return bars + 136 + (i % S::KC_BUFS) * 8; };
+    auto pl_free = [&](uint32_t i) { return bars + 152 + (i & 1) * 8; };
+    const uint32_t vc_full = bars + 168, vc_free = bars + 176;
+    auto told = [&](uint32_t i) { return bars + 184 + (i & 3) * 8; };       // what the planes say; four, as nobody waits for those who look at it
     auto one = [](uint32_t i) { return i & 1u; };
     auto two = [](uint32_t i) { return i >> 1 & 1u; };
     auto of_k = [](uint32_t i) { return i / S::K_BUFS & 1u; };
-    volatile uint32_t* dead = &meta.dead;
-    auto wait_lane = [&](uint32_t bar, uint32_t phase) -> bool {
-        // a look sleeps until the phase is complete, 10 us at the most: warps that wait leave the issue slots to the others
-        for (uint32_t look = 0; look < kLooks; ++look) {
-            uint32_t ok;
-            asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
-                         : "=r"(ok) : "r"(bar), "r"(phase), "r"(10000u) : "memory");
-            if (ok) return true;
-            if (*dead) return false;
-        }
-        *dead = 1;
-        *a.error = kErrAttentionWait;
-        return false;
+    auto of_kc = [](uint32_t i) { return i / S::KC_BUFS & 1u; };
+    // of a whole warp; what a wait that is over already takes is kept short
+    auto wait = [&](uint32_t bar, uint32_t phase) -> bool {
+        return __all_sync(kFullMask, tiles_look(bar, phase)) || __all_sync(kFullMask, tiles_wait(bar, phase, &meta.dead, a.error));
     };
-    // of a whole warp
-    auto wait = [&](uint32_t bar, uint32_t phase) -> bool { return __all_sync(kFullMask, wait_lane(bar, phase)); };
 
     if (tid == 0) {
         mbar_init(v_full, S::UNPACK_WARPS);
@@ -204,7 +209,15 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             mbar_init(s_full(i), 2);
             mbar_init(p_full(i), S::SOFT_WARPS);
             mbar_init(o_done(i), 1);
+            mbar_init(pl_full(i), 1);
+            mbar_init(pl_free(i), 2);
+            mbar_init(bars + 120 + i * 8, 1);
+            mbar_init(told(i), 2);
+            mbar_init(told(i + 2), 2);
+            mbar_init(bars + 136 + i * 8, S::UNPACK_WARPS);
         }
+        mbar_init(vc_full, 1);
+        mbar_init(vc_free, S::UNPACK_WARPS);
         mbar_init(q_full, S::SOFT_WARPS);
         mbar_init(all_done, 1);
         meta.dead = 0;
@@ -224,278 +237,256 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     tiles_fence_after();
     const uint32_t tmem = meta.tmem, count = busy ? (uint32_t)(stop - item) : 0;
 
-    if (warp >= S::SOFT_WARPS && warp < S::WARPS - 1) {
-        // ===================== unpacking =====================
-        // A thread's piece j of K (V) is sixteen elements of one token. All pieces of a token belong to one warp, which requests what it unpacks a tile
-        // ahead: codes to places of the thread's own, planes and page numbers to places of the token's; a wait for its own copies and a
-        // __syncwarp is all it takes. What lies behind the sequence, or has no page, is zeros.
-        const uint32_t u = tid - S::SOFT_WARPS * kWarp, uw = u / kWarp;
-        constexpr uint32_t kKeys = S::UNPACK / S::K_ROW;       // tokens between a thread's pieces of K
-        const uint32_t k_piece = u % S::K_ROW, v_piece = u % S::V_ROW, k_key0 = u / S::K_ROW;
-        // heads of 512 have two tokens of V to a warp and piece: those of its pieces 2 j and 2 j + 1 of K
-        const uint32_t v_key0 = D == 512 ? uw + (lane / 16) * 8 : k_key0;
-        constexpr uint32_t kVKeys = D == 512 ? 16 : kKeys;
-        const uint32_t page_mask = (1u << a.table.page_log2) - 1u, page_log2 = a.table.page_log2;
-        struct Tile { uint32_t token0, end, head; const int32_t* table; };
-        auto tile_of = [&](const Cursor<MT, TILE>& c) { return Tile{c.token0(), c.range.end, c.head, a.table.table + (size_t)c.b * a.table.stride}; };
-        auto page_place = [&](uint32_t i, uint32_t key) { return S::OFF_PG + ((i & 1) * TILE + key) * 4; };
-        auto plane_place = [&](uint32_t i, uint32_t key) { return S::OFF_PL + ((i & 3) * TILE + key) * (4 * S::PLANES); };
-        auto ask_pages = [&](const Tile& t, uint32_t i) {
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) {
-                const uint32_t key = k_key0 + j * kKeys, token = t.token0 + key;
-                if (k_piece == 0 && token < t.end) tiles_cp_async(base + page_place(i, key), t.table + (token >> page_log2), 4, true);
-            }
-        };
-        // The cache's rows of a tile's tokens (numbers below 2^32 - 1, as the entry point has checked), kNone where there is none.
-        constexpr uint32_t kNone = 0xFFFFFFFFu;
-        uint32_t rows[S::K_EACH], rows_v[S::K_EACH];           // of the tile whose K is requested next, and whose V is
-        auto find_rows = [&](const Tile& t, uint32_t i) {
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) {
-                const uint32_t key = k_key0 + j * kKeys, token = t.token0 + key;
-                const int32_t page = *reinterpret_cast<const int32_t*>(smem + page_place(i, key));
-                const bool is = token < t.end && page >= 0 && (uint32_t)page < a.table.pages;
-                rows[j] = is ? (((uint32_t)page * a.kv_heads + t.head / S::PARTS) << page_log2) + (token & page_mask) : kNone;
-            }
-        };
-        // planes: lane p of a token's first four takes plane p
-        const uint16_t* my_plane = k_piece == 0 ? a.k.scales : k_piece == 1 ? a.k.biases : k_piece == 2 ? a.v.scales : a.v.biases;
-        auto ask_k = [&](uint32_t i) {
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) {
-                const bool is = rows[j] != kNone;
-                const size_t row = is ? rows[j] : 0;
-                tiles_cp_async(base + S::OFF_KC + (j * S::UNPACK + u) * S::PIECE, a.k.codes + row * S::ROW_BYTES + k_piece * S::PIECE, S::PIECE, is);
-                if (k_piece < 4)
-                    tiles_cp_async(base + plane_place(i, k_key0 + j * kKeys) + k_piece * S::PLANES, my_plane + (S::G == 1 ? row & ~(size_t)1 : row * S::G), S::PLANES, is);
-            }
-        };
-        auto ask_v = [&](const Tile& t) {
-#pragma unroll
-            for (int j = 0; j < S::V_EACH; ++j) {
-                const uint32_t r = D == 512 ? (lane & 16 ? rows_v[(2 * j + 1) % S::K_EACH] : rows_v[2 * j % S::K_EACH]) : rows_v[j];
-                const bool is = r != kNone;
-                tiles_cp_async(base + S::OFF_VC + (j * S::UNPACK + u) * S::PIECE,
-                               a.v.codes + (size_t)(is ? r : 0) * S::ROW_BYTES + (v_piece + t.head % S::PARTS * S::V_ROW) * S::PIECE, S::PIECE, is);
-            }
-        };
-        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-        // scale and centred bias of a group of a token (which: 0 K, 2 V)
-        auto read_planes = [&](uint32_t i, uint32_t key, int which, uint32_t grp, float& s, float& b) {
-            const uint8_t* at = smem + plane_place(i, key) + which * S::PLANES + 2 * (S::G == 1 ? key & 1u : grp);
-            s = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(at));
-            b = fmaf(kCentre, s, bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(at + S::PLANES)));
-        };
-        auto magnitude = [&](float s, float b) { return fmaxf(kCentre * fabsf(s), fabsf(b)); };      // half of the largest value or more
-        // values of such sizes are fp16 numbers as they are, and exact to 2^-11 of the token's largest
-        auto plain = [&](float s, float b) {
-            const float m = magnitude(s, b);
-            return m >= 0.001953125f && m <= 16384.0f && fabsf(b) <= 16384.0f;       // the last: maxima drop a NaN
-        };
-        // sixteen codes; lanes of odd groups take the second eight first, so that eight lanes meet eight different banks when they store
-        const uint32_t k_odd = S::K_ROW >= 8 ? k_piece / 4 & 1u : 0u, v_odd = S::K_ROW >= 8 ? v_piece / 4 & 1u : 0u;
-        auto read_codes = [&](uint32_t off, uint32_t odd, uint32_t (&r)[BITS / 2]) {
-            if constexpr (BITS == 8) {
-                const uint2 x = *reinterpret_cast<const uint2*>(smem + off + 8 * odd), y = *reinterpret_cast<const uint2*>(smem + off + 8 - 8 * odd);
-                r[0] = x.x; r[1] = x.y; r[2] = y.x; r[3] = y.y;
+    if (warp >= S::SOFT_WARPS && warp < S::SOFT_WARPS + S::UNPACK_WARPS) {
+        // ===================== unpacking: a thread's piece is sixteen elements of one token =====================
+        const uint32_t u = tid - S::SOFT_WARPS * kWarp;
+        const uint32_t k_piece = u % S::K_ROW, v_piece = u % S::V_ROW, k_key0 = u / S::K_ROW, v_key0 = u / S::V_ROW;
+        constexpr int kBoth = S::K_EACH < S::V_EACH ? S::K_EACH : S::V_EACH, kAtOnce = kBoth < 4 ? kBoth : 4;
+        // K_0, K_1, V_0, K_2, V_1, ...: one body for both. A wait that runs out is told to all, whose later waits end at once; every warp goes through all tiles.
+#pragma unroll 1
+        for (uint32_t turn = 0; turn <= 2 * count; ++turn) {
+            const bool is_v = turn && turn % 2 == 0;
+            const uint32_t n = is_v ? turn / 2 - 1 : (turn + 1) / 2;
+            if (n >= count) continue;
+            if (is_v) {
+                if (n >= 1) wait(o_done(n - 1), two(n - 1));
+                wait(vc_full, one(n));
             } else {
-                r[0] = *reinterpret_cast<const uint32_t*>(smem + off + 4 * odd);
-                r[1] = *reinterpret_cast<const uint32_t*>(smem + off + 4 - 4 * odd);
+                if (n >= S::K_BUFS) wait(k_free(n), of_k(n - S::K_BUFS));
+                wait(told(n), n >> 2 & 1u);
+                wait(kc_full(n), of_kc(n));
+            }
+            const uint32_t from = is_v ? S::OFF_VC : S::OFF_KC + (n % S::KC_BUFS) * S::KC_BYTES, to = is_v ? S::OFF_V : S::OFF_K + (n % S::K_BUFS) * S::K_BYTES;
+            const uint32_t words = is_v ? S::OFF_VW + (n & 3) * (TILE * S::GV * 4) : S::OFF_KW + (n & 3) * (TILE * S::G * 4);
+            const uint32_t row_bytes = S::PARTS > 1 && is_v ? S::V_ROW_BYTES : S::ROW_BYTES, groups = S::PARTS > 1 && is_v ? S::GV : S::G;
+            const uint32_t piece = S::PARTS > 1 && is_v ? v_piece : k_piece, keys = S::PARTS > 1 && is_v ? S::UNPACK / S::V_ROW : S::UNPACK / S::K_ROW;
+            const bool odd = S::K_ROW >= 8 && (piece / 4 & 1u);
+            uint32_t key = S::PARTS > 1 && is_v ? v_key0 : k_key0;
+#pragma unroll 1
+            for (; key < (uint32_t)TILE; key += kAtOnce * keys) {
+                uint32_t r[kAtOnce][BITS / 2], w[kAtOnce];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const uint8_t* at = smem + from + (key + j * keys) * row_bytes + piece * S::PIECE;
+                    w[j] = *reinterpret_cast<const uint32_t*>(smem + words + ((key + j * keys) * groups + piece / 4) * 4);
+                    // lanes of odd groups take the second eight first, so that eight lanes meet eight different banks when they store
+                    if constexpr (BITS == 8) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(at);
+                        r[j][0] = odd ? x.z : x.x; r[j][1] = odd ? x.w : x.y; r[j][2] = odd ? x.x : x.z; r[j][3] = odd ? x.y : x.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2*>(at);
+                        r[j][0] = odd ? x.y : x.x; r[j][1] = odd ? x.x : x.y;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const uint32_t k = key + j * keys, sc = gm_prmt(w[j], 0, 0x1010), bi = gm_prmt(w[j], 0, 0x3232);
+                    uint4 h[2];
+                    tiles_unpack<BITS>(r[j], *reinterpret_cast<const __half2*>(&sc), *reinterpret_cast<const __half2*>(&bi), h);
+                    const uint32_t at = to + k * 128 + (piece / 4) * (TILE * 128), c0 = (piece % 4 * 2 + odd) ^ (k & 7u);
+                    *reinterpret_cast<uint4*>(smem + at + c0 * 16) = h[0];
+                    *reinterpret_cast<uint4*>(smem + at + (c0 ^ 1u) * 16) = h[1];
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(is_v ? v_full : k_full(n));
+                mbar_arrive(is_v ? vc_free : kc_free(n));
+            }
+        }
+    } else if (warp >= S::MEASURE && warp < S::LOADER) {
+        // ===================== what the planes say: one warp for K's, one for V's, a token per lane =====================
+        // Scale and centred bias of a token's groups as fp16, by a power of two of the token's. Values of ordinary sizes are fp16 numbers as they are, exact to
+        // 2^-11 of the token's largest.
+        const bool of_v = warp != S::MEASURE;
+        const uint32_t run_log2 = lesser(a.table.page_log2, (uint32_t)(31 - __builtin_clz(TILE)));
+        auto measure = [&](auto groups, uint32_t n, const uint4& t) {
+            constexpr int N = decltype(groups)::value;
+            uint32_t any = 0;
+            float most_up = 0.0f;
+#pragma unroll 1
+            for (uint32_t key = lane; key < (uint32_t)TILE; key += kWarp) {
+                const bool held = t.x + key < t.y, is = held && (t.z >> (key >> run_log2) & 1u);
+                const uint16_t* scales = reinterpret_cast<const uint16_t*>(smem + S::OFF_PL + ((n & 1) * 4 + 2 * of_v) * S::PLANE) + key * S::G + (of_v ? t.w : 0u);
+                uint32_t words[N], bits = 0;
+                float sc[N], bi[N], most = 0.0f;
+                bool plain = true;
+#pragma unroll
+                for (int g = 0; g < N; ++g) {
+                    sc[g] = is ? bf16_bits_to_float(scales[g]) : 0.0f;
+                    bi[g] = is ? fmaf(kCentre, sc[g], bf16_bits_to_float(scales[S::PLANE / 2 + g])) : 0.0f;
+                }
+#pragma unroll
+                for (int g = 0; g < N; ++g) {
+                    const float size = fmaxf(kCentre * fabsf(sc[g]), fabsf(bi[g]));        // half of the largest value or more
+                    const bool finite = sc[g] - sc[g] == 0.0f && bi[g] - bi[g] == 0.0f;
+                    plain = plain && finite && size >= 0.001953125f && size <= 16384.0f;
+                    most = finite ? fmaxf(most, size) : most;
+                    if (of_v && !finite) {
+                        bits |= 1u << g;
+                        sc[g] = bi[g] = 0.0f;
+                    }
+                }
+                const int e = plain || !is ? 0 : min(max(rows_exponent(most) - 7, -126), 119);       // both parts of a value below 2^8
+                const float down = rows_power(-e), up = rows_power(e);
+                any |= e != 0;
+#pragma unroll
+                for (int g = 0; g < N; ++g) words[g] = rows_half2(sc[g] * down, bi[g] * down);
+                uint32_t* to = reinterpret_cast<uint32_t*>(smem + (of_v ? S::OFF_VW : S::OFF_KW)) + ((n & 3) * TILE + key) * N;
+#pragma unroll
+                for (int g = 0; g < N; g += 4) {
+                    if constexpr (N >= 4) *reinterpret_cast<uint4*>(to + g) = make_uint4(words[g], words[g + 1], words[g + 2], words[g + 3]);
+                    else if constexpr (N == 2) *reinterpret_cast<uint2*>(to) = make_uint2(words[0], words[1]);
+                    else to[0] = words[0];
+                }
+                if (of_v) {
+                    if (held && !is) {
+                        bits = 0x80u;
+                        *a.error = kErrKvPage;
+                    }
+                    meta.v_up[n & 7][key] = up;
+                    meta.bad[n & 7][key] = (uint8_t)bits;
+                    if (bits) any |= 2u;
+                    most_up = fmaxf(most_up, up);
+                } else {
+                    meta.k_up[n & 7][key] = up * (a.scale * 1.4426950408889634f);
+                }
+            }
+            any = __reduce_or_sync(kFullMask, any);
+            most_up = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(most_up)));
+            if (lane == 0) {
+                meta.flags[n & 7][of_v] = any;
+                if (of_v) meta.v_most[n & 7] = most_up;
             }
         };
-        auto store = [&](uint32_t buffer, const uint32_t (&r)[BITS / 2], float s, float b, uint32_t key, uint32_t piece, uint32_t odd) {
-            uint4 h[2];
-            tiles_unpack<BITS>(r, s, b, h);
-            const uint32_t at = buffer + key * 128 + (piece / 4) * (TILE * 128), c0 = (piece % 4 * 2 + odd) ^ (key & 7u);
-            *reinterpret_cast<uint4*>(smem + at + c0 * 16) = h[0];
-            *reinterpret_cast<uint4*>(smem + at + (c0 ^ 1u) * 16) = h[1];
+#pragma unroll 1
+        for (uint32_t n = 0; n < count; ++n) {
+            wait(pl_full(n), two(n));
+            const uint4 t = meta.tile[n & 3];
+            if (of_v) measure(std::integral_constant<int, S::GV>(), n, t);
+            else measure(std::integral_constant<int, S::G>(), n, t);
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(pl_free(n));
+                mbar_arrive(told(n));
+            }
+        }
+    } else if (warp == S::LOADER) {
+        // ===================== loader: which rows of the cache, their codes and planes by bulk copies =====================
+        // Lane r has the tile's r-th run of tokens, which one page holds. Steps of tile n: planes of n + 1, K of n, V of n - 1: the order in which
+        // the unpacking takes them, so that no request waits for a buffer that is freed after another one's. By then V_(n-3) has been unpacked, which
+        // was behind O's taking V_(n-4): what was told about tile n - 7 is not looked at any more, nor the words of tile n - 3.
+        struct Tile { uint32_t token0, end, head; const int32_t* table; };
+        const uint32_t page_log2 = a.table.page_log2, run_log2 = lesser(page_log2, (uint32_t)(31 - __builtin_clz(TILE))), first = (uint32_t)lane << run_log2;
+        constexpr uint32_t kNone = 0xFFFFFFFFu;                // rows of the cache are below, as the entry point has checked
+        auto tile_of = [&](const Cursor<MT, TILE>& c) { return Tile{c.token0(), c.range.end, c.head, a.table.table + (size_t)c.b * a.table.stride}; };
+        auto page_of = [&](const Tile& t) -> int32_t { return first < (uint32_t)TILE && t.token0 + first < t.end ? t.table[(t.token0 + first) >> page_log2] : -1; };
+        auto row_of = [&](const Tile& t, int32_t page) -> uint32_t {
+            return page >= 0 && (uint32_t)page < a.table.pages
+                       ? (((uint32_t)page * a.kv_heads + t.head / S::PARTS) << page_log2) + ((t.token0 + first) & ((1u << page_log2) - 1u)) : kNone;
         };
-        Cursor<MT, TILE> next = now;                           // of the tile that pages are asked for
+        // tells the barrier what comes: `bytes` for every token of the runs that are there
+        auto expect = [&](uint32_t bar, uint32_t runs, uint32_t bytes) {
+            if (lane == 0) mbar_arrive_expect_tx(bar, (__popc(runs) << run_log2) * bytes);
+            __syncwarp();
+        };
+        auto ask = [&](uint32_t to, const void* plane, uint32_t row, uint32_t bytes, uint32_t bar) {
+            bulk_copy_g2s(base + to + first * bytes, static_cast<const uint8_t*>(plane) + (size_t)row * bytes, bytes << run_log2, bar);
+        };
+        auto ask_planes = [&](uint32_t n, const Tile& t, uint32_t row) {
+            const uint32_t runs = __ballot_sync(kFullMask, row != kNone);
+            if (lane == 0) meta.tile[n & 3] = make_uint4(t.token0, t.end, runs, t.head % S::PARTS * S::GV);
+            expect(pl_full(n), runs, 4 * S::G * 2);
+            if (row != kNone) {
+                const uint32_t to = S::OFF_PL + (n & 1) * (4 * S::PLANE);
+                ask(to, a.k.scales, row, S::G * 2, pl_full(n));
+                ask(to + S::PLANE, a.k.biases, row, S::G * 2, pl_full(n));
+                ask(to + 2 * S::PLANE, a.v.scales, row, S::G * 2, pl_full(n));
+                ask(to + 3 * S::PLANE, a.v.biases, row, S::G * 2, pl_full(n));
+            }
+        };
+        auto ask_k = [&](uint32_t n, uint32_t row) {
+            expect(kc_full(n), __ballot_sync(kFullMask, row != kNone), S::ROW_BYTES);
+            if (row != kNone) ask(S::OFF_KC + (n % S::KC_BUFS) * S::KC_BYTES, a.k.codes, row, S::ROW_BYTES, kc_full(n));
+        };
+        auto ask_v = [&](uint32_t row, uint32_t head) {
+            expect(vc_full, __ballot_sync(kFullMask, row != kNone), S::V_ROW_BYTES);
+            if constexpr (S::PARTS == 1) {
+                if (row != kNone) ask(S::OFF_VC, a.v.codes, row, S::ROW_BYTES, vc_full);
+            } else {                                           // half of every token's
+#pragma unroll
+                for (uint32_t key = lane; key < (uint32_t)TILE; key += kWarp) {
+                    const uint32_t r = __shfl_sync(kFullMask, row, key >> run_log2);
+                    if (r != kNone)
+                        bulk_copy_g2s(base + S::OFF_VC + key * S::V_ROW_BYTES, a.v.codes + (size_t)(r + (key & ((1u << run_log2) - 1u))) * S::ROW_BYTES + head % S::PARTS * S::V_ROW_BYTES,
+                                      S::V_ROW_BYTES, vc_full);
+                }
+            }
+        };
+        Cursor<MT, TILE> next = now;                           // of the tile whose pages are looked up
         uint32_t left = busy ? (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), stop - item) : 0, ahead = 0;
-        Tile t0 = {}, t1 = {}, t2 = {};                        // tiles i, i + 1, i + 2
-        auto step = [&] {                                      // `next` one tile on, if there is one
-            if (++ahead >= count) return;
+        auto step = [&](const Tile& t) -> Tile {               // the tile after t, if there is one; `next` is its cursor
+            if (++ahead >= count) return t;
             if (--left == 0) {
                 tiles_next_unit<MT, TILE>(a, next);
                 left = (uint32_t)lesser((uint64_t)next.range.tiles, (uint64_t)(count - ahead));
-            } else {
-                ++next.tile;
+                return tile_of(next);
             }
+            ++next.tile;
+            return Tile{t.token0 + TILE, t.end, t.head, t.table};
         };
+        // After a wait that ran out nothing more is requested; what was is waited for before the block leaves.
+        bool fine = true;
+        uint32_t k_asked = 0, v_asked = 0, p_asked = 0;
         if (count) {
-            t0 = tile_of(next);
-            ask_pages(t0, 0);
-            step();
-            t1 = tile_of(next);
-            if (count > 1) ask_pages(t1, 1);
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            __syncwarp();
-            find_rows(t0, 0);
-            ask_k(0);
-            commit();
-            commit();                                          // in the place of values: the waits below count groups
-            step();
-            t2 = tile_of(next);
-        }
-        // K_n, what is told about tile n; K_(n+1) and all planes of tile n + 1 are requested, and the pages of tile n + 2
-        bool fast_v = true;                                    // of tile n: its values need no power of two
-        auto unpack_k = [&](uint32_t n) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncwarp();
-            float ks[S::K_EACH], kb[S::K_EACH];
-            bool fast = true;
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) {
-                const uint32_t key = k_key0 + j * kKeys;
-                read_planes(n, key, 0, k_piece / 4, ks[j], kb[j]);
-                fast = fast && (plain(ks[j], kb[j]) || t0.token0 + key >= t0.end);
-            }
-#pragma unroll
-            for (int j = 0; j < S::V_EACH; ++j) {
-                const uint32_t key = v_key0 + j * kVKeys;
-                float s, b;
-                read_planes(n, key, 2, v_piece / 4 + t0.head % S::PARTS * S::GV, s, b);
-                fast = fast && (plain(s, b) || t0.token0 + key >= t0.end);
-            }
-            fast = __all_sync(kFullMask, fast);
-            if (fast) {
-#pragma unroll
-                for (int j = 0; j < S::K_EACH; ++j)
-                    if (k_piece == 0) {
-                        const uint32_t key = k_key0 + j * kKeys;
-                        meta.k_up[n & 3][key] = a.scale * 1.4426950408889634f;
-                        meta.v_up[n & 3][key] = 1.0f;
-                        meta.bad[n & 3][key] = 0;
-                    }
-                if (lane == 0) {
-                    meta.flags[n & 3][uw] = 0;
-                    meta.v_most[n & 3][uw] = 1.0f;
-                }
-            } else {
-                // a power of two per token, planes that are not finite, pages that are missing
-                uint32_t any = 0;
-                float v_most = 0.0f;
+            Tile t0 = tile_of(next), t1 = step(t0);
+            uint32_t row0 = row_of(t0, page_of(t0)), row_v = kNone, head_v = 0;
+            int32_t page1 = page_of(t1);
+            ask_planes(0, t0, row0);
+            p_asked = 1;
 #pragma unroll 1
-                for (int j = 0; j < S::K_EACH; ++j) {
-                    const uint32_t key = k_key0 + j * kKeys, token = t0.token0 + key;
-                    float s, b;
-                    read_planes(n, key, 0, k_piece / 4, s, b);
-                    float most = s - s == 0.0f && b - b == 0.0f ? magnitude(s, b) : 0.0f;
-                    for (int off = S::K_ROW / 2; off >= 4; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, off));
-                    const int e_k = min(max(rows_exponent(most) - 7, -126), 119);      // both parts of a value below 2^8
-                    most = 0.0f;
-                    uint32_t bits = 0;
-#pragma unroll 1
-                    for (int grp = 0; grp < S::GV; ++grp) {
-                        read_planes(n, key, 2, grp + t0.head % S::PARTS * S::GV, s, b);
-                        if (s - s == 0.0f && b - b == 0.0f) most = fmaxf(most, magnitude(s, b));
-                        else bits |= 1u << grp;
+            for (uint32_t n = 0; n <= count; ++n) {
+                uint32_t row1 = kNone;
+                const Tile t2 = step(t1);
+                const int32_t page2 = page_of(t2);             // needed a tile later
+                if (n + 1 < count) {
+                    row1 = row_of(t1, page1);
+                    if (n) fine = fine && wait(pl_free(n - 1), two(n - 1));
+                    if (fine) {
+                        ask_planes(n + 1, t1, row1);
+                        p_asked = n + 2;
                     }
-                    const int e_v = min(max(rows_exponent(most) - 7, -126), 119);
-                    const int32_t page = *reinterpret_cast<const int32_t*>(smem + page_place(n, key));
-                    if (token < t0.end && !(page >= 0 && (uint32_t)page < a.table.pages)) {
-                        bits |= 0x80u;
-                        *a.error = kErrKvPage;
+                }
+                if (n < count) {
+                    if (n >= S::KC_BUFS) fine = fine && wait(kc_free(n), of_kc(n - S::KC_BUFS));
+                    if (fine) {
+                        ask_k(n, row0);
+                        k_asked = n + 1;
                     }
-                    if (token >= t0.end) bits = 0;
-                    if (k_piece == 0) {
-                        meta.k_up[n & 3][key] = rows_power(e_k) * (a.scale * 1.4426950408889634f);
-                        meta.v_up[n & 3][key] = rows_power(e_v);
-                        meta.bad[n & 3][key] = (uint8_t)bits;
-                        meta.e_k[key] = (int8_t)e_k;
+                }
+                if (n) {
+                    if (n >= 2) fine = fine && wait(vc_free, one(n - 2));
+                    if (fine) {
+                        ask_v(row_v, head_v);
+                        v_asked = n;
                     }
-                    any |= bits;
-                    v_most = fmaxf(v_most, rows_power(e_v));
                 }
-                any = __any_sync(kFullMask, any != 0);
-                v_most = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(v_most)));
-                if (lane == 0) {
-                    meta.flags[n & 3][uw] = (uint8_t)any;
-                    meta.v_most[n & 3][uw] = v_most;
-                }
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < S::K_EACH; ++j) {
-                    const float down = rows_power(-meta.e_k[k_key0 + j * kKeys]);
-                    ks[j] *= down;
-                    kb[j] *= down;
-                }
-            }
-            fast_v = fast;
-            const bool more = n + 1 < count;
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) rows_v[j] = rows[j];           // of tile n: as they were
-            if (more) find_rows(t1, n + 1);
-#pragma unroll
-            for (int j = 0; j < S::K_EACH; ++j) {
-                uint32_t r[BITS / 2];
-                read_codes(S::OFF_KC + (j * S::UNPACK + u) * S::PIECE, k_odd, r);
-                store(S::OFF_K + (n % S::K_BUFS) * S::K_BYTES, r, ks[j], kb[j], k_key0 + j * kKeys, k_piece, k_odd);
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(k_full(n));
-            if (more) ask_k(n + 1);
-            if (n + 2 < count) ask_pages(t2, n + 2);
-            commit();
-        };
-        // V_n; the codes of V_(n+1) are requested
-        auto unpack_v = [&](uint32_t n, const Tile& t, const Tile& after, bool fast) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            float vs[S::V_EACH], vb[S::V_EACH];
-#pragma unroll
-            for (int j = 0; j < S::V_EACH; ++j) {
-                const uint32_t key = v_key0 + j * kVKeys;
-                read_planes(n, key, 2, v_piece / 4 + t.head % S::PARTS * S::GV, vs[j], vb[j]);
-                if (!fast) {
-                    const float down = __uint_as_float(0x7F000000u - __float_as_uint(meta.v_up[n & 3][key]));      // the reciprocal of a power of two
-                    const bool fine = vs[j] - vs[j] == 0.0f && vb[j] - vb[j] == 0.0f;
-                    vs[j] = fine ? vs[j] * down : 0.0f;
-                    vb[j] = fine ? vb[j] * down : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < S::V_EACH; ++j) {
-                uint32_t r[BITS / 2];
-                read_codes(S::OFF_VC + (j * S::UNPACK + u) * S::PIECE, v_odd, r);
-                store(S::OFF_V, r, vs[j], vb[j], v_key0 + j * kVKeys, v_piece, v_odd);
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(v_full);
-            if (n + 1 < count) ask_v(after);
-            commit();
-        };
-        // A wait that runs out is told to all, whose later waits end at once; every warp goes through all tiles. Commits alternate
-        // between K (with planes and pages) and V, as their uses do: K_(i+1), V_i, K_(i+2), ...; one later group may be pending at each wait.
-        if (count) {
-            unpack_k(0);
-            ask_v(t0);
-            commit();
-        }
-        Tile tv = t0, tv1 = t1;                                // tiles i, i + 1 of the values
-        bool fast_i = fast_v;
-#pragma unroll 1
-        for (uint32_t i = 0; i < count; ++i) {
-            const bool fast_now = fast_i;
-            if (i + 1 < count) {
+                if (!fine) break;
+                row_v = row0;
+                head_v = t0.head;
+                row0 = row1;
                 t0 = t1;
                 t1 = t2;
-                step();
-                t2 = tile_of(next);
-                if (i + 1 >= S::K_BUFS) wait(k_free(i + 1), of_k(i + 1 - S::K_BUFS));
-                unpack_k(i + 1);
-                fast_i = fast_v;
-            } else {
-                commit();
+                page1 = page2;
             }
-            if (i >= 1) wait(o_done(i - 1), two(i - 1));
-            unpack_v(i, tv, tv1, fast_now);
-            tv = tv1;
-            tv1 = t1;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        auto drain = [&](uint32_t bar, uint32_t phase) {       // whatever the others have told
+            for (uint32_t look = 0; look < kLooks && !tiles_look(bar, phase); ++look) {}
+        };
+        for (uint32_t n = k_asked > S::KC_BUFS ? k_asked - S::KC_BUFS : 0; n < k_asked; ++n) drain(kc_full(n), of_kc(n));
+        if (v_asked) drain(vc_full, one(v_asked - 1));
+        for (uint32_t n = p_asked > 2 ? p_asked - 2 : 0; n < p_asked; ++n) drain(pl_full(n), two(n));
     } else if (warp == S::WARPS - 1) {
         // ===================== MMA issuer =====================
         constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(TILE >> 3) << 17) | ((uint32_t)(MT >> 4) << 24);
@@ -507,7 +498,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             tiles_fence_after();
             if (lane == 0) {
                 const uint64_t q0 = tiles_desc(base, 16, 1024), k0 = tiles_desc(base + S::OFF_K + (i % S::K_BUFS) * S::K_BYTES, 16, 1024);
-#pragma unroll
+#pragma unroll 4
                 for (int e = 0; e < D / 16; ++e)
                     tiles_mma_ss(tmem + S::COL_S + (i & 1) * TILE, q0 + (((e / 4) * (MT * 128) + e % 4 * 32) >> 4), k0 + (((e / 4) * (TILE * 128) + e % 4 * 32) >> 4),
                                  idesc_s, e > 0);
@@ -531,18 +522,24 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             __syncwarp();
             return true;
         };
-        for (uint32_t i = 0; i <= count; ++i) {
+        bool fine = true;
+#pragma unroll 1
+        for (uint32_t i = 0; i <= count && fine; ++i) {
             // Within a unit the logits of tile i go ahead of the values of tile i - 1; at a unit's end the softmax waits for those values before it
             // lays out the next rows of q.
-            const bool new_unit = i < count && segment == 0;
-            if (new_unit || i == count) {
-                if (i > 0 && !values(i - 1)) break;
-                if (i == count) break;
-                if (i) tiles_next_unit<MT, TILE>(a, now);
-                segment = (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), (uint64_t)(count - i));
-                if (!wait(q_full, segments++ & 1u) || !logits(i)) break;
-            } else if (!logits(i) || !values(i - 1)) {
-                break;
+            const bool new_unit = i < count && segment == 0, behind = new_unit || i == count;
+#pragma unroll 1
+            for (int half = 0; half < 2 && fine; ++half) {
+                if (behind == (half == 0)) {
+                    if (i) fine = values(i - 1);
+                } else if (i < count) {
+                    if (new_unit) {
+                        if (i) tiles_next_unit<MT, TILE>(a, now);
+                        segment = (uint32_t)lesser((uint64_t)(now.range.tiles - now.tile), (uint64_t)(count - i));
+                        fine = wait(q_full, segments++ & 1u);
+                    }
+                    fine = fine && logits(i);
+                }
             }
             opens = new_unit;
             --segment;
@@ -550,12 +547,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         // nothing is in flight when the block leaves
         if (lane == 0) tiles_commit(all_done);
         __syncwarp();
-        for (uint32_t look = 0; look < kLooks; ++look) {
-            uint32_t ok;
-            asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
-                         : "=r"(ok) : "r"(all_done), "r"(0u), "r"(10000u) : "memory");
-            if (ok) break;
-        }
+        for (uint32_t look = 0; look < kLooks && !tiles_look(all_done, 0); ++look) {}
     } else {
         // ===================== softmax: two threads per row, warps w and w + 4, with half of a tile each =====================
         const uint32_t quad = warp % 4, side = warp / 4, r = quad * 32 + lane, lanes = tmem + (quad * 32u << 16);
@@ -637,16 +629,12 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 const uint32_t st = i & 1;
                 ok = wait(s_full(i), two(i));
                 tiles_fence_after();
-                uint32_t flags = 0;
-                float v_most = 0.0f;
-#pragma unroll
-                for (int w = 0; w < S::UNPACK_WARPS; w += 4) {
-                    flags |= *reinterpret_cast<const uint32_t*>(&meta.flags[i & 3][w]);
-                    const float4 v = *reinterpret_cast<const float4*>(&meta.v_most[i & 3][w]);
-                    v_most = fmaxf(fmaxf(v_most, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
-                }
-                const bool odd = flags != 0;
-                const bool open = !odd && token0 >= low_most && token0 + HALF <= open_end;
+                const uint2 flags = *reinterpret_cast<const uint2*>(meta.flags[i & 7]);
+                const float v_most = meta.v_most[i & 7];
+                const bool odd = flags.y & 2u, open = !odd && token0 >= low_most && token0 + HALF <= open_end;
+                // The usual tile: all rows see all tokens, whose powers of two are 1. What other tiles take is kept out of its way.
+                const bool usual = open && (flags.x | flags.y) == 0 && a.scale > 0.0f;
+                const float by = usual ? q_up * (a.scale * 1.4426950408889634f) : q_up;
                 // the tokens from `t0` on that the row sees, a chunk of them
                 auto see = [&](int c0) -> uint32_t {
                     const uint32_t t0 = token0 + c0;
@@ -669,26 +657,26 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                     }
                     if (odd)
                         for (int j = 0; j < CHUNK; ++j)
-                            if (meta.bad[i & 3][side * HALF + c0 + j] & 0x80u) seen &= ~(1u << j);
+                            if (meta.bad[i & 7][side * HALF + c0 + j] & 0x80u) seen &= ~(1u << j);
                     return is ? seen : 0u;
                 };
-                // the logits of a chunk, in base 2 but for the row's power of two
+                // the logits of a chunk, in base 2 but for `by`
                 auto load_logits = [&](int c0, float (&x)[CHUNK]) {
                     uint32_t raw[CHUNK];
                     tiles_ld(lanes + S::COL_S + st * TILE + side * HALF + c0, raw);
                     tiles_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < CHUNK; j += 4) {
-                        const float4 up = *reinterpret_cast<const float4*>(&meta.k_up[i & 3][side * HALF + c0 + j]);
-                        x[j] = __uint_as_float(raw[j]) * up.x;
-                        x[j + 1] = __uint_as_float(raw[j + 1]) * up.y;
-                        x[j + 2] = __uint_as_float(raw[j + 2]) * up.z;
-                        x[j + 3] = __uint_as_float(raw[j + 3]) * up.w;
-                    }
-                    if (!open) {
-                        const uint32_t seen = see(c0);
+                    for (int j = 0; j < CHUNK; ++j) x[j] = __uint_as_float(raw[j]);
+                    if (!usual) {
+                        const uint32_t seen = open ? 0xFFFFFFFFu : see(c0);
 #pragma unroll
-                        for (int j = 0; j < CHUNK; ++j) x[j] = seen >> j & 1u ? x[j] : -INFINITY;
+                        for (int j = 0; j < CHUNK; j += 4) {
+                            const float4 up = *reinterpret_cast<const float4*>(&meta.k_up[i & 7][side * HALF + c0 + j]);
+                            x[j] = seen >> j & 1u ? x[j] * up.x : -INFINITY;
+                            x[j + 1] = seen >> (j + 1) & 1u ? x[j + 1] * up.y : -INFINITY;
+                            x[j + 2] = seen >> (j + 2) & 1u ? x[j + 2] * up.z : -INFINITY;
+                            x[j + 3] = seen >> (j + 3) & 1u ? x[j + 3] * up.w : -INFINITY;
+                        }
                     }
                 };
                 // ---- maximum ----
@@ -700,8 +688,9 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                     for (int j = 0; j < CHUNK; ++j) top = fmaxf(top, x[j]);
                 }
                 float other;
-                swap(top, other);
-                top = fmaxf(top, other) * q_up;
+                const float own = top * by;
+                swap(own, other);
+                top = fmaxf(own, other);
                 float alpha = 1.0f;
                 if (top > m + 8.0f) {
                     alpha = rows_exp2(m - top);                // m = -inf: zero
@@ -710,12 +699,12 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 const float base_m = m == -INFINITY ? 0.0f : m;
                 // ---- E: a value's power of two times 2^8, the largest probability, must not leave fp16 ----
                 if (__any_sync(kFullMask, v_most * rows_power(-e_o) > 64.0f)) {
-                    float heavy = 0.0f;
+                    float heavy = usual ? rows_exp2(own - base_m) : 0.0f;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HALF; c0 += CHUNK) {
+                    for (int c0 = usual ? HALF : 0; c0 < HALF; c0 += CHUNK) {
                         if (HALF > CHUNK) load_logits(c0, x);
 #pragma unroll
-                        for (int j = 0; j < CHUNK; ++j) heavy = fmaxf(heavy, rows_exp2(fmaf(x[j], q_up, -base_m)) * meta.v_up[i & 3][side * HALF + c0 + j]);
+                        for (int j = 0; j < CHUNK; ++j) heavy = fmaxf(heavy, rows_exp2(fmaf(x[j], by, -base_m)) * meta.v_up[i & 7][side * HALF + c0 + j]);
                     }
                     swap(heavy, other);
                     heavy = fmaxf(heavy, other);
@@ -727,36 +716,41 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 }
                 // ---- probabilities, two to a column ----
                 const float shift = base_m + (float)e_o;
-                float sum = 0.0f;
+                float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
                 for (int c0 = 0; c0 < HALF; c0 += CHUNK) {
                     uint32_t p[CHUNK / 2];
                     if (HALF > CHUNK) load_logits(c0, x);
-#pragma unroll
-                    for (int j = 0; j < CHUNK; j += 4) {
-                        const float4 up = *reinterpret_cast<const float4*>(&meta.v_up[i & 3][side * HALF + c0 + j]);
-                        const float p0 = rows_exp2(fmaf(x[j], q_up, -shift)), p1 = rows_exp2(fmaf(x[j + 1], q_up, -shift));
-                        const float p2 = rows_exp2(fmaf(x[j + 2], q_up, -shift)), p3 = rows_exp2(fmaf(x[j + 3], q_up, -shift));
-                        sum += (p0 + p1) + (p2 + p3);
-                        p[j / 2] = rows_half2(p0 * up.x, p1 * up.y);
-                        p[j / 2 + 1] = rows_half2(p2 * up.z, p3 * up.w);
-                    }
-                    tiles_st(lanes + S::COL_P + st * (TILE / 2) + (side * HALF + c0) / 2, p);
                     if (odd) {
                         // a row that gives a token weight whose planes are not finite in a group becomes NaN there
 #pragma unroll 1
                         for (int j = 0; j < CHUNK; ++j) {
-                            const uint32_t bad = meta.bad[i & 3][side * HALF + c0 + j] & 0x7Fu;
+                            const uint32_t bad = meta.bad[i & 7][side * HALF + c0 + j] & 0x7Fu;
                             if (bad) {
                                 float z = -INFINITY;
 #pragma unroll
                                 for (int k = 0; k < CHUNK; ++k) z = k == j ? x[k] : z;
-                                if (rows_exp2(fmaf(z, q_up, -base_m)) > 0.0f) poison |= bad;
+                                if (rows_exp2(fmaf(z, by, -base_m)) > 0.0f) poison |= bad;
                             }
                         }
                     }
+#pragma unroll
+                    for (int j = 0; j < CHUNK; ++j) {
+                        x[j] = rows_exp2(fmaf(x[j], by, -shift));
+                        sums[j % 4] += x[j];
+                    }
+                    if (!usual) {
+#pragma unroll
+                        for (int j = 0; j < CHUNK; j += 4) {
+                            const float4 up = *reinterpret_cast<const float4*>(&meta.v_up[i & 7][side * HALF + c0 + j]);
+                            x[j] *= up.x; x[j + 1] *= up.y; x[j + 2] *= up.z; x[j + 3] *= up.w;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < CHUNK; j += 2) p[j / 2] = rows_half2(x[j], x[j + 1]);
+                    tiles_st(lanes + S::COL_P + st * (TILE / 2) + (side * HALF + c0) / 2, p);
                 }
-                l = fmaf(l, alpha, sum);
+                l = fmaf(l, alpha, (sums[0] + sums[1]) + (sums[2] + sums[3]));
                 // ---- O, when m or E moved: half of its columns ----
                 if (i > begin_i && __any_sync(kFullMask, alpha != 1.0f)) {
                     ok = wait(o_done(i - 1), two(i - 1)) && ok;
