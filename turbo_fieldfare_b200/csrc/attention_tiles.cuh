@@ -65,16 +65,19 @@ struct TilesMeta {
     float q_up[128];               // a row's power of two
 };
 
-__device__ __forceinline__ uint64_t tiles_desc(uint32_t addr, uint32_t leading, uint32_t stride) {     // 128-byte swizzle
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Operand descriptors for the 128-byte swizzle: the lower word holds the address and the leading offset, the upper one a stride of 1024 bytes. The MMAs
+// are issued by all lanes under a predicate of one: code without a branch, whose addresses the compiler can keep in uniform registers.
+__device__ __forceinline__ uint32_t tiles_desc(uint32_t addr, uint32_t leading) { return ((addr & 0x3FFFFu) >> 4) | (leading >> 4) << 16; }
+constexpr uint32_t kDescUpper = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void tiles_mma_ss(bool issues, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"((uint32_t)issues), "r"(kDescUpper) : "memory");
 }
-__device__ __forceinline__ void tiles_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void tiles_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void tiles_mma_ts(bool issues, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.b64 b, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"((uint32_t)issues), "r"(kDescUpper) : "memory");
 }
 __device__ __forceinline__ void tiles_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -496,12 +499,14 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         auto logits = [&](uint32_t i) -> bool {
             if (!wait(k_full(i), of_k(i))) return false;
             tiles_fence_after();
-            if (lane == 0) {
-                const uint64_t q0 = tiles_desc(base, 16, 1024), k0 = tiles_desc(base + S::OFF_K + (i % S::K_BUFS) * S::K_BYTES, 16, 1024);
-#pragma unroll 4
+            {
+                const uint32_t q0 = tiles_desc(base, 16), k0 = tiles_desc(base + S::OFF_K + (i % S::K_BUFS) * S::K_BYTES, 16);
+#pragma unroll
                 for (int e = 0; e < D / 16; ++e)
-                    tiles_mma_ss(tmem + S::COL_S + (i & 1) * TILE, q0 + (((e / 4) * (MT * 128) + e % 4 * 32) >> 4), k0 + (((e / 4) * (TILE * 128) + e % 4 * 32) >> 4),
+                    tiles_mma_ss(lane == 0, tmem + S::COL_S + (i & 1) * TILE, q0 + (((e / 4) * (MT * 128) + e % 4 * 32) >> 4), k0 + (((e / 4) * (TILE * 128) + e % 4 * 32) >> 4),
                                  idesc_s, e > 0);
+            }
+            if (lane == 0) {
                 tiles_commit(s_full(i));
                 tiles_commit(k_free(i));
                 mbar_arrive(s_full(i));
@@ -512,13 +517,13 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         auto values = [&](uint32_t j) -> bool {
             if (!wait(v_full, one(j)) || !wait(p_full(j), two(j))) return false;
             tiles_fence_after();
-            if (lane == 0) {
-                const uint64_t v0 = tiles_desc(base + S::OFF_V, TILE * 128, 1024);
+            {
+                const uint32_t v0 = tiles_desc(base + S::OFF_V, TILE * 128);
 #pragma unroll
                 for (int e = 0; e < TILE / 16; ++e)
-                    tiles_mma_ts(tmem + S::COL_O, tmem + S::COL_P + (j & 1) * (TILE / 2) + e * 8, v0 + (e * 2048 >> 4), idesc_o, e > 0 || !opens);
-                tiles_commit(o_done(j));
+                    tiles_mma_ts(lane == 0, tmem + S::COL_O, tmem + S::COL_P + (j & 1) * (TILE / 2) + e * 8, v0 + (e * 2048 >> 4), idesc_o, e > 0 || !opens);
             }
+            if (lane == 0) tiles_commit(o_done(j));
             __syncwarp();
             return true;
         };
