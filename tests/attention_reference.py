@@ -73,10 +73,14 @@ class Case:
         self.offsets = offsets
         return self
 
+    crowd = 0          # sequences without rows behind the others: a mean sequence has few rows then, which another kernel takes
+
     def batch(self, positions=None, rows=None, contexts=None):
         from turbo_fieldfare_b200 import attention as at
         i32 = dict(dtype=torch.int32, device=self.device)
-        return at.KVBatch(torch.tensor(self.offsets, **i32), torch.tensor(self.contexts if contexts is None else contexts, **i32), self.table.to(self.device),
+        contexts = list(self.contexts if contexts is None else contexts) + [0] * self.crowd
+        table = torch.cat([self.table, torch.full((self.crowd, self.table.shape[1]), -1, dtype=torch.int32)])
+        return at.KVBatch(torch.tensor(self.offsets + self.offsets[-1:] * self.crowd, **i32), torch.tensor(contexts, **i32), table.to(self.device),
                           None if positions is None else torch.as_tensor(positions, **i32), rows=self.offsets[-1] if rows is None else rows)
 
     def stored(self, b, first):

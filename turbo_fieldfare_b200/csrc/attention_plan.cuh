@@ -6,11 +6,10 @@
 
 namespace tf {
 
-// What a worker (a thread block or a warp) leaves for the unit that its share ends in: where the other shares are and which rows they hold.
+// What a block of the kernel for many rows leaves for the unit that its share ends in: where the other shares are and which rows they hold.
 struct ShareInfo {
     uint32_t active, last;
     uint32_t row0, flat0, valid, head;    // first row of the sequence; first (token, head) row of the unit and how many; kv head
-    uint64_t unused;
 };
 
 struct AttnArgs {

@@ -1,4 +1,4 @@
-// Attention over the quantised, paged cache for units of at most eight (or sixteen) rows: decode steps and small trees.
+// Attention over the quantised, paged cache for units of at most eight rows: decode steps and small trees.
 //
 // What bounds it is HBM: a cached token's codes and planes are read once and used for a handful of rows. So everything that is not
 // unpacking is kept out of the way. A worker is one warp: it owns its share of the tiles (16 tokens each), its ring of stages, filled by its own
@@ -37,7 +37,6 @@ struct RowsShape {
     static constexpr int SWAP = SPLIT > 1 ? 2 * WARPS * kWarp * NR * 16 : 0;                       // logits of the other warp, by turns in two buffers
     static constexpr int FIT = (227 * 1024 / BLOCKS - 1024 - 256 - SWAP) / (WARPS * STAGE), STAGES = FIT > 8 ? 8 : FIT;
     static constexpr int SMEM = WARPS * STAGES * STAGE + SWAP;
-    static constexpr int GH = G;                               // groups whose planes are in registers at a time
     static_assert(STAGES >= 2 && STAGE % 128 == 0, "a ring needs two stages");
     // 16-byte pieces are moved within their 128-byte lines so that the reads of a quarter or half warp meet every bank once
     static __host__ __device__ __forceinline__ uint32_t k_at(uint32_t row, uint32_t byte) {
@@ -95,49 +94,45 @@ __device__ __forceinline__ uint32_t rows_pair(float lo, float hi) {
 __device__ __forceinline__ int rows_exponent(float v) { return max(-126, min((int)((__float_as_uint(v) >> 23) & 255u) - 127, 126)); }
 __device__ __forceinline__ float rows_power(int e) { return __uint_as_float((uint32_t)(max(-126, min(e, 127)) + 127) << 23); }
 
-// bf16 values of one token in the N groups from `first` on, of planes of G groups.
-template <int G, int N>
+// bf16 values of one token's G groups.
+template <int G>
 struct TokenPlane {
-    uint32_t w[N / 2 + (N == 1)];
-    __device__ __forceinline__ void load(const uint8_t* plane, int token, int first) {
-        const uint8_t* p = plane + token * (2 * G) + 2 * first;
-        if constexpr (N == 1) w[0] = *reinterpret_cast<const uint16_t*>(p);
-        else if constexpr (N == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
+    uint32_t w[G / 2 + (G == 1)];
+    __device__ __forceinline__ void load(const uint8_t* plane, int token) {
+        const uint8_t* p = plane + token * (2 * G);
+        if constexpr (G == 1) w[0] = *reinterpret_cast<const uint16_t*>(p);
+        else if constexpr (G == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
         else { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
     }
     __device__ __forceinline__ float at(int grp) const { return __uint_as_float(grp % 2 ? w[grp / 2] & 0xFFFF0000u : w[grp / 2] << 16); }
 };
 
-// bf16 values of two neighbouring tokens (2i, then 2i + 1) in the N groups from `first` on, of planes of G groups. N = 1: one word holds both.
-template <int G, int N>
+// bf16 values of two neighbouring tokens (2i, then 2i + 1) in G groups. G = 1: one word holds both.
+template <int G>
 struct PlanePair {
-    uint32_t w[N];
-    __device__ __forceinline__ void load(const uint8_t* plane, int pair, int first) {
-        const uint8_t* p = plane + pair * (4 * G) + 2 * first;
-        if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
-        else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
-        else if constexpr (N == G) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
-        else {
-            const uint2 v0 = *reinterpret_cast<const uint2*>(p), v1 = *reinterpret_cast<const uint2*>(p + 2 * G);
-            w[0] = v0.x; w[1] = v0.y; w[2] = v1.x; w[3] = v1.y;
-        }
+    uint32_t w[G];
+    __device__ __forceinline__ void load(const uint8_t* plane, int pair) {
+        const uint8_t* p = plane + pair * (4 * G);
+        if constexpr (G == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else if constexpr (G == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+        else { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
     }
     __device__ __forceinline__ float at(int token, int grp) const {
-        const int i = token * N + grp;
+        const int i = token * G + grp;
         return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
     }
     __device__ __forceinline__ void raise_all(__nv_bfloat162& most) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+        for (int i = 0; i < G; ++i) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
     }
-    // The largest magnitudes of either token so far, in both halves of its word (N = 1: both tokens' in the first word); a NaN stays.
+    // The largest magnitudes of either token so far, in both halves of its word (G = 1: both tokens' in the first word); a NaN stays.
     __device__ __forceinline__ void raise(__nv_bfloat162& most0, __nv_bfloat162& most1) const {
         auto word = [&](int i) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])); };
-        if constexpr (N == 1) {
+        if constexpr (G == 1) {
             most0 = __hmax2_nan(most0, word(0));
         } else {
-            __nv_bfloat162 a = word(0), b = word(N / 2);
-            if constexpr (N == 4) { a = __hmax2_nan(a, word(1)); b = __hmax2_nan(b, word(3)); }
+            __nv_bfloat162 a = word(0), b = word(G / 2);
+            if constexpr (G == 4) { a = __hmax2_nan(a, word(1)); b = __hmax2_nan(b, word(3)); }
             most0 = __hmax2_nan(most0, __hmax2_nan(a, __lowhigh2highlow(a)));
             most1 = __hmax2_nan(most1, __hmax2_nan(b, __lowhigh2highlow(b)));
         }
@@ -516,14 +511,11 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             // ---- logits: rows of the accumulator are tokens g and g + 8, columns the rows 2t and 2t + 1 of q ----
             float x[NR][4] = {};
             const uint8_t* planes = st + 2 * S::CODES;
-            TokenPlane<G, S::GH> ks_lo, ks_hi, kb_lo, kb_hi;
+            TokenPlane<G> ks_lo, ks_hi, kb_lo, kb_hi;
+            ks_lo.load(planes, g); ks_hi.load(planes, g + 8);
+            kb_lo.load(planes + S::PLANE, g); kb_hi.load(planes + S::PLANE, g + 8);
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
-                if (grp % S::GH == 0) {
-                    ks_lo.load(planes, g, grp); ks_hi.load(planes, g + 8, grp);
-                    kb_lo.load(planes + S::PLANE, g, grp); kb_hi.load(planes + S::PLANE, g + 8, grp);
-                }
-                const int gh = grp % S::GH;
                 uint32_t w[2][4];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
@@ -553,7 +545,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                         else rows_mma(acc[n], a0, a1, a2, a3, qf[n][grp * 4 + ks][0], qf[n][grp * 4 + ks][1]);
                     }
                 }
-                const float s0 = ks_lo.at(gh), s1 = ks_hi.at(gh), b0 = kb_lo.at(gh), b1 = kb_hi.at(gh);
+                const float s0 = ks_lo.at(grp), s1 = ks_hi.at(grp), b0 = kb_lo.at(grp), b1 = kb_hi.at(grp);
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
                     x[n][0] = fmaf(s0, acc[n][0], fmaf(b0, q_sum[n][grp][0], x[n][0]));
@@ -621,26 +613,23 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
 
             // ---- does a maximum or a row's exponent move, is a value plane not finite? ----
             const uint8_t *vs_plane = planes + 2 * S::PLANE, *vb_plane = vs_plane + S::PLANE;
-            PlanePair<G, S::GH> vs_lo, vs_hi, vb_lo, vb_hi;
-            auto load_value_planes = [&](int first) {
-                vs_lo.load(vs_plane, t, first); vs_hi.load(vs_plane, t + 4, first);
-                vb_lo.load(vb_plane, t, first); vb_hi.load(vb_plane, t + 4, first);
+            PlanePair<G> vs_lo, vs_hi, vb_lo, vb_hi;
+            auto load_value_planes = [&] {
+                vs_lo.load(vs_plane, t); vs_hi.load(vs_plane, t + 4);
+                vb_lo.load(vb_plane, t); vb_hi.load(vb_plane, t + 4);
             };
             const __nv_bfloat162 none = __float2bfloat162_rn(0.0f), finite = __halves2bfloat162(__ushort_as_bfloat16(0x7F7F), __ushort_as_bfloat16(0x7F7F));
             __nv_bfloat162 most_s[4] = {none, none, none, none}, most_b = none;     // per token; a NaN stays
-#pragma unroll
-            for (int first = 0; first < G; first += S::GH) {
-                load_value_planes(first);
-                vs_lo.raise(most_s[0], most_s[1]); vs_hi.raise(most_s[2], most_s[3]);
-                vb_lo.raise_all(most_b); vb_hi.raise_all(most_b);
-            }
+            load_value_planes();
+            vs_lo.raise(most_s[0], most_s[1]); vs_hi.raise(most_s[2], most_s[3]);
+            vb_lo.raise_all(most_b); vb_hi.raise_all(most_b);
             bool moves = over > 8.0f || !__hble2(most_b, finite);
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 float most = 0.0f;
 #pragma unroll
                 for (int key = 0; key < 4; ++key) {
-                    const float s = S::GH == 1 ? __uint_as_float((*reinterpret_cast<const uint32_t*>(&most_s[key & 2])) << (key & 1 ? 0 : 16) & 0xFFFF0000u)
+                    const float s = G == 1 ? __uint_as_float((*reinterpret_cast<const uint32_t*>(&most_s[key & 2])) << (key & 1 ? 0 : 16) & 0xFFFF0000u)
                                                : __uint_as_float((*reinterpret_cast<const uint32_t*>(&most_s[key])) & 0xFFFF0000u);
                     most = rows_max_nan(most, p[n][key] * s);
                 }
@@ -674,7 +663,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
                             for (int n = 0; n < NR; ++n)
                                 if ((flags >> (key * G + grp) & 1u) && p[n][key] > 0.0f) b_sum[n][grp] = __int_as_float(0x7FC00000);
-                    load_value_planes(0);
+                    load_value_planes();
                 }
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
@@ -712,14 +701,12 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
             // ---- values ----
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
-                if (G > S::GH && grp % S::GH == 0) load_value_planes(grp);
-                const int gh = grp % S::GH;
                 uint32_t pb[NR][2];
                 float s[4], b[4];
 #pragma unroll
                 for (int key = 0; key < 4; ++key) {
-                    s[key] = key < 2 ? vs_lo.at(key, gh) : vs_hi.at(key - 2, gh);
-                    b[key] = key < 2 ? vb_lo.at(key, gh) : vb_hi.at(key - 2, gh);
+                    s[key] = key < 2 ? vs_lo.at(key, grp) : vs_hi.at(key - 2, grp);
+                    b[key] = key < 2 ? vb_lo.at(key, grp) : vb_hi.at(key - 2, grp);
                 }
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {

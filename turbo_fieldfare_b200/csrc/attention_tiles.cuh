@@ -1,13 +1,20 @@
 // Attention over the quantised, paged cache for units of up to 128 rows (trees and chains): tcgen05 with tensor-memory accumulators.
 //
 // With this many rows the products bound it, 4 * 128 * D FLOP per token and unit, next to the unpacking, which a unit pays once for its 128 rows.
-// One persistent block per SM; 8 warps unpack, one issues the MMAs, 4 do the softmax, a thread per row. For tile i of TILE tokens:
-//   unpack:  codes and planes, by cp.async a tile ahead into places of the thread's own -> K_i, V_i in fp16, [64 elements][token][128 bytes] with the
-//            128-byte swizzle (K in two buffers but for heads of 512, V in one: V_(i+1) is unpacked behind K_(i+2), while O takes V_i)
+// One persistent block per SM: 8 warps of softmax, two threads to a row; 8 that unpack; two that measure the planes; a loader; one that issues the
+// MMAs. For tile i of TILE tokens:
+//   loader:  codes and planes by bulk copies, as they lie in the cache; a page's run of tokens is one copy
+//   measure: a token's power of two (below), and scale and centred bias of its groups as fp16
+//   unpack:  K_i, V_i in fp16, [64 elements][token][128 bytes] with the 128-byte swizzle (K in two buffers but for heads of 512, V in one: V_(i+1) is
+//            unpacked behind K_(i+2), while O takes V_i)
 //   MMA:     S_i = Q K_i^T into tensor memory (two buffers), then O += P_(i-1) V_(i-1); K is K-major, V, as it lies, MN-major
 //   softmax: S_i -> registers -> mask, 2^(x - m), P_i as fp16 into tensor memory (the A operand of the second product)
-// The loops are rolled where registers allow it: three kinds of warps share an SM's instruction caches, and straight-line code of all of them
-// waited for instructions most of the time (9600 clocks a tile instead of what the notes of the measurements give).
+// What it measured: 8 trees of 61 rows over 8000 tokens, 16 heads of 256 on 8 kv heads, 8 bits: 102 us, 1.9 TB/s and 329 TFLOP/s; 333 rows over 8000
+// cached tokens, the same heads: 111 us, 408 TFLOP/s. A tile of 64 tokens takes about 4000 clocks, of which the tensor cores are busy for 1000. The
+// rest is instructions that wait for one another: the warps' roles do not share code, so what a role takes must be short. Bodies are rolled
+// and stand once (one for K and V), a wait that is over takes one look, the MMAs are issued without a branch, and the usual tile, which every row sees
+// and whose powers of two are 1, leaves out the rest: in this order 139 -> 131 -> 114 -> 101 us. The warps that unpack were 8 that also
+// loaded and measured: 127 us with all of the above left out.
 // K_i and V_i carry (code - centre) s + (bias + centre s) rounded to fp16, 2^-11 of the value: logits see it as an error of about 2^-12 |q||k| / sqrt(D),
 // of the size of the output's own rounding to 16 bits. A token's values are divided by a power of two of its own first; K's comes back with the
 // logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far: tokens that a row
@@ -834,7 +841,8 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
     }
 }
 
-// Joins the shares of the unit that block c's share ends in: a warp per row, lanes over the elements.
+// Joins the shares of the unit that block c's share ends in: a warp per row, lanes over the elements. A second launch, which is on its way while the
+// first one ends: it adds 3 us to the call.
 constexpr int kTilesJoinThreads = 128;
 template <int D, int DV, bool BF16>
 __global__ void __launch_bounds__(kTilesJoinThreads)
@@ -903,9 +911,13 @@ static tf_status launch_tiles(tf_context* ctx, cudaStream_t st, const AttnArgs& 
 
 template <int D, int BITS>
 tf_status attend(tf_context* ctx, cudaStream_t st, const AttnArgs& a, const tf_attention_workspace* ws, bool bf16) {
-    // Rows of one kv head in a mean sequence. Units of eight rows read the cache once each, units of 128 once for all.
-    const uint64_t mean = ((uint64_t)a.rows + a.sequences - 1) / a.sequences * a.group;
-    if (mean <= 32) return bf16 ? launch_rows<D, BITS, 8, true>(ctx, st, a, ws) : launch_rows<D, BITS, 8, false>(ctx, st, a, ws);
+    // Rows of one kv head in a mean sequence: units of eight read and unpack the cache once each, units of 128 once for all, but cost more to enter and leave,
+    // so it takes more rows where there are many units; where there are few, many warps share one of eight, and joining their shares costs a few us per row.
+    // Measured in us, eight / 128: 8 * 2 units of 4000 tokens with heads of 256, 4 rows: 48 / 36, 1 row: 34 / 36; 8 * 8 of 8000, 16 rows: 127 / 127, 24: 160 / 127;
+    // 8 * 32 of 3000 with 4-bit heads of 128, 24 rows: 134 / 124, of 1800 on average, 28 rows: 84 / 110. Heads of 512 are two units each, whose tiles
+    // are of 32 tokens: 2 * 32 units of 4000, 32 rows: 176 / 272, 48: 248 / 279.
+    const uint64_t mean = ((uint64_t)a.rows + a.sequences - 1) / a.sequences * a.group, units = (uint64_t)a.sequences * a.kv_heads * (D == 512 ? 4 : 1);
+    if (mean <= (units <= 32 ? 4 : units <= 128 ? 16 : 32)) return bf16 ? launch_rows<D, BITS, 8, true>(ctx, st, a, ws) : launch_rows<D, BITS, 8, false>(ctx, st, a, ws);
     return bf16 ? launch_tiles<D, BITS, true>(ctx, st, a, ws) : launch_tiles<D, BITS, false>(ctx, st, a, ws);
 }
 
