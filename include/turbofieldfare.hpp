@@ -207,6 +207,67 @@ private:
     const Context& c_;
 };
 
+// Scratch of TreeAttention for one head size; serves one call at a time.
+class AttentionWorkspace {
+public:
+    AttentionWorkspace(const Context& c, uint32_t headDim) { c.check(tf_attention_workspace_create(c.handle(), headDim, &w_)); }
+    ~AttentionWorkspace() { tf_attention_workspace_destroy(w_); }
+    AttentionWorkspace(const AttentionWorkspace&) = delete;
+    AttentionWorkspace& operator=(const AttentionWorkspace&) = delete;
+    tf_attention_workspace* handle() const { return w_; }
+private:
+    tf_attention_workspace* w_ = nullptr;
+};
+
+// Rows of heads: what the attention calls take as tensor and stride in elements.
+struct RowsRef {
+    const void* rows = nullptr;
+    uint32_t stride = 0;
+};
+struct MutableRowsRef {
+    void* rows = nullptr;
+    uint32_t stride = 0;
+};
+
+// fused_qkv_epilogue (Metal/Fusions/fused.metal:86): head norms, rotation, cache write.
+class FusedQKVEpilogue {
+public:
+    explicit FusedQKVEpilogue(const Context& c) : c_(c) {}
+    void encode(void* stream, RowsRef q, RowsRef k, RowsRef v, MutableRowsRef qOut, const tf_kv_batch& batch, const tf_kv_cache* cache,
+                uint32_t qHeads, uint32_t kvHeads, uint32_t headDim, const void* qWeight = nullptr, const void* kWeight = nullptr, bool normV = false,
+                const float* frequencies = nullptr, uint32_t rotatedPairs = 0, MutableRowsRef kOut = {}, MutableRowsRef vOut = {},
+                float eps = 1e-6f, tf_dtype type = TF_FP16) const {
+        c_.check(tf_qkv_epilogue(c_.handle(), stream, q.rows, q.stride, k.rows, k.stride, v.rows, v.stride, qWeight, kWeight, normV, frequencies,
+                                 rotatedPairs, eps, qOut.rows, qOut.stride, kOut.rows, kOut.stride, vOut.rows, vOut.stride, &batch, cache, qHeads,
+                                 kvHeads, headDim, type));
+    }
+private:
+    const Context& c_;
+};
+
+class KVCacheRead {
+public:
+    explicit KVCacheRead(const Context& c) : c_(c) {}
+    void encode(void* stream, const tf_kv_cache& cache, const tf_kv_batch& batch, MutableRowsRef kOut, MutableRowsRef vOut, tf_dtype type = TF_FP16) const {
+        c_.check(tf_kv_cache_read(c_.handle(), stream, &cache, &batch, kOut.rows, kOut.stride, vOut.rows, vOut.stride, type));
+    }
+private:
+    const Context& c_;
+};
+
+// Attention (Metal/Attention/attention.metal:135,227,343; Metal/Prefill/prefill.metal:836) over the cache: one token, a chain or a tree per sequence.
+class TreeAttention {
+public:
+    explicit TreeAttention(const Context& c) : c_(c) {}
+    void encode(void* stream, RowsRef q, MutableRowsRef out, const tf_kv_cache& cache, const tf_kv_batch& batch, const AttentionWorkspace& workspace,
+                uint32_t qHeads, float scale, uint32_t window = 0, const uint64_t* treeMask = nullptr, uint32_t maskWords = 0, tf_dtype type = TF_FP16) const {
+        c_.check(tf_tree_attention(c_.handle(), stream, q.rows, q.stride, out.rows, out.stride, &cache, &batch, treeMask, maskWords, window, scale, qHeads,
+                                   type, workspace.handle()));
+    }
+private:
+    const Context& c_;
+};
+
 // ManifestReader + PackedExpertsLayoutReader + ResidentIndexReader in one handle
 // (Infrastructure/ModelIO/ManifestReader.swift:64-152, PackedExpertsLayout.swift:57-119, ResidentIndex.swift:44-140):
 // opening validates the three documents the way the Swift codecs do; ModelError / GTurboFormatError become Error

@@ -821,7 +821,8 @@ tf_status tf_stack_forward_ep(tf_ep* ep, void* stream, const tf_moe_layer* layer
  * value = code * scale + bias) with 8- or 4-bit codes (4-bit: low nibble = even column). Caller-owned device planes:
  *   codes          [num_pages][kv_heads][page_size][head_dim * bits / 8] bytes
  *   scales, biases [num_pages][kv_heads][page_size][head_dim / 64] bf16
- * page_size: a power of two from 16 to 65536; head_dim: 64, 128, 256 or 512; every plane 16-byte aligned. The
+ * page_size: a power of two from 16 to 65536; head_dim: 64, 128, 256 or 512; every plane 16-byte aligned;
+ * num_pages * kv_heads * page_size below 2^32 - 1 (TF_ERR_UNSUPPORTED beyond). The
  * reference keeps fp16 rings and linear buffers (Runtime/KVCache/KVCacheManager.swift:26-50). */
 typedef struct tf_kv_cache {
     void *k_codes, *k_scales, *k_biases, *v_codes, *v_scales, *v_biases;
@@ -855,9 +856,10 @@ typedef struct tf_kv_batch {
  * Quantising is that of the weights (Quantization.swift:63-101,135-176): scale = bf16((max - min) / (2^bits - 1)), bias =
  * bf16(min), scale 1 where max == min; a group that holds an infinity or a NaN gets NaN planes and reads back as NaN.
  * q, k, v are act_dtype rows [rows][heads * head_dim] with strides in elements (one packed row may hold all three); k and
- * v may be the same rows. Outputs may be their own inputs, but k_out may not be k where v is k too. Pointers must be
+ * v may be the same rows. An output may be its own input (with its stride), but where v is k neither k_out nor v_out; other overlaps
+ * are not looked for. Pointers must be
  * 16-byte aligned and strides multiples of 8. Tokens of one call must be distinct: two rows that name the same slot of a page
- * (a page shared by two sequences that both append to it) leave either's values, group by group.
+ * (a page shared by two sequences that both append to it) leave a mixture of both there.
  * With cache == NULL only `rows` and `positions` of the batch are read, and all rows are done.
  * Replaces fused_qkv_epilogue (Metal/Fusions/fused.metal:86), the per-head norms (Metal/Primitives/rmsnorm.metal:101,128),
  * rope_default_neox / rope_proportional_neox (Metal/Primitives/rope.metal:52,75) and the KV blit. */
@@ -880,7 +882,7 @@ tf_status tf_kv_cache_read(tf_context* ctx, void* stream, const tf_kv_cache* cac
 
 /* Scratch of tf_tree_attention for one head_dim: partial results of long sequences that several thread blocks share.
  * A workspace serves one call at a time: calls that may overlap on the GPU (other streams, graphs replayed side by
- * side) need one each. Nothing in it has to survive between calls. */
+ * side) need one each. A call leaves it as it found it, so that any later call may use it. */
 typedef struct tf_attention_workspace tf_attention_workspace;
 tf_status tf_attention_workspace_create(tf_context* ctx, uint32_t head_dim, tf_attention_workspace** out);
 void tf_attention_workspace_destroy(tf_attention_workspace* ws);
@@ -896,7 +898,8 @@ uint64_t tf_attention_workspace_bytes(const tf_attention_workspace* ws);
  * A row that sees nothing becomes zero. Infinities and NaN in the cache reach only the rows that see them.
  * positions are read only with a tree_mask and a window. q and out: act_dtype rows [rows][q_heads * head_dim], 16-byte
  * aligned, strides multiples of 8; out may be q. softmax and sums are fp32.
- * Any number of rows, contexts and sequences; the lengths stay on the device, and the call can be captured.
+ * Any number of rows, contexts and sequences; the lengths stay on the device, and the call can be captured. Equal calls give equal
+ * bits. Every wait inside is bounded: one that runs out ends the call, and tf_device_status reports 0x7F000053.
  * Replaces attention_decode_partial / _gqa_swa_partial / _combine (Metal/Attention/attention.metal:135,227,343) and
  * attention_prefill_causal_tiled (Metal/Prefill/prefill.metal:836); the reference drafts no tokens. */
 tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32_t q_stride_elements,

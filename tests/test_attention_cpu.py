@@ -1,4 +1,5 @@
 """Attention operators without a GPU: the shares of every block, the addresses in shared memory, pages that are not there, refusals."""
+import shutil
 import subprocess
 from pathlib import Path
 
@@ -354,3 +355,45 @@ def test_rows_of_tensors():
     for t, rows, cols in ((x, 5, 96), (x, 4, 95), (x.t(), 4, 4), (x.float(), 4, 96), (x[0], 1, 96), (x[:, ::2], 4, 48)):
         with pytest.raises(ValueError):
             _row_stride("x", t, cpu, torch.float16, rows, cols)
+
+
+MIRROR = r'''
+#include <cstdio>
+#include "turbofieldfare.hpp"
+namespace tf = turbofieldfare;
+int main() {
+    try {
+        tf::Context ctx(0);
+        alignas(16) static char mem[64];
+        const tf_kv_cache cache = {mem, mem, mem, mem, mem, mem, 1, 16, 1, 64, 5};
+        const tf_kv_batch batch = {};
+        tf::AttentionWorkspace workspace(ctx, 64);
+        int refused = 0;
+        auto expect = [&](auto call) { try { call(); } catch (const tf::Error&) { ++refused; } };
+        expect([&] { tf::TreeAttention(ctx).encode(nullptr, {mem, 64}, {mem, 64}, cache, batch, workspace, 1, 1.0f); });
+        expect([&] { tf::KVCacheRead(ctx).encode(nullptr, cache, batch, {mem, 64}, {}); });
+        expect([&] { tf::FusedQKVEpilogue(ctx).encode(nullptr, {mem, 64}, {mem, 64}, {mem, 64}, {mem, 64}, batch, &cache, 1, 1, 64); });
+        expect([&] { tf::AttentionWorkspace bad(ctx, 96); });
+        std::printf("refused %d\n", refused);
+        return refused == 4 ? 0 : 1;
+    } catch (const tf::Error& e) {
+        std::printf("status %d\n", e.status);
+        return e.status == TF_ERR_NO_DEVICE ? 0 : 2;
+    }
+}
+'''
+
+
+def test_cpp_mirror_of_the_attention_calls(tmp_path):
+    """The classes of include/turbofieldfare.hpp compile, link, and hand on what the library refuses (no work on a device)."""
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    from turbo_fieldfare_b200 import build as tf_build
+    lib = tf_build.build(verbose=False)
+    src, exe = tmp_path / "mirror.cpp", tmp_path / "mirror"
+    src.write_text(MIRROR)
+    subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-Werror", "-I", str(ROOT / "include"), "-I", "/usr/local/cuda/include", str(src), "-o", str(exe),
+                    "-L", str(lib.parent), "-ltfcuda", f"-Wl,-rpath,{lib.parent}"], check=True, capture_output=True, text=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout + run.stderr

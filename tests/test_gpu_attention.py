@@ -418,7 +418,8 @@ def _check_stored(case, rows_of, y, size, first):
 
 
 @pytest.mark.parametrize("dim,pairs", [(64, 32), (64, 6), (128, 64), (128, 0), (256, 128), (256, 32), (512, 64), (512, 256)])
-@pytest.mark.parametrize("bits,dtype,rows,contexts", [(8, F16, [1], [0]), (4, BF16, [3, 1, 0, 5], [70, 900000, 3, 12]), (8, BF16, [90, 70], [1, 33])])
+@pytest.mark.parametrize("bits,dtype,rows,contexts", [(8, F16, [1], [0]), (4, BF16, [3, 1, 0, 5], [70, 900000, 3, 12]), (8, BF16, [90, 70], [1, 33]),
+                                                       (8, F16, [300, 0, 221, 33], [5, 2, 40, 64]), (4, BF16, [7] * 90, list(range(90)))])
 def test_epilogue_writes_the_cache(tf_ctx, dim, pairs, bits, dtype, rows, contexts):
     heads, kv = 6, 2
     case = Case(dim + pairs, rows, [min(c, 100) for c in contexts], kv, dim, bits, 16, DEV).upload()
@@ -494,6 +495,30 @@ def test_epilogue_padded_rows_equal_groups_and_values_that_are_not_finite(tf_ctx
     assert torch.isnan(k_out[2, :64]).all() and torch.isfinite(k_out[2, 64:]).all()
     changed = sum(int((a.view(torch.uint8) != b.view(torch.uint8)).flatten(3).any(-1).any(1).sum()) > 0 for a, b in zip(before, case.cache.planes))
     assert changed == 6
+
+
+@pytest.mark.parametrize("rows", [1, 2, 37, 333])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 19, 11), (128, 1, 1), (256, 9, 3), (512, 17, 9)])
+def test_epilogue_in_place(tf_ctx, rows, dim, heads, kv):
+    """Numbers of heads that fill no block, every output over its own input: the same bits as beside it."""
+    gen = torch.Generator().manual_seed(rows)
+    case = Case(31, [rows], [3], kv, dim, 8, 16, DEV).upload()
+    q, k, v = (torch.randn(rows, n * dim, generator=gen).to(F16).to(DEV) for n in (heads, kv, kv))
+    w = (1 + 0.2 * torch.randn(dim, generator=gen)).bfloat16().to(DEV)
+    freqs = (1e4 ** (-torch.arange(dim // 4, dtype=F64) / (dim // 4))).float().to(DEV)
+    batch, op = case.batch(torch.arange(3, 3 + rows)), _ops(tf_ctx)[0]
+    beside = [torch.zeros_like(t) for t in (q, k, v)]
+    op.encode(q, k, v, beside[0], batch, case.cache, head_dim=dim, q_weight=w, k_weight=w, norm_v=True, frequencies=freqs, k_out=beside[1], v_out=beside[2])
+    planes = [p.clone() for p in case.cache.planes]
+    raw = q.cpu()
+    op.encode(q, k, v, q, batch, case.cache, head_dim=dim, q_weight=w, k_weight=w, norm_v=True, frequencies=freqs, k_out=k, v_out=v)
+    assert tf_ctx.device_status() == 0
+    for a, b in zip((q, k, v), beside):
+        assert torch.equal(a, b)
+    for a, b in zip(case.cache.planes, planes):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    y, size = _definition(raw.unflatten(-1, (-1, dim)), w.cpu(), 1e-6, True, freqs.cpu(), torch.arange(3, 3 + rows))
+    _close(q, y.flatten(1), (half_step(F16) * y.abs() + 2.0 ** -19 * size + 1e-7).flatten(1))
 
 
 def test_epilogue_far_positions(tf_ctx):
