@@ -16,7 +16,7 @@ tf_status tf_attention_workspace_create(tf_context* ctx, uint32_t head_dim, tf_a
     TF_REQUIRE(ctx, ws != nullptr, TF_ERR_OUT_OF_MEMORY, "%s: out of host memory", name);
     ws->device = ctx->device;
     ws->head_dim = head_dim;
-    ws->row_capacity = (uint32_t)ctx->sm_count * 128;          // two blocks of 64 rows per SM, or eight of 16
+    ws->row_capacity = (uint32_t)ctx->sm_count * 128;          // per SM: a block with a unit of 128 rows, or 16 workers with units of eight
     ws->max_workers = (uint32_t)ctx->sm_count * 16;
     const uint64_t partial = (uint64_t)2 * ws->row_capacity * (head_dim + 4) * sizeof(float), info = (uint64_t)ws->max_workers * sizeof(tf::ShareInfo);
     cudaError_t e = cudaMalloc(&ws->partial, partial);

@@ -15,6 +15,11 @@
 // accumulator, against sum p (b + centre s). E is a row's own, after the largest p s so far (tokens that it does not see have p = 0
 // and no say), and m a maximum that is raised only when a logit exceeds it by 8: one vote per tile, and what was summed is
 // rescaled only when one of them moves.
+//
+// What it measured, 8-bit heads of 256 on 8 kv heads, two rows each: 64 sequences of up to 4096 tokens 130 us, 4.9 TB/s; 131000 tokens of one sequence, heads of
+// 128: 75 us, 3.7 TB/s; 4-bit heads of 512, 200 sequences of up to 8192 tokens, eight rows per kv head: 310 us, 3.6 TB/s, bound by unpacking (2200 clocks a
+// tile with two warps to a scheduler). The same with blocks that share tiles behind barriers: 268, 178, 768 us. Units of 16 rows, which would unpack half as
+// often, need so many registers that a third of the warps goes: no faster at 28 rows.
 #pragma once
 
 #include "attention_launch.cuh"

@@ -4,7 +4,7 @@
 // One persistent block per SM: 8 warps of softmax, two threads to a row; 8 that unpack; two that measure the planes; a loader; one that issues the
 // MMAs. For tile i of TILE tokens:
 //   loader:  codes and planes by bulk copies, as they lie in the cache; a page's run of tokens is one copy
-//   measure: a token's power of two (below), and scale and centred bias of its groups as fp16
+//   measure: a token's power of two (below), and scale and bias of its groups as fp16
 //   unpack:  K_i, V_i in fp16, [64 elements][token][128 bytes] with the 128-byte swizzle (K in two buffers but for heads of 512, V in one: V_(i+1) is
 //            unpacked behind K_(i+2), while O takes V_i)
 //   MMA:     S_i = Q K_i^T into tensor memory (two buffers), then O += P_(i-1) V_(i-1); K is K-major, V, as it lies, MN-major
@@ -15,8 +15,9 @@
 // and stand once (one for K and V), a wait that is over takes one look, the MMAs are issued without a branch, and the usual tile, which every row sees
 // and whose powers of two are 1, leaves out the rest: in this order 139 -> 131 -> 114 -> 101 us. The warps that unpack were 8 that also
 // loaded and measured: 127 us with all of the above left out.
-// K_i and V_i carry (code - centre) s + (bias + centre s) rounded to fp16, 2^-11 of the value: logits see it as an error of about 2^-12 |q||k| / sqrt(D),
-// of the size of the output's own rounding to 16 bits. A token's values are divided by a power of two of its own first; K's comes back with the
+// K_i and V_i carry code * scale + bias rounded once to fp16, 2^-12 of the value, and P its probabilities likewise: each adds an error of the size
+// of the output's own rounding to fp16 (together 4e-4 to 5e-4 of the output's norm against 64 bits, 2e-4 of which fp16 outputs have anyhow; nothing next to
+// bf16's 1.7e-3). Exact products of codes, as the kernel for few rows has them, would need an accumulator per group. A token's values are divided by a power of two of its own first; K's comes back with the
 // logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far: tokens that a row
 // does not see have no say, and no cache leaves fp16's range. m is raised only when a logit exceeds it by 8, and what O holds is
 // rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
@@ -123,7 +124,7 @@ __device__ __forceinline__ void tiles_wait_st() { asm volatile("tcgen05.wait::st
 __device__ __forceinline__ void tiles_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tiles_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Sixteen codes as (code - centre) s + b in fp16, two 16-byte chunks of eight elements. 4-bit codes of eight elements come in the order
+// Sixteen codes as code * s + b in fp16, rounded once (code, s and b are fp16 numbers), two 16-byte chunks of eight elements. 4-bit codes of eight elements come in the order
 // (0, 4, 1, 5, 2, 6, 3, 7), as one mask yields them: the rows of q are laid out alike, and the product's columns are put back at the end.
 template <int BITS>
 __device__ __forceinline__ void tiles_unpack(const uint32_t (&w)[BITS / 2], __half2 s, __half2 b, uint4 (&out)[2]) {
@@ -135,18 +136,18 @@ __device__ __forceinline__ void tiles_unpack(const uint32_t (&w)[BITS / 2], __ha
     if constexpr (BITS == 8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            put(2 * i, gm_prmt(w[i], 0x64646464u, 0x4140), -1152.0f, s);             // 1024 from the bits, 128 the centre
-            put(2 * i + 1, gm_prmt(w[i], 0x64646464u, 0x4342), -1152.0f, s);
+            put(2 * i, gm_prmt(w[i], 0x64646464u, 0x4140), -1024.0f, s);             // 1024 from the bits
+            put(2 * i + 1, gm_prmt(w[i], 0x64646464u, 0x4342), -1024.0f, s);
         }
     } else {
         const __half2 s16 = __hmul2(s, __float2half2_rn(0.0625f));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t v = w[i] >> 8;
-            put(4 * i, (w[i] & 0x000F000Fu) | 0x64006400u, -1032.0f, s);
-            put(4 * i + 1, (w[i] & 0x00F000F0u) | 0x64006400u, -1152.0f, s16);
-            put(4 * i + 2, (v & 0x000F000Fu) | 0x64006400u, -1032.0f, s);
-            put(4 * i + 3, (v & 0x00F000F0u) | 0x64006400u, -1152.0f, s16);
+            put(4 * i, (w[i] & 0x000F000Fu) | 0x64006400u, -1024.0f, s);
+            put(4 * i + 1, (w[i] & 0x00F000F0u) | 0x64006400u, -1024.0f, s16);
+            put(4 * i + 2, (v & 0x000F000Fu) | 0x64006400u, -1024.0f, s);
+            put(4 * i + 3, (v & 0x00F000F0u) | 0x64006400u, -1024.0f, s16);
         }
     }
     out[0] = make_uint4(h[0], h[1], h[2], h[3]);
@@ -307,7 +308,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         }
     } else if (warp >= S::MEASURE && warp < S::LOADER) {
         // ===================== what the planes say: one warp for K's, one for V's, a token per lane =====================
-        // Scale and centred bias of a token's groups as fp16, by a power of two of the token's. Values of ordinary sizes are fp16 numbers as they are, exact to
+        // Scale and bias of a token's groups as fp16 (exact, a bf16 has fewer bits), by a power of two of the token's. Values of ordinary sizes are fp16 numbers as they are, exact to
         // 2^-11 of the token's largest.
         const bool of_v = warp != S::MEASURE;
         const uint32_t run_log2 = lesser(a.table.page_log2, (uint32_t)(31 - __builtin_clz(TILE)));
@@ -325,11 +326,11 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
                 for (int g = 0; g < N; ++g) {
                     sc[g] = is ? bf16_bits_to_float(scales[g]) : 0.0f;
-                    bi[g] = is ? fmaf(kCentre, sc[g], bf16_bits_to_float(scales[S::PLANE / 2 + g])) : 0.0f;
+                    bi[g] = is ? bf16_bits_to_float(scales[S::PLANE / 2 + g]) : 0.0f;
                 }
 #pragma unroll
                 for (int g = 0; g < N; ++g) {
-                    const float size = fmaxf(kCentre * fabsf(sc[g]), fabsf(bi[g]));        // half of the largest value or more
+                    const float size = fmaxf(kCentre * fabsf(sc[g]), fabsf(bi[g]));        // a third of the largest value or more
                     const bool finite = sc[g] - sc[g] == 0.0f && bi[g] - bi[g] == 0.0f;
                     plain = plain && finite && size >= 0.001953125f && size <= 16384.0f;
                     most = finite ? fmaxf(most, size) : most;
