@@ -108,9 +108,12 @@ def visible(rows, context, window=0, masks=None, positions=None):
 def attention(case, q, see, scale, out_half_step):
     """(expected, tolerance) of [rows, heads * dim] 16-bit rows q (CPU), see: a truth table per sequence.
 
-    Tolerance, element by element, from the roundings that the kernel names (half steps 2^-11 of fp16): probabilities twice (product and sum),
-    values once and their centred bias once, the output; logits in fp32: products of a group in 4 steps, groups, factor, together under
-    2^-17 of sum |q||k|; probabilities below fp16's least step count as zero (2^-25 each, against a sum of at least one)."""
+    Tolerance, element by element, from the roundings that the kernels name (half steps 2^-11 of fp16): probabilities twice (product and sum),
+    values once and what a bias, centred, adds once, the output; logits in fp32: products of a group in 4 steps, groups, factor, together under
+    2^-17 of sum |q||k|; probabilities below fp16's least step count as zero (2^-25 each, against a sum of at least one). With many rows a key is
+    rounded to fp16 too and nothing is centred: each element moves the logit by up to 2^-12 |q_d k_d| scale, with a sign of its own, together
+    about 2^-12 sqrt(sum (q_d k_d)^2) scale, which is 2^-12 for logits of size one: the share of the centred bias and of a second rounding of the
+    probabilities, which that kernel does not have, holds it."""
     want, tol = [], []
     centre = 128.0 if case.bits == 8 else 8.0
     for b, n in enumerate(case.rows):

@@ -243,6 +243,15 @@ def test_queries_outside_of_fp16(tf_ctx, workspaces, q_scale):
     _close(got, *ref.attention(case, q, [ref.visible(2, 90), ref.visible(1, 300)], 0.2 / q_scale, half_step(BF16)))
 
 
+@pytest.mark.parametrize("scale", [-0.09, 0.0])
+@pytest.mark.parametrize("rows,contexts,dim,bits", [([1, 3], [300, 20], 128, 8), ([45, 2], [150, 700], 256, 4)])
+def test_scales_that_are_not_positive(tf_ctx, workspaces, scale, rows, contexts, dim, bits):
+    case = Case(14, rows, contexts, 2, dim, bits, 32, DEV).upload()
+    q = _q(case, 4, F16)
+    got = _run(tf_ctx, workspaces, case, q, F16, scale=scale, window=200)
+    _close(got, *ref.attention(case, q, [ref.visible(n, c, 200) for n, c in zip(rows, contexts)], scale, half_step(F16)))
+
+
 def test_peaked_logits(tf_ctx, workspaces):
     """Logits of hundreds: nearly all the weight on one token, and maxima that grow from tile to tile."""
     case = Case(11, [1, 5], [900, 500], 2, 256, 8, 64, DEV).upload()
