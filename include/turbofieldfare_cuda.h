@@ -882,7 +882,7 @@ tf_status tf_kv_cache_read(tf_context* ctx, void* stream, const tf_kv_cache* cac
 
 /* Scratch of tf_tree_attention for one head_dim: partial results of long sequences that several thread blocks share.
  * A workspace serves one call at a time: calls that may overlap on the GPU (other streams, graphs replayed side by
- * side) need one each. A call leaves it as it found it, so that any later call may use it. */
+ * side) need one each. What a call leaves in it does not matter to the next. */
 typedef struct tf_attention_workspace tf_attention_workspace;
 tf_status tf_attention_workspace_create(tf_context* ctx, uint32_t head_dim, tf_attention_workspace** out);
 void tf_attention_workspace_destroy(tf_attention_workspace* ws);
