@@ -897,7 +897,8 @@ uint64_t tf_attention_workspace_bytes(const tf_attention_workspace* ws);
  *     is the shortest), j <= i, and with a window i - j < window.
  * A row that sees nothing becomes zero. Infinities and NaN in the cache reach only the rows that see them.
  * positions are read only with a tree_mask and a window. q and out: act_dtype rows [rows][q_heads * head_dim], 16-byte
- * aligned, strides multiples of 8; out may be q. softmax and sums are fp32.
+ * aligned, strides multiples of 8; out may be q, with its stride (heads of 512 then go by units of eight rows, which takes many
+ * rows over long contexts up to 2.5 times as long). softmax and sums are fp32.
  * Any number of rows, contexts and sequences; the lengths stay on the device, and the call can be captured. Equal calls give equal
  * bits. Every wait inside is bounded: one that runs out ends the call, and tf_device_status reports 0x7F000053.
  * Replaces attention_decode_partial / _gqa_swa_partial / _combine (Metal/Attention/attention.metal:135,227,343) and

@@ -918,7 +918,9 @@ tf_status attend(tf_context* ctx, cudaStream_t st, const AttnArgs& a, const tf_a
     // 8 * 32 of 3000 with 4-bit heads of 128, 24 rows: 134 / 124, of 1800 on average, 28 rows: 84 / 110. Heads of 512 are two units each, whose tiles
     // are of 32 tokens: 2 * 32 units of 4000, 32 rows: 176 / 272, 48: 248 / 279.
     const uint64_t mean = ((uint64_t)a.rows + a.sequences - 1) / a.sequences * a.group, units = (uint64_t)a.sequences * a.kv_heads * (D == 512 ? 4 : 1);
-    if (mean <= (units <= 32 ? 4 : units <= 128 ? 16 : 32)) return bf16 ? launch_rows<D, BITS, 8, true>(ctx, st, a, ws) : launch_rows<D, BITS, 8, false>(ctx, st, a, ws);
+    // In place heads of 512 have units of eight: a unit of 128 rows reads all of a row of q for half of its values, and the other half's unit may do so
+    // later. Us beside / in place, 16 heads on 2: 200 trees of 5 rows over 40 tokens 84 / 80, 8 trees of 61 over 8000 532 / 1135, 333 rows over 8000 369 / 901.
+    if (mean <= (units <= 32 ? 4 : units <= 128 ? 16 : 32) || (D == 512 && a.out == a.q)) return bf16 ? launch_rows<D, BITS, 8, true>(ctx, st, a, ws) : launch_rows<D, BITS, 8, false>(ctx, st, a, ws);
     return bf16 ? launch_tiles<D, BITS, true>(ctx, st, a, ws) : launch_tiles<D, BITS, false>(ctx, st, a, ws);
 }
 
