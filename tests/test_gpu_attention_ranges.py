@@ -47,3 +47,39 @@ def test_attention_in_place(tf_ctx, workspaces, many, dim, bits, rows, contexts)
     _close(beside, want, tol)
     if not (many and dim == 512):                               # those have units of eight rows in place
         assert torch.equal(over, beside)
+
+
+# ---- values ----
+
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits,dtype", KINDS)
+@pytest.mark.parametrize("rows,contexts", SHAPES)
+@pytest.mark.parametrize("zeros", [64, 128, 300, 10 ** 6])
+def test_tokens_whose_value_planes_are_zero(tf_ctx, workspaces, many, dim, bits, dtype, rows, contexts, zeros):
+    """The first tokens of every sequence, or all of them, have value planes of zeros, as an empty cache has them."""
+    case = Case(70 + dim + zeros, rows, contexts, 2, dim, bits, 32, DEV)
+    for b, (n, c) in enumerate(zip(rows, contexts)):
+        t = torch.arange(min(zeros, n + c))
+        for i in (4, 5):
+            case.planes[i][case.table[b, t // 32].long(), :, t % 32] = 0.0
+    _by(case, 16, many).upload()
+    q = _q(case, 16, dtype)
+    got = _run(tf_ctx, workspaces, case, q, dtype)
+    _close(got, *ref.attention(case, q, _all_visible(case), dim ** -0.5, half_step(dtype)))
+
+
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("rows,contexts", SHAPES)
+@pytest.mark.parametrize("value_scale", [1e-37, 1e-35, 1e-20, 1e-6, 1e4, 1e30])
+def test_values_of_any_size(tf_ctx, workspaces, many, dim, bits, rows, contexts, value_scale):
+    case = _by(Case(80 + dim, rows, contexts, 2, dim, bits, 16, DEV, value_scale=value_scale), 16, many).upload()
+    q = _q(case, 16, BF16)
+    got = _run(tf_ctx, workspaces, case, q, BF16)
+    # The statement for values of size one, times the power of two that they are apart (planes times a power are exact, the sums linear in them; the
+    # tolerance's absolute share of 1e-7 goes by the values' size then, and 64 bits do not lose small ones beside it), and half of bf16's least step.
+    power = round(-np.log2(value_scale))
+    for i in (4, 5):
+        case.planes[i] = torch.ldexp(case.planes[i].float(), torch.tensor(power)).bfloat16()
+    want, tol = ref.attention(case, q, _all_visible(case), dim ** -0.5, half_step(BF16))
+    _close(got, want * 2.0 ** -power, tol * 2.0 ** -power + 2.0 ** -134)

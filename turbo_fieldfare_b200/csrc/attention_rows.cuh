@@ -30,6 +30,7 @@
 namespace tf {
 
 constexpr int kRowsTile = 16;                                  // tokens: a tile never straddles two pages
+constexpr int kLeastPower = -118;                              // of E: 2^-E times a probability, 2^8 at most, stays in fp32's range where a value scale is zero
 
 template <int D, int BITS, int RB>
 struct RowsShape {
@@ -495,8 +496,8 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0.0f;
-            e_v[n] = -126;
-            down_v[n] = rows_power(126);
+            e_v[n] = kLeastPower;
+            down_v[n] = rows_power(-kLeastPower);
 #pragma unroll
             for (int grp = 0; grp < G; ++grp)
 #pragma unroll

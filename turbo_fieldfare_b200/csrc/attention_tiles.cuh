@@ -631,8 +631,9 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 low = (uint32_t)max((int64_t)0, lesser(pos - (int64_t)a.window + 1, (int64_t)kMostTokens));
             }
             const uint32_t low_most = __reduce_max_sync(kFullMask, low), open_end = lesser(now.seq.context, now.range.end);
-            float m = -INFINITY, l = 0.0f;                     // of the row; l of this thread's tokens; l and O in units of 2^(m + E)
-            int e_o = -126;
+            float m = -INFINITY, l = 0.0f;                     // of the row; l of this thread's tokens, in units of 2^m; O is in units of 2^(m + E)
+            int e_o = -126;                                    // E
+            bool far = false;                                  // a row's E is beyond the usual tile's reach
             uint32_t poison = 0;                               // groups that are not a number
             const uint32_t begin_i = i, stop_i = i + segment;
             uint32_t token0 = now.token0() + side * HALF;
@@ -646,7 +647,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 const float v_most = meta.v_most[i & 7];
                 const bool odd = flags.y & 2u, open = !odd && token0 >= low_most && token0 + HALF <= open_end;
                 // The usual tile: all rows see all tokens, whose powers of two are 1. What other tiles take is kept out of its way.
-                const bool usual = open && (flags.x | flags.y) == 0 && a.scale > 0.0f;
+                const bool usual = open && (flags.x | flags.y) == 0 && a.scale > 0.0f && !far;
                 const float by = usual ? q_up * (a.scale * 1.4426950408889634f) : q_up;
                 // the tokens from `t0` on that the row sees, a chunk of them
                 auto see = [&](int c0) -> uint32_t {
@@ -704,9 +705,10 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 const float own = top * by;
                 swap(own, other);
                 top = fmaxf(own, other);
-                float alpha = 1.0f;
+                float alpha = 1.0f;                            // what O is multiplied with
                 if (top > m + 8.0f) {
                     alpha = rows_exp2(m - top);                // m = -inf: zero
+                    l *= alpha;
                     m = top;
                 }
                 const float base_m = m == -INFINITY ? 0.0f : m;
@@ -726,9 +728,12 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                         alpha *= rows_power(e_o - e_new);
                         e_o = e_new;
                     }
+                    far = __any_sync(kFullMask, e_o > 24);
                 }
                 // ---- probabilities, two to a column ----
-                const float shift = base_m + (float)e_o;
+                // The usual tile's come as 2^(x - m - E): all p' below 2^14, E is at most 24, so neither they nor their sum leave fp32's range. Elsewhere E may be
+                // anything (values of 2^-126, or zeros, which have no say in it) and is taken apart from them.
+                const float shift = usual ? base_m + (float)e_o : base_m;
                 float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
                 for (int c0 = 0; c0 < HALF; c0 += CHUNK) {
@@ -753,17 +758,18 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                         sums[j % 4] += x[j];
                     }
                     if (!usual) {
+                        const float down = rows_power(-e_o);
 #pragma unroll
                         for (int j = 0; j < CHUNK; j += 4) {
                             const float4 up = *reinterpret_cast<const float4*>(&meta.v_up[i & 7][side * HALF + c0 + j]);
-                            x[j] *= up.x; x[j + 1] *= up.y; x[j + 2] *= up.z; x[j + 3] *= up.w;
+                            x[j] = x[j] * up.x * down; x[j + 1] = x[j + 1] * up.y * down; x[j + 2] = x[j + 2] * up.z * down; x[j + 3] = x[j + 3] * up.w * down;
                         }
                     }
 #pragma unroll
                     for (int j = 0; j < CHUNK; j += 2) p[j / 2] = rows_half2(x[j], x[j + 1]);
                     tiles_st(lanes + S::COL_P + st * (TILE / 2) + (side * HALF + c0) / 2, p);
                 }
-                l = fmaf(l, alpha, (sums[0] + sums[1]) + (sums[2] + sums[3]));
+                l = fmaf((sums[0] + sums[1]) + (sums[2] + sums[3]), usual ? rows_power(e_o) : 1.0f, l);
                 // ---- O, when m or E moved: half of its columns ----
                 if (i > begin_i && __any_sync(kFullMask, alpha != 1.0f)) {
                     ok = wait(o_done(i - 1), two(i - 1)) && ok;
@@ -791,14 +797,15 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             poison |= __float_as_uint(other);
             ok = wait(o_done(i - 1), two(i - 1)) && ok;
             tiles_fence_after();
-            float* part = a.partial + (size_t)(2 * blockIdx.x + (from_start ? 1 : 0)) * MT * (S::DV + 2);
+            float* part = a.partial + (size_t)(2 * blockIdx.x + (from_start ? 1 : 0)) * MT * (S::DV + 3);
             if (!whole && is && side == 0) {
-                part[r] = m + (float)e_o;
+                part[r] = m;
                 part[MT + r] = l;
+                part[2 * MT + r] = (float)e_o;
             }
-            const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f, up = whole ? rows_power(e_o) : 1.0f;
             uint16_t* dst = a.out + (size_t)(now.seq.row0 + node) * a.out_stride + (size_t)(head * a.group + flat % a.group) * D + now.head % S::PARTS * S::DV;
-            float* pdst = part + 2 * MT + (size_t)r * S::DV;
+            float* pdst = part + 3 * MT + (size_t)r * S::DV;
 #pragma unroll 1
             for (int c = side * (S::DV / 2); c < (int)(side + 1) * (S::DV / 2); c += 32) {
                 uint32_t o[32];
@@ -810,7 +817,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                     for (int e = 0; e < 32; e += 8) {
                         float v[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[BITS == 8 ? j : (j / 2) + (j % 2) * 4] = __uint_as_float(o[e + j]) * by;
+                        for (int j = 0; j < 8; ++j) v[BITS == 8 ? j : (j / 2) + (j % 2) * 4] = __uint_as_float(o[e + j]) * by * up;
                         if (whole) {
                             *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(rows_pair<BF16>(v[0], v[1]), rows_pair<BF16>(v[2], v[3]), rows_pair<BF16>(v[4], v[5]),
                                                                                 rows_pair<BF16>(v[6], v[7]));
@@ -855,13 +862,21 @@ attention_tiles_join_kernel(const AttnArgs a) {
     const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, r = blockIdx.y * (kTilesJoinThreads / kWarp) + warp;
     if (!info.active || r >= info.valid) return;
     const uint32_t parts = info.last - c + 1;
-    constexpr size_t kSlot = (size_t)MT * (DV + 2);
+    // A slot: [rows] maxima, sums in units of 2^m, exponents E, then [rows][DV] products in units of 2^(m + E).
+    constexpr size_t kSlot = (size_t)MT * (DV + 3);
     auto slot = [&](uint32_t p) { return a.partial + (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * kSlot; };
-    float top = -INFINITY;
-    for (uint32_t p = lane; p < parts; p += kWarp) top = fmaxf(top, slot(p)[r]);
+    float top = -INFINITY, high = -INFINITY;                   // the largest m and m + E
+    for (uint32_t p = lane; p < parts; p += kWarp) {
+        const float* s = slot(p);
+        top = fmaxf(top, s[r]);
+        high = fmaxf(high, s[r] + s[2 * MT + r]);
+    }
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
-    const float base = top == -INFINITY ? 0.0f : top;
+    for (int off = 16; off >= 1; off >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+        high = fmaxf(high, __shfl_xor_sync(kFullMask, high, off));
+    }
+    if (top == -INFINITY) top = high = 0.0f;
     float sum = 0.0f, v[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
@@ -869,15 +884,15 @@ attention_tiles_join_kernel(const AttnArgs a) {
         float w = 0.0f, l = 0.0f;
         if (p0 + lane < parts) {
             const float* s = slot(p0 + lane);
-            w = rows_exp2(s[r] - base);
-            l = s[MT + r];
+            w = rows_exp2(s[r] + s[2 * MT + r] - high);
+            l = s[MT + r] * rows_exp2(s[r] - top);
         }
         const uint32_t n = min(parts - p0, (uint32_t)kWarp);
 #pragma unroll 4
         for (uint32_t j = 0; j < n; ++j) {
-            const float wj = __shfl_sync(kFullMask, w, j), lj = __shfl_sync(kFullMask, l, j);
-            const float* src = slot(p0 + j) + 2 * MT + (size_t)r * DV + lane * VEC;
-            sum = fmaf(wj, lj, sum);
+            const float wj = __shfl_sync(kFullMask, w, j);
+            const float* src = slot(p0 + j) + 3 * MT + (size_t)r * DV + lane * VEC;
+            sum += __shfl_sync(kFullMask, l, j);
 #pragma unroll
             for (int e = 0; e < VEC; e += 2) {
                 const float2 x = *reinterpret_cast<const float2*>(src + e);
@@ -886,11 +901,11 @@ attention_tiles_join_kernel(const AttnArgs a) {
             }
         }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, up = rows_exp2(high - top);
     const uint32_t flat = info.flat0 + r;
     uint16_t* dst = a.out + (size_t)(info.row0 + flat / a.group) * a.out_stride + (size_t)(info.head / PARTS * a.group + flat % a.group) * D + info.head % PARTS * DV + lane * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv, v[e + 1] * inv);
+    for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv * up, v[e + 1] * inv * up);
 }
 
 template <int D, int BITS, bool BF16>
