@@ -83,3 +83,33 @@ def test_values_of_any_size(tf_ctx, workspaces, many, dim, bits, rows, contexts,
         case.planes[i] = torch.ldexp(case.planes[i].float(), torch.tensor(power)).bfloat16()
     want, tol = ref.attention(case, q, _all_visible(case), dim ** -0.5, half_step(BF16))
     _close(got, want * 2.0 ** -power, tol * 2.0 ** -power + 2.0 ** -134)
+
+
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("power", [30, 60])
+@pytest.mark.parametrize("steps", [1, 9])
+@pytest.mark.parametrize("rows,contexts", SHAPES)
+def test_large_values_without_weight_take_no_precision(tf_ctx, workspaces, many, dim, bits, power, steps, rows, contexts):
+    """The first tokens have values 2^30 or 2^60 times the others' and logits 200 lower, in one step or in several on the way to the others':
+    their part of the output is below 2^-200, and the others keep their precision."""
+    case = Case(90 + dim, rows, contexts, 2, dim, bits, 32, DEV)
+    heavy = min(contexts) // 2 // steps * steps
+    for b, c in enumerate(contexts):
+        t = torch.arange(heavy)
+        where = case.table[b, t // 32].long(), slice(None), t % 32
+        # q is 4 on average: a key of -x moves the logit by 4 x sqrt(dim); the last of the heavy tokens still lie 200 below the others
+        lower = (200 + 30.0 * (steps - 1 - t // (heavy // steps))) / (4 * dim ** 0.5)
+        k = -lower[:, None, None] + 0.02 * torch.randn(heavy, 2, dim, generator=case.gen)
+        for plane, new in zip(case.planes[:3], ref.quantised(k, bits)):
+            plane[where] = new
+        for i in (4, 5):
+            case.planes[i][where] *= 2.0 ** power
+    _by(case, 16, many).upload()
+    q = (torch.randn(case.offsets[-1], 16 * dim, generator=case.gen) * 0.3 + 4).to(BF16)
+    got = _run(tf_ctx, workspaces, case, q, BF16)
+    for b in range(len(rows)):
+        t = torch.arange(heavy)
+        for i in (4, 5):
+            case.planes[i][case.table[b, t // 32].long(), :, t % 32] = 0.0
+    _close(got, *ref.attention(case, q, _all_visible(case), dim ** -0.5, half_step(BF16)))

@@ -18,9 +18,9 @@
 // K_i and V_i carry code * scale + bias rounded once to fp16, 2^-12 of the value, and P its probabilities likewise: each adds an error of the size
 // of the output's own rounding to fp16 (together 4e-4 to 5e-4 of the output's norm against 64 bits, 2e-4 of which fp16 outputs have anyhow; nothing next to
 // bf16's 1.7e-3). Exact products of codes, as the kernel for few rows has them, would need an accumulator per group. A token's values are divided by a power of two of its own first; K's comes back with the
-// logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far: tokens that a row
-// does not see have no say, and no cache leaves fp16's range. m is raised only when a logit exceeds it by 8, and what O holds is
-// rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
+// logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far, up and, as m is raised, down:
+// tokens that a row does not see, or that have lost their weight, have no say, and no cache leaves fp16's range. m is raised, to a whole number,
+// only when a logit exceeds it by 8, and what O holds is rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
 // are two units with half of the values each.
 #pragma once
 
@@ -705,11 +705,16 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 const float own = top * by;
                 swap(own, other);
                 top = fmaxf(own, other);
-                float alpha = 1.0f;                            // what O is multiplied with
-                if (top > m + 8.0f) {
-                    alpha = rows_exp2(m - top);                // m = -inf: zero
-                    l *= alpha;
-                    m = top;
+                // m is a whole number, so that what was summed follows it by powers of two. E, the power of what had weight so far, falls by as much as that weight.
+                int power = 0;                                 // O is multiplied with 2^power, at most 1
+                const bool raised = top > m + 8.0f;
+                if (raised) {
+                    const float up = ceilf(top), fall = fmaxf(m - up, -1000.0f);       // m = -inf: nothing was summed
+                    const int e_new = max(e_o + (int)fall, -126);
+                    l *= rows_exp2(fall);
+                    power = (int)fall + e_o - e_new;
+                    e_o = e_new;
+                    m = up;
                 }
                 const float base_m = m == -INFINITY ? 0.0f : m;
                 // ---- E: a value's power of two times 2^8, the largest probability, must not leave fp16 ----
@@ -723,9 +728,9 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                     }
                     swap(heavy, other);
                     heavy = fmaxf(heavy, other);
-                    if (heavy * rows_power(-e_o) > 16384.0f || e_o == -126) {
+                    if (heavy * rows_power(-e_o) > 16384.0f || raised || e_o == -126) {
                         const int e_new = min(max(e_o, rows_exponent(heavy) - 3), 119);      // the row's largest p' below 16
-                        alpha *= rows_power(e_o - e_new);
+                        power += e_o - e_new;
                         e_o = e_new;
                     }
                     far = __any_sync(kFullMask, e_o > 24);
@@ -771,7 +776,8 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 }
                 l = fmaf((sums[0] + sums[1]) + (sums[2] + sums[3]), usual ? rows_power(e_o) : 1.0f, l);
                 // ---- O, when m or E moved: half of its columns ----
-                if (i > begin_i && __any_sync(kFullMask, alpha != 1.0f)) {
+                if (i > begin_i && __any_sync(kFullMask, power != 0)) {
+                    const float alpha = rows_power(power);
                     ok = wait(o_done(i - 1), two(i - 1)) && ok;
                     tiles_fence_after();
 #pragma unroll 1
