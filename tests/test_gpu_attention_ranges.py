@@ -113,3 +113,39 @@ def test_large_values_without_weight_take_no_precision(tf_ctx, workspaces, many,
         for i in (4, 5):
             case.planes[i][case.table[b, t // 32].long(), :, t % 32] = 0.0
     _close(got, *ref.attention(case, q, _all_visible(case), dim ** -0.5, half_step(BF16)))
+
+
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (64, 4), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("which", ["keys", "values"])
+def test_narrow_groups_around_a_small_offset(tf_ctx, workspaces, many, dim, bits, which):
+    """Biases just above 2^-9 and scales far below fp16's normal numbers, halfway between two of its subnormal ones."""
+    rows, contexts = [40, 24], [300, 700]
+    case = Case(100 + dim, rows, contexts, 2, dim, bits, 32, DEV)
+    first, top = 3 * (which == "values"), 2 ** bits - 1
+    owned = ~torch.isnan(case.planes[1])
+    unit = 2.0 ** -24 if bits == 8 else 2.0 ** -20
+    steps = torch.randint(0, 2 if which == "keys" else 1, case.planes[1].shape, generator=case.gen) + 1.5      # keys: a common shift would move no output
+    case.planes[first + 1] = torch.where(owned, (steps * unit).bfloat16(), case.planes[first + 1])
+    case.planes[first + 2][owned] = 2.0 ** -9 * 1.0078125
+    codes = torch.randint(top - top // 8, top + 1, (*case.planes[0].shape[:3], dim), generator=case.gen).to(torch.uint8)
+    case.planes[first] = codes if bits == 8 else codes[..., 0::2] | codes[..., 1::2] << 4
+    _by(case, 16, many).upload()
+    # as keys: a query of large elements of one sign, so that the logits' part from the scales counts
+    q = _q(case, 16, F16, scale=300.0) + 2000 if which == "keys" else _q(case, 16, F16)
+    got = _run(tf_ctx, workspaces, case, q, F16)
+    see = _all_visible(case)
+    want, tol = ref.attention(case, q, see, dim ** -0.5, half_step(F16))
+    if which == "keys" and many:
+        # There a key is rounded to fp16 once, by 2^-11 of it at most, and here the elements of a token, whose codes are nearly alike, with one sign: logits move by
+        # up to d = 2^-11 sum |q k| scale, probabilities by p (d_j - mean of d) <= 2 d p, outputs by 2 d sum p |v|. (The bound for signs of their own is in `tol`.)
+        moved = []
+        for b, n in enumerate(rows):
+            k, v = (c * s + o for c, s, o in (case.stored(b, 0), case.stored(b, 3)))
+            qb = q[case.offsets[b]:case.offsets[b + 1]].to(F64).reshape(n, case.kv, -1, dim)
+            x = torch.einsum("nhgd,jhd->hgnj", qb, k) * dim ** -0.5
+            size = (torch.einsum("nhgd,jhd->hgnj", qb.abs(), k.abs()) * dim ** -0.5).masked_fill(~see[b], 0.0).amax(-1).permute(2, 0, 1)[..., None]
+            p = x.masked_fill(~see[b], -float("inf")).softmax(-1)
+            moved.append((2 * 2.0 ** -11 * size * torch.einsum("hgnj,jhd->nhgd", p, v.abs())).reshape(n, -1))
+        tol = tol + torch.cat(moved)
+    _close(got, want, tol)

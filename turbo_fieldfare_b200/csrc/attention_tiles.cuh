@@ -15,7 +15,7 @@
 // and stand once (one for K and V), a wait that is over takes one look, the MMAs are issued without a branch, and the usual tile, which every row sees
 // and whose powers of two are 1, leaves out the rest: in this order 139 -> 131 -> 114 -> 101 us. The warps that unpack were 8 that also
 // loaded and measured: 127 us with all of the above left out.
-// K_i and V_i carry code * scale + bias rounded once to fp16, 2^-12 of the value, and P its probabilities likewise: each adds an error of the size
+// K_i and V_i carry code * scale + bias rounded once to fp16, at most 2^-11 of the value, and P its probabilities likewise: each adds an error of the size
 // of the output's own rounding to fp16 (together 4e-4 to 5e-4 of the output's norm against 64 bits, 2e-4 of which fp16 outputs have anyhow; nothing next to
 // bf16's 1.7e-3). Exact products of codes, as the kernel for few rows has them, would need an accumulator per group. A token's values are divided by a power of two of its own first; K's comes back with the
 // logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far, up and, as m is raised, down:
@@ -308,8 +308,11 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         }
     } else if (warp >= S::MEASURE && warp < S::LOADER) {
         // ===================== what the planes say: one warp for K's, one for V's, a token per lane =====================
-        // Scale and bias of a token's groups as fp16 (exact, a bf16 has fewer bits), by a power of two of the token's. Values of ordinary sizes are fp16 numbers as they are, exact to
-        // 2^-11 of the token's largest.
+        // Scale and bias of a token's groups as fp16, by a power of two of the token's: 1 where all its groups are of ordinary sizes, else one that brings the largest to
+        // [128, 256). fp16 holds a bf16 of its normal range exactly, and one below it to 2^-25, which 255 codes (15 of 16 times the step) make 2^-17 of
+        // a value: a group whose scale is that small (kExact) is ordinary only if its bias is 2^-4 or more. So no rounding of the planes is above 2^-13 of the group's size or
+        // 2^-24 of the token's largest.
+        constexpr float kExact = BITS == 8 ? 7.62939453125e-6f : 1.220703125e-4f;              // 2^-17; 2^-13, since 4-bit codes take a sixteenth of the scale too
         const bool of_v = warp != S::MEASURE;
         const uint32_t run_log2 = lesser(a.table.page_log2, (uint32_t)(31 - __builtin_clz(TILE)));
         auto measure = [&](auto groups, uint32_t n, const uint4& t) {
@@ -332,7 +335,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 for (int g = 0; g < N; ++g) {
                     const float size = fmaxf(kCentre * fabsf(sc[g]), fabsf(bi[g]));        // a third of the largest value or more
                     const bool finite = sc[g] - sc[g] == 0.0f && bi[g] - bi[g] == 0.0f;
-                    plain = plain && finite && size >= 0.001953125f && size <= 16384.0f;
+                    plain = plain && finite && size >= (fabsf(sc[g]) >= kExact ? 0.001953125f : 0.0625f) && size <= 16384.0f;
                     most = finite ? fmaxf(most, size) : most;
                     if (of_v && !finite) {
                         bits |= 1u << g;
