@@ -149,3 +149,16 @@ def test_narrow_groups_around_a_small_offset(tf_ctx, workspaces, many, dim, bits
             moved.append((2 * 2.0 ** -11 * size * torch.einsum("hgnj,jhd->nhgd", p, v.abs())).reshape(n, -1))
         tol = tol + torch.cat(moved)
     _close(got, want, tol)
+
+
+# ---- queries ----
+
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (128, 8), (256, 8), (512, 4)])
+@pytest.mark.parametrize("q_scale", [1e-36, 1e-20, 3e-5, 1e20, 1e36])
+def test_queries_of_any_size(tf_ctx, workspaces, many, dim, bits, q_scale):
+    rows, contexts = [40, 24], [300, 700]
+    case = _by(Case(110 + dim, rows, contexts, 2, dim, bits, 16, DEV), 16, many).upload()
+    q = _q(case, 16, BF16, scale=q_scale)
+    got = _run(tf_ctx, workspaces, case, q, BF16, scale=0.1 / q_scale)
+    _close(got, *ref.attention(case, q, _all_visible(case), 0.1 / q_scale, half_step(BF16)))

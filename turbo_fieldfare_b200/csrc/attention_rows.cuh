@@ -478,7 +478,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 q_sum[n][grp][1] = sum[1] * 5.9604644775390625e-8f;
                 b_sum[n][grp] = 0.0f;
             }
-            factor[n] = 16777216.0f * rows_power(e) * a.scale * 1.4426950408889634f;
+            factor[n] = a.scale * 1.4426950408889634f * rows_power(e) * 16777216.0f;      // in this order rows of 2^127 have one too, where the scale is as small
             m[n] = -INFINITY;
             l[n] = 0.0f;
             low[n] = 0;
