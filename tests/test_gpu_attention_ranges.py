@@ -162,3 +162,32 @@ def test_queries_of_any_size(tf_ctx, workspaces, many, dim, bits, q_scale):
     q = _q(case, 16, BF16, scale=q_scale)
     got = _run(tf_ctx, workspaces, case, q, BF16, scale=0.1 / q_scale)
     _close(got, *ref.attention(case, q, _all_visible(case), 0.1 / q_scale, half_step(BF16)))
+
+
+# ---- heads of 512, unlike sequences ----
+
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits,dtype", [(512, 8, F16), (512, 4, BF16), (64, 8, BF16)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_trees_of_many_rows(tf_ctx, workspaces, many, dim, bits, dtype, window):
+    rows, contexts = [61, 1, 64, 130], [100, 0, 333, 40]
+    case = _by(Case(120, rows, contexts, 2, dim, bits, 64, DEV), 16, many).upload()
+    rng = np.random.default_rng(8)
+    trees = [_tree(n, rng) for n in rows]
+    masks, depths = [s for seen, _ in trees for s in seen], [depth for _, depth in trees]
+    positions = [c + d for c, depth in zip(contexts, depths) for d in depth]
+    q = _q(case, 16, dtype)
+    got = _run(tf_ctx, workspaces, case, q, dtype, window=window, masks=masks, positions=positions, words=3)
+    see = [ref.visible(n, c, window, seen, [c + d for d in depth]) for n, c, (seen, depth) in zip(rows, contexts, trees)]
+    _close(got, *ref.attention(case, q, see, dim ** -0.5, half_step(dtype)))
+
+
+@pytest.mark.parametrize("singles,chunk", [(64, 300), (20, 300), (3, 1000)])
+@pytest.mark.parametrize("dim,bits", [(128, 8), (512, 4)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_single_tokens_beside_a_prompt_chunk(tf_ctx, workspaces, singles, chunk, dim, bits, window):
+    rows, contexts = [1] * singles + [chunk] + [1], [17 * i for i in range(singles)] + [500, 900]
+    case = Case(130, rows, contexts, 2, dim, bits, 32, DEV).upload()
+    q = _q(case, 4, F16)
+    got = _run(tf_ctx, workspaces, case, q, F16, window=window)
+    _close(got, *ref.attention(case, q, _all_visible(case, window), dim ** -0.5, half_step(F16)))
