@@ -854,7 +854,7 @@ typedef struct tf_kv_batch {
  * (fp32 table on the device; the angle is reduced in 64 bits, so far positions keep their precision); the rest stays.
  * rotated_pairs: a multiple of head_dim / 32, at most head_dim / 2; 0: no rotation, frequencies and positions may be NULL.
  * Quantising is that of the weights (Quantization.swift:63-101,135-176): scale = bf16((max - min) / (2^bits - 1)), bias =
- * bf16(min), scale 1 where max == min; a group that holds an infinity or a NaN gets NaN planes and reads back as NaN.
+ * bf16(min), scale 1 where max == min and nowhere below 2^-126; a group that holds an infinity or a NaN gets NaN planes and reads back as NaN.
  * q, k, v are act_dtype rows [rows][heads * head_dim] with strides in elements (one packed row may hold all three); k and
  * v may be the same rows. An output may be its own input (with its stride), but where v is k neither k_out nor v_out; other overlaps
  * are not looked for. Pointers must be

@@ -191,3 +191,33 @@ def test_single_tokens_beside_a_prompt_chunk(tf_ctx, workspaces, singles, chunk,
     q = _q(case, 4, F16)
     got = _run(tf_ctx, workspaces, case, q, F16, window=window)
     _close(got, *ref.attention(case, q, _all_visible(case, window), dim ** -0.5, half_step(F16)))
+
+
+# ---- cache write ----
+
+@pytest.mark.parametrize("rows", [3, 900])                       # a warp per head; a warp per eight heads
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("size", [1e-38, 3e-37, 1e-36, 1e-30, 1e30, 3e37])
+def test_epilogue_of_values_of_any_size(tf_ctx, rows, dim, bits, size):
+    """v without a norm: scales down to the least one, 2^-126. Codes are those of the stored planes but next to a tie."""
+    case = Case(140 + dim, [rows], [5], 2, dim, bits, 16, DEV).upload()
+    x = torch.randn(rows, 4 * dim, generator=case.gen)
+    x[:, 2 * dim:] *= size
+    x[0, 2 * dim:2 * dim + 64] = size                            # equal values: scale 1
+    x = x.to(BF16)
+    dev, v_out = x.to(DEV), torch.zeros(rows, 2 * dim, dtype=BF16, device=DEV)
+    _ops(tf_ctx)[0].encode(dev[:, :dim], dev[:, :2 * dim], dev[:, 2 * dim:], torch.zeros(rows, dim, dtype=BF16, device=DEV), case.batch(), case.cache, head_dim=dim, v_out=v_out)
+    assert tf_ctx.device_status() == 0
+    assert torch.equal(v_out.cpu(), x[:, 2 * dim:])
+    token = 5 + torch.arange(rows)
+    code, s, o = (p.cpu()[case.table[0, token // 16].long(), :, token % 16] for p in case.cache.planes[3:])
+    top, g = 2 ** bits - 1, x[:, 2 * dim:].to(F64).reshape(rows, 2, -1, 64)
+    low, high = g.amin(-1), g.amax(-1)
+    step = torch.where(high == low, torch.ones_like(low), (high - low) / top)
+    s, o = s.to(F64), o.to(F64)
+    # half a step of bf16 from the quotient that fp32 has, which is off by 2^-23 at the most
+    assert ((s - step.clamp(min=2.0 ** -126)).abs() <= (2.0 ** -8 + 2.0 ** -22) * step).all() and torch.equal(o, low)
+    exact = ((g - o[..., None]) / s[..., None] + 0.5).clamp(0.25, top + 0.75)
+    c = ref.unpack(code, bits).unflatten(-1, (-1, 64))
+    near = (exact - exact.round()).abs() <= 1e-4
+    assert ((c == exact.floor()) | (near & ((c - exact.floor()).abs() <= 1))).all()

@@ -103,12 +103,13 @@ __device__ __forceinline__ void quantise_head(const float (&f)[D / 32], const Kv
     }
     const float top = bits == 8 ? 255.0f : 15.0f, part = bits == 8 ? 1.0f / 255.0f : 1.0f / 15.0f, range = high - low;
     const float about = range * part, step = fmaf(fmaf(-about, top, range), part, about);      // range / top, rounded once more
-    uint16_t s16 = __bfloat16_as_ushort(__float2bfloat16_rn(high == low ? 1.0f : step));
+    // at least 2^-126, bf16's and fp32's least normal number, whose quotient is finite
+    uint16_t s16 = (uint16_t)max(0x0080u, (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(high == low ? 1.0f : step)));
     uint16_t o16 = __bfloat16_as_ushort(__float2bfloat16_rn(low));
     const bool finite = low >= -3.402823466e38f && high <= 3.402823466e38f && (s16 & 0x7F80) != 0x7F80 && (o16 & 0x7F80) != 0x7F80;
     if (!finite) s16 = o16 = kBf16NaN;
     const float scale = bf16_bits_to_float(s16), bias = bf16_bits_to_float(o16);
-    const float inv = scale == 0.0f ? 0.0f : __frcp_rn(scale);
+    const float inv = __frcp_rn(scale);
     uint32_t code[VEC];                                       // in the low byte, under the bits of 2^23: added toward zero it leaves the whole part
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
