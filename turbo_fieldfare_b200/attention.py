@@ -236,6 +236,8 @@ class TreeAttention:
         if tree_mask is not None:
             _check("tree_mask", tree_mask, batch.device, (torch.int64,), 2)
             words = tree_mask.shape[1]
+            if words == 0:
+                raise ValueError("tree_mask has no words")     # its pointer would be NULL, which is a chain
             if tree_mask.shape[0] < batch.rows:
                 raise ValueError(f"tree_mask has {tree_mask.shape[0]} rows, the batch {batch.rows}")
         if window < 0:
