@@ -35,3 +35,17 @@ def _attend(rows=2, **more):
 def test_a_mask_without_words_is_refused():
     with pytest.raises(ValueError, match="no words"):
         _attend(tree_mask=torch.zeros(2, 0, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("window", [-1, 1 << 31, 1 << 32, (1 << 32) + 5])
+def test_windows_beyond_31_bits_are_refused(window):
+    with pytest.raises(ValueError, match="window"):
+        _attend(window=window)
+
+
+def test_strides_beyond_32_bits_are_refused():
+    from turbo_fieldfare_b200.attention import _row_stride
+    far = torch.empty_strided((2, 64), ((1 << 32) + 64, 1), dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="apart"):
+        _row_stride("x", far, far.device, torch.float16, 2, 64)
+    assert _row_stride("x", far[:1], far.device, torch.float16, 1, 64) == 64       # a lone row has no next one

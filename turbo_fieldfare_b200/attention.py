@@ -22,6 +22,7 @@ from ._capi import KVBatchDesc, KVCacheDesc, TF_BF16, TF_FP16
 from .kernels import TurboContext, _ptr, _raw_current_stream, _stream
 
 _ACT = {torch.float16: TF_FP16, torch.bfloat16: TF_BF16}
+_MOST = (1 << 32) - 1                                          # of a stride
 
 
 def _stream_of(context: TurboContext, stream) -> int:
@@ -50,7 +51,10 @@ def _row_stride(name: str, t, device, dtype, rows: int, cols: int) -> int:
             have, width = t.shape
             stride, step = t.stride()
             if have >= rows and width == cols and step == 1:
-                return stride if have > 1 or stride > cols else cols
+                if have == 1:
+                    return cols                                # a lone row has no next one
+                if stride <= _MOST:
+                    return stride
     except (AttributeError, ValueError):
         pass
     _check(name, t, device, (dtype,), 2, contiguous=False)
@@ -58,7 +62,10 @@ def _row_stride(name: str, t, device, dtype, rows: int, cols: int) -> int:
         raise ValueError(f"{name} must be [>= {rows}, {cols}], got {tuple(t.shape)}")
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the columns of a row must be next to one another")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), cols)
+    stride = t.stride(0) if t.shape[0] > 1 else cols
+    if stride > _MOST:                                         # ctypes would cut it to 32 bits
+        raise ValueError(f"{name}: rows that are {stride} elements apart are further than 2^32 - 1")
+    return stride
 
 
 def _vector(name: str, t, device, dtype) -> int:
@@ -240,8 +247,8 @@ class TreeAttention:
                 raise ValueError("tree_mask has no words")     # its pointer would be NULL, which is a chain
             if tree_mask.shape[0] < batch.rows:
                 raise ValueError(f"tree_mask has {tree_mask.shape[0]} rows, the batch {batch.rows}")
-        if window < 0:
-            raise ValueError("window must not be negative")
+        if not 0 <= window < 1 << 31:                          # ctypes would cut it to 32 bits
+            raise ValueError("window must be from 0 to 2^31 - 1")
         ctx.check(ctx.lib.tf_tree_attention(ctx.handle, _stream_of(ctx, stream), q.data_ptr(), q_stride, out.data_ptr(), out_stride, cache._ref,
                                             batch._ref, _ptr(tree_mask), words, window, scale, cols // cache.head_dim, _ACT[q.dtype],
                                             workspace.handle))
