@@ -221,3 +221,19 @@ def test_epilogue_of_values_of_any_size(tf_ctx, rows, dim, bits, size):
     c = ref.unpack(code, bits).unflatten(-1, (-1, 64))
     near = (exact - exact.round()).abs() <= 1e-4
     assert ((c == exact.floor()) | (near & ((c - exact.floor()).abs() <= 1))).all()
+
+
+# ---- calls ----
+
+def test_batches_without_rows(tf_ctx):
+    from turbo_fieldfare_b200 import attention as at
+    cache = at.KVCache.allocate(3, 16, 2, 64, 8, device=DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    batch = at.KVBatch(torch.zeros(2, **i32), torch.full((1,), 4, **i32), torch.zeros(1, 3, **i32), torch.zeros(0, **i32))
+    q, k = (torch.empty(0, n * 64, dtype=torch.float16, device=DEV) for n in (4, 2))
+    at.FusedQKVEpilogue(tf_ctx).encode(q, k, k, torch.empty_like(q), batch, cache, head_dim=64, frequencies=torch.ones(32, device=DEV))
+    at.FusedQKVEpilogue(tf_ctx).encode(q, k, k, q, batch, head_dim=64, k_out=torch.empty_like(k), v_out=torch.empty_like(k))
+    at.KVCacheRead(tf_ctx).encode(cache, batch, torch.empty_like(k))
+    for mask in (None, torch.zeros(0, 1, dtype=torch.int64, device=DEV)):
+        at.TreeAttention(tf_ctx).encode(q, torch.empty_like(q), cache, batch, at.AttentionWorkspace(tf_ctx, 64), scale=1.0, window=5, tree_mask=mask)
+    assert tf_ctx.device_status() == 0

@@ -51,7 +51,7 @@ tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32
                             float scale, uint32_t q_heads, tf_dtype act_dtype, tf_attention_workspace* ws) {
     const char* name = "tf_tree_attention";
     TF_REQUIRE(ctx, ctx != nullptr, TF_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", name);
-    TF_REQUIRE(ctx, q && out, TF_ERR_INVALID_ARGUMENT, "%s: NULL buffer", name);
+    TF_REQUIRE(ctx, (q && out) || (batch && batch->rows == 0), TF_ERR_INVALID_ARGUMENT, "%s: NULL buffer", name);
     tf_status s = tf::check_kv_cache(ctx, name, cache);
     if (s == TF_OK) s = tf::check_kv_batch(ctx, name, batch);
     if (s != TF_OK) return s;
@@ -68,7 +68,7 @@ tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32
                "%s: rows must be 16-byte aligned and strides multiples of 8 elements", name);
     TF_REQUIRE(ctx, tree_mask == nullptr || mask_words > 0, TF_ERR_INVALID_ARGUMENT, "%s: mask_words is 0", name);
     TF_REQUIRE(ctx, tf::aligned(tree_mask, 8), TF_ERR_ALIGNMENT, "%s: tree_mask must be 8-byte aligned", name);
-    TF_REQUIRE(ctx, tree_mask == nullptr || window == 0 || batch->positions != nullptr, TF_ERR_INVALID_ARGUMENT,
+    TF_REQUIRE(ctx, tree_mask == nullptr || window == 0 || batch->positions != nullptr || batch->rows == 0, TF_ERR_INVALID_ARGUMENT,
                "%s: a tree with a window needs positions", name);
     TF_REQUIRE(ctx, window <= 0x7FFFFFFFu, TF_ERR_INVALID_ARGUMENT, "%s: window must be below 2^31", name);
     TF_REQUIRE(ctx, scale - scale == 0.0f, TF_ERR_INVALID_ARGUMENT, "%s: scale must be finite", name);

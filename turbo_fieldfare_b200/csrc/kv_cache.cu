@@ -486,9 +486,10 @@ tf_status tf_qkv_epilogue(tf_context* ctx, void* stream, const void* q, uint32_t
                           uint32_t kv_heads, uint32_t head_dim, tf_dtype act_dtype) {
     const char* name = "tf_qkv_epilogue";
     TF_REQUIRE(ctx, ctx != nullptr, TF_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", name);
-    TF_REQUIRE(ctx, q && k && v && q_out, TF_ERR_INVALID_ARGUMENT, "%s: NULL buffer", name);
+    const bool empty = batch && batch->rows == 0;
+    TF_REQUIRE(ctx, empty || (q && k && v && q_out), TF_ERR_INVALID_ARGUMENT, "%s: NULL buffer", name);
     TF_REQUIRE(ctx, batch != nullptr, TF_ERR_INVALID_ARGUMENT, "%s: batch is NULL", name);
-    TF_REQUIRE(ctx, cache || (k_out && v_out), TF_ERR_INVALID_ARGUMENT, "%s: without a cache k_out and v_out are needed", name);
+    TF_REQUIRE(ctx, empty || cache || (k_out && v_out), TF_ERR_INVALID_ARGUMENT, "%s: without a cache k_out and v_out are needed", name);
     TF_REQUIRE(ctx, act_dtype == TF_FP16 || act_dtype == TF_BF16, TF_ERR_UNSUPPORTED, "%s: rows are fp16 or bf16", name);
     TF_REQUIRE(ctx, head_dim == 64 || head_dim == 128 || head_dim == 256 || head_dim == 512, TF_ERR_UNSUPPORTED,
                "%s: head_dim %u is not 64, 128, 256 or 512", name, head_dim);
@@ -511,10 +512,10 @@ tf_status tf_qkv_epilogue(tf_context* ctx, void* stream, const void* q, uint32_t
                TF_ERR_ALIGNMENT, "%s: rows and weights must be 16-byte aligned and strides multiples of 8 elements", name);
     TF_REQUIRE(ctx, rotated_pairs <= head_dim / 2 && rotated_pairs % (head_dim / 32) == 0, TF_ERR_UNSUPPORTED,
                "%s: rotated_pairs %u is not a multiple of %u up to %u", name, rotated_pairs, head_dim / 32, head_dim / 2);
-    TF_REQUIRE(ctx, rotated_pairs == 0 || (frequencies && batch->positions), TF_ERR_INVALID_ARGUMENT, "%s: a rotation needs frequencies and positions", name);
+    TF_REQUIRE(ctx, empty || rotated_pairs == 0 || (frequencies && batch->positions), TF_ERR_INVALID_ARGUMENT, "%s: a rotation needs frequencies and positions", name);
     TF_REQUIRE(ctx, tf::aligned(frequencies, 4) && tf::aligned(batch->positions, 4), TF_ERR_ALIGNMENT,
                "%s: frequencies and positions must be 4-byte aligned", name);
-    TF_REQUIRE(ctx, !(k == v && (k_out == k || v_out == k)), TF_ERR_INVALID_ARGUMENT, "%s: k_out or v_out may not overwrite rows that are both k and v", name);
+    TF_REQUIRE(ctx, empty || !(k == v && (k_out == k || v_out == k)), TF_ERR_INVALID_ARGUMENT, "%s: k_out or v_out may not overwrite rows that are both k and v", name);
     TF_REQUIRE(ctx, eps >= 0.0f && eps <= 3.4e38f, TF_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", name);
     if (batch->rows == 0 || (cache && batch->sequences == 0)) return TF_OK;
     TF_REQUIRE(ctx, batch->rows <= 0x7FFFFFFFu, TF_ERR_INVALID_ARGUMENT, "%s: rows must be below 2^31", name);
@@ -556,7 +557,7 @@ tf_status tf_kv_cache_read(tf_context* ctx, void* stream, const tf_kv_cache* cac
     tf_status s = tf::check_kv_cache(ctx, name, cache);
     if (s == TF_OK) s = tf::check_kv_batch(ctx, name, batch);
     if (s != TF_OK) return s;
-    TF_REQUIRE(ctx, k_out || v_out, TF_ERR_INVALID_ARGUMENT, "%s: NULL buffer", name);
+    TF_REQUIRE(ctx, k_out || v_out || batch->rows == 0, TF_ERR_INVALID_ARGUMENT, "%s: NULL buffer", name);
     TF_REQUIRE(ctx, act_dtype == TF_FP16 || act_dtype == TF_BF16, TF_ERR_UNSUPPORTED, "%s: rows are fp16 or bf16", name);
     const uint64_t row = (uint64_t)cache->kv_heads * cache->head_dim;
     TF_REQUIRE(ctx, (!k_out || k_out_stride >= row) && (!v_out || v_out_stride >= row), TF_ERR_INVALID_ARGUMENT,
