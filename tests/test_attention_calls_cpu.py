@@ -86,6 +86,12 @@ int main() {
                                 TF_FP16), TF_OK);
     ANSWERS(tf_tree_attention(&context, nullptr, nullptr, 256, nullptr, 256, &cache, nullptr, nullptr, 0, 0, 1.0f, 4, TF_FP16, &ws), TF_ERR_INVALID_ARGUMENT, "NULL");
     ANSWERS(tf_kv_cache_read(&context, nullptr, &cache, &batch, nullptr, 0, nullptr, 0, TF_FP16), TF_ERR_INVALID_ARGUMENT, "NULL buffer");
+    // outputs over their inputs have the inputs' stride
+    ANSWERS(tf_tree_attention(&context, nullptr, mem, 256, mem, 264, &cache, &batch, nullptr, 0, 0, 1.0f, 4, TF_FP16, &ws), TF_ERR_INVALID_ARGUMENT, "same stride");
+    for (int which = 0; which < 3; ++which)
+        ANSWERS(tf_qkv_epilogue(&context, nullptr, mem, 256, mem + 512, 128, mem + 1024, 128, nullptr, nullptr, 0, nullptr, 0, 0.0f, which == 0 ? mem : mem + 1536, which == 0 ? 264 : 256,
+                                which == 1 ? mem + 512 : nullptr, 136, which == 2 ? mem + 1024 : nullptr, 136, &batch, &cache, 4, 2, 64, TF_FP16),
+                TF_ERR_INVALID_ARGUMENT, "same stride");
     std::printf("all fine\n");
     return 0;
 }

@@ -66,6 +66,7 @@ tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32
     TF_REQUIRE(ctx, q_stride >= row && out_stride >= row, TF_ERR_INVALID_ARGUMENT, "%s: a row stride is smaller than its row", name);
     TF_REQUIRE(ctx, tf::aligned(q, 16) && tf::aligned(out, 16) && (q_stride | out_stride) % 8 == 0, TF_ERR_ALIGNMENT,
                "%s: rows must be 16-byte aligned and strides multiples of 8 elements", name);
+    TF_REQUIRE(ctx, q != out || q_stride == out_stride || batch->rows <= 1, TF_ERR_INVALID_ARGUMENT, "%s: out may be q only with the same stride", name);
     TF_REQUIRE(ctx, tree_mask == nullptr || mask_words > 0, TF_ERR_INVALID_ARGUMENT, "%s: mask_words is 0", name);
     TF_REQUIRE(ctx, tf::aligned(tree_mask, 8), TF_ERR_ALIGNMENT, "%s: tree_mask must be 8-byte aligned", name);
     TF_REQUIRE(ctx, tree_mask == nullptr || window == 0 || batch->positions != nullptr || batch->rows == 0, TF_ERR_INVALID_ARGUMENT,

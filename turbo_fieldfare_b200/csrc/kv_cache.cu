@@ -515,6 +515,8 @@ tf_status tf_qkv_epilogue(tf_context* ctx, void* stream, const void* q, uint32_t
     TF_REQUIRE(ctx, empty || rotated_pairs == 0 || (frequencies && batch->positions), TF_ERR_INVALID_ARGUMENT, "%s: a rotation needs frequencies and positions", name);
     TF_REQUIRE(ctx, tf::aligned(frequencies, 4) && tf::aligned(batch->positions, 4), TF_ERR_ALIGNMENT,
                "%s: frequencies and positions must be 4-byte aligned", name);
+    TF_REQUIRE(ctx, batch->rows <= 1 || ((q_out != q || q_out_stride == q_stride) && (k_out != k || k_out_stride == k_stride) && (v_out != v || v_out_stride == v_stride)),
+               TF_ERR_INVALID_ARGUMENT, "%s: an output may be its input only with the same stride", name);
     TF_REQUIRE(ctx, empty || !(k == v && (k_out == k || v_out == k)), TF_ERR_INVALID_ARGUMENT, "%s: k_out or v_out may not overwrite rows that are both k and v", name);
     TF_REQUIRE(ctx, eps >= 0.0f && eps <= 3.4e38f, TF_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", name);
     if (batch->rows == 0 || (cache && batch->sequences == 0)) return TF_OK;
