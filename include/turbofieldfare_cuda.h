@@ -852,7 +852,8 @@ typedef struct tf_kv_batch {
  * without a cache both are needed). Outputs are rounded once.
  * Rotation: for j < rotated_pairs the elements j and j + rotated_pairs of a head turn by positions[r] * frequencies[j]
  * (fp32 table on the device; the angle is reduced in 64 bits, so far positions keep their precision); the rest stays.
- * rotated_pairs: a multiple of head_dim / 32, at most head_dim / 2; 0: no rotation, frequencies and positions may be NULL.
+ * rotated_pairs: a multiple of head_dim / 32, at most head_dim / 2; 0: no rotation, frequencies and positions may be NULL. A layer that pairs
+ * j with j + head_dim / 2 and turns only the first pairs (rope_proportional_neox) passes head_dim / 2 frequencies, zeros behind those.
  * Quantising is that of the weights (Quantization.swift:63-101,135-176): scale = bf16((max - min) / (2^bits - 1)), bias =
  * bf16(min), scale 1 where max == min and nowhere below 2^-126; a group that holds an infinity or a NaN gets NaN planes and reads back as NaN.
  * q, k, v are act_dtype rows [rows][heads * head_dim] with strides in elements (one packed row may hold all three); k and

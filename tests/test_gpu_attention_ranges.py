@@ -223,6 +223,30 @@ def test_epilogue_of_values_of_any_size(tf_ctx, rows, dim, bits, size):
     assert ((c == exact.floor()) | (near & ((c - exact.floor()).abs() <= 1))).all()
 
 
+@pytest.mark.parametrize("rows", [4, 900])
+@pytest.mark.parametrize("dim,turning", [(64, 8), (256, 32), (512, 64), (128, 1)])
+def test_pairs_half_a_head_apart_of_which_the_first_turn(tf_ctx, rows, dim, turning):
+    """Frequencies of half a head with zeros behind those that turn: element j is paired with j + dim / 2, the rest stays as it is."""
+    gen = torch.Generator().manual_seed(dim)
+    x, position = torch.randn(rows, 3 * dim, generator=gen).to(F16), torch.arange(rows, dtype=torch.int32) * 37
+    freqs = torch.zeros(dim // 2)
+    freqs[:turning] = 1e4 ** (-torch.arange(turning) / turning)
+    from turbo_fieldfare_b200 import attention as at
+    i32 = dict(dtype=torch.int32, device=DEV)
+    batch = at.KVBatch(torch.zeros(1, **i32), torch.zeros(0, **i32), torch.zeros(0, 1, **i32), position.to(DEV))
+    dev, out = x.to(DEV), [torch.zeros(rows, dim, dtype=F16, device=DEV) for _ in range(3)]
+    _ops(tf_ctx)[0].encode(dev[:, :dim], dev[:, dim:2 * dim], dev[:, 2 * dim:], out[0], batch, head_dim=dim, frequencies=freqs.to(DEV), k_out=out[1], v_out=out[2])
+    for i in range(2):
+        y = x[:, dim * i:dim * i + dim].to(F64)
+        y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + 1e-6)
+        size, angle = y.abs(), position.to(F64)[:, None] * freqs[:turning].to(F64)
+        a, b = y[:, :turning].clone(), y[:, dim // 2:dim // 2 + turning].clone()
+        y[:, :turning], y[:, dim // 2:dim // 2 + turning] = a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()
+        size[:, :turning] = size[:, dim // 2:dim // 2 + turning] = a.abs() + b.abs()
+        _close(out[i], y, half_step(F16) * y.abs() + 2.0 ** -19 * size + 1e-7)
+    assert torch.equal(out[2].cpu(), x[:, 2 * dim:])
+
+
 # ---- calls ----
 
 def test_batches_without_rows(tf_ctx):
