@@ -13,8 +13,8 @@
 // fp16, and what the bias adds is summed in fp32. The rounding of p' shall weigh a code's distance from the centre of the codes, not the code
 // itself: sum p' (c - centre) = sum p' c - centre sum p', with sum p' of all groups by one more MMA each into the rows of a common
 // accumulator, against sum p (b + centre s). E is a row's own, after the largest p s so far (tokens that it does not see have p = 0
-// and no say; when m is raised, those before lose theirs), and m a maximum, rounded up, that is raised only when a logit exceeds it by 8: one
-// vote per tile, and what was summed is rescaled only when one of them moves.
+// and no say; when m is raised, those before lose theirs), and m a maximum that is raised only when a logit exceeds it by 8: one vote per
+// tile, and what was summed is rescaled only when one of them moves.
 //
 // What it measured, 8-bit heads of 256 on 8 kv heads, two rows each: 64 sequences of up to 4096 tokens 130 us, 4.9 TB/s; 131000 tokens of one sequence, heads of
 // 128: 75 us, 3.7 TB/s; 4-bit heads of 512, 200 sequences of up to 8192 tokens, eight rows per kv head: 310 us, 3.6 TB/s, bound by unpacking (2200 clocks a
@@ -491,12 +491,12 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
         }
         if (a.window) low_most = (int32_t)__reduce_max_sync(kFullMask, (uint32_t)low_most);
         float o[NR][G][4][4], ones[NR][4];                     // ones: sums of the rounded p', row grp for group grp
-        int e_v[NR];                                           // exponent that the row's products p s are divided by, and 2^-E
+        float e_real[NR];                                      // E, the exponent that the row's products p s are divided by, not rounded up, and 2^-E
         float down_v[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0.0f;
-            e_v[n] = kLeastPower;
+            e_real[n] = kLeastPower;
             down_v[n] = rows_power(-kLeastPower);
 #pragma unroll
             for (int grp = 0; grp < G; ++grp)
@@ -642,16 +642,16 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 moves |= !(most * down_v[n] < 16384.0f);
             }
             if (__any_sync(kFullMask, moves)) {
-                // m is a whole number, so that what was summed follows it by powers of two. E, the power of what had weight so far, falls by as much as that weight.
-                int fall[NR];
+                // E, the power of what had weight so far, falls by as much as that weight when m is raised. It is rounded up from e_real, so that many rises add up.
+                float fall[NR];
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
                     float top = fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
                     top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
-                    const float m_new = fmaxf(m[n], ceilf(top)), by = m_new == -INFINITY ? 0.0f : fmaxf(m[n] - m_new, -1000.0f);       // m = -inf: nothing was summed
-                    const float alpha = rows_exp2(by);
-                    fall[n] = (int)by;
+                    const float m_new = fmaxf(m[n], top);
+                    fall[n] = m_new == -INFINITY ? 0.0f : m[n] - m_new;
+                    const float alpha = rows_exp2(fall[n]);    // m = -inf: nothing was summed
                     m[n] = m_new;
                     l[n] *= alpha;
                     raise_p(n);
@@ -683,17 +683,18 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                             most = fmaxf(most, p[n][key] * fabsf(key < 2 ? vs_lo.at(key, grp) : vs_hi.at(key - 2, grp)));      // a NaN of p leaves it as it is
                     most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
                     most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-                    const int e_low = e_v[n] + fall[n], e_new = min(max(max(e_low, kLeastPower), rows_exponent(most) - 3), 119);      // now below 16
+                    const float e_old = ceilf(e_real[n]);
+                    e_real[n] = fminf(fmaxf(fmaxf(e_real[n] + fall[n], (float)kLeastPower), (float)(rows_exponent(most) - 3)), 119.0f);      // p' below 16 now
+                    const float e_new = ceilf(e_real[n]);
                     // what was summed of rows g + 8 n: their accumulators lie in the columns of other lanes
-                    const float f = rows_power(e_low - e_new);
+                    const float f = rows_exp2(fall[n] + (e_old - e_new));
                     const float f0 = __shfl_sync(kFullMask, f, 8 * t), f1 = __shfl_sync(kFullMask, f, 8 * t + 4);      // rows 2t, 2t + 1
                     ones[n][0] *= f0; ones[n][1] *= f1;
 #pragma unroll
                     for (int grp = 0; grp < G; ++grp)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) { o[n][grp][j][0] *= f0; o[n][grp][j][1] *= f1; o[n][grp][j][2] *= f0; o[n][grp][j][3] *= f1; }
-                    e_v[n] = e_new;
-                    down_v[n] = rows_power(-e_new);
+                    down_v[n] = rows_power(-(int)e_new);
                 }
             }
             float pd[NR][4], pc[NR][4];
@@ -776,7 +777,7 @@ attention_rows_kernel(const __grid_constant__ AttnArgs a) {
                 part[RB + g + 8 * n] = sum;
             }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const float up0 = rows_power(__shfl_sync(kFullMask, e_v[n], 8 * t)), up1 = rows_power(__shfl_sync(kFullMask, e_v[n], 8 * t + 4));
+            const float up0 = rows_power((int)ceilf(__shfl_sync(kFullMask, e_real[n], 8 * t))), up1 = rows_power((int)ceilf(__shfl_sync(kFullMask, e_real[n], 8 * t + 4)));
             const float inv0 = __shfl_sync(kFullMask, inv, 8 * t), inv1 = __shfl_sync(kFullMask, inv, 8 * t + 4);
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {

@@ -19,8 +19,8 @@
 // of the output's own rounding to fp16 (together 4e-4 to 5e-4 of the output's norm against 64 bits, 2e-4 of which fp16 outputs have anyhow; nothing next to
 // bf16's 1.7e-3). Exact products of codes, as the kernel for few rows has them, would need an accumulator per group. A token's values are divided by a power of two of its own first; K's comes back with the
 // logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far, up and, as m is raised, down:
-// tokens that a row does not see, or that have lost their weight, have no say, and no cache leaves fp16's range. m is raised, to a whole number,
-// only when a logit exceeds it by 8, and what O holds is rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
+// tokens that a row does not see, or that have lost their weight, have no say, and no cache leaves fp16's range. m is raised only
+// when a logit exceeds it by 8, and what O holds is rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
 // are two units with half of the values each.
 #pragma once
 
@@ -635,7 +635,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
             }
             const uint32_t low_most = __reduce_max_sync(kFullMask, low), open_end = lesser(now.seq.context, now.range.end);
             float m = -INFINITY, l = 0.0f;                     // of the row; l of this thread's tokens, in units of 2^m; O is in units of 2^(m + E)
-            int e_o = -126;                                    // E
+            int e_o = kLeastPower;                             // E
             bool far = false;                                  // a row's E is beyond the usual tile's reach
             uint32_t poison = 0;                               // groups that are not a number
             const uint32_t begin_i = i, stop_i = i + segment;
@@ -708,16 +708,16 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 const float own = top * by;
                 swap(own, other);
                 top = fmaxf(own, other);
-                // m is a whole number, so that what was summed follows it by powers of two. E, the power of what had weight so far, falls by as much as that weight.
-                int power = 0;                                 // O is multiplied with 2^power, at most 1
+                // E, the power of what had weight so far, falls by as much as that weight when m is raised (whole powers: at least 8 of every 9).
+                float turn_o = 0.0f;                           // O is multiplied with 2^turn_o
                 const bool raised = top > m + 8.0f;
                 if (raised) {
-                    const float up = ceilf(top), fall = fmaxf(m - up, -1000.0f);       // m = -inf: nothing was summed
-                    const int e_new = max(e_o + (int)fall, -126);
+                    const float fall = m - top;                // m = -inf: nothing was summed
+                    const int e_new = max(e_o + (int)ceilf(fmaxf(fall, -1000.0f)), kLeastPower);
                     l *= rows_exp2(fall);
-                    power = (int)fall + e_o - e_new;
+                    turn_o = fall + (float)(e_o - e_new);
                     e_o = e_new;
-                    m = up;
+                    m = top;
                 }
                 const float base_m = m == -INFINITY ? 0.0f : m;
                 // ---- E: a value's power of two times 2^8, the largest probability, must not leave fp16 ----
@@ -731,9 +731,9 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                     }
                     swap(heavy, other);
                     heavy = fmaxf(heavy, other);
-                    if (heavy * rows_power(-e_o) > 16384.0f || raised || e_o == -126) {
-                        const int e_new = min(max(e_o, rows_exponent(heavy) - 3), 119);      // the row's largest p' below 16
-                        power += e_o - e_new;
+                    const int e_new = min(rows_exponent(heavy) - 3, 119);                    // the row's largest p' below 16
+                    if (e_new > e_o && (heavy * rows_power(-e_o) > 16384.0f || raised || e_o == kLeastPower)) {
+                        turn_o += (float)(e_o - e_new);
                         e_o = e_new;
                     }
                     far = __any_sync(kFullMask, e_o > 24);
@@ -779,8 +779,8 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 }
                 l = fmaf((sums[0] + sums[1]) + (sums[2] + sums[3]), usual ? rows_power(e_o) : 1.0f, l);
                 // ---- O, when m or E moved: half of its columns ----
-                if (i > begin_i && __any_sync(kFullMask, power != 0)) {
-                    const float alpha = rows_power(power);
+                if (i > begin_i && __any_sync(kFullMask, turn_o != 0.0f)) {
+                    const float alpha = rows_exp2(turn_o);
                     ok = wait(o_done(i - 1), two(i - 1)) && ok;
                     tiles_fence_after();
 #pragma unroll 1
@@ -812,7 +812,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 part[MT + r] = l;
                 part[2 * MT + r] = (float)e_o;
             }
-            const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f, up = whole ? rows_power(e_o) : 1.0f;
+            const float inv = whole ? (l == 0.0f ? 0.0f : rows_power(e_o) / l) : 1.0f;
             uint16_t* dst = a.out + (size_t)(now.seq.row0 + node) * a.out_stride + (size_t)(head * a.group + flat % a.group) * D + now.head % S::PARTS * S::DV;
             float* pdst = part + 3 * MT + (size_t)r * S::DV;
 #pragma unroll 1
@@ -826,7 +826,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                     for (int e = 0; e < 32; e += 8) {
                         float v[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[BITS == 8 ? j : (j / 2) + (j % 2) * 4] = __uint_as_float(o[e + j]) * by * up;
+                        for (int j = 0; j < 8; ++j) v[BITS == 8 ? j : (j / 2) + (j % 2) * 4] = __uint_as_float(o[e + j]) * by;
                         if (whole) {
                             *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(rows_pair<BF16>(v[0], v[1]), rows_pair<BF16>(v[2], v[3]), rows_pair<BF16>(v[4], v[5]),
                                                                                 rows_pair<BF16>(v[6], v[7]));
@@ -910,11 +910,11 @@ attention_tiles_join_kernel(const AttnArgs a) {
             }
         }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, up = rows_exp2(high - top);
+    const float inv = sum == 0.0f ? 0.0f : rows_exp2(high - top) / sum;
     const uint32_t flat = info.flat0 + r;
     uint16_t* dst = a.out + (size_t)(info.row0 + flat / a.group) * a.out_stride + (size_t)(info.head / PARTS * a.group + flat % a.group) * D + info.head % PARTS * DV + lane * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv * up, v[e + 1] * inv * up);
+    for (int e = 0; e < VEC; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = rows_pair<BF16>(v[e] * inv, v[e + 1] * inv);
 }
 
 template <int D, int BITS, bool BF16>
