@@ -116,6 +116,37 @@ def test_large_values_without_weight_take_no_precision(tf_ctx, workspaces, many,
 
 
 @pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("size,tail", [(0.0021, 0.0014), (0.0002, 0.0003), (0.0085, 0.006), (0.07, 0.045), (0.55, 0.4), (90.0, 150.0), (150.0, 90.0), (17000.0, 12000.0)])
+def test_long_tails_beside_a_token_of_another_size(tf_ctx, workspaces, many, dim, bits, size, tail):
+    """One token has half of the weight, thousands share the other half, and a power of two that the values are divided by lies between their sizes:
+    each of the thousands' parts is far below the one's, their sum is not."""
+    rows, contexts = [40, 40], [4000, 3000]
+    case = Case(150 + dim, rows, contexts, 2, dim, bits, 64, DEV)
+    for b, (n, c) in enumerate(zip(rows, contexts)):
+        t = torch.arange(n + c)
+        where = case.table[b, t // 64].long(), slice(None), t % 64
+        # q is 1 on average: the first key moves the logit by log(c)
+        k = 0.02 * torch.randn(n + c, 2, dim, generator=case.gen)
+        k[0] += np.log(c) / dim ** 0.5
+        # a group's least and largest values, and so its size, are those asked for
+        v = torch.rand(n + c, 2, dim // 64, 64, generator=case.gen) * 1.5 - 0.25
+        v[..., 0], v[..., 1] = -1.0, 1.25
+        v = v.flatten(-2) * tail
+        v[0] *= size / tail
+        for plane, new in zip(case.planes, (*ref.quantised(k, bits), *ref.quantised(v, bits))):
+            plane[where] = new
+    _by(case, 16, many).upload()
+    q = (torch.randn(case.offsets[-1], 16 * dim, generator=case.gen) * 0.1 + 1).to(BF16)
+    got = _run(tf_ctx, workspaces, case, q, BF16)
+    power = round(-np.log2(tail))                                # the tolerance's absolute share goes by the values' size
+    for i in (4, 5):
+        case.planes[i] = torch.ldexp(case.planes[i].float(), torch.tensor(power)).bfloat16()
+    want, tol = ref.attention(case, q, _all_visible(case), dim ** -0.5, half_step(BF16))
+    _close(got, want * 2.0 ** -power, tol * 2.0 ** -power)
+
+
+@pytest.mark.parametrize("many", [True, False])
 @pytest.mark.parametrize("dim,bits", [(64, 8), (64, 4), (128, 4), (256, 8), (512, 4)])
 @pytest.mark.parametrize("which", ["keys", "values"])
 def test_narrow_groups_around_a_small_offset(tf_ctx, workspaces, many, dim, bits, which):

@@ -17,8 +17,8 @@
 // loaded and measured: 127 us with all of the above left out.
 // K_i and V_i carry code * scale + bias rounded once to fp16, at most 2^-11 of the value, and P its probabilities likewise: each adds an error of the size
 // of the output's own rounding to fp16 (together 4e-4 to 5e-4 of the output's norm against 64 bits, 2e-4 of which fp16 outputs have anyhow; nothing next to
-// bf16's 1.7e-3). Exact products of codes, as the kernel for few rows has them, would need an accumulator per group. A token's values are divided by a power of two of its own first; K's comes back with the
-// logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far, up and, as m is raised, down:
+// bf16's 1.7e-3). Exact products of codes, as the kernel for few rows has them, would need an accumulator per group. A token whose planes are
+// out of the ordinary is divided by a power of two of its own first; K's comes back with the logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far, up and, as m is raised, down:
 // tokens that a row does not see, or that have lost their weight, have no say, and no cache leaves fp16's range. m is raised only
 // when a logit exceeds it by 8, and what O holds is rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
 // are two units with half of the values each.
@@ -308,12 +308,14 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
         }
     } else if (warp >= S::MEASURE && warp < S::LOADER) {
         // ===================== what the planes say: one warp for K's, one for V's, a token per lane =====================
-        // Scale and bias of a token's groups as fp16, by a power of two of the token's: 1 where all its groups are of ordinary sizes, else one that brings the largest to
-        // [128, 256). fp16 holds a bf16 of its normal range exactly, and one below it to 2^-25, which 255 codes (15 of 16 times the step) make 2^-17 of
-        // a value: a group whose scale is that small (kExact) is ordinary only if its bias is 2^-4 or more. So no rounding of the planes is above 2^-13 of the group's size or
-        // 2^-24 of the token's largest.
+        // Scale and bias of a token's groups as fp16, by a power of two of the token's, 2^e: e = 0 where all its groups are of ordinary sizes. fp16 holds a bf16 of its normal
+        // range exactly, and one below it to 2^-25, which 255 codes (15 of 16 times the step) make 2^-17 of a value: a group whose scale is that small (kExact) is
+        // ordinary only if its bias is 2^-4 or more. Elsewhere a key's largest group is brought to [2^7, 2^8). A value's 2^e goes into fp16 probabilities, next to those of
+        // tokens with e = 0: were it far below the value's size, long tails of small probabilities would be lost there. So from 2^-1 down it is at least 2^-8, and
+        // from 2^-12 down 2^4 times the size, and ordinary values are within [2^-7, 2^7]. No rounding of the planes is above 2^-13 of the token's largest group.
         constexpr float kExact = BITS == 8 ? 7.62939453125e-6f : 1.220703125e-4f;              // 2^-17; 2^-13, since 4-bit codes take a sixteenth of the scale too
         const bool of_v = warp != S::MEASURE;
+        const float least = of_v ? 0.0078125f : 0.001953125f, largest = of_v ? 128.0f : 16384.0f;      // of an ordinary group
         const uint32_t run_log2 = lesser(a.table.page_log2, (uint32_t)(31 - __builtin_clz(TILE)));
         auto measure = [&](auto groups, uint32_t n, const uint4& t) {
             constexpr int N = decltype(groups)::value;
@@ -335,14 +337,15 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                 for (int g = 0; g < N; ++g) {
                     const float size = fmaxf(kCentre * fabsf(sc[g]), fabsf(bi[g]));        // a third of the largest value or more
                     const bool finite = sc[g] - sc[g] == 0.0f && bi[g] - bi[g] == 0.0f;
-                    plain = plain && finite && size >= (fabsf(sc[g]) >= kExact ? 0.001953125f : 0.0625f) && size <= 16384.0f;
+                    plain = plain && finite && size >= (fabsf(sc[g]) >= kExact ? least : 0.0625f) && size <= largest;
                     most = finite ? fmaxf(most, size) : most;
                     if (of_v && !finite) {
                         bits |= 1u << g;
                         sc[g] = bi[g] = 0.0f;
                     }
                 }
-                const int e = plain || !is ? 0 : min(max(rows_exponent(most) - 7, -126), 119);       // both parts of a value below 2^8
+                const int at = rows_exponent(most), brought = of_v ? min(at + 4, max(at - 7, -8)) : at - 7;
+                const int e = plain || !is ? 0 : min(max(brought, -126), 119);                       // both parts of a value below 2^8
                 const float down = rows_power(-e), up = rows_power(e);
                 any |= e != 0;
 #pragma unroll
