@@ -899,7 +899,11 @@ uint64_t tf_attention_workspace_bytes(const tf_attention_workspace* ws);
  * A row that sees nothing becomes zero. Infinities and NaN in the cache reach only the rows that see them.
  * positions are read only with a tree_mask and a window. q and out: act_dtype rows [rows][q_heads * head_dim], 16-byte
  * aligned, strides multiples of 8; out may be q, with its stride (heads of 512 then go by units of eight rows, which takes many
- * rows over long contexts up to 2.5 times as long). softmax and sums are fp32.
+ * rows over long contexts up to 2.5 times as long). softmax and sums are fp32 (the tokens that a row sees
+ * times their largest value must stay below 2^119). Factors of the tensor cores are fp16: in calls of few rows per sequence probabilities
+ * times value scales (outputs are off by 3e-4 of their norm, of which fp16 outputs have 2.1e-4 anyhow), in calls of many also
+ * keys and values, by 2^-11 of them at most (5.5e-4; bf16 outputs: 1.7e-3 in both). Which of the two a row goes by depends on the mean
+ * number of rows of the call's sequences, so its last bits do too.
  * Any number of rows, contexts and sequences; the lengths stay on the device, and the call can be captured. Equal calls give equal
  * bits. Every wait inside is bounded: one that runs out ends the call, and tf_device_status reports 0x7F000053.
  * Replaces attention_decode_partial / _gqa_swa_partial / _combine (Metal/Attention/attention.metal:135,227,343) and

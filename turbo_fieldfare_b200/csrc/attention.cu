@@ -1,4 +1,4 @@
-// Entry points of the attention over the quantised cache (kernels: attention.cuh).
+// Entry points of the attention over the quantised cache (kernels: attention_rows.cuh, attention_tiles.cuh).
 #include "attention_launch.cuh"
 
 #include <new>

@@ -98,7 +98,6 @@ struct Cursor {
         }
         range.set(a, seq, flat0, MT, TILE);
     }
-    __host__ __device__ __forceinline__ void advance(const AttnArgs& a) { if (++tile == range.tiles) next_unit(a); }
 };
 
 // Tiles of a sequence's rows for one kv head, over all its units.

@@ -18,10 +18,11 @@
 // K_i and V_i carry code * scale + bias rounded once to fp16, at most 2^-11 of the value, and P its probabilities likewise: each adds an error of the size
 // of the output's own rounding to fp16 (together 4e-4 to 5e-4 of the output's norm against 64 bits, 2e-4 of which fp16 outputs have anyhow; nothing next to
 // bf16's 1.7e-3). Exact products of codes, as the kernel for few rows has them, would need an accumulator per group. A token whose planes are
-// out of the ordinary is divided by a power of two of its own first; K's comes back with the logits, V's into the probabilities, p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far, up and, as m is raised, down:
-// tokens that a row does not see, or that have lost their weight, have no say, and no cache leaves fp16's range. m is raised only
-// when a logit exceeds it by 8, and what O holds is rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory alone,
-// are two units with half of the values each.
+// out of the ordinary is divided by a power of two of its own first; K's comes back with the logits, V's goes into the probabilities,
+// p' = 2^(x - m - E) * 2^e, where E is a row's own and follows the largest p' so far, up and, as m is raised, down: tokens that a row does not
+// see, or that have lost their weight, have no say, and no cache leaves fp16's range. m is raised only when a logit exceeds it by 8, and what O
+// holds is rescaled only when m or E moves. TILE * D is 16384 but for heads of 64; heads of 512, whose product would fill tensor memory
+// alone, are two units with half of the values each.
 #pragma once
 
 #include "async_copy.cuh"
@@ -943,7 +944,8 @@ tf_status attend(tf_context* ctx, cudaStream_t st, const AttnArgs& a, const tf_a
     // so it takes more rows where there are many units; where there are few, many warps share one of eight, and joining their shares costs a few us per row.
     // Measured in us, eight / 128: 8 * 2 units of 4000 tokens with heads of 256, 4 rows: 48 / 36, 1 row: 34 / 36; 8 * 8 of 8000, 16 rows: 127 / 127, 24: 160 / 127;
     // 8 * 32 of 3000 with 4-bit heads of 128, 24 rows: 134 / 124, of 1800 on average, 28 rows: 84 / 110. Heads of 512 are two units each, whose tiles
-    // are of 32 tokens: 2 * 32 units of 4000, 32 rows: 176 / 272, 48: 248 / 279.
+    // are of 32 tokens: 2 * 32 units of 4000, 32 rows: 176 / 272, 48: 248 / 279. All of these are batches of like sequences. The mean goes by the call's rows,
+    // padding included, and by all its sequences: single tokens beside a long prompt chunk all go by the one or the other, right but slower than apart.
     const uint64_t mean = ((uint64_t)a.rows + a.sequences - 1) / a.sequences * a.group, units = (uint64_t)a.sequences * a.kv_heads * (D == 512 ? 4 : 1);
     // In place heads of 512 have units of eight: a unit of 128 rows reads all of a row of q for half of its values, and the other half's unit may do so
     // later. Us beside / in place, 16 heads on 2: 200 trees of 5 rows over 40 tokens 84 / 80, 8 trees of 61 over 8000 532 / 1135, 333 rows over 8000 369 / 901.

@@ -336,7 +336,7 @@ qkv_epilogue_kernel(const EpilogueArgs a) {
 
 // Many rows: a block takes eight rows and up to eight heads of one kind, a warp per row. So the kind is known to the whole block (its branches and
 // addresses cost no lane's instructions), weights and angles of a lane's elements stay in registers, and no warp waits for another. 4096 rows of 32
-// heads of 256 into an 8-bit cache: 45 us, 2.6 TB/s; it is bound by issuing some 220 instructions per head. With warps of mixed kinds it was 76 us; heads two
+// heads of 256 into an 8-bit cache: 45 us, 2.6 TB/s; it is bound by issuing some 235 instructions per head. With warps of mixed kinds it was 76 us; heads two
 // by two at half the registers are 5 us faster than four by four.
 constexpr uint32_t kBlockHeads = 8;
 template <int D, bool BF16>
