@@ -224,6 +224,30 @@ def test_single_tokens_beside_a_prompt_chunk(tf_ctx, workspaces, singles, chunk,
     _close(got, *ref.attention(case, q, _all_visible(case, window), dim ** -0.5, half_step(F16)))
 
 
+# ---- pages ----
+
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("gone", [-1, 10 ** 6])
+def test_pages_that_fell_out_of_every_window(tf_ctx, workspaces, many, dim, bits, tree, gone):
+    """The table names no page at tokens that no row sees: nothing is wrong with such a call."""
+    rows, contexts, window = [40, 24], [930, 407], 100
+    case = Case(160 + dim, rows, contexts, 2, dim, bits, 16, DEV)
+    full = case.table.clone()
+    for b, c in enumerate(contexts):
+        case.table[b, :(c - window + 1) // 16] = gone
+    _by(case, 16, many).upload()
+    rng = np.random.default_rng(9)
+    trees = [_tree(n, rng) for n in rows]
+    masks, positions = [s for seen, _ in trees for s in seen], [c + d for c, (_, depth) in zip(contexts, trees) for d in depth]
+    q = _q(case, 16, F16)
+    got = _run(tf_ctx, workspaces, case, q, F16, window=window, masks=masks if tree else None, positions=positions if tree else None)
+    case.table = full
+    see = [ref.visible(n, c, window, *((seen, [c + d for d in depth]) if tree else ())) for n, c, (seen, depth) in zip(rows, contexts, trees)]
+    _close(got, *ref.attention(case, q, see, dim ** -0.5, half_step(F16)))
+
+
 # ---- cache write ----
 
 @pytest.mark.parametrize("rows", [3, 900])                       # a warp per head; a warp per eight heads

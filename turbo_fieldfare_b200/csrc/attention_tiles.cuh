@@ -359,10 +359,7 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                     else to[0] = words[0];
                 }
                 if (of_v) {
-                    if (held && !is) {
-                        bits = 0x80u;
-                        *a.error = kErrKvPage;
-                    }
+                    if (held && !is) bits = 0x80u;
                     meta.v_up[n & 7][key] = up;
                     meta.bad[n & 7][key] = (uint8_t)bits;
                     if (bits) any |= 2u;
@@ -677,8 +674,12 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
                         }
                     }
                     if (odd)
+#pragma unroll 1
                         for (int j = 0; j < CHUNK; ++j)
-                            if (meta.bad[i & 7][side * HALF + c0 + j] & 0x80u) seen &= ~(1u << j);
+                            if ((meta.bad[i & 7][side * HALF + c0 + j] & 0x80u) && (seen >> j & 1u)) {
+                                seen &= ~(1u << j);
+                                if (is) *a.error = kErrKvPage;         // (pages of tokens that no row sees may be missing: those that fell out of every window)
+                            }
                     return is ? seen : 0u;
                 };
                 // the logits of a chunk, in base 2 but for `by`
