@@ -224,6 +224,30 @@ def test_single_tokens_beside_a_prompt_chunk(tf_ctx, workspaces, singles, chunk,
     _close(got, *ref.attention(case, q, _all_visible(case, window), dim ** -0.5, half_step(F16)))
 
 
+@pytest.mark.parametrize("many", [True, False])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 8), (512, 4)])
+@pytest.mark.parametrize("planes", [(1,), (2,), (4,), (5,), (4, 5), (1, 2, 4, 5)])
+def test_planes_of_the_largest_numbers_reach_only_the_rows_that_see_them(tf_ctx, workspaces, many, dim, bits, planes):
+    """Tokens before the window in a tile with tokens inside, and drafted tokens that no row sees, with planes of 3e38, whose values leave fp32."""
+    rows, contexts, window = [40, 24], [930, 407], 100
+    case = Case(170 + dim, rows, contexts, 2, dim, bits, 16, DEV)
+    masks = [{j for j in range(i + 1) if j != 3} for n in rows for i in range(n)]
+    for b, (n, c) in enumerate(zip(rows, contexts)):
+        t = torch.tensor([*range(c - window), c + 3])
+        for i in planes:
+            case.planes[i][case.table[b, t // 16].long(), :, t % 16, 0] = 3e38 if i % 3 == 1 else -3e38
+    _by(case, 16, many).upload()
+    q = _q(case, 16, F16)
+    positions = [c + i for n, c in zip(rows, contexts) for i in range(n)]
+    got = _run(tf_ctx, workspaces, case, q, F16, window=window, masks=masks, positions=positions)
+    for b, (n, c) in enumerate(zip(rows, contexts)):
+        t = torch.tensor([*range(c - window), c + 3])
+        for i in planes:
+            case.planes[i][case.table[b, t // 16].long(), :, t % 16, 0] = 0.0
+    see = [ref.visible(n, c, window, masks[o:o + n], positions[o:o + n]) for n, c, o in zip(rows, contexts, case.offsets)]
+    _close(got, *ref.attention(case, q, see, dim ** -0.5, half_step(F16)))
+
+
 # ---- pages ----
 
 @pytest.mark.parametrize("many", [True, False])

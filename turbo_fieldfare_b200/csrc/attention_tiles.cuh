@@ -337,7 +337,8 @@ attention_tiles_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
                 for (int g = 0; g < N; ++g) {
                     const float size = fmaxf(kCentre * fabsf(sc[g]), fabsf(bi[g]));        // a third of the largest value or more
-                    const bool finite = sc[g] - sc[g] == 0.0f && bi[g] - bi[g] == 0.0f;
+                    // nor do planes whose values leave fp32 have a place in fp16 (times a probability of zero they would be no number)
+                    const bool finite = sc[g] - sc[g] == 0.0f && bi[g] - bi[g] == 0.0f && size <= 3.402823466e38f;
                     plain = plain && finite && size >= (fabsf(sc[g]) >= kExact ? least : 0.0625f) && size <= largest;
                     most = finite ? fmaxf(most, size) : most;
                     if (of_v && !finite) {
