@@ -837,7 +837,8 @@ typedef struct tf_kv_cache {
  *   where a call does not need them).
  * No call reads or writes outside a table or a plane, whatever the arrays hold: a row or token whose page is not in
  * [0, num_pages), or lies beyond the table, is left out, and tf_device_status reports 0x7F000051 (in an attention pages of tokens before
- * every row's window may be missing); offsets that descend or pass `rows` are cut, and it reports 0x7F000052. With rows == 0 a call does nothing, and its row buffers may be NULL. */
+ * every row's window may be missing); offsets that descend or pass `rows` are cut, and it reports 0x7F000052. With rows == 0 a
+ * call does nothing, and its row buffers may be NULL. */
 typedef struct tf_kv_batch {
     const int32_t* row_offsets;
     const int32_t* context_lengths;

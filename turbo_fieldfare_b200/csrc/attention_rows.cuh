@@ -12,10 +12,10 @@
 // O^T[element][row] = V^T P^T, with V's codes as A, again as subnormals: the value scale goes into the probability, p' = p s 2^-E rounded to
 // fp16, and what the bias adds is summed in fp32. The rounding of p' shall weigh a code's distance from the centre of the codes, not the code
 // itself: sum p' (c - centre) = sum p' c - centre sum p', with sum p' of all groups by one more MMA each into the rows of a common
-// accumulator, against sum p (b + centre s). (The tensor cores line a subnormal up as if it were fp16's least normal number: a sum of 4-bit codes is good to
-// 2^-16 of sum p |b|, which shows only in outputs that are a small remainder of it.) E is a row's own, after the largest p s so far (tokens that it does not see have p = 0
-// and no say; when m is raised, those before lose theirs), and m a maximum that is raised only when a logit exceeds it by 8: one vote per
-// tile, and what was summed is rescaled only when one of them moves.
+// accumulator, against sum p (b + centre s). (The tensor cores line a subnormal up as if it were fp16's least normal number: a sum of
+// 4-bit codes is good to 2^-16 of sum p |b|, which shows only in outputs that are a small remainder of it.) E is a row's own, after the largest
+// p s so far (tokens that it does not see have p = 0 and no say; when m is raised, those before lose theirs), and m a maximum that is raised
+// only when a logit exceeds it by 8: one vote per tile, and what was summed is rescaled only when one of them moves.
 //
 // What it measured, 8-bit heads of 256 on 8 kv heads, two rows each: 64 sequences of up to 4096 tokens 130 us, 4.9 TB/s; 131000 tokens of one sequence, heads of
 // 128: 75 us, 3.7 TB/s; 4-bit heads of 512, 200 sequences of up to 8192 tokens, eight rows per kv head: 310 us, 3.6 TB/s, bound by unpacking (2200 clocks a
