@@ -74,7 +74,7 @@ enum {
     TF_ERR_NOT_FOUND = 205         /* ModelError.tensorNotFound */
 };
 
-typedef enum { TF_BF16 = 0, TF_FP16 = 1 } tf_dtype;
+typedef enum { TF_BF16 = 0, TF_FP16 = 1, TF_FP32 = 2 } tf_dtype;     /* TF_FP32: where a call says so */
 
 /* Nine byte offsets into one expert blob: gate{W,S,B} | up{W,S,B} | down{W,S,B}.
  * Replaces MoEExpertOffsets (Kernels/MoE/MoE.swift:4-29) and the MSL
@@ -913,6 +913,99 @@ tf_status tf_tree_attention(tf_context* ctx, void* stream, const void* q, uint32
                             void* out, uint32_t out_stride_elements, const tf_kv_cache* cache, const tf_kv_batch* batch,
                             const uint64_t* tree_mask, uint32_t mask_words, uint32_t window, float scale,
                             uint32_t q_heads, tf_dtype act_dtype, tf_attention_workspace* ws);
+
+/* ---- a batched step with drafted tokens (the reference decodes one sequence, drafts nothing and samples on its own; these calls replace
+ * what its runner does on the CPU between the steps, Runtime/Generation/RawCompletion.swift:81-246) ----
+ * A step: tf_kv_plan, then per layer tf_qkv_epilogue and tf_tree_attention, then tf_verify_drafts on the logits and tf_kv_cache_keep. Every length
+ * stays on the device, so that one captured graph serves all steps: the next plan takes what the verification kept. */
+
+/* Drafted tokens of every sequence, device arrays [sequences][stride]. Node 0 of a sequence is the newest token that is not in the cache yet, the
+ * others hang under it: parents[b][i] < i is the node that node i continues; -1 (node 0) hangs under the cached context. parents NULL: a
+ * chain, node i continues node i - 1. A sequence of a step has as many nodes as it has rows. */
+typedef struct tf_drafts {
+    const int32_t* tokens;      /* may be NULL where a call does not need them */
+    const int32_t* parents;
+    uint32_t stride;
+} tf_drafts;
+
+/* The pages of a cache and who holds them; device arrays of the caller. Table entries [first_pages[b], held_pages[b]) of a sequence are its
+ * own (first_pages NULL: from 0); free_pages[0 .. *free_count) is a stack of the pages that nobody holds, with room for num_pages of them.
+ * At the beginning: held_pages and first_pages zero, all pages on the stack. page_size as in tf_kv_cache. */
+typedef struct tf_kv_pages {
+    int32_t *page_table, *held_pages, *first_pages, *free_pages, *free_count;
+    uint32_t page_table_stride, num_pages, page_size, sequences;
+} tf_kv_pages;
+
+/* What a plan writes: row_offsets [sequences + 1] and positions [rows], as in tf_kv_batch; and, each of them where it is not NULL, per row its sequence, the slot
+ * page * page_size + token % page_size that its keys and values go to, its token, and tree_mask [rows][mask_words] as in
+ * tf_tree_attention. rows is the room; rows behind the last sequence's stay as they were. */
+typedef struct tf_kv_rows {
+    int32_t *row_offsets, *positions, *sequences;
+    int64_t* slots;
+    int32_t* tokens;
+    uint64_t* tree_mask;
+    uint32_t mask_words, rows;
+} tf_kv_rows;
+
+/* The rows and pages of the next step, all on the device. In this order:
+ *   - context_lengths[b] += kept[b] (kept may be NULL; below zero counts as zero);
+ *   - a sequence with new_rows[b] < 0 has ended: its pages go back, its table entries become -1, its lengths and kept[b] do not matter any more and
+ *     context_lengths[b] becomes 0. With window > 0 (needs first_pages) pages that no row from context_lengths[b] on sees go back too;
+ *   - the others get their new_rows[b] rows in ascending order, behind context_lengths[b], with pages from the stack for the tokens that have none. The first sequence
+ *     whose pages or rows do not fit any more and all behind it get no rows and no pages in this step (row_offsets tells; ask again). One whose tokens
+ *     do not fit the table, or whose rows are more than drafts->stride, is passed over.
+ * Pages go back so that a page taken last is taken next: the page given back (or needed) j-th, in the order of sequences and tokens, lies (or is
+ * found) at place j from the top. Row i of a sequence: position context_lengths[b] + i, with parents context_lengths[b] + the node's depth. drafts may be NULL; it is needed for rows->tokens
+ * (its tokens) and rows->tree_mask (its parents, or a chain). A row's mask has the bits of its node and of its ancestors.
+ * Equal inputs give equal outputs. tf_device_status reports 0x7F000054 where the arrays contradict themselves (a stack outside [0, num_pages], more
+ * pages given back than it has room for, a parent that is not before its node, which then counts as -1, a node from 64 * mask_words on);
+ * nothing outside the arrays is read or written whatever they hold. A depth of d takes d steps. */
+tf_status tf_kv_plan(tf_context* ctx, void* stream, const tf_kv_pages* pages, int32_t* context_lengths, const int32_t* new_rows, const int32_t* kept,
+                     uint32_t window, const tf_drafts* drafts, const tf_kv_rows* rows);
+
+/* Scratch of tf_verify_drafts for up to max_rows rows of up to max_vocab logits (rows * vocab of a call may be at most their product). It serves one call at
+ * a time, like tf_attention_workspace; what a call leaves in it does not matter to the next. */
+typedef struct tf_verify_workspace tf_verify_workspace;
+tf_status tf_verify_workspace_create(tf_context* ctx, uint32_t max_rows, uint32_t max_vocab, tf_verify_workspace** out);
+void tf_verify_workspace_destroy(tf_verify_workspace* ws);
+uint64_t tf_verify_workspace_bytes(const tf_verify_workspace* ws);
+
+/* The distributions that drafted tokens were drawn from: values[b * sequence_stride + i * node_stride + v] is the probability with which the children of node i < nodes were
+ * drawn, each by itself. Strides in elements. Values below zero and NaN count as zero. */
+typedef struct tf_draft_probs {
+    const void* values;
+    uint64_t sequence_stride, node_stride;
+    uint32_t nodes;
+    tf_dtype dtype;             /* any of the three */
+} tf_draft_probs;
+
+/* Which drafted tokens are kept, and the next token, so that the tokens are distributed as if the target had drawn every one itself. Row row_offsets[b] + i of
+ * `logits` [rows][vocab] (any of the three types, any alignment of its elements) is what the target says behind node i:
+ *   p = softmax(l / T), l = softcap * tanh(logit / softcap) with softcap > 0, T = temperatures[b] (NULL: 1). Logits that are not finite count for nothing (a caller
+ *   cuts a distribution by setting the others to -inf).
+ * From node 0 on, the children of the current node are tried in ascending order, child i with token x and u = uniforms[b * drafts->stride + i]:
+ *   with probs (and the node's row in it), q being that row: kept if u q(x) < p_r(x), where r children were refused before: p_0 = p, p_{r+1} = max(p_r - q, 0) / its sum;
+ *   without: kept if u < p_r(x), where p_{r+1} is p_r without x, divided by its sum (the drafter took its likeliest tokens).
+ * A kept child becomes the current node. When none is kept, the next token is the first v with p_r(0) + ... + p_r(v) > uniforms[b * drafts->stride] (p itself
+ * where p_r has nothing left). A child whose token is not in [0, vocab) is passed over.
+ * T <= 0 or NaN: a child is kept if it is the target's likeliest token (lowest index), which is also the next token; no random numbers.
+ * Outputs, [sequences][drafts->stride]: out_tokens the kept tokens and behind them the next token; out_rows node 0 and the kept nodes; -1 behind them. kept[b]: how many, the next
+ * token included (0 for a sequence without rows): what tf_kv_cache_keep and the next tf_kv_plan take. logprobs (may be NULL): log p of out_tokens (T = 1 where T <= 0), zero behind
+ * them. A sequence whose last row has no finite logit gets token 0, log p = -inf. With drafts->stride 1 the call is a sampler.
+ * uniforms are in [0, 1). Sums that a token is drawn from and tests near their border are 64-bit; equal calls give equal bits. drafts->stride is at most 1024; a sequence of more rows is
+ * cut there and tf_device_status reports 0x7F000052, as for offsets that descend or pass `rows`. Calls without sequences do nothing.
+ * Replaces sample / sample_topk64 (Metal/Sampling/logit.metal:184,490,517,545) and logit_softcap_softmax (:53) for what they have in common with it. */
+tf_status tf_verify_drafts(tf_context* ctx, void* stream, const void* logits, uint64_t logits_stride_elements, tf_dtype logits_dtype, uint32_t vocab,
+                           const int32_t* row_offsets, uint32_t rows, uint32_t sequences, const tf_drafts* drafts, const float* uniforms,
+                           const tf_draft_probs* probs, const float* temperatures, float softcap,
+                           int32_t* out_tokens, int32_t* out_rows, int32_t* kept, float* logprobs, tf_verify_workspace* ws);
+
+/* The cache rows of the kept nodes behind their context: in each of the `cache_count` caches (HOST array of descriptors; the layers that share the batch's page
+ * table, all of one page size) token context_lengths[b] + kept_rows[b * kept_stride + i] goes to token context_lengths[b] + i for i < kept[b], codes and planes as they are. The nodes of a
+ * sequence ascend, as tf_verify_drafts writes them; a node that does not, or is not one of the sequence's rows, ends its sequence's moves (tf_device_status: 0x7F000052). A token whose
+ * page is missing is left out (0x7F000051). positions are not used. Sequences must not share the pages that they append to. */
+tf_status tf_kv_cache_keep(tf_context* ctx, void* stream, const tf_kv_cache* caches, uint32_t cache_count, const tf_kv_batch* batch,
+                           const int32_t* kept_rows, uint32_t kept_stride, const int32_t* kept);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "_lib" / "libtfcuda.so"
 HEADER_PATH = PKG.parent / "include" / "turbofieldfare_cuda.h"
 
-TF_BF16, TF_FP16 = 0, 1
+TF_BF16, TF_FP16, TF_FP32 = 0, 1, 2
 TF_MAX_TOP_K = 8
 
 vp, u32, u64, i32, f32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32, C.c_float
@@ -90,6 +90,27 @@ class KVBatchDesc(C.Structure):
     """tf_kv_batch: where the rows of a call belong."""
     _fields_ = ([(n, vp) for n in ("row_offsets", "context_lengths", "page_table", "positions")] +
                 [(n, u32) for n in ("page_table_stride", "sequences", "rows")])
+
+
+class Drafts(C.Structure):
+    """tf_drafts: drafted tokens of every sequence and what they continue."""
+    _fields_ = [("tokens", vp), ("parents", vp), ("stride", u32)]
+
+
+class KVPagesDesc(C.Structure):
+    """tf_kv_pages: the pages of a cache and who holds them."""
+    _fields_ = ([(n, vp) for n in ("page_table", "held_pages", "first_pages", "free_pages", "free_count")] +
+                [(n, u32) for n in ("page_table_stride", "num_pages", "page_size", "sequences")])
+
+
+class KVRowsDesc(C.Structure):
+    """tf_kv_rows: what a plan writes."""
+    _fields_ = ([(n, vp) for n in ("row_offsets", "positions", "sequences", "slots", "tokens", "tree_mask")] + [("mask_words", u32), ("rows", u32)])
+
+
+class DraftProbs(C.Structure):
+    """tf_draft_probs: the distributions that drafted tokens were drawn from."""
+    _fields_ = [("values", vp), ("sequence_stride", u64), ("node_stride", u64), ("nodes", u32), ("dtype", C.c_int)]
 
 
 _PLANES = [vp, u64, vp, u64, vp, u64]   # weights, scales, biases with offsets
@@ -219,6 +240,12 @@ SIGNATURES = {
     "tf_attention_workspace_bytes": (u64, [vp]),
     "tf_tree_attention": (C.c_int, [vp, vp, vp, u32, vp, u32, C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), vp, u32, u32, f32, u32,
                                     C.c_int, vp]),
+    "tf_kv_plan": (C.c_int, [vp, vp, C.POINTER(KVPagesDesc), vp, vp, vp, u32, C.POINTER(Drafts), C.POINTER(KVRowsDesc)]),
+    "tf_verify_workspace_create": (C.c_int, [vp, u32, u32, C.POINTER(vp)]),
+    "tf_verify_workspace_destroy": (None, [vp]),
+    "tf_verify_workspace_bytes": (u64, [vp]),
+    "tf_verify_drafts": (C.c_int, [vp, vp, vp, u64, C.c_int, u32, vp, u32, u32, C.POINTER(Drafts), vp, C.POINTER(DraftProbs), vp, f32, vp, vp, vp, vp, vp]),
+    "tf_kv_cache_keep": (C.c_int, [vp, vp, C.POINTER(KVCacheDesc), u32, C.POINTER(KVBatchDesc), vp, u32, vp]),
     "tf_layer_tail": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, f32, f32]),
 }
 

@@ -211,6 +211,7 @@ tf_status tf_rmsnorm(tf_context* ctx, void* stream, const void* x, uint64_t x_of
     TF_REQUIRE(ctx, ctx != nullptr, TF_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", name);
     TF_REQUIRE(ctx, x && y, TF_ERR_INVALID_ARGUMENT, "%s: NULL buffer", name);
     TF_REQUIRE(ctx, d > 0 && stride_elements >= d, TF_ERR_INVALID_ARGUMENT, "%s: stride is too small", name);
+    TF_REQUIRE(ctx, act_dtype != TF_FP32, TF_ERR_UNSUPPORTED, "%s: rows are fp16 or bf16", name);
     if (rows == 0) return TF_OK;
     auto xp = reinterpret_cast<const uint16_t*>(tf::byte_ptr(x, x_off));
     auto yp = reinterpret_cast<uint16_t*>(tf::byte_ptr(y, y_off));
