@@ -1,9 +1,9 @@
 // Verification of drafted tokens, and with one row per sequence a sampler (tf_verify_drafts).
 //
 // With weights w(v) = exp((l(v) - max l) / T) and Z their sum, p = w / Z. A child x drawn from q is kept when u q(x) < p_r(x), where r of its
-// siblings were refused: p_{r+1} = max(p_r - q, 0) over its sum. Written out, p_r = max(p - c_r q, 0) / S_r with S_r the sum of the numerators, c_0 = 0,
-// S_0 = 1 and c_{r+1} = c_r + S_r, so a refusal costs one sum over the vocabulary and no distribution is ever stored; here both are kept times Z.
-// Without q a refused token's weight is left out.
+// siblings were refused: p_{r+1} = max(p_r - q, 0) over its sum. Undivided, n_0 = w and n_{r+1} = max(n_r - S_r q, 0) with S_r the sum of n_r: a refusal
+// costs one sum over the vocabulary and leaves one number, and no distribution is ever stored, since n_r(v) follows from w(v), q(v) and the sums so far. (It could be written
+// as max(w - c q, 0) with one c, which cancels once little is left; step by step nothing does.) Without q a refused token's weight is left out.
 //
 // Two launches. The first reads every row that has children once, all in parallel, and leaves its maximum and sum by chunks in 32 bits: HBM bounds it.
 // The second has a cluster of thread blocks per sequence. Its first block walks the tree: a test needs a logit, a number of q and Z. Z in 32 bits is off by
@@ -243,15 +243,15 @@ __device__ __forceinline__ double logit64(float x, float cap) {
 struct Order {
     int what;                  // 0: nothing more; 1: sums; 2: sums and a draw
     uint32_t node, at;         // at: where the token goes
-    int known, summed, step, drawn, gone;      // its maximum is known; so is Z; c is to rise by S; q counts; refused tokens to leave out
+    int known, summed, step, drawn, refused;   // its maximum is known; so is Z; the last refusal's sum is not noted yet; q counts; children refused
     float most, u;
-    double z, c, s;
+    double z, s;               // Z, and the last sum
 };
 
 struct Walk {
     uint32_t i, node, at;
-    int refused, done, summed, gone, step;
-    double z, c, s, gone_weight;
+    int refused, done, summed, step;
+    double z, s, gone;         // gone: weight of the refused tokens, without q
 };
 
 __device__ __forceinline__ float prob_at(const VerifyArgs& a, uint64_t at) {
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
     __shared__ Walk walk;
     __shared__ double block_sum[2], warp_part[kWalkWarps];
     __shared__ float block_most[2], warp_most[kWalkWarps];
-    __shared__ int32_t gone[kMostNodes];
+    __shared__ union { double sum[kMostNodes]; int32_t token[kMostNodes]; } gone;      // of the node's refused children: S before each, or the tokens
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const uint32_t rank = cluster.block_rank(), ranks = cluster.num_blocks(), b = blockIdx.x / ranks;
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 best[i] = at == 0xFFFFFFFFu ? 0u : at;
             }
         }
-        if (tid == 0) walk = {1, 0, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0, 0.0};
+        if (tid == 0) walk = {1, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0};
         __syncthreads();
         if (tid == 0 && of.n) walk.z = z32[0];
     }
@@ -367,17 +367,17 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                     const double q = (double)prob[i];
                     if (w.step) ask = true;            // the last refusal's sum first
                     left = u * q * (w.refused ? w.s : w.z);
-                    if (w.refused) right = fmax(weight - w.c * q, 0.0);
-                    else if (!w.summed) ask |= fabs(left - right) < bound * left;
+                    for (int g = 0; g < w.refused && !w.step; ++g) right = fmax(right - gone.sum[g] * q, 0.0);
+                    if (!w.refused && !w.summed) ask = fabs(left - right) < bound * left;
                 } else {
                     bool before = false;
-                    for (int g = 0; g < w.gone; ++g) before |= gone[g] == token[i];
+                    for (int g = 0; g < w.refused; ++g) before |= gone.token[g] == token[i];
                     if (before) continue;              // refused already
-                    left = u * (w.z - w.gone_weight);
+                    left = u * (w.z - w.gone);
                     if (!w.summed) ask = fabs(left - right) < bound * u * w.z;
                 }
                 if (ask) {
-                    order = {1, w.node, 0, 1, w.summed, w.step, drawn, 0, most[w.node], 0.0f, w.z, w.c, w.refused > 1 ? w.s : 0.0};
+                    order = {1, w.node, 0, 1, w.summed, w.step, drawn, w.refused, most[w.node], 0.0f, w.z, w.s};
                     return;
                 }
                 keep = left < right;
@@ -388,17 +388,17 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 if (logprobs) logprobs[w.at] = (float)(x2 * kLn2 - log(w.z));
                 w.at += 1;
                 w.node = i;
-                w.refused = w.summed = w.gone = w.step = 0;
+                w.refused = w.summed = w.step = 0;
                 w.z = z32[i];
-                w.c = w.s = w.gone_weight = 0.0;
+                w.gone = 0.0;
             } else if (!heat.greedy) {
                 if (drawn) {
-                    w.refused += 1;
                     w.step = 1;
                 } else {
-                    gone[w.gone++] = token[i];
-                    w.gone_weight += weight;
+                    gone.token[w.refused] = token[i];
+                    w.gone += weight;
                 }
+                w.refused += 1;
             }
         }
         if (w.done) return;
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
             return;
         }
         const float u = fminf(fmaxf(a.uniforms[(size_t)b * a.draft_stride], 0.0f), 0x1.fffffep-1f);
-        order = {2, w.node, w.at, inner[w.node], w.summed, w.step, a.probs && w.node < a.probs_nodes, w.gone, most[w.node], u, w.z, w.c, w.refused > 1 ? w.s : 0.0};
+        order = {2, w.node, w.at, inner[w.node], w.summed, w.step, a.probs && w.node < a.probs_nodes, w.refused, most[w.node], u, w.z, w.s};
     };
 
     const double table = exp2((double)lane / 32.0);
@@ -460,7 +460,11 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
         cluster.sync();
         const Order o = *cluster.map_shared_rank(&orders[round & 1], 0);
         if (o.what == 0) break;
-        if (rank != 0) for (int g = tid; g < o.gone; g += kWalkThreads) gone[g] = *cluster.map_shared_rank(&gone[g], 0);
+        if (rank != 0) {
+            for (int g = tid; g < o.refused; g += kWalkThreads)
+                if (!o.drawn) gone.token[g] = *cluster.map_shared_rank(&gone.token[g], 0);
+                else if (!o.step || g + 1 < o.refused) gone.sum[g] = *cluster.map_shared_rank(&gone.sum[g], 0);
+        }
         __syncthreads();
 
         // ---- this warp's pieces of the row: neighbours, so that sums run in the order of the tokens ----
@@ -481,8 +485,8 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
             top = most_all(top);
         }
         const double from = top > -INFINITY ? logit64<CAP>(top, a.softcap) : 0.0;
-        // what is left of the weights of a piece: w - c q, without the refused tokens
-        auto left = [&](uint32_t piece, double c, int refused, double (&w)[E]) {
+        // what `refused` children leave of the weights of a piece
+        auto left = [&](uint32_t piece, int refused, double (&w)[E]) {
             float x[E];
             if (piece < pieces) row.load(piece, x);
             else
@@ -494,55 +498,57 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 const double v = warp_exp2(x[e] > -INFINITY ? (logit64<CAP>(x[e], a.softcap) - from) * heat.k : 0.0, table);
                 w[e] = x[e] > -INFINITY ? v : 0.0;
             }
-            if (c > 0.0 && piece < pieces)
+            if (refused && o.drawn) {
+                float q[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (first + e >= 0 && first + e < (int64_t)a.vocab) w[e] = fmax(w[e] - c * (double)prob_at(a, q_row + first + e), 0.0);
-            for (int g = 0; g < refused; ++g) {
-                const int64_t e0 = (int64_t)gone[g] - first;
+                for (int e = 0; e < E; ++e) q[e] = piece < pieces && first + e >= 0 && first + e < (int64_t)a.vocab ? prob_at(a, q_row + first + e) : 0.0f;
+                for (int g = 0; g < refused; ++g) {
+                    const double s = gone.sum[g];
 #pragma unroll
-                for (int e = 0; e < E; ++e) w[e] = e0 == e ? 0.0 : w[e];
+                    for (int e = 0; e < E; ++e) w[e] = fmax(w[e] - s * (double)q[e], 0.0);
+                }
+            } else {
+                for (int g = 0; g < refused; ++g) {
+                    const int64_t e0 = (int64_t)gone.token[g] - first;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) w[e] = e0 == e ? 0.0 : w[e];
+                }
             }
         };
-        auto sum_left = [&](double c, int refused) {
+        auto sum_left = [&](int refused) {
             double s = 0.0;
             for (uint32_t i = 0; i < steps; ++i) {
                 double w[E];
-                left(piece0 + i * kWarp, c, refused, w);
+                left(piece0 + i * kWarp, refused, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) s += w[e];
             }
             return sum_all(s);
         };
-        double z = o.z, c = o.c, s = o.s;
-        int refused = o.gone;
+        double z = o.z, s = 0.0;
+        int refused = o.what == 2 || o.drawn ? o.refused : 0;      // a test without q goes by Z alone
         bool parts = false;                        // the last sums are those that are drawn from
         if (!o.summed) {
-            z = sum_left(0.0, 0);
-            parts = true;
+            s = z = sum_left(0);
+            parts = refused == 0;
         }
-        if (o.step) c += c > 0.0 ? s : z;
-        if (!o.drawn) c = 0.0;
-        if (c > 0.0 || refused) {
-            s = sum_left(c, refused);
-            parts = true;
-            if (o.what == 2 && !(s > 0.0)) {       // nothing left: from all of it
-                c = 0.0;
-                refused = 0;
-                parts = false;
-            }
-        } else {
-            s = z;
+        if (refused) {
+            if (o.step && tid == 0) gone.sum[refused - 1] = refused == 1 ? z : o.s;
+            __syncthreads();
+            s = sum_left(refused);
+            parts = o.what == 1 || s > 0.0;
+            if (!parts) refused = 0;               // nothing left: from all of it
         }
         if (o.what == 1) {
             if (rank == 0 && tid == 0) {
-                walk.z = z; walk.c = c; walk.s = s;
+                walk.z = z;
+                walk.s = s;
                 walk.summed = 1;
                 walk.step = 0;
             }
             continue;                              // the thread that walks is the one that wrote
         }
-        if (!parts) s = sum_left(0.0, 0);
+        if (!parts) s = sum_left(0);
 
         // ---- the draw: block, warp, piece, token ----
         const double target = (double)o.u * s;
@@ -576,7 +582,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
         int64_t token_at = -1, last = -1;
         for (uint32_t i = 0; i < steps; ++i) {
             double w[E], all = 0.0;
-            left(piece0 + i * kWarp, c, refused, w);
+            left(piece0 + i * kWarp, refused, w);
 #pragma unroll
             for (int e = 0; e < E; ++e) all += w[e];
             double run = all;
