@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 
 #include <new>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
@@ -27,12 +28,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kStatsThreads = 256, kChunk = 8192;          // elements of a row that a block of the first launch takes
-constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / kWarp;
+constexpr int kStatsThreads = 256, kChunk = 8192;          // elements that a block of the first launch takes at a time
+constexpr int kWalkThreads = 256, kWalkWarps = kWalkThreads / kWarp;
 constexpr uint32_t kMostNodes = 1024;
 constexpr double kLog2E = 1.4426950408889634074;
 
-// A chunk's largest logit, the sum of its weights relative to that, and where the largest stands first.
+// The largest logit of some chunks, the sum of their weights relative to that, and where the largest stands first.
 struct ChunkStat {
     float most, sum;
     uint32_t at, unused;
@@ -49,7 +50,7 @@ struct VerifyArgs {
     float* logprobs;
     ChunkStat* stats;
     uint32_t* error;
-    uint32_t vocab, rows, sequences, draft_stride, probs_nodes, probs_dtype, chunks;
+    uint32_t vocab, rows, sequences, draft_stride, probs_nodes, probs_dtype, chunks, parts, per;       // a row's chunks are done in parts of `per`
     float softcap;
 };
 
@@ -67,7 +68,7 @@ __device__ __forceinline__ float verify_exp2(float x) {
 __device__ __forceinline__ float counted(float x) { return fabsf(x) < INFINITY ? x : -INFINITY; }
 
 // A row's elements in pieces of 16 aligned bytes: piece v holds elements [E v - lead, E v - lead + E), where the row begins `lead` elements behind
-// a 16-byte boundary. What lies outside the row is -infinity and is not read.
+// a 16-byte boundary. What lies outside the row is not read and counts for nothing.
 template <typename T>
 struct Row {
     static constexpr int E = 16 / sizeof(T);
@@ -78,17 +79,35 @@ struct Row {
     }
     __device__ __forceinline__ uint32_t pieces() const { return (uint32_t)(((uint64_t)vocab + lead + E - 1) / E); }
     __device__ __forceinline__ int64_t first(uint32_t piece) const { return (int64_t)piece * E - lead; }
-    __device__ __forceinline__ void load(uint32_t piece, float (&x)[E]) const {
+    __device__ __forceinline__ uint4 load(uint32_t piece) const {
         const int64_t at = first(piece);
-        if (at >= 0 && at + E <= (int64_t)vocab) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p + at);
-            T v[E];
-            memcpy(v, &w, 16);
+        if (at >= 0 && at + E <= (int64_t)vocab) return *reinterpret_cast<const uint4*>(p + at);
+        constexpr uint32_t nothing = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+        T v[E];
+        uint4 w = make_uint4(nothing, nothing, nothing, nothing);
+        memcpy(v, &w, 16);
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = counted(number(v[e]));
+        for (int e = 0; e < E; ++e)
+            if (at + e >= 0 && at + e < (int64_t)vocab) v[e] = p[at + e];
+        memcpy(&w, v, 16);
+        return w;
+    }
+    static __device__ __forceinline__ void numbers(const uint4& w, float (&x)[E]) {
+        T v[E];
+        memcpy(v, &w, 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = number(v[e]);
+    }
+    // The largest, without NaN
+    static __device__ __forceinline__ float most(const uint4& w) {
+        if constexpr (sizeof(T) == 4) {
+            return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
         } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = at + e >= 0 && at + e < (int64_t)vocab ? counted(number(p[at + e])) : -INFINITY;
+            using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+            T2 v[4];
+            memcpy(v, &w, 16);
+            const T2 all = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+            return number(__hmax(all.x, all.y));
         }
     }
 };
@@ -132,14 +151,42 @@ __device__ __forceinline__ int32_t parent_of(const VerifyArgs& a, uint32_t b, ui
 // maxima and sums of the rows with children
 // ---------------------------------------------------------------------------
 
+// softcap * tanh(x / softcap) where |x| <= softcap, as x P((x / softcap)^2): P is tanh(u) / u by its Chebyshev coefficients in u^2, 1.5e-7 of itself off in 32 bits. On the
+// arithmetic units, which have room here: with a reciprocal and a second power of two a logit these take as long as everything else together.
+__device__ __forceinline__ float capped_near(float x, float inverse) {
+    const float u = x * inverse, z = u * u;
+    float p = 0.0010455535957589746f;
+    p = fmaf(p, z, -0.006217069923877716f);
+    p = fmaf(p, z, 0.020305519923567772f);
+    p = fmaf(p, z, -0.05346517637372017f);
+    p = fmaf(p, z, 0.13325397670269012f);
+    p = fmaf(p, z, -0.33332857489585876f);
+    p = fmaf(p, z, 0.9999999403953552f);
+    return x * p;
+}
+
+// A thread keeps a maximum and a sum of its own over the chunks, so that no block meets at a barrier before the end, and has the next chunk's loads under way
+// while it works on one; the first chunk's before it knows whether the row has children.
 template <typename T, bool CAP>
-__global__ void __launch_bounds__(kStatsThreads) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     pdl_launch_dependents();
-    constexpr int E = Row<T>::E, PIECES = kChunk / E / kStatsThreads, WARPS = kStatsThreads / kWarp;
+    using R = Row<T>;
+    constexpr int E = R::E, PIECES = kChunk / E / kStatsThreads, WARPS = kStatsThreads / kWarp;
+    constexpr uint32_t STEP = kChunk / E;
     __shared__ uint32_t found, best;
     __shared__ float warp_most[WARPS], warp_sum_[WARPS];
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
-    const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const R r(a.logits, row * a.stride, a.vocab);
+    const uint32_t pieces = r.pieces(), end = min(pieces, (part + 1) * a.per * STEP);
+    uint32_t piece = part * a.per * STEP + tid;                // of this thread, the first of its chunk
+    uint4 next[PIECES];
+    auto request = [&] {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j)
+            if (piece + j * kStatsThreads < end) next[j] = r.load(piece + j * kStatsThreads);
+    };
+    request();
     if (tid == 0) found = best = 0xFFFFFFFFu;
     __syncthreads();
     for (uint32_t b = tid; b < a.sequences; b += kStatsThreads) {
@@ -158,42 +205,92 @@ __global__ void __launch_bounds__(kStatsThreads) verify_stats_kernel(const __gri
         else for (uint32_t j = i + 1 + tid; j < of.n; j += kStatsThreads) child |= parent_of(a, b, j) == (int32_t)i;
         if (!__syncthreads_or(child)) return;
     }
-    const Row<T> r(a.logits, row * a.stride, a.vocab);
-    const uint32_t pieces = r.pieces(), piece0 = chunk * (kChunk / E) + tid;
-    const float k = heat.k32();
-    float x[PIECES][E], most = -INFINITY;
+    const float k = heat.k32(), inverse = CAP ? 1.0f / a.softcap : 0.0f;
+    float most = -INFINITY, from = -INFINITY, sum = 0.0f;
+    uint32_t where = 0;                                        // the chunk of the first largest
+    for (; piece < end; piece += STEP) {
+        uint4 w[PIECES];
+        uint32_t n = 0;
+        float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < PIECES; ++j) {
-        if (piece0 + j * kStatsThreads < pieces) r.load(piece0 + j * kStatsThreads, x[j]);
-        else
+        for (int j = 0; j < PIECES; ++j)
+            if (piece + j * kStatsThreads < end) {
+                w[j] = next[j];
+                top = fmaxf(top, R::most(w[j]));
+                n = j + 1;
+            }
+        const uint32_t here = piece;
+        piece += STEP;
+        request();
+        piece = here;
+        if (top == INFINITY) {                                 // does not count
+            top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[j][e] = -INFINITY;
+            for (int j = 0; j < PIECES; ++j) {
+                float x[E];
+                R::numbers(w[j], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (j < n) top = fmaxf(top, counted(x[e]));
+            }
+        }
+        if (top > most) {
+            const float to = CAP ? capped(top, a.softcap) : top;
+            sum *= verify_exp2((from - to) * k);               // nothing so far: 0 times 0
+            most = top;
+            from = to;
+            where = piece;
+        }
+        if (most == -INFINITY) continue;
+        float add = 0.0f;
+        bool far = false;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j)
+            if (j < n) {
+                float x[E];
+                R::numbers(w[j], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if constexpr (CAP) {
+                        far |= !(fabsf(x[e]) <= a.softcap);
+                        x[e] = capped_near(x[e], inverse);
+                    }
+                    add += verify_exp2((x[e] - from) * k);
+                }
+            }
+        if (far || !(add < INFINITY)) {                        // logits beyond the cap's polynomial, infinities and NaN
+            add = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                float x[E];
+                R::numbers(w[j], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float c = counted(x[e]);
+                    if (j < n) add += verify_exp2(((CAP ? capped(c, a.softcap) : c) - from) * k);
+                }
+            }
+        }
+        sum += add;
     }
-#pragma unroll
-    for (int j = 0; j < PIECES; ++j)
-#pragma unroll
-        for (int e = 0; e < E; ++e) most = fmaxf(most, x[j][e]);
-    float top = most;          // of the warp, then of the block
+    float top = most;
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
     if (lane == 0) warp_most[warp] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) top = fmaxf(top, warp_most[w]);
-    float sum = 0.0f;
-    if (top > -INFINITY) {
-        const float from = CAP ? capped(top, a.softcap) : top;
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j)
-#pragma unroll
-            for (int e = 0; e < E; ++e) sum += verify_exp2(((CAP ? capped(x[j][e], a.softcap) : x[j][e]) - from) * k);
-        if (heat.greedy && most == top) {
+    if (most > -INFINITY) {
+        sum *= verify_exp2((from - (CAP ? capped(top, a.softcap) : top)) * k);
+        if (heat.greedy && most == top) {                      // few threads
             uint32_t at = 0xFFFFFFFFu;
-#pragma unroll
-            for (int j = PIECES - 1; j >= 0; --j)
+            for (int j = 0; j < PIECES && where + j * kStatsThreads < end && at == 0xFFFFFFFFu; ++j) {
+                float x[E];
+                R::numbers(r.load(where + j * kStatsThreads), x);
 #pragma unroll
                 for (int e = E - 1; e >= 0; --e)
-                    if (x[j][e] == top) at = (uint32_t)(r.first(piece0 + j * kStatsThreads) + e);
+                    if (x[e] == top) at = (uint32_t)(r.first(where + j * kStatsThreads) + e);
+            }
             atomicMin(&best, at);
         }
     }
@@ -203,7 +300,7 @@ __global__ void __launch_bounds__(kStatsThreads) verify_stats_kernel(const __gri
     if (tid == 0) {
         sum = 0.0f;
         for (int w = 0; w < WARPS; ++w) sum += warp_sum_[w];
-        a.stats[(size_t)row * a.chunks + chunk] = {top, sum, best, 0};
+        a.stats[(size_t)row * a.parts + part] = {top, sum, best, 0};
     }
 }
 
@@ -215,28 +312,40 @@ __global__ void __launch_bounds__(kStatsThreads) verify_stats_kernel(const __gri
 // add less than 2^-17; capped logits are off by at most softcap 2^-20 each.
 __device__ __forceinline__ double sum_bound(float cap, double k) { return 0x1p-15 + (cap > 0.0f ? (double)cap * k * 0x1p-19 : 0.0); }
 
-// 2^x for x <= 0 in 64 bits, by all lanes of a warp: 2^(j/32) from a table that the lanes hold, times the Taylor sum of 2^r, |r| <= 1/64, to its
-// fifth power (2e-15 of it), times a power of two. Below 2^-1000: 0.
-__device__ __forceinline__ double warp_exp2(double x, double table) {
-    const double y = fmax(x, -1000.0), shift = 6755399441055744.0;             // 1.5 2^52: the sum's last bits are the rounded number
-    const double t = fma(y, 32.0, shift);
+// 2^(y k / 32) in 64 bits by all lanes of a warp: 2^(j/32) from a table that the lanes hold, times the Taylor sum of 2^r, |r| <= 1/64, to its fifth power
+// (2e-15 of it), times a power of two. Exponents from -1000 to 1000; below, and for y = -infinity, 0.
+__device__ __forceinline__ double warp_exp2(double y, double k, double table) {
+    const double shift = 6755399441055744.0;                                    // 1.5 2^52: the sum's last bits are the rounded number
+    const double t = fma(y, k, shift);
     const int j = __double2loint(t);
-    const double r = fma(t - shift, -1.0 / 32, y);
-    double s = 0.0013333558146428443;                                           // ln(2)^i / i!, i = 5 ... 1
-    s = fma(s, r, 0.009618129107628477);
-    s = fma(s, r, 0.05550410866482158);
-    s = fma(s, r, 0.24022650695910072);
-    s = fma(s, r, 0.6931471805599453);
+    const double r = fma(y, k, shift - t);
+    constexpr double c = 0.69314718055994530942 / 32;
+    double s = c * c * c * c * c / 120;
+    s = fma(s, r, c * c * c * c / 24);
+    s = fma(s, r, c * c * c / 6);
+    s = fma(s, r, c * c / 2);
+    s = fma(s, r, c);
     s = s * r;
     const double base = __shfl_sync(kFullMask, table, j & 31);
     const double v = fma(base, s, base);
-    return x < -1000.0 ? 0.0 : __hiloint2double(__double2hiint(v) + ((j >> 5) << 20), __double2loint(v));
+    return t >= shift - 32000.0 ? __hiloint2double(__double2hiint(v) + ((j >> 5) << 20), __double2loint(v)) : 0.0;
 }
 
 template <bool CAP>
 __device__ __forceinline__ double logit64(float x, float cap) {
     if constexpr (CAP) return (double)cap * tanh((double)x / (double)cap);
     else return (double)x;
+}
+// The same by all lanes of a warp, 1e-13 softcap off: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps. twice: 64 log2(e) / cap.
+template <bool CAP>
+__device__ __forceinline__ double warp_logit64(float x, double cap, double twice, double table) {
+    if constexpr (!CAP) return (double)x;
+    const float edge = 20.0f * (float)cap;                                      // tanh is 1 to the last bit from there on
+    const double d = warp_exp2((double)fminf(fmaxf(x, -edge), edge), twice, table) + 1.0;
+    float y0;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"((float)d));
+    const double y = fma((double)y0, fma(-d, (double)y0, 1.0), (double)y0);
+    return x > -INFINITY ? fma(-2.0 * cap, y, cap) : -INFINITY;
 }
 
 // What the cluster does next, and with which row.
@@ -261,9 +370,39 @@ __device__ __forceinline__ float prob_at(const VerifyArgs& a, uint64_t at) {
     else q = __bfloat162float(static_cast<const __nv_bfloat16*>(a.probs)[at]);
     return fmaxf(q, 0.0f);     // NaN too
 }
+// E of them, of which those outside the row are zero
+template <int E>
+__device__ __forceinline__ void probs_at(const VerifyArgs& a, uint64_t row, int64_t first, float (&q)[E]) {
+    const bool whole = first >= 0 && first + E <= (int64_t)a.vocab;
+    if (a.probs_dtype == TF_FP32) {
+        const float* p = static_cast<const float*>(a.probs) + (int64_t)row + first;
+        if (whole && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+            uint4 w[E / 4];
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[e] = fmaxf(__uint_as_float(e % 4 == 0 ? w[e / 4].x : e % 4 == 1 ? w[e / 4].y : e % 4 == 2 ? w[e / 4].z : w[e / 4].w), 0.0f);
+            return;
+        }
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(a.probs) + (int64_t)row + first;
+        if (whole && reinterpret_cast<uintptr_t>(p) % (2 * E) == 0) {
+            uint32_t w[E / 2];
+            load_words<E / 2>(w, p);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const uint16_t v = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+                q[e] = fmaxf(a.probs_dtype == TF_FP16 ? f16_bits_to_float(v) : bf16_bits_to_float(v), 0.0f);
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[e] = first + e >= 0 && first + e < (int64_t)a.vocab ? prob_at(a, row + first + e) : 0.0f;
+}
 
 template <typename T, bool CAP>
-__global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
     constexpr int E = Row<T>::E;
     extern __shared__ __align__(16) uint8_t dynamic[];
     __shared__ Order orders[2];                    // by turns: one is read while the next is written
@@ -303,10 +442,10 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 if (lane == 0) most[i] = -INFINITY;
                 continue;
             }
-            const ChunkStat* s = a.stats + (size_t)(of.row0 + i) * a.chunks;
+            const ChunkStat* s = a.stats + (size_t)(of.row0 + i) * a.parts;
             float top = -INFINITY;
             uint32_t at = 0xFFFFFFFFu;
-            for (uint32_t c = lane; c < a.chunks; c += kWarp) {
+            for (uint32_t c = lane; c < a.parts; c += kWarp) {
                 const ChunkStat x = s[c];
                 if (x.most > top) { top = x.most; at = x.at; }                 // chunks ascend: the first of equals stays
             }
@@ -317,7 +456,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
             at = __reduce_min_sync(kFullMask, at);
             const float from = CAP ? capped(all, a.softcap) : all, k = heat.k32();
             double sum = 0.0;
-            for (uint32_t c = lane; c < a.chunks; c += kWarp) {
+            for (uint32_t c = lane; c < a.parts; c += kWarp) {
                 const ChunkStat x = s[c];
                 if (x.most > -INFINITY) sum += (double)(x.sum * verify_exp2(((CAP ? capped(x.most, a.softcap) : x.most) - from) * k));
             }
@@ -475,56 +614,67 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
         float top = o.most;
         if (!o.known) {
             top = -INFINITY;
-            for (uint32_t s = 0; s < steps; ++s) {
-                float x[E];
-                if (piece0 + s * kWarp >= pieces) break;
-                row.load(piece0 + s * kWarp, x);
+            for (uint32_t i = 0; i < steps; i += 4) {
+                uint4 w[4];
 #pragma unroll
-                for (int e = 0; e < E; ++e) top = fmaxf(top, x[e]);
+                for (int j = 0; j < 4; ++j)
+                    if (i + j < steps && piece0 + (i + j) * kWarp < pieces) w[j] = row.load(piece0 + (i + j) * kWarp);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j < steps && piece0 + (i + j) * kWarp < pieces) top = fmaxf(top, Row<T>::most(w[j]));
             }
             top = most_all(top);
-        }
-        const double from = top > -INFINITY ? logit64<CAP>(top, a.softcap) : 0.0;
-        // what `refused` children leave of the weights of a piece
-        auto left = [&](uint32_t piece, int refused, double (&w)[E]) {
-            float x[E];
-            if (piece < pieces) row.load(piece, x);
-            else
+            if (top == INFINITY) {                 // does not count: once more, one by one
+                top = -INFINITY;
+                for (uint32_t i = 0; i < steps; ++i) {
+                    if (piece0 + i * kWarp >= pieces) break;
+                    float x[E];
+                    Row<T>::numbers(row.load(piece0 + i * kWarp), x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = -INFINITY;
-            const int64_t first = row.first(piece);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const double v = warp_exp2(x[e] > -INFINITY ? (logit64<CAP>(x[e], a.softcap) - from) * heat.k : 0.0, table);
-                w[e] = x[e] > -INFINITY ? v : 0.0;
+                    for (int e = 0; e < E; ++e) top = fmaxf(top, counted(x[e]));
+                }
+                top = most_all(top);
             }
+        }
+        const double from = top > -INFINITY ? logit64<CAP>(top, a.softcap) : 0.0, k = heat.k * 32.0, cap = a.softcap, twice = CAP ? 64.0 * kLog2E / cap : 0.0;
+        // what `refused` children leave of the weights of a piece
+        auto left = [&](uint32_t piece, const uint4& raw, int refused, double (&w)[E]) {
+            float x[E];
+            Row<T>::numbers(raw, x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = warp_exp2(warp_logit64<CAP>(piece < pieces ? counted(x[e]) : -INFINITY, cap, twice, table) - from, k, table);
             if (refused && o.drawn) {
                 float q[E];
-#pragma unroll
-                for (int e = 0; e < E; ++e) q[e] = piece < pieces && first + e >= 0 && first + e < (int64_t)a.vocab ? prob_at(a, q_row + first + e) : 0.0f;
+                probs_at<E>(a, q_row, piece < pieces ? row.first(piece) : (int64_t)a.vocab, q);
                 for (int g = 0; g < refused; ++g) {
                     const double s = gone.sum[g];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) w[e] = fmax(w[e] - s * (double)q[e], 0.0);
+                    for (int e = 0; e < E; ++e) w[e] = fmax(fma(-s, (double)q[e], w[e]), 0.0);
                 }
             } else {
                 for (int g = 0; g < refused; ++g) {
-                    const int64_t e0 = (int64_t)gone.token[g] - first;
+                    const int64_t e0 = (int64_t)gone.token[g] - row.first(piece);
 #pragma unroll
                     for (int e = 0; e < E; ++e) w[e] = e0 == e ? 0.0 : w[e];
                 }
             }
         };
-        auto sum_left = [&](int refused) {
+        // of `count` steps of this warp from a piece on, the next one's load under way
+        auto sum_steps = [&](uint32_t piece, uint32_t count, int refused) {
             double s = 0.0;
-            for (uint32_t i = 0; i < steps; ++i) {
+            uint4 raw = make_uint4(0, 0, 0, 0), next = raw;
+            if (count && piece < pieces) next = row.load(piece);
+            for (uint32_t i = 0; i < count; ++i, piece += kWarp) {
+                raw = next;
+                if (i + 1 < count && piece + kWarp < pieces) next = row.load(piece + kWarp);
                 double w[E];
-                left(piece0 + i * kWarp, refused, w);
+                left(piece, raw, refused, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) s += w[e];
             }
-            return sum_all(s);
+            return s;
         };
+        auto sum_left = [&](int refused) { return sum_all(sum_steps(piece0, steps, refused)); };
         double z = o.z, s = 0.0;
         int refused = o.what == 2 || o.drawn ? o.refused : 0;      // a test without q goes by Z alone
         bool parts = false;                        // the last sums are those that are drawn from
@@ -567,22 +717,40 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
             before += v;
         }
         if (mine != rank) continue;
-        uint32_t its = 0;
-        double upto = before;
-        bool hit = false;
-        for (int w = 0; w < kWalkWarps; ++w) {     // rounding may leave it behind the last warp that has anything: then its last token
-            if (!(warp_part[w] > 0.0)) continue;
-            its = w;
-            before = upto;
-            upto += warp_part[w];
-            if (upto > target) { hit = true; break; }
-        }
-        if (warp != its) continue;
+        // Of sums in order, the one that the target falls in, and what stands before it. Rounding may leave the target behind the last that has anything: then its last token.
+        auto fall = [&](const double* sums, double& at, bool& hit) {
+            uint32_t its = 0;
+            double upto = at;
+            const double start = at;
+            at = start;
+            hit = false;
+            for (uint32_t w = 0; w < kWalkWarps && !hit; ++w) {
+                if (!(sums[w] > 0.0)) continue;
+                its = w;
+                at = upto;
+                upto += sums[w];
+                hit = upto > target;
+            }
+            return its;
+        };
+        bool hit;
+        const uint32_t its = fall(warp_part, before, hit);
+        // the pieces of that warp, by all of the block
+        const uint32_t fine = (steps + kWalkWarps - 1) / kWalkWarps, piece1 = (rank * kWalkWarps + its) * steps * kWarp + lane;
+        const uint32_t mine0 = min(warp * fine, steps), mine1 = min(mine0 + fine, steps);
+        double part = sum_steps(piece1 + mine0 * kWarp, mine1 - mine0, refused);
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) part += __shfl_xor_sync(kFullMask, part, off);
+        __syncthreads();                           // the sums of warps have been read
+        if (lane == 0) warp_part[warp] = part;
+        __syncthreads();
+        if (warp != fall(warp_part, before, hit)) continue;
         double sum = before;
         int64_t token_at = -1, last = -1;
-        for (uint32_t i = 0; i < steps; ++i) {
+        for (uint32_t i = mine0; i < mine1; ++i) {
             double w[E], all = 0.0;
-            left(piece0 + i * kWarp, refused, w);
+            const uint32_t piece = piece1 + i * kWarp;
+            left(piece, piece < pieces ? row.load(piece) : make_uint4(0, 0, 0, 0), refused, w);
 #pragma unroll
             for (int e = 0; e < E; ++e) all += w[e];
             double run = all;
@@ -596,7 +764,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
             if (who >= 0) {
                 int64_t found = -1, end = -1;
                 double at = sum + run - all;
-                const int64_t first = row.first(piece0 + i * kWarp);
+                const int64_t first = row.first(piece);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     at += w[e];
@@ -637,16 +805,24 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
 }
 
 template <typename T, bool CAP>
-tf_status launch_verify(tf_context* ctx, cudaStream_t st, const VerifyArgs& a) {
+tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a) {
     const char* name = "tf_verify_drafts";
+    constexpr uint32_t E = Row<T>::E;
     if (a.rows) {
-        verify_stats_kernel<T, CAP><<<a.rows * a.chunks, kStatsThreads, 0, st>>>(a);
+        const bool even = aligned(a.logits, 16) && a.stride % E == 0;          // else a row may begin anywhere in a piece
+        a.chunks = (uint32_t)(((uint64_t)a.vocab + (even ? 0 : E - 1) + kChunk - 1) / kChunk);
+        // several chunks a block, as long as that leaves every place on the chip a few blocks
+        const uint64_t all = (uint64_t)a.rows * a.chunks / ((uint64_t)ctx->sm_count * 16);
+        a.per = (uint32_t)(all < 1 ? 1 : all > 4 ? 4 : all);
+        a.parts = (a.chunks + a.per - 1) / a.per;
+        verify_stats_kernel<T, CAP><<<a.rows * a.parts, kStatsThreads, 0, st>>>(a);
         const tf_status s = check_launch(ctx, name);
         if (s != TF_OK) return s;
     }
-    constexpr uint32_t kRanks = 8;
+    uint32_t ranks = 8;
+    while (ranks > 1 && (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2) ranks /= 2;
     const size_t smem = (size_t)a.draft_stride * 36;
-    TF_CUDA(ctx, launch_pdl_cluster(verify_walk_kernel<T, CAP>, dim3(a.sequences * kRanks), dim3(kWalkThreads), smem, st, kRanks, a));
+    TF_CUDA(ctx, launch_pdl_cluster(verify_walk_kernel<T, CAP>, dim3(a.sequences * ranks), dim3(kWalkThreads), smem, st, ranks, a));
     return check_launch(ctx, name);
 }
 
@@ -725,7 +901,7 @@ tf_status tf_verify_drafts(tf_context* ctx, void* stream, const void* logits, ui
     a.out_tokens = out_tokens; a.out_rows = out_rows; a.kept = kept; a.logprobs = logprobs;
     a.stats = static_cast<tf::ChunkStat*>(ws->memory);
     a.error = ctx->device_error;
-    a.vocab = vocab; a.rows = rows; a.sequences = sequences; a.draft_stride = drafts->stride; a.chunks = (uint32_t)chunks;
+    a.vocab = vocab; a.rows = rows; a.sequences = sequences; a.draft_stride = drafts->stride;
     a.softcap = softcap;
     const tf::DeviceScope scope(ctx->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
