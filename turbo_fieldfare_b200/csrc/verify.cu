@@ -29,7 +29,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kStatsThreads = 256, kChunk = 8192;          // elements that a block of the first launch takes at a time
-constexpr int kWalkThreads = 256, kWalkWarps = kWalkThreads / kWarp;
+constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / kWarp;
 constexpr uint32_t kMostNodes = 1024;
 constexpr double kLog2E = 1.4426950408889634074;
 
@@ -350,7 +350,7 @@ __device__ __forceinline__ double warp_logit64(float x, double cap, double twice
 
 // What the cluster does next, and with which row.
 struct Order {
-    int what;                  // 0: nothing more; 1: sums; 2: sums and a draw
+    int what;                  // 0: nothing more; 1: sums; 2: sums and a draw, which is the last thing
     uint32_t node, at;         // at: where the token goes
     int known, summed, step, drawn, refused;   // its maximum is known; so is Z; the last refusal's sum is not noted yet; q counts; children refused
     float most, u;
@@ -359,9 +359,38 @@ struct Order {
 
 struct Walk {
     uint32_t i, node, at;
-    int refused, done, summed, step;
+    int known, refused, summed, step;
     double z, s, gone;         // gone: weight of the refused tokens, without q
 };
+
+// The first block's shared memory: what it knows of the nodes. 48 bytes of each.
+struct NodeTable {
+    double *z, *weight;        // of a row: its sum in 32 bits; of a token: its weight in its parent's row
+    double* gone;              // of the current node's refused children: S before each, or (as int32) the tokens
+    float *most, *prob;
+    uint32_t* best;
+    int32_t *parent, *token, *inner;       // inner: has children; -1 - place of a kept node
+    __device__ __forceinline__ NodeTable(uint8_t* memory, uint32_t n) {
+        z = reinterpret_cast<double*>(memory);
+        weight = z + n;
+        gone = weight + n;
+        most = reinterpret_cast<float*>(gone + n);
+        prob = most + n;
+        best = reinterpret_cast<uint32_t*>(prob + n);
+        parent = reinterpret_cast<int32_t*>(best + n);
+        token = parent + n;
+        inner = token + n;
+    }
+    static constexpr size_t kBytes = 48;
+};
+
+__device__ const double kPowers[32] = {               // 2^(j / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
+    1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
+    1.9152065613971474, 1.9571441241754002};
 
 __device__ __forceinline__ float prob_at(const VerifyArgs& a, uint64_t at) {
     float q;
@@ -401,398 +430,402 @@ __device__ __forceinline__ void probs_at(const VerifyArgs& a, uint64_t row, int6
     for (int e = 0; e < E; ++e) q[e] = first + e >= 0 && first + e < (int64_t)a.vocab ? prob_at(a, row + first + e) : 0.0f;
 }
 
+// Inclusive sums over a warp's lanes.
+__device__ __forceinline__ double warp_scan(double v, uint32_t lane) {
+#pragma unroll
+    for (int off = 1; off < kWarp; off <<= 1) {
+        const double o = __shfl_up_sync(kFullMask, v, off);
+        if (lane >= off) v += o;
+    }
+    return v;
+}
+
+// Among parts in the lanes' order, whose sums `upto` are, the one that the target falls in; rounding may leave it behind the last that has anything, which is then it.
+// The target becomes that within the part.
+__device__ __forceinline__ uint32_t warp_fall(double part, double upto, double& target) {
+    const uint32_t any = __ballot_sync(kFullMask, part > 0.0), over = __ballot_sync(kFullMask, part > 0.0 && upto > target);
+    const uint32_t who = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : 0;
+    const double before = __shfl_sync(kFullMask, upto - part, who);
+    target = over ? target - before : INFINITY;
+    return who;
+}
+
+// One thread goes from node to node until a sum over the vocabulary is needed, or the walk is over.
+template <bool CAP>
+__device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, const Heat& heat, uint32_t b, const NodeTable& t, Walk& w, Order& order,
+                                        int32_t* out_tokens, int32_t* out_rows) {
+    const double bound = sum_bound(a.softcap, heat.k);
+    const float* uniforms = a.uniforms + (size_t)b * a.draft_stride;
+    const int32_t* gone_tokens = reinterpret_cast<const int32_t*>(t.gone);
+    order.what = 0;
+    if (of.n == 0) return;
+    for (; w.i < of.n; ++w.i) {
+        const uint32_t i = w.i;
+        if (t.parent[i] != (int32_t)w.node || t.token[i] < 0) continue;
+        const bool drawn = a.probs && w.node < a.probs_nodes;
+        bool keep;
+        if (heat.greedy) {
+            keep = t.most[w.node] > -INFINITY && (uint32_t)t.token[i] == t.best[w.node];
+        } else {
+            const double u = (double)fminf(fmaxf(uniforms[i], 0.0f), 0x1.fffffep-1f), weight = t.weight[i];
+            bool ask = false;
+            double left, right = weight;
+            if (drawn) {
+                const double q = (double)t.prob[i];
+                if (w.step) ask = true;                // the last refusal's sum first
+                left = u * q * (w.refused ? w.s : w.z);
+                for (int g = 0; g < w.refused && !w.step; ++g) right = fmax(fma(-t.gone[g], q, right), 0.0);
+                if (!w.refused && !w.summed) ask = fabs(left - right) < bound * left;
+            } else {
+                bool before = false;
+                for (int g = 0; g < w.refused; ++g) before |= gone_tokens[g] == t.token[i];
+                if (before) continue;                  // refused already
+                left = u * (w.z - w.gone);
+                if (!w.summed) ask = fabs(left - right) < bound * u * w.z;
+            }
+            if (ask) {
+                order = {1, w.node, 0, 1, w.summed, w.step, drawn, w.refused, t.most[w.node], 0.0f, w.z, w.s};
+                return;
+            }
+            keep = left < right;
+        }
+        if (keep) {
+            out_rows[w.at + 1] = (int32_t)i;
+            out_tokens[w.at] = t.token[i];
+            w.known = t.inner[i];
+            t.inner[i] = -1 - (int32_t)w.at;
+            w.at += 1;
+            w.node = i;
+            const double z = w.z;
+            w.z = t.z[i];
+            t.z[i] = z;                                // now what the kept token's weight is a part of
+            w.refused = w.summed = w.step = 0;
+            w.gone = 0.0;
+        } else if (!heat.greedy) {
+            if (drawn) {
+                w.step = 1;
+            } else {
+                reinterpret_cast<int32_t*>(t.gone)[w.refused] = t.token[i];
+                w.gone += t.weight[i];
+            }
+            w.refused += 1;
+        }
+    }
+    if (heat.greedy) {
+        out_tokens[w.at] = (int32_t)t.best[w.node];
+        if (a.logprobs) a.logprobs[(size_t)b * a.draft_stride + w.at] = w.z > 0.0 ? (float)-log(w.z) : -INFINITY;
+        return;
+    }
+    const float u = fminf(fmaxf(uniforms[0], 0.0f), 0x1.fffffep-1f);
+    order = {2, w.node, w.at, w.known, w.summed, w.step, a.probs && w.node < a.probs_nodes, w.refused, t.most[w.node], u, w.z, w.s};
+}
+
 template <typename T, bool CAP>
-__global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
-    constexpr int E = Row<T>::E;
+__global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
+    using R = Row<T>;
+    constexpr int E = R::E;
     extern __shared__ __align__(16) uint8_t dynamic[];
     __shared__ Order orders[2];                    // by turns: one is read while the next is written
     __shared__ Walk walk;
     __shared__ double block_sum[2], warp_part[kWalkWarps];
     __shared__ float block_most[2], warp_most[kWalkWarps];
-    __shared__ union { double sum[kMostNodes]; int32_t token[kMostNodes]; } gone;      // of the node's refused children: S before each, or the tokens
+    __shared__ uint32_t likeliest;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const uint32_t rank = cluster.block_rank(), ranks = cluster.num_blocks(), b = blockIdx.x / ranks;
+    const double table = kPowers[lane];
     pdl_wait();
     const Nodes of(a, b, rank == 0 && tid == 0);
     const Heat heat(a, b);
-    // of the first block: the nodes
-    double* z32 = reinterpret_cast<double*>(dynamic);
-    float *most = reinterpret_cast<float*>(z32 + a.draft_stride), *logit = most + a.draft_stride, *prob = logit + a.draft_stride;
-    uint32_t* best = reinterpret_cast<uint32_t*>(prob + a.draft_stride);
-    int32_t *parent = reinterpret_cast<int32_t*>(best + a.draft_stride), *token = parent + a.draft_stride, *inner = token + a.draft_stride;
+    const NodeTable nodes(dynamic, a.draft_stride);
+    int32_t* gone_tokens = reinterpret_cast<int32_t*>(nodes.gone);
+    int32_t* out_tokens = a.out_tokens + (size_t)b * a.draft_stride;
+    int32_t* out_rows = a.out_rows + (size_t)b * a.draft_stride;
+    float* logprobs = a.logprobs ? a.logprobs + (size_t)b * a.draft_stride : nullptr;
+    const double k = heat.k * 32.0, cap = a.softcap, twice = CAP ? 64.0 * kLog2E / cap : 0.0;
+    constexpr double kLn2 = 0.69314718055994530942;
+    // A lone row is drawn from at once by all blocks, whatever there is to know of it.
+    const bool alone = of.n == 1 && (a.draft_stride == 1 || !heat.greedy);
+    if (tid == 0) {
+        walk = {1, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0};
+        likeliest = 0xFFFFFFFFu;
+    }
 
-    if (rank == 0) {
+    if (rank == 0 && !alone) {
         for (uint32_t i = tid; i < of.n; i += kWalkThreads) {
-            parent[i] = i ? parent_of(a, b, i) : -1;
-            token[i] = a.tokens[(size_t)b * a.draft_stride + i];
-            inner[i] = 0;
+            const int32_t x = a.tokens[(size_t)b * a.draft_stride + i];
+            nodes.parent[i] = i ? parent_of(a, b, i) : -1;
+            nodes.token[i] = x >= 0 && (uint32_t)x < a.vocab ? x : -1;
+            nodes.inner[i] = 0;
+            nodes.most[i] = -INFINITY;
         }
         __syncthreads();
         for (uint32_t i = tid; i < of.n; i += kWalkThreads) {
-            if (parent[i] < 0) continue;
-            inner[parent[i]] = 1;
-            if (token[i] < 0 || (uint32_t)token[i] >= a.vocab) continue;
-            logit[i] = counted(number(static_cast<const T*>(a.logits)[(of.row0 + (uint64_t)parent[i]) * a.stride + token[i]]));
-            prob[i] = a.probs && (uint32_t)parent[i] < a.probs_nodes ? prob_at(a, b * a.probs_sequence + parent[i] * a.probs_node + token[i]) : 0.0f;
+            const int32_t p = nodes.parent[i], x = nodes.token[i];
+            if (p < 0) continue;
+            nodes.inner[p] = 1;
+            if (x < 0) continue;
+            nodes.weight[i] = (double)counted(number(static_cast<const T*>(a.logits)[(of.row0 + (uint64_t)p) * a.stride + x]));     // for now
+            nodes.prob[i] = a.probs && (uint32_t)p < a.probs_nodes ? prob_at(a, b * a.probs_sequence + p * a.probs_node + x) : 0.0f;
         }
         __syncthreads();
         for (uint32_t i = warp; i < of.n; i += kWalkWarps) {
-            if (!inner[i] && !heat.greedy) {
-                if (lane == 0) most[i] = -INFINITY;
-                continue;
-            }
+            if (!nodes.inner[i] && !heat.greedy) continue;
             const ChunkStat* s = a.stats + (size_t)(of.row0 + i) * a.parts;
             float top = -INFINITY;
             uint32_t at = 0xFFFFFFFFu;
             for (uint32_t c = lane; c < a.parts; c += kWarp) {
                 const ChunkStat x = s[c];
-                if (x.most > top) { top = x.most; at = x.at; }                 // chunks ascend: the first of equals stays
+                if (x.most > top) { top = x.most; at = x.at; }                 // parts ascend: the first of equals stays
             }
             float all = top;
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) all = fmaxf(all, __shfl_xor_sync(kFullMask, all, off));
             if (top != all) at = 0xFFFFFFFFu;
             at = __reduce_min_sync(kFullMask, at);
-            const float from = CAP ? capped(all, a.softcap) : all, k = heat.k32();
+            const float from = CAP ? capped(all, a.softcap) : all, k32 = heat.k32();
             double sum = 0.0;
             for (uint32_t c = lane; c < a.parts; c += kWarp) {
                 const ChunkStat x = s[c];
-                if (x.most > -INFINITY) sum += (double)(x.sum * verify_exp2(((CAP ? capped(x.most, a.softcap) : x.most) - from) * k));
+                if (x.most > -INFINITY) sum += (double)(x.sum * verify_exp2(((CAP ? capped(x.most, a.softcap) : x.most) - from) * k32));
             }
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
             if (lane == 0) {
-                most[i] = all;
-                z32[i] = sum;
-                best[i] = at == 0xFFFFFFFFu ? 0u : at;
+                nodes.most[i] = all;
+                nodes.z[i] = sum;
+                nodes.best[i] = at == 0xFFFFFFFFu ? 0u : at;
             }
         }
-        if (tid == 0) walk = {1, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0};
         __syncthreads();
-        if (tid == 0 && of.n) walk.z = z32[0];
+        for (uint32_t i0 = warp * kWarp; i0 < of.n; i0 += kWalkThreads) {
+            const uint32_t i = i0 + lane;
+            const bool is = i < of.n && nodes.parent[i] >= 0 && nodes.token[i] >= 0;
+            const float x = is ? (float)nodes.weight[i] : -INFINITY, top = is ? nodes.most[nodes.parent[i]] : -INFINITY;
+            const double l = warp_logit64<CAP>(x, cap, twice, table), from = warp_logit64<CAP>(top, cap, twice, table);
+            const double w = warp_exp2(top > -INFINITY ? l - from : -INFINITY, k, table);
+            if (is) nodes.weight[i] = w;
+        }
+        __syncthreads();
+        if (tid == 0 && of.n) {
+            walk.z = nodes.z[0];
+            walk.known = nodes.inner[0];
+        }
     }
+    __syncthreads();
 
-    int32_t* out_tokens = a.out_tokens + (size_t)b * a.draft_stride;
-    int32_t* out_rows = a.out_rows + (size_t)b * a.draft_stride;
-    float* logprobs = a.logprobs ? a.logprobs + (size_t)b * a.draft_stride : nullptr;
-    // w of one logit; log(w) stays finite where w is 0
-    auto power = [&](float x, float top) { return (logit64<CAP>(x, a.softcap) - logit64<CAP>(top, a.softcap)) * heat.k; };
-    constexpr double kLn2 = 0.69314718055994530942;
-
-    // One thread goes from node to node until a sum over the vocabulary is needed; false: the walk is over.
-    auto advance = [&](Order& order) {
-        Walk& w = walk;
-        const double bound = sum_bound(a.softcap, heat.k);
-        order.what = 0;
-        if (of.n == 0) return;
-        for (; w.i < of.n; ++w.i) {
-            const uint32_t i = w.i;
-            if (parent[i] != (int32_t)w.node || token[i] < 0 || (uint32_t)token[i] >= a.vocab) continue;
-            bool keep;
-            double weight = 0.0, x2 = 0.0;
-            const bool drawn = a.probs && w.node < a.probs_nodes;
-            if (most[w.node] > -INFINITY && logit[i] > -INFINITY) {
-                x2 = power(logit[i], most[w.node]);
-                weight = exp2(x2);
-            }
-            if (heat.greedy) {
-                keep = most[w.node] > -INFINITY && (uint32_t)token[i] == best[w.node];
-            } else {
-                const double u = (double)fminf(fmaxf(a.uniforms[(size_t)b * a.draft_stride + i], 0.0f), 0x1.fffffep-1f);
-                bool ask = false;
-                double left, right = weight;
-                if (drawn) {
-                    const double q = (double)prob[i];
-                    if (w.step) ask = true;            // the last refusal's sum first
-                    left = u * q * (w.refused ? w.s : w.z);
-                    for (int g = 0; g < w.refused && !w.step; ++g) right = fmax(right - gone.sum[g] * q, 0.0);
-                    if (!w.refused && !w.summed) ask = fabs(left - right) < bound * left;
-                } else {
-                    bool before = false;
-                    for (int g = 0; g < w.refused; ++g) before |= gone.token[g] == token[i];
-                    if (before) continue;              // refused already
-                    left = u * (w.z - w.gone);
-                    if (!w.summed) ask = fabs(left - right) < bound * u * w.z;
-                }
-                if (ask) {
-                    order = {1, w.node, 0, 1, w.summed, w.step, drawn, w.refused, most[w.node], 0.0f, w.z, w.s};
-                    return;
-                }
-                keep = left < right;
-            }
-            if (keep) {
-                out_rows[w.at + 1] = (int32_t)i;
-                out_tokens[w.at] = token[i];
-                if (logprobs) logprobs[w.at] = (float)(x2 * kLn2 - log(w.z));
-                w.at += 1;
-                w.node = i;
-                w.refused = w.summed = w.step = 0;
-                w.z = z32[i];
-                w.gone = 0.0;
-            } else if (!heat.greedy) {
-                if (drawn) {
-                    w.step = 1;
-                } else {
-                    gone.token[w.refused] = token[i];
-                    w.gone += weight;
-                }
-                w.refused += 1;
-            }
+    for (uint32_t round = 0, turn = 0;; ++round) {
+        Order o = {2, 0, 0, 0, 0, 0, 0, 0, 0.0f, 0.0f, 0.0, 0.0};
+        if (alone) {
+            o.u = fminf(fmaxf(a.uniforms[(size_t)b * a.draft_stride], 0.0f), 0x1.fffffep-1f);
+        } else {
+            if (rank == 0 && tid == 0) walk_on<CAP>(a, of, heat, b, nodes, walk, orders[round & 1], out_tokens, out_rows);
+            __syncwarp();
+            cluster.sync();
+            o = *cluster.map_shared_rank(&orders[round & 1], 0);
         }
-        if (w.done) return;
-        w.done = 1;
-        if (heat.greedy) {
-            out_tokens[w.at] = (int32_t)best[w.node];
-            if (logprobs) logprobs[w.at] = w.z > 0.0 ? (float)-log(w.z) : -INFINITY;
-            return;
-        }
-        const float u = fminf(fmaxf(a.uniforms[(size_t)b * a.draft_stride], 0.0f), 0x1.fffffep-1f);
-        order = {2, w.node, w.at, inner[w.node], w.summed, w.step, a.probs && w.node < a.probs_nodes, w.refused, most[w.node], u, w.z, w.s};
-    };
-
-    const double table = exp2((double)lane / 32.0);
-    uint32_t turn = 0;
-    // Sums and maxima over the cluster, in the order of warps and blocks; the last sums of warps and blocks stay for the draw.
-    double block_part = 0.0;                       // lane r: block r's last sum
-    auto sum_all = [&](double v) {
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(kFullMask, v, off);
-        __syncthreads();
-        if (lane == 0) warp_part[warp] = v;
-        __syncthreads();
-        if (tid == 0) {
-            double s = 0.0;
-            for (int w = 0; w < kWalkWarps; ++w) s += warp_part[w];
-            block_sum[turn & 1] = s;
-        }
-        __syncwarp();
-        cluster.sync();
-        block_part = lane < ranks ? *cluster.map_shared_rank(&block_sum[turn & 1], lane) : 0.0;
-        ++turn;
-        double s = 0.0;
-        for (uint32_t r = 0; r < ranks; ++r) s += __shfl_sync(kFullMask, block_part, r);
-        return s;
-    };
-    auto most_all = [&](float v) {
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, off));
-        __syncthreads();
-        if (lane == 0) warp_most[warp] = v;
-        __syncthreads();
-        if (tid == 0) {
-            for (int w = 0; w < kWalkWarps; ++w) v = fmaxf(v, warp_most[w]);
-            block_most[turn & 1] = v;
-        }
-        __syncwarp();
-        cluster.sync();
-        v = lane < ranks ? *cluster.map_shared_rank(&block_most[turn & 1], lane) : -INFINITY;
-        ++turn;
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, off));
-        return v;
-    };
-
-    for (uint32_t round = 0;; ++round) {
-        if (rank == 0 && tid == 0) advance(orders[round & 1]);
-        __syncwarp();
-        cluster.sync();
-        const Order o = *cluster.map_shared_rank(&orders[round & 1], 0);
         if (o.what == 0) break;
         if (rank != 0) {
             for (int g = tid; g < o.refused; g += kWalkThreads)
-                if (!o.drawn) gone.token[g] = *cluster.map_shared_rank(&gone.token[g], 0);
-                else if (!o.step || g + 1 < o.refused) gone.sum[g] = *cluster.map_shared_rank(&gone.sum[g], 0);
+                if (!o.drawn) gone_tokens[g] = *cluster.map_shared_rank(&gone_tokens[g], 0);
+                else if (!o.step || g + 1 < o.refused) nodes.gone[g] = *cluster.map_shared_rank(&nodes.gone[g], 0);
+            __syncthreads();
         }
-        __syncthreads();
 
-        // ---- this warp's pieces of the row: neighbours, so that sums run in the order of the tokens ----
-        const Row<T> row(a.logits, (of.row0 + (uint64_t)o.node) * a.stride, a.vocab);
+        // ---- the pieces: a warp's are neighbours, and a block's warps, so that sums run in the order of the tokens ----
+        const R row(a.logits, (of.row0 + (uint64_t)o.node) * a.stride, a.vocab);
         const uint32_t pieces = row.pieces(), steps = (pieces + ranks * kWalkThreads - 1) / (ranks * kWalkThreads);
-        const uint32_t piece0 = (rank * kWalkWarps + warp) * steps * kWarp + lane;
         const uint64_t q_row = b * a.probs_sequence + o.node * a.probs_node;
+        uint32_t begin = rank * kWalkWarps * steps * kWarp, count = kWalkWarps * steps, sub = steps;       // first piece, steps of a warp's width, steps a warp
+        // A row without a maximum (a leaf: nothing was refused) is summed by every block relative to its own, one meeting less.
         float top = o.most;
         if (!o.known) {
             top = -INFINITY;
-            for (uint32_t i = 0; i < steps; i += 4) {
+            for (uint32_t i = 0, piece = begin + warp * steps * kWarp + lane; i < steps && piece < pieces; i += 4, piece += 4 * kWarp) {
                 uint4 w[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (i + j < steps && piece0 + (i + j) * kWarp < pieces) w[j] = row.load(piece0 + (i + j) * kWarp);
+                    if (i + j < steps && piece + j * kWarp < pieces) w[j] = row.load(piece + j * kWarp);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (i + j < steps && piece0 + (i + j) * kWarp < pieces) top = fmaxf(top, Row<T>::most(w[j]));
+                    if (i + j < steps && piece + j * kWarp < pieces) {
+                        float most = R::most(w[j]);
+                        if (most == INFINITY) {            // does not count
+                            float x[E];
+                            R::numbers(w[j], x);
+                            most = -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < E; ++e) most = fmaxf(most, counted(x[e]));
+                        }
+                        top = fmaxf(top, most);
+                    }
             }
-            top = most_all(top);
-            if (top == INFINITY) {                 // does not count: once more, one by one
-                top = -INFINITY;
-                for (uint32_t i = 0; i < steps; ++i) {
-                    if (piece0 + i * kWarp >= pieces) break;
-                    float x[E];
-                    Row<T>::numbers(row.load(piece0 + i * kWarp), x);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) top = fmaxf(top, counted(x[e]));
-                }
-                top = most_all(top);
-            }
-        }
-        const double from = top > -INFINITY ? logit64<CAP>(top, a.softcap) : 0.0, k = heat.k * 32.0, cap = a.softcap, twice = CAP ? 64.0 * kLog2E / cap : 0.0;
-        // what `refused` children leave of the weights of a piece
-        auto left = [&](uint32_t piece, const uint4& raw, int refused, double (&w)[E]) {
-            float x[E];
-            Row<T>::numbers(raw, x);
-#pragma unroll
-            for (int e = 0; e < E; ++e) w[e] = warp_exp2(warp_logit64<CAP>(piece < pieces ? counted(x[e]) : -INFINITY, cap, twice, table) - from, k, table);
-            if (refused && o.drawn) {
-                float q[E];
-                probs_at<E>(a, q_row, piece < pieces ? row.first(piece) : (int64_t)a.vocab, q);
-                for (int g = 0; g < refused; ++g) {
-                    const double s = gone.sum[g];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) w[e] = fmax(fma(-s, (double)q[e], w[e]), 0.0);
-                }
-            } else {
-                for (int g = 0; g < refused; ++g) {
-                    const int64_t e0 = (int64_t)gone.token[g] - row.first(piece);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) w[e] = e0 == e ? 0.0 : w[e];
-                }
-            }
-        };
-        // of `count` steps of this warp from a piece on, the next one's load under way
-        auto sum_steps = [&](uint32_t piece, uint32_t count, int refused) {
-            double s = 0.0;
-            uint4 raw = make_uint4(0, 0, 0, 0), next = raw;
-            if (count && piece < pieces) next = row.load(piece);
-            for (uint32_t i = 0; i < count; ++i, piece += kWarp) {
-                raw = next;
-                if (i + 1 < count && piece + kWarp < pieces) next = row.load(piece + kWarp);
-                double w[E];
-                left(piece, raw, refused, w);
-#pragma unroll
-                for (int e = 0; e < E; ++e) s += w[e];
-            }
-            return s;
-        };
-        auto sum_left = [&](int refused) { return sum_all(sum_steps(piece0, steps, refused)); };
-        double z = o.z, s = 0.0;
-        int refused = o.what == 2 || o.drawn ? o.refused : 0;      // a test without q goes by Z alone
-        bool parts = false;                        // the last sums are those that are drawn from
-        if (!o.summed) {
-            s = z = sum_left(0);
-            parts = refused == 0;
-        }
-        if (refused) {
-            if (o.step && tid == 0) gone.sum[refused - 1] = refused == 1 ? z : o.s;
+            for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+            if (lane == 0) warp_most[warp] = top;
             __syncthreads();
-            s = sum_left(refused);
-            parts = o.what == 1 || s > 0.0;
-            if (!parts) refused = 0;               // nothing left: from all of it
+            top = lane < kWalkWarps ? warp_most[lane] : -INFINITY;
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
         }
-        if (o.what == 1) {
-            if (rank == 0 && tid == 0) {
-                walk.z = z;
-                walk.s = s;
-                walk.summed = 1;
-                walk.step = 0;
-            }
-            continue;                              // the thread that walks is the one that wrote
-        }
-        if (!parts) s = sum_left(0);
+        const double from = top > -INFINITY ? warp_logit64<CAP>(top, cap, twice, table) : 0.0;
 
-        // ---- the draw: block, warp, piece, token ----
-        const double target = (double)o.u * s;
-        if (!(s > 0.0)) {
-            if (rank == 0 && tid == 0) {
-                out_tokens[o.at] = 0;
-                if (logprobs) logprobs[o.at] = -INFINITY;
+        // ---- sums, and the draw from block to warp to step to token, with one body for all of it: what runs once costs what its instructions take to fetch ----
+        enum { kAll, kLeft, kAgain, kWithin, kStep };
+        int stage = !o.summed ? kAll : o.refused && (o.drawn || o.what == 2) ? kLeft : kAgain;
+        double z = o.z, target = 0.0, whole = from;    // whole: the logit that z is relative to
+        int refused = 0;
+        for (;;) {
+            if (stage == kLeft) {
+                refused = o.refused;
+                if (o.drawn && o.step) {
+                    if (tid == 0) nodes.gone[refused - 1] = refused == 1 ? z : o.s;
+                    __syncthreads();
+                }
+            } else if (stage == kAgain) {
+                refused = 0;
             }
-            continue;
-        }
-        double before = 0.0;
-        uint32_t mine = ranks;                     // the block that the target falls in
-        for (uint32_t r = 0; r < ranks; ++r) {
-            const double v = __shfl_sync(kFullMask, block_part, r);
-            if (before + v > target) { mine = r; break; }
-            before += v;
-        }
-        if (mine != rank) continue;
-        // Of sums in order, the one that the target falls in, and what stands before it. Rounding may leave the target behind the last that has anything: then its last token.
-        auto fall = [&](const double* sums, double& at, bool& hit) {
-            uint32_t its = 0;
-            double upto = at;
-            const double start = at;
-            at = start;
-            hit = false;
-            for (uint32_t w = 0; w < kWalkWarps && !hit; ++w) {
-                if (!(sums[w] > 0.0)) continue;
-                its = w;
-                at = upto;
-                upto += sums[w];
-                hit = upto > target;
-            }
-            return its;
-        };
-        bool hit;
-        const uint32_t its = fall(warp_part, before, hit);
-        // the pieces of that warp, by all of the block
-        const uint32_t fine = (steps + kWalkWarps - 1) / kWalkWarps, piece1 = (rank * kWalkWarps + its) * steps * kWarp + lane;
-        const uint32_t mine0 = min(warp * fine, steps), mine1 = min(mine0 + fine, steps);
-        double part = sum_steps(piece1 + mine0 * kWarp, mine1 - mine0, refused);
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) part += __shfl_xor_sync(kFullMask, part, off);
-        __syncthreads();                           // the sums of warps have been read
-        if (lane == 0) warp_part[warp] = part;
-        __syncthreads();
-        if (warp != fall(warp_part, before, hit)) continue;
-        double sum = before;
-        int64_t token_at = -1, last = -1;
-        for (uint32_t i = mine0; i < mine1; ++i) {
+            // what `refused` children leave of the weights of this warp's steps; in a single step every warp has all of it
+            const uint32_t first = stage == kStep ? 0u : min(warp * sub, count), last = stage == kStep ? 1u : min(first + sub, count);
             double w[E], all = 0.0;
-            const uint32_t piece = piece1 + i * kWarp;
-            left(piece, piece < pieces ? row.load(piece) : make_uint4(0, 0, 0, 0), refused, w);
+            uint32_t piece = begin + first * kWarp + lane;
+            uint4 next = make_uint4(0, 0, 0, 0);
+            if (first < last && piece < pieces) next = row.load(piece);
+            for (uint32_t i = first; i < last; ++i, piece += kWarp) {
+                float x[E];
+                R::numbers(next, x);
+                if (i + 1 < last && piece + kWarp < pieces) next = row.load(piece + kWarp);
+                float q[E];
+                if (refused && o.drawn) probs_at<E>(a, q_row, piece < pieces ? row.first(piece) : (int64_t)a.vocab, q);
 #pragma unroll
-            for (int e = 0; e < E; ++e) all += w[e];
-            double run = all;
+                for (int e = 0; e < E; ++e)
+                    w[e] = warp_exp2(warp_logit64<CAP>(piece < pieces ? counted(x[e]) : -INFINITY, cap, twice, table) - from, k, table);
+                for (int g = 0; g < refused; ++g) {
+                    if (o.drawn) {
+                        const double s = nodes.gone[g];
 #pragma unroll
-            for (int off = 1; off < kWarp; off <<= 1) {
-                const double v = __shfl_up_sync(kFullMask, run, off);
-                if (lane >= off) run += v;
-            }
-            const uint32_t over = __ballot_sync(kFullMask, all > 0.0 && sum + run > target), any = __ballot_sync(kFullMask, all > 0.0);
-            const int who = hit && over ? __ffs(over) - 1 : any ? 31 - __clz(any) : -1;
-            if (who >= 0) {
-                int64_t found = -1, end = -1;
-                double at = sum + run - all;
-                const int64_t first = row.first(piece);
+                        for (int e = 0; e < E; ++e) w[e] = fmax(fma(-s, (double)q[e], w[e]), 0.0);
+                    } else {
+                        const int64_t e0 = (int64_t)gone_tokens[g] - row.first(piece);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    at += w[e];
-                    if (w[e] > 0.0) {
-                        end = first + e;
-                        if (found < 0 && at > target) found = first + e;
+                        for (int e = 0; e < E; ++e) w[e] = e0 == e ? 0.0 : w[e];
                     }
                 }
-                found = hit && over ? (found < 0 ? end : found) : -1;
-                last = __shfl_sync(kFullMask, end, who);
-                token_at = __shfl_sync(kFullMask, found, who);
-                if (token_at >= 0) break;
+#pragma unroll
+                for (int e = 0; e < E; ++e) all += w[e];
             }
-            sum += __shfl_sync(kFullMask, run, kWarp - 1);
-        }
-        if (token_at < 0) token_at = last;
-        if (lane == 0) {
-            out_tokens[o.at] = (int32_t)token_at;
-            if (logprobs) {
-                const float x = counted(number(row.p[token_at]));
-                logprobs[o.at] = (float)((logit64<CAP>(x, a.softcap) - from) * heat.k * kLn2 - log(z));
+            if (stage == kStep) {
+                const double upto = warp_scan(all, lane);
+                if (warp_fall(all, upto, target) == lane && warp == 0) {
+                    double at = 0.0;
+                    int found = -1, end = 0;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        at += w[e];
+                        if (w[e] > 0.0) {
+                            end = e;
+                            if (found < 0 && at > target) found = e;
+                        }
+                    }
+                    found = found < 0 ? end : found;
+                    out_tokens[o.at] = (int32_t)(row.first(begin + lane) + found);
+                    if (logprobs) {
+                        const float x = number(row.p[row.first(begin + lane) + found]);
+                        logprobs[o.at] = (float)((logit64<CAP>(x, a.softcap) - whole) * heat.k * kLn2 - log(z));
+                    }
+                }
+                break;
             }
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) all += __shfl_xor_sync(kFullMask, all, off);
+            __syncthreads();                           // the sums before these have been read
+            if (lane == 0) warp_part[warp] = all;
+            __syncthreads();
+            const double part = lane < kWalkWarps ? warp_part[lane] : 0.0, upto = warp_scan(part, lane);
+            if (stage != kWithin) {
+                // ---- over the cluster ----
+                if (tid == kWarp - 1) {
+                    block_sum[turn & 1] = upto;
+                    block_most[turn & 1] = top;
+                }
+                __syncwarp();
+                cluster.sync();
+                double mine = lane < ranks ? *cluster.map_shared_rank(&block_sum[turn & 1], lane) : 0.0, scale = 1.0;
+                if (!o.known) {
+                    const float its = lane < ranks ? *cluster.map_shared_rank(&block_most[turn & 1], lane) : -INFINITY;
+                    float most = its;
+#pragma unroll
+                    for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, off));
+                    whole = warp_logit64<CAP>(most, cap, twice, table);
+                    scale = warp_exp2(most > -INFINITY ? warp_logit64<CAP>(its, cap, twice, table) - whole : -INFINITY, k, table);
+                    mine *= scale;
+                    if (heat.greedy) {                 // alone: the likeliest token instead of a draw
+                        if (top == most && top > -INFINITY) {
+                            for (uint32_t i = 0, p = begin + warp * steps * kWarp + lane; i < steps && p < pieces; ++i, p += kWarp) {
+                                float x[E];
+                                R::numbers(row.load(p), x);
+#pragma unroll
+                                for (int e = E - 1; e >= 0; --e)
+                                    if (x[e] == top) atomicMin(cluster.map_shared_rank(&likeliest, 0), (uint32_t)(row.first(p) + e));
+                            }
+                        }
+                    }
+                }
+                ++turn;
+                const double run = warp_scan(mine, lane), s = __shfl_sync(kFullMask, run, ranks - 1);
+                if (stage == kAll) z = s;
+                if (heat.greedy) {
+                    cluster.sync();
+                    if (rank == 0 && tid == 0) {
+                        out_tokens[o.at] = likeliest == 0xFFFFFFFFu ? 0 : (int32_t)likeliest;
+                        if (logprobs) logprobs[o.at] = z > 0.0 ? (float)-log(z) : -INFINITY;
+                    }
+                    break;
+                }
+                if (stage == kAll && o.refused && (o.drawn || o.what == 2)) {
+                    stage = kLeft;
+                    continue;
+                }
+                if (o.what == 1) {
+                    if (rank == 0 && tid == 0) {       // the thread that walks
+                        walk.z = z;
+                        walk.s = s;
+                        walk.summed = 1;
+                        walk.step = 0;
+                    }
+                    break;
+                }
+                if (!(s > 0.0)) {
+                    if (stage == kLeft) {              // nothing left: from all of it
+                        stage = kAgain;
+                        continue;
+                    }
+                    if (rank == 0 && tid == 0) {
+                        out_tokens[o.at] = 0;
+                        if (logprobs) logprobs[o.at] = -INFINITY;
+                    }
+                    break;
+                }
+                target = (double)o.u * s;
+                const uint32_t who = warp_fall(mine, run, target);
+                if (who != rank) break;
+                target /= __shfl_sync(kFullMask, scale, who);
+            }
+            const uint32_t its = warp_fall(part, upto, target);
+            begin += its * sub * kWarp;
+            count = min(sub, count - its * sub);
+            sub = (count + kWalkWarps - 1) / kWalkWarps;
+            stage = count > 1 ? kWithin : kStep;
         }
+        if (o.what == 2) break;
     }
     if (rank == 0) {
+        __syncthreads();
         const uint32_t tokens = of.n ? walk.at + 1 : 0;
         for (uint32_t i = tid; i < a.draft_stride; i += kWalkThreads) {
             if (i == 0) out_rows[0] = of.n ? 0 : -1;
+            if (logprobs && !alone && i < of.n && nodes.inner[i] < 0)
+                logprobs[-1 - nodes.inner[i]] = (float)(heat.greedy ? -log(nodes.z[i]) : log(nodes.weight[i] / nodes.z[i]));
             if (i < tokens) continue;
             out_tokens[i] = -1;
             if (i) out_rows[i] = -1;
@@ -808,7 +841,7 @@ template <typename T, bool CAP>
 tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a) {
     const char* name = "tf_verify_drafts";
     constexpr uint32_t E = Row<T>::E;
-    if (a.rows) {
+    if (a.rows && a.draft_stride > 1) {            // lone rows need none of it
         const bool even = aligned(a.logits, 16) && a.stride % E == 0;          // else a row may begin anywhere in a piece
         a.chunks = (uint32_t)(((uint64_t)a.vocab + (even ? 0 : E - 1) + kChunk - 1) / kChunk);
         // several chunks a block, as long as that leaves every place on the chip a few blocks
@@ -820,8 +853,11 @@ tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a) {
         if (s != TF_OK) return s;
     }
     uint32_t ranks = 8;
-    while (ranks > 1 && (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2) ranks /= 2;
-    const size_t smem = (size_t)a.draft_stride * 36;
+    while (ranks > 1 && (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count) ranks /= 2;
+    const size_t smem = a.draft_stride * NodeTable::kBytes;
+    static DeviceSmemCache smem_cache;
+    const tf_status m = ensure_dynamic_smem(ctx, verify_walk_kernel<T, CAP>, smem_cache, smem);
+    if (m != TF_OK) return m;
     TF_CUDA(ctx, launch_pdl_cluster(verify_walk_kernel<T, CAP>, dim3(a.sequences * ranks), dim3(kWalkThreads), smem, st, ranks, a));
     return check_launch(ctx, name);
 }
