@@ -12,6 +12,7 @@
 // an error of 1e-7 in it would make up to one draw in a hundred another token. The draw itself goes from the sums of blocks to those of warps to a warp's pieces.
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <new>
 #include <type_traits>
 
@@ -29,14 +30,14 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kStatsThreads = 256, kChunk = 8192;          // elements that a block of the first launch takes at a time
-constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / kWarp;
-constexpr uint32_t kMostNodes = 1024;
+constexpr int kWalkThreads = 256, kWalkWarps = kWalkThreads / kWarp;
+constexpr uint32_t kMostNodes = 1024, kMostRanks = 16;       // blocks of a sequence: a cluster beyond eight is to be asked for
 constexpr double kLog2E = 1.4426950408889634074;
 
 // The largest logit of some chunks, the sum of their weights relative to that, and where the largest stands first.
 struct ChunkStat {
     float most, sum;
-    uint32_t at, unused;
+    uint32_t at, infinite;     // infinite: there are +infinities, which count for nothing
 };
 
 struct VerifyArgs {
@@ -73,18 +74,27 @@ template <typename T>
 struct Row {
     static constexpr int E = 16 / sizeof(T);
     const T* p;
-    uint32_t lead, vocab;
-    __device__ __forceinline__ Row(const void* base, uint64_t at, uint32_t n) : p(static_cast<const T*>(base) + at), vocab(n) {
+    const uint4* base;         // of piece 0, where the row begins at a boundary or inside the piece
+    uint32_t lead, vocab, whole0, whole;       // pieces [whole0, whole0 + whole) hold elements of the row alone
+    __device__ __forceinline__ Row(const void* start, uint64_t at, uint32_t n) : p(static_cast<const T*>(start) + at), vocab(n) {
         lead = (uint32_t)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
+        base = reinterpret_cast<const uint4*>(p - lead);
+        whole0 = lead ? 1 : 0;
+        const uint32_t end = (uint32_t)(((uint64_t)vocab + lead) / E);
+        whole = end > whole0 ? end - whole0 : 0;
     }
     __device__ __forceinline__ uint32_t pieces() const { return (uint32_t)(((uint64_t)vocab + lead + E - 1) / E); }
     __device__ __forceinline__ int64_t first(uint32_t piece) const { return (int64_t)piece * E - lead; }
+    static __device__ __forceinline__ uint4 nothing() {
+        constexpr uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+        return make_uint4(w, w, w, w);
+    }
+    // Behind the last piece too
     __device__ __forceinline__ uint4 load(uint32_t piece) const {
+        if (piece - whole0 < whole) return base[piece];
         const int64_t at = first(piece);
-        if (at >= 0 && at + E <= (int64_t)vocab) return *reinterpret_cast<const uint4*>(p + at);
-        constexpr uint32_t nothing = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
         T v[E];
-        uint4 w = make_uint4(nothing, nothing, nothing, nothing);
+        uint4 w = nothing();
         memcpy(v, &w, 16);
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -116,6 +126,9 @@ struct Row {
 __device__ __forceinline__ float capped(float x, float cap) {
     return x == -INFINITY ? x : cap * (1.0f - __fdividef(2.0f, verify_exp2(x * (float)(2 * kLog2E) / cap) + 1.0f));
 }
+
+// A random number, in [0, 1) whatever it is.
+__device__ __forceinline__ float uniform(float u) { return fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f); }
 
 struct Heat {
     bool greedy;
@@ -173,7 +186,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
     using R = Row<T>;
     constexpr int E = R::E, PIECES = kChunk / E / kStatsThreads, WARPS = kStatsThreads / kWarp;
     constexpr uint32_t STEP = kChunk / E;
-    __shared__ uint32_t found, best;
+    __shared__ uint32_t found, best, infinite;
     __shared__ float warp_most[WARPS], warp_sum_[WARPS];
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
@@ -187,7 +200,10 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
             if (piece + j * kStatsThreads < end) next[j] = r.load(piece + j * kStatsThreads);
     };
     request();
-    if (tid == 0) found = best = 0xFFFFFFFFu;
+    if (tid == 0) {
+        found = best = 0xFFFFFFFFu;
+        infinite = 0;
+    }
     __syncthreads();
     for (uint32_t b = tid; b < a.sequences; b += kStatsThreads) {
         const Nodes of(a, b, false);
@@ -224,6 +240,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
         request();
         piece = here;
         if (top == INFINITY) {                                 // does not count
+            infinite = 1;
             top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < PIECES; ++j) {
@@ -300,7 +317,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
     if (tid == 0) {
         sum = 0.0f;
         for (int w = 0; w < WARPS; ++w) sum += warp_sum_[w];
-        a.stats[(size_t)row * a.parts + part] = {top, sum, best, 0};
+        a.stats[(size_t)row * a.parts + part] = {top, sum, best, infinite};
     }
 }
 
@@ -312,40 +329,129 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
 // add less than 2^-17; capped logits are off by at most softcap 2^-20 each.
 __device__ __forceinline__ double sum_bound(float cap, double k) { return 0x1p-15 + (cap > 0.0f ? (double)cap * k * 0x1p-19 : 0.0); }
 
-// 2^(y k / 32) in 64 bits by all lanes of a warp: 2^(j/32) from a table that the lanes hold, times the Taylor sum of 2^r, |r| <= 1/64, to its fifth power
-// (2e-15 of it), times a power of two. Exponents from -1000 to 1000; below, and for y = -infinity, 0.
-__device__ __forceinline__ double warp_exp2(double y, double k, double table) {
-    const double shift = 6755399441055744.0;                                    // 1.5 2^52: the sum's last bits are the rounded number
-    const double t = fma(y, k, shift);
-    const int j = __double2loint(t);
-    const double r = fma(y, k, shift - t);
-    constexpr double c = 0.69314718055994530942 / 32;
-    double s = c * c * c * c * c / 120;
-    s = fma(s, r, c * c * c * c / 24);
-    s = fma(s, r, c * c * c / 6);
-    s = fma(s, r, c * c / 2);
-    s = fma(s, r, c);
-    s = s * r;
-    const double base = __shfl_sync(kFullMask, table, j & 31);
-    const double v = fma(base, s, base);
-    return t >= shift - 32000.0 ? __hiloint2double(__double2hiint(v) + ((j >> 5) << 20), __double2loint(v)) : 0.0;
+// y = 2^(y k / 32) in 64 bits by all lanes of a warp: 2^(j/32) from a table that the lanes hold, times the Taylor sum of 2^r, |r| <= 1/64, to its fourth power
+// (1.3e-12 of it; what a sum gathers of that moves a border between tokens by less than 1e-17 of it a token), times a power of two, which goes into the table's number: its upper words are lower by
+// what the last bits of j add there. Exponents from -1010 to 1010. All N at once, so that none waits for the eleven operations in a row.
+template <int N>
+__device__ __forceinline__ void warp_exp2(double (&y)[N], double k, int2 table) {
+    constexpr double shift = 6755399441055744.0;                                // 1.5 2^52: the sum's last bits are the rounded number
+    constexpr double c = 0.69314718055994530942 / 32, taylor[4] = {c, c * c / 2, c * c * c / 6, c * c * c * c / 24};
+    int j[N];
+    double base[N], s[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const double t = fma(y[e], k, shift);
+        j[e] = __double2loint(t);
+        y[e] = fma(y[e], k, shift - t);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int hi = __shfl_sync(kFullMask, table.x, j[e]), lo = __shfl_sync(kFullMask, table.y, j[e]);       // by their last five bits
+        base[e] = __hiloint2double(hi + j[e] * 32768, lo);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] = taylor[3];
+#pragma unroll
+    for (int i = 2; i >= 0; --i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] = fma(s[e], y[e], taylor[i]);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] *= y[e];
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = fma(base[e], s[e], base[e]);
 }
+__device__ __forceinline__ double positive(double v) { return __double2hiint(v) < 0 ? 0.0 : v; }
 
 template <bool CAP>
 __device__ __forceinline__ double logit64(float x, float cap) {
     if constexpr (CAP) return (double)cap * tanh((double)x / (double)cap);
     else return (double)x;
 }
-// The same by all lanes of a warp, 1e-13 softcap off: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps. twice: 64 log2(e) / cap.
+__device__ const double kPowers[32] = {               // 2^(j / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
+    1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
+    1.9152065613971474, 1.9571441241754002};
+__device__ __forceinline__ int2 power_table(int lane) { return make_int2(__double2hiint(kPowers[lane]) - lane * 32768, __double2loint(kPowers[lane])); }
+
+// From logits to weights, what a row has in common.
+struct Scale {
+    double from, k, cap, twice, lowest;        // the logit of weight 1, 32 log2(e) / T; softcap, 64 log2(e) / softcap; -32000 / k, where a weight is 2^-1000
+    float least;               // logits from here down count as that, where the row needs no care
+    int2 table;
+    bool careful;              // the row holds infinities, or steps of 32 bits that are as large as that
+    // With the row's largest logit, as it is; infinite: there are some that do not count. By all lanes.
+    template <bool CAP>
+    __device__ __forceinline__ void relative_to(float top, bool infinite);
+};
+constexpr double kNothing = 0x1p-900;          // more than a vocabulary of tokens that do not count
+
+// Weights in 64 bits by all lanes of a warp. Capped logits: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps, 1e-13 cap off.
+template <bool CAP, int N>
+__device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N], double (&w)[N]) {
+    if constexpr (!CAP) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = (double)fmaxf(x[e], s.least) - s.from;      // NaN too
+    } else {
+        const float edge = 20.0f * (float)s.cap;                                // tanh is 1 to the last bit from there on
+        double y[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = (double)fminf(fmaxf(x[e], -edge), edge);
+        warp_exp2(w, s.twice, s.table);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            w[e] += 1.0;
+            float y0;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"((float)w[e]));
+            y[e] = (double)y0;
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = fma(-w[e], y[e], 1.0);
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = fma(y[e], w[e], y[e]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = fma(-2.0 * s.cap, y[e], s.cap - s.from);
+    }
+    if constexpr (CAP) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = x[e] > s.least ? w[e] : s.lowest;
+    }
+    if (s.careful) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = fabsf(x[e]) < INFINITY && w[e] >= s.lowest ? w[e] : s.lowest;
+    }
+    warp_exp2(w, s.k, s.table);
+}
+// One logit by all lanes, whatever it is and what the others are.
 template <bool CAP>
-__device__ __forceinline__ double warp_logit64(float x, double cap, double twice, double table) {
+__device__ __forceinline__ double warp_logit64(const Scale& s, float x) {
     if constexpr (!CAP) return (double)x;
-    const float edge = 20.0f * (float)cap;                                      // tanh is 1 to the last bit from there on
-    const double d = warp_exp2((double)fminf(fmaxf(x, -edge), edge), twice, table) + 1.0;
-    float y0;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"((float)d));
-    const double y = fma((double)y0, fma(-d, (double)y0, 1.0), (double)y0);
-    return x > -INFINITY ? fma(-2.0 * cap, y, cap) : -INFINITY;
+    const float edge = 20.0f * (float)s.cap;
+    double d[1] = {(double)fminf(fmaxf(x, -edge), edge)};
+    warp_exp2(d, s.twice, s.table);
+    return fabsf(x) < INFINITY ? s.cap - 2.0 * s.cap / (d[0] + 1.0) : -INFINITY;
+}
+__device__ __forceinline__ double warp_weight(const Scale& s, double logit) {
+    const double y = logit - s.from;
+    const bool is = y * s.k >= -32000.0;               // not for NaN
+    double w[1] = {is ? y : 0.0};
+    warp_exp2(w, s.k, s.table);
+    return is ? w[0] : 0.0;
+}
+template <bool CAP>
+__device__ __forceinline__ void Scale::relative_to(float top, bool infinite) {
+    from = top > -INFINITY ? warp_logit64<CAP>(*this, top) : 0.0;
+    const double bottom = from + lowest;
+    if (CAP) {
+        // the cap's inverse, cap atanh(bottom / cap); 2^-23 of the cap is the widest step of its logits
+        careful = infinite || cap * 0x1p-22 * k > 320.0;
+        least = bottom > -cap && !careful ? (float)(0.5 * cap * log((cap + bottom) / (cap - bottom))) : -INFINITY;
+    } else {
+        careful = infinite || bottom < -3.4028234e38 || fabs(from) * 0x1p-22 * k > 320.0;
+        least = careful ? -3.4028234e38f : (float)bottom;
+    }
 }
 
 // What the cluster does next, and with which row.
@@ -363,11 +469,11 @@ struct Walk {
     double z, s, gone;         // gone: weight of the refused tokens, without q
 };
 
-// The first block's shared memory: what it knows of the nodes. 48 bytes of each.
+// The first block's shared memory: what it knows of the nodes.
 struct NodeTable {
     double *z, *weight;        // of a row: its sum in 32 bits; of a token: its weight in its parent's row
     double* gone;              // of the current node's refused children: S before each, or (as int32) the tokens
-    float *most, *prob;
+    float *most, *prob, *number;           // number: the random one
     uint32_t* best;
     int32_t *parent, *token, *inner;       // inner: has children; -1 - place of a kept node
     __device__ __forceinline__ NodeTable(uint8_t* memory, uint32_t n) {
@@ -376,21 +482,14 @@ struct NodeTable {
         gone = weight + n;
         most = reinterpret_cast<float*>(gone + n);
         prob = most + n;
-        best = reinterpret_cast<uint32_t*>(prob + n);
+        number = prob + n;
+        best = reinterpret_cast<uint32_t*>(number + n);
         parent = reinterpret_cast<int32_t*>(best + n);
         token = parent + n;
         inner = token + n;
     }
-    static constexpr size_t kBytes = 48;
+    static constexpr size_t kBytes = 52;
 };
-
-__device__ const double kPowers[32] = {               // 2^(j / 32)
-    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
-    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
-    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
-    1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
-    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
-    1.9152065613971474, 1.9571441241754002};
 
 __device__ __forceinline__ float prob_at(const VerifyArgs& a, uint64_t at) {
     float q;
@@ -399,36 +498,63 @@ __device__ __forceinline__ float prob_at(const VerifyArgs& a, uint64_t at) {
     else q = __bfloat162float(static_cast<const __nv_bfloat16*>(a.probs)[at]);
     return fmaxf(q, 0.0f);     // NaN too
 }
-// E of them, of which those outside the row are zero
-template <int E>
-__device__ __forceinline__ void probs_at(const VerifyArgs& a, uint64_t row, int64_t first, float (&q)[E]) {
-    const bool whole = first >= 0 && first + E <= (int64_t)a.vocab;
-    if (a.probs_dtype == TF_FP32) {
-        const float* p = static_cast<const float*>(a.probs) + (int64_t)row + first;
-        if (whole && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-            uint4 w[E / 4];
+// A node's row of probabilities by the pieces of its logits.
+template <typename T>
+struct ProbRow {
+    static constexpr int E = Row<T>::E;
+    uint64_t at;
+    bool even;                 // a piece's lie at a boundary of as many bytes, up to 16
+    __device__ __forceinline__ ProbRow(const VerifyArgs& a, uint64_t row, uint32_t lead) : at(row - lead) {
+        const uint32_t size = a.probs_dtype == TF_FP32 ? 4 : 2;
+        even = (reinterpret_cast<uintptr_t>(a.probs) + at * size) % (size * E < 16 ? size * E : 16) == 0;
+    }
+    static constexpr int WORDS = E / 4;        // a piece's as 32-bit numbers; 16-bit ones take half of it
+    __device__ __forceinline__ void load(const VerifyArgs& a, const Row<T>& row, uint32_t piece, uint4 (&w)[WORDS]) const {
+        const uint64_t from = at + (uint64_t)piece * E;
+        const bool whole = even && piece - row.whole0 < row.whole;
+        const int64_t first = row.first(piece);
+        if (a.probs_dtype == TF_FP32) {
+            const float* p = static_cast<const float*>(a.probs) + from;
+            if (whole) {
 #pragma unroll
-            for (int i = 0; i < E / 4; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+                for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+            } else {
+                float v[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) q[e] = fmaxf(__uint_as_float(e % 4 == 0 ? w[e / 4].x : e % 4 == 1 ? w[e / 4].y : e % 4 == 2 ? w[e / 4].z : w[e / 4].w), 0.0f);
-            return;
-        }
-    } else {
-        const uint16_t* p = static_cast<const uint16_t*>(a.probs) + (int64_t)row + first;
-        if (whole && reinterpret_cast<uintptr_t>(p) % (2 * E) == 0) {
-            uint32_t w[E / 2];
-            load_words<E / 2>(w, p);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const uint16_t v = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-                q[e] = fmaxf(a.probs_dtype == TF_FP16 ? f16_bits_to_float(v) : bf16_bits_to_float(v), 0.0f);
+                for (int e = 0; e < E; ++e) v[e] = first + e >= 0 && first + e < (int64_t)row.vocab ? p[e] : 0.0f;
+                memcpy(w, v, sizeof(v));
             }
-            return;
+        } else {
+            const uint16_t* p = static_cast<const uint16_t*>(a.probs) + from;
+            if (whole) {
+                if constexpr (E == 8) {
+                    w[0] = *reinterpret_cast<const uint4*>(p);
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(p);
+                    w[0].x = v.x;
+                    w[0].y = v.y;
+                }
+            } else {
+                uint16_t v[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = first + e >= 0 && first + e < (int64_t)row.vocab ? p[e] : (uint16_t)0;
+                memcpy(w, v, sizeof(v));
+            }
         }
     }
+    static __device__ __forceinline__ void numbers(const VerifyArgs& a, const uint4 (&w)[WORDS], float (&q)[E]) {
+        if (a.probs_dtype == TF_FP32) {
+            memcpy(q, w, sizeof(q));
+        } else {
+            uint16_t v[E];
+            memcpy(v, w, sizeof(v));
 #pragma unroll
-    for (int e = 0; e < E; ++e) q[e] = first + e >= 0 && first + e < (int64_t)a.vocab ? prob_at(a, row + first + e) : 0.0f;
-}
+            for (int e = 0; e < E; ++e) q[e] = a.probs_dtype == TF_FP16 ? f16_bits_to_float(v[e]) : bf16_bits_to_float(v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e] = fmaxf(q[e], 0.0f);
+    }
+};
 
 // Inclusive sums over a warp's lanes.
 __device__ __forceinline__ double warp_scan(double v, uint32_t lane) {
@@ -443,7 +569,7 @@ __device__ __forceinline__ double warp_scan(double v, uint32_t lane) {
 // Among parts in the lanes' order, whose sums `upto` are, the one that the target falls in; rounding may leave it behind the last that has anything, which is then it.
 // The target becomes that within the part.
 __device__ __forceinline__ uint32_t warp_fall(double part, double upto, double& target) {
-    const uint32_t any = __ballot_sync(kFullMask, part > 0.0), over = __ballot_sync(kFullMask, part > 0.0 && upto > target);
+    const uint32_t any = __ballot_sync(kFullMask, part > kNothing), over = __ballot_sync(kFullMask, part > kNothing && upto > target);
     const uint32_t who = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : 0;
     const double before = __shfl_sync(kFullMask, upto - part, who);
     target = over ? target - before : INFINITY;
@@ -452,10 +578,10 @@ __device__ __forceinline__ uint32_t warp_fall(double part, double upto, double& 
 
 // One thread goes from node to node until a sum over the vocabulary is needed, or the walk is over.
 template <bool CAP>
-__device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, const Heat& heat, uint32_t b, const NodeTable& t, Walk& w, Order& order,
+__device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, const Heat& heat, uint32_t b, const NodeTable& t, Walk& walk, Order& order,
                                         int32_t* out_tokens, int32_t* out_rows) {
+    Walk w = walk;                                     // in registers: it was most of the walk to fetch it back and forth
     const double bound = sum_bound(a.softcap, heat.k);
-    const float* uniforms = a.uniforms + (size_t)b * a.draft_stride;
     const int32_t* gone_tokens = reinterpret_cast<const int32_t*>(t.gone);
     order.what = 0;
     if (of.n == 0) return;
@@ -467,7 +593,7 @@ __device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, co
         if (heat.greedy) {
             keep = t.most[w.node] > -INFINITY && (uint32_t)t.token[i] == t.best[w.node];
         } else {
-            const double u = (double)fminf(fmaxf(uniforms[i], 0.0f), 0x1.fffffep-1f), weight = t.weight[i];
+            const double u = (double)t.number[i], weight = t.weight[i];
             bool ask = false;
             double left, right = weight;
             if (drawn) {
@@ -485,6 +611,7 @@ __device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, co
             }
             if (ask) {
                 order = {1, w.node, 0, 1, w.summed, w.step, drawn, w.refused, t.most[w.node], 0.0f, w.z, w.s};
+                walk = w;
                 return;
             }
             keep = left < right;
@@ -511,30 +638,111 @@ __device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, co
             w.refused += 1;
         }
     }
+    walk = w;
     if (heat.greedy) {
         out_tokens[w.at] = (int32_t)t.best[w.node];
         if (a.logprobs) a.logprobs[(size_t)b * a.draft_stride + w.at] = w.z > 0.0 ? (float)-log(w.z) : -INFINITY;
         return;
     }
-    const float u = fminf(fmaxf(uniforms[0], 0.0f), 0x1.fffffep-1f);
-    order = {2, w.node, w.at, w.known, w.summed, w.step, a.probs && w.node < a.probs_nodes, w.refused, t.most[w.node], u, w.z, w.s};
+    order = {2, w.node, w.at, w.known, w.summed, w.step, a.probs && w.node < a.probs_nodes, w.refused, t.most[w.node], t.number[0], w.z, w.s};
+}
+
+// What `refused` children leave of the weights of `steps` pieces a warp apart, from `piece` on: their sum, and the weights of the last piece. With `parts`, the sums of
+// every `per` steps go there too, kWalkThreads apart. A function of its own, with all registers for its loop; four elements at a time, so that these do.
+template <typename T, bool CAP>
+__device__ __noinline__ double sum_steps(const VerifyArgs& a, const Row<T>& of, const ProbRow<T>& its, const double* gone, uint32_t piece, uint32_t steps, int refused,
+                                         bool drawn, const Scale& by, double (&last)[Row<T>::E], double* parts, uint32_t per) {
+    using R = Row<T>;
+    using P = ProbRow<T>;
+    constexpr int E = R::E;
+    const R row = of;
+    const P probs = its;
+    const Scale s = by;
+    double all = 0.0, part = 0.0, w[E];
+    uint32_t until = per;
+    // the next two steps' logits and probabilities are on their way
+    uint4 next[2] = {steps ? row.load(piece) : R::nothing(), steps > 1 ? row.load(piece + kWarp) : R::nothing()}, next_q[2][P::WORDS] = {};
+    if (drawn) {
+        if (steps) probs.load(a, row, piece, next_q[0]);
+        if (steps > 1) probs.load(a, row, piece + kWarp, next_q[1]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = 0.0;
+#pragma unroll 1
+    for (; steps; --steps, piece += kWarp) {
+        float x[E], q[E];
+        R::numbers(next[0], x);
+        next[0] = next[1];
+        if (steps > 2) next[1] = row.load(piece + 2 * kWarp);
+        if (drawn) {
+            P::numbers(a, next_q[0], q);
+#pragma unroll
+            for (int i = 0; i < P::WORDS; ++i) next_q[0][i] = next_q[1][i];
+            if (steps > 2) probs.load(a, row, piece + 2 * kWarp, next_q[1]);
+        }
+        double sum[E / 4];
+#pragma unroll
+        for (int h = 0; h < E; h += 4) {
+            float some[4];
+            double v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) some[e] = x[h + e];
+            warp_weights<CAP>(s, some, v);
+            if (drawn) {
+#pragma unroll 1
+                for (int g = 0; g < refused; ++g) {
+                    const double taken = gone[g];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = positive(fma(-taken, (double)q[h + e], v[e]));
+                }
+            } else {
+#pragma unroll 1
+                for (int g = 0; g < refused; ++g) {
+                    const int64_t e0 = (int64_t) reinterpret_cast<const int32_t*>(gone)[g] - row.first(piece);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = e0 == h + e ? 0.0 : v[e];
+                }
+            }
+            sum[h / 4] = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[h + e] = v[e];
+        }
+        part += E == 8 ? sum[0] + sum[E / 4 - 1] : sum[0];
+        if (--until == 0) {
+            all += part;
+            if (parts) {
+                *parts = part;
+                parts += kWalkThreads;
+            }
+            part = 0.0;
+            until = per;
+        }
+    }
+    all += part;
+    if (parts) *parts = part;                  // what is left, or nothing: there is room for one more
+#pragma unroll
+    for (int e = 0; e < E; ++e) last[e] = w[e];
+    return all;
 }
 
 template <typename T, bool CAP>
-__global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
     using R = Row<T>;
+    using P = ProbRow<T>;
     constexpr int E = R::E;
     extern __shared__ __align__(16) uint8_t dynamic[];
     __shared__ Order orders[2];                    // by turns: one is read while the next is written
     __shared__ Walk walk;
-    __shared__ double block_sum[2], warp_part[kWalkWarps];
+    __shared__ double block_sum[2], warp_part[kWalkWarps], parts[(kWalkWarps + 1) * kWalkThreads];
     __shared__ float block_most[2], warp_most[kWalkWarps];
     __shared__ uint32_t likeliest;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const uint32_t rank = cluster.block_rank(), ranks = cluster.num_blocks(), b = blockIdx.x / ranks;
-    const double table = kPowers[lane];
-    pdl_wait();
+    Scale scale;
+    scale.table = power_table(lane);
+    // The first launch waits for what came before it and writes nothing but its sums: all else may be read while it is at work.
+    if (a.parts == 0) pdl_wait();
     const Nodes of(a, b, rank == 0 && tid == 0);
     const Heat heat(a, b);
     const NodeTable nodes(dynamic, a.draft_stride);
@@ -542,7 +750,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
     int32_t* out_tokens = a.out_tokens + (size_t)b * a.draft_stride;
     int32_t* out_rows = a.out_rows + (size_t)b * a.draft_stride;
     float* logprobs = a.logprobs ? a.logprobs + (size_t)b * a.draft_stride : nullptr;
-    const double k = heat.k * 32.0, cap = a.softcap, twice = CAP ? 64.0 * kLog2E / cap : 0.0;
+    scale.k = heat.k * 32.0;
+    scale.cap = a.softcap;
+    scale.twice = CAP ? 64.0 * kLog2E / scale.cap : 0.0;
+    scale.lowest = -32000.0 / scale.k;
     constexpr double kLn2 = 0.69314718055994530942;
     // A lone row is drawn from at once by all blocks, whatever there is to know of it.
     const bool alone = of.n == 1 && (a.draft_stride == 1 || !heat.greedy);
@@ -552,31 +763,30 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
     }
 
     if (rank == 0 && !alone) {
-        for (uint32_t i = tid; i < of.n; i += kWalkThreads) {
-            const int32_t x = a.tokens[(size_t)b * a.draft_stride + i];
-            nodes.parent[i] = i ? parent_of(a, b, i) : -1;
-            nodes.token[i] = x >= 0 && (uint32_t)x < a.vocab ? x : -1;
-            nodes.inner[i] = 0;
-            nodes.most[i] = -INFINITY;
-        }
+        for (uint32_t i = tid; i < of.n; i += kWalkThreads) nodes.inner[i] = 0;
         __syncthreads();
         for (uint32_t i = tid; i < of.n; i += kWalkThreads) {
-            const int32_t p = nodes.parent[i], x = nodes.token[i];
+            const int32_t x = a.tokens[(size_t)b * a.draft_stride + i], p = i ? parent_of(a, b, i) : -1;
+            const bool token = x >= 0 && (uint32_t)x < a.vocab;
+            nodes.parent[i] = p;
+            nodes.token[i] = token ? x : -1;
+            nodes.number[i] = uniform(a.uniforms[(size_t)b * a.draft_stride + i]);
             if (p < 0) continue;
-            nodes.inner[p] = 1;
-            if (x < 0) continue;
+            atomicOr(nodes.inner + p, 1);
+            if (!token) continue;
             nodes.weight[i] = (double)counted(number(static_cast<const T*>(a.logits)[(of.row0 + (uint64_t)p) * a.stride + x]));     // for now
             nodes.prob[i] = a.probs && (uint32_t)p < a.probs_nodes ? prob_at(a, b * a.probs_sequence + p * a.probs_node + x) : 0.0f;
         }
-        __syncthreads();
+        if (a.parts) pdl_wait();
+        // A leaf's numbers are whatever an earlier call left: nobody looks at them.
         for (uint32_t i = warp; i < of.n; i += kWalkWarps) {
-            if (!nodes.inner[i] && !heat.greedy) continue;
             const ChunkStat* s = a.stats + (size_t)(of.row0 + i) * a.parts;
             float top = -INFINITY;
-            uint32_t at = 0xFFFFFFFFu;
+            uint32_t at = 0xFFFFFFFFu, infinite = 0;
             for (uint32_t c = lane; c < a.parts; c += kWarp) {
                 const ChunkStat x = s[c];
                 if (x.most > top) { top = x.most; at = x.at; }                 // parts ascend: the first of equals stays
+                infinite |= x.infinite;
             }
             float all = top;
 #pragma unroll
@@ -596,28 +806,32 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
                 nodes.z[i] = sum;
                 nodes.best[i] = at == 0xFFFFFFFFu ? 0u : at;
             }
+            if (__any_sync(kFullMask, infinite) && lane == 0) atomicOr(nodes.inner + i, 2);
         }
         __syncthreads();
         for (uint32_t i0 = warp * kWarp; i0 < of.n; i0 += kWalkThreads) {
             const uint32_t i = i0 + lane;
             const bool is = i < of.n && nodes.parent[i] >= 0 && nodes.token[i] >= 0;
             const float x = is ? (float)nodes.weight[i] : -INFINITY, top = is ? nodes.most[nodes.parent[i]] : -INFINITY;
-            const double l = warp_logit64<CAP>(x, cap, twice, table), from = warp_logit64<CAP>(top, cap, twice, table);
-            const double w = warp_exp2(top > -INFINITY ? l - from : -INFINITY, k, table);
+            const double l = warp_logit64<CAP>(scale, x);
+            scale.from = warp_logit64<CAP>(scale, top);
+            const double w = warp_weight(scale, l);    // of infinities and NaN: 0
             if (is) nodes.weight[i] = w;
         }
         __syncthreads();
         if (tid == 0 && of.n) {
             walk.z = nodes.z[0];
-            walk.known = nodes.inner[0];
+            walk.known = nodes.inner[0];               // a leaf may have the second bit of another call's row: no matter
         }
+    } else if (a.parts) {
+        pdl_wait();                                    // before anything is written
     }
     __syncthreads();
 
     for (uint32_t round = 0, turn = 0;; ++round) {
         Order o = {2, 0, 0, 0, 0, 0, 0, 0, 0.0f, 0.0f, 0.0, 0.0};
         if (alone) {
-            o.u = fminf(fmaxf(a.uniforms[(size_t)b * a.draft_stride], 0.0f), 0x1.fffffep-1f);
+            o.u = uniform(a.uniforms[(size_t)b * a.draft_stride]);
         } else {
             if (rank == 0 && tid == 0) walk_on<CAP>(a, of, heat, b, nodes, walk, orders[round & 1], out_tokens, out_rows);
             __syncwarp();
@@ -635,12 +849,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
         // ---- the pieces: a warp's are neighbours, and a block's warps, so that sums run in the order of the tokens ----
         const R row(a.logits, (of.row0 + (uint64_t)o.node) * a.stride, a.vocab);
         const uint32_t pieces = row.pieces(), steps = (pieces + ranks * kWalkThreads - 1) / (ranks * kWalkThreads);
-        const uint64_t q_row = b * a.probs_sequence + o.node * a.probs_node;
-        uint32_t begin = rank * kWalkWarps * steps * kWarp, count = kWalkWarps * steps, sub = steps;       // first piece, steps of a warp's width, steps a warp
+        const P probs(a, b * a.probs_sequence + o.node * a.probs_node, row.lead);
+        uint32_t begin = rank * kWalkWarps * steps * kWarp;
+        const uint32_t per = (steps + kWalkWarps - 1) / kWalkWarps;            // steps whose sum is kept for the draw
         // A row without a maximum (a leaf: nothing was refused) is summed by every block relative to its own, one meeting less.
         float top = o.most;
-        if (!o.known) {
+        bool infinite = o.known & 2;
+        if (!(o.known & 1)) {
             top = -INFINITY;
+            infinite = false;
             for (uint32_t i = 0, piece = begin + warp * steps * kWarp + lane; i < steps && piece < pieces; i += 4, piece += 4 * kWarp) {
                 uint4 w[4];
 #pragma unroll
@@ -653,6 +870,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
                         if (most == INFINITY) {            // does not count
                             float x[E];
                             R::numbers(w[j], x);
+                            infinite = true;
                             most = -INFINITY;
 #pragma unroll
                             for (int e = 0; e < E; ++e) most = fmaxf(most, counted(x[e]));
@@ -663,18 +881,30 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
             if (lane == 0) warp_most[warp] = top;
-            __syncthreads();
+            infinite = __syncthreads_or(infinite);
             top = lane < kWalkWarps ? warp_most[lane] : -INFINITY;
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
         }
-        const double from = top > -INFINITY ? warp_logit64<CAP>(top, cap, twice, table) : 0.0;
+        scale.relative_to<CAP>(top, infinite);
 
         // ---- sums, and the draw from block to warp to step to token, with one body for all of it: what runs once costs what its instructions take to fetch ----
-        enum { kAll, kLeft, kAgain, kWithin, kStep };
+        enum { kAll, kLeft, kAgain };
         int stage = !o.summed ? kAll : o.refused && (o.drawn || o.what == 2) ? kLeft : kAgain;
-        double z = o.z, target = 0.0, whole = from;    // whole: the logit that z is relative to
+        double z = o.z, target = 0.0, whole = scale.from, part, upto;          // whole: the logit that z is relative to; part, upto: lane w's sum of warp w, and up to it
         int refused = 0;
+        // Sums of warps from those of lanes, in every warp.
+        auto warps = [&](double mine) {
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) mine += __shfl_xor_sync(kFullMask, mine, off);
+            __syncthreads();                           // the sums before these have been read
+            if (lane == 0) warp_part[warp] = mine;
+            __syncthreads();
+            part = lane < kWalkWarps ? warp_part[lane] : 0.0;
+            upto = warp_scan(part, lane);
+        };
+        bool chosen = false;                           // this block has the token
+        double w[E];
         for (;;) {
             if (stage == kLeft) {
                 refused = o.refused;
@@ -685,137 +915,114 @@ __global__ void __launch_bounds__(kWalkThreads, 1) verify_walk_kernel(const __gr
             } else if (stage == kAgain) {
                 refused = 0;
             }
-            // what `refused` children leave of the weights of this warp's steps; in a single step every warp has all of it
-            const uint32_t first = stage == kStep ? 0u : min(warp * sub, count), last = stage == kStep ? 1u : min(first + sub, count);
-            double w[E], all = 0.0;
-            uint32_t piece = begin + first * kWarp + lane;
-            uint4 next = make_uint4(0, 0, 0, 0);
-            if (first < last && piece < pieces) next = row.load(piece);
-            for (uint32_t i = first; i < last; ++i, piece += kWarp) {
-                float x[E];
-                R::numbers(next, x);
-                if (i + 1 < last && piece + kWarp < pieces) next = row.load(piece + kWarp);
-                float q[E];
-                if (refused && o.drawn) probs_at<E>(a, q_row, piece < pieces ? row.first(piece) : (int64_t)a.vocab, q);
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    w[e] = warp_exp2(warp_logit64<CAP>(piece < pieces ? counted(x[e]) : -INFINITY, cap, twice, table) - from, k, table);
-                for (int g = 0; g < refused; ++g) {
-                    if (o.drawn) {
-                        const double s = nodes.gone[g];
-#pragma unroll
-                        for (int e = 0; e < E; ++e) w[e] = fmax(fma(-s, (double)q[e], w[e]), 0.0);
-                    } else {
-                        const int64_t e0 = (int64_t)gone_tokens[g] - row.first(piece);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) w[e] = e0 == e ? 0.0 : w[e];
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < E; ++e) all += w[e];
+            warps(sum_steps<T, CAP>(a, row, probs, nodes.gone, begin + warp * steps * kWarp + lane, steps, refused, refused && o.drawn, scale, w, parts + tid, per));
+            // ---- over the cluster ----
+            if (tid == kWarp - 1) {
+                block_sum[turn & 1] = upto;
+                block_most[turn & 1] = top;
             }
-            if (stage == kStep) {
-                const double upto = warp_scan(all, lane);
-                if (warp_fall(all, upto, target) == lane && warp == 0) {
-                    double at = 0.0;
-                    int found = -1, end = 0;
+            __syncwarp();
+            cluster.sync();
+            double mine = lane < ranks ? *cluster.map_shared_rank(&block_sum[turn & 1], lane) : 0.0, share = 1.0;
+            if (!(o.known & 1)) {
+                const float its = lane < ranks ? *cluster.map_shared_rank(&block_most[turn & 1], lane) : -INFINITY;
+                float most = its;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        at += w[e];
-                        if (w[e] > 0.0) {
-                            end = e;
-                            if (found < 0 && at > target) found = e;
+                for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, off));
+                const double logit = warp_logit64<CAP>(scale, its);
+                whole = warp_logit64<CAP>(scale, most);
+                Scale to = scale;
+                to.from = whole;
+                share = warp_weight(to, logit);            // 0 where there is no finite logit
+                mine *= share;
+                if (heat.greedy) {                 // alone: the likeliest token instead of a draw
+                    if (top == most && top > -INFINITY) {
+                        for (uint32_t i = 0, p = begin + warp * steps * kWarp + lane; i < steps && p < pieces; ++i, p += kWarp) {
+                            float x[E];
+                            R::numbers(row.load(p), x);
+#pragma unroll
+                            for (int e = E - 1; e >= 0; --e)
+                                if (x[e] == top) atomicMin(cluster.map_shared_rank(&likeliest, 0), (uint32_t)(row.first(p) + e));
                         }
                     }
-                    found = found < 0 ? end : found;
-                    out_tokens[o.at] = (int32_t)(row.first(begin + lane) + found);
-                    if (logprobs) {
-                        const float x = number(row.p[row.first(begin + lane) + found]);
-                        logprobs[o.at] = (float)((logit64<CAP>(x, a.softcap) - whole) * heat.k * kLn2 - log(z));
+                }
+            }
+            ++turn;
+            __syncwarp();
+            const double run = warp_scan(mine, lane), s = __shfl_sync(kFullMask, run, ranks - 1);
+            if (stage == kAll) z = s;
+            if (heat.greedy) {
+                cluster.sync();
+                if (rank == 0 && tid == 0) {
+                    out_tokens[o.at] = likeliest == 0xFFFFFFFFu ? 0 : (int32_t)likeliest;
+                    if (logprobs) logprobs[o.at] = z > kNothing ? (float)-log(z) : -INFINITY;
+                }
+                break;
+            }
+            if (stage == kAll && o.refused && (o.drawn || o.what == 2)) {
+                stage = kLeft;
+                continue;
+            }
+            if (o.what == 1) {
+                if (rank == 0 && tid == 0) {       // the thread that walks
+                    walk.z = z;
+                    walk.s = s;
+                    walk.summed = 1;
+                    walk.step = 0;
+                }
+                break;
+            }
+            if (!(s > kNothing)) {
+                if (stage == kLeft) {              // nothing left: from all of it
+                    stage = kAgain;
+                    continue;
+                }
+                if (rank == 0 && tid == 0) {
+                    out_tokens[o.at] = 0;
+                    if (logprobs) logprobs[o.at] = -INFINITY;
+                }
+                break;
+            }
+            target = (double)o.u * s;
+            const uint32_t who = warp_fall(mine, run, target);
+            chosen = who == rank;
+            target /= __shfl_sync(kFullMask, share, who);
+            break;
+        }
+        if (chosen) {
+            // ---- the draw: the warp whose sum the target falls in, its group of steps by the sums that were kept, the step, the lane, the token ----
+            const uint32_t its = warp_fall(part, upto, target);
+            warps(warp * per < steps ? parts[warp * kWalkThreads + its * kWarp + lane] : 0.0);
+            uint32_t group = warp_fall(part, upto, target), count = min(per, steps - group * per);
+            begin += (its * steps + group * per) * kWarp;
+            for (;;) {
+                const uint32_t sub = (count + kWalkWarps - 1) / kWalkWarps, first = min(warp * sub, count), last = min(first + sub, count);
+                const double all = sum_steps<T, CAP>(a, row, probs, nodes.gone, begin + first * kWarp + lane, last - first, refused, refused && o.drawn, scale, w, nullptr, 1);
+                warps(all);
+                group = warp_fall(part, upto, target);
+                begin += group * sub * kWarp;
+                count = min(sub, count - group * sub);
+                if (sub > 1) continue;
+                if (warp == group) {                   // a step of its own
+                    const double lanes = warp_scan(all, lane);
+                    if (warp_fall(all, lanes, target) == lane) {
+                        double at = 0.0;
+                        int found = -1, end = 0;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            at += w[e];
+                            if (w[e] > kNothing) {
+                                end = e;
+                                if (found < 0 && at > target) found = e;
+                            }
+                        }
+                        const int64_t token = row.first(begin + lane) + (found < 0 ? end : found);
+                        out_tokens[o.at] = (int32_t)token;
+                        if (logprobs) logprobs[o.at] = (float)((logit64<CAP>(number(row.p[token]), a.softcap) - whole) * heat.k * kLn2 - log(z));
                     }
                 }
                 break;
             }
-#pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) all += __shfl_xor_sync(kFullMask, all, off);
-            __syncthreads();                           // the sums before these have been read
-            if (lane == 0) warp_part[warp] = all;
-            __syncthreads();
-            const double part = lane < kWalkWarps ? warp_part[lane] : 0.0, upto = warp_scan(part, lane);
-            if (stage != kWithin) {
-                // ---- over the cluster ----
-                if (tid == kWarp - 1) {
-                    block_sum[turn & 1] = upto;
-                    block_most[turn & 1] = top;
-                }
-                __syncwarp();
-                cluster.sync();
-                double mine = lane < ranks ? *cluster.map_shared_rank(&block_sum[turn & 1], lane) : 0.0, scale = 1.0;
-                if (!o.known) {
-                    const float its = lane < ranks ? *cluster.map_shared_rank(&block_most[turn & 1], lane) : -INFINITY;
-                    float most = its;
-#pragma unroll
-                    for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, off));
-                    whole = warp_logit64<CAP>(most, cap, twice, table);
-                    scale = warp_exp2(most > -INFINITY ? warp_logit64<CAP>(its, cap, twice, table) - whole : -INFINITY, k, table);
-                    mine *= scale;
-                    if (heat.greedy) {                 // alone: the likeliest token instead of a draw
-                        if (top == most && top > -INFINITY) {
-                            for (uint32_t i = 0, p = begin + warp * steps * kWarp + lane; i < steps && p < pieces; ++i, p += kWarp) {
-                                float x[E];
-                                R::numbers(row.load(p), x);
-#pragma unroll
-                                for (int e = E - 1; e >= 0; --e)
-                                    if (x[e] == top) atomicMin(cluster.map_shared_rank(&likeliest, 0), (uint32_t)(row.first(p) + e));
-                            }
-                        }
-                    }
-                }
-                ++turn;
-                const double run = warp_scan(mine, lane), s = __shfl_sync(kFullMask, run, ranks - 1);
-                if (stage == kAll) z = s;
-                if (heat.greedy) {
-                    cluster.sync();
-                    if (rank == 0 && tid == 0) {
-                        out_tokens[o.at] = likeliest == 0xFFFFFFFFu ? 0 : (int32_t)likeliest;
-                        if (logprobs) logprobs[o.at] = z > 0.0 ? (float)-log(z) : -INFINITY;
-                    }
-                    break;
-                }
-                if (stage == kAll && o.refused && (o.drawn || o.what == 2)) {
-                    stage = kLeft;
-                    continue;
-                }
-                if (o.what == 1) {
-                    if (rank == 0 && tid == 0) {       // the thread that walks
-                        walk.z = z;
-                        walk.s = s;
-                        walk.summed = 1;
-                        walk.step = 0;
-                    }
-                    break;
-                }
-                if (!(s > 0.0)) {
-                    if (stage == kLeft) {              // nothing left: from all of it
-                        stage = kAgain;
-                        continue;
-                    }
-                    if (rank == 0 && tid == 0) {
-                        out_tokens[o.at] = 0;
-                        if (logprobs) logprobs[o.at] = -INFINITY;
-                    }
-                    break;
-                }
-                target = (double)o.u * s;
-                const uint32_t who = warp_fall(mine, run, target);
-                if (who != rank) break;
-                target /= __shfl_sync(kFullMask, scale, who);
-            }
-            const uint32_t its = warp_fall(part, upto, target);
-            begin += its * sub * kWarp;
-            count = min(sub, count - its * sub);
-            sub = (count + kWalkWarps - 1) / kWalkWarps;
-            stage = count > 1 ? kWithin : kStep;
         }
         if (o.what == 2) break;
     }
@@ -852,12 +1059,18 @@ tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a) {
         const tf_status s = check_launch(ctx, name);
         if (s != TF_OK) return s;
     }
-    uint32_t ranks = 8;
-    while (ranks > 1 && (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count) ranks /= 2;
+    uint32_t ranks = kMostRanks;
+    while (ranks > 1 && (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2) ranks /= 2;
     const size_t smem = a.draft_stride * NodeTable::kBytes;
     static DeviceSmemCache smem_cache;
     const tf_status m = ensure_dynamic_smem(ctx, verify_walk_kernel<T, CAP>, smem_cache, smem);
     if (m != TF_OK) return m;
+    static std::atomic<uint64_t> wide{0};          // devices whose kernel may run in clusters of sixteen
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (ranks > 8 && !(wide.load(std::memory_order_relaxed) & bit)) {
+        TF_CUDA(ctx, cudaFuncSetAttribute(verify_walk_kernel<T, CAP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        wide.fetch_or(bit, std::memory_order_relaxed);
+    }
     TF_CUDA(ctx, launch_pdl_cluster(verify_walk_kernel<T, CAP>, dim3(a.sequences * ranks), dim3(kWalkThreads), smem, st, ranks, a));
     return check_launch(ctx, name);
 }
