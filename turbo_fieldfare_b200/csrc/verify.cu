@@ -389,7 +389,7 @@ struct Scale {
 constexpr double kNothing = 0x1p-900;          // more than a vocabulary of tokens that do not count
 
 // Weights in 64 bits by all lanes of a warp. Capped logits: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps, 1e-13 cap off.
-template <bool CAP, int N>
+template <bool CAP, int N, bool CARE = true>
 __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N], double (&w)[N]) {
     if constexpr (!CAP) {
 #pragma unroll
@@ -418,7 +418,7 @@ __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N]
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = x[e] > s.least ? w[e] : s.lowest;
     }
-    if (s.careful) {
+    if (CARE && s.careful) {
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = fabsf(x[e]) < INFINITY && w[e] >= s.lowest ? w[e] : s.lowest;
     }
@@ -647,82 +647,186 @@ __device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, co
     order = {2, w.node, w.at, w.known, w.summed, w.step, a.probs && w.node < a.probs_nodes, w.refused, t.most[w.node], t.number[0], w.z, w.s};
 }
 
-// What `refused` children leave of the weights of `steps` pieces a warp apart, from `piece` on: their sum, and the weights of the last piece. With `parts`, the sums of
-// every `per` steps go there too, kWalkThreads apart. A function of its own, with all registers for its loop; four elements at a time, so that these do.
+// What the refused children of a node leave of its weights: without q the refused tokens are left out, with q each refusal takes its sum times q.
+struct Refused {
+    int count;
+    bool drawn;
+    const double* gone;        // in shared memory: sums, or (as int32) tokens
+};
+
+// Sums of a lane's pieces, every `per` steps apart in `parts` too (kWalkThreads apart), where that is given.
+struct Tally {
+    double all = 0.0, part = 0.0;
+    double* parts;
+    uint32_t per, until;
+    __device__ __forceinline__ void add(double v) {
+        part += v;
+        if (--until == 0) close();
+    }
+    __device__ __forceinline__ void close() {
+        all += part;
+        if (parts) {
+            *parts = part;
+            parts += kWalkThreads;
+        }
+        part = 0.0;
+        until = per;
+    }
+};
+
+// The weights of one piece, wherever it lies, and their sum.
 template <typename T, bool CAP>
-__device__ __noinline__ double sum_steps(const VerifyArgs& a, const Row<T>& of, const ProbRow<T>& its, const double* gone, uint32_t piece, uint32_t steps, int refused,
-                                         bool drawn, const Scale& by, double (&last)[Row<T>::E], double* parts, uint32_t per) {
-    using R = Row<T>;
+__device__ __noinline__ double one_step(const VerifyArgs& a, const Row<T>& row, const ProbRow<T>& probs, const Refused& r, const Scale& s, uint32_t piece, double (&w)[Row<T>::E]) {
     using P = ProbRow<T>;
-    constexpr int E = R::E;
-    const R row = of;
-    const P probs = its;
-    const Scale s = by;
-    double all = 0.0, part = 0.0, w[E];
-    uint32_t until = per;
-    // the next two steps' logits and probabilities are on their way
-    uint4 next[2] = {steps ? row.load(piece) : R::nothing(), steps > 1 ? row.load(piece + kWarp) : R::nothing()}, next_q[2][P::WORDS] = {};
-    if (drawn) {
-        if (steps) probs.load(a, row, piece, next_q[0]);
-        if (steps > 1) probs.load(a, row, piece + kWarp, next_q[1]);
+    constexpr int E = Row<T>::E;
+    float x[E], q[E];
+    Row<T>::numbers(row.load(piece), x);
+    if (r.drawn) {
+        uint4 raw[P::WORDS] = {};
+        probs.load(a, row, piece, raw);
+        P::numbers(a, raw, q);
     }
+    double all = 0.0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = 0.0;
-#pragma unroll 1
-    for (; steps; --steps, piece += kWarp) {
-        float x[E], q[E];
-        R::numbers(next[0], x);
-        next[0] = next[1];
-        if (steps > 2) next[1] = row.load(piece + 2 * kWarp);
-        if (drawn) {
-            P::numbers(a, next_q[0], q);
+    for (int h = 0; h < E; h += 4) {
+        float some[4];
+        double v[4];
 #pragma unroll
-            for (int i = 0; i < P::WORDS; ++i) next_q[0][i] = next_q[1][i];
-            if (steps > 2) probs.load(a, row, piece + 2 * kWarp, next_q[1]);
-        }
-        double sum[E / 4];
+        for (int e = 0; e < 4; ++e) some[e] = x[h + e];
+        warp_weights<CAP>(s, some, v);
+        for (int g = 0; g < r.count; ++g) {
+            if (r.drawn) {
 #pragma unroll
-        for (int h = 0; h < E; h += 4) {
-            float some[4];
-            double v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) some[e] = x[h + e];
-            warp_weights<CAP>(s, some, v);
-            if (drawn) {
-#pragma unroll 1
-                for (int g = 0; g < refused; ++g) {
-                    const double taken = gone[g];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = positive(fma(-taken, (double)q[h + e], v[e]));
-                }
+                for (int e = 0; e < 4; ++e) v[e] = positive(fma(-r.gone[g], (double)q[h + e], v[e]));
             } else {
-#pragma unroll 1
-                for (int g = 0; g < refused; ++g) {
-                    const int64_t e0 = (int64_t) reinterpret_cast<const int32_t*>(gone)[g] - row.first(piece);
+                const int64_t e0 = (int64_t) reinterpret_cast<const int32_t*>(r.gone)[g] - row.first(piece);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = e0 == h + e ? 0.0 : v[e];
-                }
+                for (int e = 0; e < 4; ++e) v[e] = e0 == h + e ? 0.0 : v[e];
             }
-            sum[h / 4] = (v[0] + v[1]) + (v[2] + v[3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[h + e] = v[e];
         }
-        part += E == 8 ? sum[0] + sum[E / 4 - 1] : sum[0];
-        if (--until == 0) {
-            all += part;
-            if (parts) {
-                *parts = part;
-                parts += kWalkThreads;
-            }
-            part = 0.0;
-            until = per;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            all += v[e];
+            w[h + e] = v[e];
         }
     }
-    all += part;
-    if (parts) *parts = part;                  // what is left, or nothing: there is room for one more
-#pragma unroll
-    for (int e = 0; e < E; ++e) last[e] = w[e];
     return all;
+}
+
+// Where the time goes: `steps` whole pieces from p on, a warp apart, whose weights need no care. Nothing but this in a function, without a branch on what a call fixes: inside of the walk, with the
+// edges' checks, a warp took 1500 clocks a step of eight elements a lane where it takes FIXME here. Q: the type of q, 0 none, else as tf_dtype + 1; EVEN: q's pieces lie at boundaries.
+template <typename T, bool CAP, int Q, bool EVEN>
+__device__ __noinline__ void many_steps(const uint4* p, const void* q_at, uint32_t steps, int32_t first, const Refused& refused, const Scale& by, Tally& tally) {
+    constexpr int E = Row<T>::E, WORDS = Q == 0 ? 1 : Q == TF_FP32 + 1 ? E / 4 : 1;
+    using V = std::conditional_t<Q == TF_FP32 + 1, float, std::conditional_t<Q == TF_FP16 + 1, __half, __nv_bfloat16>>;
+    const Scale s = by;
+    const Refused r = refused;
+    Tally t = tally;
+    const V* q = static_cast<const V*>(q_at);
+    auto load_q = [&](const V* from, uint4 (&w)[WORDS]) {
+        if constexpr (Q == 0) {
+        } else if constexpr (!EVEN) {
+            V v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = from[e];
+            memcpy(w, v, sizeof(v));
+        } else if constexpr (E * sizeof(V) == 8) {
+            memcpy(w, static_cast<const uint2*>(static_cast<const void*>(from)), 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4*>(from)[i];
+        }
+    };
+    // the next two steps' logits and probabilities are on their way
+    uint4 next[2] = {p[0], steps > 1 ? p[kWarp] : p[0]}, next_q[2][WORDS] = {};
+    if constexpr (Q != 0) {
+        load_q(q, next_q[0]);
+        if (steps > 1) load_q(q + E * kWarp, next_q[1]);
+    }
+#pragma unroll 1
+    for (; steps; --steps) {
+        float x[E], u[E];
+        Row<T>::numbers(next[0], x);
+        next[0] = next[1];
+        p += kWarp;
+        if (steps > 2) next[1] = p[kWarp];
+        if constexpr (Q != 0) {
+            V v[E];
+            memcpy(v, next_q[0], sizeof(v));
+#pragma unroll
+            for (int e = 0; e < E; ++e) u[e] = fmaxf(number(v[e]), 0.0f);
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) next_q[0][i] = next_q[1][i];
+            q += E * kWarp;
+            if (steps > 2) load_q(q + E * kWarp, next_q[1]);
+        }
+        constexpr int N = CAP ? 4 : E;             // capped, eight at once take more registers than there are
+        double w[E];
+#pragma unroll
+        for (int h = 0; h < E; h += N) {
+            float some[N];
+            double v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) some[e] = x[h + e];
+            warp_weights<CAP, N, false>(s, some, v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[h + e] = v[e];
+        }
+        if constexpr (Q != 0) {
+#pragma unroll 1
+            for (int g = 0; g < r.count; ++g) {
+                const double taken = r.gone[g];
+#pragma unroll
+                for (int e = 0; e < E; ++e) w[e] = positive(fma(-taken, (double)u[e], w[e]));
+            }
+        } else {
+#pragma unroll 1
+            for (int g = 0; g < r.count; ++g) {
+                const uint32_t at = (uint32_t)(reinterpret_cast<const int32_t*>(r.gone)[g] - first);
+                if (at < E)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) w[e] = at == e ? 0.0 : w[e];
+            }
+            first += E * kWarp;
+        }
+        if constexpr (E == 8) t.add(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+        else t.add((w[0] + w[1]) + (w[2] + w[3]));
+    }
+    tally = t;
+}
+
+// The sum of what is left of the weights of `steps` pieces, a warp apart, from `piece` on, with the sums of every `per` in `parts`: room for one more than there are.
+template <typename T, bool CAP>
+__device__ __forceinline__ double sum_steps(const VerifyArgs& a, const Row<T>& row, const ProbRow<T>& probs, const Refused& r, const Scale& s, uint32_t piece, uint32_t steps,
+                                            double* parts, uint32_t per) {
+    constexpr int E = Row<T>::E;
+    Tally t;
+    t.parts = parts;
+    t.per = t.until = per;
+    const uint32_t piece0 = piece - threadIdx.x % kWarp, end = row.whole0 + row.whole;
+    // steps of whole pieces; a row's first and last ones, and all of a row that needs care, go one by one
+    const uint32_t lo = min(piece0 < row.whole0 || s.careful ? (s.careful ? steps : 1u) : 0u, steps), hi = max(lo, min(end > piece0 ? (end - piece0) / kWarp : 0u, steps));
+    for (uint32_t i = 0; i < steps;) {
+        if (i == lo && hi > lo) {
+            const uint32_t at = piece + lo * kWarp;
+            const uint4* p = row.base + at;
+            const void* q = static_cast<const uint8_t*>(a.probs) + (probs.at + (uint64_t)at * E) * (a.probs_dtype == TF_FP32 ? 4 : 2);
+            const int32_t first = (int32_t)row.first(at);
+            switch (r.drawn ? (int)a.probs_dtype + 1 : 0) {
+                case 0: many_steps<T, CAP, 0, true>(p, q, hi - lo, first, r, s, t); break;
+                case TF_FP32 + 1: probs.even ? many_steps<T, CAP, TF_FP32 + 1, true>(p, q, hi - lo, first, r, s, t) : many_steps<T, CAP, TF_FP32 + 1, false>(p, q, hi - lo, first, r, s, t); break;
+                case TF_FP16 + 1: probs.even ? many_steps<T, CAP, TF_FP16 + 1, true>(p, q, hi - lo, first, r, s, t) : many_steps<T, CAP, TF_FP16 + 1, false>(p, q, hi - lo, first, r, s, t); break;
+                default: probs.even ? many_steps<T, CAP, TF_BF16 + 1, true>(p, q, hi - lo, first, r, s, t) : many_steps<T, CAP, TF_BF16 + 1, false>(p, q, hi - lo, first, r, s, t);
+            }
+            i = hi;
+        } else {
+            double w[E];
+            t.add(piece0 + i * kWarp < row.pieces() ? one_step<T, CAP>(a, row, probs, r, s, piece + i * kWarp, w) : 0.0);
+            ++i;
+        }
+    }
+    t.close();
+    return t.all;
 }
 
 template <typename T, bool CAP>
@@ -904,7 +1008,6 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             upto = warp_scan(part, lane);
         };
         bool chosen = false;                           // this block has the token
-        double w[E];
         for (;;) {
             if (stage == kLeft) {
                 refused = o.refused;
@@ -915,7 +1018,8 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             } else if (stage == kAgain) {
                 refused = 0;
             }
-            warps(sum_steps<T, CAP>(a, row, probs, nodes.gone, begin + warp * steps * kWarp + lane, steps, refused, refused && o.drawn, scale, w, parts + tid, per));
+            const Refused by = {refused, refused && o.drawn, nodes.gone};
+            warps(sum_steps<T, CAP>(a, row, probs, by, scale, begin + warp * steps * kWarp + lane, steps, parts + tid, per));
             // ---- over the cluster ----
             if (tid == kWarp - 1) {
                 block_sum[turn & 1] = upto;
@@ -995,9 +1099,11 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             warps(warp * per < steps ? parts[warp * kWalkThreads + its * kWarp + lane] : 0.0);
             uint32_t group = warp_fall(part, upto, target), count = min(per, steps - group * per);
             begin += (its * steps + group * per) * kWarp;
+            const Refused by = {refused, refused && o.drawn, nodes.gone};
             for (;;) {
                 const uint32_t sub = (count + kWalkWarps - 1) / kWalkWarps, first = min(warp * sub, count), last = min(first + sub, count);
-                const double all = sum_steps<T, CAP>(a, row, probs, nodes.gone, begin + first * kWarp + lane, last - first, refused, refused && o.drawn, scale, w, nullptr, 1);
+                double all = 0.0, w[E];
+                for (uint32_t i = first; i < last; ++i) all += one_step<T, CAP>(a, row, probs, by, scale, begin + i * kWarp + lane, w);
                 warps(all);
                 group = warp_fall(part, upto, target);
                 begin += group * sub * kWarp;
