@@ -179,7 +179,8 @@ __device__ __forceinline__ float capped_near(float x, float inverse) {
 }
 
 // A thread keeps a maximum and a sum of its own over the chunks, so that no block meets at a barrier before the end, and has the next chunk's loads under way
-// while it works on one; the first chunk's before it knows whether the row has children.
+// while it works on one; the first chunk's before it knows whether the row has children. Chunks with a row's edge are done apart. The powers of two bound it beside HBM: sixteen a clock and SM
+// are 4.5e12 a second, what 16-bit logits at the full 6.5 TB/s would ask for is 3.3e12. 200 chains of four, all rows needed: 60 us, 5.2 TB/s.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     pdl_launch_dependents();
@@ -191,15 +192,14 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const R r(a.logits, row * a.stride, a.vocab);
-    const uint32_t pieces = r.pieces(), end = min(pieces, (part + 1) * a.per * STEP);
-    uint32_t piece = part * a.per * STEP + tid;                // of this thread, the first of its chunk
+    const uint32_t pieces = r.pieces(), chunk0 = part * a.per, chunk1 = min(chunk0 + a.per, (pieces + STEP - 1) / STEP);
+    // chunks [full0, full1) have nothing but whole pieces
+    const uint32_t full0 = max(chunk0, r.whole0 ? 1u : 0u), full1 = max(full0, min(chunk1, (r.whole0 + r.whole) / STEP));
+    const uint4* p = r.base + (size_t)full0 * STEP + tid;
     uint4 next[PIECES];
-    auto request = [&] {
+    if (full0 < full1)
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j)
-            if (piece + j * kStatsThreads < end) next[j] = r.load(piece + j * kStatsThreads);
-    };
-    request();
+        for (int j = 0; j < PIECES; ++j) next[j] = p[j * kStatsThreads];
     if (tid == 0) {
         found = best = 0xFFFFFFFFu;
         infinite = 0;
@@ -224,21 +224,10 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
     const float k = heat.k32(), inverse = CAP ? 1.0f / a.softcap : 0.0f;
     float most = -INFINITY, from = -INFINITY, sum = 0.0f;
     uint32_t where = 0;                                        // the chunk of the first largest
-    for (; piece < end; piece += STEP) {
-        uint4 w[PIECES];
-        uint32_t n = 0;
-        float top = -INFINITY;
+    auto take = [&](const uint4 (&w)[PIECES], uint32_t chunk) {
+        float top = R::most(w[0]);
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j)
-            if (piece + j * kStatsThreads < end) {
-                w[j] = next[j];
-                top = fmaxf(top, R::most(w[j]));
-                n = j + 1;
-            }
-        const uint32_t here = piece;
-        piece += STEP;
-        request();
-        piece = here;
+        for (int j = 1; j < PIECES; ++j) top = fmaxf(top, R::most(w[j]));
         if (top == INFINITY) {                                 // does not count
             infinite = 1;
             top = -INFINITY;
@@ -247,8 +236,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
                 float x[E];
                 R::numbers(w[j], x);
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (j < n) top = fmaxf(top, counted(x[e]));
+                for (int e = 0; e < E; ++e) top = fmaxf(top, counted(x[e]));
             }
         }
         if (top > most) {
@@ -256,26 +244,24 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
             sum *= verify_exp2((from - to) * k);               // nothing so far: 0 times 0
             most = top;
             from = to;
-            where = piece;
+            where = chunk;
         }
-        if (most == -INFINITY) continue;
-        float add = 0.0f;
-        bool far = false;
+        if (most == -INFINITY) return;
+        float add = 0.0f, widest = 0.0f;
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j)
-            if (j < n) {
-                float x[E];
-                R::numbers(w[j], x);
+        for (int j = 0; j < PIECES; ++j) {
+            float x[E];
+            R::numbers(w[j], x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if constexpr (CAP) {
-                        far |= !(fabsf(x[e]) <= a.softcap);
-                        x[e] = capped_near(x[e], inverse);
-                    }
-                    add += verify_exp2((x[e] - from) * k);
+            for (int e = 0; e < E; ++e) {
+                if constexpr (CAP) {
+                    widest = fmaxf(widest, fabsf(x[e]));
+                    x[e] = capped_near(x[e], inverse);
                 }
+                add += verify_exp2((x[e] - from) * k);
             }
-        if (far || !(add < INFINITY)) {                        // logits beyond the cap's polynomial, infinities and NaN
+        }
+        if (!(widest <= (CAP ? a.softcap : 0.0f)) || !(add < INFINITY)) {      // logits beyond the cap's polynomial, infinities and NaN
             add = 0.0f;
 #pragma unroll
             for (int j = 0; j < PIECES; ++j) {
@@ -284,11 +270,32 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float c = counted(x[e]);
-                    if (j < n) add += verify_exp2(((CAP ? capped(c, a.softcap) : c) - from) * k);
+                    add += verify_exp2(((CAP ? capped(c, a.softcap) : c) - from) * k);
                 }
             }
         }
         sum += add;
+    };
+    for (uint32_t chunk = chunk0; chunk < chunk1;) {
+        if (chunk == full0 && full0 < full1) {
+#pragma unroll 1
+            for (; chunk < full1; ++chunk) {
+                uint4 w[PIECES];
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j) w[j] = next[j];
+                p += STEP;
+                if (chunk + 1 < full1)
+#pragma unroll
+                    for (int j = 0; j < PIECES; ++j) next[j] = p[j * kStatsThreads];
+                take(w, chunk);
+            }
+        } else {
+            uint4 w[PIECES];
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) w[j] = r.load(chunk * STEP + tid + j * kStatsThreads);
+            take(w, chunk);
+            ++chunk;
+        }
     }
     float top = most;
 #pragma unroll
@@ -301,12 +308,13 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
         sum *= verify_exp2((from - (CAP ? capped(top, a.softcap) : top)) * k);
         if (heat.greedy && most == top) {                      // few threads
             uint32_t at = 0xFFFFFFFFu;
-            for (int j = 0; j < PIECES && where + j * kStatsThreads < end && at == 0xFFFFFFFFu; ++j) {
+            for (int j = 0; j < PIECES && at == 0xFFFFFFFFu; ++j) {
+                const uint32_t piece = where * STEP + tid + j * kStatsThreads;
                 float x[E];
-                R::numbers(r.load(where + j * kStatsThreads), x);
+                R::numbers(r.load(piece), x);
 #pragma unroll
                 for (int e = E - 1; e >= 0; --e)
-                    if (x[e] == top) at = (uint32_t)(r.first(where + j * kStatsThreads) + e);
+                    if (x[e] == top) at = (uint32_t)(r.first(piece) + e);
             }
             atomicMin(&best, at);
         }
@@ -1157,9 +1165,10 @@ tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a) {
     if (a.rows && a.draft_stride > 1) {            // lone rows need none of it
         const bool even = aligned(a.logits, 16) && a.stride % E == 0;          // else a row may begin anywhere in a piece
         a.chunks = (uint32_t)(((uint64_t)a.vocab + (even ? 0 : E - 1) + kChunk - 1) / kChunk);
-        // several chunks a block, as long as that leaves every place on the chip a few blocks
-        const uint64_t all = (uint64_t)a.rows * a.chunks / ((uint64_t)ctx->sm_count * 16);
-        a.per = (uint32_t)(all < 1 ? 1 : all > 4 ? 4 : all);
+        // Several chunks a block, as long as that leaves every place on the chip two blocks: a block's start and end take as long as a chunk or two (200 chains of four: 102 us with
+        // one chunk, 76 with two, 66 with four, 64 with eight; one chain of six, whose blocks would be too few: 29 with one, 31 with eight).
+        const uint64_t all = (uint64_t)a.rows * a.chunks / ((uint64_t)ctx->sm_count * 8);
+        a.per = (uint32_t)(all < 1 ? 1 : all > 8 ? 8 : all);
         a.parts = (a.chunks + a.per - 1) / a.per;
         verify_stats_kernel<T, CAP><<<a.rows * a.parts, kStatsThreads, 0, st>>>(a);
         const tf_status s = check_launch(ctx, name);
