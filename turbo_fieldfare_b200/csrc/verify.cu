@@ -745,6 +745,15 @@ __device__ __noinline__ void many_steps(const uint4* p, const void* q_at, uint32
             for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4*>(from)[i];
         }
     };
+    // The first eight steps towards L2, a line of 128 bytes a lane: where there are no more, all of HBM's latency is met at once. (In the loop it cost more than it brought.)
+    const uint32_t lane = threadIdx.x % kWarp, some = min(steps, 8u);
+    if (lane * 128 < some * kWarp * 16) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(p - lane) + lane * 128));
+    if constexpr (Q != 0) {
+        constexpr uint32_t kBytes = kWarp * E * sizeof(V);
+#pragma unroll
+        for (uint32_t at = 0; at < 8 * kBytes; at += kWarp * 128)
+            if (at + lane * 128 < some * kBytes) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(q - lane * E) + at + lane * 128));
+    }
     // the next two steps' logits and probabilities are on their way
     uint4 next[2] = {p[0], steps > 1 ? p[kWarp] : p[0]}, next_q[2][WORDS] = {};
     if constexpr (Q != 0) {
@@ -970,25 +979,24 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
         if (!(o.known & 1)) {
             top = -INFINITY;
             infinite = false;
-            for (uint32_t i = 0, piece = begin + warp * steps * kWarp + lane; i < steps && piece < pieces; i += 4, piece += 4 * kWarp) {
-                uint4 w[4];
+            constexpr int LOADS = 8;
+            for (uint32_t i = 0, piece = begin + warp * steps * kWarp + lane; i < steps && piece < pieces; i += LOADS, piece += LOADS * kWarp) {
+                uint4 w[LOADS];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i + j < steps && piece + j * kWarp < pieces) w[j] = row.load(piece + j * kWarp);
+                for (int j = 0; j < LOADS; ++j) w[j] = i + j < steps && piece + j * kWarp < pieces ? row.load(piece + j * kWarp) : R::nothing();
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i + j < steps && piece + j * kWarp < pieces) {
-                        float most = R::most(w[j]);
-                        if (most == INFINITY) {            // does not count
-                            float x[E];
-                            R::numbers(w[j], x);
-                            infinite = true;
-                            most = -INFINITY;
+                for (int j = 0; j < LOADS; ++j) {
+                    float most = R::most(w[j]);
+                    if (most == INFINITY) {            // does not count
+                        float x[E];
+                        R::numbers(w[j], x);
+                        infinite = true;
+                        most = -INFINITY;
 #pragma unroll
-                            for (int e = 0; e < E; ++e) most = fmaxf(most, counted(x[e]));
-                        }
-                        top = fmaxf(top, most);
+                        for (int e = 0; e < E; ++e) most = fmaxf(most, counted(x[e]));
                     }
+                    top = fmaxf(top, most);
+                }
             }
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
