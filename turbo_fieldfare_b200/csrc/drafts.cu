@@ -10,6 +10,7 @@ namespace tf {
 
 constexpr uint32_t kErrPlan = 0x7F000054u;         // the arrays of a plan contradict themselves
 constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / kWarp;
+constexpr int kPlanRows = 128;                     // rows of a block of the second launch
 constexpr uint32_t kPlanTokens = 0x7FFFFF00u;      // tokens of a sequence: as far as the attention looks
 
 struct PlanArgs {
@@ -84,13 +85,12 @@ struct PlanSequence {
     static __device__ __forceinline__ uint32_t lesser_u32(uint32_t a, uint32_t b) { return a < b ? a : b; }
 };
 
-// One row of the step: sequence b, node i. `page` entries, contexts and offsets are those that the sums left.
-__device__ __forceinline__ void plan_row(const PlanArgs& a, uint32_t row, uint32_t b, uint32_t i) {
+// One row of the step: sequence b, node i, whose tree is `parents`. Page entries and contexts are those that the sums left.
+__device__ __forceinline__ void plan_row(const PlanArgs& a, uint32_t row, uint32_t b, uint32_t i, const int32_t* parents) {
     const uint32_t context = (uint32_t)a.context_lengths[b], token = context + i;
     uint32_t depth = i;
     if (a.drafted && (a.parents || a.tree_mask)) {
         // ancestors descend, so the words of the mask are done one by one from the node's own down
-        const int32_t* parents = a.parents ? a.parents + (size_t)b * a.draft_stride : nullptr;
         unsigned long long* mask = a.tree_mask ? a.tree_mask + (size_t)row * a.mask_words : nullptr;
         if (mask) {
             if ((i >> 6) >= a.mask_words) *a.error = kErrPlan;
@@ -125,28 +125,29 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, uint32_t row, uint32
     }
 }
 
-// Rows `row`, row + step, ... up to the last sequence's.
-__device__ __forceinline__ void plan_rows(const PlanArgs& a, const int32_t* offsets, uint32_t row, uint32_t step) {
-    const uint32_t all = (uint32_t)offsets[a.sequences];
-    for (; row < all; row += step) {
-        uint32_t lo = 0, hi = a.sequences;         // offsets[lo] <= row < offsets[hi]
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if ((uint32_t)offsets[mid] <= row) lo = mid;
-            else hi = mid;
-        }
-        plan_row(a, row, lo, row - (uint32_t)offsets[lo]);
+// The sequence of a row: offsets[b] <= row < offsets[b + 1].
+__device__ __forceinline__ uint32_t plan_sequence(const PlanArgs& a, const int32_t* offsets, uint32_t row) {
+    uint32_t lo = 0, hi = a.sequences;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if ((uint32_t)offsets[mid] <= row) lo = mid;
+        else hi = mid;
     }
+    return lo;
 }
 
-constexpr uint32_t kPlanHeld = 4095;               // sequences whose offsets are kept in shared memory for the rows
+// Kept in shared memory for the rows, since both are chased: the offsets of so many sequences, and so many nodes' parents.
+constexpr uint32_t kPlanHeld = 2047, kPlanTree = 4096;
 
 template <bool ROWS>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanArgs a) {
     __shared__ PlanScan scan;
     __shared__ uint32_t row_limit, page_limit;
-    __shared__ int32_t held_offsets[ROWS ? kPlanHeld + 1 : 1];
+    __shared__ int32_t held_offsets[ROWS ? kPlanHeld + 1 : 1], held_tree[ROWS ? kPlanTree : 1];
     const uint32_t tid = threadIdx.x, lane = tid % kWarp;
+    const uint64_t nodes = (uint64_t)a.sequences * a.draft_stride;
+    if (ROWS && a.parents && nodes <= kPlanTree)
+        for (uint32_t i = tid; i < nodes; i += kPlanThreads) held_tree[i] = a.parents[i];
     if constexpr (!ROWS) pdl_launch_dependents();  // the rows' launch
     if (tid == 0) row_limit = page_limit = 0xFFFFFFFFu;
     const int32_t stack = *a.free_count;
@@ -245,13 +246,47 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
     if constexpr (ROWS) {
         __syncthreads();
-        plan_rows(a, a.sequences <= kPlanHeld ? held_offsets : a.row_offsets, tid, kPlanThreads);
+        const int32_t *offsets = a.sequences <= kPlanHeld ? held_offsets : a.row_offsets, *trees = a.parents && nodes <= kPlanTree ? held_tree : a.parents;
+        const uint32_t all = (uint32_t)offsets[a.sequences];
+        for (uint32_t row = tid; row < all; row += kPlanThreads) {
+            const uint32_t b = plan_sequence(a, offsets, row);
+            plan_row(a, row, b, row - (uint32_t)offsets[b], trees ? trees + (size_t)b * a.draft_stride : nullptr);
+        }
     }
 }
 
-__global__ void __launch_bounds__(256) plan_rows_kernel(const __grid_constant__ PlanArgs a) {
+__global__ void __launch_bounds__(kPlanRows) plan_rows_kernel(const __grid_constant__ PlanArgs a) {
+    __shared__ int32_t held_offsets[kPlanHeld + 1], held_tree[kPlanTree];
+    const uint32_t tid = threadIdx.x;
     pdl_wait();
-    plan_rows(a, a.row_offsets, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    const int32_t* offsets = a.row_offsets;
+    if (a.sequences <= kPlanHeld) {
+        for (uint32_t i = tid; i <= a.sequences; i += kPlanRows) held_offsets[i] = a.row_offsets[i];
+        offsets = held_offsets;
+    }
+    __syncthreads();
+    const uint32_t all = (uint32_t)offsets[a.sequences];
+    for (uint32_t row0 = blockIdx.x * kPlanRows; row0 < all; row0 += gridDim.x * kPlanRows) {
+        const int32_t* trees = a.parents;
+        uint32_t first = 0;
+        if (a.parents) {                           // the trees of this block's rows
+            first = plan_sequence(a, offsets, row0);
+            const uint32_t last = plan_sequence(a, offsets, min(row0 + kPlanRows, all) - 1);
+            const uint64_t nodes = (uint64_t)(last - first + 1) * a.draft_stride;
+            if (nodes <= kPlanTree) {
+                __syncthreads();                   // those of the rows before have been followed
+                for (uint32_t i = tid; i < nodes; i += kPlanRows) held_tree[i] = a.parents[(size_t)first * a.draft_stride + i];
+                trees = held_tree;
+                __syncthreads();
+            } else {
+                first = 0;
+            }
+        }
+        if (row0 + tid < all) {
+            const uint32_t b = plan_sequence(a, offsets, row0 + tid);
+            plan_row(a, row0 + tid, b, row0 + tid - (uint32_t)offsets[b], trees ? trees + (size_t)(b - first) * a.draft_stride : nullptr);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -410,8 +445,8 @@ tf_status tf_kv_plan(tf_context* ctx, void* stream, const tf_kv_pages* pages, in
     tf::plan_kernel<false><<<1, tf::kPlanThreads, 0, st>>>(a);
     tf_status s = tf::check_launch(ctx, name);
     if (s != TF_OK) return s;
-    const uint32_t blocks = (rows->rows + 255) / 256, most = (uint32_t)ctx->sm_count * 8;
-    TF_CUDA(ctx, tf::launch_pdl(tf::plan_rows_kernel, dim3(blocks < most ? blocks : most), dim3(256), 0, st, a));
+    const uint32_t blocks = (uint32_t)(((uint64_t)rows->rows + tf::kPlanRows - 1) / tf::kPlanRows), most = (uint32_t)ctx->sm_count * 8;
+    TF_CUDA(ctx, tf::launch_pdl(tf::plan_rows_kernel, dim3(blocks < most ? blocks : most), dim3(tf::kPlanRows), 0, st, a));
     return tf::check_launch(ctx, name);
 }
 

@@ -1183,7 +1183,7 @@ tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a) {
         if (s != TF_OK) return s;
     }
     uint32_t ranks = kMostRanks;
-    while (ranks > 1 && (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2) ranks /= 2;
+    while (ranks > 1 && ((uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2 || (uint64_t)a.vocab < (uint64_t)ranks * kWalkThreads * 2 * E)) ranks /= 2;
     const size_t smem = a.draft_stride * NodeTable::kBytes;
     static DeviceSmemCache smem_cache;
     const tf_status m = ensure_dynamic_smem(ctx, verify_walk_kernel<T, CAP>, smem_cache, smem);

@@ -26,6 +26,23 @@ _VALUE = {torch.float16: TF_FP16, torch.bfloat16: TF_BF16, torch.float32: TF_FP3
 _I32 = (torch.int32,)
 
 
+def _is(t, dtype, index: int, shape) -> bool:
+    """The common case in one go: what follows where it is not costs a microsecond a tensor."""
+    try:
+        return t.dtype is dtype and t.get_device() == index and t.shape == shape and t.is_contiguous()
+    except AttributeError:
+        return False
+
+
+def _need(name: str, t, dtype, like, shape) -> int:
+    """Address of a contiguous tensor of a type and shape on the device of `like`."""
+    if not _is(t, dtype, like.get_device(), shape):
+        _check(name, t, like.device, (dtype,), len(shape))
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return t.data_ptr()
+
+
 def _ints(name: str, t, device, dims: int, shape=None):
     _check(name, t, device, _I32, dims)
     if shape is not None and tuple(t.shape) != tuple(shape):
@@ -79,6 +96,7 @@ class KVRows:
             if tree_mask.shape[0] != self.rows or words == 0:
                 raise ValueError(f"tree_mask must be [{self.rows}, words], got {list(tree_mask.shape)}")
         self.row_offsets, self.positions, self.sequences, self.slots, self.tokens, self.tree_mask = row_offsets, positions, sequences, slots, tokens, tree_mask
+        self.sequence_count = row_offsets.shape[0] - 1
         self._c = KVRowsDesc(_ptr(row_offsets), _ptr(positions), _ptr(sequences), _ptr(slots), _ptr(tokens), _ptr(tree_mask), words, self.rows)
         self._ref, self._index = C.byref(self._c), row_offsets.get_device()
 
@@ -89,15 +107,18 @@ class KVRows:
                    tree_mask=torch.zeros(rows, mask_words, dtype=torch.int64, device=device) if mask_words else None)
 
 
-def _drafts(device, sequences: int, tokens, parents, stride: int | None = None) -> Drafts | None:
+def _drafts(like, sequences: int, tokens, parents, stride: int | None = None) -> Drafts | None:
     """``tf_drafts`` over tensors of [sequences, stride]."""
-    for name, t in (("tokens", tokens), ("parents", parents)):
-        if t is not None:
-            if not (isinstance(t, torch.Tensor) and t.dim() == 2):
-                _check(name, t, device, _I32, 2)
-            stride = t.shape[1] if stride is None else stride
-            _ints(name, t, device, 2, (sequences, stride))
-    return None if stride is None else Drafts(_ptr(tokens), _ptr(parents), stride)
+    if stride is None:
+        first = tokens if tokens is not None else parents
+        if first is None:
+            return None
+        if not isinstance(first, torch.Tensor) or first.dim() != 2:
+            _check("tokens" if tokens is not None else "parents", first, like.device, _I32, 2)
+        stride = first.shape[1]
+    shape = (sequences, stride)
+    return Drafts(None if tokens is None else _need("tokens", tokens, torch.int32, like, shape),
+                  None if parents is None else _need("parents", parents, torch.int32, like, shape), stride)
 
 
 class KVPlan:
@@ -112,19 +133,20 @@ class KVPlan:
         ended. ``tokens`` and ``parents`` int32 [sequences, nodes]: the drafted nodes, without parents chains (``nodes`` says how many at most where neither is given
         and ``rows`` has a mask)."""
         ctx, n = self.context, pages.sequences
-        _same_device(ctx, pages, rows)
-        _ints("context_lengths", context_lengths, pages.device, 1, (n,))
-        _ints("new_rows", new_rows, pages.device, 1, (n,))
+        if pages._index != ctx.device or rows._index != ctx.device:
+            _same_device(ctx, pages, rows)
+        like, one, i32 = pages.page_table, (n,), torch.int32
+        context_lengths, new_rows = _need("context_lengths", context_lengths, i32, like, one), _need("new_rows", new_rows, i32, like, one)
         if kept is not None:
-            _ints("kept", kept, pages.device, 1, (n,))
-        if rows.row_offsets.shape[0] != n + 1:
-            raise ValueError(f"{n} sequences, but {rows.row_offsets.shape[0]} row offsets")
+            kept = _need("kept", kept, i32, like, one)
+        if rows.sequence_count != n:
+            raise ValueError(f"{n} sequences, but {rows.sequence_count + 1} row offsets")
         if not 0 <= window < 1 << 31:                          # ctypes would cut it to 32 bits
             raise ValueError("window must be from 0 to 2^31 - 1")
         if nodes is not None and not 0 < nodes < 1 << 31:
             raise ValueError("nodes must be from 1 to 2^31 - 1")
-        drafts = _drafts(pages.device, n, tokens, parents, nodes)
-        ctx.check(ctx.lib.tf_kv_plan(ctx.handle, _stream_of(ctx, stream), pages._ref, context_lengths.data_ptr(), new_rows.data_ptr(), _ptr(kept), window,
+        drafts = _drafts(like, n, tokens, parents, nodes)
+        ctx.check(ctx.lib.tf_kv_plan(ctx.handle, _stream_of(ctx, stream), pages._ref, context_lengths, new_rows, kept, window,
                                      None if drafts is None else C.byref(drafts), rows._ref))
 
 
@@ -168,43 +190,42 @@ class DraftVerification:
         ctx = self.context
         if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _VALUE:
             raise ValueError("logits must be [rows, vocab] of float16, bfloat16 or float32")
-        device, (rows, vocab) = logits.device, logits.shape
+        rows, vocab = logits.shape
         if logits.get_device() != ctx.device:
-            raise ValueError(f"logits are on {device}, the context on cuda:{ctx.device}")
-        if vocab == 0 or vocab > 1 and logits.stride(1) != 1:
+            raise ValueError(f"logits are on {logits.device}, the context on cuda:{ctx.device}")
+        stride, step = logits.stride()
+        if vocab == 0 or vocab > 1 and step != 1:
             raise ValueError("the logits of a row must be next to one another, one at the least")
-        _check("row_offsets", row_offsets, device, _I32, 1)
+        if not _is(row_offsets, torch.int32, ctx.device, (out_tokens.shape[0] + 1,) if isinstance(out_tokens, torch.Tensor) and out_tokens.dim() else ()):
+            _check("row_offsets", row_offsets, logits.device, _I32, 1)
         n = row_offsets.shape[0] - 1
         if n < 0:
             raise ValueError("row_offsets is empty")
         if tokens is None:
             raise ValueError("tokens are needed")
-        drafts = _drafts(device, n, tokens, parents)
-        shape = (n, drafts.stride)
-        _check("uniforms", uniforms, device, (torch.float32,), 2)
-        if tuple(uniforms.shape) != shape:
-            raise ValueError(f"uniforms must be {list(shape)}, got {list(uniforms.shape)}")
-        _ints("out_tokens", out_tokens, device, 2, shape)
-        _ints("out_rows", out_rows, device, 2, shape)
-        _ints("kept", kept, device, 1, (n,))
-        for name, t, want in (("temperatures", temperatures, (n,)), ("logprobs", logprobs, shape)):
-            if t is not None:
-                _check(name, t, device, (torch.float32,), len(want))
-                if tuple(t.shape) != want:
-                    raise ValueError(f"{name} must be {list(want)}, got {list(t.shape)}")
+        drafts = _drafts(logits, n, tokens, parents)
+        shape, one, i32, f32 = (n, drafts.stride), (n,), torch.int32, torch.float32
+        uniforms = _need("uniforms", uniforms, f32, logits, shape)
+        out_tokens, out_rows, kept = _need("out_tokens", out_tokens, i32, logits, shape), _need("out_rows", out_rows, i32, logits, shape), _need("kept", kept, i32, logits, one)
+        if temperatures is not None:
+            temperatures = _need("temperatures", temperatures, f32, logits, one)
+        if logprobs is not None:
+            logprobs = _need("logprobs", logprobs, f32, logits, shape)
         probs = None
         if draft_probs is not None:
-            _check("draft_probs", draft_probs, device, tuple(_VALUE), 3, contiguous=False)
-            if draft_probs.shape[0] != n or draft_probs.shape[2] != vocab:
+            if not isinstance(draft_probs, torch.Tensor) or draft_probs.dim() != 3 or draft_probs.dtype not in _VALUE or draft_probs.get_device() != ctx.device:
+                _check("draft_probs", draft_probs, logits.device, tuple(_VALUE), 3, contiguous=False)
+            have, count, width = draft_probs.shape
+            if have != n or width != vocab:
                 raise ValueError(f"draft_probs must be [{n}, nodes, {vocab}], got {list(draft_probs.shape)}")
-            if vocab > 1 and draft_probs.stride(2) != 1:
+            sequence_stride, node_stride, step = draft_probs.stride()
+            if vocab > 1 and step != 1:
                 raise ValueError("the probabilities of a node must be next to one another")
-            if n and draft_probs.shape[1]:
-                probs = DraftProbs(_ptr(draft_probs), draft_probs.stride(0), draft_probs.stride(1), draft_probs.shape[1], _VALUE[draft_probs.dtype])
+            if n and count:
+                probs = C.byref(DraftProbs(draft_probs.data_ptr(), sequence_stride, node_stride, count, _VALUE[draft_probs.dtype]))
         ctx.check(ctx.lib.tf_verify_drafts(
-            ctx.handle, _stream_of(ctx, stream), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _VALUE[logits.dtype], vocab, row_offsets.data_ptr(), rows, n,
-            C.byref(drafts), uniforms.data_ptr(), None if probs is None else C.byref(probs), _ptr(temperatures), softcap, out_tokens.data_ptr(), out_rows.data_ptr(),
-            kept.data_ptr(), _ptr(logprobs), workspace.handle))
+            ctx.handle, _stream_of(ctx, stream), logits.data_ptr(), stride if rows > 1 else vocab, _VALUE[logits.dtype], vocab, row_offsets.data_ptr(), rows, n,
+            C.byref(drafts), uniforms, probs, temperatures, softcap, out_tokens, out_rows, kept, logprobs, workspace.handle))
 
 
 class KVCacheKeep:
@@ -217,11 +238,16 @@ class KVCacheKeep:
         """``caches``: the layers' caches that share the batch's page table; ``kept_rows`` int32 [sequences, nodes] and ``kept`` int32 [sequences] as
         :class:`DraftVerification` writes them, before the next plan raises the context lengths."""
         ctx = self.context
-        caches = [caches] if isinstance(caches, KVCache) else list(caches)
-        _same_device(ctx, batch, *caches)
-        _check("kept_rows", kept_rows, batch.device, _I32, 2)
-        if kept_rows.shape[0] != batch.sequences:
-            raise ValueError(f"kept_rows has {kept_rows.shape[0]} sequences, the batch {batch.sequences}")
-        _ints("kept", kept, batch.device, 1, (batch.sequences,))
-        ctx.check(ctx.lib.tf_kv_cache_keep(ctx.handle, _stream_of(ctx, stream), (KVCacheDesc * len(caches))(*[c._c for c in caches]), len(caches), batch._ref,
-                                           kept_rows.data_ptr(), kept_rows.shape[1], kept.data_ptr()))
+        if isinstance(caches, KVCache):
+            caches = (caches,)
+        if batch._index != ctx.device or any(c._index != ctx.device for c in caches):
+            _same_device(ctx, batch, *caches)
+        if not isinstance(kept_rows, torch.Tensor) or kept_rows.dim() != 2:
+            _check("kept_rows", kept_rows, batch.device, _I32, 2)
+        have, stride = kept_rows.shape
+        if have != batch.sequences:
+            raise ValueError(f"kept_rows has {have} sequences, the batch {batch.sequences}")
+        like = batch.row_offsets
+        kept_rows, kept = _need("kept_rows", kept_rows, torch.int32, like, (have, stride)), _need("kept", kept, torch.int32, like, (have,))
+        descriptors = caches[0]._ref if len(caches) == 1 else (KVCacheDesc * len(caches))(*[c._c for c in caches])
+        ctx.check(ctx.lib.tf_kv_cache_keep(ctx.handle, _stream_of(ctx, stream), descriptors, len(caches), batch._ref, kept_rows, stride, kept))
