@@ -1001,7 +1001,7 @@ tf_status tf_verify_drafts(tf_context* ctx, void* stream, const void* logits, ui
                            int32_t* out_tokens, int32_t* out_rows, int32_t* kept, float* logprobs, tf_verify_workspace* ws);
 
 /* The cache rows of the kept nodes behind their context: in each of the `cache_count` caches (HOST array of descriptors; the layers that share the batch's page
- * table, all of one page size) token context_lengths[b] + kept_rows[b * kept_stride + i] goes to token context_lengths[b] + i for i < kept[b], codes and planes as they are. The nodes of a
+ * table, all of one page size, each of them once) token context_lengths[b] + kept_rows[b * kept_stride + i] goes to token context_lengths[b] + i for i < kept[b], codes and planes as they are. The nodes of a
  * sequence ascend, as tf_verify_drafts writes them; a node that does not, or is not one of the sequence's rows, ends its sequence's moves (tf_device_status: 0x7F000052). A token whose
  * page is missing is left out (0x7F000051). positions are not used. Sequences must not share the pages that they append to. */
 tf_status tf_kv_cache_keep(tf_context* ctx, void* stream, const tf_kv_cache* caches, uint32_t cache_count, const tf_kv_batch* batch,

@@ -67,9 +67,9 @@ def signed(word):
 def softmax64(x, temperature, cap):
     """Weights of the finite logits relative to the largest (64 bits), and the lowest index of the largest."""
     x = x.double()
+    good = x.isfinite()                                            # of the logits as they are: a cap would make infinities finite
     if cap:
         x = cap * torch.tanh(x / cap)
-    good = x.isfinite()
     if not bool(good.any()):
         return torch.zeros_like(x), 0
     x = torch.where(good, x, torch.full_like(x, -math.inf))

@@ -247,6 +247,46 @@ def test_a_single_token_is_drawn_by_its_number(tf_ctx):
     assert bool((drawn[1:] >= drawn[:-1]).all()) and not bool((drawn % 5 == 0).any()) and len(set(drawn.tolist())) > 30
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.0, 12.0])
+def test_lone_rows(tf_ctx, dtype, cap):
+    """The sampler: greedy and drawn rows side by side, sequences without a row, infinities, ties of the likeliest token in parts that different blocks have."""
+    for vocab in (1, 37, 5000, 70001, 262144):
+        counts = [1, 1, 0, 1, 1, 1, 0, 1]
+        d = Draft(vocab, counts, 1, vocab, dtype=dtype)
+        heat = [0.0, 0.9, 0.0, 0.0, 3.0, math.nan, 1.0, 1.0]
+        d.logits[1, ::3] = -math.inf
+        d.logits[2, :] = 1.5                                       # all the same
+        d.logits[3, vocab // 2:] = math.nan
+        d.logits[5, vocab // 3] = d.logits[5, vocab - 1] = math.inf
+        d.logits[4, [vocab // 5, vocab - 1]] = 40.0
+        d.compare(tf_ctx, temperatures=heat, cap=cap)
+        d.compare(tf_ctx, cap=cap)
+    assert tf_ctx.device_status() == 0
+
+
+def test_more_sequences_than_blocks_of_the_chip(tf_ctx):
+    counts = ([3, 1, 2, 0] * 90)[:350]
+    for probs in (None, torch.float32):
+        d = Draft(7, counts, 3, 3001, probs=probs)
+        d.compare(tf_ctx, temperatures=([1.0, 0.0, 0.8] * 120)[:350])
+
+
+def test_offsets_beyond_32_bits(tf_ctx):
+    """Rows of logits and of probabilities more than 2^32 elements apart."""
+    d = Draft(9, [2], 2, 1500, probs=torch.float16, padded=0)
+    far = (1 << 32) + 24
+    room = torch.empty(far + 1500, dtype=torch.float16, device=DEV)
+    x = room.as_strided((2, 1500), (far, 1))
+    x.copy_(d.logits)
+    q = torch.empty(far + 1500, dtype=torch.float16, device=DEV).as_strided((1, 2, 1500), (7, far, 1))
+    q[:, :1].copy_(d.probs)
+    q[:, 1:] = 0
+    d.compare(tf_ctx, logits=x, probs=q)
+    d.uniforms[:] = 0.9999
+    d.compare(tf_ctx, logits=x, probs=q)
+
+
 @pytest.mark.parametrize("probs", [None, torch.float32])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_tests_at_their_border(tf_ctx, probs, dtype):

@@ -461,6 +461,8 @@ tf_status tf_kv_cache_keep(tf_context* ctx, void* stream, const tf_kv_cache* cac
         if (s != TF_OK) break;
         TF_REQUIRE(ctx, caches[i].page_size == caches[0].page_size, TF_ERR_DIMENSION_MISMATCH, "%s: cache %u has pages of %u tokens, the first of %u", name, i,
                    caches[i].page_size, caches[0].page_size);
+        for (uint32_t j = 0; j < i; ++j)           // two warps would move the same bytes
+            TF_REQUIRE(ctx, caches[j].k_codes != caches[i].k_codes && caches[j].v_codes != caches[i].v_codes, TF_ERR_INVALID_ARGUMENT, "%s: caches %u and %u are the same", name, j, i);
         TF_REQUIRE(ctx, ((uint64_t)batch->sequences * caches[i].kv_heads + tf::kKeepWarps - 1) / tf::kKeepWarps <= 0x7FFFFFFFu, TF_ERR_UNSUPPORTED,
                    "%s: too many sequences for the number of heads", name);
     }

@@ -30,7 +30,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kStatsThreads = 256, kChunk = 8192;          // elements that a block of the first launch takes at a time
-constexpr int kWalkThreads = 256, kWalkWarps = kWalkThreads / kWarp;
+constexpr int kWalkThreads = 256, kWalkWarps = kWalkThreads / kWarp, kGroups = 8;
 constexpr uint32_t kMostNodes = 1024, kMostRanks = 16;       // blocks of a sequence: a cluster beyond eight is to be asked for
 constexpr double kLog2E = 1.4426950408889634074;
 
@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
     extern __shared__ __align__(16) uint8_t dynamic[];
     __shared__ Order orders[2];                    // by turns: one is read while the next is written
     __shared__ Walk walk;
-    __shared__ double block_sum[2], warp_part[kWalkWarps], parts[(kWalkWarps + 1) * kWalkThreads];
+    __shared__ double block_sum[2], warp_part[kWalkWarps], parts[(kGroups + 1) * kWalkThreads];
     __shared__ float block_most[2], warp_most[kWalkWarps];
     __shared__ uint32_t likeliest;
     const cg::cluster_group cluster = cg::this_cluster();
@@ -876,8 +876,8 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
     scale.twice = CAP ? 64.0 * kLog2E / scale.cap : 0.0;
     scale.lowest = -32000.0 / scale.k;
     constexpr double kLn2 = 0.69314718055994530942;
-    // A lone row is drawn from at once by all blocks, whatever there is to know of it.
-    const bool alone = of.n == 1 && (a.draft_stride == 1 || !heat.greedy);
+    // Where sequences have one row, all blocks draw from it at once. (A property of the call: whether blocks meet must not hang on what they read.)
+    const bool alone = a.draft_stride == 1;
     if (tid == 0) {
         walk = {1, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0};
         likeliest = 0xFFFFFFFFu;
@@ -968,11 +968,11 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
         }
 
         // ---- the pieces: a warp's are neighbours, and a block's warps, so that sums run in the order of the tokens ----
-        const R row(a.logits, (of.row0 + (uint64_t)o.node) * a.stride, a.vocab);
-        const uint32_t pieces = row.pieces(), steps = (pieces + ranks * kWalkThreads - 1) / (ranks * kWalkThreads);
+        const R row(a.logits, of.n ? (of.row0 + (uint64_t)o.node) * a.stride : 0, of.n ? a.vocab : 0u);        // alone, there may be none
+        const uint32_t pieces = row.pieces(), steps = max(1u, (pieces + ranks * kWalkThreads - 1) / (ranks * kWalkThreads));
         const P probs(a, b * a.probs_sequence + o.node * a.probs_node, row.lead);
         uint32_t begin = rank * kWalkWarps * steps * kWarp;
-        const uint32_t per = (steps + kWalkWarps - 1) / kWalkWarps;            // steps whose sum is kept for the draw
+        const uint32_t per = (steps + kGroups - 1) / kGroups;  // steps whose sum is kept for the draw
         // A row without a maximum (a leaf: nothing was refused) is summed by every block relative to its own, one meeting less.
         float top = o.most;
         bool infinite = o.known & 2;
@@ -1055,7 +1055,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
                 to.from = whole;
                 share = warp_weight(to, logit);            // 0 where there is no finite logit
                 mine *= share;
-                if (heat.greedy) {                 // alone: the likeliest token instead of a draw
+                if (heat.greedy) {                     // alone: the likeliest token instead of a draw
                     if (top == most && top > -INFINITY) {
                         for (uint32_t i = 0, p = begin + warp * steps * kWarp + lane; i < steps && p < pieces; ++i, p += kWarp) {
                             float x[E];
@@ -1071,9 +1071,9 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             __syncwarp();
             const double run = warp_scan(mine, lane), s = __shfl_sync(kFullMask, run, ranks - 1);
             if (stage == kAll) z = s;
-            if (heat.greedy) {
-                cluster.sync();
-                if (rank == 0 && tid == 0) {
+            if (alone) cluster.sync();                 // the likeliest token has been found
+            if (alone && (heat.greedy || of.n == 0)) {
+                if (rank == 0 && tid == 0 && of.n) {
                     out_tokens[o.at] = likeliest == 0xFFFFFFFFu ? 0 : (int32_t)likeliest;
                     if (logprobs) logprobs[o.at] = z > kNothing ? (float)-log(z) : -INFINITY;
                 }
