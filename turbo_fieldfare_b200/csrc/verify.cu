@@ -108,6 +108,11 @@ struct Row {
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = number(v[e]);
     }
+    // The magnitudes of a piece
+    static __device__ __forceinline__ uint4 magnitudes(uint4 w) {
+        constexpr uint32_t mask = sizeof(T) == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+        return make_uint4(w.x & mask, w.y & mask, w.z & mask, w.w & mask);
+    }
     // The largest, without NaN
     static __device__ __forceinline__ float most(const uint4& w) {
         if constexpr (sizeof(T) == 4) {
@@ -252,12 +257,10 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
         for (int j = 0; j < PIECES; ++j) {
             float x[E];
             R::numbers(w[j], x);
+            if constexpr (CAP) widest = fmaxf(widest, R::most(R::magnitudes(w[j])));
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                if constexpr (CAP) {
-                    widest = fmaxf(widest, fabsf(x[e]));
-                    x[e] = capped_near(x[e], inverse);
-                }
+                if constexpr (CAP) x[e] = capped_near(x[e], inverse);
                 add += verify_exp2((x[e] - from) * k);
             }
         }
@@ -386,7 +389,7 @@ __device__ __forceinline__ int2 power_table(int lane) { return make_int2(__doubl
 
 // From logits to weights, what a row has in common.
 struct Scale {
-    double from, k, cap, twice, lowest;        // the logit of weight 1, 32 log2(e) / T; softcap, 64 log2(e) / softcap; -32000 / k, where a weight is 2^-1000
+    double from, k, cap, twice, inverse, lowest;       // the logit of weight 1, 32 log2(e) / T; softcap, 64 log2(e) / softcap, 1 / softcap; -32000 / k, where a weight is 2^-1000
     float least;               // logits from here down count as that, where the row needs no care
     int2 table;
     bool careful;              // the row holds infinities, or steps of 32 bits that are as large as that
@@ -397,11 +400,29 @@ struct Scale {
 constexpr double kNothing = 0x1p-900;          // more than a vocabulary of tokens that do not count
 
 // Weights in 64 bits by all lanes of a warp. Capped logits: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps, 1e-13 cap off.
-template <bool CAP, int N, bool CARE = true>
+// NEAR: no logit that counts is wider than the cap. Then x P((x / cap)^2), P being tanh(u) / u by its Chebyshev coefficients in u^2 on [0, 1], 1.5e-14 off: half of the instructions.
+template <bool CAP, int N, bool CARE = true, bool NEAR = false>
 __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N], double (&w)[N]) {
     if constexpr (!CAP) {
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = (double)fmaxf(x[e], s.least) - s.from;      // NaN too
+    } else if constexpr (NEAR) {
+        constexpr double c[13] = {0.9999999999999823, -0.3333333333272711, 0.13333333298786137, -0.05396824620692592, 0.021869397540056224, -0.008862596767873559, 0.0035892253083668387,
+                                  -0.0014468841456978221, 0.0005707702734400899, -0.0002097698327657338, 6.496419251345914e-05, -1.4302828371933043e-05, 1.5987624655853251e-06};
+        double z[N], p[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            w[e] = (double)x[e];
+            z[e] = w[e] * s.inverse;
+            z[e] *= z[e];
+            p[e] = c[12];
+        }
+#pragma unroll
+        for (int i = 11; i >= 0; --i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) p[e] = fma(p[e], z[e], c[i]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = fma(w[e], p[e], -s.from);
     } else {
         const float edge = 20.0f * (float)s.cap;                                // tanh is 1 to the last bit from there on
         double y[N];
@@ -764,6 +785,8 @@ __device__ __noinline__ void many_steps(const uint4* p, const void* q_at, uint32
     for (; steps; --steps) {
         float x[E], u[E];
         Row<T>::numbers(next[0], x);
+        // wider than the cap: a whole warp's step the long way
+        const bool far = CAP && __any_sync(kFullMask, Row<T>::most(Row<T>::magnitudes(next[0])) > (float)s.cap);
         next[0] = next[1];
         p += kWarp;
         if (steps > 2) next[1] = p[kWarp];
@@ -785,7 +808,8 @@ __device__ __noinline__ void many_steps(const uint4* p, const void* q_at, uint32
             double v[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) some[e] = x[h + e];
-            warp_weights<CAP, N, false>(s, some, v);
+            if (CAP && far) warp_weights<CAP, N, false>(s, some, v);
+            else warp_weights<CAP, N, false, CAP>(s, some, v);
 #pragma unroll
             for (int e = 0; e < N; ++e) w[h + e] = v[e];
         }
@@ -874,6 +898,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
     scale.k = heat.k * 32.0;
     scale.cap = a.softcap;
     scale.twice = CAP ? 64.0 * kLog2E / scale.cap : 0.0;
+    scale.inverse = CAP ? 1.0 / scale.cap : 0.0;
     scale.lowest = -32000.0 / scale.k;
     constexpr double kLn2 = 0.69314718055994530942;
     // Where sequences have one row, all blocks draw from it at once. (A property of the call: whether blocks meet must not hang on what they read.)
