@@ -20,7 +20,7 @@
 
 struct tf_verify_workspace {
     int device = 0;
-    uint64_t stats = 0, bytes = 0;     // room, in chunks of rows
+    uint64_t room = 0, stats = 0, bytes = 0;   // chunks of rows that calls may have; sums that there is place for
     void* memory = nullptr;
 };
 
@@ -36,8 +36,10 @@ constexpr double kLog2E = 1.4426950408889634074;
 
 // The largest logit of some chunks, the sum of their weights relative to that, and where the largest stands first.
 struct ChunkStat {
-    float most, sum;
+    double sum;
+    float most;
     uint32_t at, infinite;     // infinite: there are +infinities, which count for nothing
+    uint32_t unused;
 };
 
 struct VerifyArgs {
@@ -51,8 +53,9 @@ struct VerifyArgs {
     float* logprobs;
     ChunkStat* stats;
     uint32_t* error;
-    uint32_t vocab, rows, sequences, draft_stride, probs_nodes, probs_dtype, chunks, parts, per;       // a row's chunks are done in parts of `per`
+    uint32_t vocab, rows, sequences, draft_stride, probs_nodes, probs_dtype, chunks, parts, per;       // a row's chunks are done in parts of `per`; exact: pieces of a thread
     float softcap;
+    bool exact;                // all rows have been summed in 64 bits
 };
 
 template <typename T> __device__ __forceinline__ float number(T v);
@@ -127,8 +130,22 @@ struct Row {
     }
 };
 
-// softcap * tanh(x / softcap); tanh(u) = 1 - 2 / (exp(2 u) + 1), which needs no care at either end: 2^x is 0 or infinite there.
+// softcap * tanh(x / softcap) where |x| <= softcap, as x + x z R(z), z = (x / softcap)^2: R is (tanh(u) / u - 1) / u^2 by its Chebyshev coefficients in u^2. 3e-9 of it off, and one rounding of
+// the result. On the arithmetic units, which have room here: with a reciprocal and a second power of two a logit these take as long as everything else together.
+__device__ __forceinline__ float capped_near(float x, float inverse) {
+    const float u = x * inverse, z = u * u;
+    float r = -0.00042374664917588234f;
+    r = fmaf(r, z, 0.0025196776259690523f);
+    r = fmaf(r, z, -0.008229382336139679f);
+    r = fmaf(r, z, 0.021665599197149277f);
+    r = fmaf(r, z, -0.05393609404563904f);
+    r = fmaf(r, z, 0.13333140313625336f);
+    r = fmaf(r, z, -0.3333333134651184f);
+    return fmaf(x, r * z, x);
+}
+// The same of any logit; tanh(u) = 1 - 2 / (exp(2 u) + 1), which needs no care at either end: 2^x is 0 or infinite there.
 __device__ __forceinline__ float capped(float x, float cap) {
+    if (fabsf(x) <= cap) return capped_near(x, 1.0f / cap);
     return x == -INFINITY ? x : cap * (1.0f - __fdividef(2.0f, verify_exp2(x * (float)(2 * kLog2E) / cap) + 1.0f));
 }
 
@@ -168,20 +185,6 @@ __device__ __forceinline__ int32_t parent_of(const VerifyArgs& a, uint32_t b, ui
 // ---------------------------------------------------------------------------
 // maxima and sums of the rows with children
 // ---------------------------------------------------------------------------
-
-// softcap * tanh(x / softcap) where |x| <= softcap, as x P((x / softcap)^2): P is tanh(u) / u by its Chebyshev coefficients in u^2, 1.5e-7 of itself off in 32 bits. On the
-// arithmetic units, which have room here: with a reciprocal and a second power of two a logit these take as long as everything else together.
-__device__ __forceinline__ float capped_near(float x, float inverse) {
-    const float u = x * inverse, z = u * u;
-    float p = 0.0010455535957589746f;
-    p = fmaf(p, z, -0.006217069923877716f);
-    p = fmaf(p, z, 0.020305519923567772f);
-    p = fmaf(p, z, -0.05346517637372017f);
-    p = fmaf(p, z, 0.13325397670269012f);
-    p = fmaf(p, z, -0.33332857489585876f);
-    p = fmaf(p, z, 0.9999999403953552f);
-    return x * p;
-}
 
 // A thread keeps a maximum and a sum of its own over the chunks, so that no block meets at a barrier before the end, and has the next chunk's loads under way
 // while it works on one; the first chunk's before it knows whether the row has children. Chunks with a row's edge are done apart. The powers of two bound it beside HBM: sixteen a clock and SM
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
     if (tid == 0) {
         sum = 0.0f;
         for (int w = 0; w < WARPS; ++w) sum += warp_sum_[w];
-        a.stats[(size_t)row * a.parts + part] = {top, sum, best, infinite};
+        a.stats[(size_t)row * a.parts + part] = {(double)sum, top, best, infinite, 0};
     }
 }
 
@@ -393,6 +396,15 @@ struct Scale {
     float least;               // logits from here down count as that, where the row needs no care
     int2 table;
     bool careful;              // the row holds infinities, or steps of 32 bits that are as large as that
+    template <bool CAP>
+    __device__ __forceinline__ void set(float softcap, double log2e_by_heat, int lane) {
+        table = power_table(lane);
+        k = log2e_by_heat * 32.0;
+        cap = softcap;
+        twice = CAP ? 64.0 * kLog2E / cap : 0.0;
+        inverse = CAP ? 1.0 / cap : 0.0;
+        lowest = -32000.0 / k;
+    }
     // With the row's largest logit, as it is; infinite: there are some that do not count. By all lanes.
     template <bool CAP>
     __device__ __forceinline__ void relative_to(float top, bool infinite);
@@ -480,6 +492,111 @@ __device__ __forceinline__ void Scale::relative_to(float top, bool infinite) {
     } else {
         careful = infinite || bottom < -3.4028234e38 || fabs(from) * 0x1p-22 * k > 320.0;
         least = careful ? -3.4028234e38f : (float)bottom;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// all rows in 64 bits
+// ---------------------------------------------------------------------------
+//
+// Where there are few logits, or one row a sequence: the same sums for every row, in 64 bits, by blocks all over the chip. The walk then needs no sum but those behind
+// a refusal, and a draw no more than a part's logits again. 64-bit arithmetic bounds it: eleven operations a logit (25 capped) at 64 a clock and SM, 1.6e12 logits a second (7e11).
+constexpr int kMostPieces = 8;
+
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(kStatsThreads, 2) verify_sums_kernel(const __grid_constant__ VerifyArgs a) {
+    pdl_launch_dependents();
+    using R = Row<T>;
+    constexpr int E = R::E, WARPS = kStatsThreads / kWarp;
+    __shared__ uint32_t found, best, infinite;
+    __shared__ float warp_most[WARPS];
+    __shared__ double warp_sum_[WARPS];
+    const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const R r(a.logits, row * a.stride, a.vocab);
+    const uint32_t piece = part * a.per * kStatsThreads + tid;
+    uint4 w[kMostPieces];
+#pragma unroll
+    for (int j = 0; j < kMostPieces; ++j) w[j] = (uint32_t)j < a.per ? r.load(piece + j * kStatsThreads) : R::nothing();
+    if (tid == 0) {
+        found = best = 0xFFFFFFFFu;
+        infinite = 0;
+    }
+    __syncthreads();
+    for (uint32_t b = tid; b < a.sequences; b += kStatsThreads) {
+        const Nodes of(a, b, false);
+        if (row >= of.row0 && row - of.row0 < of.n) atomicMin(&found, b);
+    }
+    float most = -INFINITY, widest = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kMostPieces; ++j) {
+        float top = R::most(w[j]);
+        if (CAP && (uint32_t)j < a.per) widest = fmaxf(widest, R::most(R::magnitudes(w[j])));
+        if (top == INFINITY) {
+            infinite = 1;
+            float x[E];
+            R::numbers(w[j], x);
+            top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, counted(x[e]));
+        }
+        most = fmaxf(most, top);
+    }
+    float top = most;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+    if (lane == 0) warp_most[warp] = top;
+    __syncthreads();
+    const uint32_t b = found;
+    if (b == 0xFFFFFFFFu) return;
+    top = lane < WARPS ? warp_most[lane] : -INFINITY;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+    const Heat heat(a, b);
+    Scale scale;
+    scale.set<CAP>(a.softcap, heat.k, lane);
+    scale.relative_to<CAP>(top, infinite);
+    const bool far = CAP && __any_sync(kFullMask, !(widest <= a.softcap));     // masked ones too: a block with them goes the long way
+    double sum = 0.0;
+    if (top > -INFINITY) {
+#pragma unroll
+        for (int j = 0; j < kMostPieces; ++j) {
+            if ((uint32_t)j >= a.per) break;
+            float x[E];
+            R::numbers(w[j], x);
+#pragma unroll
+            for (int h = 0; h < E; h += 4) {
+                float some[4];
+                double v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) some[e] = x[h + e];
+                if (CAP && !far && !scale.careful) warp_weights<CAP, 4, false, CAP>(scale, some, v);
+                else warp_weights<CAP>(scale, some, v);
+                sum += (v[0] + v[1]) + (v[2] + v[3]);
+            }
+        }
+        if (heat.greedy && most == top) {
+            uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+            for (int j = kMostPieces - 1; j >= 0; --j) {
+                float x[E];
+                R::numbers(w[j], x);
+#pragma unroll
+                for (int e = E - 1; e >= 0; --e)
+                    if ((uint32_t)j < a.per && x[e] == top) at = (uint32_t)(r.first(piece + j * kStatsThreads) + e);
+            }
+            atomicMin(&best, at);
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
+    if (lane == 0) warp_sum_[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        sum = 0.0;
+        for (int i = 0; i < WARPS; ++i) sum += warp_sum_[i];
+        a.stats[(size_t)row * a.parts + part] = {sum, top, best, infinite, 0};
     }
 }
 
@@ -655,7 +772,8 @@ __device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, co
             const double z = w.z;
             w.z = t.z[i];
             t.z[i] = z;                                // now what the kept token's weight is a part of
-            w.refused = w.summed = w.step = 0;
+            w.refused = w.step = 0;
+            w.summed = a.exact;
             w.gone = 0.0;
         } else if (!heat.greedy) {
             if (drawn) {
@@ -870,6 +988,14 @@ __device__ __forceinline__ double sum_steps(const VerifyArgs& a, const Row<T>& r
     return t.all;
 }
 
+// The weight of a part of a row whose 64-bit sums these are, relative to s.from; by all lanes.
+template <bool CAP>
+__device__ __forceinline__ double part_weight(const Scale& s, const ChunkStat* stats, uint32_t c, uint32_t parts) {
+    ChunkStat x = {0.0, -INFINITY, 0, 0, 0};
+    if (c < parts) x = stats[c];
+    return x.sum * warp_weight(s, warp_logit64<CAP>(s, x.most));               // 0 where there is no finite logit
+}
+
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
     using R = Row<T>;
@@ -880,12 +1006,10 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
     __shared__ Walk walk;
     __shared__ double block_sum[2], warp_part[kWalkWarps], parts[(kGroups + 1) * kWalkThreads];
     __shared__ float block_most[2], warp_most[kWalkWarps];
-    __shared__ uint32_t likeliest;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const uint32_t rank = cluster.block_rank(), ranks = cluster.num_blocks(), b = blockIdx.x / ranks;
     Scale scale;
-    scale.table = power_table(lane);
     // The first launch waits for what came before it and writes nothing but its sums: all else may be read while it is at work.
     if (a.parts == 0) pdl_wait();
     const Nodes of(a, b, rank == 0 && tid == 0);
@@ -895,20 +1019,11 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
     int32_t* out_tokens = a.out_tokens + (size_t)b * a.draft_stride;
     int32_t* out_rows = a.out_rows + (size_t)b * a.draft_stride;
     float* logprobs = a.logprobs ? a.logprobs + (size_t)b * a.draft_stride : nullptr;
-    scale.k = heat.k * 32.0;
-    scale.cap = a.softcap;
-    scale.twice = CAP ? 64.0 * kLog2E / scale.cap : 0.0;
-    scale.inverse = CAP ? 1.0 / scale.cap : 0.0;
-    scale.lowest = -32000.0 / scale.k;
+    scale.set<CAP>(a.softcap, heat.k, lane);
     constexpr double kLn2 = 0.69314718055994530942;
-    // Where sequences have one row, all blocks draw from it at once. (A property of the call: whether blocks meet must not hang on what they read.)
-    const bool alone = a.draft_stride == 1;
-    if (tid == 0) {
-        walk = {1, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0};
-        likeliest = 0xFFFFFFFFu;
-    }
+    if (tid == 0) walk = {1, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0};
 
-    if (rank == 0 && !alone) {
+    if (rank == 0) {
         for (uint32_t i = tid; i < of.n; i += kWalkThreads) nodes.inner[i] = 0;
         __syncthreads();
         for (uint32_t i = tid; i < of.n; i += kWalkThreads) {
@@ -941,9 +1056,14 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             at = __reduce_min_sync(kFullMask, at);
             const float from = CAP ? capped(all, a.softcap) : all, k32 = heat.k32();
             double sum = 0.0;
-            for (uint32_t c = lane; c < a.parts; c += kWarp) {
-                const ChunkStat x = s[c];
-                if (x.most > -INFINITY) sum += (double)(x.sum * verify_exp2(((CAP ? capped(x.most, a.softcap) : x.most) - from) * k32));
+            if (a.exact) {
+                scale.from = warp_logit64<CAP>(scale, all);
+                for (uint32_t c0 = 0; c0 < a.parts; c0 += kWarp) sum += part_weight<CAP>(scale, s, c0 + lane, a.parts);
+            } else {
+                for (uint32_t c = lane; c < a.parts; c += kWarp) {
+                    const ChunkStat x = s[c];
+                    if (x.most > -INFINITY) sum += (double)((float)x.sum * verify_exp2(((CAP ? capped(x.most, a.softcap) : x.most) - from) * k32));
+                }
             }
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
@@ -952,7 +1072,8 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
                 nodes.z[i] = sum;
                 nodes.best[i] = at == 0xFFFFFFFFu ? 0u : at;
             }
-            if (__any_sync(kFullMask, infinite) && lane == 0) atomicOr(nodes.inner + i, 2);
+            infinite = (__any_sync(kFullMask, infinite) ? 2u : 0u) | (a.exact ? 1u : 0u);
+            if (infinite && lane == 0) atomicOr(nodes.inner + i, (int)infinite);
         }
         __syncthreads();
         for (uint32_t i0 = warp * kWarp; i0 < of.n; i0 += kWalkThreads) {
@@ -968,6 +1089,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
         if (tid == 0 && of.n) {
             walk.z = nodes.z[0];
             walk.known = nodes.inner[0];               // a leaf may have the second bit of another call's row: no matter
+            walk.summed = a.exact;
         }
     } else if (a.parts) {
         pdl_wait();                                    // before anything is written
@@ -975,15 +1097,10 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
     __syncthreads();
 
     for (uint32_t round = 0, turn = 0;; ++round) {
-        Order o = {2, 0, 0, 0, 0, 0, 0, 0, 0.0f, 0.0f, 0.0, 0.0};
-        if (alone) {
-            o.u = uniform(a.uniforms[(size_t)b * a.draft_stride]);
-        } else {
-            if (rank == 0 && tid == 0) walk_on<CAP>(a, of, heat, b, nodes, walk, orders[round & 1], out_tokens, out_rows);
-            __syncwarp();
-            cluster.sync();
-            o = *cluster.map_shared_rank(&orders[round & 1], 0);
-        }
+        if (rank == 0 && tid == 0) walk_on<CAP>(a, of, heat, b, nodes, walk, orders[round & 1], out_tokens, out_rows);
+        __syncwarp();
+        cluster.sync();
+        const Order o = *cluster.map_shared_rank(&orders[round & 1], 0);
         if (o.what == 0) break;
         if (rank != 0) {
             for (int g = tid; g < o.refused; g += kWalkThreads)
@@ -993,8 +1110,8 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
         }
 
         // ---- the pieces: a warp's are neighbours, and a block's warps, so that sums run in the order of the tokens ----
-        const R row(a.logits, of.n ? (of.row0 + (uint64_t)o.node) * a.stride : 0, of.n ? a.vocab : 0u);        // alone, there may be none
-        const uint32_t pieces = row.pieces(), steps = max(1u, (pieces + ranks * kWalkThreads - 1) / (ranks * kWalkThreads));
+        const R row(a.logits, (of.row0 + (uint64_t)o.node) * a.stride, a.vocab);
+        const uint32_t pieces = row.pieces(), steps = (pieces + ranks * kWalkThreads - 1) / (ranks * kWalkThreads);
         const P probs(a, b * a.probs_sequence + o.node * a.probs_node, row.lead);
         uint32_t begin = rank * kWalkWarps * steps * kWarp;
         const uint32_t per = (steps + kGroups - 1) / kGroups;  // steps whose sum is kept for the draw
@@ -1049,7 +1166,43 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             upto = warp_scan(part, lane);
         };
         bool chosen = false;                           // this block has the token
-        for (;;) {
+        uint32_t count = 0;                            // steps that it is among
+        const bool direct = a.exact && o.what == 2 && o.refused == 0;
+        if (direct) {
+            // ---- from the sums of the first launch, by the first block ----
+            if (rank != 0) break;
+            const ChunkStat* s = a.stats + (size_t)(of.row0 + o.node) * a.parts;
+            if (!(z > kNothing)) {
+                if (tid == 0) {
+                    out_tokens[o.at] = 0;
+                    if (logprobs) logprobs[o.at] = -INFINITY;
+                }
+                break;
+            }
+            target = (double)o.u * z;
+            uint32_t last = 0;
+            double before = 0.0, of_last = 0.0;
+            bool hit = false;
+            for (uint32_t c0 = 0; c0 < a.parts && !hit; c0 += kWarp) {
+                const double mine = part_weight<CAP>(scale, s, c0 + lane, a.parts), run = before + warp_scan(mine, lane);
+                const uint32_t any = __ballot_sync(kFullMask, mine > kNothing), over = __ballot_sync(kFullMask, mine > kNothing && run > target);
+                hit = over != 0;
+                if (any) {                             // behind the last one that has anything: its last token
+                    const uint32_t who = hit ? __ffs(over) - 1 : 31 - __clz(any);
+                    last = c0 + who;
+                    of_last = __shfl_sync(kFullMask, run - mine, who);
+                }
+                before = __shfl_sync(kFullMask, run, kWarp - 1);
+            }
+            const ChunkStat chunk = s[last];
+            const double share = warp_weight(scale, warp_logit64<CAP>(scale, chunk.most));
+            target = hit ? (target - of_last) / share : INFINITY;
+            scale.relative_to<CAP>(chunk.most, chunk.infinite);
+            chosen = true;
+            begin = last * a.per * kStatsThreads;
+            count = a.per * (kStatsThreads / kWarp);
+        }
+        while (!direct) {
             if (stage == kLeft) {
                 refused = o.refused;
                 if (o.drawn && o.step) {
@@ -1080,30 +1233,11 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
                 to.from = whole;
                 share = warp_weight(to, logit);            // 0 where there is no finite logit
                 mine *= share;
-                if (heat.greedy) {                     // alone: the likeliest token instead of a draw
-                    if (top == most && top > -INFINITY) {
-                        for (uint32_t i = 0, p = begin + warp * steps * kWarp + lane; i < steps && p < pieces; ++i, p += kWarp) {
-                            float x[E];
-                            R::numbers(row.load(p), x);
-#pragma unroll
-                            for (int e = E - 1; e >= 0; --e)
-                                if (x[e] == top) atomicMin(cluster.map_shared_rank(&likeliest, 0), (uint32_t)(row.first(p) + e));
-                        }
-                    }
-                }
             }
             ++turn;
             __syncwarp();
             const double run = warp_scan(mine, lane), s = __shfl_sync(kFullMask, run, ranks - 1);
             if (stage == kAll) z = s;
-            if (alone) cluster.sync();                 // the likeliest token has been found
-            if (alone && (heat.greedy || of.n == 0)) {
-                if (rank == 0 && tid == 0 && of.n) {
-                    out_tokens[o.at] = likeliest == 0xFFFFFFFFu ? 0 : (int32_t)likeliest;
-                    if (logprobs) logprobs[o.at] = z > kNothing ? (float)-log(z) : -INFINITY;
-                }
-                break;
-            }
             if (stage == kAll && o.refused && (o.drawn || o.what == 2)) {
                 stage = kLeft;
                 continue;
@@ -1136,15 +1270,20 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
         }
         if (chosen) {
             // ---- the draw: the warp whose sum the target falls in, its group of steps by the sums that were kept, the step, the lane, the token ----
-            const uint32_t its = warp_fall(part, upto, target);
-            warps(warp * per < steps ? parts[warp * kWalkThreads + its * kWarp + lane] : 0.0);
-            uint32_t group = warp_fall(part, upto, target), count = min(per, steps - group * per);
-            begin += (its * steps + group * per) * kWarp;
+            uint32_t group;
+            if (!direct) {
+                const uint32_t its = warp_fall(part, upto, target);
+                warps(warp * per < steps ? parts[warp * kWalkThreads + its * kWarp + lane] : 0.0);
+                group = warp_fall(part, upto, target);
+                count = min(per, steps - group * per);
+                begin += (its * steps + group * per) * kWarp;
+            }
             const Refused by = {refused, refused && o.drawn, nodes.gone};
             for (;;) {
                 const uint32_t sub = (count + kWalkWarps - 1) / kWalkWarps, first = min(warp * sub, count), last = min(first + sub, count);
                 double all = 0.0, w[E];
-                for (uint32_t i = first; i < last; ++i) all += one_step<T, CAP>(a, row, probs, by, scale, begin + i * kWarp + lane, w);
+                if (sub > 2) all = sum_steps<T, CAP>(a, row, probs, by, scale, begin + first * kWarp + lane, last - first, nullptr, 1);
+                else for (uint32_t i = first; i < last; ++i) all += one_step<T, CAP>(a, row, probs, by, scale, begin + i * kWarp + lane, w);
                 warps(all);
                 group = warp_fall(part, upto, target);
                 begin += group * sub * kWarp;
@@ -1178,7 +1317,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
         const uint32_t tokens = of.n ? walk.at + 1 : 0;
         for (uint32_t i = tid; i < a.draft_stride; i += kWalkThreads) {
             if (i == 0) out_rows[0] = of.n ? 0 : -1;
-            if (logprobs && !alone && i < of.n && nodes.inner[i] < 0)
+            if (logprobs && i < of.n && nodes.inner[i] < 0)
                 logprobs[-1 - nodes.inner[i]] = (float)(heat.greedy ? -log(nodes.z[i]) : log(nodes.weight[i] / nodes.z[i]));
             if (i < tokens) continue;
             out_tokens[i] = -1;
@@ -1192,23 +1331,37 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
 }
 
 template <typename T, bool CAP>
-tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a) {
+tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a, uint64_t room) {
     const char* name = "tf_verify_drafts";
     constexpr uint32_t E = Row<T>::E;
-    if (a.rows && a.draft_stride > 1) {            // lone rows need none of it
+    uint32_t ranks = kMostRanks;
+    // All rows in 64 bits (us a call, beside the 32-bit sums): 6 rows of 262144 logits 19, beside 23, 16 rows 36, beside 38, 32 rows 38, beside 39, but 270 rows of 32000 37, beside 35;
+    // capped 6 rows 37, beside 43, 16 rows 49, beside 53, 32 rows 61, beside 58.
+    a.exact = a.draft_stride == 1 || (uint64_t)a.rows * a.vocab <= (CAP ? 4000000u : 6000000u);
+    if (a.rows) {
         const bool even = aligned(a.logits, 16) && a.stride % E == 0;          // else a row may begin anywhere in a piece
-        a.chunks = (uint32_t)(((uint64_t)a.vocab + (even ? 0 : E - 1) + kChunk - 1) / kChunk);
-        // Several chunks a block, as long as that leaves every place on the chip two blocks: a block's start and end take as long as a chunk or two (200 chains of four: 102 us with
-        // one chunk, 76 with two, 66 with four, 64 with eight; one chain of six, whose blocks would be too few: 29 with one, 31 with eight).
-        const uint64_t all = (uint64_t)a.rows * a.chunks / ((uint64_t)ctx->sm_count * 8);
-        a.per = (uint32_t)(all < 1 ? 1 : all > 8 ? 8 : all);
-        a.parts = (a.chunks + a.per - 1) / a.per;
-        verify_stats_kernel<T, CAP><<<a.rows * a.parts, kStatsThreads, 0, st>>>(a);
+        if (a.exact) {
+            // Pieces of a thread: as many as leave every place on the chip a block, but no more than 64 parts of a row, which the walk goes through 32 at a time (128 where a logit
+            // takes twice as long), and as the workspace needs.
+            const uint64_t pieces = ((uint64_t)a.vocab + (even ? 0 : E - 1) + E - 1) / E;
+            auto parts = [&](uint32_t per) { return (pieces + (uint64_t)kStatsThreads * per - 1) / ((uint64_t)kStatsThreads * per); };
+            a.per = kMostPieces;
+            while (a.per > 1 && a.rows * parts(a.per) < (uint64_t)ctx->sm_count * 2 && parts(a.per / 2) <= (CAP ? 128 : 64) && a.rows * parts(a.per / 2) <= room) a.per /= 2;
+            a.parts = (uint32_t)parts(a.per);
+            verify_sums_kernel<T, CAP><<<(uint32_t)(a.rows * (uint64_t)a.parts), kStatsThreads, 0, st>>>(a);
+        } else {
+            a.chunks = (uint32_t)(((uint64_t)a.vocab + (even ? 0 : E - 1) + kChunk - 1) / kChunk);
+            // Several chunks a block, as long as that leaves every place on the chip two blocks: a block's start and end take as long as a chunk or two (200 chains of four: 102 us
+            // with one chunk, 76 with two, 66 with four, 64 with eight).
+            const uint64_t all = (uint64_t)a.rows * a.chunks / ((uint64_t)ctx->sm_count * 8);
+            a.per = (uint32_t)(all < 1 ? 1 : all > 8 ? 8 : all);
+            a.parts = (a.chunks + a.per - 1) / a.per;
+            verify_stats_kernel<T, CAP><<<a.rows * a.parts, kStatsThreads, 0, st>>>(a);
+        }
         const tf_status s = check_launch(ctx, name);
         if (s != TF_OK) return s;
     }
-    uint32_t ranks = kMostRanks;
-    while (ranks > 1 && ((uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2 || (uint64_t)a.vocab < (uint64_t)ranks * kWalkThreads * 2 * E)) ranks /= 2;
+    while (ranks > 1 && (a.draft_stride == 1 || (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2 || (uint64_t)a.vocab < (uint64_t)ranks * kWalkThreads * 2 * E)) ranks /= 2;
     const size_t smem = a.draft_stride * NodeTable::kBytes;
     static DeviceSmemCache smem_cache;
     const tf_status m = ensure_dynamic_smem(ctx, verify_walk_kernel<T, CAP>, smem_cache, smem);
@@ -1237,7 +1390,8 @@ tf_status tf_verify_workspace_create(tf_context* ctx, uint32_t max_rows, uint32_
     tf_verify_workspace* ws = new (std::nothrow) tf_verify_workspace();
     TF_REQUIRE(ctx, ws != nullptr, TF_ERR_OUT_OF_MEMORY, "%s: out of host memory", name);
     ws->device = ctx->device;
-    ws->stats = (uint64_t)max_rows * (((uint64_t)max_vocab + 7 + tf::kChunk - 1) / tf::kChunk);
+    ws->room = (uint64_t)max_rows * (((uint64_t)max_vocab + 7 + tf::kChunk - 1) / tf::kChunk);
+    ws->stats = ws->room + (uint64_t)ctx->sm_count * 512;      // more where there are few rows, in smaller parts
     ws->bytes = ws->stats * sizeof(tf::ChunkStat);
     const cudaError_t e = cudaMalloc(&ws->memory, ws->bytes);
     if (e != cudaSuccess) {
@@ -1281,8 +1435,8 @@ tf_status tf_verify_drafts(tf_context* ctx, void* stream, const void* logits, ui
                         tf::aligned(out_tokens, 4) && tf::aligned(out_rows, 4) && tf::aligned(kept, 4) && tf::aligned(logprobs, 4) && tf::aligned(drafts->tokens, 4) &&
                         tf::aligned(drafts->parents, 4), TF_ERR_ALIGNMENT, "%s: arrays must be aligned to their elements", name);
     const uint64_t chunks = ((uint64_t)vocab + 7 + tf::kChunk - 1) / tf::kChunk;
-    TF_REQUIRE(ctx, rows * chunks <= ws->stats, TF_ERR_SCRATCH_TOO_SMALL, "%s: the workspace has room for %llu chunks of rows, not %llu", name,
-               (unsigned long long)ws->stats, (unsigned long long)(rows * chunks));
+    TF_REQUIRE(ctx, rows * chunks <= ws->room, TF_ERR_SCRATCH_TOO_SMALL, "%s: the workspace has room for %llu chunks of rows, not %llu", name,
+               (unsigned long long)ws->room, (unsigned long long)(rows * chunks));
     TF_REQUIRE(ctx, rows * chunks <= 0x7FFFFFFFu, TF_ERR_UNSUPPORTED, "%s: too many rows for the vocabulary", name);
     tf::VerifyArgs a = {};
     if (probs && probs->nodes) {
@@ -1304,9 +1458,9 @@ tf_status tf_verify_drafts(tf_context* ctx, void* stream, const void* logits, ui
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool cap = softcap > 0.0f;
     switch (logits_dtype) {
-        case TF_FP16: return cap ? tf::launch_verify<__half, true>(ctx, st, a) : tf::launch_verify<__half, false>(ctx, st, a);
-        case TF_BF16: return cap ? tf::launch_verify<__nv_bfloat16, true>(ctx, st, a) : tf::launch_verify<__nv_bfloat16, false>(ctx, st, a);
-        default: return cap ? tf::launch_verify<float, true>(ctx, st, a) : tf::launch_verify<float, false>(ctx, st, a);
+        case TF_FP16: return cap ? tf::launch_verify<__half, true>(ctx, st, a, ws->stats) : tf::launch_verify<__half, false>(ctx, st, a, ws->stats);
+        case TF_BF16: return cap ? tf::launch_verify<__nv_bfloat16, true>(ctx, st, a, ws->stats) : tf::launch_verify<__nv_bfloat16, false>(ctx, st, a, ws->stats);
+        default: return cap ? tf::launch_verify<float, true>(ctx, st, a, ws->stats) : tf::launch_verify<float, false>(ctx, st, a, ws->stats);
     }
 }
 
