@@ -268,6 +268,73 @@ private:
     const Context& c_;
 };
 
+// Around the layers of a batched step with drafted tokens (Runtime/Generation/RawCompletion.swift:81-246 does this for one sequence on the CPU).
+// Rows and pages of the step from its request lengths.
+class KVPlan {
+public:
+    explicit KVPlan(const Context& c) : c_(c) {}
+    void encode(void* stream, const tf_kv_pages& pages, int32_t* contextLengths, const int32_t* newRows, const tf_kv_rows& rows, const int32_t* kept = nullptr,
+                uint32_t window = 0, const tf_drafts* drafts = nullptr) const {
+        c_.check(tf_kv_plan(c_.handle(), stream, &pages, contextLengths, newRows, kept, window, drafts, &rows));
+    }
+private:
+    const Context& c_;
+};
+
+// Scratch of DraftVerification; serves one call at a time.
+class VerificationWorkspace {
+public:
+    VerificationWorkspace(const Context& c, uint32_t rows, uint32_t vocab) { c.check(tf_verify_workspace_create(c.handle(), rows, vocab, &w_)); }
+    ~VerificationWorkspace() { tf_verify_workspace_destroy(w_); }
+    VerificationWorkspace(const VerificationWorkspace&) = delete;
+    VerificationWorkspace& operator=(const VerificationWorkspace&) = delete;
+    tf_verify_workspace* handle() const { return w_; }
+    uint64_t bytes() const { return tf_verify_workspace_bytes(w_); }
+private:
+    tf_verify_workspace* w_ = nullptr;
+};
+
+// Rows of logits, `stride` elements apart.
+struct LogitsRef {
+    const void* rows = nullptr;
+    uint64_t stride = 0;
+    tf_dtype type = TF_FP16;
+    uint32_t vocab = 0;
+};
+// Where a verification writes: tokens, rows and logarithms (or null) [sequences][nodes], kept [sequences].
+struct VerifiedRef {
+    int32_t* tokens = nullptr;
+    int32_t* rows = nullptr;
+    int32_t* kept = nullptr;
+    float* logprobs = nullptr;
+};
+
+// Which drafted tokens are kept and what comes next; with one node per sequence the sampler (Metal/Sampling/logit.metal:184,490).
+class DraftVerification {
+public:
+    explicit DraftVerification(const Context& c) : c_(c) {}
+    void encode(void* stream, LogitsRef logits, const int32_t* rowOffsets, uint32_t rows, uint32_t sequences, const tf_drafts& drafts, const float* uniforms,
+                VerifiedRef out, const VerificationWorkspace& workspace, const tf_draft_probs* probs = nullptr, const float* temperatures = nullptr,
+                float softcap = 0.0f) const {
+        c_.check(tf_verify_drafts(c_.handle(), stream, logits.rows, logits.stride, logits.type, logits.vocab, rowOffsets, rows, sequences, &drafts, uniforms,
+                                  probs, temperatures, softcap, out.tokens, out.rows, out.kept, out.logprobs, workspace.handle()));
+    }
+private:
+    const Context& c_;
+};
+
+// The cache rows of the kept nodes behind their context, in all layers' caches at once.
+class KVCacheKeep {
+public:
+    explicit KVCacheKeep(const Context& c) : c_(c) {}
+    void encode(void* stream, const tf_kv_cache* caches, uint32_t cacheCount, const tf_kv_batch& batch, const int32_t* keptRows, uint32_t keptStride,
+                const int32_t* kept) const {
+        c_.check(tf_kv_cache_keep(c_.handle(), stream, caches, cacheCount, &batch, keptRows, keptStride, kept));
+    }
+private:
+    const Context& c_;
+};
+
 // ManifestReader + PackedExpertsLayoutReader + ResidentIndexReader in one handle
 // (Infrastructure/ModelIO/ManifestReader.swift:64-152, PackedExpertsLayout.swift:57-119, ResidentIndex.swift:44-140):
 // opening validates the three documents the way the Swift codecs do; ModelError / GTurboFormatError become Error

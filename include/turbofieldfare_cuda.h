@@ -963,8 +963,8 @@ typedef struct tf_kv_rows {
 tf_status tf_kv_plan(tf_context* ctx, void* stream, const tf_kv_pages* pages, int32_t* context_lengths, const int32_t* new_rows, const int32_t* kept,
                      uint32_t window, const tf_drafts* drafts, const tf_kv_rows* rows);
 
-/* Scratch of tf_verify_drafts for up to max_rows rows of up to max_vocab logits (rows * vocab of a call may be at most their product). It serves one call at
- * a time, like tf_attention_workspace; what a call leaves in it does not matter to the next. */
+/* Scratch of tf_verify_drafts for up to max_rows rows of up to max_vocab logits. A call may have more rows of a smaller vocabulary, or the other way round, as long as
+ * rows * ceil((vocab + 7) / 8192) is no more than with these two (else TF_ERR_SCRATCH_TOO_SMALL). It serves one call at a time, like tf_attention_workspace; what a call leaves in it does not matter to the next. */
 typedef struct tf_verify_workspace tf_verify_workspace;
 tf_status tf_verify_workspace_create(tf_context* ctx, uint32_t max_rows, uint32_t max_vocab, tf_verify_workspace** out);
 void tf_verify_workspace_destroy(tf_verify_workspace* ws);

@@ -242,3 +242,35 @@ def test_calls_of_the_library_without_a_device(tmp_path):
     assert built.returncode == 0, built.stdout + built.stderr
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and "all fine" in run.stdout, run.stdout + run.stderr
+
+
+CALLER = r"""
+#include "turbofieldfare.hpp"
+namespace tf = turbofieldfare;
+void step(const tf::Context& c, void* stream, tf_kv_pages pages, tf_kv_rows rows, tf_kv_batch batch, tf_kv_cache cache, tf_drafts drafts, int32_t* numbers, float* uniforms,
+          const void* logits, const tf::VerificationWorkspace& workspace) {
+    tf::KVPlan(c).encode(stream, pages, numbers, numbers, rows, numbers, 0, &drafts);
+    tf::DraftVerification(c).encode(stream, {logits, 1000, TF_FP32, 1000}, rows.row_offsets, rows.rows, pages.sequences, drafts, uniforms, {numbers, numbers, numbers}, workspace);
+    tf::KVCacheKeep(c).encode(stream, &cache, 1, batch, numbers, drafts.stride, numbers);
+}
+int main() {
+    try {
+        tf::Context c(0);
+        tf::VerificationWorkspace w(c, 0, 1000);
+        return 2;                                  // no rows: refused
+    } catch (const tf::Error& e) {
+        return e.status == TF_ERR_NO_DEVICE || e.status == TF_ERR_INVALID_ARGUMENT ? 0 : 3;
+    }
+}
+"""
+
+
+def test_the_cpp_classes_compile_and_raise(tmp_path):
+    from turbo_fieldfare_b200 import build as tf_build
+    lib = tf_build.build(verbose=False)
+    src, exe = tmp_path / "caller.cpp", tmp_path / "caller"
+    src.write_text(CALLER)
+    built = subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-I", str(ROOT / "include"), str(src), "-o", str(exe), "-L", str(lib.parent), "-ltfcuda",
+                            f"-Wl,-rpath,{lib.parent}"], capture_output=True, text=True)
+    assert built.returncode == 0, built.stderr
+    assert subprocess.run([str(exe)], timeout=120).returncode == 0

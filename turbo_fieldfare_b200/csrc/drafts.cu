@@ -438,7 +438,9 @@ tf_status tf_kv_plan(tf_context* ctx, void* stream, const tf_kv_pages* pages, in
     a.error = ctx->device_error;
     a.table_stride = pages->page_table_stride; a.num_pages = pages->num_pages; a.page_log2 = tf::log2_of(pages->page_size);
     a.sequences = pages->sequences; a.window = window; a.rows = rows->rows;
-    if (rows->rows <= 2048) {
+    // Few rows: by the block of the sums, one launch (us a call, one launch / two; trees of so many nodes each: 4 x 64 4.5 / 6.4, 64 x 16 6.3 / 6.7, 64 x 32 10.1 / 6.9,
+    // 64 x 128 31 / 6.9; chains 4 x 64 3.7 / 5.2, 1 x 1024 3.8 / 5.1, 64 x 32 5.1 / 5.1, 64 x 128 10.6 / 5.1).
+    if (rows->rows <= 1024) {
         tf::plan_kernel<true><<<1, tf::kPlanThreads, 0, st>>>(a);
         return tf::check_launch(ctx, name);
     }
