@@ -344,20 +344,21 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
 // add less than 2^-17; capped logits are off by at most softcap 2^-20 each.
 __device__ __forceinline__ double sum_bound(float cap, double k) { return 0x1p-15 + (cap > 0.0f ? (double)cap * k * 0x1p-19 : 0.0); }
 
-// y = 2^(y k / 32) in 64 bits by all lanes of a warp: 2^(j/32) from a table that the lanes hold, times the Taylor sum of 2^r, |r| <= 1/64, to its fourth power
-// (1.3e-12 of it; what a sum gathers of that moves a border between tokens by less than 1e-17 of it a token), times a power of two, which goes into the table's number: its upper words are lower by
-// what the last bits of j add there. Exponents from -1010 to 1010. All N at once, so that none waits for the eleven operations in a row.
+// 2^((y k + shift - kShift) / 32) in 64 bits by all lanes of a warp, as base times y: 2^(j/32) from a table that the lanes hold, with a power of two that goes into its number (whose upper words
+// are lower by what the last bits of j add there), and 2^(r/32), |r| <= 1/2, by its Chebyshev sum to the fourth power (8e-14 of it: a border between tokens moves by no more than that of all). The
+// caller's sums multiply: eight operations a logit. shift is kShift, or that less a whole number. Exponents from -1010 to 1010. All N at once, so that none waits for the operations in a row.
+constexpr double kShift = 6755399441055744.0;                                   // 1.5 2^52: the sum's last bits are the rounded number
 template <int N>
-__device__ __forceinline__ void warp_exp2(double (&y)[N], double k, int2 table) {
-    constexpr double shift = 6755399441055744.0;                                // 1.5 2^52: the sum's last bits are the rounded number
-    constexpr double c = 0.69314718055994530942 / 32, taylor[4] = {c, c * c / 2, c * c * c / 6, c * c * c * c / 24};
+__device__ __forceinline__ void warp_exp2(double (&y)[N], double k, double shift, int2 table, double (&base)[N]) {
+    constexpr double c = 0.69314718055994530942 / 32, fifth = c * c * c * c * c / 120;
+    constexpr double poly[4] = {c - fifth * 5 / 256, c * c / 2, c * c * c / 6 + fifth * 5 / 16, c * c * c * c / 24};
     int j[N];
-    double base[N], s[N];
+    double r[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         const double t = fma(y[e], k, shift);
         j[e] = __double2loint(t);
-        y[e] = fma(y[e], k, shift - t);
+        r[e] = fma(y[e], k, shift - t);
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -365,15 +366,20 @@ __device__ __forceinline__ void warp_exp2(double (&y)[N], double k, int2 table) 
         base[e] = __hiloint2double(hi + j[e] * 32768, lo);
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) s[e] = taylor[3];
+    for (int e = 0; e < N; ++e) y[e] = poly[3];
 #pragma unroll
     for (int i = 2; i >= 0; --i)
 #pragma unroll
-        for (int e = 0; e < N; ++e) s[e] = fma(s[e], y[e], taylor[i]);
+        for (int e = 0; e < N; ++e) y[e] = fma(y[e], r[e], poly[i]);
 #pragma unroll
-    for (int e = 0; e < N; ++e) s[e] *= y[e];
+    for (int e = 0; e < N; ++e) y[e] = fma(y[e], r[e], 1.0);
+}
+template <int N>
+__device__ __forceinline__ void warp_exp2(double (&y)[N], double k, int2 table) {
+    double base[N];
+    warp_exp2(y, k, kShift, table, base);
 #pragma unroll
-    for (int e = 0; e < N; ++e) y[e] = fma(base[e], s[e], base[e]);
+    for (int e = 0; e < N; ++e) y[e] *= base[e];
 }
 __device__ __forceinline__ double positive(double v) { return __double2hiint(v) < 0 ? 0.0 : v; }
 
@@ -393,7 +399,9 @@ __device__ __forceinline__ int2 power_table(int lane) { return make_int2(__doubl
 
 // From logits to weights, what a row has in common.
 struct Scale {
-    double from, k, cap, twice, inverse, lowest;       // the logit of weight 1, 32 log2(e) / T; softcap, 64 log2(e) / softcap, 1 / softcap; -32000 / k, where a weight is 2^-1000
+    double from, k, shift;     // the logit of weight 1, 32 log2(e) / T; kShift - from k
+    double cap, twice, inverse;        // softcap, 64 log2(e) / softcap, 1 / softcap
+    double lowest;             // -32000 / k: that far below a weight is 2^-1000
     float least;               // logits from here down count as that, where the row needs no care
     int2 table;
     bool careful;              // the row holds infinities, or steps of 32 bits that are as large as that
@@ -406,6 +414,11 @@ struct Scale {
         inverse = CAP ? 1.0 / cap : 0.0;
         lowest = -32000.0 / k;
     }
+    // What the weights of a row with such a logit are relative to: one nearby that k makes a whole number.
+    __device__ __forceinline__ double unit(double logit) const {
+        const double by = logit * k;
+        return fabs(by) < 0x1p40 ? rint(by) * (lowest * (-1.0 / 32000.0)) : logit;
+    }
     // With the row's largest logit, as it is; infinite: there are some that do not count. By all lanes.
     template <bool CAP>
     __device__ __forceinline__ void relative_to(float top, bool infinite);
@@ -413,12 +426,12 @@ struct Scale {
 constexpr double kNothing = 0x1p-900;          // more than a vocabulary of tokens that do not count
 
 // Weights in 64 bits by all lanes of a warp. Capped logits: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps, 1e-13 cap off.
-// NEAR: no logit that counts is wider than the cap. Then x P((x / cap)^2), P being tanh(u) / u by its Chebyshev coefficients in u^2 on [0, 1], 1.5e-14 off: half of the instructions.
+// They come as products base w, which sums multiply. NEAR: no logit that counts is wider than the cap. Then x P((x / cap)^2), P being tanh(u) / u by its Chebyshev coefficients in u^2 on [0, 1], 1.5e-14 off: half of the instructions.
 template <bool CAP, int N, bool CARE = true, bool NEAR = false>
-__device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N], double (&w)[N]) {
+__device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N], double (&w)[N], double (&base)[N]) {
     if constexpr (!CAP) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = (double)fmaxf(x[e], s.least) - s.from;      // NaN too
+        for (int e = 0; e < N; ++e) w[e] = (double)fmaxf(x[e], s.least);       // NaN too
     } else if constexpr (NEAR) {
         constexpr double c[13] = {0.9999999999999823, -0.3333333333272711, 0.13333333298786137, -0.05396824620692592, 0.021869397540056224, -0.008862596767873559, 0.0035892253083668387,
                                   -0.0014468841456978221, 0.0005707702734400899, -0.0002097698327657338, 6.496419251345914e-05, -1.4302828371933043e-05, 1.5987624655853251e-06};
@@ -435,7 +448,7 @@ __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N]
 #pragma unroll
             for (int e = 0; e < N; ++e) p[e] = fma(p[e], z[e], c[i]);
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = fma(w[e], p[e], -s.from);
+        for (int e = 0; e < N; ++e) w[e] *= p[e];
     } else {
         const float edge = 20.0f * (float)s.cap;                                // tanh is 1 to the last bit from there on
         double y[N];
@@ -454,17 +467,22 @@ __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N]
 #pragma unroll
         for (int e = 0; e < N; ++e) y[e] = fma(y[e], w[e], y[e]);
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = fma(-2.0 * s.cap, y[e], s.cap - s.from);
+        for (int e = 0; e < N; ++e) w[e] = fma(-2.0 * s.cap, y[e], s.cap);
     }
     if constexpr (CAP) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = x[e] > s.least ? w[e] : s.lowest;
+        for (int e = 0; e < N; ++e) w[e] = x[e] > s.least ? w[e] : s.from + s.lowest;
     }
+    double shift = s.shift;
     if (CARE && s.careful) {
+        shift = kShift;
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = fabsf(x[e]) < INFINITY && w[e] >= s.lowest ? w[e] : s.lowest;
+        for (int e = 0; e < N; ++e) {
+            w[e] -= s.from;
+            w[e] = fabsf(x[e]) < INFINITY && w[e] >= s.lowest ? w[e] : s.lowest;
+        }
     }
-    warp_exp2(w, s.k, s.table);
+    warp_exp2(w, s.k, shift, s.table, base);
 }
 // One logit by all lanes, whatever it is and what the others are.
 template <bool CAP>
@@ -484,7 +502,8 @@ __device__ __forceinline__ double warp_weight(const Scale& s, double logit) {
 }
 template <bool CAP>
 __device__ __forceinline__ void Scale::relative_to(float top, bool infinite) {
-    from = top > -INFINITY ? warp_logit64<CAP>(*this, top) : 0.0;
+    from = top > -INFINITY ? unit(warp_logit64<CAP>(*this, top)) : 0.0;
+    shift = kShift - rint(from * k);                   // exact where no care is needed
     const double bottom = from + lowest;
     if (CAP) {
         // the cap's inverse, cap atanh(bottom / cap); 2^-23 of the cap is the widest step of its logits
@@ -558,7 +577,7 @@ __global__ void __launch_bounds__(kStatsThreads, 2) verify_sums_kernel(const __g
     scale.set<CAP>(a.softcap, heat.k, lane);
     scale.relative_to<CAP>(top, infinite);
     const bool far = CAP && __any_sync(kFullMask, !(widest <= a.softcap));     // masked ones too: a block with them goes the long way
-    double sum = 0.0;
+    double sums[4] = {};
     if (top > -INFINITY) {
 #pragma unroll
         for (int j = 0; j < kMostPieces; ++j) {
@@ -568,12 +587,13 @@ __global__ void __launch_bounds__(kStatsThreads, 2) verify_sums_kernel(const __g
 #pragma unroll
             for (int h = 0; h < E; h += 4) {
                 float some[4];
-                double v[4];
+                double v[4], base[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) some[e] = x[h + e];
-                if (CAP && !far && !scale.careful) warp_weights<CAP, 4, false, CAP>(scale, some, v);
-                else warp_weights<CAP>(scale, some, v);
-                sum += (v[0] + v[1]) + (v[2] + v[3]);
+                if (CAP && !far && !scale.careful) warp_weights<CAP, 4, false, CAP>(scale, some, v, base);
+                else warp_weights<CAP>(scale, some, v, base);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sums[e] = fma(base[e], v[e], sums[e]);
             }
         }
         if (heat.greedy && most == top) {
@@ -590,6 +610,7 @@ __global__ void __launch_bounds__(kStatsThreads, 2) verify_sums_kernel(const __g
         }
     }
     __syncwarp();
+    double sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
     if (lane == 0) warp_sum_[warp] = sum;
@@ -838,10 +859,12 @@ __device__ __noinline__ double one_step(const VerifyArgs& a, const Row<T>& row, 
 #pragma unroll
     for (int h = 0; h < E; h += 4) {
         float some[4];
-        double v[4];
+        double v[4], base[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) some[e] = x[h + e];
-        warp_weights<CAP>(s, some, v);
+        warp_weights<CAP>(s, some, v, base);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= base[e];
         for (int g = 0; g < r.count; ++g) {
             if (r.drawn) {
 #pragma unroll
@@ -894,6 +917,7 @@ __device__ __noinline__ void many_steps(const uint4* p, const void* q_at, uint32
         for (uint32_t at = 0; at < 8 * kBytes; at += kWarp * 128)
             if (at + lane * 128 < some * kBytes) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(q - lane * E) + at + lane * 128));
     }
+    double sums[4] = {};                           // without q: the products' sums so far
     // the next two steps' logits and probabilities are on their way
     uint4 next[2] = {p[0], steps > 1 ? p[kWarp] : p[0]}, next_q[2][WORDS] = {};
     if constexpr (Q != 0) {
@@ -920,38 +944,51 @@ __device__ __noinline__ void many_steps(const uint4* p, const void* q_at, uint32
             if (steps > 2) load_q(q + E * kWarp, next_q[1]);
         }
         constexpr int N = CAP ? 4 : E;             // capped, eight at once take more registers than there are
-        double w[E];
+        double w[E], base[E];
 #pragma unroll
         for (int h = 0; h < E; h += N) {
             float some[N];
-            double v[N];
+            double v[N], its[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) some[e] = x[h + e];
-            if (CAP && far) warp_weights<CAP, N, false>(s, some, v);
-            else warp_weights<CAP, N, false, CAP>(s, some, v);
+            if (CAP && far) warp_weights<CAP, N, false>(s, some, v, its);
+            else warp_weights<CAP, N, false, CAP>(s, some, v, its);
 #pragma unroll
-            for (int e = 0; e < N; ++e) w[h + e] = v[e];
+            for (int e = 0; e < N; ++e) {
+                w[h + e] = v[e];
+                base[h + e] = its[e];
+            }
         }
         if constexpr (Q != 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] *= base[e];
 #pragma unroll 1
             for (int g = 0; g < r.count; ++g) {
                 const double taken = r.gone[g];
 #pragma unroll
                 for (int e = 0; e < E; ++e) w[e] = positive(fma(-taken, (double)u[e], w[e]));
             }
+            if constexpr (E == 8) t.add(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+            else t.add((w[0] + w[1]) + (w[2] + w[3]));
         } else {
 #pragma unroll 1
             for (int g = 0; g < r.count; ++g) {
                 const uint32_t at = (uint32_t)(reinterpret_cast<const int32_t*>(r.gone)[g] - first);
                 if (at < E)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) w[e] = at == e ? 0.0 : w[e];
+                    for (int e = 0; e < E; ++e) base[e] = at == e ? 0.0 : base[e];
             }
             first += E * kWarp;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sums[e % 4] = fma(base[e], w[e], sums[e % 4]);
+            if (--t.until == 0) {
+                t.part += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                sums[0] = sums[1] = sums[2] = sums[3] = 0.0;
+                t.close();
+            }
         }
-        if constexpr (E == 8) t.add(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-        else t.add((w[0] + w[1]) + (w[2] + w[3]));
     }
+    t.part += (sums[0] + sums[1]) + (sums[2] + sums[3]);
     tally = t;
 }
 
@@ -994,7 +1031,7 @@ template <bool CAP>
 __device__ __forceinline__ double part_weight(const Scale& s, const ChunkStat* stats, uint32_t c, uint32_t parts) {
     ChunkStat x = {0.0, -INFINITY, 0, 0, 0};
     if (c < parts) x = stats[c];
-    return x.sum * warp_weight(s, warp_logit64<CAP>(s, x.most));               // 0 where there is no finite logit
+    return x.sum * warp_weight(s, s.unit(warp_logit64<CAP>(s, x.most)));       // 0 where there is no finite logit
 }
 
 template <typename T, bool CAP>
@@ -1057,14 +1094,17 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             at = __reduce_min_sync(kFullMask, at);
             const float from = CAP ? capped(all, a.softcap) : all, k32 = heat.k32();
             double sum = 0.0;
+            // Relative to the unit of the row, but of a greedy sequence to the largest itself, whose weight is what is asked for
+            const double logit = warp_logit64<CAP>(scale, all);
+            scale.from = heat.greedy ? logit : scale.unit(logit);
             if (a.exact) {
-                scale.from = warp_logit64<CAP>(scale, all);
                 for (uint32_t c0 = 0; c0 < a.parts; c0 += kWarp) sum += part_weight<CAP>(scale, s, c0 + lane, a.parts);
             } else {
                 for (uint32_t c = lane; c < a.parts; c += kWarp) {
                     const ChunkStat x = s[c];
                     if (x.most > -INFINITY) sum += (double)((float)x.sum * verify_exp2(((CAP ? capped(x.most, a.softcap) : x.most) - from) * k32));
                 }
+                sum *= warp_weight(scale, logit);
             }
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
@@ -1082,7 +1122,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
             const bool is = i < of.n && nodes.parent[i] >= 0 && nodes.token[i] >= 0;
             const float x = is ? (float)nodes.weight[i] : -INFINITY, top = is ? nodes.most[nodes.parent[i]] : -INFINITY;
             const double l = warp_logit64<CAP>(scale, x);
-            scale.from = warp_logit64<CAP>(scale, top);
+            scale.from = scale.unit(warp_logit64<CAP>(scale, top));
             const double w = warp_weight(scale, l);    // of infinities and NaN: 0
             if (is) nodes.weight[i] = w;
         }
@@ -1196,7 +1236,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
                 before = __shfl_sync(kFullMask, run, kWarp - 1);
             }
             const ChunkStat chunk = s[last];
-            const double share = warp_weight(scale, warp_logit64<CAP>(scale, chunk.most));
+            const double share = warp_weight(scale, scale.unit(warp_logit64<CAP>(scale, chunk.most)));
             target = hit ? (target - of_last) / share : INFINITY;
             scale.relative_to<CAP>(chunk.most, chunk.infinite);
             chosen = true;
@@ -1228,8 +1268,8 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
                 float most = its;
 #pragma unroll
                 for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, off));
-                const double logit = warp_logit64<CAP>(scale, its);
-                whole = warp_logit64<CAP>(scale, most);
+                const double logit = scale.unit(warp_logit64<CAP>(scale, its));
+                whole = scale.unit(warp_logit64<CAP>(scale, most));
                 Scale to = scale;
                 to.from = whole;
                 share = warp_weight(to, logit);            // 0 where there is no finite logit
