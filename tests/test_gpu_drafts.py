@@ -272,6 +272,13 @@ def test_more_sequences_than_blocks_of_the_chip(tf_ctx):
         d.compare(tf_ctx, temperatures=([1.0, 0.0, 0.8] * 120)[:350])
 
 
+@pytest.mark.parametrize("vocab,counts,tree", [(40, [2, 0, 1, 3, 0, 0] * 900, False), (1100, [2] * 3000, False), (300, [0] * 1500 + [4] + [0] * 1500 + [3], True)])
+def test_rows_find_their_sequence_among_many(tf_ctx, vocab, counts, tree):
+    d = Draft(8, counts, 4, vocab, tree=tree)
+    d.compare(tf_ctx, temperatures=([0.9, 0.0, 1.3] * len(counts))[:len(counts)])
+    assert tf_ctx.device_status() == 0
+
+
 def test_offsets_beyond_32_bits(tf_ctx):
     """Rows of logits and of probabilities more than 2^32 elements apart."""
     d = Draft(9, [2], 2, 1500, probs=torch.float16, padded=0)

@@ -176,6 +176,22 @@ struct Nodes {                 // a sequence's rows, cut to what the arrays can 
         if (n > a.draft_stride) n = a.draft_stride;
     }
 };
+// Whose row it is, into `found` (which stays as it is where it is nobody's), by all threads of a block: a block a row must not look through all of many sequences, so from 1024 on it
+// first takes a 256th, in which the last one lies that begins no later. Offsets that contradict themselves find one of those that have the row, or none.
+__device__ __forceinline__ void owner_of(const VerifyArgs& a, uint32_t row, uint32_t* found) {
+    uint32_t lo = 0, n = a.sequences;
+    while (n > 1024) {
+        const uint32_t part = (n + kStatsThreads - 1) / kStatsThreads, at = threadIdx.x * part;
+        const uint32_t before = (uint32_t)__syncthreads_count(at < n && a.row_offsets[lo + at] <= (int32_t)row);
+        const uint32_t skip = (before ? before - 1 : 0) * part;
+        lo += skip;
+        n = min(part, n - skip);
+    }
+    for (uint32_t b = lo + threadIdx.x; b < lo + n; b += kStatsThreads) {
+        const Nodes of(a, b, false);
+        if (row >= of.row0 && row - of.row0 < of.n) atomicMin(found, b);
+    }
+}
 // The node that node i > 0 continues, or -1.
 __device__ __forceinline__ int32_t parent_of(const VerifyArgs& a, uint32_t b, uint32_t i) {
     if (!a.parents) return (int32_t)i - 1;
@@ -214,10 +230,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
         infinite = 0;
     }
     __syncthreads();
-    for (uint32_t b = tid; b < a.sequences; b += kStatsThreads) {
-        const Nodes of(a, b, false);
-        if (row >= of.row0 && row - of.row0 < of.n) atomicMin(&found, b);      // one, unless the offsets contradict themselves
-    }
+    owner_of(a, row, &found);
     __syncthreads();
     const uint32_t b = found;
     if (b == 0xFFFFFFFFu) return;
@@ -543,10 +556,7 @@ __global__ void __launch_bounds__(kStatsThreads, 2) verify_sums_kernel(const __g
         infinite = 0;
     }
     __syncthreads();
-    for (uint32_t b = tid; b < a.sequences; b += kStatsThreads) {
-        const Nodes of(a, b, false);
-        if (row >= of.row0 && row - of.row0 < of.n) atomicMin(&found, b);
-    }
+    owner_of(a, row, &found);
     float most = -INFINITY, widest = 0.0f;
 #pragma unroll
     for (int j = 0; j < kMostPieces; ++j) {
