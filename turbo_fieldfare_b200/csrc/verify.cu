@@ -1044,6 +1044,162 @@ __device__ __forceinline__ double part_weight(const Scale& s, const ChunkStat* s
     return x.sum * warp_weight(s, s.unit(warp_logit64<CAP>(s, x.most)));       // 0 where there is no finite logit
 }
 
+// The part that the target falls in, from the sums of the first launch, by all lanes. The target becomes that within the part, and the scale the part's.
+template <bool CAP>
+__device__ __forceinline__ uint32_t part_of(Scale& scale, const ChunkStat* s, uint32_t parts, double& target) {
+    uint32_t last = 0;
+    double before = 0.0, of_last = 0.0;
+    bool hit = false;
+    for (uint32_t c0 = 0; c0 < parts && !hit; c0 += kWarp) {
+        const uint32_t lane = threadIdx.x % kWarp;
+        const double mine = part_weight<CAP>(scale, s, c0 + lane, parts), run = before + warp_scan(mine, lane);
+        const uint32_t any = __ballot_sync(kFullMask, mine > kNothing), over = __ballot_sync(kFullMask, mine > kNothing && run > target);
+        hit = over != 0;
+        if (any) {                                     // behind the last one that has anything: its last token
+            const uint32_t who = hit ? __ffs(over) - 1 : 31 - __clz(any);
+            last = c0 + who;
+            of_last = __shfl_sync(kFullMask, run - mine, who);
+        }
+        before = __shfl_sync(kFullMask, run, kWarp - 1);
+    }
+    const ChunkStat part = s[last];
+    const double share = warp_weight(scale, scale.unit(warp_logit64<CAP>(scale, part.most)));
+    target = hit ? (target - of_last) / share : INFINITY;
+    scale.relative_to<CAP>(part.most, part.infinite);
+    return last;
+}
+
+// One row a sequence: nothing to walk, and all that a draw needs is there. A block takes the part that the token lies in as the first launch did, all its logits at once, and sums them by steps
+// of a warp; the step's warp draws. Latency bounds it: six loads, one after another, and what stands between them. A token of 262144 takes 13.3 us
+// in all and 1000 rows of 300 34; by the walk, which goes from part to token in three readings, 15.5 and 93.
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(kStatsThreads, 2) verify_lone_kernel(const __grid_constant__ VerifyArgs a) {
+    using R = Row<T>;
+    constexpr int E = R::E, WARPS = kStatsThreads / kWarp;
+    static_assert(kMostPieces * WARPS == 2 * kWarp, "two steps a lane");
+    constexpr double kLn2 = 0.69314718055994530942;
+    __shared__ double step_sum[kMostPieces * WARPS];
+    const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, b = blockIdx.x;
+    if (a.parts == 0) pdl_wait();
+    const Nodes of(a, b, tid == 0);
+    const Heat heat(a, b);
+    const double u = (double)uniform(a.uniforms[b]);
+    Scale scale;
+    scale.set<CAP>(a.softcap, heat.k, lane);
+    if (a.parts) pdl_wait();
+    if (tid == 0) {
+        a.out_rows[b] = of.n ? 0 : -1;
+        a.kept[b] = of.n;
+    }
+    auto leave = [&](int32_t token, float logprob) {
+        a.out_tokens[b] = token;
+        if (a.logprobs) a.logprobs[b] = logprob;
+    };
+    if (of.n == 0) {
+        if (tid == 0) leave(-1, 0.0f);
+        return;
+    }
+    const ChunkStat* s = a.stats + (size_t)of.row0 * a.parts;
+    float top = -INFINITY;
+    for (uint32_t c = lane; c < a.parts; c += kWarp) top = fmaxf(top, s[c].most);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+    const double logit = warp_logit64<CAP>(scale, top);
+    scale.from = heat.greedy ? logit : scale.unit(logit);
+    double z = 0.0;
+    for (uint32_t c0 = 0; c0 < a.parts; c0 += kWarp) z += part_weight<CAP>(scale, s, c0 + lane, a.parts);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) z += __shfl_xor_sync(kFullMask, z, off);
+    if (heat.greedy) {
+        uint32_t at = 0xFFFFFFFFu;
+        for (uint32_t c = lane; c < a.parts; c += kWarp)
+            if (s[c].most == top) at = min(at, s[c].at);
+        at = __reduce_min_sync(kFullMask, at);
+        if (tid == 0) leave(at == 0xFFFFFFFFu ? 0 : (int32_t)at, z > 0.0 ? (float)-log(z) : -INFINITY);
+        return;
+    }
+    if (!(z > kNothing)) {
+        if (tid == 0) leave(0, -INFINITY);
+        return;
+    }
+    const double whole = scale.from;
+    double target = u * z;
+    const uint32_t part = part_of<CAP>(scale, s, a.parts, target);
+    const R row(a.logits, of.row0 * a.stride, a.vocab);
+    const uint32_t piece = part * a.per * kStatsThreads + tid;
+    uint4 w[kMostPieces];
+#pragma unroll
+    for (int j = 0; j < kMostPieces; ++j) w[j] = (uint32_t)j < a.per ? row.load(piece + j * kStatsThreads) : R::nothing();
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < kMostPieces; ++j)
+        if (CAP && (uint32_t)j < a.per) far |= !(R::most(R::magnitudes(w[j])) <= a.softcap);
+    far = CAP && __any_sync(kFullMask, far);
+#pragma unroll
+    for (int j = 0; j < kMostPieces; ++j) {
+        if ((uint32_t)j >= a.per) {
+            if (lane == 0) step_sum[j * WARPS + warp] = 0.0;
+            continue;
+        }
+        double sums[4] = {};
+        float x[E];
+        R::numbers(w[j], x);
+#pragma unroll
+        for (int h = 0; h < E; h += 4) {
+            float some[4];
+            double v[4], base[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) some[e] = x[h + e];
+            if (CAP && !far && !scale.careful) warp_weights<CAP, 4, false, CAP>(scale, some, v, base);
+            else warp_weights<CAP>(scale, some, v, base);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[e] = fma(base[e], v[e], sums[e]);
+        }
+        double sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFullMask, sum, off);
+        if (lane == 0) step_sum[j * WARPS + warp] = sum;
+    }
+    __syncthreads();
+    const double first = step_sum[2 * lane], second = step_sum[2 * lane + 1], pair = first + second;
+    const uint32_t who = warp_fall(pair, warp_scan(pair, lane), target);
+    const double one = __shfl_sync(kFullMask, first, who), two = __shfl_sync(kFullMask, second, who);
+    uint32_t step = 2 * who;
+    if (!(one > kNothing && (one > target || !(two > kNothing)))) {
+        step += 1;
+        target -= one;
+    }
+    if (warp != step % WARPS) return;
+    const uint32_t mine = piece + step / WARPS * kStatsThreads;
+    float x[E];
+    R::numbers(row.load(mine), x);
+    double v[E], all = 0.0;
+#pragma unroll
+    for (int h = 0; h < E; h += 4) {
+        float some[4];
+        double some_v[4], base[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) some[e] = x[h + e];
+        if (CAP && !far && !scale.careful) warp_weights<CAP, 4, false, CAP>(scale, some, some_v, base);
+        else warp_weights<CAP>(scale, some, some_v, base);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) all += v[h + e] = some_v[e] * base[e];
+    }
+    if (warp_fall(all, warp_scan(all, lane), target) != lane) return;
+    double at = 0.0;
+    int found = -1, end = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        at += v[e];
+        if (v[e] > kNothing / 8) {                 // of a lane that has more than kNothing one has
+            end = e;
+            if (found < 0 && at > target) found = e;
+        }
+    }
+    const int64_t token = row.first(mine) + (found < 0 ? end : found);
+    leave((int32_t)token, a.logprobs ? (float)((logit64<CAP>(number(row.p[token]), a.softcap) - whole) * heat.k * kLn2 - log(z)) : 0.0f);
+}
+
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
     using R = Row<T>;
@@ -1231,24 +1387,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
                 break;
             }
             target = (double)o.u * z;
-            uint32_t last = 0;
-            double before = 0.0, of_last = 0.0;
-            bool hit = false;
-            for (uint32_t c0 = 0; c0 < a.parts && !hit; c0 += kWarp) {
-                const double mine = part_weight<CAP>(scale, s, c0 + lane, a.parts), run = before + warp_scan(mine, lane);
-                const uint32_t any = __ballot_sync(kFullMask, mine > kNothing), over = __ballot_sync(kFullMask, mine > kNothing && run > target);
-                hit = over != 0;
-                if (any) {                             // behind the last one that has anything: its last token
-                    const uint32_t who = hit ? __ffs(over) - 1 : 31 - __clz(any);
-                    last = c0 + who;
-                    of_last = __shfl_sync(kFullMask, run - mine, who);
-                }
-                before = __shfl_sync(kFullMask, run, kWarp - 1);
-            }
-            const ChunkStat chunk = s[last];
-            const double share = warp_weight(scale, scale.unit(warp_logit64<CAP>(scale, chunk.most)));
-            target = hit ? (target - of_last) / share : INFINITY;
-            scale.relative_to<CAP>(chunk.most, chunk.infinite);
+            const uint32_t last = part_of<CAP>(scale, s, a.parts, target);
             chosen = true;
             begin = last * a.per * kStatsThreads;
             count = a.per * (kStatsThreads / kWarp);
@@ -1348,7 +1487,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
                             at += w[e];
-                            if (w[e] > kNothing) {
+                            if (w[e] > kNothing / 8) {             // of a lane that has more than kNothing one has
                                 end = e;
                                 if (found < 0 && at > target) found = e;
                             }
@@ -1397,6 +1536,7 @@ tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a, uint64_t
             const uint64_t pieces = ((uint64_t)a.vocab + (even ? 0 : E - 1) + E - 1) / E;
             auto parts = [&](uint32_t per) { return (pieces + (uint64_t)kStatsThreads * per - 1) / ((uint64_t)kStatsThreads * per); };
             a.per = kMostPieces;
+            while (a.per > 1 && parts(a.per / 2) == 1) a.per /= 2;             // short rows: 1000 of 300 67 us with eight pieces, 37 with one
             while (a.per > 1 && a.rows * parts(a.per) < (uint64_t)ctx->sm_count * 2 && parts(a.per / 2) <= (CAP ? 128 : 64) && a.rows * parts(a.per / 2) <= room) a.per /= 2;
             a.parts = (uint32_t)parts(a.per);
             verify_sums_kernel<T, CAP><<<(uint32_t)(a.rows * (uint64_t)a.parts), kStatsThreads, 0, st>>>(a);
@@ -1412,9 +1552,13 @@ tf_status launch_verify(tf_context* ctx, cudaStream_t st, VerifyArgs a, uint64_t
         const tf_status s = check_launch(ctx, name);
         if (s != TF_OK) return s;
     }
+    if (a.draft_stride == 1) {
+        TF_CUDA(ctx, launch_pdl(verify_lone_kernel<T, CAP>, dim3(a.sequences), dim3(kStatsThreads), 0, st, a));
+        return check_launch(ctx, name);
+    }
     // Blocks of a sequence: 16, 8, 4 or 2 of them take 22, 33, 55, 96 us for a lone row that is not summed yet, 81, 80, 95, 123 for 33 trees of 12, 114, 114, 113, 156 for 64 chains of seven.
-    // So as many as are on the chip at once, two an SM, with two steps a warp; beyond that they wait for one another's places. One where the sums are there: it draws from one part.
-    while (ranks > 1 && (a.draft_stride == 1 || (uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2 || (uint64_t)a.vocab < (uint64_t)ranks * kWalkThreads * 2 * E)) ranks /= 2;
+    // So as many as are on the chip at once, two an SM, with two steps a warp; beyond that they wait for one another's places.
+    while (ranks > 1 && ((uint64_t)a.sequences * ranks > (uint64_t)ctx->sm_count * 2 || (uint64_t)a.vocab < (uint64_t)ranks * kWalkThreads * 2 * E)) ranks /= 2;
     const size_t smem = a.draft_stride * NodeTable::kBytes;
     static DeviceSmemCache smem_cache;
     const tf_status m = ensure_dynamic_smem(ctx, verify_walk_kernel<T, CAP>, smem_cache, smem);
