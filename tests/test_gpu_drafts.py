@@ -418,6 +418,19 @@ def test_offsets_that_contradict_themselves_are_reported(tf_ctx):
     assert tf_ctx.device_status() == 0
 
 
+@pytest.mark.parametrize("nodes", [1, 3])
+@pytest.mark.parametrize("sequences", [40, 2500])
+def test_offsets_out_of_order_draw_tokens_of_the_row(tf_ctx, sequences, nodes):
+    from turbo_fieldfare_b200.kernels import TFError
+    vocab = 4001
+    d = Draft(12, [1] * sequences, nodes, vocab)
+    d.offsets = np.random.default_rng(3).integers(-3, sequences + 3, sequences + 1).tolist()
+    out = d.run(tf_ctx)
+    with pytest.raises(TFError, match="7F000052|7f000052"):
+        tf_ctx.device_status()
+    assert bool(((out[0] >= -1) & (out[0] < vocab)).all()) and bool(((out[2] >= 0) & (out[2] <= nodes)).all())
+
+
 def test_equal_calls_give_equal_bits(tf_ctx):
     d = Draft(81, [9] * 20, 9, 30011, probs=torch.float32, tree=True)
     first = d.run(tf_ctx)

@@ -89,6 +89,8 @@ struct Row {
     }
     __device__ __forceinline__ uint32_t pieces() const { return (uint32_t)(((uint64_t)vocab + lead + E - 1) / E); }
     __device__ __forceinline__ int64_t first(uint32_t piece) const { return (int64_t)piece * E - lead; }
+    // A drawn element, which is one of the row's unless offsets contradict themselves and the sums are of another call
+    __device__ __forceinline__ int64_t inside(int64_t at) const { return at < 0 ? 0 : at < (int64_t)vocab ? at : (int64_t)vocab - 1; }
     static __device__ __forceinline__ uint4 nothing() {
         constexpr uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
         return make_uint4(w, w, w, w);
@@ -533,7 +535,7 @@ __device__ __forceinline__ void Scale::relative_to(float top, bool infinite) {
 // ---------------------------------------------------------------------------
 //
 // Where there are few logits, or one row a sequence: the same sums for every row, in 64 bits, by blocks all over the chip. The walk then needs no sum but those behind
-// a refusal, and a draw no more than a part's logits again. 64-bit arithmetic bounds it: eleven operations a logit (25 capped) at 64 a clock and SM, 1.6e12 logits a second (7e11).
+// a refusal, and a draw no more than a part's logits again. 64-bit arithmetic is its floor: eight operations a logit (23 capped) at 64 a clock and SM, 2.2e12 logits a second (8e11).
 constexpr int kMostPieces = 8;
 
 template <typename T, bool CAP>
@@ -895,7 +897,8 @@ __device__ __noinline__ double one_step(const VerifyArgs& a, const Row<T>& row, 
 }
 
 // Where the time goes: `steps` whole pieces from p on, a warp apart, whose weights need no care. Nothing but this in a function, without a branch on what a call fixes: as a part of the walk, with the
-// edges' checks, 64 chains of seven took 138 us; as a function 127, without the checks 114. 64-bit arithmetic bounds it: 11 operations a logit and one more a refusal, 25 capped. Q: the type of q, 0 none, else as tf_dtype + 1; EVEN: q's pieces lie at boundaries.
+// edges' checks, 64 chains of seven took 138 us; as a function 127, without the checks 114. Eight operations of 64 bits a logit, two more
+// a refusal, 23 capped; a step takes 205 clocks a warp with four warps a sub-core, by issue slots and latencies together (without loads, shuffles and most of the series still 150). Q: the type of q, 0 none, else as tf_dtype + 1; EVEN: q's pieces lie at boundaries.
 template <typename T, bool CAP, int Q, bool EVEN>
 __device__ __noinline__ void many_steps(const uint4* p, const void* q_at, uint32_t steps, int32_t first, const Refused& refused, const Scale& by, Tally& tally) {
     constexpr int E = Row<T>::E, WORDS = Q == 0 ? 1 : Q == TF_FP32 + 1 ? E / 4 : 1;
@@ -1196,7 +1199,7 @@ __global__ void __launch_bounds__(kStatsThreads, 2) verify_lone_kernel(const __g
             if (found < 0 && at > target) found = e;
         }
     }
-    const int64_t token = row.first(mine) + (found < 0 ? end : found);
+    const int64_t token = row.inside(row.first(mine) + (found < 0 ? end : found));
     leave((int32_t)token, a.logprobs ? (float)((logit64<CAP>(number(row.p[token]), a.softcap) - whole) * heat.k * kLn2 - log(z)) : 0.0f);
 }
 
@@ -1492,7 +1495,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
                                 if (found < 0 && at > target) found = e;
                             }
                         }
-                        const int64_t token = row.first(begin + lane) + (found < 0 ? end : found);
+                        const int64_t token = row.inside(row.first(begin + lane) + (found < 0 ? end : found));
                         out_tokens[o.at] = (int32_t)token;
                         if (logprobs) logprobs[o.at] = (float)((logit64<CAP>(number(row.p[token]), a.softcap) - whole) * heat.k * kLn2 - log(z));
                     }
