@@ -218,8 +218,8 @@ __device__ __forceinline__ float gelu_tanh(float x) {
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// A table that a gate/up launch reads after its pdl_wait and the down launch that follows it before its own. What holds for the latter:
-// the launches that wrote the table had completed, and their writes were visible, when gate/up returned from its wait, and
+// A table that a gate/up launch reads after its pdl_wait and the down launch that follows it before its own (likewise what the two launches of a verification
+// are given). What holds for the latter: the launches that wrote the table had completed, and their writes were visible, when gate/up returned from its wait, and
 // only after that did gate/up let the down launch start. Nothing is promised to a grid that has not waited itself about lines
 // that its SM's L1 may hold, so it reads with relaxed loads at GPU scope, which L2 serves, where the writes are. (Gate/up keeps
 // plain ones: every warp of the chip reads the same few lines there, and without L1 a one-token layer took 1 us longer.)
@@ -234,6 +234,12 @@ struct EarlyTable {
             static_assert(sizeof(T) == 16, "one vector load");
             T v;
             asm volatile("ld.relaxed.gpu.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p + i));
+            return v;
+        } else if constexpr (sizeof(T) == 2) {
+            uint16_t bits;
+            asm volatile("ld.relaxed.gpu.global.u16 %0, [%1];" : "=h"(bits) : "l"(p + i));
+            T v;
+            memcpy(&v, &bits, 2);
             return v;
         } else {
             static_assert(sizeof(T) % 4 == 0 && alignof(T) == 4, "by 32-bit words: the pairs of a streamed call are aligned to four bytes");

@@ -46,8 +46,8 @@ struct ChunkStat {
 struct VerifyArgs {
     const void* logits;
     uint64_t stride;
-    const int32_t *row_offsets, *tokens, *parents;
-    const float *uniforms, *temperatures;
+    EarlyTable<int32_t> row_offsets, tokens, parents;          // the first launch reads them plainly: it is an ordinary one
+    EarlyTable<float> uniforms, temperatures;
     const void* probs;
     uint64_t probs_sequence, probs_node;
     int32_t *out_tokens, *out_rows, *kept;
@@ -155,11 +155,16 @@ __device__ __forceinline__ float capped(float x, float cap) {
 // A random number, in [0, 1) whatever it is.
 __device__ __forceinline__ float uniform(float u) { return fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f); }
 
+// What a launch reads before its wait comes past L1 (see EarlyTable): the second launches say so of what they call there.
+constexpr std::true_type kEarly{};
+constexpr std::false_type kWaited{};
+
 struct Heat {
     bool greedy;
     double k;                  // log2(e) / T
-    __device__ __forceinline__ Heat(const VerifyArgs& a, uint32_t b) {
-        const float t = a.temperatures ? a.temperatures[b] : 1.0f;
+    template <bool EARLY>
+    __device__ __forceinline__ Heat(const VerifyArgs& a, uint32_t b, std::bool_constant<EARLY>) {
+        const float t = a.temperatures.p ? a.temperatures.at<EARLY>(b) : 1.0f;
         greedy = !(t > 0.0f);
         k = kLog2E / (greedy ? 1.0 : (double)fminf(t, 1e30f));
     }
@@ -169,8 +174,9 @@ struct Heat {
 
 struct Nodes {                 // a sequence's rows, cut to what the arrays can hold
     uint32_t row0, n;
-    __device__ __forceinline__ Nodes(const VerifyArgs& a, uint32_t b, bool report) {
-        const int32_t begin = a.row_offsets[b], end = a.row_offsets[b + 1], most = (int32_t)a.rows;
+    template <bool EARLY>
+    __device__ __forceinline__ Nodes(const VerifyArgs& a, uint32_t b, bool report, std::bool_constant<EARLY>) {
+        const int32_t begin = a.row_offsets.at<EARLY>(b), end = a.row_offsets.at<EARLY>(b + 1), most = (int32_t)a.rows;
         const int32_t lo = begin < 0 ? 0 : begin > most ? most : begin, hi = end < lo ? lo : end > most ? most : end;
         row0 = (uint32_t)lo;
         n = (uint32_t)(hi - lo);
@@ -184,20 +190,21 @@ __device__ __forceinline__ void owner_of(const VerifyArgs& a, uint32_t row, uint
     uint32_t lo = 0, n = a.sequences;
     while (n > 1024) {
         const uint32_t part = (n + kStatsThreads - 1) / kStatsThreads, at = threadIdx.x * part;
-        const uint32_t before = (uint32_t)__syncthreads_count(at < n && a.row_offsets[lo + at] <= (int32_t)row);
+        const uint32_t before = (uint32_t)__syncthreads_count(at < n && a.row_offsets.at<false>(lo + at) <= (int32_t)row);
         const uint32_t skip = (before ? before - 1 : 0) * part;
         lo += skip;
         n = min(part, n - skip);
     }
     for (uint32_t b = lo + threadIdx.x; b < lo + n; b += kStatsThreads) {
-        const Nodes of(a, b, false);
+        const Nodes of(a, b, false, kWaited);
         if (row >= of.row0 && row - of.row0 < of.n) atomicMin(found, b);
     }
 }
 // The node that node i > 0 continues, or -1.
-__device__ __forceinline__ int32_t parent_of(const VerifyArgs& a, uint32_t b, uint32_t i) {
-    if (!a.parents) return (int32_t)i - 1;
-    const int32_t p = a.parents[(size_t)b * a.draft_stride + i];
+template <bool EARLY>
+__device__ __forceinline__ int32_t parent_of(const VerifyArgs& a, uint32_t b, uint32_t i, std::bool_constant<EARLY>) {
+    if (!a.parents.p) return (int32_t)i - 1;
+    const int32_t p = a.parents.at<EARLY>((size_t)b * a.draft_stride + i);
     return p >= 0 && p < (int32_t)i ? p : -1;
 }
 
@@ -236,13 +243,13 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
     __syncthreads();
     const uint32_t b = found;
     if (b == 0xFFFFFFFFu) return;
-    const Nodes of(a, b, false);
+    const Nodes of(a, b, false, kWaited);
     const uint32_t i = row - of.row0;
-    const Heat heat(a, b);
+    const Heat heat(a, b, kWaited);
     if (!heat.greedy) {        // a greedy sequence ends with the likeliest token of any of its rows; of others' leaves at most one is looked at
         bool child = false;
-        if (!a.parents) child = i + 1 < of.n;
-        else for (uint32_t j = i + 1 + tid; j < of.n; j += kStatsThreads) child |= parent_of(a, b, j) == (int32_t)i;
+        if (!a.parents.p) child = i + 1 < of.n;
+        else for (uint32_t j = i + 1 + tid; j < of.n; j += kStatsThreads) child |= parent_of(a, b, j, kWaited) == (int32_t)i;
         if (!__syncthreads_or(child)) return;
     }
     const float k = heat.k32(), inverse = CAP ? 1.0f / a.softcap : 0.0f;
@@ -584,7 +591,7 @@ __global__ void __launch_bounds__(kStatsThreads, 2) verify_sums_kernel(const __g
     top = lane < WARPS ? warp_most[lane] : -INFINITY;
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
-    const Heat heat(a, b);
+    const Heat heat(a, b, kWaited);
     Scale scale;
     scale.set<CAP>(a.softcap, heat.k, lane);
     scale.relative_to<CAP>(top, infinite);
@@ -671,11 +678,12 @@ struct NodeTable {
     static constexpr size_t kBytes = 52;
 };
 
+// Before the wait
 __device__ __forceinline__ float prob_at(const VerifyArgs& a, uint64_t at) {
     float q;
-    if (a.probs_dtype == TF_FP32) q = static_cast<const float*>(a.probs)[at];
-    else if (a.probs_dtype == TF_FP16) q = __half2float(static_cast<const __half*>(a.probs)[at]);
-    else q = __bfloat162float(static_cast<const __nv_bfloat16*>(a.probs)[at]);
+    if (a.probs_dtype == TF_FP32) q = EarlyTable<float>{static_cast<const float*>(a.probs)}.at<true>(at);
+    else if (a.probs_dtype == TF_FP16) q = __half2float(EarlyTable<__half>{static_cast<const __half*>(a.probs)}.at<true>(at));
+    else q = __bfloat162float(EarlyTable<__nv_bfloat16>{static_cast<const __nv_bfloat16*>(a.probs)}.at<true>(at));
     return fmaxf(q, 0.0f);     // NaN too
 }
 // A node's row of probabilities by the pieces of its logits.
@@ -1084,9 +1092,9 @@ __global__ void __launch_bounds__(kStatsThreads, 2) verify_lone_kernel(const __g
     __shared__ double step_sum[kMostPieces * WARPS];
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, b = blockIdx.x;
     if (a.parts == 0) pdl_wait();
-    const Nodes of(a, b, tid == 0);
-    const Heat heat(a, b);
-    const double u = (double)uniform(a.uniforms[b]);
+    const Nodes of(a, b, tid == 0, kEarly);
+    const Heat heat(a, b, kEarly);
+    const double u = (double)uniform(a.uniforms.at<true>(b));
     Scale scale;
     scale.set<CAP>(a.softcap, heat.k, lane);
     if (a.parts) pdl_wait();
@@ -1217,10 +1225,10 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
     const uint32_t tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const uint32_t rank = cluster.block_rank(), ranks = cluster.num_blocks(), b = blockIdx.x / ranks;
     Scale scale;
-    // The first launch waits for what came before it and writes nothing but its sums: all else may be read while it is at work.
+    // The first launch starts when what came before it has ended and writes nothing but its sums: all else may be read while it is at work, past L1.
     if (a.parts == 0) pdl_wait();
-    const Nodes of(a, b, rank == 0 && tid == 0);
-    const Heat heat(a, b);
+    const Nodes of(a, b, rank == 0 && tid == 0, kEarly);
+    const Heat heat(a, b, kEarly);
     const NodeTable nodes(dynamic, a.draft_stride);
     int32_t* gone_tokens = reinterpret_cast<int32_t*>(nodes.gone);
     int32_t* out_tokens = a.out_tokens + (size_t)b * a.draft_stride;
@@ -1234,15 +1242,16 @@ __global__ void __launch_bounds__(kWalkThreads, 2) verify_walk_kernel(const __gr
         for (uint32_t i = tid; i < of.n; i += kWalkThreads) nodes.inner[i] = 0;
         __syncthreads();
         for (uint32_t i = tid; i < of.n; i += kWalkThreads) {
-            const int32_t x = a.tokens[(size_t)b * a.draft_stride + i], p = i ? parent_of(a, b, i) : -1;
+            const int32_t x = a.tokens.at<true>((size_t)b * a.draft_stride + i), p = i ? parent_of(a, b, i, kEarly) : -1;
             const bool token = x >= 0 && (uint32_t)x < a.vocab;
             nodes.parent[i] = p;
             nodes.token[i] = token ? x : -1;
-            nodes.number[i] = uniform(a.uniforms[(size_t)b * a.draft_stride + i]);
+            nodes.number[i] = uniform(a.uniforms.at<true>((size_t)b * a.draft_stride + i));
             if (p < 0) continue;
             atomicOr(nodes.inner + p, 1);
             if (!token) continue;
-            nodes.weight[i] = (double)counted(number(static_cast<const T*>(a.logits)[(of.row0 + (uint64_t)p) * a.stride + x]));     // for now
+            const EarlyTable<T> logits{static_cast<const T*>(a.logits)};
+            nodes.weight[i] = (double)counted(number(logits.template at<true>((of.row0 + (uint64_t)p) * a.stride + x)));     // for now
             nodes.prob[i] = a.probs && (uint32_t)p < a.probs_nodes ? prob_at(a, b * a.probs_sequence + p * a.probs_node + x) : 0.0f;
         }
         if (a.parts) pdl_wait();
@@ -1647,8 +1656,8 @@ tf_status tf_verify_drafts(tf_context* ctx, void* stream, const void* logits, ui
         a.probs = probs->values; a.probs_sequence = probs->sequence_stride; a.probs_node = probs->node_stride; a.probs_nodes = probs->nodes;
         a.probs_dtype = probs->dtype;
     }
-    a.logits = logits; a.stride = logits_stride; a.row_offsets = row_offsets; a.tokens = drafts->tokens; a.parents = drafts->parents;
-    a.uniforms = uniforms; a.temperatures = temperatures;
+    a.logits = logits; a.stride = logits_stride; a.row_offsets = {row_offsets}; a.tokens = {drafts->tokens}; a.parents = {drafts->parents};
+    a.uniforms = {uniforms}; a.temperatures = {temperatures};
     a.out_tokens = out_tokens; a.out_rows = out_rows; a.kept = kept; a.logprobs = logprobs;
     a.stats = static_cast<tf::ChunkStat*>(ws->memory);
     a.error = ctx->device_error;
