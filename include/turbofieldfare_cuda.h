@@ -958,7 +958,8 @@ typedef struct tf_kv_rows {
  * found) at place j from the top. Row i of a sequence: position context_lengths[b] + i, with parents context_lengths[b] + the node's depth. drafts may be NULL; it is needed for rows->tokens
  * (its tokens) and rows->tree_mask (its parents, or a chain). A row's mask has the bits of its node and of its ancestors.
  * Equal inputs give equal outputs. tf_device_status reports 0x7F000054 where the arrays contradict themselves (a stack outside [0, num_pages], more
- * pages given back than it has room for, a parent that is not before its node, which then counts as -1, a node from 64 * mask_words on);
+ * pages given back than it has room for, a page outside [0, num_pages) that goes back, is taken or has a row on it, which stands as -1 on the stack, in the table
+ * and as the row's slot, a parent that is not before its node, which then counts as -1, a node from 64 * mask_words on); that a page is named twice it does not notice;
  * nothing outside the arrays is read or written whatever they hold. A depth of d takes d steps. */
 tf_status tf_kv_plan(tf_context* ctx, void* stream, const tf_kv_pages* pages, int32_t* context_lengths, const int32_t* new_rows, const int32_t* kept,
                      uint32_t window, const tf_drafts* drafts, const tf_kv_rows* rows);

@@ -31,6 +31,13 @@ __device__ __forceinline__ uint32_t plan_add(uint32_t a, uint32_t b) {
     return s < a ? 0xFFFFFFFFu : s;
 }
 
+// A page that goes back, is taken or has a row on it: -1, and a report, where there is no such page.
+__device__ __forceinline__ int32_t plan_page(const PlanArgs& a, int32_t page) {
+    if ((uint32_t)page < a.num_pages) return page;
+    *a.error = kErrPlan;
+    return -1;
+}
+
 // Inclusive sums of two numbers over the block, and the block's totals.
 struct PlanScan {
     uint32_t warp_sum[2][kPlanWarps];
@@ -120,7 +127,7 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, uint32_t row, uint32
     if (a.row_sequences) a.row_sequences[row] = (int32_t)b;
     if (a.row_tokens) a.row_tokens[row] = a.draft_tokens[(size_t)b * a.draft_stride + i];
     if (a.slots) {
-        const int32_t page = a.page_table[(size_t)b * a.table_stride + (token >> a.page_log2)];
+        const int32_t page = plan_page(a, a.page_table[(size_t)b * a.table_stride + (token >> a.page_log2)]);
         a.slots[row] = page < 0 ? -1ll : ((int64_t)page << a.page_log2) + (token & ((1u << a.page_log2) - 1u));
     }
 }
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
                 int32_t* entries = a.page_table + (size_t)(b0 + tid - lane + who) * a.table_stride + __shfl_sync(kFullMask, s.lo, who);
                 for (uint32_t e = lane; e < n; e += kWarp) {
                     const uint32_t j = plan_add(from, e);
-                    if (j < back) a.free_pages[count + back - 1 - j] = entries[e];
+                    if (j < back) a.free_pages[count + back - 1 - j] = plan_page(a, entries[e]);
                     entries[e] = -1;
                 }
             }
@@ -232,7 +239,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
             todo &= todo - 1;
             const uint32_t from = __shfl_sync(kFullMask, pages_from, who), n = __shfl_sync(kFullMask, need, who);
             int32_t* entries = a.page_table + (size_t)(b0 + tid - lane + who) * a.table_stride + __shfl_sync(kFullMask, held, who);
-            for (uint32_t e = lane; e < n; e += kWarp) entries[e] = a.free_pages[count - 1 - (from + e)];
+            for (uint32_t e = lane; e < n; e += kWarp) entries[e] = plan_page(a, a.free_pages[count - 1 - (from + e)]);
         }
         pages_before = plan_add(pages_before, total[0]);
         rows_before = plan_add(rows_before, total[1]);
