@@ -109,13 +109,17 @@ def test_temperatures_at_the_ends(tf_ctx):
         d.compare(tf_ctx, temperatures=[0.0, -2.0, 1e-6, 1e-30, 0.05, 50.0, 1e6, 1e-3])
 
 
-def test_caps_at_the_ends(tf_ctx):
-    """So low that its inverse is no number of 32 bits: all logits count alike, those of zero among them; so high that it changes nothing."""
-    for cap in (1e-39, 2e-38, 1e-3, 1e5, 3e38):
-        for counts, vocab in (([3] * 8, 240007), ([3, 2], 3001)):  # sums in 32 bits, and in 64
-            d = Draft(9, counts, 3, vocab, dtype=torch.float32, tree=True)
-            d.logits[:, ::5] = 0.0
-            d.compare(tf_ctx, cap=cap)
+@pytest.mark.parametrize("cap", [1e-3, 300.0, 4000.0, 1e5, 1e9, 1e20, 3e38])
+@pytest.mark.parametrize("counts,vocab", [([3] * 8, 240007), ([3, 2], 3001), ([1] * 8, 30011)])      # sums in 32 bits, in 64, lone rows
+def test_caps_at_the_ends(tf_ctx, cap, counts, vocab):
+    """From so low that nearly all logits count alike to so high that it changes nothing; some logits are wider than any cap."""
+    for dtype, far in ((torch.float16, -6e4), (torch.float32, -3.4e38)):
+        d = Draft(9, counts, max(counts), vocab, dtype=dtype, tree=max(counts) > 1)
+        d.logits[:, ::5] = 0.0
+        d.logits[:, 1::97] = far
+        d.uniforms[1, 1:] = 0.0
+        for heat in (None, [0.0, 1.0, 0.8, 2.0] * 2):
+            d.compare(tf_ctx, cap=cap, temperatures=None if heat is None else heat[:len(counts)])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -213,10 +217,10 @@ def test_two_graphs_replayed_with_new_inputs(tf_ctx):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nodes", [1, 6])
-@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("cap", [0.0, 30.0, 1e9])
 def test_logarithms_of_sums_in_64_bits(tf_ctx, dtype, nodes, cap):
     """Where all rows are summed in 64 bits a logarithm is off by its rounding to 32 bits alone: 2^-24 of it, and less than 1e-10 of what 64 bits leave
-    (powers of two 8e-14 of a weight; capped logits 1e-13 of the cap, over the lowest temperature)."""
+    (powers of two 8e-14 of a weight; capped logits, none wider than the cap, 2e-14 of themselves, over the lowest temperature)."""
     counts = [nodes, max(1, nodes // 2), nodes, 1]
     for probs in (None, torch.float32):
         for vocab in (5003, 200003):

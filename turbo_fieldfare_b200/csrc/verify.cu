@@ -426,7 +426,7 @@ struct Scale {
     double lowest;             // -32000 / k: that far below a weight is 2^-1000
     float least;               // logits from here down count as that, where the row needs no care
     int2 table;
-    bool careful;              // the row holds infinities, or steps of 32 bits that are as large as that
+    bool careful;              // the row holds infinities, steps of 32 bits that are as large as that, or a cap far above T
     template <bool CAP>
     __device__ __forceinline__ void set(float softcap, double log2e_by_heat, int lane) {
         table = power_table(lane);
@@ -447,30 +447,37 @@ struct Scale {
 };
 constexpr double kNothing = 0x1p-900;          // more than a vocabulary of tokens that do not count
 
-// Weights in 64 bits by all lanes of a warp. Capped logits: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps, 1e-13 cap off.
-// They come as products base w, which sums multiply. NEAR: no logit that counts is wider than the cap. Then x P((x / cap)^2), P being tanh(u) / u by its Chebyshev coefficients in u^2 on [0, 1], 1.5e-14 off: half of the instructions.
+// Logits that are no wider than the cap: x P((x / cap)^2), P being tanh(u) / u by its Chebyshev coefficients in u^2 on [0, 1], 2e-14 of it off.
+template <int N>
+__device__ __forceinline__ void near_capped(const float (&x)[N], double inverse, double (&w)[N]) {
+    constexpr double c[13] = {0.9999999999999823, -0.3333333333272711, 0.13333333298786137, -0.05396824620692592, 0.021869397540056224, -0.008862596767873559, 0.0035892253083668387,
+                              -0.0014468841456978221, 0.0005707702734400899, -0.0002097698327657338, 6.496419251345914e-05, -1.4302828371933043e-05, 1.5987624655853251e-06};
+    double z[N], p[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        w[e] = (double)x[e];
+        z[e] = w[e] * inverse;
+        z[e] *= z[e];
+        p[e] = c[12];
+    }
+#pragma unroll
+    for (int i = 11; i >= 0; --i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) p[e] = fma(p[e], z[e], c[i]);
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] *= p[e];
+}
+
+// Weights in 64 bits by all lanes of a warp. Capped logits: cap - 2 cap / (exp(2 x / cap) + 1), the quotient from 23 bits by one of Newton's steps, 1e-13 cap off; a row whose weights
+// that would move is a careful one, where logits no wider than the cap go by the series of near_capped.
+// They come as products base w, which sums multiply. NEAR: no logit that counts is wider than the cap, the series for all: half of the instructions.
 template <bool CAP, int N, bool CARE = true, bool NEAR = false>
 __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N], double (&w)[N], double (&base)[N]) {
     if constexpr (!CAP) {
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = (double)fmaxf(x[e], s.least);       // NaN too
     } else if constexpr (NEAR) {
-        constexpr double c[13] = {0.9999999999999823, -0.3333333333272711, 0.13333333298786137, -0.05396824620692592, 0.021869397540056224, -0.008862596767873559, 0.0035892253083668387,
-                                  -0.0014468841456978221, 0.0005707702734400899, -0.0002097698327657338, 6.496419251345914e-05, -1.4302828371933043e-05, 1.5987624655853251e-06};
-        double z[N], p[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            w[e] = (double)x[e];
-            z[e] = w[e] * s.inverse;
-            z[e] *= z[e];
-            p[e] = c[12];
-        }
-#pragma unroll
-        for (int i = 11; i >= 0; --i)
-#pragma unroll
-            for (int e = 0; e < N; ++e) p[e] = fma(p[e], z[e], c[i]);
-#pragma unroll
-        for (int e = 0; e < N; ++e) w[e] *= p[e];
+        near_capped(x, s.inverse, w);
     } else {
         const float edge = 20.0f * (float)s.cap;                                // tanh is 1 to the last bit from there on
         double y[N];
@@ -490,6 +497,11 @@ __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N]
         for (int e = 0; e < N; ++e) y[e] = fma(y[e], w[e], y[e]);
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = fma(-2.0 * s.cap, y[e], s.cap);
+        if (CARE && s.careful) {
+            near_capped(x, s.inverse, y);
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = fabsf(x[e]) <= (float)s.cap ? y[e] : w[e];
+        }
     }
     if constexpr (CAP) {
 #pragma unroll
@@ -510,10 +522,11 @@ __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N]
 template <bool CAP>
 __device__ __forceinline__ double warp_logit64(const Scale& s, float x) {
     if constexpr (!CAP) return (double)x;
-    const float edge = 20.0f * (float)s.cap;
-    double d[1] = {(double)fminf(fmaxf(x, -edge), edge)};
+    const float edge = 20.0f * (float)s.cap, its[1] = {x};
+    double d[1] = {(double)fminf(fmaxf(x, -edge), edge)}, near[1];
     warp_exp2(d, s.twice, s.table);
-    return fabsf(x) < INFINITY ? s.cap - 2.0 * s.cap / (d[0] + 1.0) : -INFINITY;
+    near_capped(its, s.inverse, near);
+    return fabsf(x) <= (float)s.cap ? near[0] : fabsf(x) < INFINITY ? s.cap - 2.0 * s.cap / (d[0] + 1.0) : -INFINITY;
 }
 __device__ __forceinline__ double warp_weight(const Scale& s, double logit) {
     const double y = logit - s.from;
@@ -528,8 +541,8 @@ __device__ __forceinline__ void Scale::relative_to(float top, bool infinite) {
     shift = kShift - rint(from * k);                   // exact where no care is needed
     const double bottom = from + lowest;
     if (CAP) {
-        // the cap's inverse, cap atanh(bottom / cap); 2^-23 of the cap is the widest step of its logits
-        careful = infinite || cap * 0x1p-22 * k > 320.0;
+        // the cap's inverse, cap atanh(bottom / cap); beyond 2800 T of cap what the quotients are off by would move weights by more than 3e-10
+        careful = infinite || cap * k > 0x1p17;
         least = bottom > -cap && !careful ? (float)(0.5 * cap * log((cap + bottom) / (cap - bottom))) : -INFINITY;
     } else {
         careful = infinite || bottom < -3.4028234e38 || fabs(from) * 0x1p-22 * k > 320.0;
