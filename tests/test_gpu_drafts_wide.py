@@ -109,10 +109,10 @@ def test_temperatures_at_the_ends(tf_ctx):
         d.compare(tf_ctx, temperatures=[0.0, -2.0, 1e-6, 1e-30, 0.05, 50.0, 1e6, 1e-3])
 
 
-@pytest.mark.parametrize("cap", [1e-3, 300.0, 4000.0, 1e5, 1e9, 1e20, 3e38])
+@pytest.mark.parametrize("cap", [1e-45, 1e-39, 2e-38, 1e-3, 300.0, 4000.0, 1e5, 1e9, 1e20, 3e38])
 @pytest.mark.parametrize("counts,vocab", [([3] * 8, 240007), ([3, 2], 3001), ([1] * 8, 30011)])      # sums in 32 bits, in 64, lone rows
 def test_caps_at_the_ends(tf_ctx, cap, counts, vocab):
-    """From so low that nearly all logits count alike to so high that it changes nothing; some logits are wider than any cap."""
+    """From so low that all logits count alike (and that the cap's inverse is no number of 32 bits) to so high that it changes nothing; some logits are wider than any cap."""
     for dtype, far in ((torch.float16, -6e4), (torch.float32, -3.4e38)):
         d = Draft(9, counts, max(counts), vocab, dtype=dtype, tree=max(counts) > 1)
         d.logits[:, ::5] = 0.0

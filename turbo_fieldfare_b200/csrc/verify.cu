@@ -146,9 +146,11 @@ __device__ __forceinline__ float capped_near(float x, float inverse) {
     r = fmaf(r, z, -0.3333333134651184f);
     return fmaf(x, r * z, x);
 }
+// 1 / cap, of caps below 2^-128 the largest number: with an infinity a logit of zero would be NaN.
+__device__ __forceinline__ float inverse_of(float cap) { return fminf(1.0f / cap, 3.402823466e38f); }
 // The same of any logit; tanh(u) = 1 - 2 / (exp(2 u) + 1), which needs no care at either end: 2^x is 0 or infinite there.
 __device__ __forceinline__ float capped(float x, float cap) {
-    if (fabsf(x) <= cap) return capped_near(x, 1.0f / cap);
+    if (fabsf(x) <= cap) return capped_near(x, inverse_of(cap));
     return x == -INFINITY ? x : cap * (1.0f - __fdividef(2.0f, verify_exp2(x * (float)(2 * kLog2E) / cap) + 1.0f));
 }
 
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __
         else for (uint32_t j = i + 1 + tid; j < of.n; j += kStatsThreads) child |= parent_of(a, b, j, kWaited) == (int32_t)i;
         if (!__syncthreads_or(child)) return;
     }
-    const float k = heat.k32(), inverse = CAP ? 1.0f / a.softcap : 0.0f;
+    const float k = heat.k32(), inverse = CAP ? inverse_of(a.softcap) : 0.0f;
     float most = -INFINITY, from = -INFINITY, sum = 0.0f;
     uint32_t where = 0;                                        // the chunk of the first largest
     auto take = [&](const uint4 (&w)[PIECES], uint32_t chunk) {
