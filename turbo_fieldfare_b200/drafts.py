@@ -49,6 +49,12 @@ def _ints(name: str, t, device, dims: int, shape=None):
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
+def _number(name: str, value) -> None:
+    """ctypes would cut a larger number to 32 bits."""
+    if not 0 < value < 1 << 31:
+        raise ValueError(f"{name} must be from 1 to 2^31 - 1, got {value}")
+
+
 class KVPages:
     """``tf_kv_pages``: ``page_table`` int32 [sequences, pages of the longest], ``held_pages`` and ``first_pages`` int32 [sequences], ``free_pages`` int32 [pages], a
     stack of which the first ``free_count`` [1] are nobody's. ``first_pages`` is needed with a window."""
@@ -62,6 +68,7 @@ class KVPages:
         _ints("free_count", free_count, self.device, 1, (1,))
         if first_pages is not None:
             _ints("first_pages", first_pages, self.device, 1, (self.sequences,))
+        _number("page_size", page_size)
         self.page_table, self.held_pages, self.free_pages, self.free_count, self.first_pages = page_table, held_pages, free_pages, free_count, first_pages
         self.page_size, self.num_pages = page_size, free_pages.shape[0]
         self._c = KVPagesDesc(_ptr(page_table), _ptr(held_pages), _ptr(first_pages), _ptr(free_pages), _ptr(free_count), stride, self.num_pages, page_size, self.sequences)
@@ -155,6 +162,8 @@ class VerificationWorkspace:
 
     def __init__(self, context: TurboContext, rows: int, vocab: int):
         self.context = context
+        _number("rows", rows)
+        _number("vocab", vocab)
         handle = C.c_void_p()
         context.check(context.lib.tf_verify_workspace_create(context.handle, rows, vocab, C.byref(handle)))
         self.handle = handle
