@@ -103,10 +103,22 @@ def test_rows_cut_by_the_caller(tf_ctx, dtype, cap):
             d.compare(tf_ctx, temperatures=heat, cap=cap)
 
 
+@pytest.mark.parametrize("nodes", [1, 4])
+def test_calls_without_rows(tf_ctx, nodes):
+    from turbo_fieldfare_b200 import drafts as dr
+    d = Draft(1, [0, 0, 0], nodes, 100, padded=0)
+    d.workspace = dr.VerificationWorkspace(tf_ctx, 1, 100)
+    for heat in (None, [0.0, 1.0, 0.5]):
+        out = d.compare(tf_ctx, temperatures=heat)
+        assert out[2].tolist() == [0, 0, 0]
+    assert tf_ctx.device_status() == 0
+
+
 def test_temperatures_at_the_ends(tf_ctx):
     for dtype in TYPES:
         d = wide(8, [3] * 8, 3, 240007, dtype=dtype, probs=torch.float32)
         d.compare(tf_ctx, temperatures=[0.0, -2.0, 1e-6, 1e-30, 0.05, 50.0, 1e6, 1e-3])
+        d.compare(tf_ctx, temperatures=[math.inf, 1e35, 1e30, math.inf, 1e-45, 1e-38, math.inf, -math.inf])
 
 
 @pytest.mark.parametrize("cap", [1e-45, 1e-39, 2e-38, 1e-3, 300.0, 4000.0, 1e5, 1e9, 1e20, 3e38])
