@@ -993,6 +993,9 @@ typedef struct tf_draft_probs {
  * Outputs, [sequences][drafts->stride]: out_tokens the kept tokens and behind them the next token; out_rows node 0 and the kept nodes; -1 behind them. kept[b]: how many, the next
  * token included (0 for a sequence without rows): what tf_kv_cache_keep and the next tf_kv_plan take. logprobs (may be NULL): log p of out_tokens (T = 1 where T <= 0), zero behind
  * them. A sequence whose last row has no finite logit gets token 0, log p = -inf. With drafts->stride 1 the call is a sampler.
+ * logprobs are rounded to 32 bits from 64 (2^-24 of themselves) for the token drawn, and for all where rows * vocab is at most 6e6 (4e6 with a softcap) or drafts->stride is 1. Else those of kept
+ * tokens, and of a greedy sequence, may come from a row's 32-bit sum: 2^-15 off at the most, and softcap / T * 2^-18 more with a softcap (measured 2e-7 and less, root of the mean square).
+ * T above 1e30 counts as 1e30.
  * uniforms are in [0, 1). Sums that a token is drawn from and tests near their border are 64-bit; equal calls give equal bits. drafts->stride is at most 1024; a sequence of more rows is
  * cut there and tf_device_status reports 0x7F000052, as for offsets that descend or pass `rows`. Calls without sequences do nothing.
  * Replaces sample / sample_topk64 (Metal/Sampling/logit.metal:184,490,517,545) and logit_softcap_softmax (:53) for what they have in common with it. */

@@ -216,7 +216,8 @@ __device__ __forceinline__ int32_t parent_of(const VerifyArgs& a, uint32_t b, ui
 
 // A thread keeps a maximum and a sum of its own over the chunks, so that no block meets at a barrier before the end, and has the next chunk's loads under way
 // while it works on one; the first chunk's before it knows whether the row has children. Chunks with a row's edge are done apart. The powers of two bound it beside HBM: sixteen a clock and SM
-// are 4.5e12 a second, what 16-bit logits at the full 6.5 TB/s would ask for is 3.3e12. 200 chains of four, all rows needed: 60 us, 5.2 TB/s.
+// are 4.5e12 a second, what 16-bit logits at the full 6.5 TB/s would ask for is 3.3e12. 200 chains of four, all rows needed: 58 us cold, 5.4 TB/s. In 64 registers the two sets of eight pieces that
+// fp32 logits take do not fit: 172 bytes of a thread are spilled (272 capped; 16-bit ones none, 16 of bf16 capped). Capped pieces with a logit wider than the cap, -infinity among them, are done twice.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     pdl_launch_dependents();
@@ -557,7 +558,9 @@ __device__ __forceinline__ void Scale::relative_to(float top, bool infinite) {
 // ---------------------------------------------------------------------------
 //
 // Where there are few logits, or one row a sequence: the same sums for every row, in 64 bits, by blocks all over the chip. The walk then needs no sum but those behind
-// a refusal, and a draw no more than a part's logits again. 64-bit arithmetic is its floor: eight operations a logit (23 capped) at 64 a clock and SM, 2.2e12 logits a second (8e11).
+// a refusal, and a draw no more than a part's logits again. Eight 64-bit operations a logit (23 capped) at 64 a clock and SM would let 2.2e12 logits a second through (8e11), HBM 3.3e12 of 16 bits;
+// 200 rows of 262144 take 76 us with their draws (175 capped), 7e11 (3e11): conversions, the table's shuffles and latencies, not one unit. A block with a capped logit wider than the cap, -infinity among
+// them, goes the long way: 207 us where all but 64 logits of a row are masked.
 constexpr int kMostPieces = 8;
 
 template <typename T, bool CAP>
@@ -779,7 +782,8 @@ __device__ __forceinline__ uint32_t warp_fall(double part, double upto, double& 
     return who;
 }
 
-// One thread goes from node to node until a sum over the vocabulary is needed, or the walk is over.
+// One thread goes from node to node until a sum over the vocabulary is needed, or the walk is over. A child's test goes through all refusals of its siblings before it: 63 refused ones without q
+// over 2000 logits take 0.18 ms in all, 255 0.47, 1023 3.6.
 template <bool CAP>
 __device__ __forceinline__ void walk_on(const VerifyArgs& a, const Nodes& of, const Heat& heat, uint32_t b, const NodeTable& t, Walk& walk, Order& order,
                                         int32_t* out_tokens, int32_t* out_rows) {
