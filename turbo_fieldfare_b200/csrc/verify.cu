@@ -217,7 +217,7 @@ __device__ __forceinline__ int32_t parent_of(const VerifyArgs& a, uint32_t b, ui
 // A thread keeps a maximum and a sum of its own over the chunks, so that no block meets at a barrier before the end, and has the next chunk's loads under way
 // while it works on one; the first chunk's before it knows whether the row has children. Chunks with a row's edge are done apart. The powers of two bound it beside HBM: sixteen a clock and SM
 // are 4.5e12 a second, what 16-bit logits at the full 6.5 TB/s would ask for is 3.3e12. 200 chains of four, all rows needed: 58 us cold, 5.4 TB/s. In 64 registers the two sets of eight pieces that
-// fp32 logits take do not fit: 172 bytes of a thread are spilled (272 capped; 16-bit ones none, 16 of bf16 capped). Capped pieces with a logit wider than the cap, -infinity among them, are done twice.
+// fp32 logits take do not fit: 172 bytes of a thread are spilled (272 capped; 16-bit ones none, up to 16 capped). Capped pieces with a logit wider than the cap, -infinity among them, are done twice.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kStatsThreads, 4) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     pdl_launch_dependents();
@@ -1100,8 +1100,8 @@ __device__ __forceinline__ uint32_t part_of(Scale& scale, const ChunkStat* s, ui
 }
 
 // One row a sequence: nothing to walk, and all that a draw needs is there. A block takes the part that the token lies in as the first launch did, all its logits at once, and sums them by steps
-// of a warp; the step's warp draws. Latency bounds it: six loads, one after another, and what stands between them. A token of 262144 takes 13.3 us
-// in all and 1000 rows of 300 34; by the walk, which goes from part to token in three readings, 15.5 and 93.
+// of a warp; the step's warp draws. Latency bounds it: six loads, one after another, and what stands between them. A token of 262144 takes 13.9 us
+// in all (13.6 before logits under high caps had a series of their own) and 1000 rows of 300 34; by the walk, which goes from part to token in three readings, 15.5 and 93.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kStatsThreads, 2) verify_lone_kernel(const __grid_constant__ VerifyArgs a) {
     using R = Row<T>;
