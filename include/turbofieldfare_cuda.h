@@ -928,7 +928,7 @@ typedef struct tf_drafts {
     uint32_t stride;
 } tf_drafts;
 
-/* The pages of a cache and who holds them; device arrays of the caller. Table entries [first_pages[b], held_pages[b]) of a sequence are its
+/* The pages of a cache and who holds them; device arrays of the caller. Pages are numbers below num_pages, also where a plan has only some of them (its stack still has room for all). Table entries [first_pages[b], held_pages[b]) of a sequence are its
  * own (first_pages NULL: from 0); free_pages[0 .. *free_count) is a stack of the pages that nobody holds, with room for num_pages of them.
  * At the beginning: held_pages and first_pages zero, all pages on the stack. page_size as in tf_kv_cache. */
 typedef struct tf_kv_pages {

@@ -57,7 +57,7 @@ def _number(name: str, value) -> None:
 
 class KVPages:
     """``tf_kv_pages``: ``page_table`` int32 [sequences, pages of the longest], ``held_pages`` and ``first_pages`` int32 [sequences], ``free_pages`` int32 [pages], a
-    stack of which the first ``free_count`` [1] are nobody's. ``first_pages`` is needed with a window."""
+    stack of which the first ``free_count`` [1] are nobody's (it is as long as the cache has pages, also where these are only some of them). ``first_pages`` is needed with a window."""
 
     def __init__(self, page_table, held_pages, free_pages, free_count, page_size: int, first_pages=None):
         self.device = page_table.device
