@@ -525,11 +525,17 @@ __device__ __forceinline__ void warp_weights(const Scale& s, const float (&x)[N]
 template <bool CAP>
 __device__ __forceinline__ double warp_logit64(const Scale& s, float x) {
     if constexpr (!CAP) return (double)x;
-    const float edge = 20.0f * (float)s.cap, its[1] = {x};
-    double d[1] = {(double)fminf(fmaxf(x, -edge), edge)}, near[1];
-    warp_exp2(d, s.twice, s.table);
+    const float its[1] = {x};
+    double near[1];
     near_capped(its, s.inverse, near);
-    return fabsf(x) <= (float)s.cap ? near[0] : fabsf(x) < INFINITY ? s.cap - 2.0 * s.cap / (d[0] + 1.0) : -INFINITY;
+    const bool finite = fabsf(x) < INFINITY, far = finite && fabsf(x) > (float)s.cap;
+    if (__any_sync(kFullMask, far)) {              // seldom
+        const float edge = 20.0f * (float)s.cap;
+        double d[1] = {(double)fminf(fmaxf(x, -edge), edge)};
+        warp_exp2(d, s.twice, s.table);
+        if (far) near[0] = s.cap - 2.0 * s.cap / (d[0] + 1.0);
+    }
+    return finite ? near[0] : -INFINITY;
 }
 __device__ __forceinline__ double warp_weight(const Scale& s, double logit) {
     const double y = logit - s.from;
@@ -1101,8 +1107,8 @@ __device__ __forceinline__ uint32_t part_of(Scale& scale, const ChunkStat* s, ui
 }
 
 // One row a sequence: nothing to walk, and all that a draw needs is there. A block takes the part that the token lies in as the first launch did, all its logits at once, and sums them by steps
-// of a warp; the step's warp draws. Latency bounds it: six loads, one after another, and what stands between them. A token of 262144 takes 13.9 us
-// in all (13.6 before logits under high caps had a series of their own) and 1000 rows of 300 34; by the walk, which goes from part to token in three readings, 15.5 and 93.
+// of a warp; the step's warp draws. Latency bounds it: six loads, one after another, and what stands between them. A token of 262144 takes 13.6 us
+// in all and 1000 rows of 300 34; by the walk, which goes from part to token in three readings, 15.5 and 93.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kStatsThreads, 2) verify_lone_kernel(const __grid_constant__ VerifyArgs a) {
     using R = Row<T>;
