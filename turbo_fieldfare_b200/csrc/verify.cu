@@ -566,8 +566,8 @@ __device__ __forceinline__ void Scale::relative_to(float top, bool infinite) {
 //
 // Where there are few logits, or one row a sequence: the same sums for every row, in 64 bits, by blocks all over the chip. The walk then needs no sum but those behind
 // a refusal, and a draw no more than a part's logits again. Eight 64-bit operations a logit (23 capped) at 64 a clock and SM would let 2.2e12 logits a second through (8e11), HBM 3.3e12 of 16 bits;
-// 200 rows of 262144 take 76 us with their draws (175 capped), 7e11 (3e11): conversions, the table's shuffles and latencies, not one unit. A block with a capped logit wider than the cap, -infinity among
-// them, goes the long way: 207 us where all but 64 logits of a row are masked.
+// 200 rows of 262144 take 76 us with their draws (177 capped), 7e11 (3e11): conversions, the table's shuffles and latencies, not one unit. A block with a capped logit wider than the cap, -infinity among
+// them, goes the long way: 208 us where all but 64 logits of a row are masked.
 constexpr int kMostPieces = 8;
 
 template <typename T, bool CAP>
